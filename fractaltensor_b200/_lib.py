@@ -66,6 +66,12 @@ SIGNATURES = {
     "ftb_lstm_project_softmax_rows": (_i, [_vp, _vp, _vp, _vp, ctypes.c_longlong, _i, _i, _i, _vp, _sz, _vp]),
     "ftb_project_softmax_scratch_bytes": (_sz, [ctypes.c_longlong, _i, _i, _i, _i]),
     "ftb_project_softmax_fwd": (_i, [_vp, _vp, _i, _vp, ctypes.c_longlong, ctypes.c_longlong, _i, _i, _i, _vp, _sz, _vp, _sz, _vp]),
+    "ftb_paged_cache_write": (_i, [_vp, _vp] + [ctypes.c_longlong] * 4 + [_vp] * 7 + [_i] * 8 + [_vp, _sz, _vp]),
+    "ftb_paged_cache_read": (_i, [_vp] * 9 + [_i] * 8 + [_vp, _sz, _vp]),
+    "ftb_paged_attn_scratch_bytes": (_sz, [_i] * 5),
+    "ftb_paged_attn_fwd": (_i, [_vp, ctypes.c_longlong, ctypes.c_longlong] + [_vp] * 8 + [_i] * 9 + [_f, _i, _vp, _sz, _vp, _sz, _vp]),
+    "ftb_verify_drafts": (_i, [_vp, ctypes.c_longlong, ctypes.c_longlong, _vp, ctypes.c_longlong, ctypes.c_longlong] + [_vp] * 5 +
+                          [_i] * 3 + [_vp, _sz, _vp]),
     "ftb_gemm_nt": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, ctypes.POINTER(_i), _vp, _sz, _vp]),
 }
 

@@ -1,0 +1,75 @@
+// What the kernels over a paged cache share: where a row of new tokens belongs, and reading 8-bit rows.
+//
+// A batch is described by starts [B + 1] (first row of each sequence's new tokens), lens [B] (keys of each
+// sequence, the new ones included) and table [B, W] (its pages).  Token i of the n new ones of sequence b is at
+// position lens[b] - n + i.  Pages are [kv_heads, page_size, d]: the rows of one head of a page lie side by side.
+//
+// 8-bit rows: d e4m3 codes and one exponent byte e, a row's numbers being code * 2^(e - 127).  A scale that is
+// a power of two costs e4m3 nothing (the codes are floating-point numbers themselves, with the same relative step at
+// every scale) and makes scaling exact in both directions; a byte of it is 1 / d of the row.
+#pragma once
+#include <cuda_fp8.h>
+
+#include "ptx.cuh"
+
+namespace ftb {
+
+struct PagedBatch {
+  const int* table;
+  const int* lens;
+  const int* starts;
+  int B, W, pages, page_shift;
+};
+
+// The sequence that row t belongs to, or B; the whole warp asks for the same t.  32 probes a round: one round trip
+// to memory up to 32 sequences, two up to 1024.
+__device__ __forceinline__ int sequence_of_row(const PagedBatch& x, int t, int lane) {
+  int lo = 0, hi = x.B;  // the smallest b with starts[b + 1] > t is in [lo, hi], where hi = B stands for none
+  while (lo < hi) {
+    const int step = (hi - lo + 31) >> 5;
+    const int at = lo + (lane + 1) * step - 1;
+    const unsigned above = __ballot_sync(0xffffffffu, at < hi ? x.starts[at + 1] > t : true);
+    const int first = __ffs(above) - 1;
+    if (first < 0) {
+      lo = hi;
+      break;
+    }
+    lo += first * step;
+    if (step == 1) break;
+    hi = min(hi, lo + step - 1);
+  }
+  return lo < x.B && x.starts[lo] <= t && x.starts[lo + 1] > t ? lo : x.B;
+}
+
+// Position of row t of sequence b in it; negative: in front of the sequence.
+__device__ __forceinline__ long long position_of_row(const PagedBatch& x, int b, int t) {
+  return static_cast<long long>(x.lens[b]) - x.starts[b + 1] + t;
+}
+
+// The page that holds position pos of sequence b, or -1 where the table has none (recorded in the status word).
+__device__ __forceinline__ int page_of(const PagedBatch& x, int b, long long pos, int* status) {
+  const long long i = pos >> x.page_shift;
+  const int page = i < x.W ? x.table[static_cast<long long>(b) * x.W + i] : -1;
+  if (page >= 0 && page < x.pages) return page;
+  atomicCAS(status, 0, FTB_ERR_INDEX);
+  return -1;
+}
+
+__device__ __forceinline__ float exponent_scale(int e) { return __uint_as_float(static_cast<uint32_t>(e) << 23); }
+
+// Two e4m3 codes -> two fp16 numbers (exact; a NaN stays one).
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t codes) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes), __NV_E4M3);
+  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+}
+
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t v);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+
+}  // namespace ftb

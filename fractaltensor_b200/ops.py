@@ -669,3 +669,186 @@ def embedding_gather(table, ids, out=None):
         check(lib.ftb_embedding_gather(_ptr(table), _ptr(ids), _ptr(out), T, V, H, _dtype_code(table), _ptr(ws),
                                        ws.numel(), _stream()), "ftb_embedding_gather")
     return out
+
+
+# ------------------------------------------------------------------- paged cache, attention over it, drafts
+def paged_cache(pages, kv_heads, page_size, d, dtype, device="cuda"):
+    """Room for keys and values: (k, v), each [pages, kv_heads, page_size, d] of a 16-bit dtype, or for
+    torch.float8_e4m3fn (k, v, k_exp, v_exp) with an exponent byte a row, uint8 [pages, kv_heads, page_size].
+    page_size 16, 32, 64 or 128; d 64 or 128.  A program may as well make these tensors itself."""
+    if page_size not in (16, 32, 64, 128) or d not in (64, 128) or pages <= 0 or kv_heads <= 0:
+        raise ValueError("paged_cache: page_size 16, 32, 64 or 128 and d 64 or 128 are supported, got %s and %s" % (page_size, d))
+    if dtype not in (torch.float16, torch.bfloat16, torch.float8_e4m3fn):
+        raise TypeError("paged_cache: unsupported dtype %s (float16, bfloat16 or float8_e4m3fn)" % dtype)
+    rows = (int(pages), int(kv_heads), int(page_size))
+    made = tuple(torch.zeros(rows + (int(d),), dtype=torch.uint8 if dtype == torch.float8_e4m3fn else dtype, device=device) for _ in range(2))
+    if dtype != torch.float8_e4m3fn:
+        return made
+    return tuple(t.view(dtype) for t in made) + tuple(torch.ones(rows, dtype=torch.uint8, device=device) for _ in range(2))
+
+
+def _paged_args(where, cache, table, lens, starts):
+    """Checks a cache and a batch's description -> (k, v, k_exp, v_exp, table, lens, starts as pointers, B, W, cache's shape)."""
+    if not isinstance(cache, (tuple, list)) or len(cache) not in (2, 4):
+        raise TypeError("%s: the cache is (k, v) or (k, v, k_exp, v_exp)" % where)
+    k, v = cache[0], cache[1]
+    _req(k, "cache keys")
+    if k.dim() != 4:
+        raise ValueError("%s: cache pages are [pages, kv_heads, page_size, d], got %s" % (where, tuple(k.shape)))
+    _req_like(v, "cache values", k.dtype, k.shape, k)
+    if k.dtype != torch.float8_e4m3fn and k.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError("%s: unsupported cache dtype %s (float16, bfloat16 or float8_e4m3fn)" % (where, k.dtype))
+    if (k.dtype == torch.float8_e4m3fn) != (len(cache) == 4):
+        raise ValueError("%s: float8_e4m3fn caches, and no others, come with exponents" % where)
+    for e in cache[2:]:
+        _req_like(e, "cache exponents", torch.uint8, k.shape[:3], k)
+    if k.shape[2] not in (16, 32, 64, 128) or k.shape[3] not in (64, 128):
+        raise ValueError("%s: page_size 16, 32, 64 or 128 and d 64 or 128 are supported, got %s and %s" % (where, k.shape[2], k.shape[3]))
+    _req(table, "table", torch.int32)
+    if table.dim() != 2 or 0 in table.shape or table.device != k.device:
+        raise ValueError("%s: the table is [sequences, pages of one], on the cache's device" % where)
+    B, W = table.shape
+    _req_like(lens, "lens", torch.int32, (B,), k)
+    _req_like(starts, "starts", torch.int32, (B + 1,), k)
+    exps = [_ptr(e) for e in cache[2:]] or [0, 0]
+    return [_ptr(k), _ptr(v)] + exps + [_ptr(table), _ptr(lens), _ptr(starts)], B, W
+
+
+def _rows_of(t, name, dtype, like, heads=None):
+    """Rows of heads as they come out of a product, [T, heads, d], the numbers of a head side by side: (pointer, distances)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a torch.Tensor" % name)
+    if not t.is_cuda:
+        raise RuntimeError("%s must live on a CUDA device: there is no CPU path" % name)
+    if t.device != like.device:
+        raise ValueError("%s lives on %s, the cache on %s" % (name, t.device, like.device))
+    if t.dim() != 3 or t.shape[2] != like.shape[3] or (heads is not None and t.shape[1] != heads):
+        raise ValueError("%s must be [T, heads, d] with the cache's d%s, got %s" % (name, "" if heads is None else " and heads", tuple(t.shape)))
+    if t.dtype not in (torch.float16, torch.bfloat16) or (dtype is not None and t.dtype != dtype):
+        raise TypeError("%s must have dtype %s, got %s" % (name, dtype or "float16 or bfloat16", t.dtype))
+    row, head = (t.stride(0) if t.shape[0] > 1 else 0), (t.stride(1) if t.shape[1] > 1 else 0)
+    if t.stride(2) != 1 or row % 8 or head % 8 or t.data_ptr() % 16:
+        raise ValueError("%s: the numbers of a head must lie side by side, heads and rows on 16-byte boundaries" % name)
+    return t.data_ptr(), row, head
+
+
+def paged_cache_write(cache, k, v, table, lens, starts):
+    """Stores the keys and values of new tokens in the cache, quantised where it has 8 bits.
+
+    k, v: [T, kv_heads, d] (fp16 or bf16, the cache's own type if it has 16 bits; slices of a fused product as they are);
+    table: int32 [B, W], the pages of each sequence; lens: int32 [B], the keys of each sequence with the new ones;
+    starts: int32 [B+1], the first row of each sequence's new tokens, the last one's end behind them.  Token i of the n new
+    ones of sequence b goes to position lens[b] - n + i.  Rows that belong to no sequence (padding) are not stored.  The
+    pages that new tokens fall into must belong to one sequence each."""
+    args, B, W = _paged_args("paged_cache_write", cache, table, lens, starts)
+    kc = cache[0]
+    pages, kv, page_size, d = kc.shape
+    own = None if len(cache) == 4 else kc.dtype
+    (kp, kr, kh), (vp, vr, vh) = _rows_of(k, "k", own, kc, kv), _rows_of(v, "v", own or k.dtype, kc, kv)
+    if k.shape[0] != v.shape[0]:
+        raise ValueError("paged_cache_write: k has %d rows, v has %d" % (k.shape[0], v.shape[0]))
+    ws = workspace(kc.device)
+    with _on(kc.device):
+        check(lib.ftb_paged_cache_write(kp, vp, kr, kh, vr, vh, *args, k.shape[0], B, W, pages, kv, page_size, d, _dtype_code(k),
+                                        _ptr(ws), ws.numel(), _stream()), "ftb_paged_cache_write")
+
+
+def paged_cache_read(cache, table, lens, starts, rows, dtype=None, out=None):
+    """The keys and values that paged_cache_write stored for the same table, lens and starts -> (k, v), [rows, kv_heads, d].
+
+    With starts[b+1] - starts[b] == lens[b] that is sequence b whole.  rows: what starts ends with, or more: rows that belong to
+    no sequence are left as they were.  dtype: 16-bit caches: their own; 8-bit ones: float32, float16 or bfloat16 (the
+    default, which holds every such number exactly)."""
+    args, B, W = _paged_args("paged_cache_read", cache, table, lens, starts)
+    kc = cache[0]
+    pages, kv, page_size, d = kc.shape
+    if dtype is None:
+        dtype = torch.bfloat16 if len(cache) == 4 else kc.dtype
+    if len(cache) == 2 and dtype != kc.dtype:
+        raise TypeError("paged_cache_read: a cache of %s is read as that, not as %s" % (kc.dtype, dtype))
+    if dtype not in _DT:
+        raise TypeError("unsupported dtype %s (float32, float16 or bfloat16)" % dtype)
+    shape = (int(rows), kv, d)
+    if out is None:
+        out = tuple(torch.empty(shape, dtype=dtype, device=kc.device) for _ in range(2))
+    for t in out:
+        _req_like(t, "out", dtype, shape, kc)
+    ws = workspace(kc.device)
+    with _on(kc.device):
+        check(lib.ftb_paged_cache_read(*args, _ptr(out[0]), _ptr(out[1]), shape[0], B, W, pages, kv, page_size, d,
+                                       _DT[dtype], _ptr(ws), ws.numel(), _stream()), "ftb_paged_cache_read")
+    return tuple(out)
+
+
+def paged_attention(q, cache, table, lens, starts, scale=None, window=None, out=None):
+    """Attention of new tokens over a paged cache that holds their keys and values already (paged_cache_write).
+
+    q: [T, heads, d], heads a multiple of the cache's kv_heads, rows as in paged_cache_write -> [T, heads, d]: for a token
+    at position p softmax(scale * q . k_j) v over the keys j <= p, with `window` over p - window < j <= p only.  Tokens that see
+    nothing get zeros; rows that belong to no sequence are left as they were."""
+    args, B, W = _paged_args("paged_attention", cache, table, lens, starts)
+    kc = cache[0]
+    pages, kv, page_size, d = kc.shape
+    qp, qr, qh = _rows_of(q, "q", None if len(cache) == 4 else kc.dtype, kc)
+    T, heads = q.shape[0], q.shape[1]
+    if heads == 0 or heads % kv:
+        raise ValueError("paged_attention: %d heads are no multiple of the cache's %d" % (heads, kv))
+    if window is not None and window < 1:
+        raise ValueError("paged_attention: a window holds one key or more, got %s" % window)
+    if out is None:
+        out = torch.empty(T, heads, d, dtype=q.dtype, device=q.device)
+    _req_like(out, "out", q.dtype, (T, heads, d), q)
+    # of the call's own: calls on other streams, and graphs replayed at the same time, have others
+    n = lib.ftb_paged_attn_scratch_bytes(T, B, kv, heads // kv, d)
+    ws = workspace(kc.device)
+    with _on(kc.device):
+        scratch = torch.empty(n, dtype=torch.uint8, device=kc.device) if n else None
+        check(lib.ftb_paged_attn_fwd(qp, qr, qh, *args, _ptr(out), T, B, W, pages, kv, heads // kv, page_size, d,
+                                     min(int(window), 0x7fffffff) if window is not None else 0, 1.0 if scale is None else float(scale),
+                                     _dtype_code(q), _ptr(scratch), n, _ptr(ws), ws.numel(), _stream()), "ftb_paged_attn_fwd")
+    return out
+
+
+def verify_drafts(probs, drafts, u, draft_probs=None, counts=None):
+    """Drafted tokens against the target's probabilities, from random numbers of the caller's.
+
+    probs: fp32 [B, K+1, V] (of project_softmax_rows, say); drafts: int64 [B, K]; u: fp32 [B, K+1] in [0, 1); draft_probs: fp32
+    [B, K, V] that the drafts were drawn from, or None: each was certain; counts: int32 [B], how many of its drafts a
+    sequence has, or None: K.  Draft i is taken if u[i] * q_i(x_i) < p_i(x_i); behind the n taken ones a token
+    is drawn by u[K] from max(p_n - q_n, 0) (from p_n if all were taken).  -> (tokens int64 [B, K+1]: the taken drafts, the drawn
+    token, then -1; int32 [B]: n + 1)."""
+    def rows(t, name, n):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError("%s must be a torch.Tensor" % name)
+        if not t.is_cuda:
+            raise RuntimeError("%s must live on a CUDA device: there is no CPU path" % name)
+        if t.dtype != torch.float32:
+            raise TypeError("%s must have dtype torch.float32, got %s" % (name, t.dtype))
+        if t.dim() != 3 or t.shape[0] != B or t.shape[1] != n or (t.shape[2] != 1 and t.stride(2) != 1):
+            raise ValueError("%s must be [B, %d, V] with the numbers of a row side by side, got %s" % (name, n, tuple(t.shape)))
+        return t
+
+    _req(drafts, "drafts", torch.int64)
+    if drafts.dim() != 2:
+        raise ValueError("verify_drafts: drafts must be [B, K], got %s" % (tuple(drafts.shape),))
+    B, K = drafts.shape
+    rows(probs, "probs", K + 1)
+    V = probs.shape[2]
+    if probs.device != drafts.device or V == 0:
+        raise ValueError("verify_drafts: probs %s on %s do not match the drafts on %s" % (tuple(probs.shape), probs.device, drafts.device))
+    _req_like(u, "u", torch.float32, (B, K + 1), drafts)
+    if draft_probs is not None:
+        rows(draft_probs, "draft_probs", K)
+        if draft_probs.shape[2] != V or draft_probs.device != drafts.device:
+            raise ValueError("verify_drafts: draft_probs %s do not match probs %s" % (tuple(draft_probs.shape), tuple(probs.shape)))
+    if counts is not None:
+        _req_like(counts, "counts", torch.int32, (B,), drafts)
+    tokens = torch.empty(B, K + 1, dtype=torch.int64, device=drafts.device)
+    taken = torch.empty(B, dtype=torch.int32, device=drafts.device)
+    ws = workspace(drafts.device)
+    q = draft_probs
+    with _on(drafts.device):
+        check(lib.ftb_verify_drafts(_ptr(probs), probs.stride(0), probs.stride(1), _ptr(q), q.stride(0) if q is not None else 0,
+                                    q.stride(1) if q is not None else 0, _ptr(drafts), _ptr(u), _ptr(counts), _ptr(tokens),
+                                    _ptr(taken), B, K, V, _ptr(ws), ws.numel(), _stream()), "ftb_verify_drafts")
+    return tokens, taken

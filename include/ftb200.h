@@ -400,6 +400,61 @@ int ftb_project_softmax_fwd(const void* h, const void* P, int unpacked, float* p
 int ftb_gemm_nt(const void* A, const void* Bt, void* out, int M, int N, int K, int dtype, const int* tuning,
                 void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- Paged cache of keys and values, attention over it, drafted tokens: what a program that answers step by step needs beside
+ * ftb_flash_attn_* and the projection.  No counterpart in the reference, whose attention program
+ * (examples/flash_attention/flash_attention.py:75-88) has all keys in one tensor.
+ *
+ * Cache: pages [pages, kv_heads, page_size, d] for keys and the same for values; page_size 16, 32, 64 or 128, d 64 or 128.
+ * 16-bit pages hold the model's type.  8-bit pages (k_exp and v_exp not NULL) hold e4m3 codes, with an exponent byte e for each
+ * row of d numbers, [pages, kv_heads, page_size]: a number is code * 2^(e - 127), and e the smallest from 1 on with
+ * max |row| <= 448 * 2^(e - 127).  A row with a number that is not finite is stored as NaN (e = 255).
+ *
+ * Batch: int32 arrays on the device: starts [B + 1], non-decreasing, the first row of each sequence's new tokens among the
+ * T rows; lens [B], the keys of each sequence, the new ones included; table [B, W], its pages in order.  Token i of the n new ones of
+ * sequence b is at position lens[b] - n + i; at a negative position there is no token (nothing is stored; it is read and attended
+ * to as zeros).  Sequences may have no new tokens and no keys.  Rows in front of the first and behind the last sequence are left as they
+ * were.  A position whose page the table does not have (behind its width, or a number outside [0, pages)) is not stored, read as
+ * zeros, and attended to as whatever page 0 has in its place; it sets the (sticky) status word to 22.  Pages that new tokens fall
+ * into belong to one sequence each; others may be shared.
+ *
+ * ftb_paged_cache_write: k, v: T rows of kv_heads rows of d numbers of `dtype` (fp16 or bf16), `*_row` and `*_head` numbers apart
+ * (multiples of 8; the slices of a fused product are taken as they are).
+ * ftb_paged_cache_read: the same tokens out of the cache into k_out, v_out [T, kv_heads, d] of `dtype` (16-bit pages: their own type;
+ * 8-bit ones: fp32, fp16 or bf16). */
+int ftb_paged_cache_write(const void* k, const void* v, long long k_row, long long k_head, long long v_row, long long v_head,
+                          void* k_cache, void* v_cache, unsigned char* k_exp, unsigned char* v_exp, const int* table,
+                          const int* lens, const int* starts, int T, int B, int W, int pages, int kv_heads, int page_size,
+                          int d, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+int ftb_paged_cache_read(const void* k_cache, const void* v_cache, const unsigned char* k_exp, const unsigned char* v_exp,
+                         const int* table, const int* lens, const int* starts, void* k_out, void* v_out, int T, int B, int W,
+                         int pages, int kv_heads, int page_size, int d, int dtype, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/* Attention of the new tokens, whose keys and values are in the cache already: o = softmax(scale * q . k^T) v over the keys
+ * j <= pos of a token at position pos, with window > 0 over pos - window < j <= pos only.  q: T rows of kv_heads * group heads of d
+ * numbers of `dtype`, `q_row` and `q_head` numbers apart; head i reads the keys of kv head i / group; o [T, kv_heads * group, d].
+ * scale > 0.  A token that sees nothing gets zeros.  Keys that a token does not see have no part in its result, whatever they and the
+ * unwritten rows of a page hold.  16-bit pages have the type of q.  scratch: ftb_paged_attn_scratch_bytes. */
+size_t ftb_paged_attn_scratch_bytes(int T, int B, int kv_heads, int group, int d);
+int ftb_paged_attn_fwd(const void* q, long long q_row, long long q_head, const void* k_cache, const void* v_cache,
+                       const unsigned char* k_exp, const unsigned char* v_exp, const int* table, const int* lens,
+                       const int* starts, void* o, int T, int B, int W, int pages, int kv_heads, int group, int page_size,
+                       int d, int window, float scale, int dtype, void* scratch, size_t scratch_bytes, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* Drafted tokens against the target's probabilities, from random numbers that the caller gives.  probs: fp32, for each of B
+ * sequences K + 1 rows of V probabilities (`p_seq` and `p_row` numbers apart; ftb_project_softmax_fwd gives such rows);
+ * draft_probs: fp32, K rows that the drafts were drawn from, or NULL: each draft was certain; drafts: int64 [B, K]; u: fp32
+ * [B, K + 1] in [0, 1); counts: int32 [B], drafts of each sequence (cut to 0 .. K), or NULL: K.
+ * Draft i is taken if u_i * q_i(x_i) < p_i(x_i); the first that is not ends the run at n (n = counts[b] if all are taken).  tokens
+ * (int64 [B, K + 1]): the n taken drafts, then the first j with w_0 + .. + w_j > u_K * sum(w), w = max(p_n - q_n, 0) behind a
+ * draft that was not taken (p_n without the draft where draft_probs is NULL; p_n itself where nothing is left) and p_n behind the
+ * last one; then -1.  counts_out (int32 [B]): n + 1.  Sums in 64 bits.  Probabilities that are not positive and finite count as 0; a
+ * row without any gives -1 and, as a draft outside [0, V), which is not taken, sets the (sticky) status word to 22. */
+int ftb_verify_drafts(const float* probs, long long p_seq, long long p_row, const float* draft_probs, long long q_seq,
+                      long long q_row, const long long* drafts, const float* u, const int* counts, long long* tokens,
+                      int* counts_out, int B, int K, int V, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
