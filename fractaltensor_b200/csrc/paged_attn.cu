@@ -5,51 +5,24 @@
 
 #include "../../include/ftb200.h"
 #include "paged_attn.cuh"
+#include "paged_short.h"
 #include "tmap.h"
 
 namespace ftb {
 namespace {
 
-constexpr int kRowWarps = 4;
-
-// The simplest form: a warp a (token, head).
-template <typename T, bool k8, int D>
-__global__ void __launch_bounds__(kRowWarps * 32)
-paged_rows_kernel(PagedAttn a) {
-  __shared__ float s_q[kRowWarps][D];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long row = static_cast<long long>(blockIdx.x) * kRowWarps + warp;
-  grid_launch_dependents();
-  grid_dependency_wait();
-  const int heads = a.kv_heads * a.group;
-  if (row >= static_cast<long long>(a.T) * heads) return;
-  const int t = static_cast<int>(row / heads), head = static_cast<int>(row - static_cast<long long>(t) * heads);
-  const int b = sequence_of_row(a.batch, t, lane);
-  if (b >= a.batch.B) return;
-  attend_row<T, k8, D>(a, b, t, head, position_of_row(a.batch, b, t), s_q[warp], lane);
-}
-
-template <typename T, bool k8, int D>
-int launch_rows(const PagedAttn& a, cudaStream_t stream) {
-  const long long rows = static_cast<long long>(a.T) * a.kv_heads * a.group, grid = (rows + kRowWarps - 1) / kRowWarps;
-  if (grid > INT_MAX) return FTB_ERR_ARG;
-  const cudaError_t err = launch_light(paged_rows_kernel<T, k8, D>, dim3(static_cast<unsigned>(grid)), dim3(kRowWarps * 32), 0, stream, a);
-  count_launch();
-  if (err != cudaSuccess) cudaGetLastError();
-  return err == cudaSuccess ? FTB_OK : FTB_ERR_LAUNCH;
-}
-template <typename T>
-int launch_rows(const PagedAttn& a, int d, cudaStream_t stream) {
-  if (a.k_exp != nullptr) return d == 128 ? launch_rows<T, true, 128>(a, stream) : launch_rows<T, true, 64>(a, stream);
-  return d == 128 ? launch_rows<T, false, 128>(a, stream) : launch_rows<T, false, 64>(a, stream);
-}
+// Rows of a tile / 8, by the rows (token, head of a group) that a sequence has on average.
+int short_form(int T, int B, int group) { return static_cast<long long>(T) * group <= 8ll * B ? 1 : 2; }
 
 }  // namespace
 }  // namespace ftb
 
 using namespace ftb;
 
-extern "C" size_t ftb_paged_attn_scratch_bytes(int T, int B, int kv_heads, int group, int d) { return 0; }
+extern "C" size_t ftb_paged_attn_scratch_bytes(int T, int B, int kv_heads, int group, int d) {
+  if (T <= 0 || B <= 0 || kv_heads <= 0 || group <= 0 || d <= 0) return 0;
+  return paged_short_scratch_bytes(short_form(T, B, group), d);
+}
 
 extern "C" int ftb_paged_attn_fwd(const void* q, long long q_row, long long q_head, const void* k_cache, const void* v_cache,
                                   const unsigned char* k_exp, const unsigned char* v_exp, const int* table, const int* lens,
@@ -87,5 +60,7 @@ extern "C" int ftb_paged_attn_fwd(const void* q, long long q_row, long long q_he
   a.scale_log2 = scale * 1.4426950408889634f;
   a.status = static_cast<int*>(workspace);
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  return dtype == FTB_F16 ? launch_rows<__half>(a, d, stream) : launch_rows<__nv_bfloat16>(a, d, stream);
+  if (scratch == nullptr || scratch_bytes < ftb_paged_attn_scratch_bytes(T, B, kv_heads, group, d)) return FTB_ERR_WORKSPACE;
+  if ((reinterpret_cast<uintptr_t>(scratch) & 15) != 0) return FTB_ERR_ALIGN;
+  return paged_short_launch(a, d, dtype, short_form(T, B, group), static_cast<float*>(scratch), stream);
 }

@@ -23,6 +23,12 @@ __device__ __forceinline__ long long cache_row(const PagedAttn& a, int b, int h,
   return ((static_cast<long long>(page) * a.kv_heads + h) << a.batch.page_shift) + (key & ((1 << a.batch.page_shift) - 1));
 }
 
+// Whether a row at position pos of a tile that multiplies keys lo .. hi - 1 has some of them with weight 0 that it does not see: what
+// they hold could have made its result a NaN.
+__device__ __forceinline__ bool hides(const PagedAttn& a, long long pos, int lo, int hi) {
+  return pos + 1 < hi || (a.window > 0 && pos + 1 - a.window > lo);
+}
+
 // The output of one (token, head) by one warp, key by key: nothing of a key that the token does not see is touched, not
 // even with a weight of 0, which an infinity or a NaN there would make a NaN.  q: D floats of shared memory of the warp's.
 template <typename T, bool k8, int D>

@@ -1,0 +1,564 @@
+// Attention over a paged cache for few rows: a token or a few drafts of each sequence, up to 16 rows (token, head of a
+// group) to a tile.
+//
+// Bound by the bytes of the keys and values, which go from global memory into the registers that the products take them
+// from, without a stop in shared memory: with the keys on the M side, S^T = K Q^T and O^T = V^T P^T
+// (mma.m16n8k16), every lane's pieces of K and V are 16 contiguous bytes of a row, because the order of d under the sum, of
+// the keys under the other, and of the output's rows is free:
+//   S^T  lane (g, c) = (lane / 4, lane % 4) holds d = 32 j + 8 c .. + 7 of keys g and g + 8 (8-bit: 64 j + 16 c .. + 15), and
+//        the same numbers of query g as the other operand
+//   O^T  lane (g, c) holds d = 64 x + 8 g .. + 7 (8-bit, d 128: 16 g .. + 15) of keys 2c, 2c + 1, 2c + 8, 2c + 9: pairs of keys are put
+//        together by byte permutes
+// and P^T is the transpose of what the first product leaves, 8 x 8 numbers an instruction (movmatrix).
+// A warp walks every fourth chunk of 16 keys of its CTA's piece on its own, with its own maximum and sum; the next
+// chunk's keys are on their way while this one's weights are made, its values behind the second product.  Maxima are only looked
+// for among lanes when some score is 2^8 above the one in use.
+// 8-bit caches are taken as fp16, which holds every e4m3 number: a query row is scaled into fp16's range by a power of two
+// (what it loses is below 2^-24 of the row's largest number), a key's scale 2^ke goes to its scores, and a value's 2^ve into its
+// weight: 2^(x_j + ve_j - m) with m the largest x_j + ve_j, so that fp16 weights are as exact as the largest share in a row's result
+// allows, whatever the keys' values are sized like.  The sum that divides takes the weights times 2^-ve_j.
+#include <climits>
+#include <type_traits>
+
+#include "../../include/ftb200.h"
+#include "paged_work.cuh"
+#include "paged_short.h"
+#include "tmap.h"
+
+namespace ftb {
+namespace {
+
+constexpr int kWarps = 4, kUnitKeys = 16 * kWarps, kAtLeast = 2;
+static_assert(kWarps * 32 == kLineThreads, "the line is laid out by a block");
+constexpr float kAbove = 8.f;  // weights up to 2^8 (fp16 ends at 2^16): scores may lie that far above the maximum in use
+
+template <typename C>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                                 uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                        uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint4 load_once(const unsigned char* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+template <int D, int NT>
+struct Merge {
+  float o[kWarps][NT * 8][D + 4];  // (rows 16 bytes apart in the banks)
+  float m[kWarps][NT * 8], l[kWarps][NT * 8];
+};
+
+template <typename T, bool k8, int D, int NT>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
+paged_short_kernel(PagedAttn a, int most_pieces, float* __restrict__ parts) {
+  using C = typename std::conditional<k8, __half, T>::type;
+  constexpr int R = NT * 8, kSteps = D / 16, kKLoads = k8 ? D / 64 : D / 32;
+  constexpr int kVWords = k8 ? D / 32 : D / 16;  // 32-bit words of one key's values a lane
+  extern __shared__ __align__(16) unsigned char smem[];
+  Merge<D, NT>& mg = *reinterpret_cast<Merge<D, NT>*>(smem);
+  __shared__ int s_odd[R];
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  int b;
+  long long at;
+  const PagedLine line = paged_line<R, kUnitKeys>(a, blockIdx.x, most_pieces, kAtLeast, &b, &at);
+  if (static_cast<int>(blockIdx.x) >= line.pieces) return;
+  long long u = piece_begin(line, blockIdx.x);
+  const long long u_end = piece_begin(line, blockIdx.x + 1);
+  const int page_mask = (1 << a.batch.page_shift) - 1;
+  PagedSeq s = paged_sequence<R, kUnitKeys>(a, b < a.batch.B ? b : 0);
+
+  while (u < u_end) {
+    // the tile that unit u belongs to
+    long long cost = static_cast<long long>(s.tiles) * a.kv_heads * s.units;
+    while (u >= at + cost) {
+      at += cost;
+      s = paged_sequence<R, kUnitKeys>(a, ++b);
+      cost = static_cast<long long>(s.tiles) * a.kv_heads * s.units;
+    }
+    const long long off = u - at;
+    const int index = static_cast<int>(off / s.units), r0 = static_cast<int>(off - static_cast<long long>(index) * s.units);
+    const int r1 = static_cast<int>(min(static_cast<long long>(s.units), r0 + (u_end - u)));
+    const int h = index / s.tiles, tile = index - h * s.tiles;
+    const long long flat0 = static_cast<long long>(tile) * R, flats = static_cast<long long>(s.n) * a.group;
+    const int rows = static_cast<int>(min(static_cast<long long>(R), flats - flat0));
+    const int* table = a.batch.table + static_cast<long long>(b) * a.batch.W;
+    // keys that the tile's rows see: [lo, hi)
+    const long long first_pos = s.pos0 + s.first + flat0 / a.group, last_pos = s.pos0 + s.first + (flat0 + rows - 1) / a.group;
+    const int hi = static_cast<int>(min(static_cast<long long>(s.hi), max(0ll, last_pos + 1)));
+    const int lo = a.window > 0 ? static_cast<int>(min(static_cast<long long>(hi), max(0ll, first_pos - a.window + 1))) : 0;
+    const int unit0 = s.lo / kUnitKeys;
+
+    // ---- queries: lane (g, c) holds of row g what it holds of a key; limits and factors of rows 2c and 2c + 1
+    uint32_t q[NT][kSteps][2];
+    float factor[NT][2];
+    int see_lo[NT][2], see_hi[NT][2];  // keys see_lo .. see_hi
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = nt * 8 + g;
+      const long long flat = flat0 + row;
+      const int token = static_cast<int>(flat / a.group);
+      const T* src = static_cast<const T*>(a.q) + static_cast<long long>(s.first + token) * a.q_row +
+                     (h * a.group + static_cast<int>(flat - static_cast<long long>(token) * a.group)) * a.q_head;
+      uint4 x[D / 32];
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+        x[j] = make_uint4(0u, 0u, 0u, 0u);
+        const int d0 = k8 ? (j >> 1) * 64 + c * 16 + (j & 1) * 8 : j * 32 + c * 8;
+        if (row < rows) x[j] = *reinterpret_cast<const uint4*>(src + d0);
+      }
+      float mine = a.scale_log2;
+      if constexpr (k8 && !std::is_same<T, __half>::value) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+          const uint32_t w = __vmaxu2(__vmaxu2(x[j].x & 0x7fff7fffu, x[j].y & 0x7fff7fffu), __vmaxu2(x[j].z & 0x7fff7fffu, x[j].w & 0x7fff7fffu));
+          m = max(m, max(w & 0xffffu, w >> 16));
+        }
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        // the row times 2^(127 - e), e its largest number's exponent: that one is in [1, 2).  (A row that is not finite stays so.)
+        const int e = min(253, max(1, static_cast<int>(m >> 7)));
+        const float by = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+        mine *= __uint_as_float(static_cast<uint32_t>(e) << 23);
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+          uint32_t* w = reinterpret_cast<uint32_t*>(&x[j]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = unpack2<T>(w[i]);
+            w[i] = Fmt<__half>::pack2(f.x * by, f.y * by);
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+        q[nt][2 * j][0] = x[j].x;
+        q[nt][2 * j][1] = x[j].y;
+        q[nt][2 * j + 1][0] = x[j].z;
+        q[nt][2 * j + 1][1] = x[j].w;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        factor[nt][e] = __shfl_sync(0xffffffffu, mine, (2 * c + e) * 4);
+        const int r = nt * 8 + 2 * c + e;
+        const long long pos = r < rows ? s.pos0 + s.first + (flat0 + r) / a.group : -1;
+        see_hi[nt][e] = static_cast<int>(max(-1ll, min(pos, static_cast<long long>(hi) - 1)));
+        see_lo[nt][e] = a.window > 0 ? static_cast<int>(max(0ll, min(pos - a.window + 1, static_cast<long long>(INT_MAX)))) : 0;
+      }
+    }
+    // chunks that every row sees whole need no mask: [all_lo, all_hi]
+    int all_lo = 0, all_hi = static_cast<int>(max(-1ll, min(first_pos, static_cast<long long>(hi) - 1)));
+    if (a.window > 0) all_lo = static_cast<int>(max(0ll, min(last_pos - a.window + 1, static_cast<long long>(INT_MAX))));
+
+    float oacc[kSteps][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -FLT_MAX;
+      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) oacc[i][nt][0] = oacc[i][nt][1] = oacc[i][nt][2] = oacc[i][nt][3] = 0.f;
+    }
+
+    // ---- the walk
+    int key0 = (unit0 + r0) * kUnitKeys + warp * 16;
+    if (key0 + 15 < lo) key0 += (lo - key0) / kUnitKeys * kUnitKeys;
+    const int key_end = min(hi, (unit0 + r1) * kUnitKeys);
+    auto row_of = [&](int page, int key) {  // the cache row of key: a page that the table does not have reads as page 0
+      return ((static_cast<long long>(page) * a.kv_heads + h) << a.batch.page_shift) + (key & page_mask);
+    };
+    auto page_at = [&](int key) {
+      const int page = key < key_end ? __ldg(table + (key >> a.batch.page_shift)) : 0;
+      if (page >= 0 && page < a.batch.pages) return page;
+      atomicCAS(a.status, 0, FTB_ERR_INDEX);
+      return 0;
+    };
+    uint4 kf[2][kKLoads];
+    uint32_t vf[4][kVWords];
+    int ke[2] = {127, 127}, ve[2] = {127, 127};
+    auto load_k = [&](long long row) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < kKLoads; ++j)
+          kf[i][j] = load_once(a.k + (row + g + 8 * i) * (k8 ? D : 2 * D) + j * 64 + c * 16);
+      if constexpr (k8) {
+        ke[0] = a.k_exp[row + g];
+        ke[1] = a.k_exp[row + g + 8];
+        ve[0] = a.v_exp[row + g];
+        ve[1] = a.v_exp[row + g + 8];
+      }
+    };
+    auto load_v = [&](long long row) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned char* src = a.v + (row + 2 * c + (i & 1) + (i >> 1) * 8) * (k8 ? D : 2 * D);
+        if constexpr (kVWords == 2) {
+          const uint2 x = *reinterpret_cast<const uint2*>(src + g * 8);
+          vf[i][0] = x.x;
+          vf[i][1] = x.y;
+        } else {
+#pragma unroll
+          for (int j = 0; j < kVWords / 4; ++j) {
+            const uint4 x = load_once(src + j * 128 + g * 16);
+            vf[i][4 * j] = x.x;
+            vf[i][4 * j + 1] = x.y;
+            vf[i][4 * j + 2] = x.z;
+            vf[i][4 * j + 3] = x.w;
+          }
+        }
+      }
+    };
+    long long row = 0, row_next = 0;
+    int page_next = 0;
+    if (key0 < key_end) {
+      row = row_of(page_at(key0), key0);
+      page_next = page_at(key0 + kUnitKeys);
+      load_k(row);
+      load_v(row);
+    }
+    for (; key0 < key_end; key0 += kUnitKeys) {
+      const bool more = key0 + kUnitKeys < key_end;
+      row_next = row_of(page_next, key0 + kUnitKeys);
+      page_next = page_at(key0 + 2 * kUnitKeys);
+      // scores, in log2: [key g | g + 8][row 2c | 2c + 1]
+      float sc[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+#pragma unroll
+      for (int j = 0; j < kKLoads; ++j) {
+        const uint32_t w0[4] = {kf[0][j].x, kf[0][j].y, kf[0][j].z, kf[0][j].w}, w1[4] = {kf[1][j].x, kf[1][j].y, kf[1][j].z, kf[1][j].w};
+        if constexpr (k8) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t a0 = e4m3x2_to_f16x2(w0[i] & 0xffffu), a1 = e4m3x2_to_f16x2(w1[i] & 0xffffu);
+            const uint32_t a2 = e4m3x2_to_f16x2(w0[i] >> 16), a3 = e4m3x2_to_f16x2(w1[i] >> 16);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16816<C>(sc[nt], a0, a1, a2, a3, q[nt][4 * j + i][0], q[nt][4 * j + i][1]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma16816<C>(sc[nt], w0[2 * i], w1[2 * i], w0[2 * i + 1], w1[2 * i + 1], q[nt][2 * j + i][0], q[nt][2 * j + i][1]);
+        }
+      }
+      float inv0 = 1.f, inv1 = 1.f, add0 = 0.f, add1 = 0.f;
+      if constexpr (k8) {
+        const float s0 = exponent_scale(ke[0]), s1 = exponent_scale(ke[1]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          sc[nt][0] *= s0;
+          sc[nt][1] *= s0;
+          sc[nt][2] *= s1;
+          sc[nt][3] *= s1;
+        }
+        add0 = static_cast<float>(ve[0] - 127);
+        add1 = static_cast<float>(ve[1] - 127);
+        inv0 = exponent_scale(max(0, 254 - ve[0]));
+        inv1 = exponent_scale(max(0, 254 - ve[1]));
+      }
+      if (more) load_k(row_next);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[nt][i] = fmaf(sc[nt][i], factor[nt][i & 1], i < 2 ? add0 : add1);
+      const bool edge = key0 + 15 > all_hi || key0 < all_lo;
+      if (edge) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = key0 + g + (i >> 1) * 8;
+            if (key > see_hi[nt][i & 1] || key < see_lo[nt][i & 1]) sc[nt][i] = -INFINITY;
+          }
+      }
+      bool above = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) above |= sc[nt][i] > m[nt][i & 1] + kAbove;
+      if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float keep[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = fmaxf(sc[nt][e], sc[nt][2 + e]);
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            x = fmaxf(x, m[nt][e]);
+            keep[e] = exp2_fast(m[nt][e] - x);
+            m[nt][e] = x;
+            l[nt][e] *= keep[e];
+          }
+#pragma unroll
+          for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) oacc[i][nt][e] *= keep[e & 1];
+        }
+      }
+      uint32_t p[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = exp2_fast(sc[nt][i] - m[nt][i & 1]);
+        l[nt][0] += fmaf(e[0], inv0, e[2] * inv1);
+        l[nt][1] += fmaf(e[1], inv0, e[3] * inv1);
+        p[nt][0] = transpose8x8(Fmt<C>::pack2(e[0], e[1]));
+        p[nt][1] = transpose8x8(Fmt<C>::pack2(e[2], e[3]));
+      }
+      if (key0 < lo || key0 + 15 >= hi) {  // rows that nobody sees may hold anything: 0 * NaN is NaN
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = key0 + 2 * c + (i & 1) + (i >> 1) * 8;
+          if (key < lo || key >= hi) {
+#pragma unroll
+            for (int w = 0; w < kVWords; ++w) vf[i][w] = 0u;
+          }
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < kVWords; ++w) {
+        if constexpr (k8) {
+          const uint32_t x01 = __byte_perm(vf[0][w], vf[1][w], 0x5140), x23 = __byte_perm(vf[0][w], vf[1][w], 0x7362);
+          const uint32_t y01 = __byte_perm(vf[2][w], vf[3][w], 0x5140), y23 = __byte_perm(vf[2][w], vf[3][w], 0x7362);
+          const uint32_t a0 = e4m3x2_to_f16x2(x01 & 0xffffu), a1 = e4m3x2_to_f16x2(x01 >> 16);
+          const uint32_t a2 = e4m3x2_to_f16x2(y01 & 0xffffu), a3 = e4m3x2_to_f16x2(y01 >> 16);
+          const uint32_t b0 = e4m3x2_to_f16x2(x23 & 0xffffu), b1 = e4m3x2_to_f16x2(x23 >> 16);
+          const uint32_t b2 = e4m3x2_to_f16x2(y23 & 0xffffu), b3 = e4m3x2_to_f16x2(y23 >> 16);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma16816<C>(oacc[2 * w][nt], a0, a1, a2, a3, p[nt][0], p[nt][1]);
+            mma16816<C>(oacc[2 * w + 1][nt], b0, b1, b2, b3, p[nt][0], p[nt][1]);
+          }
+        } else {
+          const uint32_t a0 = __byte_perm(vf[0][w], vf[1][w], 0x5410), a1 = __byte_perm(vf[0][w], vf[1][w], 0x7632);
+          const uint32_t a2 = __byte_perm(vf[2][w], vf[3][w], 0x5410), a3 = __byte_perm(vf[2][w], vf[3][w], 0x7632);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma16816<C>(oacc[w][nt], a0, a1, a2, a3, p[nt][0], p[nt][1]);
+        }
+      }
+      if (more) load_v(row_next);
+    }
+
+    // ---- the four warps' results
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = l[nt][e];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        const int r = nt * 8 + 2 * c + e;
+        if (g == 0) {
+          mg.m[warp][r] = m[nt][e];
+          mg.l[warp][r] = x;
+        }
+        // rows g and g + 8 of product i are numbers d and d + 1 of the output
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          const int d = kVWords == 2 ? g * 8 + 2 * i : (i >> (k8 ? 3 : 2)) * (k8 ? 128 : 64) + g * (k8 ? 16 : 8) + (i & (k8 ? 7 : 3)) * 2;
+          *reinterpret_cast<float2*>(&mg.o[warp][r][d]) = make_float2(oacc[i][nt][e], oacc[i][nt][2 + e]);
+        }
+      }
+    if (threadIdx.x < R) s_odd[threadIdx.x] = 0;
+    __syncthreads();
+    const bool whole = r0 == 0 && r1 == s.units;
+    float* part = parts + (static_cast<long long>(blockIdx.x) * 2 + (r0 == 0 ? 1 : 0)) * (R * (D + 2));
+    for (int i = threadIdx.x; i < R * (D / 4); i += kWarps * 32) {
+      const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+      if (r >= rows) break;
+      float top = mg.m[0][r];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, mg.m[w][r]);
+      float sum = 0.f;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float k = exp2_fast(mg.m[w][r] - top);
+        const float4 y = *reinterpret_cast<const float4*>(&mg.o[w][r][d]);
+        sum = fmaf(mg.l[w][r], k, sum);
+        x.x = fmaf(y.x, k, x.x);
+        x.y = fmaf(y.y, k, x.y);
+        x.z = fmaf(y.z, k, x.z);
+        x.w = fmaf(y.w, k, x.w);
+      }
+      if (whole) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        x.x *= inv;
+        x.y *= inv;
+        x.z *= inv;
+        x.w *= inv;
+        const float all = x.x + x.y + x.z + x.w;
+        if (all != all) s_odd[r] = 1;
+        const long long flat = flat0 + r, t = s.first + flat / a.group, head = h * a.group + flat % a.group;
+        *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + (t * a.kv_heads * a.group + head) * D + d) =
+            make_uint2(Fmt<T>::pack2(x.x, x.y), Fmt<T>::pack2(x.z, x.w));
+      } else {
+        *reinterpret_cast<float4*>(part + r * D + d) = x;
+        if (d == 0) {
+          part[R * D + 2 * r] = top;
+          part[R * D + 2 * r + 1] = sum;
+        }
+      }
+    }
+    __syncthreads();
+    if (whole) {
+      for (int r = warp; r < rows; r += kWarps) {
+        const long long flat = flat0 + r;
+        const int t = s.first + static_cast<int>(flat / a.group);
+        const long long pos = s.pos0 + t;
+        if (s_odd[r] != 0 && hides(a, pos, lo, hi))
+          attend_row<T, k8, D>(a, b, t, h * a.group + static_cast<int>(flat % a.group), pos, &mg.o[warp][0][0], lane);
+      }
+      __syncthreads();
+    }
+    u += r1 - r0;
+  }
+}
+
+// Tiles that the cuts went through.  Block (g, y): if cut g is the first one inside a tile, rows y * 4 .. + 3 of that tile.
+template <typename T, bool k8, int D, int NT>
+__global__ void __launch_bounds__(kLineThreads)
+paged_join_kernel(PagedAttn a, int most_pieces, const float* __restrict__ parts) {
+  constexpr int R = NT * 8, kPart = R * (D + 2), kRows = kLineThreads / (D / 4);
+  __shared__ int s_odd[kRows];
+  __shared__ float s_q[kLineThreads / 32][D];
+  const int cut = blockIdx.x + 1;
+  int b;
+  long long at;
+  // (starts and lens were there before the kernel in front began, which lets this one start only behind its own wait)
+  const PagedLine line = paged_line<R, kUnitKeys>(a, cut, most_pieces, kAtLeast, &b, &at);
+  bool mine = cut < line.pieces;
+  PagedSeq s;
+  long long tile0 = 0;
+  int index = 0;
+  if (mine) {
+    s = paged_sequence<R, kUnitKeys>(a, b);
+    const long long u = piece_begin(line, cut);
+    index = static_cast<int>((u - at) / s.units);
+    tile0 = at + static_cast<long long>(index) * s.units;
+    mine = u > tile0 && piece_begin(line, cut - 1) <= tile0;
+  }
+  if (threadIdx.x < kRows) s_odd[threadIdx.x] = 0;
+  __syncthreads();
+  grid_dependency_wait();
+  grid_launch_dependents();
+  if (!mine) return;
+  const long long tile1 = tile0 + s.units;
+  int last = cut;  // the last piece with a part of the tile
+  while (last + 1 < line.pieces && piece_begin(line, last + 1) < tile1) ++last;
+  const int h = index / s.tiles, tile = index - h * s.tiles;
+  const long long flat0 = static_cast<long long>(tile) * R, flats = static_cast<long long>(s.n) * a.group;
+  const int rows = static_cast<int>(min(static_cast<long long>(R), flats - flat0));
+  const int sub = threadIdx.x / (D / 4), r = blockIdx.y * kRows + sub, d = (threadIdx.x - sub * (D / 4)) * 4;
+  const long long flat = flat0 + r;
+  const int t = s.first + static_cast<int>(flat / a.group), head = h * a.group + static_cast<int>(flat % a.group);
+  if (r < rows) {
+    // piece cut - 1 left the tile's beginning (its second place), the others what follows (their first)
+    auto part = [&](int piece) { return parts + (static_cast<long long>(piece) * 2 + (piece == cut - 1 ? 1 : 0)) * kPart; };
+    float top = -FLT_MAX;
+    for (int i = cut - 1; i <= last; ++i) top = fmaxf(top, part(i)[R * D + 2 * r]);
+    float sum = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = cut - 1; i <= last; ++i) {
+      const float* p = part(i);
+      const float2 ml = *reinterpret_cast<const float2*>(p + R * D + 2 * r);
+      const float4 y = *reinterpret_cast<const float4*>(p + r * D + d);
+      const float k = exp2_fast(ml.x - top);
+      sum = fmaf(ml.y, k, sum);
+      x.x = fmaf(y.x, k, x.x);
+      x.y = fmaf(y.y, k, x.y);
+      x.z = fmaf(y.z, k, x.z);
+      x.w = fmaf(y.w, k, x.w);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    x.x *= inv;
+    x.y *= inv;
+    x.z *= inv;
+    x.w *= inv;
+    const float all = x.x + x.y + x.z + x.w;
+    if (all != all) s_odd[sub] = 1;
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + (static_cast<long long>(t) * a.kv_heads * a.group + head) * D + d) =
+        make_uint2(Fmt<T>::pack2(x.x, x.y), Fmt<T>::pack2(x.z, x.w));
+  }
+  __syncthreads();
+  const int warp = threadIdx.x >> 5;
+  for (int i = warp; i < kRows; i += kLineThreads / 32) {
+    const int ri = blockIdx.y * kRows + i;
+    if (ri >= rows || s_odd[i] == 0) continue;
+    const long long f = flat0 + ri, first_pos = s.pos0 + s.first + flat0 / a.group, last_pos = s.pos0 + s.first + (flat0 + rows - 1) / a.group;
+    const int hi = static_cast<int>(min(static_cast<long long>(s.hi), max(0ll, last_pos + 1)));
+    const int lo = a.window > 0 ? static_cast<int>(min(static_cast<long long>(hi), max(0ll, first_pos - a.window + 1))) : 0;
+    const int ti = s.first + static_cast<int>(f / a.group);
+    if (hides(a, s.pos0 + ti, lo, hi))
+      attend_row<T, k8, D>(a, b, ti, h * a.group + static_cast<int>(f % a.group), s.pos0 + ti, s_q[warp], threadIdx.x & 31);
+  }
+}
+
+constexpr int blocks_per_sm(int nt) { return nt == 1 ? 3 : 2; }
+
+template <typename T, bool k8, int D, int NT>
+int launch(const PagedAttn& a, float* parts, cudaStream_t stream) {
+  static std::atomic<unsigned long long> configured{0};
+  auto kfn = paged_short_kernel<T, k8, D, NT>;
+  constexpr int kSmem = sizeof(Merge<D, NT>);
+  if (!ensure_dynamic_smem(kfn, kSmem, configured)) return FTB_ERR_LAUNCH;
+  const int pieces = current_sm_count() * blocks_per_sm(NT);
+  cudaError_t err = launch_dependent(kfn, dim3(pieces), dim3(kWarps * 32), kSmem, stream, a, pieces, parts);
+  count_launch();
+  if (err == cudaSuccess) {
+    constexpr int kRows = kLineThreads / (D / 4);
+    err = launch_dependent(paged_join_kernel<T, k8, D, NT>, dim3(pieces - 1, NT * 8 / kRows), dim3(kLineThreads), 0, stream, a, pieces,
+                           static_cast<const float*>(parts));
+    count_launch();
+  }
+  if (err != cudaSuccess) cudaGetLastError();
+  return err == cudaSuccess ? FTB_OK : FTB_ERR_LAUNCH;
+}
+template <typename T, int D, int NT>
+int launch(const PagedAttn& a, float* parts, cudaStream_t stream) {
+  return a.k_exp != nullptr ? launch<T, true, D, NT>(a, parts, stream) : launch<T, false, D, NT>(a, parts, stream);
+}
+template <typename T, int D>
+int launch(const PagedAttn& a, int nt, float* parts, cudaStream_t stream) {
+  return nt == 1 ? launch<T, D, 1>(a, parts, stream) : launch<T, D, 2>(a, parts, stream);
+}
+
+}  // namespace
+
+size_t paged_short_scratch_bytes(int nt, int d) {
+  return static_cast<size_t>(current_sm_count()) * blocks_per_sm(nt) * 2 * (nt * 8) * (d + 2) * sizeof(float);
+}
+
+int paged_short_launch(const PagedAttn& a, int d, int dtype, int nt, float* parts, cudaStream_t stream) {
+  if (dtype == FTB_F16) return d == 128 ? launch<__half, 128>(a, nt, parts, stream) : launch<__half, 64>(a, nt, parts, stream);
+  return d == 128 ? launch<__nv_bfloat16, 128>(a, nt, parts, stream) : launch<__nv_bfloat16, 64>(a, nt, parts, stream);
+}
+
+}  // namespace ftb

@@ -109,13 +109,15 @@ def tolerance(o, bound, dtype, d, eight_bit, keys):
     cache), which moves the result by that much of the sum of weight * |value|, and the sum of weights in 32 bits by the rest; scores in
     32 bits: (d + 4) additions and products, each off by half a step (2^-24) of at most scale * sum |q| |k|, in numerator and sum of
     the weights, and 2^-21 for two exponentials; fp16 weights, the largest of them 1 or more, are off by up to half of its
-    smallest number (2^-25) each."""
+    smallest number (2^-25) each.  Over an 8-bit cache a weight carries its value's scale, the sizes of a row's largest number
+    and of its scale being less than 2^9 apart where 448 is not reached by a factor below 2: 2^-24 of the largest value; the scale's
+    exponent (below 2^7) is added to the score, off by half a step of their sum (2^-17 with what the sum reaches)."""
     mean, size, most = bound
     eps = torch.finfo(dtype).eps
     weights = torch.finfo(torch.float16).eps if eight_bit else eps
-    score = (2 * (d + 4) * 2.0 ** -24 * size + 2.0 ** -21)[..., None]
+    score = (2 * (d + 4) * 2.0 ** -24 * size + 2.0 ** -21 + (2.0 ** -16 if eight_bit else 0.0))[..., None]
     tol = eps / 2 * o.abs() + (weights / 2 + 2 * score + 2.0 ** -20) * mean
     if eight_bit or dtype == torch.float16:
-        tol = tol + keys * 2.0 ** -25 * most[..., None]
+        tol = tol + keys * 2.0 ** (-24 if eight_bit else -25) * most[..., None]
         tol = tol + 2.0 ** -25  # half of fp16's smallest number, of results that are smaller still
     return tol * (1 + eps)
