@@ -1,0 +1,17 @@
+// The two kernels of the attention over a paged cache.  Both leave partial tiles in scratch: two places for each of their pieces
+// (part_floats numbers each), then a PagedCut for each piece.
+#pragma once
+#include <cuda_runtime.h>
+#include <stddef.h>
+
+namespace ftb {
+struct PagedAttn;
+
+// Few rows (paged_short.cu); nt: rows of a tile / 8, 1 or 2.
+int paged_short_pieces(int nt);
+int paged_short_launch(const PagedAttn& a, int d, int dtype, int nt, void* scratch, cudaStream_t stream);
+
+// Many rows (paged_tile.cu): tiles of 128 or 256.
+int paged_tile_pieces();
+int paged_tile_launch(const PagedAttn& a, int d, int dtype, int rows, void* scratch, cudaStream_t stream);
+}  // namespace ftb

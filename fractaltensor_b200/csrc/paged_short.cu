@@ -22,7 +22,7 @@
 
 #include "../../include/ftb200.h"
 #include "paged_work.cuh"
-#include "paged_short.h"
+#include "paged_forms.h"
 #include "tmap.h"
 
 namespace ftb {
@@ -65,48 +65,47 @@ struct Merge {
   float m[kWarps][NT * 8], l[kWarps][NT * 8];
 };
 
+constexpr int blocks_per_sm(int nt) { return nt == 1 ? 3 : 2; }
+
 template <typename T, bool k8, int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
-paged_short_kernel(PagedAttn a, int most_pieces, float* __restrict__ parts) {
+__global__ void __launch_bounds__(kWarps * 32, blocks_per_sm(NT))
+paged_short_kernel(PagedAttn a, float* __restrict__ parts, PagedCut* __restrict__ cuts) {
   using C = typename std::conditional<k8, __half, T>::type;
   constexpr int R = NT * 8, kSteps = D / 16, kKLoads = k8 ? D / 64 : D / 32;
   constexpr int kVWords = k8 ? D / 32 : D / 16;  // 32-bit words of one key's values a lane
   extern __shared__ __align__(16) unsigned char smem[];
   Merge<D, NT>& mg = *reinterpret_cast<Merge<D, NT>*>(smem);
   __shared__ int s_odd[R];
+  __shared__ PagedLineRoom s_line;
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  const int piece = blockIdx.x;
   grid_dependency_wait();
   grid_launch_dependents();
-  int b;
-  long long at;
-  const PagedLine line = paged_line<R, kUnitKeys>(a, blockIdx.x, most_pieces, kAtLeast, &b, &at);
-  if (static_cast<int>(blockIdx.x) >= line.pieces) return;
-  long long u = piece_begin(line, blockIdx.x);
-  const long long u_end = piece_begin(line, blockIdx.x + 1);
-  const int page_mask = (1 << a.batch.page_shift) - 1;
-  PagedSeq s = paged_sequence<R, kUnitKeys>(a, b < a.batch.B ? b : 0);
-
-  while (u < u_end) {
-    // the tile that unit u belongs to
-    long long cost = static_cast<long long>(s.tiles) * a.kv_heads * s.units;
-    while (u >= at + cost) {
-      at += cost;
-      s = paged_sequence<R, kUnitKeys>(a, ++b);
-      cost = static_cast<long long>(s.tiles) * a.kv_heads * s.units;
+  PagedWalk<R, kUnitKeys> walk;
+  {
+    int b;
+    long long at;
+    const PagedLine line = paged_line<R, kUnitKeys>(a, piece, gridDim.x, kAtLeast, s_line, &b, &at);
+    if (piece >= line.pieces || line.total == 0) {
+      if (threadIdx.x == 0) cuts[piece].last = -1;
+      return;
     }
-    const long long off = u - at;
-    const int index = static_cast<int>(off / s.units), r0 = static_cast<int>(off - static_cast<long long>(index) * s.units);
-    const int r1 = static_cast<int>(min(static_cast<long long>(s.units), r0 + (u_end - u)));
-    const int h = index / s.tiles, tile = index - h * s.tiles;
-    const long long flat0 = static_cast<long long>(tile) * R, flats = static_cast<long long>(s.n) * a.group;
-    const int rows = static_cast<int>(min(static_cast<long long>(R), flats - flat0));
-    const int* table = a.batch.table + static_cast<long long>(b) * a.batch.W;
-    // keys that the tile's rows see: [lo, hi)
+    walk.begin(a, line, piece, b, at);
+  }
+  const int page_mask = (1 << a.batch.page_shift) - 1;
+
+  for (bool first_tile = true; walk.more(); first_tile = false) {
+    const PagedTile w = walk.next(a);
+    const PagedSeq& s = walk.s;
+    const int h = w.h, rows = w.rows, flat0 = w.flat0, lo = w.keys.lo, hi = w.keys.hi;
+    const int* table = a.batch.table + static_cast<long long>(w.b) * a.batch.W;
     const long long first_pos = s.pos0 + s.first + flat0 / a.group, last_pos = s.pos0 + s.first + (flat0 + rows - 1) / a.group;
-    const int hi = static_cast<int>(min(static_cast<long long>(s.hi), max(0ll, last_pos + 1)));
-    const int lo = a.window > 0 ? static_cast<int>(min(static_cast<long long>(hi), max(0ll, first_pos - a.window + 1))) : 0;
-    const int unit0 = s.lo / kUnitKeys;
+    if (first_tile && threadIdx.x == 0) {
+      const int last = last_piece_of(walk.line, piece, w);
+      cuts[piece].last = last;
+      if (last >= 0) cuts[piece] = PagedCut{last, w.b, s.first, flat0, rows, h, lo, hi, s.pos0};
+    }
 
     // ---- queries: lane (g, c) holds of row g what it holds of a key; limits and factors of rows 2c and 2c + 1
     uint32_t q[NT][kSteps][2];
@@ -115,10 +114,9 @@ paged_short_kernel(PagedAttn a, int most_pieces, float* __restrict__ parts) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int row = nt * 8 + g;
-      const long long flat = flat0 + row;
-      const int token = static_cast<int>(flat / a.group);
+      const int flat = flat0 + row, token = flat / a.group;
       const T* src = static_cast<const T*>(a.q) + static_cast<long long>(s.first + token) * a.q_row +
-                     (h * a.group + static_cast<int>(flat - static_cast<long long>(token) * a.group)) * a.q_head;
+                     static_cast<long long>(h * a.group + flat - token * a.group) * a.q_head;
       uint4 x[D / 32];
 #pragma unroll
       for (int j = 0; j < D / 32; ++j) {
@@ -161,7 +159,7 @@ paged_short_kernel(PagedAttn a, int most_pieces, float* __restrict__ parts) {
       for (int e = 0; e < 2; ++e) {
         factor[nt][e] = __shfl_sync(0xffffffffu, mine, (2 * c + e) * 4);
         const int r = nt * 8 + 2 * c + e;
-        const long long pos = r < rows ? s.pos0 + s.first + (flat0 + r) / a.group : -1;
+        const long long pos = r < rows ? s.pos0 + s.first + (flat0 + r) / a.group : -1ll;
         see_hi[nt][e] = static_cast<int>(max(-1ll, min(pos, static_cast<long long>(hi) - 1)));
         see_lo[nt][e] = a.window > 0 ? static_cast<int>(max(0ll, min(pos - a.window + 1, static_cast<long long>(INT_MAX)))) : 0;
       }
@@ -180,9 +178,9 @@ paged_short_kernel(PagedAttn a, int most_pieces, float* __restrict__ parts) {
     }
 
     // ---- the walk
-    int key0 = (unit0 + r0) * kUnitKeys + warp * 16;
-    if (key0 + 15 < lo) key0 += (lo - key0) / kUnitKeys * kUnitKeys;
-    const int key_end = min(hi, (unit0 + r1) * kUnitKeys);
+    int key0 = (lo / kUnitKeys + w.r0) * kUnitKeys + warp * 16;
+    if (key0 + 15 < lo) key0 += kUnitKeys;  // (pages in front of the window need not be there)
+    const int key_end = min(hi, (lo / kUnitKeys + w.r1) * kUnitKeys);
     auto row_of = [&](int page, int key) {  // the cache row of key: a page that the table does not have reads as page 0
       return ((static_cast<long long>(page) * a.kv_heads + h) << a.batch.page_shift) + (key & page_mask);
     };
@@ -387,8 +385,8 @@ paged_short_kernel(PagedAttn a, int most_pieces, float* __restrict__ parts) {
       }
     if (threadIdx.x < R) s_odd[threadIdx.x] = 0;
     __syncthreads();
-    const bool whole = r0 == 0 && r1 == s.units;
-    float* part = parts + (static_cast<long long>(blockIdx.x) * 2 + (r0 == 0 ? 1 : 0)) * (R * (D + 2));
+    const bool whole = w.r0 == 0 && w.r1 == w.units;
+    float* part = parts + (static_cast<long long>(piece) * 2 + (w.r0 == 0 ? 1 : 0)) * part_floats<R, D>();
     for (int i = threadIdx.x; i < R * (D / 4); i += kWarps * 32) {
       const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
       if (r >= rows) break;
@@ -415,8 +413,8 @@ paged_short_kernel(PagedAttn a, int most_pieces, float* __restrict__ parts) {
         x.w *= inv;
         const float all = x.x + x.y + x.z + x.w;
         if (all != all) s_odd[r] = 1;
-        const long long flat = flat0 + r, t = s.first + flat / a.group, head = h * a.group + flat % a.group;
-        *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + (t * a.kv_heads * a.group + head) * D + d) =
+        const int flat = flat0 + r, t = s.first + flat / a.group, head = h * a.group + flat % a.group;
+        *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + (static_cast<long long>(t) * a.kv_heads * a.group + head) * D + d) =
             make_uint2(Fmt<T>::pack2(x.x, x.y), Fmt<T>::pack2(x.z, x.w));
       } else {
         *reinterpret_cast<float4*>(part + r * D + d) = x;
@@ -429,136 +427,46 @@ paged_short_kernel(PagedAttn a, int most_pieces, float* __restrict__ parts) {
     __syncthreads();
     if (whole) {
       for (int r = warp; r < rows; r += kWarps) {
-        const long long flat = flat0 + r;
-        const int t = s.first + static_cast<int>(flat / a.group);
+        const int flat = flat0 + r, t = s.first + flat / a.group;
         const long long pos = s.pos0 + t;
         if (s_odd[r] != 0 && hides(a, pos, lo, hi))
-          attend_row<T, k8, D>(a, b, t, h * a.group + static_cast<int>(flat % a.group), pos, &mg.o[warp][0][0], lane);
+          attend_row<T, k8, D>(a, w.b, t, h * a.group + flat % a.group, pos, lane, 0, D);
       }
       __syncthreads();
     }
-    u += r1 - r0;
   }
 }
 
-// Tiles that the cuts went through.  Block (g, y): if cut g is the first one inside a tile, rows y * 4 .. + 3 of that tile.
 template <typename T, bool k8, int D, int NT>
-__global__ void __launch_bounds__(kLineThreads)
-paged_join_kernel(PagedAttn a, int most_pieces, const float* __restrict__ parts) {
-  constexpr int R = NT * 8, kPart = R * (D + 2), kRows = kLineThreads / (D / 4);
-  __shared__ int s_odd[kRows];
-  __shared__ float s_q[kLineThreads / 32][D];
-  const int cut = blockIdx.x + 1;
-  int b;
-  long long at;
-  // (starts and lens were there before the kernel in front began, which lets this one start only behind its own wait)
-  const PagedLine line = paged_line<R, kUnitKeys>(a, cut, most_pieces, kAtLeast, &b, &at);
-  bool mine = cut < line.pieces;
-  PagedSeq s;
-  long long tile0 = 0;
-  int index = 0;
-  if (mine) {
-    s = paged_sequence<R, kUnitKeys>(a, b);
-    const long long u = piece_begin(line, cut);
-    index = static_cast<int>((u - at) / s.units);
-    tile0 = at + static_cast<long long>(index) * s.units;
-    mine = u > tile0 && piece_begin(line, cut - 1) <= tile0;
-  }
-  if (threadIdx.x < kRows) s_odd[threadIdx.x] = 0;
-  __syncthreads();
-  grid_dependency_wait();
-  grid_launch_dependents();
-  if (!mine) return;
-  const long long tile1 = tile0 + s.units;
-  int last = cut;  // the last piece with a part of the tile
-  while (last + 1 < line.pieces && piece_begin(line, last + 1) < tile1) ++last;
-  const int h = index / s.tiles, tile = index - h * s.tiles;
-  const long long flat0 = static_cast<long long>(tile) * R, flats = static_cast<long long>(s.n) * a.group;
-  const int rows = static_cast<int>(min(static_cast<long long>(R), flats - flat0));
-  const int sub = threadIdx.x / (D / 4), r = blockIdx.y * kRows + sub, d = (threadIdx.x - sub * (D / 4)) * 4;
-  const long long flat = flat0 + r;
-  const int t = s.first + static_cast<int>(flat / a.group), head = h * a.group + static_cast<int>(flat % a.group);
-  if (r < rows) {
-    // piece cut - 1 left the tile's beginning (its second place), the others what follows (their first)
-    auto part = [&](int piece) { return parts + (static_cast<long long>(piece) * 2 + (piece == cut - 1 ? 1 : 0)) * kPart; };
-    float top = -FLT_MAX;
-    for (int i = cut - 1; i <= last; ++i) top = fmaxf(top, part(i)[R * D + 2 * r]);
-    float sum = 0.f;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = cut - 1; i <= last; ++i) {
-      const float* p = part(i);
-      const float2 ml = *reinterpret_cast<const float2*>(p + R * D + 2 * r);
-      const float4 y = *reinterpret_cast<const float4*>(p + r * D + d);
-      const float k = exp2_fast(ml.x - top);
-      sum = fmaf(ml.y, k, sum);
-      x.x = fmaf(y.x, k, x.x);
-      x.y = fmaf(y.y, k, x.y);
-      x.z = fmaf(y.z, k, x.z);
-      x.w = fmaf(y.w, k, x.w);
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    x.x *= inv;
-    x.y *= inv;
-    x.z *= inv;
-    x.w *= inv;
-    const float all = x.x + x.y + x.z + x.w;
-    if (all != all) s_odd[sub] = 1;
-    *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + (static_cast<long long>(t) * a.kv_heads * a.group + head) * D + d) =
-        make_uint2(Fmt<T>::pack2(x.x, x.y), Fmt<T>::pack2(x.z, x.w));
-  }
-  __syncthreads();
-  const int warp = threadIdx.x >> 5;
-  for (int i = warp; i < kRows; i += kLineThreads / 32) {
-    const int ri = blockIdx.y * kRows + i;
-    if (ri >= rows || s_odd[i] == 0) continue;
-    const long long f = flat0 + ri, first_pos = s.pos0 + s.first + flat0 / a.group, last_pos = s.pos0 + s.first + (flat0 + rows - 1) / a.group;
-    const int hi = static_cast<int>(min(static_cast<long long>(s.hi), max(0ll, last_pos + 1)));
-    const int lo = a.window > 0 ? static_cast<int>(min(static_cast<long long>(hi), max(0ll, first_pos - a.window + 1))) : 0;
-    const int ti = s.first + static_cast<int>(f / a.group);
-    if (hides(a, s.pos0 + ti, lo, hi))
-      attend_row<T, k8, D>(a, b, ti, h * a.group + static_cast<int>(f % a.group), s.pos0 + ti, s_q[warp], threadIdx.x & 31);
-  }
-}
-
-constexpr int blocks_per_sm(int nt) { return nt == 1 ? 3 : 2; }
-
-template <typename T, bool k8, int D, int NT>
-int launch(const PagedAttn& a, float* parts, cudaStream_t stream) {
+int launch(const PagedAttn& a, void* scratch, cudaStream_t stream) {
   static std::atomic<unsigned long long> configured{0};
   auto kfn = paged_short_kernel<T, k8, D, NT>;
   constexpr int kSmem = sizeof(Merge<D, NT>);
   if (!ensure_dynamic_smem(kfn, kSmem, configured)) return FTB_ERR_LAUNCH;
-  const int pieces = current_sm_count() * blocks_per_sm(NT);
-  cudaError_t err = launch_dependent(kfn, dim3(pieces), dim3(kWarps * 32), kSmem, stream, a, pieces, parts);
+  const int pieces = paged_short_pieces(NT);
+  float* parts = static_cast<float*>(scratch);
+  const cudaError_t err = launch_dependent(kfn, dim3(pieces), dim3(kWarps * 32), kSmem, stream, a, parts,
+                                           reinterpret_cast<PagedCut*>(parts + 2 * pieces * part_floats<NT * 8, D>()));
   count_launch();
-  if (err == cudaSuccess) {
-    constexpr int kRows = kLineThreads / (D / 4);
-    err = launch_dependent(paged_join_kernel<T, k8, D, NT>, dim3(pieces - 1, NT * 8 / kRows), dim3(kLineThreads), 0, stream, a, pieces,
-                           static_cast<const float*>(parts));
-    count_launch();
-  }
   if (err != cudaSuccess) cudaGetLastError();
   return err == cudaSuccess ? FTB_OK : FTB_ERR_LAUNCH;
 }
 template <typename T, int D, int NT>
-int launch(const PagedAttn& a, float* parts, cudaStream_t stream) {
-  return a.k_exp != nullptr ? launch<T, true, D, NT>(a, parts, stream) : launch<T, false, D, NT>(a, parts, stream);
+int launch(const PagedAttn& a, void* scratch, cudaStream_t stream) {
+  return a.k_exp != nullptr ? launch<T, true, D, NT>(a, scratch, stream) : launch<T, false, D, NT>(a, scratch, stream);
 }
 template <typename T, int D>
-int launch(const PagedAttn& a, int nt, float* parts, cudaStream_t stream) {
-  return nt == 1 ? launch<T, D, 1>(a, parts, stream) : launch<T, D, 2>(a, parts, stream);
+int launch(const PagedAttn& a, int nt, void* scratch, cudaStream_t stream) {
+  return nt == 1 ? launch<T, D, 1>(a, scratch, stream) : launch<T, D, 2>(a, scratch, stream);
 }
 
 }  // namespace
 
-size_t paged_short_scratch_bytes(int nt, int d) {
-  return static_cast<size_t>(current_sm_count()) * blocks_per_sm(nt) * 2 * (nt * 8) * (d + 2) * sizeof(float);
-}
+int paged_short_pieces(int nt) { return current_sm_count() * blocks_per_sm(nt); }
 
-int paged_short_launch(const PagedAttn& a, int d, int dtype, int nt, float* parts, cudaStream_t stream) {
-  if (dtype == FTB_F16) return d == 128 ? launch<__half, 128>(a, nt, parts, stream) : launch<__half, 64>(a, nt, parts, stream);
-  return d == 128 ? launch<__nv_bfloat16, 128>(a, nt, parts, stream) : launch<__nv_bfloat16, 64>(a, nt, parts, stream);
+int paged_short_launch(const PagedAttn& a, int d, int dtype, int nt, void* scratch, cudaStream_t stream) {
+  if (dtype == FTB_F16) return d == 128 ? launch<__half, 128>(a, nt, scratch, stream) : launch<__half, 64>(a, nt, scratch, stream);
+  return d == 128 ? launch<__nv_bfloat16, 128>(a, nt, scratch, stream) : launch<__nv_bfloat16, 64>(a, nt, scratch, stream);
 }
 
 }  // namespace ftb

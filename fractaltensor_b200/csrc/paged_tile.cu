@@ -1,0 +1,833 @@
+// Attention over a paged cache for many rows: chunks of prompts, drafted tokens of large groups.  Tiles of query rows (token, head
+// of a group) against blocks of 128 keys on the tensor cores (tcgen05), S = Q K^T and O += P V with accumulators in tensor
+// memory, online softmax between them.
+//
+// One persistent CTA per SM walks its piece of the line of work (paged_work.cuh):
+//   warp 0        the walk, announced to the others through a ring of stretches, and the loads of K and V, page by page:
+//                 TMA boxes of a page's rows into the swizzled tiles that the products read, 8-bit pages as they are
+//   warp 1        issues the products
+//   warps 2..9    softmax: two slots of 128 threads, a thread a row; they also fetch the queries and write the results
+//   16-bit caches: warp 10 zeroes values in front of and behind the keys that the tile sees (what lies there may be
+//                 anything, and 0 * NaN is NaN)
+//   8-bit caches: warps 10..13 turn codes into fp16 tiles
+// kTwo: a tile has 256 rows, 128 to a slot, and a K or V block serves both; else 128 rows, and the slots take turns at the blocks: each
+// has sums of its own for the same rows, which lie in the same lanes of tensor memory and are put together there.
+//
+// 8-bit caches: a block's codes become fp16 numbers code * 2^(e - e_max), e_max the largest exponent of the block's keys: exact
+// where exponents are within 15 of each other, and off by 2^-33 of the block's largest number otherwise.  2^e_max goes to the
+// scores (keys) and into the weights (values, as in paged_short.cu), once a block.  bf16 queries are scaled into fp16's range, row by
+// row, by a power of two.
+#include <algorithm>
+#include <cfloat>
+#include <climits>
+#include <type_traits>
+
+#include "../../include/ftb200.h"
+#include "paged_forms.h"
+#include "paged_work.cuh"
+#include "tmap.h"
+
+namespace ftb {
+namespace {
+
+constexpr int kKeys = 128, kAtLeast = 1, kStretches = 4, kRefs = 8;
+constexpr int kMostSlots = 14;
+constexpr float kAbove = 8.f;  // as in flash_attn.cu: the maximum in use may lie 2^8 below the real one
+
+struct Stretch {
+  int b, h, flat0, rows, first, hi_all;
+  PagedKeys keys;
+  int block0, blocks;  // of 128 keys; blocks 0: nobody sees anything
+  int whole, place;    // place: of the parts, where the tile is not whole
+  long long pos0;
+  int last;            // nothing behind this one
+};
+
+template <bool k8, bool kTwo>
+struct Control {
+  PagedLineRoom line;
+  Stretch ring[kStretches];
+  uint64_t ring_full[kStretches], ring_empty[kStretches];
+  uint64_t q_full[2], s_full[2], p_full[2], pv_done[2], o_free[2], fin;
+  uint64_t kv_full[kMostSlots], kv_empty[kMostSlots];    // tiles that the products read
+  uint64_t raw_full[k8 ? kMostSlots : 1], raw_empty[k8 ? kMostSlots : 1];  // 8-bit blocks
+  uint64_t v_fixed, scales;
+  float xchg[kTwo ? 1 : 2][2][kTwo ? 1 : 128];  // [slot][maximum | sum][row]
+  int k_ref[kRefs], v_ref[kRefs];
+  int warp_max[2][4];
+  uint32_t k_scale[k8 ? 128 : 1], v_scale[k8 ? kRefs : 1][k8 ? 128 : 1];  // fp16 pairs
+  uint32_t tmem_base;
+  int abort, dead;
+};
+
+template <bool k8, int D, bool kTwo>
+struct Plan {
+  static constexpr int kHalf = 128 * 128, kTile = D / 64 * kHalf, kRaw = 128 * D;
+  static constexpr int kQ = (kTwo ? 2 : 1) * kTile;
+  static constexpr int kSmem = 232448, kControl = (sizeof(Control<k8, kTwo>) + 15) / 16 * 16;
+  static constexpr int kRoom = kSmem - 1024 - kControl - kQ;
+  // 8-bit: as many bytes on their way as converted tiles leave room for
+  static constexpr int kSlots = k8 ? (D == 128 ? (kTwo ? 3 : 4) : 6) : (kRoom / kTile < kMostSlots ? kRoom / kTile : kMostSlots);
+  static constexpr int kRawSlots = k8 ? ((kRoom - kSlots * kTile) / kRaw < kMostSlots ? (kRoom - kSlots * kTile) / kRaw : kMostSlots) : 0;
+  static constexpr int kThreads = 32 * (k8 ? 14 : 11);
+  static_assert(kSlots >= 3 && (!k8 || kRawSlots >= 3), "shared memory budget");
+};
+
+__device__ __forceinline__ void tmem_ld32p(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+
+// 16-byte piece `piece` of row `row` in a tile of 64-column halves of 128-byte swizzled rows.
+__device__ __forceinline__ uint8_t* piece_ptr(uint8_t* tile, int row, int piece) {
+  return tile + (piece >> 3) * (128 * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
+}
+
+// Tile n of the stream of K and V blocks of a stretch.  kTwo: K0, V0, K1, V1, ..; else, the slots taking turns at the blocks,
+// K0, K1, V0, K2, V1, .., the order in which the products come.
+struct StreamTile {
+  bool is_v;
+  int j;
+};
+template <bool kTwo>
+__device__ __forceinline__ StreamTile stream_tile(int n, int blocks) {
+  if (kTwo) return {(n & 1) != 0, n >> 1};
+  if (n == 0) return {false, 0};
+  if (blocks == 1) return {true, 0};
+  if (n == 1) return {false, 1};
+  const int r = n - 2, turn = 2 * (blocks - 2);
+  if (r >= turn) return {true, blocks - 2 + r - turn};
+  return {(r & 1) == 0, (r & 1) == 0 ? r >> 1 : 2 + (r >> 1)};
+}
+
+// Blocks of a stretch that slot t takes part in: of kTwo j0 .. j1, else every second one; how many.
+struct Mine {
+  int j0, j1, n;
+};
+template <bool kTwo>
+__device__ __forceinline__ Mine blocks_of_slot(const PagedAttn& a, const Stretch& x, int t) {
+  if (!kTwo) return {t, x.blocks - 1, (x.blocks - t + 1) / 2};
+  const int rows = min(128, x.rows - t * 128);
+  if (rows <= 0 || x.blocks == 0) return {0, -1, 0};
+  const PagedKeys k = keys_of_rows(a, x.pos0, x.first, x.hi_all, x.flat0 + t * 128, rows);
+  if (k.hi <= k.lo) return {0, -1, 0};
+  const int j0 = max(0, k.lo / kKeys - x.block0), j1 = min(x.blocks - 1, (k.hi - 1) / kKeys - x.block0);
+  return {j0, j1, max(0, j1 - j0 + 1)};
+}
+
+template <typename T, bool k8, int D, bool kTwo>
+__global__ void __launch_bounds__(Plan<k8, D, kTwo>::kThreads, 1)
+paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
+                  float* __restrict__ parts, PagedCut* __restrict__ cuts) {
+  using P = Plan<k8, D, kTwo>;
+  using C = typename std::conditional<k8, __half, T>::type;
+  constexpr int R = kTwo ? 256 : 128, kSlots = P::kSlots, kRawSlots = P::kRawSlots;
+  constexpr bool kKeep = !k8;  // a row's scores stay in registers between their maximum and the weights
+  extern __shared__ uint8_t smem_raw[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, piece = blockIdx.x;
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* sQ = smem;
+  uint8_t* sKV = sQ + P::kQ;
+  uint8_t* sRaw = sKV + kSlots * P::kTile;
+  Control<k8, kTwo>& ctl = *reinterpret_cast<Control<k8, kTwo>*>(sRaw + (k8 ? kRawSlots * P::kRaw : 0));
+  volatile int* s_abort = &ctl.abort;
+  int* status = a.status;
+
+  if (threadIdx.x == 0) {
+    if constexpr (!k8) {
+      prefetch_tmap(&mapK);
+      prefetch_tmap(&mapV);
+    }
+    for (int i = 0; i < kStretches; ++i) {
+      mbar_init(&ctl.ring_full[i], 1);
+      mbar_init(&ctl.ring_empty[i], 1 + 8 + (k8 ? 4 : 1));
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&ctl.q_full[i], kTwo ? 4 : 8);
+      mbar_init(&ctl.s_full[i], 1);
+      mbar_init(&ctl.p_full[i], 4);
+      mbar_init(&ctl.pv_done[i], 1);
+      mbar_init(&ctl.o_free[i], kTwo ? 4 : 8);
+    }
+    mbar_init(&ctl.fin, 8);
+    for (int i = 0; i < kMostSlots; ++i) {
+      mbar_init(&ctl.kv_full[i], k8 ? 4 : 1);
+      mbar_init(&ctl.kv_empty[i], 1);
+      if constexpr (k8) {
+        mbar_init(&ctl.raw_full[i], 1);
+        mbar_init(&ctl.raw_empty[i], 4);
+      }
+    }
+    mbar_init(&ctl.v_fixed, 1);
+    mbar_init(&ctl.scales, 4);
+    ctl.abort = 0;
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  grid_dependency_wait();
+  grid_launch_dependents();
+  if (threadIdx.x == 0) {  // an earlier wait ran out: do nothing.  (An index out of its range was that call's error.)
+    const int before = *reinterpret_cast<volatile int*>(status);
+    ctl.dead = before != 0 && before != FTB_ERR_INDEX;
+  }
+  int seq0;
+  long long at0;
+  const PagedLine line = paged_line<R, kKeys>(a, piece, gridDim.x, kAtLeast, ctl.line, &seq0, &at0);
+  const bool idle = piece >= line.pieces || line.total == 0;
+  if (idle || ctl.dead != 0) {
+    if (threadIdx.x == 0) cuts[piece].last = -1;
+    return;
+  }
+  if (warp == 1) {
+    tmem_alloc(&ctl.tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = ctl.tmem_base;
+  // tensor memory: S0 [0, 128), S1 [128, 256), O0 [256, 256 + D), O1 [384, 384 + D); P_t (16-bit pairs) over the first 64 columns of S_t.
+
+  // Stretch i of this CTA, as every role but the first warp gets it.
+  auto await = [&](int i) -> bool {
+    return mbar_wait_warp(&ctl.ring_full[i % kStretches], (i / kStretches) & 1, s_abort, status, FTB_ERR_TIMEOUT_TMA);
+  };
+  auto give_back = [&](int i) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&ctl.ring_empty[i % kStretches]);
+  };
+
+  if (warp == 0) {
+    // --------------------------------------------------------- the walk, and the loads
+    PagedWalk<R, kKeys> walk;
+    walk.begin(a, line, piece, seq0, at0);
+    const int pages = kKeys >> a.batch.page_shift;  // of a block
+    int slot = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int i = 0; ok && walk.more(); ++i) {
+      const PagedTile w = walk.next(a);
+      if (i >= kStretches && !mbar_wait_warp(&ctl.ring_empty[i % kStretches], (i / kStretches - 1) & 1, s_abort, status, FTB_ERR_TIMEOUT_SLOT)) break;
+      const bool some = w.keys.hi > w.keys.lo;
+      const int block0 = w.keys.lo / kKeys + w.r0, blocks = some ? w.r1 - w.r0 : 0;
+      if (lane == 0) {
+        Stretch& x = ctl.ring[i % kStretches];
+        x.b = w.b;
+        x.h = w.h;
+        x.flat0 = w.flat0;
+        x.rows = w.rows;
+        x.first = walk.s.first;
+        x.hi_all = walk.s.hi;
+        x.keys = w.keys;
+        x.block0 = block0;
+        x.blocks = blocks;
+        x.whole = w.r0 == 0 && w.r1 == w.units;
+        x.place = 2 * piece + (w.r0 == 0 ? 1 : 0);
+        x.pos0 = walk.s.pos0;
+        x.last = !walk.more();
+        mbar_arrive(&ctl.ring_full[i % kStretches]);
+        if (i == 0) {
+          const int last = last_piece_of(line, piece, w);
+          cuts[piece].last = last;
+          if (last >= 0) cuts[piece] = PagedCut{last, w.b, walk.s.first, w.flat0, w.rows, w.h, w.keys.lo, w.keys.hi, walk.s.pos0};
+        }
+      }
+      const int* table = a.batch.table + static_cast<long long>(w.b) * a.batch.W;
+      for (int n = 0; ok && n < 2 * blocks; ++n) {
+        const StreamTile x = stream_tile<kTwo>(n, blocks);
+        // one lane a page; those that nobody sees need not be there
+        const int key0 = (block0 + x.j) * kKeys;
+        const int p0 = w.keys.lo > key0 ? (w.keys.lo - key0) >> a.batch.page_shift : 0;
+        const int p1 = min(pages, (w.keys.hi - key0 + (1 << a.batch.page_shift) - 1) >> a.batch.page_shift);
+        const bool here = lane >= p0 && lane < p1;
+        int page = 0;
+        if (here) {
+          page = __ldg(table + (key0 >> a.batch.page_shift) + lane);
+          if (page < 0 || page >= a.batch.pages) {
+            atomicCAS(status, 0, FTB_ERR_INDEX);
+            page = 0;
+          }
+        }
+        uint64_t* full = k8 ? &ctl.raw_full[slot] : &ctl.kv_full[slot];
+        uint64_t* empty = k8 ? &ctl.raw_empty[slot] : &ctl.kv_empty[slot];
+        ok = mbar_wait_warp(empty, phase ^ 1u, s_abort, status, FTB_ERR_TIMEOUT_SLOT);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(full, ((p1 - p0) << a.batch.page_shift) * (k8 ? D : 2 * D));
+        __syncwarp();
+        if (here) {
+          if constexpr (k8) {
+            const long long at = ((static_cast<long long>(page) * a.kv_heads + w.h) << a.batch.page_shift) * D;
+            bulk_load_1d(sRaw + slot * P::kRaw + (lane << a.batch.page_shift) * D, (x.is_v ? a.v : a.k) + at, D << a.batch.page_shift, full);
+          } else {
+            const CUtensorMap* m = x.is_v ? &mapV : &mapK;
+            uint8_t* dst = sKV + slot * P::kTile + (lane << a.batch.page_shift) * 128;
+            const int y = (page * a.kv_heads + w.h) << a.batch.page_shift;
+            tma_load_2d(dst, m, full, 0, y);
+            if constexpr (D == 128) tma_load_2d(dst + P::kHalf, m, full, 64, y);
+          }
+        }
+        if (++slot == (k8 ? kRawSlots : kSlots)) {
+          slot = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------- the products
+    const bool leader = elect_one();
+    constexpr uint32_t idesc_qk = make_idesc_f16(128, 128, Fmt<C>::kind, 0, 0);
+    constexpr uint32_t idesc_pv = make_idesc_f16(128, D, Fmt<C>::kind, 0, 1);  // V is MN-major
+    const uint64_t dQ = make_sdesc_sw128(smem_u32(sQ), 16, 1024);
+    const uint64_t dK = make_sdesc_sw128(smem_u32(sKV), 16, 1024);
+    const uint64_t dV = make_sdesc_sw128(smem_u32(sKV), P::kHalf, 1024);
+    uint32_t full_bits = 0, fixed_phase = 0, p_phase[2] = {0, 0};
+    int slot = 0;  // of the next tile of the stream
+    bool ok = true;
+    auto issue_s = [&](int t, int at) {
+      const uint64_t dq = dQ + static_cast<uint64_t>(kTwo ? (t * P::kTile) >> 4 : 0), dk = dK + static_cast<uint64_t>((at * P::kTile) >> 4);
+      if (leader) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = ((k >> 2) * P::kHalf + (k & 3) * 32) >> 4;
+          umma_ss(tmem_base + t * 128, dq + off, dk + off, idesc_qk, k != 0 ? 1u : 0u);
+        }
+        umma_commit(&ctl.s_full[t]);
+      }
+    };
+    auto issue_pv = [&](int t, int at, bool first) {
+      const uint64_t dv = dV + static_cast<uint64_t>((at * P::kTile) >> 4);
+      if (leader) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          umma_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + k * 8, dv + k * (2048 >> 4), idesc_pv, (!first || k != 0) ? 1u : 0u);
+        umma_commit(&ctl.pv_done[t]);
+      }
+    };
+    auto step = [&](int at) { return at + 1 == kSlots ? 0 : at + 1; };
+    auto wait_tile = [&](int at) -> bool {
+      if (!mbar_wait_warp(&ctl.kv_full[at], (full_bits >> at) & 1u, s_abort, status, FTB_ERR_TIMEOUT_TMA)) return false;
+      full_bits ^= 1u << at;
+      return true;
+    };
+    for (int i = 0; ok; ++i) {
+      if (!await(i)) break;
+      const Stretch x = ctl.ring[i % kStretches];
+      give_back(i);
+      const Mine m[2] = {blocks_of_slot<kTwo>(a, x, 0), blocks_of_slot<kTwo>(a, x, 1)};
+      auto wait_v = [&](int at, int j) -> bool {  // values at the edges of what the tile sees have been zeroed
+        if (!wait_tile(at)) return false;
+        const int key0 = (x.block0 + j) * kKeys;
+        if (k8 || (key0 >= x.keys.lo && key0 + kKeys <= x.keys.hi)) return true;
+        const bool fine = mbar_wait_warp(&ctl.v_fixed, fixed_phase, s_abort, status, FTB_ERR_TIMEOUT_TMA);
+        fixed_phase ^= 1u;
+        return fine;
+      };
+      auto wait_p = [&](int t) -> bool {
+        if (!mbar_wait_warp(&ctl.p_full[t], p_phase[t], s_abort, status, FTB_ERR_TIMEOUT_EPI)) return false;
+        p_phase[t] ^= 1u;
+        tc_fence_after();
+        return true;
+      };
+      // the queries are there, and the results of the stretch in front have been taken out of tensor memory
+      for (int t = 0; t < (kTwo ? 2 : 1) && ok; ++t)
+        ok = mbar_wait_warp(&ctl.q_full[t], i & 1, s_abort, status, FTB_ERR_TIMEOUT_EPI) &&
+             (i == 0 || mbar_wait_warp(&ctl.o_free[t], (i - 1) & 1, s_abort, status, FTB_ERR_TIMEOUT_EPI));
+      tc_fence_after();
+      if constexpr (kTwo) {
+        if (x.blocks > 0 && ok) {
+          int k_at = slot;
+          ok = wait_tile(k_at);
+          if (ok) {
+            for (int t = 0; t < 2; ++t)
+              if (m[t].n > 0 && m[t].j0 == 0) issue_s(t, k_at);
+            if (leader) umma_commit(&ctl.kv_empty[k_at]);
+          }
+          for (int j = 0; j < x.blocks && ok; ++j) {
+            const bool more = j + 1 < x.blocks;
+            const int v_at = step(k_at), next = step(v_at);
+            ok = wait_v(v_at, j) && (!more || wait_tile(next));
+            for (int t = 0; t < 2 && ok; ++t) {
+              if (j >= m[t].j0 && j <= m[t].j1) {
+                ok = wait_p(t);
+                if (!ok) break;
+                issue_pv(t, v_at, j == m[t].j0);
+              }
+              // (the tensor pipe runs in the order of issue: S_t(j + 1) overwrites P_t only after its product)
+              if (more && j + 1 >= m[t].j0 && j + 1 <= m[t].j1) issue_s(t, next);
+            }
+            if (!ok) break;
+            if (leader) {
+              umma_commit(&ctl.kv_empty[v_at]);
+              if (more) umma_commit(&ctl.kv_empty[next]);
+            }
+            k_at = next;
+          }
+          if (ok) slot = k_at;
+        }
+      } else {
+        auto done = [&] {
+          if (leader) umma_commit(&ctl.kv_empty[slot]);
+          slot = step(slot);
+        };
+        for (int t = 0; t < 2 && t < x.blocks && ok; ++t) {
+          ok = wait_tile(slot);
+          if (!ok) break;
+          issue_s(t, slot);
+          done();
+        }
+        for (int j = 0; j < x.blocks && ok; ++j) {
+          const int t = j & 1;
+          ok = wait_v(slot, j) && wait_p(t);
+          if (!ok) break;
+          issue_pv(t, slot, j < 2);
+          done();
+          if (j + 2 < x.blocks) {
+            ok = wait_tile(slot);
+            if (!ok) break;
+            issue_s(t, slot);
+            done();
+          }
+        }
+      }
+      if (x.last) break;
+    }
+  } else if (warp < 10) {
+    // ------------------------------------------------ softmax: slot t, row r of its 128
+    const int t = (warp - 2) >> 2, quad = warp & 3, r = quad * 32 + lane;
+    const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
+    const uint32_t s_addr = lane_addr + t * 128;
+    const uint32_t o_addr = lane_addr + 256 + t * 128;
+    uint32_t s_phase = 0;
+    int pv_count[2] = {0, 0};  // products P V of the slots so far
+    int fins = 0;
+    bool ok = true;
+    for (int i = 0; ok; ++i) {
+      if (!await(i)) break;
+      const Stretch x = ctl.ring[i % kStretches];
+      give_back(i);
+      const int row = (kTwo ? t * 128 : 0) + r;     // of the tile
+      const int row0 = (kTwo ? t * 128 : 0) + quad * 32;
+      const bool busy = row0 < x.rows;              // this warp has rows
+      const bool mine = row < x.rows;
+      const int flat = x.flat0 + row, token = flat / a.group, tok = x.first + token, head = x.h * a.group + flat - token * a.group;
+      const long long pos = mine ? x.pos0 + tok : -1;
+      const int see_hi = static_cast<int>(max(-1ll, min(pos, static_cast<long long>(x.keys.hi) - 1)));
+      const int see_lo = a.window > 0 ? static_cast<int>(max(0ll, min(pos - a.window + 1, static_cast<long long>(INT_MAX)))) : 0;
+      float factor = a.scale_log2;
+
+      // ---- queries
+      if (busy) {
+        uint8_t* tile = sQ + (kTwo ? t * P::kTile : 0);
+        const T* src = static_cast<const T*>(a.q) + static_cast<long long>(tok) * a.q_row + static_cast<long long>(head) * a.q_head;
+        constexpr int kPieces = kTwo ? D / 8 : D / 16;  // that this thread writes
+        const int p0 = kTwo ? 0 : t * kPieces;
+        if constexpr (k8 && !std::is_same<T, __half>::value) {
+          uint32_t top = 0;
+          if (mine) {
+#pragma unroll
+            for (int p = 0; p < D / 8; ++p) {
+              const uint4 v = *reinterpret_cast<const uint4*>(src + p * 8);
+              const uint32_t y = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+              top = max(top, max(y & 0xffffu, y >> 16));
+            }
+          }
+          const int e = min(253, max(1, static_cast<int>(top >> 7)));
+          const float by = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+          factor *= __uint_as_float(static_cast<uint32_t>(e) << 23);
+#pragma unroll
+          for (int p = 0; p < kPieces; ++p) {
+            uint4 v = mine ? *reinterpret_cast<const uint4*>(src + (p0 + p) * 8) : make_uint4(0u, 0u, 0u, 0u);
+            uint32_t* y = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 f = unpack2<T>(y[k]);
+              y[k] = Fmt<__half>::pack2(f.x * by, f.y * by);
+            }
+            *reinterpret_cast<uint4*>(piece_ptr(tile, r, p0 + p)) = v;
+          }
+        } else {
+#pragma unroll
+          for (int p = 0; p < kPieces; ++p)
+            *reinterpret_cast<uint4*>(piece_ptr(tile, r, p0 + p)) = mine ? *reinterpret_cast<const uint4*>(src + (p0 + p) * 8) : make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_proxy_async_smem();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl.q_full[kTwo ? t : 0]);
+
+      // ---- blocks
+      const Mine m = blocks_of_slot<kTwo>(a, x, t);
+      float top = 0.f, l = 0.f;
+      for (int k = 0; k < m.n && ok; ++k) {
+        const int j = kTwo ? m.j0 + k : 2 * k + t;
+        ok = mbar_wait_warp(&ctl.s_full[t], s_phase, s_abort, status, FTB_ERR_TIMEOUT_MMA);
+        if (!ok) break;
+        s_phase ^= 1u;
+        tc_fence_after();
+        if (busy) {
+          float f = factor, add = 0.f, inv = 1.f;
+          if constexpr (k8) {
+            const int kr = ctl.k_ref[j & (kRefs - 1)], vr = ctl.v_ref[j & (kRefs - 1)];
+            f *= exponent_scale(kr);
+            add = static_cast<float>(vr - 127);
+            inv = exponent_scale(254 - vr);
+          }
+          const int key0 = (x.block0 + j) * kKeys;
+          const int lo_col = see_lo - key0, hi_col = see_hi - key0;
+          const bool cut = __any_sync(0xffffffffu, mine && (lo_col > 0 || hi_col < kKeys - 1));
+          uint32_t s[kKeep ? 128 : 64];
+          float mx = -INFINITY;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t* y = s + (kKeep ? half * 64 : 0);
+            tmem_ld32p(s_addr + half * 64, y);
+            tmem_ld32p(s_addr + half * 64 + 32, y + 32);
+            tmem_ld_wait();
+            if (cut) {
+#pragma unroll
+              for (int e = 0; e < 64; ++e)
+                if (half * 64 + e < lo_col || half * 64 + e > hi_col) y[e] = 0xff800000u;
+            }
+            float mx8[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx8[e] = fmaxf(__uint_as_float(y[e]), __uint_as_float(y[8 + e]));
+#pragma unroll
+            for (int e = 16; e < 64; e += 16)
+#pragma unroll
+              for (int q = 0; q < 8; ++q) mx8[q] = fmax3(mx8[q], __uint_as_float(y[e + q]), __uint_as_float(y[e + 8 + q]));
+            mx = fmaxf(mx, fmaxf(fmax3(mx8[0], mx8[1], mx8[2]), fmaxf(fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]))));
+          }
+          // (a row may see nothing of a block: the lowest finite number keeps its weights 0)
+          const float m_new = fmaxf(fmaf(mx, f, add), -FLT_MAX);
+          if (k == 0) {
+            top = m_new;
+          } else {
+            const bool need = m_new - top > kAbove;
+            if (__any_sync(0xffffffffu, need)) {
+              // the product in front has to be done: O is at rest then
+              ok = mbar_wait_warp(&ctl.pv_done[t], (pv_count[t] + k - 1) & 1, s_abort, status, FTB_ERR_TIMEOUT_MMA);
+              if (!ok) break;
+              tc_fence_after();
+              const float keep = need ? exp2_fast(top - m_new) : 1.f;
+              if (need) top = m_new;
+              l *= keep;
+#pragma unroll 1
+              for (int ch = 0; ch < D / 16; ++ch) {
+                uint32_t o[16];
+                tmem_ld16(o_addr + ch * 16, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                tmem_st16(o_addr + ch * 16, o);
+              }
+              tmem_st_wait();
+            }
+          }
+          const float minus = add - top;
+          float sum8[8] = {};
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t* y = s + (kKeep ? half * 64 : 0);
+            if constexpr (!kKeep) {
+              tmem_ld32p(s_addr + half * 64, y);
+              tmem_ld32p(s_addr + half * 64 + 32, y + 32);
+              tmem_ld_wait();
+              if (cut) {
+#pragma unroll
+                for (int e = 0; e < 64; ++e)
+                  if (half * 64 + e < lo_col || half * 64 + e > hi_col) y[e] = 0xff800000u;
+              }
+            }
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int c = 0; c < 16; ++c) {
+                const float p0 = exp2_fast(fmaf(__uint_as_float(y[32 * part + 2 * c]), f, minus));
+                const float p1 = exp2_fast(fmaf(__uint_as_float(y[32 * part + 2 * c + 1]), f, minus));
+                sum8[(2 * c) & 7] += p0;
+                sum8[(2 * c + 1) & 7] += p1;
+                pk[c] = Fmt<C>::pack2(p0, p1);
+              }
+              tmem_st16(s_addr + half * 32 + part * 16, pk);
+            }
+          }
+          l = fmaf(((sum8[0] + sum8[1]) + (sum8[2] + sum8[3])) + ((sum8[4] + sum8[5]) + (sum8[6] + sum8[7])), inv, l);
+          tmem_st_wait();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.p_full[t]);
+      }
+      if (!ok) break;
+      if (m.n == 0) top = -FLT_MAX;
+
+      // ---- results
+      constexpr int kCols = kTwo ? D : D / 2;  // that this thread finishes
+      const int c0 = kTwo ? 0 : t * kCols;
+      float other_m = -FLT_MAX, other_l = 0.f;
+      int n_other = 0;
+      if (!kTwo && x.blocks > 0) {
+        ctl.xchg[kTwo ? 0 : t][0][kTwo ? 0 : r] = top;
+        ctl.xchg[kTwo ? 0 : t][1][kTwo ? 0 : r] = l;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.fin);
+        n_other = blocks_of_slot<kTwo>(a, x, t ^ 1).n;
+        ok = mbar_wait_warp(&ctl.fin, fins & 1, s_abort, status, FTB_ERR_TIMEOUT_EPI);
+        ++fins;
+        if (!ok) break;
+        other_m = ctl.xchg[kTwo ? 0 : t ^ 1][0][kTwo ? 0 : r];
+        other_l = ctl.xchg[kTwo ? 0 : t ^ 1][1][kTwo ? 0 : r];
+      }
+      if (m.n > 0) ok = mbar_wait_warp(&ctl.pv_done[t], (pv_count[t] + m.n - 1) & 1, s_abort, status, FTB_ERR_TIMEOUT_MMA);
+      if (ok && n_other > 0) ok = mbar_wait_warp(&ctl.pv_done[t ^ 1], (pv_count[t ^ 1] + n_other - 1) & 1, s_abort, status, FTB_ERR_TIMEOUT_MMA);
+      if (!ok) break;
+      pv_count[t] += m.n;
+      pv_count[t ^ 1] += n_other;
+      tc_fence_after();
+      const float all_m = fmaxf(top, other_m), keep = exp2_fast(top - all_m), take = exp2_fast(other_m - all_m);
+      const float sum = l * keep + other_l * take;
+      const float scale = x.whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
+      bool odd = false;
+      if (busy) {
+        T* out = static_cast<T*>(a.o) + (static_cast<long long>(tok) * a.kv_heads * a.group + head) * D + c0;
+        float* part = parts + static_cast<size_t>(x.place) * part_floats<R, D>();
+#pragma unroll 1
+        for (int ch = 0; ch < kCols / 16; ++ch) {
+          uint32_t o[16], o2[16];
+          if (m.n > 0) tmem_ld16(o_addr + c0 + ch * 16, o);
+          if (n_other > 0) tmem_ld16(lane_addr + 256 + (t ^ 1) * 128 + c0 + ch * 16, o2);
+          tmem_ld_wait();
+          float y[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            y[e] = (m.n > 0 ? __uint_as_float(o[e]) * keep : 0.f) + (n_other > 0 ? __uint_as_float(o2[e]) * take : 0.f);
+            y[e] *= scale;
+            odd |= y[e] != y[e];
+          }
+          if (mine) {
+            if (x.whole) {
+              uint4* dst = reinterpret_cast<uint4*>(out + ch * 16);
+              dst[0] = make_uint4(Fmt<T>::pack2(y[0], y[1]), Fmt<T>::pack2(y[2], y[3]), Fmt<T>::pack2(y[4], y[5]), Fmt<T>::pack2(y[6], y[7]));
+              dst[1] = make_uint4(Fmt<T>::pack2(y[8], y[9]), Fmt<T>::pack2(y[10], y[11]), Fmt<T>::pack2(y[12], y[13]), Fmt<T>::pack2(y[14], y[15]));
+            } else {
+              float4* dst = reinterpret_cast<float4*>(part + row * D + c0 + ch * 16);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) dst[e] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
+            }
+          }
+        }
+        if (mine && !x.whole && (kTwo || t == 0)) *reinterpret_cast<float2*>(part + R * D + 2 * row) = make_float2(all_m, sum);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl.o_free[kTwo ? t : 0]);
+      // rows that something unseen has made a NaN, key by key
+      if (busy && x.whole) {
+        unsigned again = __ballot_sync(0xffffffffu, mine && odd && hides(a, pos, x.keys.lo, x.keys.hi));
+        while (again != 0) {
+          const int k = __ffs(again) - 1;
+          again &= again - 1;
+          const int flat_k = x.flat0 + row0 + k, tok_k = x.first + flat_k / a.group;
+          attend_row<T, k8, D>(a, x.b, tok_k, x.h * a.group + flat_k % a.group, x.pos0 + tok_k, lane, c0, c0 + kCols);
+        }
+      }
+      if (x.last) break;
+    }
+  } else if constexpr (!k8) {
+    // ------------------------------------------------ values that nobody of the tile sees become zeros
+    int slot = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int i = 0; ok; ++i) {
+      if (!await(i)) break;
+      const Stretch x = ctl.ring[i % kStretches];
+      give_back(i);
+      for (int n = 0; n < 2 * x.blocks && ok; ++n) {
+        const StreamTile y = stream_tile<kTwo>(n, x.blocks);
+        const int key0 = (x.block0 + y.j) * kKeys;
+        if (y.is_v && (key0 < x.keys.lo || key0 + kKeys > x.keys.hi)) {
+          ok = mbar_wait_warp(&ctl.kv_full[slot], phase, s_abort, status, FTB_ERR_TIMEOUT_TMA);
+          if (!ok) break;
+          uint8_t* tile = sKV + slot * P::kTile;
+          for (int k = lane; k < kKeys * (D / 8); k += 32) {
+            const int key = k / (D / 8), c = k - key * (D / 8);
+            if (key0 + key < x.keys.lo || key0 + key >= x.keys.hi) *reinterpret_cast<uint4*>(piece_ptr(tile, key, c)) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl.v_fixed);
+        }
+        if (++slot == kSlots) {
+          slot = 0;
+          phase ^= 1u;
+        }
+      }
+      if (x.last) break;
+    }
+  } else {
+    // ------------------------------------------------------------- codes to fp16
+    const int ct = threadIdx.x - 320, cw = warp - 10;  // this thread's key of a block
+    int slot = 0, raw = 0;
+    uint32_t phase = 0, raw_phase = 0, scale_phase = 0;
+    bool ok = true;
+    for (int i = 0; ok; ++i) {
+      if (!await(i)) break;
+      const Stretch x = ctl.ring[i % kStretches];
+      give_back(i);
+      const int* table = a.batch.table + static_cast<long long>(x.b) * a.batch.W;
+      // exponents of this thread's key of block j: both, or 0 where nobody sees it
+      auto exponents = [&](int j, int* ke, int* ve) {
+        const int key = (x.block0 + j) * kKeys + ct;
+        *ke = *ve = 0;
+        if (j >= x.blocks || key < x.keys.lo || key >= x.keys.hi) return;
+        int page = __ldg(table + (key >> a.batch.page_shift));
+        if (page < 0 || page >= a.batch.pages) page = 0;
+        const long long row = ((static_cast<long long>(page) * a.kv_heads + x.h) << a.batch.page_shift) + (key & ((1 << a.batch.page_shift) - 1));
+        *ke = a.k_exp[row];
+        *ve = a.v_exp[row];
+      };
+      int ke = 0, ve = 0;
+      if (x.blocks > 0) exponents(0, &ke, &ve);
+      for (int n = 0; n < 2 * x.blocks && ok; ++n) {
+        const StreamTile y = stream_tile<kTwo>(n, x.blocks);
+        const int ref = y.j & (kRefs - 1);
+        if (!y.is_v) {
+          // scales of the block's keys and values, relative to its largest ones
+          const int kt = __reduce_max_sync(0xffffffffu, ke == 255 ? 0 : ke), vt = __reduce_max_sync(0xffffffffu, ve == 255 ? 0 : ve);
+          if (lane == 0) {
+            ctl.warp_max[0][cw] = kt;
+            ctl.warp_max[1][cw] = vt;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl.scales);
+          ok = mbar_wait_warp(&ctl.scales, scale_phase, s_abort, status, FTB_ERR_TIMEOUT_EPI);
+          scale_phase ^= 1u;
+          if (!ok) break;
+          const int k_top = max(1, max(max(ctl.warp_max[0][0], ctl.warp_max[0][1]), max(ctl.warp_max[0][2], ctl.warp_max[0][3])));
+          const int v_top = max(1, max(max(ctl.warp_max[1][0], ctl.warp_max[1][1]), max(ctl.warp_max[1][2], ctl.warp_max[1][3])));
+          auto pair_of = [](int below) -> uint32_t {  // 2^-below as fp16, twice
+            const uint32_t h = below < 15 ? static_cast<uint32_t>(15 - below) << 10 : below <= 24 ? 1u << (24 - below) : 0u;
+            return h | (h << 16);
+          };
+          ctl.k_scale[ct] = pair_of(max(0, k_top - ke));
+          ctl.v_scale[ref][ct] = pair_of(max(0, v_top - ve));
+          if (ct == 0) {
+            ctl.k_ref[ref] = k_top;
+            ctl.v_ref[ref] = v_top;
+          }
+          exponents(y.j + 1, &ke, &ve);  // on their way
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl.scales);
+          ok = mbar_wait_warp(&ctl.scales, scale_phase, s_abort, status, FTB_ERR_TIMEOUT_EPI);
+          scale_phase ^= 1u;
+          if (!ok) break;
+        }
+        ok = mbar_wait_warp(&ctl.raw_full[raw], raw_phase, s_abort, status, FTB_ERR_TIMEOUT_TMA) &&
+             mbar_wait_warp(&ctl.kv_empty[slot], phase ^ 1u, s_abort, status, FTB_ERR_TIMEOUT_SLOT);
+        if (!ok) break;
+        const uint4* src = reinterpret_cast<const uint4*>(sRaw + raw * P::kRaw);
+        uint8_t* tile = sKV + slot * P::kTile;
+        const uint32_t* scale = y.is_v ? ctl.v_scale[ref] : ctl.k_scale;
+        const int key0 = (x.block0 + y.j) * kKeys;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const int at = k * 128 + ct, key = at / (D / 16), c = at - key * (D / 16);
+          const uint4 v = src[at];
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          const __half2 by = *reinterpret_cast<const __half2*>(&scale[key]);
+          uint32_t o[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t lo = e4m3x2_to_f16x2(w[e] & 0xffffu), hi = e4m3x2_to_f16x2(w[e] >> 16);
+            __half2 l2 = __hmul2(*reinterpret_cast<__half2*>(&lo), by), h2 = __hmul2(*reinterpret_cast<__half2*>(&hi), by);
+            o[2 * e] = *reinterpret_cast<uint32_t*>(&l2);
+            o[2 * e + 1] = *reinterpret_cast<uint32_t*>(&h2);
+          }
+          if (y.is_v && (key0 + key < x.keys.lo || key0 + key >= x.keys.hi)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = 0u;
+          }
+          *reinterpret_cast<uint4*>(piece_ptr(tile, key, 2 * c)) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(piece_ptr(tile, key, 2 * c + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&ctl.kv_full[slot]);
+          mbar_arrive(&ctl.raw_empty[raw]);
+        }
+        if (++slot == kSlots) {
+          slot = 0;
+          phase ^= 1u;
+        }
+        if (++raw == kRawSlots) {
+          raw = 0;
+          raw_phase ^= 1u;
+        }
+      }
+      if (x.last) break;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    if (ctl.abort) {
+      const uint64_t t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+    }
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+template <typename T, bool k8, int D, bool kTwo>
+int launch(const PagedAttn& a, const CUtensorMap& mK, const CUtensorMap& mV, void* scratch, cudaStream_t stream) {
+  using P = Plan<k8, D, kTwo>;
+  static std::atomic<unsigned long long> configured{0};
+  auto kfn = paged_tile_kernel<T, k8, D, kTwo>;
+  if (!ensure_dynamic_smem(kfn, P::kSmem, configured)) return FTB_ERR_LAUNCH;
+  const int pieces = paged_tile_pieces();
+  float* parts = static_cast<float*>(scratch);
+  const cudaError_t err = launch_dependent(kfn, dim3(pieces), dim3(P::kThreads), P::kSmem, stream, a, mK, mV, parts,
+                                           reinterpret_cast<PagedCut*>(parts + 2 * pieces * part_floats<kTwo ? 256 : 128, D>()));
+  count_launch();
+  if (err != cudaSuccess) cudaGetLastError();
+  return err == cudaSuccess ? FTB_OK : FTB_ERR_LAUNCH;
+}
+template <typename T, int D, bool kTwo>
+int launch(const PagedAttn& a, int dtype, void* scratch, cudaStream_t stream) {
+  CUtensorMap mK = {}, mV = {};
+  if (a.k_exp != nullptr) return launch<T, true, D, kTwo>(a, mK, mV, scratch, stream);
+  const uint64_t rows = (static_cast<uint64_t>(a.batch.pages) * a.kv_heads) << a.batch.page_shift;
+  if (rows > 0x7fffffffull) return FTB_ERR_ARG;  // a copy's coordinates have 32 bits
+  int rc;
+  if ((rc = make_tmap_2d(&mK, a.k, dtype, rows, D, D, 1u << a.batch.page_shift, 64))) return rc;
+  if ((rc = make_tmap_2d(&mV, a.v, dtype, rows, D, D, 1u << a.batch.page_shift, 64))) return rc;
+  return launch<T, false, D, kTwo>(a, mK, mV, scratch, stream);
+}
+template <typename T>
+int launch(const PagedAttn& a, int d, int dtype, bool two, void* scratch, cudaStream_t stream) {
+  if (d == 128) return two ? launch<T, 128, true>(a, dtype, scratch, stream) : launch<T, 128, false>(a, dtype, scratch, stream);
+  return two ? launch<T, 64, true>(a, dtype, scratch, stream) : launch<T, 64, false>(a, dtype, scratch, stream);
+}
+
+}  // namespace
+
+int paged_tile_pieces() { return current_sm_count(); }
+
+int paged_tile_launch(const PagedAttn& a, int d, int dtype, int rows, void* scratch, cudaStream_t stream) {
+  return dtype == FTB_F16 ? launch<__half>(a, d, dtype, rows == 256, scratch, stream)
+                          : launch<__nv_bfloat16>(a, d, dtype, rows == 256, scratch, stream);
+}
+
+}  // namespace ftb

@@ -192,6 +192,11 @@ SHAPES = [
     (1, 8, 64, 128, [257], [300], None),
     (1, 7, 128, 16, [40, 1, 90, 1], [41, 600, 333, 2], None),
     (1, 2, 128, 32, [300], [3000], None),
+    (1, 1, 128, 16, [40], [5000], None),
+    (2, 2, 128, 64, [260], [2000], None),
+    (1, 8, 64, 32, [30, 31], [4000, 900], None),
+    (1, 1, 64, 16, [600, 1, 129], [600, 40, 1000], None),
+    (3, 1, 128, 128, [128], [128], None),
     (2, 4, 128, 16, [1, 1], [500, 40], 1),
     (2, 4, 128, 16, [1, 3], [500, 40], 100),
     (1, 4, 64, 16, [200], [400], 33),
@@ -216,6 +221,24 @@ def test_attention(dtype, eight_bit, kv, group, d, page, new, lens, window):
     ops.check_status()
     assert got is out and bool((out[0] == 5.0).all()) and bool((out[-2:] == 5.0).all())
     _check(out, q, cache, table, ln, st, scale, window)
+
+
+@pytest.mark.parametrize("eight_bit", [False, True])
+@pytest.mark.parametrize("new,lens,window", [([1, 1], [700, 333], 100), ([40, 1], [700, 333], 77), ([300], [900], 130), ([20, 20], [400, 500], 64)])
+def test_pages_in_front_of_the_window_may_be_gone(eight_bit, new, lens, window):
+    ops = _ops()
+    kv, group, d, page = 2, 4, 128, 16
+    table, ln, st, pages = _batch(new, lens, page)
+    cache = _full_cache(pages, kv, page, d, E4M3 if eight_bit else BF16, 3, table, ln)
+    q = _numbers((int(st[-1]), kv * group, d), BF16, 1).cuda()
+    want = ops.paged_attention(q, cache, table.cuda(), ln.cuda(), st.cuda(), scale=0.1, window=window)
+    gone = table.clone()
+    for b, (n, m) in enumerate(zip(lens, new)):
+        gone[b, : max(0, n - m + 1 - window) // page] = -1
+    got = ops.paged_attention(q, cache, gone.cuda(), ln.cuda(), st.cuda(), scale=0.1, window=window)
+    ops.check_status()
+    assert torch.equal(got, want)
+    _check(got, q, cache, table, ln, st, 0.1, window)
 
 
 @pytest.mark.parametrize("eight_bit", [False, True])
