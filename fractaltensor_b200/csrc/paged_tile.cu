@@ -8,7 +8,7 @@
 //   warp 1        issues the products
 //   warps 2..9    softmax: two slots of 128 threads, a thread a row; they also fetch the queries and write the results
 //   16-bit caches: warp 10 zeroes values in front of and behind the keys that the tile sees (what lies there may be
-//                 anything, and 0 * NaN is NaN)
+//                 anything, and 0 * NaN is NaN), told by warp 0 which blocks need it
 //   8-bit caches: warps 10..13 turn codes into fp16 tiles
 // kTwo: a tile has 256 rows, 128 to a slot, and a K or V block serves both; else 128 rows, and the slots take turns at the blocks: each
 // has sums of its own for the same rows, which lie in the same lanes of tensor memory and are put together there.
@@ -43,15 +43,21 @@ struct Stretch {
   int last;            // nothing behind this one
 };
 
+struct Edge {  // values in ring slot `slot`, with its next fill's parity: of the keys from key0 on only lo .. hi - 1 are seen
+  int slot, key0, lo, hi;
+  uint32_t phase;
+};
+
 template <bool k8, bool kTwo>
 struct Control {
   PagedLineRoom line;
   Stretch ring[kStretches];
   uint64_t ring_full[kStretches], ring_empty[kStretches];
-  uint64_t q_full[2], s_full[2], p_full[2], pv_done[2], o_free[2], fin;
+  uint64_t q_full[2], s_full[2], p_full[2], pv_done[2], o_free[2], begun, fin;
   uint64_t kv_full[kMostSlots], kv_empty[kMostSlots];    // tiles that the products read
   uint64_t raw_full[k8 ? kMostSlots : 1], raw_empty[k8 ? kMostSlots : 1];  // 8-bit blocks
-  uint64_t v_fixed, scales;
+  Edge edges[kStretches];
+  uint64_t edge_full[kStretches], edge_empty[kStretches], v_fixed[kMostSlots], scales;
   float xchg[kTwo ? 1 : 2][2][kTwo ? 1 : 128];  // [slot][maximum | sum][row]
   int k_ref[kRefs], v_ref[kRefs];
   int warp_max[2][4];
@@ -148,7 +154,7 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
     }
     for (int i = 0; i < kStretches; ++i) {
       mbar_init(&ctl.ring_full[i], 1);
-      mbar_init(&ctl.ring_empty[i], 1 + 8 + (k8 ? 4 : 1));
+      mbar_init(&ctl.ring_empty[i], 1 + 8 + (k8 ? 4 : 0));
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl.q_full[i], kTwo ? 4 : 8);
@@ -157,16 +163,21 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
       mbar_init(&ctl.pv_done[i], 1);
       mbar_init(&ctl.o_free[i], kTwo ? 4 : 8);
     }
+    mbar_init(&ctl.begun, 1);
     mbar_init(&ctl.fin, 8);
     for (int i = 0; i < kMostSlots; ++i) {
       mbar_init(&ctl.kv_full[i], k8 ? 4 : 1);
       mbar_init(&ctl.kv_empty[i], 1);
+      mbar_init(&ctl.v_fixed[i], 1);
       if constexpr (k8) {
         mbar_init(&ctl.raw_full[i], 1);
         mbar_init(&ctl.raw_empty[i], 4);
       }
     }
-    mbar_init(&ctl.v_fixed, 1);
+    for (int i = 0; i < kStretches; ++i) {
+      mbar_init(&ctl.edge_full[i], 1);
+      mbar_init(&ctl.edge_empty[i], 1);
+    }
     mbar_init(&ctl.scales, 4);
     ctl.abort = 0;
     fence_barrier_init();
@@ -210,9 +221,19 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
     PagedWalk<R, kKeys> walk;
     walk.begin(a, line, piece, seq0, at0);
     const int pages = kKeys >> a.batch.page_shift;  // of a block
-    int slot = 0;
+    int slot = 0, edges = 0;
     uint32_t phase = 0;
     bool ok = true;
+    auto tell = [&](const Edge& e) -> bool {
+      const int at = edges % kStretches;
+      if (edges >= kStretches && !mbar_wait_warp(&ctl.edge_empty[at], (edges / kStretches - 1) & 1, s_abort, status, FTB_ERR_TIMEOUT_SLOT)) return false;
+      if (lane == 0) {
+        ctl.edges[at] = e;
+        mbar_arrive(&ctl.edge_full[at]);
+      }
+      ++edges;
+      return true;
+    };
     for (int i = 0; ok && walk.more(); ++i) {
       const PagedTile w = walk.next(a);
       if (i >= kStretches && !mbar_wait_warp(&ctl.ring_empty[i % kStretches], (i / kStretches - 1) & 1, s_abort, status, FTB_ERR_TIMEOUT_SLOT)) break;
@@ -274,12 +295,14 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
             if constexpr (D == 128) tma_load_2d(dst + P::kHalf, m, full, 64, y);
           }
         }
+        if (!k8 && x.is_v && (key0 < w.keys.lo || key0 + kKeys > w.keys.hi)) ok = tell({slot, key0, w.keys.lo, w.keys.hi, phase});
         if (++slot == (k8 ? kRawSlots : kSlots)) {
           slot = 0;
           phase ^= 1u;
         }
       }
     }
+    if (!k8 && ok) tell({-1, 0, 0, 0, 0u});
   } else if (warp == 1) {
     // ------------------------------------------------------------------- the products
     const bool leader = elect_one();
@@ -288,7 +311,7 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
     const uint64_t dQ = make_sdesc_sw128(smem_u32(sQ), 16, 1024);
     const uint64_t dK = make_sdesc_sw128(smem_u32(sKV), 16, 1024);
     const uint64_t dV = make_sdesc_sw128(smem_u32(sKV), P::kHalf, 1024);
-    uint32_t full_bits = 0, fixed_phase = 0, p_phase[2] = {0, 0};
+    uint32_t full_bits = 0, fixed_bits = 0, p_phase[2] = {0, 0};
     int slot = 0;  // of the next tile of the stream
     bool ok = true;
     auto issue_s = [&](int t, int at) {
@@ -326,8 +349,8 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
         if (!wait_tile(at)) return false;
         const int key0 = (x.block0 + j) * kKeys;
         if (k8 || (key0 >= x.keys.lo && key0 + kKeys <= x.keys.hi)) return true;
-        const bool fine = mbar_wait_warp(&ctl.v_fixed, fixed_phase, s_abort, status, FTB_ERR_TIMEOUT_TMA);
-        fixed_phase ^= 1u;
+        const bool fine = mbar_wait_warp(&ctl.v_fixed[at], (fixed_bits >> at) & 1u, s_abort, status, FTB_ERR_TIMEOUT_TMA);
+        fixed_bits ^= 1u << at;
         return fine;
       };
       auto wait_p = [&](int t) -> bool {
@@ -340,9 +363,11 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
       for (int t = 0; t < (kTwo ? 2 : 1) && ok; ++t)
         ok = mbar_wait_warp(&ctl.q_full[t], i & 1, s_abort, status, FTB_ERR_TIMEOUT_EPI) &&
              (i == 0 || mbar_wait_warp(&ctl.o_free[t], (i - 1) & 1, s_abort, status, FTB_ERR_TIMEOUT_EPI));
+      if (!ok) break;
+      if (lane == 0) mbar_arrive(&ctl.begun);
       tc_fence_after();
       if constexpr (kTwo) {
-        if (x.blocks > 0 && ok) {
+        if (x.blocks > 0) {
           int k_at = slot;
           ok = wait_tile(k_at);
           if (ok) {
@@ -407,7 +432,7 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
     const uint32_t o_addr = lane_addr + 256 + t * 128;
     uint32_t s_phase = 0;
     int pv_count[2] = {0, 0};  // products P V of the slots so far
-    int fins = 0;
+    int fins = 0, blocks0 = 0;  // blocks of the stretches so far
     bool ok = true;
     for (int i = 0; ok; ++i) {
       if (!await(i)) break;
@@ -475,7 +500,7 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
         if (busy) {
           float f = factor, add = 0.f, inv = 1.f;
           if constexpr (k8) {
-            const int kr = ctl.k_ref[j & (kRefs - 1)], vr = ctl.v_ref[j & (kRefs - 1)];
+            const int kr = ctl.k_ref[(blocks0 + j) & (kRefs - 1)], vr = ctl.v_ref[(blocks0 + j) & (kRefs - 1)];
             f *= exponent_scale(kr);
             add = static_cast<float>(vr - 127);
             inv = exponent_scale(254 - vr);
@@ -567,7 +592,11 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl.p_full[t]);
       }
+      // (a slot without blocks waits for no product: it must not hand over its next queries and results before the products have
+      // taken notice of these)
+      if (ok) ok = mbar_wait_warp(&ctl.begun, i & 1, s_abort, status, FTB_ERR_TIMEOUT_MMA);
       if (!ok) break;
+      blocks0 += x.blocks;
       if (m.n == 0) top = -FLT_MAX;
 
       // ---- results
@@ -644,39 +673,27 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
     }
   } else if constexpr (!k8) {
     // ------------------------------------------------ values that nobody of the tile sees become zeros
-    int slot = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    for (int i = 0; ok; ++i) {
-      if (!await(i)) break;
-      const Stretch x = ctl.ring[i % kStretches];
-      give_back(i);
-      for (int n = 0; n < 2 * x.blocks && ok; ++n) {
-        const StreamTile y = stream_tile<kTwo>(n, x.blocks);
-        const int key0 = (x.block0 + y.j) * kKeys;
-        if (y.is_v && (key0 < x.keys.lo || key0 + kKeys > x.keys.hi)) {
-          ok = mbar_wait_warp(&ctl.kv_full[slot], phase, s_abort, status, FTB_ERR_TIMEOUT_TMA);
-          if (!ok) break;
-          uint8_t* tile = sKV + slot * P::kTile;
-          for (int k = lane; k < kKeys * (D / 8); k += 32) {
-            const int key = k / (D / 8), c = k - key * (D / 8);
-            if (key0 + key < x.keys.lo || key0 + key >= x.keys.hi) *reinterpret_cast<uint4*>(piece_ptr(tile, key, c)) = make_uint4(0u, 0u, 0u, 0u);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&ctl.v_fixed);
-        }
-        if (++slot == kSlots) {
-          slot = 0;
-          phase ^= 1u;
-        }
+    for (int i = 0;; ++i) {
+      const int at = i % kStretches;
+      if (!mbar_wait_warp(&ctl.edge_full[at], (i / kStretches) & 1, s_abort, status, FTB_ERR_TIMEOUT_TMA)) break;
+      const Edge e = ctl.edges[at];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl.edge_empty[at]);
+      // (the products wait for this warp before they give the slot back: the fill is the one that was meant)
+      if (e.slot < 0 || !mbar_wait_warp(&ctl.kv_full[e.slot], e.phase, s_abort, status, FTB_ERR_TIMEOUT_TMA)) break;
+      uint8_t* tile = sKV + e.slot * P::kTile;
+      for (int k = lane; k < kKeys * (D / 8); k += 32) {
+        const int key = k / (D / 8), c = k - key * (D / 8);
+        if (e.key0 + key < e.lo || e.key0 + key >= e.hi) *reinterpret_cast<uint4*>(piece_ptr(tile, key, c)) = make_uint4(0u, 0u, 0u, 0u);
       }
-      if (x.last) break;
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl.v_fixed[e.slot]);
     }
   } else {
     // ------------------------------------------------------------- codes to fp16
     const int ct = threadIdx.x - 320, cw = warp - 10;  // this thread's key of a block
-    int slot = 0, raw = 0;
+    int slot = 0, raw = 0, blocks0 = 0;
     uint32_t phase = 0, raw_phase = 0, scale_phase = 0;
     bool ok = true;
     for (int i = 0; ok; ++i) {
@@ -699,7 +716,7 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
       if (x.blocks > 0) exponents(0, &ke, &ve);
       for (int n = 0; n < 2 * x.blocks && ok; ++n) {
         const StreamTile y = stream_tile<kTwo>(n, x.blocks);
-        const int ref = y.j & (kRefs - 1);
+        const int ref = (blocks0 + y.j) & (kRefs - 1);
         if (!y.is_v) {
           // scales of the block's keys and values, relative to its largest ones
           const int kt = __reduce_max_sync(0xffffffffu, ke == 255 ? 0 : ke), vt = __reduce_max_sync(0xffffffffu, ve == 255 ? 0 : ve);
@@ -774,6 +791,7 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
           raw_phase ^= 1u;
         }
       }
+      blocks0 += x.blocks;
       if (x.last) break;
     }
   }

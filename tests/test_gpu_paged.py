@@ -313,6 +313,48 @@ def test_page_offsets_beyond_32_bits():
     _check(one, q[-1:], small, torch.tensor([[0, 1, 2]]), ln, torch.tensor([0, 1]), 0.1, None)
 
 
+@pytest.mark.parametrize("eight_bit", [False, True])
+@pytest.mark.parametrize("kv,group,d,page,new,lens,window", [
+    (8, 4, 128, 16, [40] * 40, [300 + 50 * b for b in range(40)], None),
+    (8, 2, 64, 32, [150] * 12, [1000 + 77 * b for b in range(12)], None),
+    (8, 4, 128, 64, [700], [2500], None),
+    (8, 4, 128, 64, [1000], [1000], None),
+    (8, 2, 128, 16, [900, 1, 400], [1200, 77, 2222], 300),
+    (8, 8, 128, 16, [1 + b % 9 for b in range(60)], [10 + 40 * b for b in range(60)], None),
+    (4, 4, 64, 16, [1 if b % 5 else 90 for b in range(70)], [90 + 20 * b for b in range(70)], None),
+])
+def test_many_tiles(eight_bit, kv, group, d, page, new, lens, window):
+    """More tiles than CTAs: each walks several, many blocks long.  On the device in 64 bits, and three calls without a wait between them."""
+    ops = _ops()
+    table, ln, st, pages = _batch(new, lens, page)
+    cache = _full_cache(pages, kv, page, d, E4M3 if eight_bit else BF16, 3, table, ln)
+    q = _numbers((int(st[-1]), kv * group, d), BF16, 1, spread=0.3).cuda()
+    scale = 1.0 / math.sqrt(d)
+    args = (cache, table.cuda(), ln.cuda(), st.cuda())
+    got = [ops.paged_attention(q, *args, scale=scale, window=window) for _ in range(3)]
+    ops.check_status()
+    k, v = (paged.dense(cache, i).cuda() for i in range(2))
+    for b, (n, m) in enumerate(zip(lens, new)):
+        j = torch.arange(n, device="cuda")
+        rows = table[b].cuda().long()[j // page]
+        pos = torch.arange(n - m, n, device="cuda")[:, None]
+        hidden = j > pos
+        if window:
+            hidden = hidden | (j <= pos - window)
+        for h in range(kv * group):
+            kj, vj = k[rows, h // group, j % page], v[rows, h // group, j % page]
+            x = q[int(st[b]):int(st[b]) + m, h].double()
+            w = torch.softmax((x @ kj.T * scale).masked_fill(hidden, -math.inf), -1)
+            want = w @ vj
+            size = (x.abs() @ kj.abs().T * scale).masked_fill(hidden, 0).amax(-1)
+            bound = (w @ vj.abs(), size, vj.abs().amax().expand(m))
+            tol = paged.tolerance(want, bound, BF16, d, eight_bit, n)
+            for o in got:
+                err = (o[int(st[b]):int(st[b]) + m, h].double() - want).abs()
+                assert bool((err <= tol).all()), (b, h, float((err / tol).max()))
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+
+
 def test_many_sequences():
     """More sequences than a warp or a block has threads."""
     ops = _ops()
