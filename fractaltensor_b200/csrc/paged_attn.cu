@@ -28,11 +28,26 @@ struct Pieces {
 // Block (x, y): the tile with cut x of the two kernels' cuts, every kJoinBlocks-th group of its rows.
 template <typename T, bool k8, int D>
 __global__ void __launch_bounds__(kJoinThreads)
-paged_join_kernel(PagedAttn a, Pieces few, Pieces many) {
+paged_join_kernel(const __grid_constant__ PagedAttn a, Pieces few, Pieces many) {
   constexpr int kRows = kJoinThreads / (D / 4);
   __shared__ int s_odd[kRows];
   grid_dependency_wait();
   grid_launch_dependents();
+  // rows of whole tiles that have to be computed again (none, unless something in the cache is not finite)
+  {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = a.kv_heads * a.group;
+    const long long rows = static_cast<long long>(a.T) * heads, step = static_cast<long long>(gridDim.x) * gridDim.y * kJoinThreads;
+    for (long long r0 = (static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x) * kJoinThreads + warp * 32; r0 < rows; r0 += step) {
+      unsigned again = __ballot_sync(0xffffffffu, r0 + lane < rows && a.odd[min(r0 + lane, rows - 1)] != 0);
+      while (again != 0) {
+        const long long row = r0 + __ffs(again) - 1;
+        again &= again - 1;
+        const int t = static_cast<int>(row / heads), b = sequence_of_row(a.batch, t, lane);
+        if (b < a.batch.B)  // (what no sequence has was not written either)
+          attend_row<T, k8, D>(a, b, t, static_cast<int>(row - static_cast<long long>(t) * heads), position_of_row(a.batch, b, t), lane);
+      }
+    }
+  }
   const bool is_few = static_cast<int>(blockIdx.x) < few.pieces;
   const Pieces& p = is_few ? few : many;
   const int cut = blockIdx.x - (is_few ? 0 : few.pieces);
@@ -79,7 +94,7 @@ paged_join_kernel(PagedAttn a, Pieces few, Pieces many) {
     for (int i = warp; i < kRows; i += kJoinThreads / 32) {
       const int flat_i = c.flat0 + r0 + i, ti = c.first + flat_i / a.group;
       if (r0 + i < rows && s_odd[i] != 0 && hides(a, c.pos0 + ti, c.lo, c.hi))
-        attend_row<T, k8, D>(a, c.b, ti, c.h * a.group + flat_i % a.group, c.pos0 + ti, threadIdx.x & 31, 0, D);
+        attend_row<T, k8, D>(a, c.b, ti, c.h * a.group + flat_i % a.group, c.pos0 + ti, threadIdx.x & 31);
     }
     __syncthreads();
   }
@@ -126,7 +141,7 @@ using namespace ftb;
 extern "C" size_t ftb_paged_attn_scratch_bytes(int T, int B, int kv_heads, int group, int d) {
   if (T <= 0 || B <= 0 || kv_heads <= 0 || group <= 0 || d <= 0) return 0;
   const Form f = form_of(T, B, group);
-  size_t n = 0;
+  size_t n = rounded(static_cast<size_t>(T) * kv_heads * group * sizeof(uint32_t));
   if (f.nt > 0) n += rounded(places(paged_short_pieces(f.nt), 8 * f.nt, d));
   if (f.rows > 0) n += rounded(places(paged_tile_pieces(), f.rows, d));
   return n;
@@ -172,6 +187,8 @@ extern "C" int ftb_paged_attn_fwd(const void* q, long long q_row, long long q_he
   if ((reinterpret_cast<uintptr_t>(scratch) & 15) != 0) return FTB_ERR_ALIGN;
   const Form f = form_of(T, B, group);
   unsigned char* at = static_cast<unsigned char*>(scratch);
+  a.odd = static_cast<uint32_t*>(scratch);
+  at += rounded(static_cast<size_t>(T) * kv_heads * group * sizeof(uint32_t));
   auto pieces_at = [&](int pieces, int rows) {
     float* parts = reinterpret_cast<float*>(at);
     return Pieces{parts, reinterpret_cast<const PagedCut*>(parts + 2 * static_cast<size_t>(pieces) * rows * (d + 2)), pieces, rows};

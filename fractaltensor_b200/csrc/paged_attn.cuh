@@ -16,6 +16,7 @@ struct PagedAttn {
   int least_rows, most_rows;       // sequences with so many rows (token, head of a group) of a kv head are this launch's
   float scale_log2;
   int* status;
+  uint32_t* odd;                   // [T, heads]: not 0 where a row of the output has to be computed again, key by key
 };
 
 // Whether a row at position pos of a tile that multiplies keys lo .. hi - 1 has some of them with weight 0 that it does not see: what
@@ -24,11 +25,11 @@ __device__ __forceinline__ bool hides(const PagedAttn& a, long long pos, int lo,
   return pos + 1 < hi || (a.window > 0 && pos + 1 - a.window > lo);
 }
 
-// Columns c0 .. c1 - 1 of the output of one (token, head) by one warp, key by key: nothing of a key that the token does not see is
+// The output of one (token, head) by one warp, key by key: nothing of a key that the token does not see is
 // touched, not even with a weight of 0, which an infinity or a NaN there would make a NaN.  A lane holds D / 32 numbers of a row; eight
 // keys at a time, which are of one page.  For rows that the kernels' products have made a NaN through such keys.
 template <typename T, bool k8, int D>
-__device__ __noinline__ void attend_row(const PagedAttn& a, int b, int t, int head, long long pos, int lane, int c0, int c1) {
+__device__ __noinline__ void attend_row(const PagedAttn& a, int b, int t, int head, long long pos, int lane) {
   constexpr int kPer = D / 32, kBatch = 8;
   const int h = head / a.group;
   const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.q) + t * a.q_row + head * a.q_head) + lane * (kPer / 2);
@@ -98,7 +99,6 @@ __device__ __noinline__ void attend_row(const PagedAttn& a, int b, int t, int he
       for (int c = 0; c < kPer; ++c) acc[c] = fmaf(p, v[i][c], acc[c]);
     }
   }
-  if (lane * kPer < c0 || lane * kPer >= c1) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(a.o) + (static_cast<long long>(t) * a.kv_heads * a.group + head) * D) + lane * (kPer / 2);
 #pragma unroll

@@ -69,7 +69,7 @@ constexpr int blocks_per_sm(int nt) { return nt == 1 ? 3 : 2; }
 
 template <typename T, bool k8, int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm(NT))
-paged_short_kernel(PagedAttn a, float* __restrict__ parts, PagedCut* __restrict__ cuts) {
+paged_short_kernel(const __grid_constant__ PagedAttn a, float* __restrict__ parts, PagedCut* __restrict__ cuts) {
   using C = typename std::conditional<k8, __half, T>::type;
   constexpr int R = NT * 8, kSteps = D / 16, kKLoads = k8 ? D / 64 : D / 32;
   constexpr int kVWords = k8 ? D / 32 : D / 16;  // 32-bit words of one key's values a lane
@@ -425,14 +425,11 @@ paged_short_kernel(PagedAttn a, float* __restrict__ parts, PagedCut* __restrict_
       }
     }
     __syncthreads();
-    if (whole) {
-      for (int r = warp; r < rows; r += kWarps) {
-        const int flat = flat0 + r, t = s.first + flat / a.group;
-        const long long pos = s.pos0 + t;
-        if (s_odd[r] != 0 && hides(a, pos, lo, hi))
-          attend_row<T, k8, D>(a, w.b, t, h * a.group + flat % a.group, pos, lane, 0, D);
-      }
-      __syncthreads();
+    // (rows that something unseen may have made a NaN are left to the joining kernel, which goes through them key by key)
+    if (threadIdx.x < rows) {
+      const int flat = flat0 + threadIdx.x, t = s.first + flat / a.group;
+      a.odd[static_cast<long long>(t) * a.kv_heads * a.group + h * a.group + flat % a.group] =
+          s_odd[threadIdx.x] != 0 && hides(a, s.pos0 + t, lo, hi) ? 1u : 0u;
     }
   }
 }

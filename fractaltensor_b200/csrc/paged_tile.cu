@@ -6,10 +6,12 @@
 //   warp 0        the walk, announced to the others through a ring of stretches, and the loads of K and V, page by page:
 //                 TMA boxes of a page's rows into the swizzled tiles that the products read, 8-bit pages as they are
 //   warp 1        issues the products
-//   warps 2..9    softmax: two slots of 128 threads, a thread a row; they also fetch the queries and write the results
-//   16-bit caches: warp 10 zeroes values in front of and behind the keys that the tile sees (what lies there may be
+//   softmax       two slots of 128 rows; their warps also fetch the queries and write the results.  16-bit caches: 16 warps, two
+//                 threads a row with 64 keys each (a row's chain from scores to weights sits between two products, and is what bounds
+//                 a tile); 8-bit: 8 warps, a thread a row, which leaves the registers of the others to the conversion
+//   16-bit caches: one more warp zeroes values in front of and behind the keys that the tile sees (what lies there may be
 //                 anything, and 0 * NaN is NaN), told by warp 0 which blocks need it
-//   8-bit caches: warps 10..13 turn codes into fp16 tiles
+//   8-bit caches: four more warps turn codes into fp16 tiles, each a quarter of a block's keys
 // kTwo: a tile has 256 rows, 128 to a slot, and a K or V block serves both; else 128 rows, and the slots take turns at the blocks: each
 // has sums of its own for the same rows, which lie in the same lanes of tensor memory and are put together there.
 //
@@ -53,14 +55,14 @@ struct Control {
   PagedLineRoom line;
   Stretch ring[kStretches];
   uint64_t ring_full[kStretches], ring_empty[kStretches];
-  uint64_t q_full[2], s_full[2], p_full[2], pv_done[2], o_free[2], begun, fin;
+  uint64_t q_full[2], s_full[2], p_full[2], pv_done[2], o_free[2], begun, fin[2];
+  uint64_t row_max[2][4];  // [slot][quadrant of rows]: the two warps that share 32 rows
   uint64_t kv_full[kMostSlots], kv_empty[kMostSlots];    // tiles that the products read
   uint64_t raw_full[k8 ? kMostSlots : 1], raw_empty[k8 ? kMostSlots : 1];  // 8-bit blocks
   Edge edges[kStretches];
-  uint64_t edge_full[kStretches], edge_empty[kStretches], v_fixed[kMostSlots], scales;
-  float xchg[kTwo ? 1 : 2][2][kTwo ? 1 : 128];  // [slot][maximum | sum][row]
+  uint64_t edge_full[kStretches], edge_empty[kStretches], v_fixed[kMostSlots];
+  float half_max[2][2][128], half_sum[2][2][128], top[2][128];  // [slot][part of the keys][row]
   int k_ref[kRefs], v_ref[kRefs];
-  int warp_max[2][4];
   uint32_t k_scale[k8 ? 128 : 1], v_scale[k8 ? kRefs : 1][k8 ? 128 : 1];  // fp16 pairs
   uint32_t tmem_base;
   int abort, dead;
@@ -75,7 +77,8 @@ struct Plan {
   // 8-bit: as many bytes on their way as converted tiles leave room for
   static constexpr int kSlots = k8 ? (D == 128 ? (kTwo ? 3 : 4) : 6) : (kRoom / kTile < kMostSlots ? kRoom / kTile : kMostSlots);
   static constexpr int kRawSlots = k8 ? ((kRoom - kSlots * kTile) / kRaw < kMostSlots ? (kRoom - kSlots * kTile) / kRaw : kMostSlots) : 0;
-  static constexpr int kThreads = 32 * (k8 ? 14 : 11);
+  static constexpr int kParts = k8 ? 1 : 2;  // threads of a row
+  static constexpr int kSoftmax = 8 * kParts, kThreads = 32 * (2 + kSoftmax + (k8 ? 4 : 1));
   static_assert(kSlots >= 3 && (!k8 || kRawSlots >= 3), "shared memory budget");
 };
 
@@ -131,12 +134,12 @@ __device__ __forceinline__ Mine blocks_of_slot(const PagedAttn& a, const Stretch
 
 template <typename T, bool k8, int D, bool kTwo>
 __global__ void __launch_bounds__(Plan<k8, D, kTwo>::kThreads, 1)
-paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
+paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
                   float* __restrict__ parts, PagedCut* __restrict__ cuts) {
   using P = Plan<k8, D, kTwo>;
   using C = typename std::conditional<k8, __half, T>::type;
   constexpr int R = kTwo ? 256 : 128, kSlots = P::kSlots, kRawSlots = P::kRawSlots;
-  constexpr bool kKeep = !k8;  // a row's scores stay in registers between their maximum and the weights
+  constexpr int kParts = P::kParts, kMyKeys = kKeys / kParts;
   extern __shared__ uint8_t smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, piece = blockIdx.x;
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -154,17 +157,18 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
     }
     for (int i = 0; i < kStretches; ++i) {
       mbar_init(&ctl.ring_full[i], 1);
-      mbar_init(&ctl.ring_empty[i], 1 + 8 + (k8 ? 4 : 0));
+      mbar_init(&ctl.ring_empty[i], 1 + P::kSoftmax + (k8 ? 4 : 0));
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&ctl.q_full[i], kTwo ? 4 : 8);
+      mbar_init(&ctl.q_full[i], (kTwo ? 4 : 8) * kParts);
       mbar_init(&ctl.s_full[i], 1);
-      mbar_init(&ctl.p_full[i], 4);
+      mbar_init(&ctl.p_full[i], 4 * kParts);
       mbar_init(&ctl.pv_done[i], 1);
-      mbar_init(&ctl.o_free[i], kTwo ? 4 : 8);
+      mbar_init(&ctl.o_free[i], (kTwo ? 4 : 8) * kParts);
+      mbar_init(&ctl.fin[i], (kTwo ? 4 : 8) * kParts);
+      for (int k = 0; k < 4; ++k) mbar_init(&ctl.row_max[i][k], 2);
     }
     mbar_init(&ctl.begun, 1);
-    mbar_init(&ctl.fin, 8);
     for (int i = 0; i < kMostSlots; ++i) {
       mbar_init(&ctl.kv_full[i], k8 ? 4 : 1);
       mbar_init(&ctl.kv_empty[i], 1);
@@ -178,7 +182,6 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
       mbar_init(&ctl.edge_full[i], 1);
       mbar_init(&ctl.edge_empty[i], 1);
     }
-    mbar_init(&ctl.scales, 4);
     ctl.abort = 0;
     fence_barrier_init();
     fence_proxy_async_smem();
@@ -205,7 +208,8 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = ctl.tmem_base;
-  // tensor memory: S0 [0, 128), S1 [128, 256), O0 [256, 256 + D), O1 [384, 384 + D); P_t (16-bit pairs) over the first 64 columns of S_t.
+  // tensor memory: S0 [0, 128), S1 [128, 256), O0 [256, 256 + D), O1 [384, 384 + D); P_t (16-bit pairs)
+  // over the first half of the columns that each part of a row's keys has in S_t.
 
   // Stretch i of this CTA, as every role but the first warp gets it.
   auto await = [&](int i) -> bool {
@@ -330,7 +334,7 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
       if (leader) {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          umma_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + k * 8, dv + k * (2048 >> 4), idesc_pv, (!first || k != 0) ? 1u : 0u);
+          umma_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + (k * 16 / kMyKeys) * kMyKeys + (k * 16 % kMyKeys) / 2, dv + k * (2048 >> 4), idesc_pv, (!first || k != 0) ? 1u : 0u);
         umma_commit(&ctl.pv_done[t]);
       }
     };
@@ -424,36 +428,43 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
       }
       if (x.last) break;
     }
-  } else if (warp < 10) {
-    // ------------------------------------------------ softmax: slot t, row r of its 128
-    const int t = (warp - 2) >> 2, quad = warp & 3, r = quad * 32 + lane;
+  } else if (warp < 2 + P::kSoftmax) {
+    // ------------------------------------------------ softmax: slot t, part h of the keys, row r of the slot's 128
+    const int t = (warp - 2) / (4 * kParts), h = (warp - 2) / 4 % kParts, quad = warp & 3, r = quad * 32 + lane;
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
-    const uint32_t s_addr = lane_addr + t * 128;
-    const uint32_t o_addr = lane_addr + 256 + t * 128;
-    uint32_t s_phase = 0;
+    const uint32_t s_addr = lane_addr + t * 128 + h * kMyKeys;
+    // the columns of the output that this thread rescales, and those that it finishes
+    constexpr int kScale = D / kParts, kCols = kTwo ? D / kParts : D / (2 * kParts);
+    const uint32_t o_addr = lane_addr + 256 + t * 128 + h * kScale;
+    const int c0 = kTwo ? h * kCols : (t * kParts + h) * kCols;
+    uint32_t s_phase = 0, max_phase = 0, fin_phase = 0;
     int pv_count[2] = {0, 0};  // products P V of the slots so far
-    int fins = 0, blocks0 = 0;  // blocks of the stretches so far
+    int blocks0 = 0;           // blocks of the stretches so far
     bool ok = true;
     for (int i = 0; ok; ++i) {
       if (!await(i)) break;
-      const Stretch x = ctl.ring[i % kStretches];
-      give_back(i);
-      const int row = (kTwo ? t * 128 : 0) + r;     // of the tile
-      const int row0 = (kTwo ? t * 128 : 0) + quad * 32;
-      const bool busy = row0 < x.rows;              // this warp has rows
+      const Stretch& x = ctl.ring[i % kStretches];  // (read again where it is needed, and given back behind the results: registers)
+      const int row0 = (kTwo ? t * 128 : 0) + quad * 32, row = row0 + lane;  // of the tile
+      const bool busy = row0 < x.rows;                                       // this warp has rows
       const bool mine = row < x.rows;
-      const int flat = x.flat0 + row, token = flat / a.group, tok = x.first + token, head = x.h * a.group + flat - token * a.group;
+      int tok, head;
+      auto place = [&] {
+        const int flat = x.flat0 + row, token = flat / a.group;
+        tok = x.first + token;
+        head = x.h * a.group + flat - token * a.group;
+      };
+      place();
       const long long pos = mine ? x.pos0 + tok : -1;
       const int see_hi = static_cast<int>(max(-1ll, min(pos, static_cast<long long>(x.keys.hi) - 1)));
       const int see_lo = a.window > 0 ? static_cast<int>(max(0ll, min(pos - a.window + 1, static_cast<long long>(INT_MAX)))) : 0;
       float factor = a.scale_log2;
 
-      // ---- queries
+      // ---- queries: this thread's columns are those that it finishes
       if (busy) {
         uint8_t* tile = sQ + (kTwo ? t * P::kTile : 0);
         const T* src = static_cast<const T*>(a.q) + static_cast<long long>(tok) * a.q_row + static_cast<long long>(head) * a.q_head;
-        constexpr int kPieces = kTwo ? D / 8 : D / 16;  // that this thread writes
-        const int p0 = kTwo ? 0 : t * kPieces;
+        constexpr int kPieces = kCols / 8;
+        const int p0 = c0 / 8;
         if constexpr (k8 && !std::is_same<T, __half>::value) {
           uint32_t top = 0;
           if (mine) {
@@ -479,9 +490,11 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
             *reinterpret_cast<uint4*>(piece_ptr(tile, r, p0 + p)) = v;
           }
         } else {
+          uint4 v[kPieces];
 #pragma unroll
-          for (int p = 0; p < kPieces; ++p)
-            *reinterpret_cast<uint4*>(piece_ptr(tile, r, p0 + p)) = mine ? *reinterpret_cast<const uint4*>(src + (p0 + p) * 8) : make_uint4(0u, 0u, 0u, 0u);
+          for (int p = 0; p < kPieces; ++p) v[p] = mine ? *reinterpret_cast<const uint4*>(src + (p0 + p) * 8) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+          for (int p = 0; p < kPieces; ++p) *reinterpret_cast<uint4*>(piece_ptr(tile, r, p0 + p)) = v[p];
         }
         fence_proxy_async_smem();
       }
@@ -505,30 +518,39 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
             add = static_cast<float>(vr - 127);
             inv = exponent_scale(254 - vr);
           }
-          const int key0 = (x.block0 + j) * kKeys;
+          const int key0 = (x.block0 + j) * kKeys + h * kMyKeys;
           const int lo_col = see_lo - key0, hi_col = see_hi - key0;
-          const bool cut = __any_sync(0xffffffffu, mine && (lo_col > 0 || hi_col < kKeys - 1));
-          uint32_t s[kKeep ? 128 : 64];
-          float mx = -INFINITY;
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t* y = s + (kKeep ? half * 64 : 0);
-            tmem_ld32p(s_addr + half * 64, y);
-            tmem_ld32p(s_addr + half * 64 + 32, y + 32);
+          const bool cut = __any_sync(0xffffffffu, mine && (lo_col > 0 || hi_col < kMyKeys - 1));
+          // (32 scores at a time, read again for the weights: a thread that spills goes to L2 for it, shared memory has taken L1's room)
+          uint32_t s[32];
+          auto scores = [&](int n) {
+            tmem_ld32p(s_addr + n * 32, s);
             tmem_ld_wait();
             if (cut) {
 #pragma unroll
-              for (int e = 0; e < 64; ++e)
-                if (half * 64 + e < lo_col || half * 64 + e > hi_col) y[e] = 0xff800000u;
+              for (int e = 0; e < 32; ++e)
+                if (n * 32 + e < lo_col || n * 32 + e > hi_col) s[e] = 0xff800000u;
             }
+          };
+          float mx = -INFINITY;
+#pragma unroll
+          for (int n = 0; n < kMyKeys / 32; ++n) {
+            scores(n);
             float mx8[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) mx8[e] = fmaxf(__uint_as_float(y[e]), __uint_as_float(y[8 + e]));
-#pragma unroll
-            for (int e = 16; e < 64; e += 16)
-#pragma unroll
-              for (int q = 0; q < 8; ++q) mx8[q] = fmax3(mx8[q], __uint_as_float(y[e + q]), __uint_as_float(y[e + 8 + q]));
+            for (int e = 0; e < 8; ++e) mx8[e] = fmax3(__uint_as_float(s[e]), __uint_as_float(s[8 + e]), fmaxf(__uint_as_float(s[16 + e]), __uint_as_float(s[24 + e])));
             mx = fmaxf(mx, fmaxf(fmax3(mx8[0], mx8[1], mx8[2]), fmaxf(fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]))));
+          }
+          if constexpr (kParts == 2) {
+            // The larger of the two halves.  (What is overwritten here the other thread has read before its weights of the block in
+            // front, which the product that these scores came behind waited for.)
+            ctl.half_max[t][h][r] = mx;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl.row_max[t][quad]);
+            ok = mbar_wait_warp(&ctl.row_max[t][quad], max_phase, s_abort, status, FTB_ERR_TIMEOUT_EPI);
+            if (!ok) break;
+            max_phase ^= 1u;
+            mx = fmaxf(mx, ctl.half_max[t][h ^ 1][r]);
           }
           // (a row may see nothing of a block: the lowest finite number keeps its weights 0)
           const float m_new = fmaxf(fmaf(mx, f, add), -FLT_MAX);
@@ -545,7 +567,7 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
               if (need) top = m_new;
               l *= keep;
 #pragma unroll 1
-              for (int ch = 0; ch < D / 16; ++ch) {
+              for (int ch = 0; ch < kScale / 16; ++ch) {
                 uint32_t o[16];
                 tmem_ld16(o_addr + ch * 16, o);
                 tmem_ld_wait();
@@ -559,31 +581,18 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
           const float minus = add - top;
           float sum8[8] = {};
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t* y = s + (kKeep ? half * 64 : 0);
-            if constexpr (!kKeep) {
-              tmem_ld32p(s_addr + half * 64, y);
-              tmem_ld32p(s_addr + half * 64 + 32, y + 32);
-              tmem_ld_wait();
-              if (cut) {
+          for (int n = 0; n < kMyKeys / 32; ++n) {
+            scores(n);
+            uint32_t pk[16];
 #pragma unroll
-                for (int e = 0; e < 64; ++e)
-                  if (half * 64 + e < lo_col || half * 64 + e > hi_col) y[e] = 0xff800000u;
-              }
+            for (int c = 0; c < 16; ++c) {
+              const float p0 = exp2_fast(fmaf(__uint_as_float(s[2 * c]), f, minus));
+              const float p1 = exp2_fast(fmaf(__uint_as_float(s[2 * c + 1]), f, minus));
+              sum8[(2 * c) & 7] += p0;
+              sum8[(2 * c + 1) & 7] += p1;
+              pk[c] = Fmt<C>::pack2(p0, p1);
             }
-#pragma unroll
-            for (int part = 0; part < 2; ++part) {
-              uint32_t pk[16];
-#pragma unroll
-              for (int c = 0; c < 16; ++c) {
-                const float p0 = exp2_fast(fmaf(__uint_as_float(y[32 * part + 2 * c]), f, minus));
-                const float p1 = exp2_fast(fmaf(__uint_as_float(y[32 * part + 2 * c + 1]), f, minus));
-                sum8[(2 * c) & 7] += p0;
-                sum8[(2 * c + 1) & 7] += p1;
-                pk[c] = Fmt<C>::pack2(p0, p1);
-              }
-              tmem_st16(s_addr + half * 32 + part * 16, pk);
-            }
+            tmem_st16(s_addr + n * 16, pk);  // over scores that this thread has read
           }
           l = fmaf(((sum8[0] + sum8[1]) + (sum8[2] + sum8[3])) + ((sum8[4] + sum8[5]) + (sum8[6] + sum8[7])), inv, l);
           tmem_st_wait();
@@ -599,22 +608,25 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
       blocks0 += x.blocks;
       if (m.n == 0) top = -FLT_MAX;
 
-      // ---- results
-      constexpr int kCols = kTwo ? D : D / 2;  // that this thread finishes
-      const int c0 = kTwo ? 0 : t * kCols;
+      // ---- results: the parts of a row, and without kTwo those of the other slot
       float other_m = -FLT_MAX, other_l = 0.f;
       int n_other = 0;
-      if (!kTwo && x.blocks > 0) {
-        ctl.xchg[kTwo ? 0 : t][0][kTwo ? 0 : r] = top;
-        ctl.xchg[kTwo ? 0 : t][1][kTwo ? 0 : r] = l;
+      if (kTwo ? kParts == 2 && m.n > 0 : x.blocks > 0) {
+        if (h == 0) ctl.top[t][r] = top;
+        ctl.half_sum[t][h][r] = l;
+        uint64_t* fin = &ctl.fin[kTwo ? t : 0];
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl.fin);
-        n_other = blocks_of_slot<kTwo>(a, x, t ^ 1).n;
-        ok = mbar_wait_warp(&ctl.fin, fins & 1, s_abort, status, FTB_ERR_TIMEOUT_EPI);
-        ++fins;
+        if (lane == 0) mbar_arrive(fin);
+        ok = mbar_wait_warp(fin, fin_phase, s_abort, status, FTB_ERR_TIMEOUT_EPI);
         if (!ok) break;
-        other_m = ctl.xchg[kTwo ? 0 : t ^ 1][0][kTwo ? 0 : r];
-        other_l = ctl.xchg[kTwo ? 0 : t ^ 1][1][kTwo ? 0 : r];
+        fin_phase ^= 1u;
+        if constexpr (kParts == 2) l += ctl.half_sum[t][h ^ 1][r];
+        if constexpr (!kTwo) {
+          n_other = blocks_of_slot<kTwo>(a, x, t ^ 1).n;
+          other_m = ctl.top[t ^ 1][r];
+#pragma unroll
+          for (int k = 0; k < kParts; ++k) other_l += ctl.half_sum[t ^ 1][k][r];
+        }
       }
       if (m.n > 0) ok = mbar_wait_warp(&ctl.pv_done[t], (pv_count[t] + m.n - 1) & 1, s_abort, status, FTB_ERR_TIMEOUT_MMA);
       if (ok && n_other > 0) ok = mbar_wait_warp(&ctl.pv_done[t ^ 1], (pv_count[t ^ 1] + n_other - 1) & 1, s_abort, status, FTB_ERR_TIMEOUT_MMA);
@@ -627,12 +639,13 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
       const float scale = x.whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
       bool odd = false;
       if (busy) {
+        place();
         T* out = static_cast<T*>(a.o) + (static_cast<long long>(tok) * a.kv_heads * a.group + head) * D + c0;
         float* part = parts + static_cast<size_t>(x.place) * part_floats<R, D>();
 #pragma unroll 1
         for (int ch = 0; ch < kCols / 16; ++ch) {
           uint32_t o[16], o2[16];
-          if (m.n > 0) tmem_ld16(o_addr + c0 + ch * 16, o);
+          if (m.n > 0) tmem_ld16(lane_addr + 256 + t * 128 + c0 + ch * 16, o);
           if (n_other > 0) tmem_ld16(lane_addr + 256 + (t ^ 1) * 128 + c0 + ch * 16, o2);
           tmem_ld_wait();
           float y[16];
@@ -654,22 +667,20 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
             }
           }
         }
-        if (mine && !x.whole && (kTwo || t == 0)) *reinterpret_cast<float2*>(part + R * D + 2 * row) = make_float2(all_m, sum);
+        // rows that something unseen may have made a NaN are left to the joining kernel, which goes through them key by key
+        if (mine) {
+          const bool again = odd && x.whole && hides(a, x.pos0 + tok, x.keys.lo, x.keys.hi);
+          using Flag = typename std::conditional<kCols == D, uint32_t, typename std::conditional<2 * kCols == D, uint16_t, uint8_t>::type>::type;
+          reinterpret_cast<Flag*>(a.odd + static_cast<long long>(tok) * a.kv_heads * a.group + head)[c0 / kCols] = again ? 1 : 0;
+        }
+        if (mine && !x.whole && c0 == 0) *reinterpret_cast<float2*>(part + R * D + 2 * row) = make_float2(all_m, sum);
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&ctl.o_free[kTwo ? t : 0]);
-      // rows that something unseen has made a NaN, key by key
-      if (busy && x.whole) {
-        unsigned again = __ballot_sync(0xffffffffu, mine && odd && hides(a, pos, x.keys.lo, x.keys.hi));
-        while (again != 0) {
-          const int k = __ffs(again) - 1;
-          again &= again - 1;
-          const int flat_k = x.flat0 + row0 + k, tok_k = x.first + flat_k / a.group;
-          attend_row<T, k8, D>(a, x.b, tok_k, x.h * a.group + flat_k % a.group, x.pos0 + tok_k, lane, c0, c0 + kCols);
-        }
-      }
-      if (x.last) break;
+      const bool last = x.last != 0;
+      give_back(i);
+      if (last) break;
     }
   } else if constexpr (!k8) {
     // ------------------------------------------------ values that nobody of the tile sees become zeros
@@ -692,89 +703,105 @@ paged_tile_kernel(PagedAttn a, const __grid_constant__ CUtensorMap mapK, const _
     }
   } else {
     // ------------------------------------------------------------- codes to fp16
-    const int ct = threadIdx.x - 320, cw = warp - 10;  // this thread's key of a block
+    // Warp cw converts keys 32 cw .. + 31 of every block; each warp finds the block's largest exponents on its own.
+    const int cw = warp - 2 - P::kSoftmax;
     int slot = 0, raw = 0, blocks0 = 0;
-    uint32_t phase = 0, raw_phase = 0, scale_phase = 0;
+    uint32_t phase = 0, raw_phase = 0;
     bool ok = true;
     for (int i = 0; ok; ++i) {
       if (!await(i)) break;
       const Stretch x = ctl.ring[i % kStretches];
       give_back(i);
       const int* table = a.batch.table + static_cast<long long>(x.b) * a.batch.W;
-      // exponents of this thread's key of block j: both, or 0 where nobody sees it
-      auto exponents = [&](int j, int* ke, int* ve) {
-        const int key = (x.block0 + j) * kKeys + ct;
-        *ke = *ve = 0;
-        if (j >= x.blocks || key < x.keys.lo || key >= x.keys.hi) return;
-        int page = __ldg(table + (key >> a.batch.page_shift));
-        if (page < 0 || page >= a.batch.pages) page = 0;
-        const long long row = ((static_cast<long long>(page) * a.kv_heads + x.h) << a.batch.page_shift) + (key & ((1 << a.batch.page_shift) - 1));
-        *ke = a.k_exp[row];
-        *ve = a.v_exp[row];
+      // exponents of keys lane, lane + 32, .. of block j, keys in the low bytes, values in the next; 0 where nobody sees them
+      int exps[4];
+      auto exponents = [&](int j) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int key = (x.block0 + j) * kKeys + q * 32 + lane;
+          exps[q] = 0;
+          if (j >= x.blocks || key < x.keys.lo || key >= x.keys.hi) continue;
+          int page = __ldg(table + (key >> a.batch.page_shift));
+          if (page < 0 || page >= a.batch.pages) page = 0;
+          const long long row = ((static_cast<long long>(page) * a.kv_heads + x.h) << a.batch.page_shift) + (key & ((1 << a.batch.page_shift) - 1));
+          exps[q] = a.k_exp[row] | (a.v_exp[row] << 8);
+        }
       };
-      int ke = 0, ve = 0;
-      if (x.blocks > 0) exponents(0, &ke, &ve);
+      if (x.blocks > 0) exponents(0);
       for (int n = 0; n < 2 * x.blocks && ok; ++n) {
         const StreamTile y = stream_tile<kTwo>(n, x.blocks);
         const int ref = (blocks0 + y.j) & (kRefs - 1);
         if (!y.is_v) {
-          // scales of the block's keys and values, relative to its largest ones
-          const int kt = __reduce_max_sync(0xffffffffu, ke == 255 ? 0 : ke), vt = __reduce_max_sync(0xffffffffu, ve == 255 ? 0 : ve);
-          if (lane == 0) {
-            ctl.warp_max[0][cw] = kt;
-            ctl.warp_max[1][cw] = vt;
+          // scales of this warp's keys and values, relative to the block's largest ones
+          int kt = 1, vt = 1, ke = 0, ve = 0;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int k1 = exps[q] & 0xff, v1 = exps[q] >> 8;
+            kt = max(kt, k1 == 255 ? 0 : k1);
+            vt = max(vt, v1 == 255 ? 0 : v1);
+            if (q == cw) {
+              ke = k1;
+              ve = v1;
+            }
           }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&ctl.scales);
-          ok = mbar_wait_warp(&ctl.scales, scale_phase, s_abort, status, FTB_ERR_TIMEOUT_EPI);
-          scale_phase ^= 1u;
-          if (!ok) break;
-          const int k_top = max(1, max(max(ctl.warp_max[0][0], ctl.warp_max[0][1]), max(ctl.warp_max[0][2], ctl.warp_max[0][3])));
-          const int v_top = max(1, max(max(ctl.warp_max[1][0], ctl.warp_max[1][1]), max(ctl.warp_max[1][2], ctl.warp_max[1][3])));
+          kt = __reduce_max_sync(0xffffffffu, kt);
+          vt = __reduce_max_sync(0xffffffffu, vt);
           auto pair_of = [](int below) -> uint32_t {  // 2^-below as fp16, twice
-            const uint32_t h = below < 15 ? static_cast<uint32_t>(15 - below) << 10 : below <= 24 ? 1u << (24 - below) : 0u;
-            return h | (h << 16);
+            const uint32_t e = below < 15 ? static_cast<uint32_t>(15 - below) << 10 : below <= 24 ? 1u << (24 - below) : 0u;
+            return e | (e << 16);
           };
-          ctl.k_scale[ct] = pair_of(max(0, k_top - ke));
-          ctl.v_scale[ref][ct] = pair_of(max(0, v_top - ve));
-          if (ct == 0) {
-            ctl.k_ref[ref] = k_top;
-            ctl.v_ref[ref] = v_top;
+          ctl.k_scale[cw * 32 + lane] = pair_of(max(0, kt - ke));
+          ctl.v_scale[ref][cw * 32 + lane] = pair_of(max(0, vt - ve));
+          if (cw == 0 && lane == 0) {
+            ctl.k_ref[ref] = kt;
+            ctl.v_ref[ref] = vt;
           }
-          exponents(y.j + 1, &ke, &ve);  // on their way
+          exponents(y.j + 1);  // on their way
           __syncwarp();
-          if (lane == 0) mbar_arrive(&ctl.scales);
-          ok = mbar_wait_warp(&ctl.scales, scale_phase, s_abort, status, FTB_ERR_TIMEOUT_EPI);
-          scale_phase ^= 1u;
-          if (!ok) break;
         }
         ok = mbar_wait_warp(&ctl.raw_full[raw], raw_phase, s_abort, status, FTB_ERR_TIMEOUT_TMA) &&
              mbar_wait_warp(&ctl.kv_empty[slot], phase ^ 1u, s_abort, status, FTB_ERR_TIMEOUT_SLOT);
         if (!ok) break;
-        const uint4* src = reinterpret_cast<const uint4*>(sRaw + raw * P::kRaw);
+        // a lane: piece c of keys first, first + 32 / kRow, ..
+        constexpr int kRow = D / 16, kPieces = kRow;
+        const int first = cw * 32 + lane / kRow, c = lane % kRow;
+        const uint4* src = reinterpret_cast<const uint4*>(sRaw + raw * P::kRaw) + first * kRow + c;
         uint8_t* tile = sKV + slot * P::kTile;
-        const uint32_t* scale = y.is_v ? ctl.v_scale[ref] : ctl.k_scale;
-        const int key0 = (x.block0 + y.j) * kKeys;
+        const uint32_t* scale = (y.is_v ? ctl.v_scale[ref] : ctl.k_scale) + first;
+        uint4 v[kPieces];
+        uint32_t by[kPieces];
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const int at = k * 128 + ct, key = at / (D / 16), c = at - key * (D / 16);
-          const uint4 v = src[at];
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-          const __half2 by = *reinterpret_cast<const __half2*>(&scale[key]);
+        for (int k = 0; k < kPieces; ++k) {
+          v[k] = src[k * 32];
+          by[k] = scale[k * (32 / kRow)];
+        }
+        const int key0 = (x.block0 + y.j) * kKeys;
+        if (y.is_v && (key0 < x.keys.lo || key0 + kKeys > x.keys.hi)) {  // values that nobody sees become zeros
+#pragma unroll
+          for (int k = 0; k < kPieces; ++k) {
+            const int key = key0 + first + k * (32 / kRow);
+            if (key < x.keys.lo || key >= x.keys.hi) v[k] = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+        // (the two halves of a piece go to neighbouring 16 bytes; d 128: lanes of the upper half of a row begin with the second, so
+        // that eight lanes reach all banks)
+        const bool swap = D == 128 && c >= 4;
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) {
+          const uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+          const __half2 b2 = *reinterpret_cast<const __half2*>(&by[k]);
           uint32_t o[8];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             uint32_t lo = e4m3x2_to_f16x2(w[e] & 0xffffu), hi = e4m3x2_to_f16x2(w[e] >> 16);
-            __half2 l2 = __hmul2(*reinterpret_cast<__half2*>(&lo), by), h2 = __hmul2(*reinterpret_cast<__half2*>(&hi), by);
-            o[2 * e] = *reinterpret_cast<uint32_t*>(&l2);
-            o[2 * e + 1] = *reinterpret_cast<uint32_t*>(&h2);
+            const __half2 l2 = __hmul2(*reinterpret_cast<__half2*>(&lo), b2), h2 = __hmul2(*reinterpret_cast<__half2*>(&hi), b2);
+            o[2 * e] = *reinterpret_cast<const uint32_t*>(&l2);
+            o[2 * e + 1] = *reinterpret_cast<const uint32_t*>(&h2);
           }
-          if (y.is_v && (key0 + key < x.keys.lo || key0 + key >= x.keys.hi)) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] = 0u;
-          }
-          *reinterpret_cast<uint4*>(piece_ptr(tile, key, 2 * c)) = make_uint4(o[0], o[1], o[2], o[3]);
-          *reinterpret_cast<uint4*>(piece_ptr(tile, key, 2 * c + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+          const int key = first + k * (32 / kRow);
+          const uint4 even = make_uint4(o[0], o[1], o[2], o[3]), uneven = make_uint4(o[4], o[5], o[6], o[7]);
+          *reinterpret_cast<uint4*>(piece_ptr(tile, key, 2 * c + (swap ? 1 : 0))) = swap ? uneven : even;
+          *reinterpret_cast<uint4*>(piece_ptr(tile, key, 2 * c + (swap ? 0 : 1))) = swap ? even : uneven;
         }
         fence_proxy_async_smem();
         __syncwarp();
