@@ -11,7 +11,7 @@
 //                 a tile); 8-bit: 8 warps, a thread a row, which leaves the registers of the others to the conversion
 //   16-bit caches: one more warp zeroes values in front of and behind the keys that the tile sees (what lies there may be
 //                 anything, and 0 * NaN is NaN), told by warp 0 which blocks need it
-//   8-bit caches: four more warps turn codes into fp16 tiles, each a quarter of a block's keys
+//   8-bit caches: eight more warps turn codes into fp16 tiles, four of them one tile, the other four the next
 // kTwo: a tile has 256 rows, 128 to a slot, and a K or V block serves both; else 128 rows, and the slots take turns at the blocks: each
 // has sums of its own for the same rows, which lie in the same lanes of tensor memory and are put together there.
 //
@@ -62,8 +62,8 @@ struct Control {
   Edge edges[kStretches];
   uint64_t edge_full[kStretches], edge_empty[kStretches], v_fixed[kMostSlots];
   float half_max[2][2][128], half_sum[2][2][128], top[2][128];  // [slot][part of the keys][row]
+  int see_lo[2][128], see_hi[2][128];
   int k_ref[kRefs], v_ref[kRefs];
-  uint32_t k_scale[k8 ? 128 : 1], v_scale[k8 ? kRefs : 1][k8 ? 128 : 1];  // fp16 pairs
   uint32_t tmem_base;
   int abort, dead;
 };
@@ -77,8 +77,9 @@ struct Plan {
   // 8-bit: as many bytes on their way as converted tiles leave room for
   static constexpr int kSlots = k8 ? (D == 128 ? (kTwo ? 3 : 4) : 6) : (kRoom / kTile < kMostSlots ? kRoom / kTile : kMostSlots);
   static constexpr int kRawSlots = k8 ? ((kRoom - kSlots * kTile) / kRaw < kMostSlots ? (kRoom - kSlots * kTile) / kRaw : kMostSlots) : 0;
-  static constexpr int kParts = k8 ? 1 : 2;  // threads of a row
-  static constexpr int kSoftmax = 8 * kParts, kThreads = 32 * (2 + kSoftmax + (k8 ? 4 : 1));
+  static constexpr int kParts = 1;  // threads of a row
+  static constexpr int kSoftmax = 8 * kParts, kConvert = 8;  // warps that turn codes into numbers
+  static constexpr int kThreads = 32 * (2 + kSoftmax + (k8 ? kConvert : 1));
   static_assert(kSlots >= 3 && (!k8 || kRawSlots >= 3), "shared memory budget");
 };
 
@@ -157,7 +158,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
     }
     for (int i = 0; i < kStretches; ++i) {
       mbar_init(&ctl.ring_full[i], 1);
-      mbar_init(&ctl.ring_empty[i], 1 + P::kSoftmax + (k8 ? 4 : 0));
+      mbar_init(&ctl.ring_empty[i], 1 + P::kSoftmax + (k8 ? P::kConvert : 0));
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl.q_full[i], (kTwo ? 4 : 8) * kParts);
@@ -266,25 +267,29 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
         }
       }
       const int* table = a.batch.table + static_cast<long long>(w.b) * a.batch.W;
+      // this lane's page of tile n, or -1: one lane a page; those that nobody sees need not be there
+      auto page_of_tile = [&](int n) -> int {
+        const int key0 = (block0 + stream_tile<kTwo>(n, blocks).j) * kKeys, at = key0 + (lane << a.batch.page_shift);
+        if (n >= 2 * blocks || lane >= pages || at >= w.keys.hi || at + (1 << a.batch.page_shift) <= w.keys.lo) return -1;
+        return __ldg(table + (at >> a.batch.page_shift));
+      };
+      int page_next = page_of_tile(0);
       for (int n = 0; ok && n < 2 * blocks; ++n) {
         const StreamTile x = stream_tile<kTwo>(n, blocks);
-        // one lane a page; those that nobody sees need not be there
         const int key0 = (block0 + x.j) * kKeys;
         const int p0 = w.keys.lo > key0 ? (w.keys.lo - key0) >> a.batch.page_shift : 0;
         const int p1 = min(pages, (w.keys.hi - key0 + (1 << a.batch.page_shift) - 1) >> a.batch.page_shift);
         const bool here = lane >= p0 && lane < p1;
-        int page = 0;
-        if (here) {
-          page = __ldg(table + (key0 >> a.batch.page_shift) + lane);
-          if (page < 0 || page >= a.batch.pages) {
-            atomicCAS(status, 0, FTB_ERR_INDEX);
-            page = 0;
-          }
-        }
+        int page = page_next;
+        page_next = page_of_tile(n + 1);  // on its way while this one waits for room
         uint64_t* full = k8 ? &ctl.raw_full[slot] : &ctl.kv_full[slot];
         uint64_t* empty = k8 ? &ctl.raw_empty[slot] : &ctl.kv_empty[slot];
         ok = mbar_wait_warp(empty, phase ^ 1u, s_abort, status, FTB_ERR_TIMEOUT_SLOT);
         if (!ok) break;
+        if (here && (page < 0 || page >= a.batch.pages)) {
+          atomicCAS(status, 0, FTB_ERR_INDEX);
+          page = 0;
+        }
         if (lane == 0) mbar_arrive_expect_tx(full, ((p1 - p0) << a.batch.page_shift) * (k8 ? D : 2 * D));
         __syncwarp();
         if (here) {
@@ -437,9 +442,9 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
     constexpr int kScale = D / kParts, kCols = kTwo ? D / kParts : D / (2 * kParts);
     const uint32_t o_addr = lane_addr + 256 + t * 128 + h * kScale;
     const int c0 = kTwo ? h * kCols : (t * kParts + h) * kCols;
-    uint32_t s_phase = 0, max_phase = 0, fin_phase = 0;
-    int pv_count[2] = {0, 0};  // products P V of the slots so far
-    int blocks0 = 0;           // blocks of the stretches so far
+    // parities: bit 0 the next scores, 1 the rows' maxima, 2 fin, 4 + t the next product P V of slot t in a stretch
+    uint32_t par = 0;
+    int blocks0 = 0;  // blocks of the stretches so far
     bool ok = true;
     for (int i = 0; ok; ++i) {
       if (!await(i)) break;
@@ -454,9 +459,11 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
         head = x.h * a.group + flat - token * a.group;
       };
       place();
-      const long long pos = mine ? x.pos0 + tok : -1;
-      const int see_hi = static_cast<int>(max(-1ll, min(pos, static_cast<long long>(x.keys.hi) - 1)));
-      const int see_lo = a.window > 0 ? static_cast<int>(max(0ll, min(pos - a.window + 1, static_cast<long long>(INT_MAX)))) : 0;
+      {  // (every part of a row writes the same; read back a block at a time, which saves registers)
+        const long long pos = mine ? x.pos0 + tok : -1;
+        ctl.see_hi[t][r] = static_cast<int>(max(-1ll, min(pos, static_cast<long long>(x.keys.hi) - 1)));
+        ctl.see_lo[t][r] = a.window > 0 ? static_cast<int>(max(0ll, min(pos - a.window + 1, static_cast<long long>(INT_MAX)))) : 0;
+      }
       float factor = a.scale_log2;
 
       // ---- queries: this thread's columns are those that it finishes
@@ -506,9 +513,9 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
       float top = 0.f, l = 0.f;
       for (int k = 0; k < m.n && ok; ++k) {
         const int j = kTwo ? m.j0 + k : 2 * k + t;
-        ok = mbar_wait_warp(&ctl.s_full[t], s_phase, s_abort, status, FTB_ERR_TIMEOUT_MMA);
+        ok = mbar_wait_warp(&ctl.s_full[t], par & 1u, s_abort, status, FTB_ERR_TIMEOUT_MMA);
         if (!ok) break;
-        s_phase ^= 1u;
+        par ^= 1u;
         tc_fence_after();
         if (busy) {
           float f = factor, add = 0.f, inv = 1.f;
@@ -519,26 +526,33 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
             inv = exponent_scale(254 - vr);
           }
           const int key0 = (x.block0 + j) * kKeys + h * kMyKeys;
-          const int lo_col = see_lo - key0, hi_col = see_hi - key0;
+          const int lo_col = ctl.see_lo[t][r] - key0, hi_col = ctl.see_hi[t][r] - key0;
           const bool cut = __any_sync(0xffffffffu, mine && (lo_col > 0 || hi_col < kMyKeys - 1));
-          // (32 scores at a time, read again for the weights: a thread that spills goes to L2 for it, shared memory has taken L1's room)
-          uint32_t s[32];
+          // kChunk scores at a time, read again for the weights.  (A thread that spills goes to L2 for it: shared memory has taken
+          // L1's room.)
+          constexpr int kChunk = k8 ? 32 : 64;
+          uint32_t s[kChunk];
           auto scores = [&](int n) {
-            tmem_ld32p(s_addr + n * 32, s);
+#pragma unroll
+            for (int e = 0; e < kChunk; e += 32) tmem_ld32p(s_addr + n * kChunk + e, s + e);
             tmem_ld_wait();
             if (cut) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (n * 32 + e < lo_col || n * 32 + e > hi_col) s[e] = 0xff800000u;
+              for (int e = 0; e < kChunk; ++e)
+                if (n * kChunk + e < lo_col || n * kChunk + e > hi_col) s[e] = 0xff800000u;
             }
           };
           float mx = -INFINITY;
 #pragma unroll
-          for (int n = 0; n < kMyKeys / 32; ++n) {
+          for (int n = 0; n < kMyKeys / kChunk; ++n) {
             scores(n);
             float mx8[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) mx8[e] = fmax3(__uint_as_float(s[e]), __uint_as_float(s[8 + e]), fmaxf(__uint_as_float(s[16 + e]), __uint_as_float(s[24 + e])));
+            for (int e = 0; e < 8; ++e) mx8[e] = fmaxf(__uint_as_float(s[e]), __uint_as_float(s[8 + e]));
+#pragma unroll
+            for (int e = 16; e < kChunk; e += 16)
+#pragma unroll
+              for (int q = 0; q < 8; ++q) mx8[q] = fmax3(mx8[q], __uint_as_float(s[e + q]), __uint_as_float(s[e + 8 + q]));
             mx = fmaxf(mx, fmaxf(fmax3(mx8[0], mx8[1], mx8[2]), fmaxf(fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]))));
           }
           if constexpr (kParts == 2) {
@@ -547,9 +561,9 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
             ctl.half_max[t][h][r] = mx;
             __syncwarp();
             if (lane == 0) mbar_arrive(&ctl.row_max[t][quad]);
-            ok = mbar_wait_warp(&ctl.row_max[t][quad], max_phase, s_abort, status, FTB_ERR_TIMEOUT_EPI);
+            ok = mbar_wait_warp(&ctl.row_max[t][quad], par >> 1 & 1u, s_abort, status, FTB_ERR_TIMEOUT_EPI);
             if (!ok) break;
-            max_phase ^= 1u;
+            par ^= 2u;
             mx = fmaxf(mx, ctl.half_max[t][h ^ 1][r]);
           }
           // (a row may see nothing of a block: the lowest finite number keeps its weights 0)
@@ -560,7 +574,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
             const bool need = m_new - top > kAbove;
             if (__any_sync(0xffffffffu, need)) {
               // the product in front has to be done: O is at rest then
-              ok = mbar_wait_warp(&ctl.pv_done[t], (pv_count[t] + k - 1) & 1, s_abort, status, FTB_ERR_TIMEOUT_MMA);
+              ok = mbar_wait_warp(&ctl.pv_done[t], ((par >> (4 + t)) + k - 1) & 1u, s_abort, status, FTB_ERR_TIMEOUT_MMA);
               if (!ok) break;
               tc_fence_after();
               const float keep = need ? exp2_fast(top - m_new) : 1.f;
@@ -581,18 +595,21 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
           const float minus = add - top;
           float sum8[8] = {};
 #pragma unroll
-          for (int n = 0; n < kMyKeys / 32; ++n) {
+          for (int n = 0; n < kMyKeys / kChunk; ++n) {
             scores(n);
-            uint32_t pk[16];
 #pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              const float p0 = exp2_fast(fmaf(__uint_as_float(s[2 * c]), f, minus));
-              const float p1 = exp2_fast(fmaf(__uint_as_float(s[2 * c + 1]), f, minus));
-              sum8[(2 * c) & 7] += p0;
-              sum8[(2 * c + 1) & 7] += p1;
-              pk[c] = Fmt<C>::pack2(p0, p1);
+            for (int part = 0; part < kChunk / 32; ++part) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int c = 0; c < 16; ++c) {
+                const float p0 = exp2_fast(fmaf(__uint_as_float(s[32 * part + 2 * c]), f, minus));
+                const float p1 = exp2_fast(fmaf(__uint_as_float(s[32 * part + 2 * c + 1]), f, minus));
+                sum8[(2 * c) & 7] += p0;
+                sum8[(2 * c + 1) & 7] += p1;
+                pk[c] = Fmt<C>::pack2(p0, p1);
+              }
+              tmem_st16(s_addr + n * (kChunk / 2) + part * 16, pk);  // over scores that this thread has read
             }
-            tmem_st16(s_addr + n * 16, pk);  // over scores that this thread has read
           }
           l = fmaf(((sum8[0] + sum8[1]) + (sum8[2] + sum8[3])) + ((sum8[4] + sum8[5]) + (sum8[6] + sum8[7])), inv, l);
           tmem_st_wait();
@@ -617,9 +634,9 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
         uint64_t* fin = &ctl.fin[kTwo ? t : 0];
         __syncwarp();
         if (lane == 0) mbar_arrive(fin);
-        ok = mbar_wait_warp(fin, fin_phase, s_abort, status, FTB_ERR_TIMEOUT_EPI);
+        ok = mbar_wait_warp(fin, par >> 2 & 1u, s_abort, status, FTB_ERR_TIMEOUT_EPI);
         if (!ok) break;
-        fin_phase ^= 1u;
+        par ^= 4u;
         if constexpr (kParts == 2) l += ctl.half_sum[t][h ^ 1][r];
         if constexpr (!kTwo) {
           n_other = blocks_of_slot<kTwo>(a, x, t ^ 1).n;
@@ -628,11 +645,10 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
           for (int k = 0; k < kParts; ++k) other_l += ctl.half_sum[t ^ 1][k][r];
         }
       }
-      if (m.n > 0) ok = mbar_wait_warp(&ctl.pv_done[t], (pv_count[t] + m.n - 1) & 1, s_abort, status, FTB_ERR_TIMEOUT_MMA);
-      if (ok && n_other > 0) ok = mbar_wait_warp(&ctl.pv_done[t ^ 1], (pv_count[t ^ 1] + n_other - 1) & 1, s_abort, status, FTB_ERR_TIMEOUT_MMA);
+      if (m.n > 0) ok = mbar_wait_warp(&ctl.pv_done[t], ((par >> (4 + t)) + m.n - 1) & 1u, s_abort, status, FTB_ERR_TIMEOUT_MMA);
+      if (ok && n_other > 0) ok = mbar_wait_warp(&ctl.pv_done[t ^ 1], ((par >> (4 + (t ^ 1))) + n_other - 1) & 1u, s_abort, status, FTB_ERR_TIMEOUT_MMA);
       if (!ok) break;
-      pv_count[t] += m.n;
-      pv_count[t ^ 1] += n_other;
+      par ^= static_cast<uint32_t>(m.n & 1) << (4 + t) ^ static_cast<uint32_t>(n_other & 1) << (4 + (t ^ 1));
       tc_fence_after();
       const float all_m = fmaxf(top, other_m), keep = exp2_fast(top - all_m), take = exp2_fast(other_m - all_m);
       const float sum = l * keep + other_l * take;
@@ -703,62 +719,73 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
     }
   } else {
     // ------------------------------------------------------------- codes to fp16
-    // Warp cw converts keys 32 cw .. + 31 of every block; each warp finds the block's largest exponents on its own.
-    const int cw = warp - 2 - P::kSoftmax;
-    int slot = 0, raw = 0, blocks0 = 0;
-    uint32_t phase = 0, raw_phase = 0;
+    // Two groups of four warps take the tiles in turn; warp cw of a group converts keys 32 cw .. + 31.  Each warp finds the block's
+    // largest exponents on its own: lane i holds those of keys i, i + 32, i + 64 and i + 96.  They are loaded a tile of the group's
+    // ahead, the pages that they lie in two.
+    const int cw = (warp - 2 - P::kSoftmax) & 3, group = (warp - 2 - P::kSoftmax) >> 2;
+    int count = 0, blocks0 = 0;  // tiles and blocks of the stretches so far
     bool ok = true;
     for (int i = 0; ok; ++i) {
       if (!await(i)) break;
       const Stretch x = ctl.ring[i % kStretches];
       give_back(i);
+      const int tiles = 2 * x.blocks, n0 = (group - count) & 1;
       const int* table = a.batch.table + static_cast<long long>(x.b) * a.batch.W;
-      // exponents of keys lane, lane + 32, .. of block j, keys in the low bytes, values in the next; 0 where nobody sees them
-      int exps[4];
-      auto exponents = [&](int j) {
+      int pages[4], kx[4], vx[4];  // of keys that nobody sees: exponents 0
+      auto key_of = [&](int n, int q) { return (x.block0 + stream_tile<kTwo>(n, x.blocks).j) * kKeys + q * 32 + lane; };
+      auto load_pages = [&](int n) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int key = (x.block0 + j) * kKeys + q * 32 + lane;
-          exps[q] = 0;
-          if (j >= x.blocks || key < x.keys.lo || key >= x.keys.hi) continue;
-          int page = __ldg(table + (key >> a.batch.page_shift));
-          if (page < 0 || page >= a.batch.pages) page = 0;
-          const long long row = ((static_cast<long long>(page) * a.kv_heads + x.h) << a.batch.page_shift) + (key & ((1 << a.batch.page_shift) - 1));
-          exps[q] = a.k_exp[row] | (a.v_exp[row] << 8);
+          const int key = key_of(n, q);
+          pages[q] = -1;
+          if (n < tiles && key >= x.keys.lo && key < x.keys.hi) pages[q] = __ldg(table + (key >> a.batch.page_shift));
         }
       };
-      if (x.blocks > 0) exponents(0);
-      for (int n = 0; n < 2 * x.blocks && ok; ++n) {
+      auto load_exponents = [&](int n) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int key = key_of(n, q), page = pages[q] < a.batch.pages ? max(0, pages[q]) : 0;
+          const long long row = ((static_cast<long long>(page) * a.kv_heads + x.h) << a.batch.page_shift) + (key & ((1 << a.batch.page_shift) - 1));
+          kx[q] = vx[q] = 0;
+          if (n < tiles && key >= x.keys.lo && key < x.keys.hi) {
+            kx[q] = a.k_exp[row];
+            vx[q] = a.v_exp[row];
+          }
+        }
+      };
+      load_pages(n0);
+      load_exponents(n0);
+      load_pages(n0 + 2);
+      for (int n = n0; n < tiles && ok; n += 2) {
         const StreamTile y = stream_tile<kTwo>(n, x.blocks);
         const int ref = (blocks0 + y.j) & (kRefs - 1);
-        if (!y.is_v) {
-          // scales of this warp's keys and values, relative to the block's largest ones
-          int kt = 1, vt = 1, ke = 0, ve = 0;
+        const int slot = (count + n) % kSlots, raw = (count + n) % kRawSlots;
+        const uint32_t phase = (count + n) / kSlots & 1, raw_phase = (count + n) / kRawSlots & 1;
+        // scales of this warp's rows, relative to the block's largest one
+        int top = 1, mine = 0;
+        {
+          int other = 1;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const int k1 = exps[q] & 0xff, v1 = exps[q] >> 8;
-            kt = max(kt, k1 == 255 ? 0 : k1);
-            vt = max(vt, v1 == 255 ? 0 : v1);
-            if (q == cw) {
-              ke = k1;
-              ve = v1;
+            const int e = y.is_v ? vx[q] : kx[q];
+            top = max(top, e == 255 ? 0 : e);
+            other = max(other, vx[q] == 255 ? 0 : vx[q]);
+            if (q == cw) mine = e;
+          }
+          top = __reduce_max_sync(0xffffffffu, top);
+          if (!y.is_v) {
+            other = __reduce_max_sync(0xffffffffu, other);
+            if (cw == 0 && lane == 0) {
+              ctl.k_ref[ref] = top;
+              ctl.v_ref[ref] = other;
             }
           }
-          kt = __reduce_max_sync(0xffffffffu, kt);
-          vt = __reduce_max_sync(0xffffffffu, vt);
-          auto pair_of = [](int below) -> uint32_t {  // 2^-below as fp16, twice
-            const uint32_t e = below < 15 ? static_cast<uint32_t>(15 - below) << 10 : below <= 24 ? 1u << (24 - below) : 0u;
-            return e | (e << 16);
-          };
-          ctl.k_scale[cw * 32 + lane] = pair_of(max(0, kt - ke));
-          ctl.v_scale[ref][cw * 32 + lane] = pair_of(max(0, vt - ve));
-          if (cw == 0 && lane == 0) {
-            ctl.k_ref[ref] = kt;
-            ctl.v_ref[ref] = vt;
-          }
-          exponents(y.j + 1);  // on their way
-          __syncwarp();
         }
+        load_exponents(n + 2);
+        load_pages(n + 4);
+        const int below = max(0, top - mine);
+        uint32_t by = below < 15 ? static_cast<uint32_t>(15 - below) << 10 : below <= 24 ? 1u << (24 - below) : 0u;  // 2^-below as fp16
+        by |= by << 16;
         ok = mbar_wait_warp(&ctl.raw_full[raw], raw_phase, s_abort, status, FTB_ERR_TIMEOUT_TMA) &&
              mbar_wait_warp(&ctl.kv_empty[slot], phase ^ 1u, s_abort, status, FTB_ERR_TIMEOUT_SLOT);
         if (!ok) break;
@@ -767,14 +794,9 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
         const int first = cw * 32 + lane / kRow, c = lane % kRow;
         const uint4* src = reinterpret_cast<const uint4*>(sRaw + raw * P::kRaw) + first * kRow + c;
         uint8_t* tile = sKV + slot * P::kTile;
-        const uint32_t* scale = (y.is_v ? ctl.v_scale[ref] : ctl.k_scale) + first;
         uint4 v[kPieces];
-        uint32_t by[kPieces];
 #pragma unroll
-        for (int k = 0; k < kPieces; ++k) {
-          v[k] = src[k * 32];
-          by[k] = scale[k * (32 / kRow)];
-        }
+        for (int k = 0; k < kPieces; ++k) v[k] = src[k * 32];
         const int key0 = (x.block0 + y.j) * kKeys;
         if (y.is_v && (key0 < x.keys.lo || key0 + kKeys > x.keys.hi)) {  // values that nobody sees become zeros
 #pragma unroll
@@ -789,7 +811,8 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
 #pragma unroll
         for (int k = 0; k < kPieces; ++k) {
           const uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-          const __half2 b2 = *reinterpret_cast<const __half2*>(&by[k]);
+          const uint32_t scale = __shfl_sync(0xffffffffu, by, lane / kRow + k * (32 / kRow));
+          const __half2 b2 = *reinterpret_cast<const __half2*>(&scale);
           uint32_t o[8];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -809,15 +832,8 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
           mbar_arrive(&ctl.kv_full[slot]);
           mbar_arrive(&ctl.raw_empty[raw]);
         }
-        if (++slot == kSlots) {
-          slot = 0;
-          phase ^= 1u;
-        }
-        if (++raw == kRawSlots) {
-          raw = 0;
-          raw_phase ^= 1u;
-        }
       }
+      count += tiles;
       blocks0 += x.blocks;
       if (x.last) break;
     }
