@@ -102,6 +102,7 @@ class _NoHost:
 
     b2b_gemm = flash_attention = sparse_attention = _decline
     embedding_gather = lstm_pack_weights = lstm_stacked_ragged = project_softmax = _decline
+    paged_cache_write = paged_cache_read = paged_attention = verify_drafts = _decline
 
     @staticmethod
     def current_stream(dev):

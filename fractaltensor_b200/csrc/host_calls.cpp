@@ -6,7 +6,8 @@
 // take the call's objects as they are, read shapes, types and pointers from the tensors in C++,
 // allocate the result through the same caching allocator and enter the C ABI with the current
 // stream of the inputs' device (4..6 us per call, most of it the allocation and the launch).  The calls of the word
-// program (lookup, packing, ragged LSTM, projection) are here too: a pass of a small model was bound by their host time.
+// program (lookup, packing, ragged LSTM, projection) are here too: a pass of a small model was bound by their host time; and those
+// of a decoding step (paged cache, attention over it, drafts), which a program makes once a layer.
 //
 // They are the accepting half only: whatever is not the plain, valid call (a wrong type or shape, a
 // tensor on the CPU, no workspace on that device yet, no memory for the result) is answered with
@@ -384,6 +385,201 @@ PyObject* project_softmax(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
+// A cache and a batch's description as the paged entry points take them.
+struct PagedCall {
+  const at::Tensor *k, *v, *k_exp = nullptr, *v_exp = nullptr, *table, *lens, *starts;
+  int B, W, pages, kv, page_size, d;
+
+  const unsigned char* exps(const at::Tensor* t) const { return t ? static_cast<const unsigned char*>(t->data_ptr()) : nullptr; }
+  const int* ints(const at::Tensor* t) const { return static_cast<const int*>(t->data_ptr()); }
+};
+bool paged_call(PyObject* cache, PyObject* table, PyObject* lens, PyObject* starts, PagedCall* c) {
+  if (!PyTuple_CheckExact(cache) || (PyTuple_GET_SIZE(cache) != 2 && PyTuple_GET_SIZE(cache) != 4)) return false;
+  const bool eight = PyTuple_GET_SIZE(cache) == 4;
+  c->k = cuda_tensor(PyTuple_GET_ITEM(cache, 0));
+  c->v = cuda_tensor(PyTuple_GET_ITEM(cache, 1));
+  if (!c->k || !c->v || c->k->dim() != 4 || !same_kind(*c->k, *c->v) || c->k->sizes() != c->v->sizes()) return false;
+  const auto type = c->k->scalar_type();
+  if (eight ? type != at::kFloat8_e4m3fn : type != at::kHalf && type != at::kBFloat16) return false;
+  for (int i = 0; i < 4; ++i)
+    if (c->k->size(i) > 0x7fffffff) return false;
+  if (eight) {
+    c->k_exp = cuda_tensor(PyTuple_GET_ITEM(cache, 2));
+    c->v_exp = cuda_tensor(PyTuple_GET_ITEM(cache, 3));
+    for (const at::Tensor* e : {c->k_exp, c->v_exp})
+      if (!e || e->scalar_type() != at::kByte || e->device() != c->k->device() || e->sizes() != c->k->sizes().slice(0, 3)) return false;
+  }
+  c->table = cuda_tensor(table);
+  c->lens = cuda_tensor(lens);
+  c->starts = cuda_tensor(starts);
+  for (const at::Tensor* t : {c->table, c->lens, c->starts})
+    if (!t || t->scalar_type() != at::kInt || t->device() != c->k->device()) return false;
+  if (c->table->dim() != 2 || c->table->size(0) <= 0 || c->table->size(1) <= 0 || c->table->size(0) >= 0x7fffffff ||
+      c->table->size(1) > 0x7fffffff)
+    return false;
+  if (c->lens->dim() != 1 || c->lens->size(0) != c->table->size(0) || c->starts->dim() != 1 || c->starts->size(0) != c->table->size(0) + 1)
+    return false;
+  c->B = static_cast<int>(c->table->size(0));
+  c->W = static_cast<int>(c->table->size(1));
+  c->pages = static_cast<int>(c->k->size(0));
+  c->kv = static_cast<int>(c->k->size(1));
+  c->page_size = static_cast<int>(c->k->size(2));
+  c->d = static_cast<int>(c->k->size(3));
+  return (c->page_size == 16 || c->page_size == 32 || c->page_size == 64 || c->page_size == 128) && (c->d == 64 || c->d == 128);
+}
+// Rows [T, heads, d], the numbers of a head side by side; nullptr where they are not on 16-byte boundaries or of another type or device.
+const at::Tensor* rows_of(PyObject* o, const PagedCall& c, int64_t* row, int64_t* head) {
+  if (!THPVariable_Check(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_cuda() || t.device() != c.k->device() || t.dim() != 3 || t.size(2) != c.d || t.size(0) > 0x7fffffff || t.size(1) > 0x7fffffff)
+    return nullptr;
+  if (c.k_exp ? t.scalar_type() != at::kHalf && t.scalar_type() != at::kBFloat16 : t.scalar_type() != c.k->scalar_type()) return nullptr;
+  *row = t.size(0) > 1 ? t.stride(0) : 0;
+  *head = t.size(1) > 1 ? t.stride(1) : 0;
+  if (t.stride(2) != 1 || ((*row | *head) & 7) != 0 || (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) != 0) return nullptr;
+  return &t;
+}
+
+// (cache, k, v, table, lens, starts, workspaces) -> True
+PyObject* paged_cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    DECLINE_UNLESS(n == 7);
+    PagedCall c;
+    DECLINE_UNLESS(paged_call(args[0], args[3], args[4], args[5], &c));
+    int64_t kr, kh, vr, vh;
+    const at::Tensor *k = rows_of(args[1], c, &kr, &kh), *v = rows_of(args[2], c, &vr, &vh);
+    DECLINE_UNLESS(k && v && same_kind(*k, *v) && k->size(1) == c.kv && v->size(1) == c.kv && k->size(0) == v->size(0));
+    const c10::DeviceIndex dev = c.k->device().index();
+    const at::Tensor ws = workspace_of(args[6], dev, ftb_workspace_bytes());
+    DECLINE_UNLESS(ws.defined());
+    int rc;
+    {
+      const WithoutGil released;
+      const c10::cuda::CUDAGuard guard(dev);
+      rc = ftb_paged_cache_write(k->data_ptr(), v->data_ptr(), kr, kh, vr, vh, c.k->data_ptr(), c.v->data_ptr(),
+                                 const_cast<unsigned char*>(c.exps(c.k_exp)), const_cast<unsigned char*>(c.exps(c.v_exp)), c.ints(c.table),
+                                 c.ints(c.lens), c.ints(c.starts), static_cast<int>(k->size(0)), c.B, c.W, c.pages, c.kv, c.page_size, c.d,
+                                 dtype_code(*k), ws.data_ptr(), ws.numel(), stream_of(dev));
+    }
+    if (rc != 0) return PyLong_FromLong(rc);
+    Py_RETURN_TRUE;
+  });
+}
+
+// (cache, table, lens, starts, rows, dtype code, workspaces) -> (k, v)
+PyObject* paged_cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    DECLINE_UNLESS(n == 7);
+    PagedCall c;
+    int64_t rows, dt;
+    DECLINE_UNLESS(paged_call(args[0], args[1], args[2], args[3], &c) && get_int(args[4], &rows) && get_int(args[5], &dt) && rows >= 0);
+    DECLINE_UNLESS(dt >= FTB_DTYPE_F32 && dt <= FTB_DTYPE_BF16);
+    const auto type = dt == FTB_DTYPE_F32 ? at::kFloat : dt == FTB_DTYPE_F16 ? at::kHalf : at::kBFloat16;
+    DECLINE_UNLESS(c.k_exp || type == c.k->scalar_type());
+    const c10::DeviceIndex dev = c.k->device().index();
+    const at::Tensor ws = workspace_of(args[6], dev, ftb_workspace_bytes());
+    DECLINE_UNLESS(ws.defined());
+    at::Tensor k, v;
+    int rc;
+    {
+      const WithoutGil released;
+      const c10::cuda::CUDAGuard guard(dev);
+      const auto like = at::TensorOptions().dtype(type).device(c.k->device());
+      k = at::empty({rows, c.kv, c.d}, like);
+      v = at::empty({rows, c.kv, c.d}, like);
+      rc = ftb_paged_cache_read(c.k->data_ptr(), c.v->data_ptr(), c.exps(c.k_exp), c.exps(c.v_exp), c.ints(c.table), c.ints(c.lens),
+                                c.ints(c.starts), k.data_ptr(), v.data_ptr(), static_cast<int>(rows), c.B, c.W, c.pages, c.kv,
+                                c.page_size, c.d, static_cast<int>(dt), ws.data_ptr(), ws.numel(), stream_of(dev));
+    }
+    if (rc != 0) return PyLong_FromLong(rc);
+    return Py_BuildValue("(NN)", THPVariable_Wrap(k), THPVariable_Wrap(v));
+  });
+}
+
+// (q, cache, table, lens, starts, out | None, scale, window (0: none), workspaces)
+PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    DECLINE_UNLESS(n == 9);
+    PagedCall c;
+    DECLINE_UNLESS(paged_call(args[1], args[2], args[3], args[4], &c));
+    int64_t qr, qh, window;
+    float scale;
+    const at::Tensor* q = rows_of(args[0], c, &qr, &qh);
+    DECLINE_UNLESS(q && get_float(args[6], &scale) && get_int(args[7], &window) && window >= 0 && c.kv > 0 && q->size(1) > 0 &&
+                   q->size(1) % c.kv == 0);
+    const c10::DeviceIndex dev = c.k->device().index();
+    const at::Tensor ws = workspace_of(args[8], dev, ftb_workspace_bytes());
+    DECLINE_UNLESS(ws.defined());
+    at::Tensor out;
+    DECLINE_UNLESS(given_result(args[5], *q, q->sizes(), &out));
+    int rc;
+    {
+      const WithoutGil released;
+      const c10::cuda::CUDAGuard guard(dev);
+      if (!out.defined()) out = new_result(*q, q->sizes());
+      const int T = static_cast<int>(q->size(0)), group = static_cast<int>(q->size(1) / c.kv);
+      const size_t bytes = ftb_paged_attn_scratch_bytes(T, c.B, c.kv, group, c.d);
+      at::Tensor scratch;
+      if (bytes > 0) scratch = at::empty({static_cast<int64_t>(bytes)}, at::TensorOptions().dtype(at::kByte).device(q->device()));
+      rc = ftb_paged_attn_fwd(q->data_ptr(), qr, qh, c.k->data_ptr(), c.v->data_ptr(), c.exps(c.k_exp), c.exps(c.v_exp), c.ints(c.table),
+                              c.ints(c.lens), c.ints(c.starts), out.data_ptr(), T, c.B, c.W, c.pages, c.kv, group, c.page_size, c.d,
+                              static_cast<int>(window), scale, dtype_code(*q), bytes > 0 ? scratch.data_ptr() : nullptr, bytes,
+                              ws.data_ptr(), ws.numel(), stream_of(dev));
+    }
+    return rc == 0 ? THPVariable_Wrap(out) : PyLong_FromLong(rc);
+  });
+}
+
+// (probs, drafts, u, draft_probs | None, counts | None, workspaces) -> (tokens, counts)
+PyObject* verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    DECLINE_UNLESS(n == 6);
+    const at::Tensor *drafts = cuda_tensor(args[1]), *u = cuda_tensor(args[2]);
+    DECLINE_UNLESS(drafts && u && drafts->dim() == 2 && drafts->scalar_type() == at::kLong);
+    const int64_t B = drafts->size(0), K = drafts->size(1);
+    DECLINE_UNLESS(B <= 0x7fffffff && K < 0x7fffffff);
+    int64_t V = -1;
+    auto rows = [&](PyObject* o, int64_t count) -> const at::Tensor* {
+      if (!THPVariable_Check(o)) return nullptr;
+      const at::Tensor& t = THPVariable_Unpack(o);
+      if (!t.is_cuda() || t.device() != drafts->device() || t.scalar_type() != at::kFloat || t.dim() != 3 || t.size(0) != B || t.size(1) != count)
+        return nullptr;
+      if (V < 0) V = t.size(2);
+      return t.size(2) == V && V > 0 && V <= 0x7fffffff && (V == 1 || t.stride(2) == 1) ? &t : nullptr;
+    };
+    const at::Tensor *p = rows(args[0], K + 1), *q = nullptr, *counts = nullptr;
+    DECLINE_UNLESS(p);
+    if (args[3] != Py_None) {
+      q = rows(args[3], K);
+      DECLINE_UNLESS(q);
+    }
+    DECLINE_UNLESS(u->scalar_type() == at::kFloat && u->device() == drafts->device() && u->dim() == 2 && u->size(0) == B && u->size(1) == K + 1);
+    if (args[4] != Py_None) {
+      counts = cuda_tensor(args[4]);
+      DECLINE_UNLESS(counts && counts->scalar_type() == at::kInt && counts->device() == drafts->device() && counts->dim() == 1 && counts->size(0) == B);
+    }
+    const c10::DeviceIndex dev = drafts->device().index();
+    const at::Tensor ws = workspace_of(args[5], dev, ftb_workspace_bytes());
+    DECLINE_UNLESS(ws.defined());
+    at::Tensor tokens, taken;
+    int rc;
+    {
+      const WithoutGil released;
+      const c10::cuda::CUDAGuard guard(dev);
+      tokens = new_result(*drafts, {B, K + 1});
+      taken = at::empty({B}, at::TensorOptions().dtype(at::kInt).device(drafts->device()));
+      rc = ftb_verify_drafts(static_cast<const float*>(p->data_ptr()), p->stride(0), p->stride(1),
+                             q ? static_cast<const float*>(q->data_ptr()) : nullptr, q ? q->stride(0) : 0, q ? q->stride(1) : 0,
+                             static_cast<const long long*>(drafts->data_ptr()), static_cast<const float*>(u->data_ptr()),
+                             counts ? static_cast<const int*>(counts->data_ptr()) : nullptr, static_cast<long long*>(tokens.data_ptr()),
+                             static_cast<int*>(taken.data_ptr()), static_cast<int>(B), static_cast<int>(K), static_cast<int>(V),
+                             ws.data_ptr(), ws.numel(), stream_of(dev));
+    }
+    if (rc != 0) return PyLong_FromLong(rc);
+    return Py_BuildValue("(NN)", THPVariable_Wrap(tokens), THPVariable_Wrap(taken));
+  });
+}
+
 // (device index, -1: the current one) -> handle of its current stream.  (torch.cuda.current_stream makes a
 // stream object for it: 2 us, three times in a call of the word program.)
 PyObject* current_stream(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -411,6 +607,10 @@ PyMethodDef kMethods[] = {
     {"lstm_pack_weights", as_method(lstm_pack_weights), METH_FASTCALL, nullptr},
     {"lstm_stacked_ragged", as_method(lstm_stacked_ragged), METH_FASTCALL, nullptr},
     {"project_softmax", as_method(project_softmax), METH_FASTCALL, nullptr},
+    {"paged_cache_write", as_method(paged_cache_write), METH_FASTCALL, nullptr},
+    {"paged_cache_read", as_method(paged_cache_read), METH_FASTCALL, nullptr},
+    {"paged_attention", as_method(paged_attention), METH_FASTCALL, nullptr},
+    {"verify_drafts", as_method(verify_drafts), METH_FASTCALL, nullptr},
     {"current_stream", as_method(current_stream), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -7,6 +7,10 @@
 //
 // Only one row of p (and of q) a sequence is read whole.  Sums are kept in 64 bits: the chosen index follows from a
 // comparison with a partial sum of up to V numbers, and in 32 bits the order of summation would decide it.
+//
+// Bound by the bytes of those rows.  A cluster of CTAs takes a sequence, every warp a stretch of the row: one pass for the
+// stretches' sums, which the CTAs hand each other through distributed shared memory, and a second look at the one stretch (a 64th of
+// the row or less) in which the limit is passed.  Every CTA finds n on its own, which saves a step of waiting.
 #include "../../include/ftb200.h"
 #include "ptx.cuh"
 #include "tmap.h"
@@ -14,7 +18,7 @@
 namespace ftb {
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kThreads = 512, kWarps = kThreads / 32, kUnroll = 8;
 
 struct Drafts {
   const float* p;
@@ -26,11 +30,9 @@ struct Drafts {
   int K, V;
 };
 
-__device__ __forceinline__ double weight(const float* p, const float* q, int j, int without) {
-  const float x = p[j];
-  double w = x;
-  if (q != nullptr) w -= static_cast<double>(q[j]);
-  return w > 0.0 && x < __int_as_float(0x7f800000) && j != without ? w : 0.0;
+__device__ __forceinline__ double weight_of(float p, float q, int j, int without) {
+  const double w = static_cast<double>(p) - static_cast<double>(q);
+  return w > 0.0 && p < __int_as_float(0x7f800000) && j != without ? w : 0.0;
 }
 
 __device__ __forceinline__ double warp_sum(double x) {
@@ -39,98 +41,172 @@ __device__ __forceinline__ double warp_sum(double x) {
   return x;
 }
 
+__device__ __forceinline__ double ld_cluster_f64(uint32_t addr) {
+  double x;
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(x) : "r"(addr) : "memory");
+  return x;
+}
+
+// C: CTAs of a cluster, 1 or 8.
+template <int C>
 __global__ void __launch_bounds__(kThreads)
 verify_drafts_kernel(Drafts a, long long* __restrict__ tokens, int* __restrict__ counts_out, int* __restrict__ status) {
-  __shared__ double sums[kWarps];
-  __shared__ int s_n, s_found;
-  const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  grid_launch_dependents();
+  __shared__ double sums[kWarps], totals[2];  // of the warps; of this CTA (in the two tries)
+  __shared__ double s_total[C];
+  __shared__ int s_n;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int b = blockIdx.x / C, rank = C > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  if (threadIdx.x == 0) s_n = a.K;
+  __syncthreads();
   grid_dependency_wait();
+  grid_launch_dependents();
   const int K = a.K, V = a.V;
   const int mine = a.counts != nullptr ? min(max(a.counts[b], 0), K) : K;
   const long long* x = a.drafts + static_cast<long long>(b) * K;
   const float* u = a.u + static_cast<long long>(b) * (K + 1);
   const float* p = a.p + b * a.p_seq;
   const float* q = a.q != nullptr ? a.q + b * a.q_seq : nullptr;
-  if (threadIdx.x == 0) {
-    s_n = mine;
-    s_found = V;
-  }
-  __syncthreads();
   for (int i = threadIdx.x; i < mine; i += kThreads) {
     const long long id = x[i];
     bool taken = false;
     if (id >= 0 && id < V) {
       const double qx = q != nullptr ? static_cast<double>(q[i * a.q_row + id]) : 1.0;
       taken = static_cast<double>(u[i]) * qx < static_cast<double>(p[i * a.p_row + id]);
-    } else {
+    } else if (rank == 0) {
       atomicCAS(status, 0, FTB_ERR_INDEX);
     }
     if (!taken) atomicMin(&s_n, i);
   }
+  const double share = u[K];
   __syncthreads();
-  const int n = s_n;
+  const int n = min(s_n, mine);
   const float* pr = p + n * a.p_row;
   const float* qr = q != nullptr && n < mine ? q + n * a.q_row : nullptr;
   int without = q == nullptr && n < mine && x[n] >= 0 && x[n] < V ? static_cast<int>(x[n]) : -1;
-  // a warp's part of the row: whole groups of 32
-  const int part = ((V + kThreads - 1) / kThreads) * 32, from = min(V, warp * part), to = min(V, from + part);
-  double total = 0.0;
+  // a warp's stretch of the row: whole groups of 32
+  const int stretch = ((V + C * kThreads - 1) / (C * kThreads)) * 32;
+  const int from = static_cast<int>(min(static_cast<long long>(V), static_cast<long long>(rank * kWarps + warp) * stretch)), to = min(V, from + stretch);
+  double total = 0.0, before = 0.0;  // of the row; of the CTAs in front of this one
   for (int tries = 0; tries < 2; ++tries) {  // where p and q are the same, nothing is left of the difference: p itself
     double s = 0.0;
-    for (int j = from + lane; j < to; j += 32) s += weight(pr, qr, j, without);
+    for (int j = from; j < to; j += 32 * kUnroll) {
+      float pv[kUnroll], qv[kUnroll];
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k) {
+        const int at = j + k * 32 + lane;
+        pv[k] = at < to ? pr[at] : 0.f;
+        qv[k] = qr != nullptr && at < to ? qr[at] : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k) s += weight_of(pv[k], qv[k], j + k * 32 + lane, without);
+    }
     s = warp_sum(s);
-    __syncthreads();
     if (lane == 0) sums[warp] = s;
     __syncthreads();
-    total = 0.0;
-    for (int w = 0; w < kWarps; ++w) total += sums[w];
+    double cta = 0.0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) cta += sums[w];
+    if constexpr (C == 1) {
+      total = cta;
+      __syncthreads();
+    } else {
+      if (threadIdx.x == 0) totals[tries] = cta;
+      cluster_sync_all();
+      if (threadIdx.x < C) s_total[threadIdx.x] = ld_cluster_f64(map_to_cta(smem_u32(&totals[tries]), threadIdx.x));
+      __syncthreads();
+      total = before = 0.0;
+#pragma unroll
+      for (int r = 0; r < C; ++r) {
+        if (r < rank) before += s_total[r];
+        total += s_total[r];
+      }
+    }
     if (total > 0.0) break;
     qr = nullptr;
     without = -1;
   }
-  const double limit = static_cast<double>(u[K]) * total;
-  double before = 0.0;
-  int last = -1, first = kWarps;  // the last part that weighs anything, the first whose end is above the limit
-  double at = 0.0;
-  for (int w = 0; w < kWarps; ++w) {
-    if (first == kWarps && at + sums[w] > limit) {
-      first = w;
-      before = at;
+  // The stretch in which the limit is passed: sums[] are this CTA's still.  (u of 1 or above, or sums that round down: the last
+  // stretch that weighs anything.)
+  const double limit = share * total;
+  // Which CTA has it follows from the CTAs' sums alone, the same in all of them.
+  const bool passed = total > limit;
+  bool past = false, own = C == 1;
+  if constexpr (C > 1) {
+    double at = 0.0;
+    int weighs = -1;
+#pragma unroll
+    for (int r = 0; r < C; ++r) {
+      at += s_total[r];
+      if (passed && !past && at > limit) {
+        past = true;
+        own = r == rank;
+      }
+      if (s_total[r] > 0.0) weighs = r;
     }
-    at += sums[w];
+    if (!passed) own = weighs == rank;
+  }
+  int first = -1, last = -1;
+  double in_front = before, begin = before;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (first < 0 && begin + sums[w] > limit) {
+      first = w;
+      in_front = begin;
+    }
+    begin += sums[w];
     if (sums[w] > 0.0) last = w;
   }
-  if (first == kWarps && last >= 0) {  // u of 1 or above, or sums that round down: the last token that weighs anything
-    first = last;
-    before = -1e300;
-  }
-  if (warp == first) {
+  const bool heaviest = !passed || first < 0;  // (sums that round differently: the last one too)
+  if (heaviest) first = last;
+  const bool here = own && total > 0.0;  // of all CTAs, one
+  if (here && warp == first) {
     int found = -1, heavy = -1;
-    double run = before;
+    double run = in_front;
     for (int j0 = from; j0 < to && found < 0; j0 += 32) {
       const int j = j0 + lane;
-      const double w = j < to ? weight(pr, qr, j, without) : 0.0;
+      const double w = j < to ? weight_of(pr[j], qr != nullptr ? qr[j] : 0.f, j, without) : 0.0;
       double s = w;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const double y = __shfl_up_sync(0xffffffffu, s, o);
         if (lane >= o) s += y;
       }
-      const unsigned above = __ballot_sync(0xffffffffu, w > 0.0 && run + s > limit), some = __ballot_sync(0xffffffffu, w > 0.0);
+      const unsigned above = __ballot_sync(0xffffffffu, !heaviest && w > 0.0 && run + s > limit), some = __ballot_sync(0xffffffffu, w > 0.0);
       if (above != 0) found = j0 + __ffs(above) - 1;
       if (some != 0) heavy = j0 + 31 - __clz(some);
       run += __shfl_sync(0xffffffffu, s, 31);
     }
-    if (lane == 0) s_found = found >= 0 ? found : heavy;
+    if (lane == 0) tokens[static_cast<long long>(b) * (K + 1) + n] = found >= 0 ? found : heavy;
   }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    if (!(total > 0.0)) atomicCAS(status, 0, FTB_ERR_INDEX);
-    counts_out[b] = n + 1;
+  if (rank == 0) {
+    for (int i = threadIdx.x; i <= K; i += kThreads)
+      if (i != n || !(total > 0.0)) tokens[static_cast<long long>(b) * (K + 1) + i] = i < n ? x[i] : -1;
+    if (threadIdx.x == 0) {
+      if (!(total > 0.0)) atomicCAS(status, 0, FTB_ERR_INDEX);
+      counts_out[b] = n + 1;
+    }
   }
-  for (int i = threadIdx.x; i <= K; i += kThreads)
-    tokens[static_cast<long long>(b) * (K + 1) + i] = i < n ? x[i] : i > n || !(total > 0.0) ? -1 : s_found;
+  if constexpr (C > 1) cluster_sync_all();  // nobody leaves while its sum may be read
+}
+
+// Clusters where a row has more than a few numbers a thread.
+constexpr int kOneCta = 8 * kThreads;
+
+template <int C>
+cudaError_t launch(const Drafts& a, int B, long long* tokens, int* counts_out, int* status, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(B) * C);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = C;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = C > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, verify_drafts_kernel<C>, a, tokens, counts_out, status);
 }
 
 }  // namespace
@@ -148,8 +224,10 @@ extern "C" int ftb_verify_drafts(const float* probs, long long p_seq, long long 
   const int rc = check_device_sm100();
   if (rc) return rc;
   const Drafts a{probs, draft_probs, drafts, u, counts, p_seq, p_row, q_seq, q_row, K, V};
-  const cudaError_t err = launch_light(verify_drafts_kernel, dim3(B), dim3(kThreads), 0, static_cast<cudaStream_t>(stream), a,
-                                       tokens, counts_out, static_cast<int*>(workspace));
+  if (B > 0x7fffffff / 8) return FTB_ERR_ARG;
+  int* st = static_cast<int*>(workspace);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t err = V > kOneCta ? launch<8>(a, B, tokens, counts_out, st, s) : launch<1>(a, B, tokens, counts_out, st, s);
   count_launch();
   if (err != cudaSuccess) cudaGetLastError();
   return err == cudaSuccess ? FTB_OK : FTB_ERR_LAUNCH;

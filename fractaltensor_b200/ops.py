@@ -740,6 +740,10 @@ def paged_cache_write(cache, k, v, table, lens, starts):
     starts: int32 [B+1], the first row of each sequence's new tokens, the last one's end behind them.  Token i of the n new
     ones of sequence b goes to position lens[b] - n + i.  Rows that belong to no sequence (padding) are not stored.  The
     pages that new tokens fall into must belong to one sequence each."""
+    done = host.paged_cache_write(cache, k, v, table, lens, starts, _workspaces)
+    if done is not None:
+        _done(done, "ftb_paged_cache_write")
+        return
     args, B, W = _paged_args("paged_cache_write", cache, table, lens, starts)
     kc = cache[0]
     pages, kv, page_size, d = kc.shape
@@ -753,17 +757,26 @@ def paged_cache_write(cache, k, v, table, lens, starts):
                                         _ptr(ws), ws.numel(), _stream()), "ftb_paged_cache_write")
 
 
+def _read_dtype(cache, dtype):
+    if dtype is not None:
+        return dtype
+    return torch.bfloat16 if len(cache) == 4 else getattr(cache[0], "dtype", None)
+
+
 def paged_cache_read(cache, table, lens, starts, rows, dtype=None, out=None):
     """The keys and values that paged_cache_write stored for the same table, lens and starts -> (k, v), [rows, kv_heads, d].
 
     With starts[b+1] - starts[b] == lens[b] that is sequence b whole.  rows: what starts ends with, or more: rows that belong to
     no sequence are left as they were.  dtype: 16-bit caches: their own; 8-bit ones: float32, float16 or bfloat16 (the
     default, which holds every such number exactly)."""
+    if out is None:
+        done = host.paged_cache_read(cache, table, lens, starts, rows, _DT.get(_read_dtype(cache, dtype), -1), _workspaces)
+        if done is not None:
+            return _done(done, "ftb_paged_cache_read")
     args, B, W = _paged_args("paged_cache_read", cache, table, lens, starts)
     kc = cache[0]
     pages, kv, page_size, d = kc.shape
-    if dtype is None:
-        dtype = torch.bfloat16 if len(cache) == 4 else kc.dtype
+    dtype = _read_dtype(cache, dtype)
     if len(cache) == 2 and dtype != kc.dtype:
         raise TypeError("paged_cache_read: a cache of %s is read as that, not as %s" % (kc.dtype, dtype))
     if dtype not in _DT:
@@ -786,6 +799,10 @@ def paged_attention(q, cache, table, lens, starts, scale=None, window=None, out=
     q: [T, heads, d], heads a multiple of the cache's kv_heads, rows as in paged_cache_write -> [T, heads, d]: for a token
     at position p softmax(scale * q . k_j) v over the keys j <= p, with `window` over p - window < j <= p only.  Tokens that see
     nothing get zeros; rows that belong to no sequence are left as they were."""
+    done = host.paged_attention(q, cache, table, lens, starts, out, 1.0 if scale is None else scale, 0 if window is None else window or -1,
+                                _workspaces)
+    if done is not None:
+        return _done(done, "ftb_paged_attn_fwd")
     args, B, W = _paged_args("paged_attention", cache, table, lens, starts)
     kc = cache[0]
     pages, kv, page_size, d = kc.shape
@@ -817,6 +834,10 @@ def verify_drafts(probs, drafts, u, draft_probs=None, counts=None):
     sequence has, or None: K.  Draft i is taken if u[i] * q_i(x_i) < p_i(x_i); behind the n taken ones a token
     is drawn by u[K] from max(p_n - q_n, 0) (from p_n if all were taken).  -> (tokens int64 [B, K+1]: the taken drafts, the drawn
     token, then -1; int32 [B]: n + 1)."""
+    done = host.verify_drafts(probs, drafts, u, draft_probs, counts, _workspaces)
+    if done is not None:
+        return _done(done, "ftb_verify_drafts")
+
     def rows(t, name, n):
         if not isinstance(t, torch.Tensor):
             raise TypeError("%s must be a torch.Tensor" % name)
