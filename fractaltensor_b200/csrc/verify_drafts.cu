@@ -18,7 +18,7 @@
 namespace ftb {
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kUnroll = 8;
+constexpr int kUnroll = 8;
 
 struct Drafts {
   const float* p;
@@ -48,9 +48,10 @@ __device__ __forceinline__ double ld_cluster_f64(uint32_t addr) {
 }
 
 // C: CTAs of a cluster, 1 or 8.
-template <int C>
-__global__ void __launch_bounds__(kThreads)
+template <int C, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1536 / kThreads)
 verify_drafts_kernel(Drafts a, long long* __restrict__ tokens, int* __restrict__ counts_out, int* __restrict__ status) {
+  constexpr int kWarps = kThreads / 32;
   __shared__ double sums[kWarps], totals[2];  // of the warps; of this CTA (in the two tries)
   __shared__ double s_total[C];
   __shared__ int s_n;
@@ -160,21 +161,44 @@ verify_drafts_kernel(Drafts a, long long* __restrict__ tokens, int* __restrict__
   if (heaviest) first = last;
   const bool here = own && total > 0.0;  // of all CTAs, one
   if (here && warp == first) {
+    // kUnroll numbers side by side a lane: one scan over the lanes for 32 * kUnroll of them
     int found = -1, heavy = -1;
     double run = in_front;
-    for (int j0 = from; j0 < to && found < 0; j0 += 32) {
-      const int j = j0 + lane;
-      const double w = j < to ? weight_of(pr[j], qr != nullptr ? qr[j] : 0.f, j, without) : 0.0;
-      double s = w;
+    for (int j0 = from; j0 < to && found < 0; j0 += 32 * kUnroll) {
+      const int j = j0 + lane * kUnroll;
+      double w[kUnroll], s = 0.0;
+      float pv[kUnroll], qv[kUnroll];
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k) {
+        pv[k] = j + k < to ? pr[j + k] : 0.f;
+        qv[k] = qr != nullptr && j + k < to ? qr[j + k] : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k) {
+        w[k] = weight_of(pv[k], qv[k], j + k, without);
+        s += w[k];
+      }
+      double ends = s;  // sum of the lanes up to this one
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const double y = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += y;
+        const double y = __shfl_up_sync(0xffffffffu, ends, o);
+        if (lane >= o) ends += y;
       }
-      const unsigned above = __ballot_sync(0xffffffffu, !heaviest && w > 0.0 && run + s > limit), some = __ballot_sync(0xffffffffu, w > 0.0);
-      if (above != 0) found = j0 + __ffs(above) - 1;
-      if (some != 0) heavy = j0 + 31 - __clz(some);
-      run += __shfl_sync(0xffffffffu, s, 31);
+      const double begins = __shfl_up_sync(0xffffffffu, ends, 1);
+      double upto = run + (lane > 0 ? begins : 0.0);
+      int here_found = -1, here_heavy = -1;
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k) {
+        upto += w[k];
+        if (w[k] > 0.0) {
+          if (here_found < 0 && !heaviest && upto > limit) here_found = j + k;
+          here_heavy = j + k;
+        }
+      }
+      const unsigned above = __ballot_sync(0xffffffffu, here_found >= 0), some = __ballot_sync(0xffffffffu, here_heavy >= 0);
+      if (above != 0) found = __shfl_sync(0xffffffffu, here_found, __ffs(above) - 1);
+      if (some != 0) heavy = __shfl_sync(0xffffffffu, here_heavy, 31 - __clz(some));
+      run += __shfl_sync(0xffffffffu, ends, 31);
     }
     if (lane == 0) tokens[static_cast<long long>(b) * (K + 1) + n] = found >= 0 ? found : heavy;
   }
@@ -189,10 +213,7 @@ verify_drafts_kernel(Drafts a, long long* __restrict__ tokens, int* __restrict__
   if constexpr (C > 1) cluster_sync_all();  // nobody leaves while its sum may be read
 }
 
-// Clusters where a row has more than a few numbers a thread.
-constexpr int kOneCta = 8 * kThreads;
-
-template <int C>
+template <int C, int kThreads>
 cudaError_t launch(const Drafts& a, int B, long long* tokens, int* counts_out, int* status, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(B) * C);
@@ -206,7 +227,7 @@ cudaError_t launch(const Drafts& a, int B, long long* tokens, int* counts_out, i
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = C > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, verify_drafts_kernel<C>, a, tokens, counts_out, status);
+  return cudaLaunchKernelEx(&cfg, verify_drafts_kernel<C, kThreads>, a, tokens, counts_out, status);
 }
 
 }  // namespace
@@ -227,7 +248,11 @@ extern "C" int ftb_verify_drafts(const float* probs, long long p_seq, long long 
   if (B > 0x7fffffff / 8) return FTB_ERR_ARG;
   int* st = static_cast<int*>(workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t err = V > kOneCta ? launch<8>(a, B, tokens, counts_out, st, s) : launch<1>(a, B, tokens, counts_out, st, s);
+  // Clusters where a row has more than a few numbers a thread; small CTAs where there are so many that their beginnings, which
+  // wait for single numbers, have to lie under the reading of others.
+  const cudaError_t err = V <= 4096                              ? launch<1, 512>(a, B, tokens, counts_out, st, s)
+                          : B <= current_sm_count() / 8 ? launch<8, 512>(a, B, tokens, counts_out, st, s)
+                                                                 : launch<8, 256>(a, B, tokens, counts_out, st, s);
   count_launch();
   if (err != cudaSuccess) cudaGetLastError();
   return err == cudaSuccess ? FTB_OK : FTB_ERR_LAUNCH;
