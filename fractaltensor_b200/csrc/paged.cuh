@@ -63,6 +63,18 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t codes) {
   return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
 }
 
+// Four codes -> fp16 numbers of the lower and the upper two.
+__device__ __forceinline__ void e4m3x4_to_f16x2(uint32_t codes, uint32_t& lower, uint32_t& upper) {
+  asm("{\n.reg .b16 l, u;\nmov.b32 {l, u}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, u;\n}"
+      : "=&r"(lower), "=r"(upper)
+      : "r"(codes));
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
 template <typename T>
 __device__ __forceinline__ float2 unpack2(uint32_t v);
 template <>

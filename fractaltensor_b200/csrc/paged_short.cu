@@ -248,8 +248,9 @@ paged_short_kernel(const __grid_constant__ PagedAttn a, float* __restrict__ part
         if constexpr (k8) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint32_t a0 = e4m3x2_to_f16x2(w0[i] & 0xffffu), a1 = e4m3x2_to_f16x2(w1[i] & 0xffffu);
-            const uint32_t a2 = e4m3x2_to_f16x2(w0[i] >> 16), a3 = e4m3x2_to_f16x2(w1[i] >> 16);
+            uint32_t a0, a1, a2, a3;
+            e4m3x4_to_f16x2(w0[i], a0, a2);
+            e4m3x4_to_f16x2(w1[i], a1, a3);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma16816<C>(sc[nt], a0, a1, a2, a3, q[nt][4 * j + i][0], q[nt][4 * j + i][1]);
           }
@@ -343,10 +344,11 @@ paged_short_kernel(const __grid_constant__ PagedAttn a, float* __restrict__ part
         if constexpr (k8) {
           const uint32_t x01 = __byte_perm(vf[0][w], vf[1][w], 0x5140), x23 = __byte_perm(vf[0][w], vf[1][w], 0x7362);
           const uint32_t y01 = __byte_perm(vf[2][w], vf[3][w], 0x5140), y23 = __byte_perm(vf[2][w], vf[3][w], 0x7362);
-          const uint32_t a0 = e4m3x2_to_f16x2(x01 & 0xffffu), a1 = e4m3x2_to_f16x2(x01 >> 16);
-          const uint32_t a2 = e4m3x2_to_f16x2(y01 & 0xffffu), a3 = e4m3x2_to_f16x2(y01 >> 16);
-          const uint32_t b0 = e4m3x2_to_f16x2(x23 & 0xffffu), b1 = e4m3x2_to_f16x2(x23 >> 16);
-          const uint32_t b2 = e4m3x2_to_f16x2(y23 & 0xffffu), b3 = e4m3x2_to_f16x2(y23 >> 16);
+          uint32_t a0, a1, a2, a3, b0, b1, b2, b3;
+          e4m3x4_to_f16x2(x01, a0, a1);
+          e4m3x4_to_f16x2(y01, a2, a3);
+          e4m3x4_to_f16x2(x23, b0, b1);
+          e4m3x4_to_f16x2(y23, b2, b3);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             mma16816<C>(oacc[2 * w][nt], a0, a1, a2, a3, p[nt][0], p[nt][1]);
