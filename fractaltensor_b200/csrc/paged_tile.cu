@@ -546,7 +546,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
           const int lo_col = ctl.see_lo[t][r] - key0, hi_col = ctl.see_hi[t][r] - key0;
           const bool cut = __any_sync(0xffffffffu, mine && (lo_col > 0 || hi_col < kMyKeys - 1));
           // kChunk scores at a time, read again for the weights.  (A thread that spills goes to L2 for it: shared memory has taken
-          // L1's room.)
+          // L1's room.  And loops instead of straight code: with several roles on an SM its instruction cache is what runs out.)
           constexpr int kChunk = k8 ? 32 : 64;
           uint32_t s[kChunk];
           auto scores = [&](int n) {
@@ -554,13 +554,15 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
             for (int e = 0; e < kChunk; e += 32) tmem_ld32p(s_addr + n * kChunk + e, s + e);
             tmem_ld_wait();
             if (cut) {
+              const int lo = lo_col - n * kChunk, hi = hi_col - n * kChunk;
+              asm volatile("" ::: "memory");  // (a branch, not a select for every score)
 #pragma unroll
               for (int e = 0; e < kChunk; ++e)
-                if (n * kChunk + e < lo_col || n * kChunk + e > hi_col) s[e] = 0xff800000u;
+                if (e < lo || e > hi) s[e] = 0xff800000u;
             }
           };
           float mx = -INFINITY;
-#pragma unroll
+#pragma unroll 1
           for (int n = 0; n < kMyKeys / kChunk; ++n) {
             scores(n);
             float mx8[8];
@@ -570,7 +572,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
             for (int e = 16; e < kChunk; e += 16)
 #pragma unroll
               for (int q = 0; q < 8; ++q) mx8[q] = fmax3(mx8[q], __uint_as_float(s[e + q]), __uint_as_float(s[e + 8 + q]));
-            mx = fmaxf(mx, fmaxf(fmax3(mx8[0], mx8[1], mx8[2]), fmaxf(fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]))));
+            mx = fmax3(mx, fmax3(mx8[0], mx8[1], mx8[2]), fmaxf(fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
           }
           if constexpr (kParts == 2) {
             // The larger of the two halves.  (What is overwritten here the other thread has read before its weights of the block in
@@ -611,7 +613,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
           }
           const float minus = add - top;
           float sum8[8] = {};
-#pragma unroll
+#pragma unroll 1
           for (int n = 0; n < kMyKeys / kChunk; ++n) {
             scores(n);
 #pragma unroll
