@@ -4,16 +4,16 @@
 //
 // One persistent CTA per SM walks its piece of the line of work (paged_work.cuh):
 //   warp 0        the walk, announced to the others through a ring of stretches, and the loads of K and V, page by page: TMA boxes
-//                 of a page's rows into the swizzled tiles that the products read; 8-bit pages only into L2, some tiles ahead
+//                 of a page's rows into the swizzled tiles that the products read; 8-bit pages and their exponents as they are
 //   warp 1        issues the products
 //   softmax       two slots of 128 rows; their warps also fetch the queries and write the results.  16-bit caches: 16 warps, two
 //                 threads a row with 64 keys each (a row's chain from scores to weights sits between two products, and is what bounds
 //                 a tile); 8-bit: 8 warps, a thread a row, which leaves the registers of the others to the conversion
 //   16-bit caches: one more warp zeroes values in front of and behind the keys that the tile sees (what lies there may be
 //                 anything, and 0 * NaN is NaN), told by warp 0 which blocks need it
-//   8-bit caches: eight more warps load codes, turn them into fp16 and write the tiles, four of them one tile, the other four
-//                 the next (codes through shared memory took that from the products, whose operands are read from it at close to
-//                 what it gives)
+//   8-bit caches: eight more warps turn codes into fp16 tiles, four of them one tile, the other four the next.  (They could load
+//                 codes themselves, which would spare shared memory two passes; measured, they then wait for addresses to be
+//                 translated, one load behind the other: 739 against 4xx us.)
 // kTwo: a tile has 256 rows, 128 to a slot, and a K or V block serves both; else 128 rows, and the slots take turns at the blocks: each
 // has sums of its own for the same rows, which lie in the same lanes of tensor memory and are put together there.
 //
@@ -35,7 +35,7 @@ namespace ftb {
 namespace {
 
 constexpr int kKeys = 128, kAtLeast = 1, kStretches = 4, kRefs = 8;
-constexpr int kMostSlots = 14, kAhead = 12;  // kAhead: 8-bit tiles between L2 and registers
+constexpr int kMostSlots = 14;
 constexpr float kAbove = 8.f;  // as in flash_attn.cu: the maximum in use may lie 2^8 below the real one
 
 struct Stretch {
@@ -60,12 +60,12 @@ struct Control {
   uint64_t q_full[2], s_full[2], p_full[2], pv_done[2], o_free[2], begun, fin[2];
   uint64_t row_max[2][4];  // [slot][quadrant of rows]: the two warps that share 32 rows
   uint64_t kv_full[kMostSlots], kv_empty[kMostSlots];    // tiles that the products read
+  uint64_t raw_full[k8 ? kMostSlots : 1], raw_empty[k8 ? kMostSlots : 1];  // 8-bit blocks
   Edge edges[kStretches];
   uint64_t edge_full[kStretches], edge_empty[kStretches], v_fixed[kMostSlots];
   float half_max[2][2][128], half_sum[2][2][128], top[2][128];  // [slot][part of the keys][row]
   int see_lo[2][128], see_hi[2][128];
   int k_ref[kRefs], v_ref[kRefs];
-  volatile int taken[2];  // 8-bit caches: tiles behind the last one that each group of converting warps has taken
   uint32_t tmem_base;
   int abort, dead;
 };
@@ -74,13 +74,16 @@ template <bool k8, int D, bool kTwo>
 struct Plan {
   static constexpr int kHalf = 128 * 128, kTile = D / 64 * kHalf;
   static constexpr int kQ = (kTwo ? 2 : 1) * kTile;
-  static constexpr int kSmem = 232448, kControl = (sizeof(Control<k8, kTwo>) + 15) / 16 * 16;
-  static constexpr int kRoom = kSmem - 1024 - kControl - kQ;
-  static constexpr int kSlots = kRoom / kTile < kMostSlots ? kRoom / kTile : kMostSlots;
+  static constexpr int kControl = (sizeof(Control<k8, kTwo>) + 15) / 16 * 16, kRoom = 232448 - 1024 - kControl - kQ;
+  static constexpr int kSlots = k8 ? (D == 128 ? 3 : 6) : kRoom / kTile < kMostSlots ? kRoom / kTile : kMostSlots;
+  // 8-bit: a block's codes, and the exponents of its keys and values; as many on their way as there is room for
+  static constexpr int kRaw = 128 * D + 256, kRawRoom = (kRoom - kSlots * kTile) / kRaw;
+  static constexpr int kRawSlots = k8 ? (kRawRoom < kMostSlots ? kRawRoom : kMostSlots) : 0;
+  static constexpr int kSmem = 1024 + kControl + kQ + kSlots * kTile + kRawSlots * kRaw;
   static constexpr int kParts = 1;  // threads of a row
   static constexpr int kSoftmax = 8 * kParts, kConvert = 8;  // warps that turn codes into numbers
   static constexpr int kThreads = 32 * (2 + kSoftmax + (k8 ? kConvert : 1));
-  static_assert(kSlots >= 4, "shared memory budget");
+  static_assert(kSlots >= 3 && (!k8 || kRawSlots >= 3) && kSmem <= 232448, "shared memory budget");
 };
 
 __device__ __forceinline__ void tmem_ld32p(uint32_t taddr, uint32_t* r) {
@@ -99,27 +102,6 @@ __device__ __forceinline__ void tmem_ld32p(uint32_t taddr, uint32_t* r) {
 // 16-byte piece `piece` of row `row` in a tile of 64-column halves of 128-byte swizzled rows.
 __device__ __forceinline__ uint8_t* piece_ptr(uint8_t* tile, int row, int piece) {
   return tile + (piece >> 3) * (128 * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
-}
-
-__device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
-  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
-}
-
-// The loading warp stays at most so far ahead that one group has taken a tile behind tile `behind`.  (It may fall behind them:
-// what it would have brought into L2 they have loaded themselves.)
-__device__ __forceinline__ bool keep_pace(volatile int* taken, int behind, volatile int* s_abort, int* status) {
-  if (max(taken[0], taken[1]) > behind) return true;
-  const uint64_t t0 = globaltimer_ns();
-  while (max(taken[0], taken[1]) <= behind) {
-    if (*s_abort) return false;
-    if (globaltimer_ns() - t0 > FTB_WAIT_TIMEOUT_NS) {
-      *s_abort = 1;
-      atomicCAS(status, 0, FTB_ERR_TIMEOUT_SLOT);
-      return false;
-    }
-    __nanosleep(100);
-  }
-  return true;
 }
 
 // Tile n of the stream of K and V blocks of a stretch.  kTwo: K0, V0, K1, V1, ..; else, the slots taking turns at the blocks,
@@ -160,14 +142,15 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
                   float* __restrict__ parts, PagedCut* __restrict__ cuts) {
   using P = Plan<k8, D, kTwo>;
   using C = typename std::conditional<k8, __half, T>::type;
-  constexpr int R = kTwo ? 256 : 128, kSlots = P::kSlots;
+  constexpr int R = kTwo ? 256 : 128, kSlots = P::kSlots, kRawSlots = P::kRawSlots;
   constexpr int kParts = P::kParts, kMyKeys = kKeys / kParts;
   extern __shared__ uint8_t smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, piece = blockIdx.x;
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* sQ = smem;
   uint8_t* sKV = sQ + P::kQ;
-  Control<k8, kTwo>& ctl = *reinterpret_cast<Control<k8, kTwo>*>(sKV + kSlots * P::kTile);
+  uint8_t* sRaw = sKV + kSlots * P::kTile;
+  Control<k8, kTwo>& ctl = *reinterpret_cast<Control<k8, kTwo>*>(sRaw + kRawSlots * P::kRaw);
   volatile int* s_abort = &ctl.abort;
   int* status = a.status;
 
@@ -195,7 +178,12 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
       mbar_init(&ctl.kv_empty[i], 1);
       mbar_init(&ctl.v_fixed[i], 1);
     }
-    ctl.taken[0] = ctl.taken[1] = 0;
+    if constexpr (k8) {
+      for (int i = 0; i < kMostSlots; ++i) {
+        mbar_init(&ctl.raw_full[i], 1);
+        mbar_init(&ctl.raw_empty[i], 4);
+      }
+    }
     for (int i = 0; i < kStretches; ++i) {
       mbar_init(&ctl.edge_full[i], 1);
       mbar_init(&ctl.edge_empty[i], 1);
@@ -243,7 +231,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
     PagedWalk<R, kKeys> walk;
     walk.begin(a, line, piece, seq0, at0);
     const int pages = kKeys >> a.batch.page_shift;  // of a block
-    int slot = 0, edges = 0, tiles0 = 0;  // tiles0: tiles of the stretches so far
+    int slot = 0, edges = 0;
     uint32_t phase = 0;
     bool ok = true;
     auto tell = [&](const Edge& e) -> bool {
@@ -299,34 +287,37 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
         const bool here = lane >= p0 && lane < p1;
         int page = page_next;
         page_next = page_of_tile(n + 1);  // on its way while this one waits for room
-        ok = k8 ? keep_pace(ctl.taken, tiles0 + n - kAhead, s_abort, status)
-                : mbar_wait_warp(&ctl.kv_empty[slot], phase ^ 1u, s_abort, status, FTB_ERR_TIMEOUT_SLOT);
+        uint64_t* full = k8 ? &ctl.raw_full[slot] : &ctl.kv_full[slot];
+        ok = mbar_wait_warp(k8 ? &ctl.raw_empty[slot] : &ctl.kv_empty[slot], phase ^ 1u, s_abort, status, FTB_ERR_TIMEOUT_SLOT);
         if (!ok) break;
         if (here && (page < 0 || page >= a.batch.pages)) {
           atomicCAS(status, 0, FTB_ERR_INDEX);
           page = 0;
         }
-        if constexpr (k8) {
-          const long long at = ((static_cast<long long>(page) * a.kv_heads + w.h) << a.batch.page_shift) * D;
-          if (here) prefetch_l2((x.is_v ? a.v : a.k) + at, D << a.batch.page_shift);
-        } else {
-          if (lane == 0) mbar_arrive_expect_tx(&ctl.kv_full[slot], ((p1 - p0) << a.batch.page_shift) * (2 * D));
-          __syncwarp();
-          if (here) {
+        if (lane == 0) mbar_arrive_expect_tx(full, ((p1 - p0) << a.batch.page_shift) * (k8 ? D + (x.is_v ? 1 : 2) : 2 * D));
+        __syncwarp();
+        if (here) {
+          if constexpr (k8) {
+            const long long row = (static_cast<long long>(page) * a.kv_heads + w.h) << a.batch.page_shift;
+            const uint32_t rows = 1u << a.batch.page_shift;
+            uint8_t* dst = sRaw + slot * P::kRaw;
+            bulk_load_1d(dst + lane * rows * D, (x.is_v ? a.v : a.k) + row * D, rows * D, full);
+            bulk_load_1d(dst + 128 * D + 128 + lane * rows, a.v_exp + row, rows, full);
+            if (!x.is_v) bulk_load_1d(dst + 128 * D + lane * rows, a.k_exp + row, rows, full);
+          } else {
             const CUtensorMap* m = x.is_v ? &mapV : &mapK;
             uint8_t* dst = sKV + slot * P::kTile + (lane << a.batch.page_shift) * 128;
             const int y = (page * a.kv_heads + w.h) << a.batch.page_shift;
-            tma_load_2d(dst, m, &ctl.kv_full[slot], 0, y);
-            if constexpr (D == 128) tma_load_2d(dst + P::kHalf, m, &ctl.kv_full[slot], 64, y);
+            tma_load_2d(dst, m, full, 0, y);
+            if constexpr (D == 128) tma_load_2d(dst + P::kHalf, m, full, 64, y);
           }
         }
         if (!k8 && x.is_v && (key0 < w.keys.lo || key0 + kKeys > w.keys.hi)) ok = tell({slot, key0, w.keys.lo, w.keys.hi, phase});
-        if (++slot == kSlots) {
+        if (++slot == (k8 ? kRawSlots : kSlots)) {
           slot = 0;
           phase ^= 1u;
         }
       }
-      tiles0 += 2 * blocks;
     }
     if (!k8 && ok) tell({-1, 0, 0, 0, 0u});
   } else if (warp == 1) {
@@ -739,73 +730,42 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
   } else {
     // ------------------------------------------------------------- codes to fp16
     // Two groups of four warps take the tiles in turn; warp cw of a group converts keys 32 cw .. + 31.  Each warp finds the block's
-    // largest exponents on its own: lane i holds the four bytes of keys 4 i .. + 3, which are of one page.  Exponents and codes
-    // are loaded a tile of the group's ahead, the pages that they lie in two; nothing is done with them before (a use waits).
+    // largest exponents on its own: lane i holds the four bytes of keys 4 i .. + 3.
     const int cw = warp & 3, group = (warp - 2 - P::kSoftmax) >> 2;
     int count = 0, blocks0 = 0;  // tiles and blocks of the stretches so far
     bool ok = true;
-    constexpr uint32_t kNone = 0xffffffffu;
+    // a lane: piece c of keys first, first + 32 / kRow, ..
+    constexpr int kRow = D / 16, kPieces = kRow;
+    const int first = cw * 32 + lane / kRow, c = lane % kRow;
+    // Where the two halves of a piece go in a tile, rows of `first` apart.  d 128: lanes of the upper half of a row begin with
+    // the second one, so that eight lanes reach all banks.
+    const bool swap = D == 128 && c >= 4;
+    constexpr int kTurns = kRow / 4;  // after so many pieces the rows are 8 apart, and the swizzle is the same again
+    uint32_t off[kTurns][2];
+#pragma unroll
+    for (int k = 0; k < kTurns; ++k)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int key = first + k * (32 / kRow), to = 2 * c + (swap ? 1 - e : e);
+        off[k][e] = (to >> 3) * P::kHalf + first * 128 + (((to & 7) ^ (key & 7)) << 4);
+      }
     for (int i = 0; ok; ++i) {
       if (!await(i)) break;
-      const Stretch x = ctl.ring[i % kStretches];
-      give_back(i);
-      const int tiles = 2 * x.blocks, n0 = (group - count) & 1;
-      const int* table = a.batch.table + static_cast<long long>(x.b) * a.batch.W;
-      auto is_v = [&](int n) { return stream_tile<kTwo>(n, x.blocks).is_v; };
-      auto key_of = [&](int n) { return (x.block0 + stream_tile<kTwo>(n, x.blocks).j) * kKeys + 4 * lane; };
-      auto seen = [&](int n) { const int key = key_of(n); return n < tiles && key + 3 >= x.keys.lo && key < x.keys.hi; };
-      auto load_page = [&](int n) -> int { return seen(n) ? __ldg(table + (key_of(n) >> a.batch.page_shift)) : 0; };
-      // the cache row of key 4 lane of tile n, or none
-      auto row_of = [&](int n, int page) -> uint32_t {
-        if (!seen(n)) return kNone;
-        if (page < 0 || page >= a.batch.pages) page = 0;
-        return ((static_cast<uint32_t>(page) * a.kv_heads + x.h) << a.batch.page_shift) + (key_of(n) & ((1 << a.batch.page_shift) - 1));
-      };
-      uint32_t kw = 0, vw = 0;  // exponents
-      auto load_exponents = [&](uint32_t row) {
-        kw = vw = 0;
-        if (row != kNone) {
-          kw = *reinterpret_cast<const uint32_t*>(a.k_exp + row);
-          vw = *reinterpret_cast<const uint32_t*>(a.v_exp + row);
-        }
-      };
-      // a lane: piece c of keys cw * 32 + lane / kRow, + 32 / kRow, ..
-      constexpr int kRow = D / 16, kPieces = kRow;
-      const int first = cw * 32 + lane / kRow, c = lane % kRow;
-      uint4 v[kPieces];
-      // Where the two halves of a piece go in a tile, rows of `first` apart.  d 128: lanes of the upper half of a row begin with
-      // the second one, so that eight lanes reach all banks.
-      const bool swap = D == 128 && c >= 4;
-      constexpr int kTurns = kRow / 4;  // after so many pieces the rows are 8 apart, and the swizzle is the same again
-      uint32_t off[kTurns][2];
-#pragma unroll
-      for (int k = 0; k < kTurns; ++k)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int key = first + k * (32 / kRow), to = 2 * c + (swap ? 1 - e : e);
-          off[k][e] = (to >> 3) * P::kHalf + first * 128 + (((to & 7) ^ (key & 7)) << 4);
-        }
-      auto load_piece = [&](const unsigned char* from, uint32_t row4, int k) {
-        const int key = first + k * (32 / kRow);
-        const uint32_t row = __shfl_sync(0xffffffffu, row4, key >> 2);
-        v[k] = make_uint4(0u, 0u, 0u, 0u);
-        if (row != kNone) v[k] = *reinterpret_cast<const uint4*>(from + (static_cast<size_t>(row) + (key & 3)) * D + c * 16);
-      };
-      {
-        const uint32_t row = row_of(n0, load_page(n0));
-        load_exponents(row);
-        const unsigned char* from = is_v(n0) ? a.v : a.k;
-#pragma unroll
-        for (int k = 0; k < kPieces; ++k) load_piece(from, row, k);
-      }
-      int page = load_page(n0 + 2);
-      for (int n = n0; n < tiles && ok; n += 2) {
+      const Stretch& x = ctl.ring[i % kStretches];
+      const int tiles = 2 * x.blocks;
+      for (int n = (group - count) & 1; n < tiles && ok; n += 2) {
         const StreamTile y = stream_tile<kTwo>(n, x.blocks);
-        const int ref = (blocks0 + y.j) & (kRefs - 1);
-        const int slot = (count + n) % kSlots;
-        const uint32_t phase = (count + n) / kSlots & 1;
+        const int slot = (count + n) % kSlots, raw = (count + n) % kRawSlots;
         const int key0 = (x.block0 + y.j) * kKeys;
         const bool edge = key0 < x.keys.lo || key0 + kKeys > x.keys.hi;
+        ok = mbar_wait_warp(&ctl.raw_full[raw], (count + n) / kRawSlots & 1, s_abort, status, FTB_ERR_TIMEOUT_TMA);
+        if (!ok) break;
+        const uint8_t* from = sRaw + raw * P::kRaw;
+        const uint4* src = reinterpret_cast<const uint4*>(from) + first * kRow + c;
+        uint4 v[kPieces];
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) v[k] = src[k * 32];
+        uint32_t kw = reinterpret_cast<const uint32_t*>(from + 128 * D)[lane], vw = reinterpret_cast<const uint32_t*>(from + 128 * D + 128)[lane];
         if (edge) {  // keys that nobody sees: exponents 0
           uint32_t keep = 0;
 #pragma unroll
@@ -820,25 +780,23 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
           w = __vmaxu4(w, w >> 16);
           return static_cast<int>(max(1u, max(w & 0xffu, w >> 8 & 0xffu)));
         };
-        const int top = __reduce_max_sync(0xffffffffu, largest(y.is_v ? vw : kw));
+        const uint32_t mine = y.is_v ? vw : kw;
+        const int top = __reduce_max_sync(0xffffffffu, largest(mine));
         if (!y.is_v) {
           const int v_top = __reduce_max_sync(0xffffffffu, largest(vw));
           if (cw == 0 && lane == 0) {
+            const int ref = (blocks0 + y.j) & (kRefs - 1);
             ctl.k_ref[ref] = top;
             ctl.v_ref[ref] = v_top;
           }
         }
-        const int mine = __shfl_sync(0xffffffffu, y.is_v ? vw : kw, cw * 8 + (lane >> 2)) >> (8 * (lane & 3)) & 0xff;
-        const int below = max(0, top - mine);
+        const int e = __shfl_sync(0xffffffffu, mine, cw * 8 + (lane >> 2)) >> (8 * (lane & 3)) & 0xff;  // of key cw * 32 + lane
+        const int below = max(0, top - e);
         uint32_t by = below < 15 ? static_cast<uint32_t>(15 - below) << 10 : below <= 24 ? 1u << (24 - below) : 0u;  // 2^-below as fp16
         by |= by << 16;
-        const uint32_t row_next = row_of(n + 2, page);
-        load_exponents(row_next);
-        page = load_page(n + 4);
-        ok = mbar_wait_warp(&ctl.kv_empty[slot], phase ^ 1u, s_abort, status, FTB_ERR_TIMEOUT_SLOT);
+        ok = mbar_wait_warp(&ctl.kv_empty[slot], ((count + n) / kSlots & 1) ^ 1u, s_abort, status, FTB_ERR_TIMEOUT_SLOT);
         if (!ok) break;
         uint8_t* tile = sKV + slot * P::kTile;
-        const unsigned char* from = is_v(n + 2) ? a.v : a.k;
 #pragma unroll
         for (int k = 0; k < kPieces; ++k) {
           const int key = first + k * (32 / kRow);
@@ -857,15 +815,15 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
+          mbar_arrive(&ctl.raw_empty[raw]);
           mbar_arrive(&ctl.kv_full[slot]);
-          if (cw == 0) ctl.taken[group] = count + n + 1;
         }
-#pragma unroll
-        for (int k = 0; k < kPieces; ++k) load_piece(from, row_next, k);  // the group's next tile: on its way while the other one works
       }
-      count += tiles;
+      const bool last = x.last != 0;
       blocks0 += x.blocks;
-      if (x.last) break;
+      give_back(i);
+      count += tiles;
+      if (last) break;
     }
   }
 
