@@ -125,7 +125,7 @@ Form form_of(int T, int B, int group) {
   // are read through L2.)
   if (T <= B) return {rows <= 8ll * B ? 1 : 2, INT_MAX, 0};
   if (rows <= 16) return {rows <= 8 ? 1 : 2, INT_MAX, 0};
-  const int tile = rows > 128ll * B ? 256 : 128;
+  const int tile = rows > 128ll * B ? 256 : rows > 64ll * B ? 128 : 64;
   if (B == 1) return {0, 0, tile};
   return {group <= 8 ? 1 : 2, group <= 8 ? 8 : 16, tile};
 }

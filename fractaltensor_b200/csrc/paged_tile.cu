@@ -6,16 +6,17 @@
 //   warp 0        the walk, announced to the others through a ring of stretches, and the loads of K and V, page by page: TMA boxes
 //                 of a page's rows into the swizzled tiles that the products read; 8-bit pages and their exponents as they are
 //   warp 1        issues the products
-//   softmax       two slots of 128 rows; their warps also fetch the queries and write the results.  16-bit caches: 16 warps, two
-//                 threads a row with 64 keys each (a row's chain from scores to weights sits between two products, and is what bounds
-//                 a tile); 8-bit: 8 warps, a thread a row, which leaves the registers of the others to the conversion
+//   warps 2..9    softmax: two slots of 128 threads, a thread a row; they also fetch the queries and write the results
 //   16-bit caches: one more warp zeroes values in front of and behind the keys that the tile sees (what lies there may be
 //                 anything, and 0 * NaN is NaN), told by warp 0 which blocks need it
 //   8-bit caches: eight more warps turn codes into fp16 tiles, four of them one tile, the other four the next.  (They could load
 //                 codes themselves, which would spare shared memory two passes; measured, they then wait for addresses to be
 //                 translated, one load behind the other: 739 against 4xx us.)
-// kTwo: a tile has 256 rows, 128 to a slot, and a K or V block serves both; else 128 rows, and the slots take turns at the blocks: each
-// has sums of its own for the same rows, which lie in the same lanes of tensor memory and are put together there.
+// A row's chain from scores to weights sits between two products, so that two slots keep the tensor cores busy.  Tiles of 256 rows:
+// 128 to a slot, and a K or V block serves both.  Of 128: the slots take turns at the blocks; each has sums of its own for the same
+// rows, which lie in the same lanes of tensor memory and are put together there.  Of 64: the rows are there twice, in the lower
+// and the upper 64 lanes, the ones for the first 64 keys of a block and the others for the rest (weights of the other half
+// are 0), which halves the chain.
 //
 // 8-bit caches: a block's codes become fp16 numbers code * 2^(e - e_max), e_max the largest exponent of the block's keys: exact
 // where exponents are within 15 of each other, and off by 2^-33 of the block's largest number otherwise.  2^e_max goes to the
@@ -57,21 +58,21 @@ struct Control {
   PagedLineRoom line;
   Stretch ring[kStretches];
   uint64_t ring_full[kStretches], ring_empty[kStretches];
-  uint64_t q_full[2], s_full[2], p_full[2], pv_done[2], o_free[2], begun, fin[2];
-  uint64_t row_max[2][4];  // [slot][quadrant of rows]: the two warps that share 32 rows
+  uint64_t q_full[2], s_full[2], p_full[2], pv_done[2], o_free[2], begun, fin, fin_rows;
   uint64_t kv_full[kMostSlots], kv_empty[kMostSlots];    // tiles that the products read
   uint64_t raw_full[k8 ? kMostSlots : 1], raw_empty[k8 ? kMostSlots : 1];  // 8-bit blocks
   Edge edges[kStretches];
   uint64_t edge_full[kStretches], edge_empty[kStretches], v_fixed[kMostSlots];
-  float half_max[2][2][128], half_sum[2][2][128], top[2][128];  // [slot][part of the keys][row]
+  float top[2][128], sum[2][128];  // [slot][row]
   int see_lo[2][128], see_hi[2][128];
   int k_ref[kRefs], v_ref[kRefs];
   uint32_t tmem_base;
   int abort, dead;
 };
 
-template <bool k8, int D, bool kTwo>
+template <bool k8, int D, int R>
 struct Plan {
+  static constexpr bool kTwo = R == 256, kDup = R == 64;
   static constexpr int kHalf = 128 * 128, kTile = D / 64 * kHalf;
   static constexpr int kQ = (kTwo ? 2 : 1) * kTile;
   static constexpr int kControl = (sizeof(Control<k8, kTwo>) + 15) / 16 * 16, kRoom = 232448 - 1024 - kControl - kQ;
@@ -80,8 +81,7 @@ struct Plan {
   static constexpr int kRaw = 128 * D + 256, kRawRoom = (kRoom - kSlots * kTile) / kRaw;
   static constexpr int kRawSlots = k8 ? (kRawRoom < kMostSlots ? kRawRoom : kMostSlots) : 0;
   static constexpr int kSmem = 1024 + kControl + kQ + kSlots * kTile + kRawSlots * kRaw;
-  static constexpr int kParts = 1;  // threads of a row
-  static constexpr int kSoftmax = 8 * kParts, kConvert = 8;  // warps that turn codes into numbers
+  static constexpr int kSoftmax = 8, kConvert = 8;  // warps
   static constexpr int kThreads = 32 * (2 + kSoftmax + (k8 ? kConvert : 1));
   static_assert(kSlots >= 3 && (!k8 || kRawSlots >= 3) && kSmem <= 232448, "shared memory budget");
 };
@@ -136,14 +136,15 @@ __device__ __forceinline__ Mine blocks_of_slot(const PagedAttn& a, const Stretch
   return {j0, j1, max(0, j1 - j0 + 1)};
 }
 
-template <typename T, bool k8, int D, bool kTwo>
-__global__ void __launch_bounds__(Plan<k8, D, kTwo>::kThreads, 1)
+template <typename T, bool k8, int D, int R>
+__global__ void __launch_bounds__(Plan<k8, D, R>::kThreads, 1)
 paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
                   float* __restrict__ parts, PagedCut* __restrict__ cuts) {
-  using P = Plan<k8, D, kTwo>;
+  using P = Plan<k8, D, R>;
   using C = typename std::conditional<k8, __half, T>::type;
-  constexpr int R = kTwo ? 256 : 128, kSlots = P::kSlots, kRawSlots = P::kRawSlots;
-  constexpr int kParts = P::kParts, kMyKeys = kKeys / kParts;
+  constexpr bool kTwo = P::kTwo, kDup = P::kDup;
+  constexpr int kSlots = P::kSlots, kRawSlots = P::kRawSlots;
+  constexpr int kMyKeys = kDup ? 64 : 128;  // of a block, that a row's lane has
   extern __shared__ uint8_t smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, piece = blockIdx.x;
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -164,15 +165,15 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
       mbar_init(&ctl.ring_empty[i], 1 + P::kSoftmax + (k8 ? P::kConvert : 0));
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&ctl.q_full[i], (kTwo ? 4 : 8) * kParts);
+      mbar_init(&ctl.q_full[i], kTwo ? 4 : 8);
       mbar_init(&ctl.s_full[i], 1);
-      mbar_init(&ctl.p_full[i], 4 * kParts);
+      mbar_init(&ctl.p_full[i], 4);
       mbar_init(&ctl.pv_done[i], 1);
-      mbar_init(&ctl.o_free[i], (kTwo ? 4 : 8) * kParts);
-      mbar_init(&ctl.fin[i], (kTwo ? 4 : 8) * kParts);
-      for (int k = 0; k < 4; ++k) mbar_init(&ctl.row_max[i][k], 2);
+      mbar_init(&ctl.o_free[i], kTwo ? 4 : 8);
     }
     mbar_init(&ctl.begun, 1);
+    mbar_init(&ctl.fin, 8);
+    mbar_init(&ctl.fin_rows, 8);
     for (int i = 0; i < kMostSlots; ++i) {
       mbar_init(&ctl.kv_full[i], k8 ? 4 : 1);
       mbar_init(&ctl.kv_empty[i], 1);
@@ -215,7 +216,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
   tc_fence_after();
   const uint32_t tmem_base = ctl.tmem_base;
   // tensor memory: S0 [0, 128), S1 [128, 256), O0 [256, 256 + D), O1 [384, 384 + D); P_t (16-bit pairs)
-  // over the first half of the columns that each part of a row's keys has in S_t.
+  // over the first half of S_t's columns; where rows are there twice over the first half of each of S_t's halves.
 
   // Stretch i of this CTA, as every role but the first warp gets it.
   auto await = [&](int i) -> bool {
@@ -442,23 +443,22 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
       if (x.last) break;
     }
   } else if (warp < 2 + P::kSoftmax) {
-    // ------------------------------------------------ softmax: slot t, part h of the keys, row r of the slot's 128
-    const int t = (warp - 2) / (4 * kParts), h = (warp - 2) / 4 % kParts, quad = warp & 3, r = quad * 32 + lane;
+    // ------------------------------------------------ softmax: slot t, row r of its 128
+    const int t = (warp - 2) / 4, quad = warp & 3, r = quad * 32 + lane;
+    const int part = kDup ? quad >> 1 : 0;  // of a block's keys
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
-    const uint32_t s_addr = lane_addr + t * 128 + h * kMyKeys;
-    // the columns of the output that this thread rescales, and those that it finishes
-    constexpr int kScale = D / kParts, kCols = kTwo ? D / kParts : D / (2 * kParts);
-    const uint32_t o_addr = lane_addr + 256 + t * 128 + h * kScale;
-    const int c0 = kTwo ? h * kCols : (t * kParts + h) * kCols;
-    // parities: bit 0 the next scores, 1 the rows' maxima, 2 fin, 4 + t the next product P V of slot t in a stretch
+    const uint32_t s_addr = lane_addr + t * 128 + part * 64, o_addr = lane_addr + 256 + t * 128;
+    constexpr int kCols = kTwo ? D : D / 2;  // of the output, that this thread finishes
+    const int c0 = kTwo ? 0 : t * kCols;
+    // parities: bit 0 the next scores, 2 fin, 3 fin_rows, 4 + t the next product P V of slot t in a stretch
     uint32_t par = 0;
     int blocks0 = 0;  // blocks of the stretches so far
     bool ok = true;
     for (int i = 0; ok; ++i) {
       if (!await(i)) break;
       const Stretch& x = ctl.ring[i % kStretches];  // (read again where it is needed, and given back behind the results: registers)
-      const int row0 = (kTwo ? t * 128 : 0) + quad * 32, row = row0 + lane;  // of the tile
-      const bool busy = row0 < x.rows;                                       // this warp has rows
+      const int row0 = kTwo ? t * 128 + quad * 32 : kDup ? (quad & 1) * 32 : quad * 32, row = row0 + lane;  // of the tile
+      const bool busy = row0 < x.rows;  // this warp has rows
       const bool mine = row < x.rows;
       int tok, head;
       auto place = [&] {
@@ -467,7 +467,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
         head = x.h * a.group + flat - token * a.group;
       };
       place();
-      {  // (every part of a row writes the same; read back a block at a time, which saves registers)
+      {  // (read back a block at a time, which saves registers)
         const long long pos = mine ? x.pos0 + tok : -1;
         ctl.see_hi[t][r] = static_cast<int>(max(-1ll, min(pos, static_cast<long long>(x.keys.hi) - 1)));
         ctl.see_lo[t][r] = a.window > 0 ? static_cast<int>(max(0ll, min(pos - a.window + 1, static_cast<long long>(INT_MAX)))) : 0;
@@ -533,7 +533,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
             add = static_cast<float>(vr - 127);
             inv = exponent_scale(254 - vr);
           }
-          const int key0 = (x.block0 + j) * kKeys + h * kMyKeys;
+          const int key0 = (x.block0 + j) * kKeys + part * 64;
           const int lo_col = ctl.see_lo[t][r] - key0, hi_col = ctl.see_hi[t][r] - key0;
           const bool cut = __any_sync(0xffffffffu, mine && (lo_col > 0 || hi_col < kMyKeys - 1));
           // kChunk scores at a time, read again for the weights.  (A thread that spills goes to L2 for it: shared memory has taken
@@ -565,17 +565,6 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
               for (int q = 0; q < 8; ++q) mx8[q] = fmax3(mx8[q], __uint_as_float(s[e + q]), __uint_as_float(s[e + 8 + q]));
             mx = fmax3(mx, fmax3(mx8[0], mx8[1], mx8[2]), fmaxf(fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
           }
-          if constexpr (kParts == 2) {
-            // The larger of the two halves.  (What is overwritten here the other thread has read before its weights of the block in
-            // front, which the product that these scores came behind waited for.)
-            ctl.half_max[t][h][r] = mx;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ctl.row_max[t][quad]);
-            ok = mbar_wait_warp(&ctl.row_max[t][quad], par >> 1 & 1u, s_abort, status, FTB_ERR_TIMEOUT_EPI);
-            if (!ok) break;
-            par ^= 2u;
-            mx = fmaxf(mx, ctl.half_max[t][h ^ 1][r]);
-          }
           // (a row may see nothing of a block: the lowest finite number keeps its weights 0)
           const float m_new = fmaxf(fmaf(mx, f, add), -FLT_MAX);
           if (k == 0) {
@@ -591,7 +580,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
               if (need) top = m_new;
               l *= keep;
 #pragma unroll 1
-              for (int ch = 0; ch < kScale / 16; ++ch) {
+              for (int ch = 0; ch < D / 16; ++ch) {
                 uint32_t o[16];
                 tmem_ld16(o_addr + ch * 16, o);
                 tmem_ld_wait();
@@ -608,18 +597,23 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
           for (int n = 0; n < kMyKeys / kChunk; ++n) {
             scores(n);
 #pragma unroll
-            for (int part = 0; part < kChunk / 32; ++part) {
+            for (int half = 0; half < kChunk / 32; ++half) {
               uint32_t pk[16];
 #pragma unroll
               for (int c = 0; c < 16; ++c) {
-                const float p0 = exp2_fast(fmaf(__uint_as_float(s[32 * part + 2 * c]), f, minus));
-                const float p1 = exp2_fast(fmaf(__uint_as_float(s[32 * part + 2 * c + 1]), f, minus));
+                const float p0 = exp2_fast(fmaf(__uint_as_float(s[32 * half + 2 * c]), f, minus));
+                const float p1 = exp2_fast(fmaf(__uint_as_float(s[32 * half + 2 * c + 1]), f, minus));
                 sum8[(2 * c) & 7] += p0;
                 sum8[(2 * c + 1) & 7] += p1;
                 pk[c] = Fmt<C>::pack2(p0, p1);
               }
-              tmem_st16(s_addr + n * (kChunk / 2) + part * 16, pk);  // over scores that this thread has read
+              tmem_st16(s_addr + n * (kChunk / 2) + half * 16, pk);  // over scores that this thread has read
             }
+          }
+          if constexpr (kDup) {
+            const uint32_t none[16] = {};
+            tmem_st16(lane_addr + t * 128 + (part ^ 1) * 64, none);
+            tmem_st16(lane_addr + t * 128 + (part ^ 1) * 64 + 16, none);
           }
           l = fmaf(((sum8[0] + sum8[1]) + (sum8[2] + sum8[3])) + ((sum8[4] + sum8[5]) + (sum8[6] + sum8[7])), inv, l);
           tmem_st_wait();
@@ -635,49 +629,95 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
       blocks0 += x.blocks;
       if (m.n == 0) top = -FLT_MAX;
 
-      // ---- results: the parts of a row, and without kTwo those of the other slot
+      // ---- results: of both slots, where they share the rows
       float other_m = -FLT_MAX, other_l = 0.f;
       int n_other = 0;
-      if (kTwo ? kParts == 2 && m.n > 0 : x.blocks > 0) {
-        if (h == 0) ctl.top[t][r] = top;
-        ctl.half_sum[t][h][r] = l;
-        uint64_t* fin = &ctl.fin[kTwo ? t : 0];
+      if (!kTwo && x.blocks > 0) {
+        ctl.top[t][r] = top;
+        ctl.sum[t][r] = l;
         __syncwarp();
-        if (lane == 0) mbar_arrive(fin);
-        ok = mbar_wait_warp(fin, par >> 2 & 1u, s_abort, status, FTB_ERR_TIMEOUT_EPI);
+        if (lane == 0) mbar_arrive(&ctl.fin);
+        ok = mbar_wait_warp(&ctl.fin, par >> 2 & 1u, s_abort, status, FTB_ERR_TIMEOUT_EPI);
         if (!ok) break;
         par ^= 4u;
-        if constexpr (kParts == 2) l += ctl.half_sum[t][h ^ 1][r];
-        if constexpr (!kTwo) {
-          n_other = blocks_of_slot<kTwo>(a, x, t ^ 1).n;
-          other_m = ctl.top[t ^ 1][r];
-#pragma unroll
-          for (int k = 0; k < kParts; ++k) other_l += ctl.half_sum[t ^ 1][k][r];
-        }
+        n_other = blocks_of_slot<kTwo>(a, x, t ^ 1).n;
+        other_m = ctl.top[t ^ 1][r];
+        other_l = ctl.sum[t ^ 1][r];
       }
       if (m.n > 0) ok = mbar_wait_warp(&ctl.pv_done[t], ((par >> (4 + t)) + m.n - 1) & 1u, s_abort, status, FTB_ERR_TIMEOUT_MMA);
       if (ok && n_other > 0) ok = mbar_wait_warp(&ctl.pv_done[t ^ 1], ((par >> (4 + (t ^ 1))) + n_other - 1) & 1u, s_abort, status, FTB_ERR_TIMEOUT_MMA);
       if (!ok) break;
       par ^= static_cast<uint32_t>(m.n & 1) << (4 + t) ^ static_cast<uint32_t>(n_other & 1) << (4 + (t ^ 1));
       tc_fence_after();
-      const float all_m = fmaxf(top, other_m), keep = exp2_fast(top - all_m), take = exp2_fast(other_m - all_m);
-      const float sum = l * keep + other_l * take;
+      float all_m = fmaxf(top, other_m);
+      float keep = exp2_fast(top - all_m), take = exp2_fast(other_m - all_m), sum = l * keep + other_l * take;
+      // this thread's columns, 16 at a time
+      auto columns = [&](int ch, float (&y)[16]) {
+        uint32_t o[16], o2[16];
+        if (m.n > 0) tmem_ld16(lane_addr + 256 + t * 128 + c0 + ch * 16, o);
+        if (n_other > 0) tmem_ld16(lane_addr + 256 + (t ^ 1) * 128 + c0 + ch * 16, o2);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          y[e] = (m.n > 0 ? __uint_as_float(o[e]) * keep : 0.f) + (n_other > 0 ? __uint_as_float(o2[e]) * take : 0.f);
+      };
+      // Rows that are there twice: the upper lanes give what they have to the lower ones, through the queries' place, which is free
+      // now: [column / 4][row], four columns each.
+      float4* give = reinterpret_cast<float4*>(sQ);
+      float up = 0.f;  // what the upper lanes' columns are multiplied by
+      if (kDup && x.blocks > 0) {
+        auto everyone = [&]() -> bool {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl.fin_rows);
+          const bool fine = mbar_wait_warp(&ctl.fin_rows, par >> 3 & 1u, s_abort, status, FTB_ERR_TIMEOUT_EPI);
+          par ^= 8u;
+          return fine;
+        };
+        if (part == 1 && busy) {
+#pragma unroll 1
+          for (int ch = 0; ch < kCols / 16; ++ch) {
+            float y[16];
+            columns(ch, y);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) give[(c0 / 4 + ch * 4 + e) * 64 + row] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
+          }
+        }
+        // (top and sum of all slots and lanes are there still: nobody writes the next ones before its queries are taken)
+        ok = everyone();
+        if (!ok) break;
+        if (part == 0) {
+          const float m0 = ctl.top[t][r + 64], m1 = ctl.top[t ^ 1][r + 64], mu = fmaxf(m0, m1);
+          const float lu = ctl.sum[t][r + 64] * exp2_fast(m0 - mu) + ctl.sum[t ^ 1][r + 64] * exp2_fast(m1 - mu);
+          const float m_both = fmaxf(all_m, mu), down = exp2_fast(all_m - m_both);
+          up = exp2_fast(mu - m_both);
+          keep *= down;
+          take *= down;
+          sum = sum * down + lu * up;
+          all_m = m_both;
+        }
+      }
       const float scale = x.whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
       bool odd = false;
-      if (busy) {
+      if (busy && part == 0) {
         place();
         T* out = static_cast<T*>(a.o) + (static_cast<long long>(tok) * a.kv_heads * a.group + head) * D + c0;
-        float* part = parts + static_cast<size_t>(x.place) * part_floats<R, D>();
+        float* place_of = parts + static_cast<size_t>(x.place) * part_floats<R, D>();
 #pragma unroll 1
         for (int ch = 0; ch < kCols / 16; ++ch) {
-          uint32_t o[16], o2[16];
-          if (m.n > 0) tmem_ld16(lane_addr + 256 + t * 128 + c0 + ch * 16, o);
-          if (n_other > 0) tmem_ld16(lane_addr + 256 + (t ^ 1) * 128 + c0 + ch * 16, o2);
-          tmem_ld_wait();
           float y[16];
+          columns(ch, y);
+          if (kDup && x.blocks > 0) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float4 z = give[(c0 / 4 + ch * 4 + e) * 64 + row];
+              y[4 * e] = fmaf(z.x, up, y[4 * e]);
+              y[4 * e + 1] = fmaf(z.y, up, y[4 * e + 1]);
+              y[4 * e + 2] = fmaf(z.z, up, y[4 * e + 2]);
+              y[4 * e + 3] = fmaf(z.w, up, y[4 * e + 3]);
+            }
+          }
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            y[e] = (m.n > 0 ? __uint_as_float(o[e]) * keep : 0.f) + (n_other > 0 ? __uint_as_float(o2[e]) * take : 0.f);
             y[e] *= scale;
             odd |= y[e] != y[e];
           }
@@ -687,7 +727,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
               dst[0] = make_uint4(Fmt<T>::pack2(y[0], y[1]), Fmt<T>::pack2(y[2], y[3]), Fmt<T>::pack2(y[4], y[5]), Fmt<T>::pack2(y[6], y[7]));
               dst[1] = make_uint4(Fmt<T>::pack2(y[8], y[9]), Fmt<T>::pack2(y[10], y[11]), Fmt<T>::pack2(y[12], y[13]), Fmt<T>::pack2(y[14], y[15]));
             } else {
-              float4* dst = reinterpret_cast<float4*>(part + row * D + c0 + ch * 16);
+              float4* dst = reinterpret_cast<float4*>(place_of + row * D + c0 + ch * 16);
 #pragma unroll
               for (int e = 0; e < 4; ++e) dst[e] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
             }
@@ -696,14 +736,20 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
         // rows that something unseen may have made a NaN are left to the joining kernel, which goes through them key by key
         if (mine) {
           const bool again = odd && x.whole && hides(a, x.pos0 + tok, x.keys.lo, x.keys.hi);
-          using Flag = typename std::conditional<kCols == D, uint32_t, typename std::conditional<2 * kCols == D, uint16_t, uint8_t>::type>::type;
+          using Flag = typename std::conditional<kCols == D, uint32_t, uint16_t>::type;
           reinterpret_cast<Flag*>(a.odd + static_cast<long long>(tok) * a.kv_heads * a.group + head)[c0 / kCols] = again ? 1 : 0;
         }
-        if (mine && !x.whole && c0 == 0) *reinterpret_cast<float2*>(part + R * D + 2 * row) = make_float2(all_m, sum);
+        if (mine && !x.whole && c0 == 0) *reinterpret_cast<float2*>(place_of + R * D + 2 * row) = make_float2(all_m, sum);
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&ctl.o_free[kTwo ? t : 0]);
+      if (kDup && x.blocks > 0) {  // the upper lanes' numbers have been read: the next queries may take their place
+        if (lane == 0) mbar_arrive(&ctl.fin_rows);
+        ok = mbar_wait_warp(&ctl.fin_rows, par >> 3 & 1u, s_abort, status, FTB_ERR_TIMEOUT_EPI);
+        par ^= 8u;
+        if (!ok) break;
+      }
       const bool last = x.last != 0;
       give_back(i);
       if (last) break;
@@ -839,38 +885,36 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
   }
 }
 
-template <typename T, bool k8, int D, bool kTwo>
+template <typename T, bool k8, int D, int R>
 int launch(const PagedAttn& a, const CUtensorMap& mK, const CUtensorMap& mV, void* scratch, cudaStream_t stream) {
-  using P = Plan<k8, D, kTwo>;
+  using P = Plan<k8, D, R>;
   static std::atomic<unsigned long long> configured{0};
-  auto kfn = paged_tile_kernel<T, k8, D, kTwo>;
+  auto kfn = paged_tile_kernel<T, k8, D, R>;
   if (!ensure_dynamic_smem(kfn, P::kSmem, configured)) return FTB_ERR_LAUNCH;
   const int pieces = paged_tile_pieces();
   float* parts = static_cast<float*>(scratch);
   const cudaError_t err = launch_dependent(kfn, dim3(pieces), dim3(P::kThreads), P::kSmem, stream, a, mK, mV, parts,
-                                           reinterpret_cast<PagedCut*>(parts + 2 * pieces * part_floats<kTwo ? 256 : 128, D>()));
+                                           reinterpret_cast<PagedCut*>(parts + 2 * pieces * part_floats<R, D>()));
   count_launch();
   if (err != cudaSuccess) cudaGetLastError();
   return err == cudaSuccess ? FTB_OK : FTB_ERR_LAUNCH;
 }
-template <typename T, int D, bool kTwo>
+template <typename T, int D, int R>
 int launch(const PagedAttn& a, int dtype, void* scratch, cudaStream_t stream) {
   CUtensorMap mK = {}, mV = {};
   const uint64_t rows = (static_cast<uint64_t>(a.batch.pages) * a.kv_heads) << a.batch.page_shift;
-  if (a.k_exp != nullptr) {
-    if (rows >= 0xffffffffull) return FTB_ERR_ARG;  // rows are counted in 32 bits
-    return launch<T, true, D, kTwo>(a, mK, mV, scratch, stream);
-  }
+  if (a.k_exp != nullptr) return launch<T, true, D, R>(a, mK, mV, scratch, stream);
   if (rows > 0x7fffffffull) return FTB_ERR_ARG;  // a copy's coordinates have 32 bits
   int rc;
   if ((rc = make_tmap_2d(&mK, a.k, dtype, rows, D, D, 1u << a.batch.page_shift, 64))) return rc;
   if ((rc = make_tmap_2d(&mV, a.v, dtype, rows, D, D, 1u << a.batch.page_shift, 64))) return rc;
-  return launch<T, false, D, kTwo>(a, mK, mV, scratch, stream);
+  return launch<T, false, D, R>(a, mK, mV, scratch, stream);
 }
-template <typename T>
-int launch(const PagedAttn& a, int d, int dtype, bool two, void* scratch, cudaStream_t stream) {
-  if (d == 128) return two ? launch<T, 128, true>(a, dtype, scratch, stream) : launch<T, 128, false>(a, dtype, scratch, stream);
-  return two ? launch<T, 64, true>(a, dtype, scratch, stream) : launch<T, 64, false>(a, dtype, scratch, stream);
+template <typename T, int D>
+int launch(const PagedAttn& a, int dtype, int rows, void* scratch, cudaStream_t stream) {
+  return rows == 256   ? launch<T, D, 256>(a, dtype, scratch, stream)
+         : rows == 128 ? launch<T, D, 128>(a, dtype, scratch, stream)
+                       : launch<T, D, 64>(a, dtype, scratch, stream);
 }
 
 }  // namespace
@@ -878,8 +922,8 @@ int launch(const PagedAttn& a, int d, int dtype, bool two, void* scratch, cudaSt
 int paged_tile_pieces() { return current_sm_count(); }
 
 int paged_tile_launch(const PagedAttn& a, int d, int dtype, int rows, void* scratch, cudaStream_t stream) {
-  return dtype == FTB_F16 ? launch<__half>(a, d, dtype, rows == 256, scratch, stream)
-                          : launch<__nv_bfloat16>(a, d, dtype, rows == 256, scratch, stream);
+  if (dtype == FTB_F16) return d == 128 ? launch<__half, 128>(a, dtype, rows, scratch, stream) : launch<__half, 64>(a, dtype, rows, scratch, stream);
+  return d == 128 ? launch<__nv_bfloat16, 128>(a, dtype, rows, scratch, stream) : launch<__nv_bfloat16, 64>(a, dtype, rows, scratch, stream);
 }
 
 }  // namespace ftb
