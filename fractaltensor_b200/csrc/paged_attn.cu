@@ -114,20 +114,24 @@ int launch_join(const PagedAttn& a, int d, const Pieces& few, const Pieces& many
   return d == 128 ? launch_join<T, false, 128>(a, few, many, stream) : launch_join<T, false, 64>(a, few, many, stream);
 }
 
-// What runs: nt > 0: paged_short.cu with tiles of 8 nt rows for sequences of up to `few` rows; rows > 0: paged_tile.cu with tiles
-// of so many rows for the others.  `few` is the most rows that one tile of paged_short.cu holds: a second one would read the keys again.
+// What runs: few > 0: paged_short.cu with tiles of so many rows for sequences of up to `most` rows; many > 0: paged_tile.cu with tiles
+// of so many for the others.
 struct Form {
-  int nt, few, rows;
+  int few, most, many;
 };
 Form form_of(int T, int B, int group) {
   const long long rows = static_cast<long long>(T) * group;
   // Not more tokens than sequences: a decoding step.  (Where one of them has them all the others are empty, and its tiles
   // are read through L2.)
-  if (T <= B) return {rows <= 8ll * B ? 1 : 2, INT_MAX, 0};
-  if (rows <= 16) return {rows <= 8 ? 1 : 2, INT_MAX, 0};
-  const int tile = rows > 128ll * B ? 256 : rows > 64ll * B ? 128 : 64;
-  if (B == 1) return {0, 0, tile};
-  return {group <= 8 ? 1 : 2, group <= 8 ? 8 : 16, tile};
+  if (T <= B) return {rows <= 8ll * B ? 8 : 16, INT_MAX, 0};
+  if (rows <= 16) return {rows <= 8 ? 8 : 16, INT_MAX, 0};
+  const int many = rows > 128ll * B ? 256 : 128;
+  if (B == 1) return {0, 0, many};
+  // One tile of paged_short.cu: a second one would read the keys again.  16 rows of it take 1.4 to 1.9 times what 8 take, and
+  // about what a tile of 128 does (96 sequences of 4500 keys of 16 bits, 8 kv heads: 8 rows 268 us, 16 378, 128 392; of 8500 of
+  // 8 bits: 310, 509, 657).
+  const int few = group <= 8 && rows > 16ll * B ? 8 : 16;
+  return {few, few, many};
 }
 
 size_t places(int pieces, int rows, int d) { return 2 * static_cast<size_t>(pieces) * rows * (d + 2) * sizeof(float) + pieces * sizeof(PagedCut); }
@@ -142,8 +146,8 @@ extern "C" size_t ftb_paged_attn_scratch_bytes(int T, int B, int kv_heads, int g
   if (T <= 0 || B <= 0 || kv_heads <= 0 || group <= 0 || d <= 0) return 0;
   const Form f = form_of(T, B, group);
   size_t n = rounded(static_cast<size_t>(T) * kv_heads * group * sizeof(uint32_t));
-  if (f.nt > 0) n += rounded(places(paged_short_pieces(f.nt), 8 * f.nt, d));
-  if (f.rows > 0) n += rounded(places(paged_tile_pieces(), f.rows, d));
+  if (f.few > 0) n += rounded(places(paged_short_pieces(f.few), f.few, d));
+  if (f.many > 0) n += rounded(places(paged_tile_pieces(), f.many, d));
   return n;
 }
 
@@ -195,18 +199,18 @@ extern "C" int ftb_paged_attn_fwd(const void* q, long long q_row, long long q_he
   };
   Pieces few{nullptr, nullptr, 0, 0}, many{nullptr, nullptr, 0, 0};
   int err = FTB_OK;
-  if (f.rows > 0) {
-    a.least_rows = f.few + 1;
+  if (f.many > 0) {
+    a.least_rows = f.most + 1;
     a.most_rows = INT_MAX;
-    many = pieces_at(paged_tile_pieces(), f.rows);
-    err = paged_tile_launch(a, d, dtype, f.rows, at, stream);
-    at += rounded(places(many.pieces, f.rows, d));
+    many = pieces_at(paged_tile_pieces(), f.many);
+    err = paged_tile_launch(a, d, dtype, f.many, at, stream);
+    at += rounded(places(many.pieces, f.many, d));
   }
-  if (f.nt > 0 && err == FTB_OK) {
+  if (f.few > 0 && err == FTB_OK) {
     a.least_rows = 1;
-    a.most_rows = f.few;
-    few = pieces_at(paged_short_pieces(f.nt), 8 * f.nt);
-    err = paged_short_launch(a, d, dtype, f.nt, at, stream);
+    a.most_rows = f.most;
+    few = pieces_at(paged_short_pieces(f.few), f.few);
+    err = paged_short_launch(a, d, dtype, f.few, at, stream);
   }
   if (err != FTB_OK) return err;
   return dtype == FTB_F16 ? launch_join<__half>(a, d, few, many, stream) : launch_join<__nv_bfloat16>(a, d, few, many, stream);

@@ -7,11 +7,11 @@
 namespace ftb {
 struct PagedAttn;
 
-// Few rows (paged_short.cu); nt: rows of a tile / 8, 1 or 2.
-int paged_short_pieces(int nt);
-int paged_short_launch(const PagedAttn& a, int d, int dtype, int nt, void* scratch, cudaStream_t stream);
+// Few rows (paged_short.cu): tiles of 8 or 16.
+int paged_short_pieces(int rows);
+int paged_short_launch(const PagedAttn& a, int d, int dtype, int rows, void* scratch, cudaStream_t stream);
 
-// Many rows (paged_tile.cu): tiles of 64, 128 or 256.
+// Many rows (paged_tile.cu): tiles of 128 or 256.
 int paged_tile_pieces();
 int paged_tile_launch(const PagedAttn& a, int d, int dtype, int rows, void* scratch, cudaStream_t stream);
 }  // namespace ftb

@@ -65,6 +65,8 @@ struct Merge {
   float m[kWarps][NT * 8], l[kWarps][NT * 8];
 };
 
+// Warps enough for 8 KB each on their way.  (16 rows a warp leave registers for two blocks; more rows for few tokens, as 24 and 48 in
+// tiles of two groups of warps that share the keys through L1, were slower than the tiles of paged_tile.cu by 2 to 4 times.)
 constexpr int blocks_per_sm(int nt) { return nt == 1 ? 3 : 2; }
 
 template <typename T, bool k8, int D, int NT>
@@ -442,7 +444,7 @@ int launch(const PagedAttn& a, void* scratch, cudaStream_t stream) {
   auto kfn = paged_short_kernel<T, k8, D, NT>;
   constexpr int kSmem = sizeof(Merge<D, NT>);
   if (!ensure_dynamic_smem(kfn, kSmem, configured)) return FTB_ERR_LAUNCH;
-  const int pieces = paged_short_pieces(NT);
+  const int pieces = paged_short_pieces(NT * 8);
   float* parts = static_cast<float*>(scratch);
   const cudaError_t err = launch_dependent(kfn, dim3(pieces), dim3(kWarps * 32), kSmem, stream, a, parts,
                                            reinterpret_cast<PagedCut*>(parts + 2 * pieces * part_floats<NT * 8, D>()));
@@ -455,17 +457,17 @@ int launch(const PagedAttn& a, void* scratch, cudaStream_t stream) {
   return a.k_exp != nullptr ? launch<T, true, D, NT>(a, scratch, stream) : launch<T, false, D, NT>(a, scratch, stream);
 }
 template <typename T, int D>
-int launch(const PagedAttn& a, int nt, void* scratch, cudaStream_t stream) {
-  return nt == 1 ? launch<T, D, 1>(a, scratch, stream) : launch<T, D, 2>(a, scratch, stream);
+int launch(const PagedAttn& a, int rows, void* scratch, cudaStream_t stream) {
+  return rows == 8 ? launch<T, D, 1>(a, scratch, stream) : launch<T, D, 2>(a, scratch, stream);
 }
 
 }  // namespace
 
-int paged_short_pieces(int nt) { return current_sm_count() * blocks_per_sm(nt); }
+int paged_short_pieces(int rows) { return current_sm_count() * blocks_per_sm(rows / 8); }
 
-int paged_short_launch(const PagedAttn& a, int d, int dtype, int nt, void* scratch, cudaStream_t stream) {
-  if (dtype == FTB_F16) return d == 128 ? launch<__half, 128>(a, nt, scratch, stream) : launch<__half, 64>(a, nt, scratch, stream);
-  return d == 128 ? launch<__nv_bfloat16, 128>(a, nt, scratch, stream) : launch<__nv_bfloat16, 64>(a, nt, scratch, stream);
+int paged_short_launch(const PagedAttn& a, int d, int dtype, int rows, void* scratch, cudaStream_t stream) {
+  if (dtype == FTB_F16) return d == 128 ? launch<__half, 128>(a, rows, scratch, stream) : launch<__half, 64>(a, rows, scratch, stream);
+  return d == 128 ? launch<__nv_bfloat16, 128>(a, rows, scratch, stream) : launch<__nv_bfloat16, 64>(a, rows, scratch, stream);
 }
 
 }  // namespace ftb

@@ -14,9 +14,7 @@
 //                 translated, one load behind the other: 739 against 4xx us.)
 // A row's chain from scores to weights sits between two products, so that two slots keep the tensor cores busy.  Tiles of 256 rows:
 // 128 to a slot, and a K or V block serves both.  Of 128: the slots take turns at the blocks; each has sums of its own for the same
-// rows, which lie in the same lanes of tensor memory and are put together there.  Of 64: the rows are there twice, in the lower
-// and the upper 64 lanes, the ones for the first 64 keys of a block and the others for the rest (weights of the other half
-// are 0), which halves the chain.
+// rows, which lie in the same lanes of tensor memory and are put together there.
 //
 // 8-bit caches: a block's codes become fp16 numbers code * 2^(e - e_max), e_max the largest exponent of the block's keys: exact
 // where exponents are within 15 of each other, and off by 2^-33 of the block's largest number otherwise.  2^e_max goes to the
@@ -58,7 +56,7 @@ struct Control {
   PagedLineRoom line;
   Stretch ring[kStretches];
   uint64_t ring_full[kStretches], ring_empty[kStretches];
-  uint64_t q_full[2], s_full[2], p_full[2], pv_done[2], o_free[2], begun, fin, fin_rows;
+  uint64_t q_full[2], s_full[2], p_full[2], pv_done[2], o_free[2], begun, fin;
   uint64_t kv_full[kMostSlots], kv_empty[kMostSlots];    // tiles that the products read
   uint64_t raw_full[k8 ? kMostSlots : 1], raw_empty[k8 ? kMostSlots : 1];  // 8-bit blocks
   Edge edges[kStretches];
@@ -72,7 +70,7 @@ struct Control {
 
 template <bool k8, int D, int R>
 struct Plan {
-  static constexpr bool kTwo = R == 256, kDup = R == 64;
+  static constexpr bool kTwo = R == 256;
   static constexpr int kHalf = 128 * 128, kTile = D / 64 * kHalf;
   static constexpr int kQ = (kTwo ? 2 : 1) * kTile;
   static constexpr int kControl = (sizeof(Control<k8, kTwo>) + 15) / 16 * 16, kRoom = 232448 - 1024 - kControl - kQ;
@@ -142,9 +140,8 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
                   float* __restrict__ parts, PagedCut* __restrict__ cuts) {
   using P = Plan<k8, D, R>;
   using C = typename std::conditional<k8, __half, T>::type;
-  constexpr bool kTwo = P::kTwo, kDup = P::kDup;
+  constexpr bool kTwo = P::kTwo;
   constexpr int kSlots = P::kSlots, kRawSlots = P::kRawSlots;
-  constexpr int kMyKeys = kDup ? 64 : 128;  // of a block, that a row's lane has
   extern __shared__ uint8_t smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, piece = blockIdx.x;
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -173,7 +170,6 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
     }
     mbar_init(&ctl.begun, 1);
     mbar_init(&ctl.fin, 8);
-    mbar_init(&ctl.fin_rows, 8);
     for (int i = 0; i < kMostSlots; ++i) {
       mbar_init(&ctl.kv_full[i], k8 ? 4 : 1);
       mbar_init(&ctl.kv_empty[i], 1);
@@ -216,7 +212,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
   tc_fence_after();
   const uint32_t tmem_base = ctl.tmem_base;
   // tensor memory: S0 [0, 128), S1 [128, 256), O0 [256, 256 + D), O1 [384, 384 + D); P_t (16-bit pairs)
-  // over the first half of S_t's columns; where rows are there twice over the first half of each of S_t's halves.
+  // over the first half of S_t's columns.
 
   // Stretch i of this CTA, as every role but the first warp gets it.
   auto await = [&](int i) -> bool {
@@ -348,7 +344,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
       if (leader) {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          umma_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + (k * 16 / kMyKeys) * kMyKeys + (k * 16 % kMyKeys) / 2, dv + k * (2048 >> 4), idesc_pv, (!first || k != 0) ? 1u : 0u);
+          umma_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + k * 8, dv + k * (2048 >> 4), idesc_pv, (!first || k != 0) ? 1u : 0u);
         umma_commit(&ctl.pv_done[t]);
       }
     };
@@ -445,19 +441,18 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
   } else if (warp < 2 + P::kSoftmax) {
     // ------------------------------------------------ softmax: slot t, row r of its 128
     const int t = (warp - 2) / 4, quad = warp & 3, r = quad * 32 + lane;
-    const int part = kDup ? quad >> 1 : 0;  // of a block's keys
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
-    const uint32_t s_addr = lane_addr + t * 128 + part * 64, o_addr = lane_addr + 256 + t * 128;
+    const uint32_t s_addr = lane_addr + t * 128, o_addr = lane_addr + 256 + t * 128;
     constexpr int kCols = kTwo ? D : D / 2;  // of the output, that this thread finishes
     const int c0 = kTwo ? 0 : t * kCols;
-    // parities: bit 0 the next scores, 2 fin, 3 fin_rows, 4 + t the next product P V of slot t in a stretch
+    // parities: bit 0 the next scores, 2 fin, 4 + t the next product P V of slot t in a stretch
     uint32_t par = 0;
     int blocks0 = 0;  // blocks of the stretches so far
     bool ok = true;
     for (int i = 0; ok; ++i) {
       if (!await(i)) break;
       const Stretch& x = ctl.ring[i % kStretches];  // (read again where it is needed, and given back behind the results: registers)
-      const int row0 = kTwo ? t * 128 + quad * 32 : kDup ? (quad & 1) * 32 : quad * 32, row = row0 + lane;  // of the tile
+      const int row0 = (kTwo ? t * 128 : 0) + quad * 32, row = row0 + lane;  // of the tile
       const bool busy = row0 < x.rows;  // this warp has rows
       const bool mine = row < x.rows;
       int tok, head;
@@ -533,9 +528,9 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
             add = static_cast<float>(vr - 127);
             inv = exponent_scale(254 - vr);
           }
-          const int key0 = (x.block0 + j) * kKeys + part * 64;
+          const int key0 = (x.block0 + j) * kKeys;
           const int lo_col = ctl.see_lo[t][r] - key0, hi_col = ctl.see_hi[t][r] - key0;
-          const bool cut = __any_sync(0xffffffffu, mine && (lo_col > 0 || hi_col < kMyKeys - 1));
+          const bool cut = __any_sync(0xffffffffu, mine && (lo_col > 0 || hi_col < kKeys - 1));
           // kChunk scores at a time, read again for the weights.  (A thread that spills goes to L2 for it: shared memory has taken
           // L1's room.  And loops instead of straight code: with several roles on an SM its instruction cache is what runs out.)
           constexpr int kChunk = k8 ? 32 : 64;
@@ -554,7 +549,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
           };
           float mx = -INFINITY;
 #pragma unroll 1
-          for (int n = 0; n < kMyKeys / kChunk; ++n) {
+          for (int n = 0; n < kKeys / kChunk; ++n) {
             scores(n);
             float mx8[8];
 #pragma unroll
@@ -594,7 +589,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
           const float minus = add - top;
           float sum8[8] = {};
 #pragma unroll 1
-          for (int n = 0; n < kMyKeys / kChunk; ++n) {
+          for (int n = 0; n < kKeys / kChunk; ++n) {
             scores(n);
 #pragma unroll
             for (int half = 0; half < kChunk / 32; ++half) {
@@ -609,11 +604,6 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
               }
               tmem_st16(s_addr + n * (kChunk / 2) + half * 16, pk);  // over scores that this thread has read
             }
-          }
-          if constexpr (kDup) {
-            const uint32_t none[16] = {};
-            tmem_st16(lane_addr + t * 128 + (part ^ 1) * 64, none);
-            tmem_st16(lane_addr + t * 128 + (part ^ 1) * 64 + 16, none);
           }
           l = fmaf(((sum8[0] + sum8[1]) + (sum8[2] + sum8[3])) + ((sum8[4] + sum8[5]) + (sum8[6] + sum8[7])), inv, l);
           tmem_st_wait();
@@ -649,8 +639,8 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
       if (!ok) break;
       par ^= static_cast<uint32_t>(m.n & 1) << (4 + t) ^ static_cast<uint32_t>(n_other & 1) << (4 + (t ^ 1));
       tc_fence_after();
-      float all_m = fmaxf(top, other_m);
-      float keep = exp2_fast(top - all_m), take = exp2_fast(other_m - all_m), sum = l * keep + other_l * take;
+      const float all_m = fmaxf(top, other_m), keep = exp2_fast(top - all_m), take = exp2_fast(other_m - all_m);
+      const float sum = l * keep + other_l * take;
       // this thread's columns, 16 at a time
       auto columns = [&](int ch, float (&y)[16]) {
         uint32_t o[16], o2[16];
@@ -661,44 +651,9 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
         for (int e = 0; e < 16; ++e)
           y[e] = (m.n > 0 ? __uint_as_float(o[e]) * keep : 0.f) + (n_other > 0 ? __uint_as_float(o2[e]) * take : 0.f);
       };
-      // Rows that are there twice: the upper lanes give what they have to the lower ones, through the queries' place, which is free
-      // now: [column / 4][row], four columns each.
-      float4* give = reinterpret_cast<float4*>(sQ);
-      float up = 0.f;  // what the upper lanes' columns are multiplied by
-      if (kDup && x.blocks > 0) {
-        auto everyone = [&]() -> bool {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&ctl.fin_rows);
-          const bool fine = mbar_wait_warp(&ctl.fin_rows, par >> 3 & 1u, s_abort, status, FTB_ERR_TIMEOUT_EPI);
-          par ^= 8u;
-          return fine;
-        };
-        if (part == 1 && busy) {
-#pragma unroll 1
-          for (int ch = 0; ch < kCols / 16; ++ch) {
-            float y[16];
-            columns(ch, y);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) give[(c0 / 4 + ch * 4 + e) * 64 + row] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
-          }
-        }
-        // (top and sum of all slots and lanes are there still: nobody writes the next ones before its queries are taken)
-        ok = everyone();
-        if (!ok) break;
-        if (part == 0) {
-          const float m0 = ctl.top[t][r + 64], m1 = ctl.top[t ^ 1][r + 64], mu = fmaxf(m0, m1);
-          const float lu = ctl.sum[t][r + 64] * exp2_fast(m0 - mu) + ctl.sum[t ^ 1][r + 64] * exp2_fast(m1 - mu);
-          const float m_both = fmaxf(all_m, mu), down = exp2_fast(all_m - m_both);
-          up = exp2_fast(mu - m_both);
-          keep *= down;
-          take *= down;
-          sum = sum * down + lu * up;
-          all_m = m_both;
-        }
-      }
       const float scale = x.whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
       bool odd = false;
-      if (busy && part == 0) {
+      if (busy) {
         place();
         T* out = static_cast<T*>(a.o) + (static_cast<long long>(tok) * a.kv_heads * a.group + head) * D + c0;
         float* place_of = parts + static_cast<size_t>(x.place) * part_floats<R, D>();
@@ -706,16 +661,6 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
         for (int ch = 0; ch < kCols / 16; ++ch) {
           float y[16];
           columns(ch, y);
-          if (kDup && x.blocks > 0) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float4 z = give[(c0 / 4 + ch * 4 + e) * 64 + row];
-              y[4 * e] = fmaf(z.x, up, y[4 * e]);
-              y[4 * e + 1] = fmaf(z.y, up, y[4 * e + 1]);
-              y[4 * e + 2] = fmaf(z.z, up, y[4 * e + 2]);
-              y[4 * e + 3] = fmaf(z.w, up, y[4 * e + 3]);
-            }
-          }
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             y[e] *= scale;
@@ -744,12 +689,6 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&ctl.o_free[kTwo ? t : 0]);
-      if (kDup && x.blocks > 0) {  // the upper lanes' numbers have been read: the next queries may take their place
-        if (lane == 0) mbar_arrive(&ctl.fin_rows);
-        ok = mbar_wait_warp(&ctl.fin_rows, par >> 3 & 1u, s_abort, status, FTB_ERR_TIMEOUT_EPI);
-        par ^= 8u;
-        if (!ok) break;
-      }
       const bool last = x.last != 0;
       give_back(i);
       if (last) break;
@@ -912,9 +851,7 @@ int launch(const PagedAttn& a, int dtype, void* scratch, cudaStream_t stream) {
 }
 template <typename T, int D>
 int launch(const PagedAttn& a, int dtype, int rows, void* scratch, cudaStream_t stream) {
-  return rows == 256   ? launch<T, D, 256>(a, dtype, scratch, stream)
-         : rows == 128 ? launch<T, D, 128>(a, dtype, scratch, stream)
-                       : launch<T, D, 64>(a, dtype, scratch, stream);
+  return rows == 256 ? launch<T, D, 256>(a, dtype, scratch, stream) : launch<T, D, 128>(a, dtype, scratch, stream);
 }
 
 }  // namespace

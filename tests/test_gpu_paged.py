@@ -193,6 +193,11 @@ SHAPES = [
     (1, 7, 128, 16, [40, 1, 90, 1], [41, 600, 333, 2], None),
     (1, 2, 128, 32, [300], [3000], None),
     (1, 1, 128, 16, [40], [5000], None),
+    (2, 8, 128, 64, [5, 5, 5], [400, 1333, 5], None),
+    (1, 8, 64, 16, [6, 4, 1], [777, 100, 2000], 400),
+    (2, 10, 128, 32, [3, 2, 3], [600, 64, 1500], None),
+    (1, 6, 64, 128, [4, 5], [3000, 129], None),
+    (1, 45, 128, 16, [1, 1], [900, 17], None),
     (2, 2, 128, 64, [260], [2000], None),
     (1, 8, 64, 32, [30, 31], [4000, 900], None),
     (1, 1, 64, 16, [600, 1, 129], [600, 40, 1000], None),
@@ -321,6 +326,8 @@ def test_page_offsets_beyond_32_bits():
     (8, 4, 128, 64, [1000], [1000], None),
     (8, 2, 128, 16, [900, 1, 400], [1200, 77, 2222], 300),
     (8, 8, 128, 16, [1 + b % 9 for b in range(60)], [10 + 40 * b for b in range(60)], None),
+    (8, 8, 128, 32, [5] * 50, [100 + 60 * b for b in range(50)], None),
+    (8, 5, 64, 16, [6] * 50, [100 + 60 * b for b in range(50)], 700),
     (4, 4, 64, 16, [1 if b % 5 else 90 for b in range(70)], [90 + 20 * b for b in range(70)], None),
 ])
 def test_many_tiles(eight_bit, kv, group, d, page, new, lens, window):
