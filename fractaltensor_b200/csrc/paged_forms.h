@@ -7,6 +7,10 @@
 namespace ftb {
 struct PagedAttn;
 
+// Shared memory of an SM for the kernel for few rows and the joining one: the same for both, since another division waits for the SM
+// to be empty.
+constexpr int kPagedCarveout = 76 * 1024;
+
 // Few rows (paged_short.cu): tiles of 8 or 16.
 int paged_short_pieces(int rows);
 int paged_short_launch(const PagedAttn& a, int d, int dtype, int rows, void* scratch, cudaStream_t stream);

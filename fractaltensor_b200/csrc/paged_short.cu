@@ -444,6 +444,11 @@ int launch(const PagedAttn& a, void* scratch, cudaStream_t stream) {
   auto kfn = paged_short_kernel<T, k8, D, NT>;
   constexpr int kSmem = sizeof(Merge<D, NT>);
   if (!ensure_dynamic_smem(kfn, kSmem, configured)) return FTB_ERR_LAUNCH;
+  // No more shared memory than the blocks need: what is on its way to registers passes L1, which has the rest.  (Left to itself
+  // the division may stay as a kernel in front had it: 378 against 290 us for 96 sequences of 16 rows.)
+  static std::atomic<unsigned long long> divided{0};
+  static_assert(blocks_per_sm(NT) * (kSmem + 2048) <= kPagedCarveout, "the blocks of an SM");
+  if (!set_smem_carveout(kfn, kPagedCarveout, divided)) return FTB_ERR_LAUNCH;
   const int pieces = paged_short_pieces(NT * 8);
   float* parts = static_cast<float*>(scratch);
   const cudaError_t err = launch_dependent(kfn, dim3(pieces), dim3(kWarps * 32), kSmem, stream, a, parts,

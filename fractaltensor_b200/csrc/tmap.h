@@ -62,6 +62,23 @@ inline bool ensure_dynamic_smem(Kernel kfn, int bytes, std::atomic<unsigned long
   return true;
 }
 
+// Asks for `bytes` of an SM's shared memory and L1 as shared memory for kernel `kfn`, the rest as L1; `configured` as above.
+template <typename Kernel>
+inline bool set_smem_carveout(Kernel kfn, int bytes, std::atomic<unsigned long long>& configured) {
+  int dev = 0, most = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return false;
+  const unsigned long long bit = dev < 64 ? (1ull << dev) : 0ull;
+  if (bit != 0 && (configured.load(std::memory_order_acquire) & bit) != 0) return true;
+  if (cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerMultiprocessor, dev) != cudaSuccess || most <= 0) return false;
+  const int percent = (bytes * 100 + most - 1) / most;
+  if (cudaFuncSetAttribute(kfn, cudaFuncAttributePreferredSharedMemoryCarveout, percent < 100 ? percent : 100) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  configured.fetch_or(bit, std::memory_order_release);
+  return true;
+}
+
 // Launches `kfn` so that it may start while the kernel before it in the stream is still draining
 // (programmatic dependent launch): its CTAs are scheduled as SMs free up and run their set-up
 // (barriers, tensor memory, descriptor prefetch) early.  The kernel must execute
