@@ -21,29 +21,29 @@ struct PagedBatch {
   int B, W, pages, page_shift;
 };
 
-// The sequence that row t belongs to, or B; the whole warp asks for the same t.  32 probes a round: one round trip
-// to memory up to 32 sequences, two up to 1024.
-__device__ __forceinline__ int sequence_of_row(const PagedBatch& x, int t, int lane) {
+// Sequence b and position of row t (b = B: none has it; a negative position: in front of the sequence); the whole warp asks for the
+// same t.  32 probes a round, the last one with all that the answer needs: one round trip to memory up to 32 sequences, two up to 1024.
+struct RowPlace {
+  int b;
+  long long pos;
+};
+__device__ __forceinline__ RowPlace place_of_row(const PagedBatch& x, int t, int lane) {
   int lo = 0, hi = x.B;  // the smallest b with starts[b + 1] > t is in [lo, hi], where hi = B stands for none
-  while (lo < hi) {
+  while (hi - lo > 32) {
     const int step = (hi - lo + 31) >> 5;
     const int at = lo + (lane + 1) * step - 1;
     const unsigned above = __ballot_sync(0xffffffffu, at < hi ? x.starts[at + 1] > t : true);
-    const int first = __ffs(above) - 1;
-    if (first < 0) {
-      lo = hi;
-      break;
-    }
-    lo += first * step;
-    if (step == 1) break;
-    hi = min(hi, lo + step - 1);
+    if (above == 0) return {x.B, 0};
+    lo += (__ffs(above) - 1) * step;
+    hi = min(hi, lo + step - 1) + 1;  // (one more, so that it is among the probes)
+    hi = min(hi, x.B);
   }
-  return lo < x.B && x.starts[lo] <= t && x.starts[lo + 1] > t ? lo : x.B;
-}
-
-// Position of row t of sequence b in it; negative: in front of the sequence.
-__device__ __forceinline__ long long position_of_row(const PagedBatch& x, int b, int t) {
-  return static_cast<long long>(x.lens[b]) - x.starts[b + 1] + t;
+  const int at = lo + lane, b = min(at, x.B - 1);
+  const int begin = x.starts[b], end = x.starts[b + 1], len = x.lens[b];
+  const unsigned here = __ballot_sync(0xffffffffu, at < x.B && begin <= t && end > t);
+  if (here == 0) return {x.B, 0};
+  const int first = __ffs(here) - 1;
+  return {lo + first, static_cast<long long>(__shfl_sync(0xffffffffu, len, first)) - __shfl_sync(0xffffffffu, end, first) + t};
 }
 
 // The page that holds position pos of sequence b, or -1 where the table has none (recorded in the status word).

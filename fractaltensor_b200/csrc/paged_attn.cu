@@ -36,9 +36,10 @@ __device__ __forceinline__ void again_rows(const PagedAttn& a, long long warp, l
     while (again != 0) {
       const long long row = r0 + __ffs(again) - 1;
       again &= again - 1;
-      const int t = static_cast<int>(row / heads), b = sequence_of_row(a.batch, t, lane);
-      if (b < a.batch.B)  // (what no sequence has was not written either)
-        attend_row<T, k8, D>(a, b, t, static_cast<int>(row - static_cast<long long>(t) * heads), position_of_row(a.batch, b, t), lane);
+      const int t = static_cast<int>(row / heads);
+      const RowPlace at = place_of_row(a.batch, t, lane);
+      if (at.b < a.batch.B)  // (what no sequence has was not written either)
+        attend_row<T, k8, D>(a, at.b, t, static_cast<int>(row - static_cast<long long>(t) * heads), at.pos, lane);
     }
   }
 }

@@ -1,7 +1,8 @@
 // Keys and values of new tokens into a paged cache, and back out of it.
 //
-// A warp takes one token: its kv_heads rows of keys and of values, 16 bytes a lane, eight pieces in flight.  The
-// rows do not wait for their place: a token's sequence, position and page are found while they are on their way.
+// A warp takes one token: its kv_heads rows of keys and of values, 16 bytes of a 16-bit row a lane, several pieces in flight; into
+// 8-bit rows 16 numbers a lane (whole sectors to write), out of them 8 (whole sectors again).  Rows that are written do not
+// wait for their place: a token's sequence, position and page are found while they are on their way.
 // 8-bit caches: a row's largest magnitude is found among the lanes that hold it, on the bit patterns; its exponent
 // is the smallest e with max <= 448 * 2^(e - 127), taken from the bits of max as fp32: 448 = 1.75 * 2^8.
 // Bound by memory: kv_heads * d * 2 * (2 + size in the cache) bytes a token.
@@ -14,7 +15,7 @@
 namespace ftb {
 namespace {
 
-constexpr int kThreads = 128, kPieces = 8;
+constexpr int kThreads = 128;
 
 struct Rows {
   const void* k;
@@ -40,6 +41,7 @@ __device__ __forceinline__ int row_exponent(uint32_t largest_bits) {
   return max(1, E - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0));
 }
 
+// Eight numbers as codes.
 template <typename T>
 __device__ __forceinline__ uint2 to_codes(const uint4& x, int e) {
   if (e == 255) return make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
@@ -56,58 +58,64 @@ __device__ __forceinline__ uint2 to_codes(const uint4& x, int e) {
   return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
 }
 
+// A lane's piece of a row.
+template <int kNumbers_, int D>
+struct Pieces {
+  static constexpr int kNumbers = kNumbers_, kOfRow = D / kNumbers, kAtOnce = 64 / kNumbers;
+};
+
 template <typename T, bool k8, int D>
 __global__ void __launch_bounds__(kThreads)
 paged_write_kernel(Rows in, Cache cache, PagedBatch batch, int T_rows, int kv_heads, int* __restrict__ status) {
-  constexpr int kRowPieces = D / 8, kShift = D == 128 ? 4 : 3;
+  using P = Pieces<k8 ? 16 : 8, D>;
   const int lane = threadIdx.x & 31;
   const int t = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   grid_launch_dependents();
   grid_dependency_wait();
   if (t >= T_rows) return;
-  const int half = kv_heads * kRowPieces, pieces = 2 * half;  // keys, then values
+  const int half = kv_heads * P::kOfRow, pieces = 2 * half;  // keys, then values
   long long row0 = -1;  // the row of head 0 in the cache
-  for (int p0 = 0; p0 < pieces; p0 += 32 * kPieces) {
-    uint4 x[kPieces];
+  for (int p0 = 0; p0 < pieces; p0 += 32 * P::kAtOnce) {
+    uint4 x[P::kAtOnce][k8 ? 2 : 1];
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
+    for (int i = 0; i < P::kAtOnce; ++i) {
       const int p = p0 + i * 32 + lane;
-      x[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (p < pieces) {
-        const bool is_v = p >= half;
-        const int q = is_v ? p - half : p, head = q >> kShift, c = q & (kRowPieces - 1);
-        const T* src = is_v ? static_cast<const T*>(in.v) + t * in.v_row + head * in.v_head
-                            : static_cast<const T*>(in.k) + t * in.k_row + head * in.k_head;
-        x[i] = __ldcs(reinterpret_cast<const uint4*>(src) + c);
+      const bool is_v = p >= half;
+      const int q = is_v ? p - half : p, head = q / P::kOfRow, c = q % P::kOfRow;
+      const T* src = is_v ? static_cast<const T*>(in.v) + t * in.v_row + head * in.v_head
+                          : static_cast<const T*>(in.k) + t * in.k_row + head * in.k_head;
+#pragma unroll
+      for (int k = 0; k < (k8 ? 2 : 1); ++k) {
+        x[i][k] = make_uint4(0u, 0u, 0u, 0u);
+        if (p < pieces) x[i][k] = __ldcs(reinterpret_cast<const uint4*>(src + c * P::kNumbers) + k);
       }
     }
     if (p0 == 0) {
-      const int b = sequence_of_row(batch, t, lane);
-      if (b >= batch.B) return;
-      const long long pos = position_of_row(batch, b, t);
-      if (pos < 0) return;
-      const int page = page_of(batch, b, pos, status);
+      const RowPlace at = place_of_row(batch, t, lane);
+      if (at.b >= batch.B || at.pos < 0) return;
+      const int page = page_of(batch, at.b, at.pos, status);
       if (page < 0) return;
-      row0 = ((static_cast<long long>(page) * kv_heads) << batch.page_shift) + (pos & ((1 << batch.page_shift) - 1));
+      row0 = ((static_cast<long long>(page) * kv_heads) << batch.page_shift) + (at.pos & ((1 << batch.page_shift) - 1));
     }
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
+    for (int i = 0; i < P::kAtOnce; ++i) {
       const int p = p0 + i * 32 + lane;
       const bool is_v = p >= half;
-      const int q = is_v ? p - half : p, head = q >> kShift, c = q & (kRowPieces - 1);
+      const int q = is_v ? p - half : p, head = q / P::kOfRow, c = q % P::kOfRow;
       const long long row = row0 + (static_cast<long long>(head) << batch.page_shift);
       unsigned char* dst = is_v ? cache.v : cache.k;
       if constexpr (k8) {
-        uint32_t m = largest(x[i]);
+        uint32_t m = max(largest(x[i][0]), largest(x[i][1]));
 #pragma unroll
-        for (int o = kRowPieces / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        for (int o = P::kOfRow / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
         const int e = row_exponent<T>(m);
         if (p < pieces) {
-          *reinterpret_cast<uint2*>(dst + row * D + c * 8) = to_codes<T>(x[i], e);
+          const uint2 lower = to_codes<T>(x[i][0], e), upper = to_codes<T>(x[i][1], e);
+          *reinterpret_cast<uint4*>(dst + row * D + c * 16) = make_uint4(lower.x, lower.y, upper.x, upper.y);
           if (c == 0) (is_v ? cache.v_exp : cache.k_exp)[row] = static_cast<unsigned char>(e);
         }
       } else if (p < pieces) {
-        *reinterpret_cast<uint4*>(dst + row * (2 * D) + c * 16) = x[i];
+        *reinterpret_cast<uint4*>(dst + row * (2 * D) + c * 16) = x[i][0];
       }
     }
   }
@@ -115,12 +123,12 @@ paged_write_kernel(Rows in, Cache cache, PagedBatch batch, int T_rows, int kv_he
 
 // Piece `at` of the output: eight numbers.
 template <typename T>
-__device__ __forceinline__ void put8(T* out, long long at, const float (&f)[8]) {
+__device__ __forceinline__ void put8(T* out, long long at, const float* f) {
   __stcs(reinterpret_cast<uint4*>(out) + at, make_uint4(Fmt<T>::pack2(f[0], f[1]), Fmt<T>::pack2(f[2], f[3]),
                                                         Fmt<T>::pack2(f[4], f[5]), Fmt<T>::pack2(f[6], f[7])));
 }
 template <>
-__device__ __forceinline__ void put8<float>(float* out, long long at, const float (&f)[8]) {
+__device__ __forceinline__ void put8<float>(float* out, long long at, const float* f) {
   __stcs(reinterpret_cast<float4*>(out) + 2 * at, make_float4(f[0], f[1], f[2], f[3]));
   __stcs(reinterpret_cast<float4*>(out) + 2 * at + 1, make_float4(f[4], f[5], f[6], f[7]));
 }
@@ -129,55 +137,57 @@ template <typename T, bool k8, int D>
 __global__ void __launch_bounds__(kThreads)
 paged_read_kernel(Cache cache, PagedBatch batch, T* __restrict__ k_out, T* __restrict__ v_out, int T_rows, int kv_heads,
                   int* __restrict__ status) {
-  constexpr int kRowPieces = D / 8, kShift = D == 128 ? 4 : 3;
+  using P = Pieces<8, D>;
   const int lane = threadIdx.x & 31;
   const int t = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   grid_launch_dependents();
   grid_dependency_wait();
   if (t >= T_rows) return;
-  const int b = sequence_of_row(batch, t, lane);
-  if (b >= batch.B) return;
-  const long long pos = position_of_row(batch, b, t);
-  const int page = pos >= 0 ? page_of(batch, b, pos, status) : -1;
-  const long long row0 = ((static_cast<long long>(page) * kv_heads) << batch.page_shift) + (pos & ((1 << batch.page_shift) - 1));
-  const int half = kv_heads * kRowPieces, pieces = 2 * half;
-  for (int p0 = 0; p0 < pieces; p0 += 32 * kPieces) {
+  const RowPlace at = place_of_row(batch, t, lane);
+  if (at.b >= batch.B) return;
+  const int page = at.pos >= 0 ? page_of(batch, at.b, at.pos, status) : -1;
+  const long long row0 = ((static_cast<long long>(page) * kv_heads) << batch.page_shift) + (at.pos & ((1 << batch.page_shift) - 1));
+  const int half = kv_heads * P::kOfRow, pieces = 2 * half;
+  for (int p0 = 0; p0 < pieces; p0 += 32 * P::kAtOnce) {
     using Piece = typename std::conditional<k8, uint2, uint4>::type;
-    Piece x[kPieces];
-    int e[kPieces];
+    Piece x[P::kAtOnce];
+    int e[P::kAtOnce];
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
+    for (int i = 0; i < P::kAtOnce; ++i) {
       const int p = p0 + i * 32 + lane;
       x[i] = Piece{};
       e[i] = 0;
       if (p < pieces && page >= 0) {
         const bool is_v = p >= half;
-        const int q = is_v ? p - half : p, head = q >> kShift, c = q & (kRowPieces - 1);
+        const int q = is_v ? p - half : p, head = q / P::kOfRow, c = q % P::kOfRow;
         const long long row = row0 + (static_cast<long long>(head) << batch.page_shift);
         x[i] = __ldcs(reinterpret_cast<const Piece*>((is_v ? cache.v : cache.k) + row * (k8 ? D : 2 * D)) + c);
         if constexpr (k8) e[i] = (is_v ? cache.v_exp : cache.k_exp)[row];
       }
     }
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
+    for (int i = 0; i < P::kAtOnce; ++i) {
       const int p = p0 + i * 32 + lane;
       if (p < pieces) {
         const bool is_v = p >= half;
-        const long long at = static_cast<long long>(t) * half + (is_v ? p - half : p);
+        const long long to = static_cast<long long>(t) * half + (is_v ? p - half : p);
         T* out = is_v ? v_out : k_out;
         if constexpr (k8) {
           const float scale = exponent_scale(e[i]);
-          const uint32_t w[4] = {x[i].x & 0xffffu, x[i].x >> 16, x[i].y & 0xffffu, x[i].y >> 16};
           float f[8];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 h = unpack2<__half>(e4m3x2_to_f16x2(w[j]));
-            f[2 * j] = h.x * scale;
-            f[2 * j + 1] = h.y * scale;
+          for (int j = 0; j < 2; ++j) {
+            uint32_t lower, upper;
+            e4m3x4_to_f16x2(j == 0 ? x[i].x : x[i].y, lower, upper);
+            const float2 l = unpack2<__half>(lower), u = unpack2<__half>(upper);
+            f[4 * j] = l.x * scale;
+            f[4 * j + 1] = l.y * scale;
+            f[4 * j + 2] = u.x * scale;
+            f[4 * j + 3] = u.y * scale;
           }
-          put8(out, at, f);
+          put8(out, to, f);
         } else {
-          __stcs(reinterpret_cast<uint4*>(out) + at, x[i]);
+          __stcs(reinterpret_cast<uint4*>(out) + to, x[i]);
         }
       }
     }

@@ -9,9 +9,9 @@
 //   warps 2..9    softmax: two slots of 128 threads, a thread a row; they also fetch the queries and write the results
 //   16-bit caches: one more warp zeroes values in front of and behind the keys that the tile sees (what lies there may be
 //                 anything, and 0 * NaN is NaN), told by warp 0 which blocks need it
-//   8-bit caches: eight more warps turn codes into fp16 tiles, four of them one tile, the other four the next.  (They could load
-//                 codes themselves, which would spare shared memory two passes; measured, they then wait for addresses to be
-//                 translated, one load behind the other: 739 against 4xx us.)
+//   8-bit caches: four more warps turn codes into fp16 tiles, or, with 128 rows, eight, four of them one tile and the other four
+//                 the next.  (They could load codes themselves, which would spare shared memory two passes; measured, they then
+//                 wait for addresses to be translated, one load behind the other: 739 against 650 us for the drafts of 96 sequences.)
 // A row's chain from scores to weights sits between two products, so that two slots keep the tensor cores busy.  Tiles of 256 rows:
 // 128 to a slot, and a K or V block serves both.  Of 128: the slots take turns at the blocks; each has sums of its own for the same
 // rows, which lie in the same lanes of tensor memory and are put together there.
@@ -79,7 +79,9 @@ struct Plan {
   static constexpr int kRaw = 128 * D + 256, kRawRoom = (kRoom - kSlots * kTile) / kRaw;
   static constexpr int kRawSlots = k8 ? (kRawRoom < kMostSlots ? kRawRoom : kMostSlots) : 0;
   static constexpr int kSmem = 1024 + kControl + kQ + kSlots * kTile + kRawSlots * kRaw;
-  static constexpr int kSoftmax = 8, kConvert = 8;  // warps
+  // Warps: a block of 256 rows keeps the softmax busy longer than four warps need for its tiles, and with fewer warps each has more
+  // registers.
+  static constexpr int kSoftmax = 8, kConvert = kTwo ? 4 : 8;
   static constexpr int kThreads = 32 * (2 + kSoftmax + (k8 ? kConvert : 1));
   static_assert(kSlots >= 3 && (!k8 || kRawSlots >= 3) && kSmem <= 232448, "shared memory budget");
 };
@@ -533,7 +535,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
           const bool cut = __any_sync(0xffffffffu, mine && (lo_col > 0 || hi_col < kKeys - 1));
           // kChunk scores at a time, read again for the weights.  (A thread that spills goes to L2 for it: shared memory has taken
           // L1's room.  And loops instead of straight code: with several roles on an SM its instruction cache is what runs out.)
-          constexpr int kChunk = k8 ? 32 : 64;
+          constexpr int kChunk = k8 && !kTwo ? 32 : 64;
           uint32_t s[kChunk];
           auto scores = [&](int n) {
 #pragma unroll
@@ -714,9 +716,10 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
     }
   } else {
     // ------------------------------------------------------------- codes to fp16
-    // Two groups of four warps take the tiles in turn; warp cw of a group converts keys 32 cw .. + 31.  Each warp finds the block's
+    // Groups of four warps take the tiles in turn; warp cw of a group converts keys 32 cw .. + 31.  Each warp finds the block's
     // largest exponents on its own: lane i holds the four bytes of keys 4 i .. + 3.
     const int cw = warp & 3, group = (warp - 2 - P::kSoftmax) >> 2;
+    constexpr int kGroups = P::kConvert / 4;
     int count = 0, blocks0 = 0;  // tiles and blocks of the stretches so far
     bool ok = true;
     // a lane: piece c of keys first, first + 32 / kRow, ..
@@ -738,7 +741,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
       if (!await(i)) break;
       const Stretch& x = ctl.ring[i % kStretches];
       const int tiles = 2 * x.blocks;
-      for (int n = (group - count) & 1; n < tiles && ok; n += 2) {
+      for (int n = (group - count) & (kGroups - 1); n < tiles && ok; n += kGroups) {
         const StreamTile y = stream_tile<kTwo>(n, x.blocks);
         const int slot = (count + n) % kSlots, raw = (count + n) % kRawSlots;
         const int key0 = (x.block0 + y.j) * kKeys;
