@@ -270,9 +270,8 @@ Form form_of(int T, int B, int group) {
   if (rows <= 16) return {rows <= 8 ? 8 : 16, INT_MAX, 0};
   const int many = rows > 128ll * B ? 256 : 128;
   if (B == 1) return {0, 0, many};
-  // One tile of paged_short.cu: a second one would read the keys again.  16 rows of it take 1.4 to 1.9 times what 8 take, and
-  // about what a tile of 128 does (96 sequences of 4500 keys of 16 bits, 8 kv heads: 8 rows 268 us, 16 378, 128 392; of 8500 of
-  // 8 bits: 310, 509, 657).
+  // One tile of paged_short.cu: a second one would read the keys again.  96 sequences, 8 kv heads, 4500 keys of 16 bits: 8 rows
+  // 270 us, 16 rows 296, as rows of paged_tile.cu 24 336, 64 360, 128 398; 8500 keys of 8 bits: 311, 433, then 660, 640, 656.
   const int few = group <= 8 && rows > 16ll * B ? 8 : 16;
   return {few, few, many};
 }
@@ -304,6 +303,7 @@ extern "C" int ftb_paged_attn_fwd(const void* q, long long q_row, long long q_he
   if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) return FTB_ERR_ARG;
   if ((d != 64 && d != 128) || (dtype != FTB_F16 && dtype != FTB_BF16)) return FTB_ERR_ARG;
   if (!(scale > 0.f) || !(scale <= FLT_MAX)) return FTB_ERR_ARG;  // hidden scores are -inf behind the scale
+  if (T > 0 && q == o) return FTB_ERR_ARG;  // queries are read again by other blocks than those that write their rows
   if (static_cast<long long>(kv_heads) * group > 65536 || static_cast<long long>(T) * group > INT_MAX) return FTB_ERR_ARG;
   if (((q_row | q_head) & 7) != 0) return FTB_ERR_ALIGN;
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(k_cache) |

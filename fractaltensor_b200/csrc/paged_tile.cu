@@ -18,8 +18,9 @@
 //
 // 8-bit caches: a block's codes become fp16 numbers code * 2^(e - e_max), e_max the largest exponent of the block's keys: exact
 // where exponents are within 15 of each other, and off by 2^-33 of the block's largest number otherwise.  2^e_max goes to the
-// scores (keys) and into the weights (values, as in paged_short.cu), once a block.  bf16 queries are scaled into fp16's range, row by
-// row, by a power of two.
+// scores (keys) and into the weights (values, as in paged_short.cu), once a block.  Where exponents of a block lie further apart and a
+// row does not see all of its keys, the largest may be of one that is hidden from it: that row is made a NaN, and gone through key by
+// key as those are.  bf16 queries are scaled into fp16's range, row by row, by a power of two.
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -33,7 +34,7 @@
 namespace ftb {
 namespace {
 
-constexpr int kKeys = 128, kAtLeast = 1, kStretches = 4, kRefs = 8;
+constexpr int kKeys = 128, kAtLeast = 1, kStretches = 4, kRefs = 8, kFar = 256;
 constexpr int kMostSlots = 14;
 constexpr float kAbove = 8.f;  // as in flash_attn.cu: the maximum in use may lie 2^8 below the real one
 
@@ -63,7 +64,7 @@ struct Control {
   uint64_t edge_full[kStretches], edge_empty[kStretches], v_fixed[kMostSlots];
   float top[2][128], sum[2][128];  // [slot][row]
   int see_lo[2][128], see_hi[2][128];
-  int k_ref[kRefs], v_ref[kRefs];
+  int k_ref[kRefs], v_ref[kRefs];  // e_max of a block; + kFar: exponents more than 15 apart, in one that not every row sees all of
   uint32_t tmem_base;
   int abort, dead;
 };
@@ -523,16 +524,22 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
         par ^= 1u;
         tc_fence_after();
         if (busy) {
+          const int key0 = (x.block0 + j) * kKeys;
+          const int lo_col = ctl.see_lo[t][r] - key0, hi_col = ctl.see_hi[t][r] - key0;
+          const bool cut = __any_sync(0xffffffffu, mine && (lo_col > 0 || hi_col < kKeys - 1));
           float f = factor, add = 0.f, inv = 1.f;
           if constexpr (k8) {
-            const int kr = ctl.k_ref[(blocks0 + j) & (kRefs - 1)], vr = ctl.v_ref[(blocks0 + j) & (kRefs - 1)];
+            int kr = ctl.k_ref[(blocks0 + j) & (kRefs - 1)], vr = ctl.v_ref[(blocks0 + j) & (kRefs - 1)];
+            if ((kr | vr) & kFar) {
+              kr &= kFar - 1;
+              vr &= kFar - 1;
+              if (lo_col > max(0, x.keys.lo - key0) || hi_col < min(kKeys, x.keys.hi - key0) - 1) factor = __uint_as_float(0x7fffffffu);
+              f = factor;
+            }
             f *= exponent_scale(kr);
             add = static_cast<float>(vr - 127);
             inv = exponent_scale(254 - vr);
           }
-          const int key0 = (x.block0 + j) * kKeys;
-          const int lo_col = ctl.see_lo[t][r] - key0, hi_col = ctl.see_hi[t][r] - key0;
-          const bool cut = __any_sync(0xffffffffu, mine && (lo_col > 0 || hi_col < kKeys - 1));
           // kChunk scores at a time, read again for the weights.  (A thread that spills goes to L2 for it: shared memory has taken
           // L1's room.  And loops instead of straight code: with several roles on an SM its instruction cache is what runs out.)
           constexpr int kChunk = k8 && !kTwo ? 32 : 64;
@@ -741,6 +748,9 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
       if (!await(i)) break;
       const Stretch& x = ctl.ring[i % kStretches];
       const int tiles = 2 * x.blocks;
+      // keys that every row sees: up to the first one's position, from the last one's window on
+      const long long all_hi = x.pos0 + x.first + x.flat0 / a.group;
+      const long long all_lo = a.window > 0 ? x.pos0 + x.first + (x.flat0 + x.rows - 1) / a.group - a.window + 1 : 0;
       for (int n = (group - count) & (kGroups - 1); n < tiles && ok; n += kGroups) {
         const StreamTile y = stream_tile<kTwo>(n, x.blocks);
         const int slot = (count + n) % kSlots, raw = (count + n) % kRawSlots;
@@ -771,11 +781,23 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
         const uint32_t mine = y.is_v ? vw : kw;
         const int top = __reduce_max_sync(0xffffffffu, largest(mine));
         if (!y.is_v) {
-          const int v_top = __reduce_max_sync(0xffffffffu, largest(vw));
-          if (cw == 0 && lane == 0) {
+          if (cw == 0) {
             const int ref = (blocks0 + y.j) & (kRefs - 1);
-            ctl.k_ref[ref] = top;
-            ctl.v_ref[ref] = v_top;
+            int v_top = __reduce_max_sync(0xffffffffu, largest(vw)), far = 0;
+            if (key0 + kKeys - 1 > all_hi || key0 < all_lo) {
+              auto smallest = [](uint32_t w) -> uint32_t {  // (of those above 1: rows of zeros lose nothing)
+                w |= __vcmpleu4(w, 0x01010101u);
+                w = __vminu4(w, w >> 16 | w << 16);
+                return min(w & 0xffu, w >> 8 & 0xffu);
+              };
+              if (top - static_cast<int>(__reduce_min_sync(0xffffffffu, smallest(kw))) > 15 ||
+                  v_top - static_cast<int>(__reduce_min_sync(0xffffffffu, smallest(vw))) > 15)
+                far = kFar;
+            }
+            if (lane == 0) {
+              ctl.k_ref[ref] = top | far;
+              ctl.v_ref[ref] = v_top;
+            }
           }
         }
         const int e = __shfl_sync(0xffffffffu, mine, cw * 8 + (lane >> 2)) >> (8 * (lane & 3)) & 0xff;  // of key cw * 32 + lane

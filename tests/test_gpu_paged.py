@@ -297,6 +297,38 @@ def test_what_is_not_seen_has_no_part(worst, eight_bit, new, n, at, window):
             assert not bool(torch.isfinite(o[sees.cuda()][:, group:].float()).all(-1).any())
 
 
+@pytest.mark.parametrize("steps", [14, 17, 60, -60])
+@pytest.mark.parametrize("eight_bit", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new,n,begin,end,window", [(3, 40, 38, 40, None), (20, 333, 320, 333, None), (200, 333, 250, 333, None), (300, 300, 100, 101, None),
+                                                    (20, 700, 500, 560, 130), (200, 700, 400, 520, 150), (129, 2000, 1990, 1995, None)])
+def test_the_size_of_what_is_not_seen_has_no_part(steps, eight_bit, d, new, n, begin, end, window):
+    """Keys and values 2^steps times as large at positions begin .. end - 1: tokens that see none of them have what they had."""
+    ops = _ops()
+    kv, group, page = 2, 4, 16
+    table, ln, st, pages = _batch([new], [n], page)
+    cache = _full_cache(pages, kv, page, d, E4M3 if eight_bit else BF16, 3, table, ln)
+    j = torch.arange(begin, end)
+    at = table[0][j // page].long().cuda(), slice(None), (j % page).cuda()
+    for i in range(2):
+        if eight_bit:
+            cache[2 + i][at] = (cache[2 + i][at].int() + steps).clamp(1, 254).byte()
+        else:
+            cache[i][at] = cache[i][at] * 2.0 ** steps
+    q = _numbers((new, kv * group, d), BF16, 1).cuda()
+    o = ops.paged_attention(q, cache, table.cuda(), ln.cuda(), st.cuda(), scale=0.1, window=window)
+    ops.check_status()
+    pos = torch.arange(n - new, n)
+    sees = pos >= begin
+    if window:
+        sees &= pos - window < end - 1
+    assert bool(sees.any()) and not bool(sees.all())
+    want, bound = paged.attention(q, cache, table, ln, st, 0.1, window)
+    tol = paged.tolerance(want, bound, BF16, d, eight_bit, n)
+    err = ((o.double().cpu() - want).abs() / tol)[~sees]
+    assert bool((err <= 1).all()), float(err.nan_to_num(9e9).max())
+
+
 def test_page_offsets_beyond_32_bits():
     ops = _ops()
     kv, d, page = 8, 128, 128
@@ -571,7 +603,7 @@ def test_refusals():
         (lambda: att(q=torch.zeros(1, 64, 4, dtype=BF16, device="cuda").transpose(1, 2)), ValueError),
         (lambda: att(q=torch.zeros(257, dtype=BF16, device="cuda")[1:].view(1, 4, 64)), ValueError),
         (lambda: att(window=0), ValueError), (lambda: att(scale=0.0), RuntimeError), (lambda: att(scale=float("inf")), RuntimeError),
-        (lambda: att(scale=float("nan")), RuntimeError), (lambda: att(out=q[:, :2]), ValueError), (lambda: att(out=q.half()), TypeError),
+        (lambda: att(scale=float("nan")), RuntimeError), (lambda: att(out=q[:, :2]), ValueError), (lambda: att(out=q.half()), TypeError), (lambda: att(out=q), RuntimeError),
         (lambda: att(cache=cache[:1]), TypeError), (lambda: att(cache=(cache[0], cache[1][:3])), ValueError),
         (lambda: att(cache=(cache[0].float(), cache[1].float())), TypeError), (lambda: att(cache=(cache[0].view(torch.uint8).view(E4M3),) * 2), ValueError),
         (lambda: att(cache=tuple(c.transpose(1, 2) for c in cache)), ValueError), (lambda: att(cache=tuple(c[:, :, :8].contiguous() for c in cache)), ValueError),
