@@ -303,7 +303,6 @@ extern "C" int ftb_paged_attn_fwd(const void* q, long long q_row, long long q_he
   if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) return FTB_ERR_ARG;
   if ((d != 64 && d != 128) || (dtype != FTB_F16 && dtype != FTB_BF16)) return FTB_ERR_ARG;
   if (!(scale > 0.f) || !(scale <= FLT_MAX)) return FTB_ERR_ARG;  // hidden scores are -inf behind the scale
-  if (T > 0 && q == o) return FTB_ERR_ARG;  // queries are read again by other blocks than those that write their rows
   if (static_cast<long long>(kv_heads) * group > 65536 || static_cast<long long>(T) * group > INT_MAX) return FTB_ERR_ARG;
   if (((q_row | q_head) & 7) != 0) return FTB_ERR_ALIGN;
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(k_cache) |
@@ -311,6 +310,7 @@ extern "C" int ftb_paged_attn_fwd(const void* q, long long q_row, long long q_he
     return FTB_ERR_ALIGN;
   if (workspace == nullptr || workspace_bytes < ftb_workspace_bytes()) return FTB_ERR_WORKSPACE;
   if (T == 0) return FTB_OK;
+  if (q == o) return FTB_ERR_ARG;  // queries are read again by other blocks than those that write their rows
   const int rc = check_device_sm100();
   if (rc) return rc;
   PagedAttn a;

@@ -10,6 +10,9 @@
     python -m fractaltensor_b200.run_case sparse_attn --B 2 --heads 16 --S 4096 --dtype fp32
     python -m fractaltensor_b200.run_case project --M 2240 --H 512 --V 10000
     python -m fractaltensor_b200.run_case rnn_attn --L 50 --N 64 --H 512
+    python -m fractaltensor_b200.run_case paged --B 64 --S 4096 --heads 32 --kv-heads 8                # a token for each sequence
+    python -m fractaltensor_b200.run_case paged --B 16 --S 8192 --new 8 --cache e4m3                   # drafts
+    python -m fractaltensor_b200.run_case verify --B 64 --new 4 --V 50000
 
 A small, fixed workload to put under a profiler or to time by hand; prints the
 average time per call measured with CUDA events.
@@ -26,7 +29,7 @@ DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("case", choices=["lstm", "varlen", "dilated", "grid", "b2b", "attn", "softmax", "sparse_attn", "project", "rnn_attn"])
+    ap.add_argument("case", choices=["lstm", "varlen", "dilated", "grid", "b2b", "attn", "softmax", "sparse_attn", "project", "rnn_attn", "paged", "verify"])
     ap.add_argument("--D", type=int, default=16)
     ap.add_argument("--L", type=int, default=20)
     ap.add_argument("--N", type=int, default=256)
@@ -53,6 +56,10 @@ def main():
     ap.add_argument("--V", type=int, default=10000, help="project: vocabulary, over M rows of H")
     ap.add_argument("--head-dim", type=int, default=64, help="sparse_attn: elements per head")
     ap.add_argument("--as-shipped", action="store_true", help="sparse_attn: the softmax dimension of the shipped example")
+    ap.add_argument("--new", type=int, default=1, help="paged: new tokens of each of B sequences of S keys; verify: drafts")
+    ap.add_argument("--kv-heads", type=int, default=8, help="paged: kv heads that the heads share")
+    ap.add_argument("--page-size", type=int, default=64, help="paged: keys of a page")
+    ap.add_argument("--cache", default="16", choices=["16", "e4m3"], help="paged: 16-bit pages, or codes with an exponent a row")
     ap.add_argument("--graph", action="store_true",
                     help="capture one call in a CUDA graph and time replays (schedules with one launch per level)")
     a = ap.parse_args()
@@ -132,6 +139,28 @@ def main():
         biases, projections = [uni(bound, a.H) for _ in range(2)], [uni(1.0, a.H).to(dt) for _ in range(2)]
         lens = (torch.arange(a.N, device=dev, dtype=torch.int32) % a.L) + 1
         fn = lambda: ops.rnn_attention(src, trg, *weights, *biases, *projections, lens)
+    elif a.case == "paged":
+        # the new tokens are written to the cache and attend to it; page numbers in random order
+        per = -(-a.S // a.page_size)
+        kv, d = a.kv_heads, 128
+        cache = ops.paged_cache(a.B * per, kv, a.page_size, d, dt if a.cache == "16" else torch.float8_e4m3fn, dev)
+        table = torch.randperm(a.B * per, device=dev, generator=g).int().view(a.B, per)
+        lens = torch.full((a.B,), a.S, dtype=torch.int32, device=dev)
+        whole = torch.arange(a.B + 1, device=dev, dtype=torch.int32)
+        for b in range(a.B):  # (a sequence at a time: all of them at once would take the cache's room again)
+            ops.paged_cache_write(cache, rnd(a.S, kv, d).to(dt), rnd(a.S, kv, d).to(dt), table[b:b + 1], lens[:1], whole[:2] * a.S)
+        starts, T = whole * a.new, a.B * a.new
+        qkv = rnd(T, (a.heads + 2 * kv) * d).to(dt)
+        q, k, v = (x.unflatten(1, (-1, d)) for x in qkv.split([a.heads * d, kv * d, kv * d], 1))
+
+        def fn():
+            ops.paged_cache_write(cache, k, v, table, lens, starts)
+            return ops.paged_attention(q, cache, table, lens, starts, scale=1 / math.sqrt(d), window=a.window)
+    elif a.case == "verify":
+        p, q = (torch.softmax(2 * rnd(a.B, a.new + i, a.V), -1) for i in (1, 0))
+        drafts = torch.multinomial(q.view(-1, a.V), 1, generator=g).view(a.B, a.new)
+        u = torch.rand(a.B, a.new + 1, device=dev, generator=g)
+        fn = lambda: ops.verify_drafts(p, drafts, u, q)
     elif a.form:
         left, right = a.local if a.local is not None else (a.window - 1 if a.window is not None else -1, 0)
         q, k, v = (rnd(a.B, a.heads, a.S, 128).to(dt) for _ in range(3))

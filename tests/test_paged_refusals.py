@@ -62,6 +62,7 @@ def test_alignment_and_workspace(lib):
     odd = ctypes.c_void_p(24)
     for kw in (dict(q=odd), dict(k=odd), dict(v=odd), dict(o=odd), dict(q_row=4), dict(q_head=63)):
         assert _attn(lib, **kw) == 2, kw
+    assert _attn(lib, o=P) == 1  # over the queries
     for kw in (dict(k=odd), dict(vc=odd), dict(kr=4), dict(vh=1)):
         assert _write(lib, **kw) == 2, kw
     for kw in (dict(k=odd), dict(vc=odd)):
