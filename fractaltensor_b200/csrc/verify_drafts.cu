@@ -12,6 +12,8 @@
 // behind the other: the drafts' probabilities, the row, the stretch).  A cluster of CTAs takes a sequence, every warp a stretch of the row: one pass for the
 // stretches' sums, which the CTAs hand each other through distributed shared memory, and a second look at the one stretch (a 64th of
 // the row or less) in which the limit is passed.  Every CTA finds n on its own, which saves a step of waiting.
+#include <climits>
+
 #include "../../include/ftb200.h"
 #include "ptx.cuh"
 #include "tmap.h"
@@ -55,7 +57,7 @@ verify_drafts_kernel(Drafts a, long long* __restrict__ tokens, int* __restrict__
   constexpr int kWarps = kThreads / 32;
   __shared__ double sums[kWarps], totals[2];  // of the warps; of this CTA (in the two tries)
   __shared__ double s_total[C];
-  __shared__ int s_n;
+  __shared__ int s_n, s_found, s_heavy;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = blockIdx.x / C, rank = C > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   if (threadIdx.x == 0) s_n = a.K;
@@ -63,13 +65,15 @@ verify_drafts_kernel(Drafts a, long long* __restrict__ tokens, int* __restrict__
   grid_dependency_wait();
   grid_launch_dependents();
   const int K = a.K, V = a.V;
-  const int mine = a.counts != nullptr ? min(max(a.counts[b], 0), K) : K;
   const long long* x = a.drafts + static_cast<long long>(b) * K;
   const float* u = a.u + static_cast<long long>(b) * (K + 1);
   const float* p = a.p + b * a.p_seq;
   const float* q = a.q != nullptr ? a.q + b * a.q_seq : nullptr;
+  const double share = u[K];
+  long long id = threadIdx.x < K ? x[threadIdx.x] : 0;  // (on its way beside the count)
+  const int mine = a.counts != nullptr ? min(max(a.counts[b], 0), K) : K;
   for (int i = threadIdx.x; i < mine; i += kThreads) {
-    const long long id = x[i];
+    if (i >= kThreads) id = x[i];
     bool taken = false;
     if (id >= 0 && id < V) {
       const double qx = q != nullptr ? static_cast<double>(q[i * a.q_row + id]) : 1.0;
@@ -79,7 +83,6 @@ verify_drafts_kernel(Drafts a, long long* __restrict__ tokens, int* __restrict__
     }
     if (!taken) atomicMin(&s_n, i);
   }
-  const double share = u[K];
   __syncthreads();
   const int n = min(s_n, mine);
   const float* pr = p + n * a.p_row;
@@ -160,48 +163,66 @@ verify_drafts_kernel(Drafts a, long long* __restrict__ tokens, int* __restrict__
   }
   const bool heaviest = !passed || first < 0;  // (sums that round differently: the last one too)
   if (heaviest) first = last;
-  const bool here = own && total > 0.0;  // of all CTAs, one
-  if (here && warp == first) {
-    // kUnroll numbers side by side a lane: one scan over the lanes for 32 * kUnroll of them
-    int found = -1, heavy = -1;
+  // That stretch again, by all warps of the CTA, kUnroll numbers side by side a lane: one scan over the warps' sums for
+  // kThreads * kUnroll of them.
+  if (own && total > 0.0) {  // of all CTAs, one
+    const int begin_at = static_cast<int>(min(static_cast<long long>(V), static_cast<long long>(rank * kWarps + first) * stretch)), end_at = min(V, begin_at + stretch);
+    int found = INT_MAX, heavy = -1;
     double run = in_front;
-    for (int j0 = from; j0 < to && found < 0; j0 += 32 * kUnroll) {
-      const int j = j0 + lane * kUnroll;
-      double w[kUnroll], s = 0.0;
+    for (int j0 = begin_at; j0 < end_at && found == INT_MAX; j0 += kThreads * kUnroll) {
+      const int j = j0 + static_cast<int>(threadIdx.x) * kUnroll;
+      double w[kUnroll], sum = 0.0;
       float pv[kUnroll], qv[kUnroll];
 #pragma unroll
       for (int k = 0; k < kUnroll; ++k) {
-        pv[k] = j + k < to ? pr[j + k] : 0.f;
-        qv[k] = qr != nullptr && j + k < to ? qr[j + k] : 0.f;
+        pv[k] = j + k < end_at ? pr[j + k] : 0.f;
+        qv[k] = qr != nullptr && j + k < end_at ? qr[j + k] : 0.f;
       }
 #pragma unroll
       for (int k = 0; k < kUnroll; ++k) {
         w[k] = weight_of(pv[k], qv[k], j + k, without);
-        s += w[k];
+        sum += w[k];
       }
-      double ends = s;  // sum of the lanes up to this one
+      double ends = sum;  // sum of the warp's lanes up to this one
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const double y = __shfl_up_sync(0xffffffffu, ends, o);
         if (lane >= o) ends += y;
       }
       const double begins = __shfl_up_sync(0xffffffffu, ends, 1);
+      __syncthreads();  // (sums, s_found and s_heavy have been read)
+      if (lane == 31) sums[warp] = ends;
+      if (threadIdx.x == 0) {
+        s_found = INT_MAX;
+        s_heavy = -1;
+      }
+      __syncthreads();
       double upto = run + (lane > 0 ? begins : 0.0);
-      int here_found = -1, here_heavy = -1;
+#pragma unroll
+      for (int v = 0; v < kWarps; ++v) {
+        if (v < warp) upto += sums[v];
+        run += sums[v];
+      }
+      int here_found = INT_MAX, here_heavy = -1;
 #pragma unroll
       for (int k = 0; k < kUnroll; ++k) {
         upto += w[k];
         if (w[k] > 0.0) {
-          if (here_found < 0 && !heaviest && upto > limit) here_found = j + k;
+          if (here_found == INT_MAX && !heaviest && upto > limit) here_found = j + k;
           here_heavy = j + k;
         }
       }
-      const unsigned above = __ballot_sync(0xffffffffu, here_found >= 0), some = __ballot_sync(0xffffffffu, here_heavy >= 0);
-      if (above != 0) found = __shfl_sync(0xffffffffu, here_found, __ffs(above) - 1);
-      if (some != 0) heavy = __shfl_sync(0xffffffffu, here_heavy, 31 - __clz(some));
-      run += __shfl_sync(0xffffffffu, ends, 31);
+      here_found = __reduce_min_sync(0xffffffffu, here_found);
+      here_heavy = __reduce_max_sync(0xffffffffu, here_heavy);
+      if (lane == 0) {
+        if (here_found != INT_MAX) atomicMin(&s_found, here_found);
+        if (here_heavy >= 0) atomicMax(&s_heavy, here_heavy);
+      }
+      __syncthreads();
+      found = s_found;
+      if (s_heavy >= 0) heavy = s_heavy;
     }
-    if (lane == 0) tokens[static_cast<long long>(b) * (K + 1) + n] = found >= 0 ? found : heavy;
+    if (threadIdx.x == 0) tokens[static_cast<long long>(b) * (K + 1) + n] = found != INT_MAX ? found : heavy;
   }
   if (rank == 0) {
     for (int i = threadIdx.x; i <= K; i += kThreads)
@@ -239,7 +260,7 @@ using namespace ftb;
 extern "C" int ftb_verify_drafts(const float* probs, long long p_seq, long long p_row, const float* draft_probs, long long q_seq,
                                  long long q_row, const long long* drafts, const float* u, const int* counts, long long* tokens,
                                  int* counts_out, int B, int K, int V, void* workspace, size_t workspace_bytes, void* stream) {
-  if (B < 0 || K < 0 || V <= 0) return FTB_ERR_ARG;
+  if (B < 0 || K < 0 || V <= 0 || V > 1 << 30) return FTB_ERR_ARG;
   if (B > 0 && (!probs || (!drafts && K > 0) || !u || !tokens || !counts_out)) return FTB_ERR_ARG;
   if (workspace == nullptr || workspace_bytes < ftb_workspace_bytes()) return FTB_ERR_WORKSPACE;
   if (B == 0) return FTB_OK;

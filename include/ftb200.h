@@ -443,7 +443,7 @@ int ftb_paged_attn_fwd(const void* q, long long q_row, long long q_head, const v
                        size_t workspace_bytes, void* stream);
 
 /* Drafted tokens against the target's probabilities, from random numbers that the caller gives.  probs: fp32, for each of B
- * sequences K + 1 rows of V probabilities (`p_seq` and `p_row` numbers apart; ftb_project_softmax_fwd gives such rows);
+ * sequences K + 1 rows of V (up to 2^30) probabilities (`p_seq` and `p_row` numbers apart; ftb_project_softmax_fwd gives such rows);
  * draft_probs: fp32, K rows that the drafts were drawn from, or NULL: each draft was certain; drafts: int64 [B, K]; u: fp32
  * [B, K + 1] in [0, 1); counts: int32 [B], drafts of each sequence (cut to 0 .. K), or NULL: K.
  * Draft i is taken if u_i * q_i(x_i) < p_i(x_i); the first that is not ends the run at n (n = counts[b] if all are taken).  tokens
