@@ -87,14 +87,6 @@ __device__ __forceinline__ void umma_ts_pair_rows(uint32_t d_tmem, uint32_t a_tm
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(off0), "r"(off1), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ uint64_t fma_to_f32x2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ void unpair_f32x2(uint64_t v, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
 // Whether the phase is over, without waiting.
 __device__ __forceinline__ bool mbar_test(const uint64_t* bar, uint32_t parity) {
   uint32_t ok;

@@ -2,9 +2,11 @@
 // of a group) against blocks of 128 keys on the tensor cores (tcgen05), S = Q K^T and O += P V with accumulators in tensor
 // memory, online softmax between them.
 //
-// 2048 tokens behind 14 336 keys, 32 heads of 128 over 8 kv heads, bf16: 565 us, 0.91 PFLOP/s; bound by the chain of a row's scores, 4300
+// 2048 tokens behind 14 336 keys, 32 heads of 128 over 8 kv heads, bf16: 558 us, 0.92 PFLOP/s; bound by the chain of a row's scores, 4300
 // cycles a block of 256 rows beside 2048 of products, and by the joins (35 us).  96 sequences of 8500 keys on average in 8 bits, 5 tokens
-// of 64 heads: 650 us, 0.2 PFLOP/s and 2.5 TB/s; bound by the instructions that make 8-bit keys operands (1.6 to 1.9 a cycle and SM).
+// of 64 heads: 645 us, 0.2 PFLOP/s and 2.5 TB/s; bound by the instructions that make 8-bit keys operands (1.6 to 1.9 a cycle and SM).
+// Measured and not kept, the chunk: all 128 scores of a row in registers 616 us (spills; L1 is shared memory's), 32 scores loaded ahead of
+// 32 in work 580, a warp for each slot's products 617, the slots' exponentials in turns 575, the second product in two halves 568 (of 566).
 //
 // One persistent CTA per SM walks its piece of the line of work (paged_work.cuh):
 //   warp 0        the walk, announced to the others through a ring of stretches, and the loads of K and V, page by page: TMA boxes
@@ -600,7 +602,8 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
             }
           }
           const float minus = add - top;
-          float sum8[8] = {};
+          const uint64_t f2 = dup_f32x2(f), minus2 = dup_f32x2(minus);
+          uint64_t sum4[4] = {0, 0, 0, 0};
 #pragma unroll 1
           for (int n = 0; n < kKeys / kChunk; ++n) {
             scores(n);
@@ -609,16 +612,23 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
               uint32_t pk[16];
 #pragma unroll
               for (int c = 0; c < 16; ++c) {
-                const float p0 = exp2_fast(fmaf(__uint_as_float(s[32 * half + 2 * c]), f, minus));
-                const float p1 = exp2_fast(fmaf(__uint_as_float(s[32 * half + 2 * c + 1]), f, minus));
-                sum8[(2 * c) & 7] += p0;
-                sum8[(2 * c + 1) & 7] += p1;
+                const int at = 32 * half + 2 * c;
+                float p0, p1;
+                unpair_f32x2(fma_to_f32x2(pair_f32x2(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), f2, minus2), p0, p1);
+                p0 = exp2_fast(p0);
+                p1 = exp2_fast(p1);
+                add_f32x2(sum4[c & 3], pair_f32x2(p0, p1));
                 pk[c] = Fmt<C>::pack2(p0, p1);
               }
               tmem_st16(s_addr + n * (kChunk / 2) + half * 16, pk);  // over scores that this thread has read
             }
           }
-          l = fmaf(((sum8[0] + sum8[1]) + (sum8[2] + sum8[3])) + ((sum8[4] + sum8[5]) + (sum8[6] + sum8[7])), inv, l);
+          add_f32x2(sum4[0], sum4[1]);
+          add_f32x2(sum4[2], sum4[3]);
+          add_f32x2(sum4[0], sum4[2]);
+          float l0, l1;
+          unpair_f32x2(sum4[0], l0, l1);
+          l = fmaf(l0 + l1, inv, l);
           tmem_st_wait();
         }
         tc_fence_before();

@@ -160,6 +160,14 @@ __device__ __forceinline__ void fma_f32x2(uint64_t& acc, uint64_t a, uint64_t b)
 __device__ __forceinline__ void add_f32x2(uint64_t& acc, uint64_t a) {
   asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc) : "l"(a));
 }
+__device__ __forceinline__ uint64_t fma_to_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ void unpair_f32x2(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
 
 // ------------------------------------------------- global -> shared without a register on the way
 // 16 bytes through L2; zeros when !valid (src is not read then, but has to be an address of the array).

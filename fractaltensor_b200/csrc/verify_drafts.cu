@@ -8,7 +8,7 @@
 // Only one row of p (and of q) a sequence is read whole.  Sums are kept in 64 bits: the chosen index follows from a
 // comparison with a partial sum of up to V numbers, and in 32 bits the order of summation would decide it.
 //
-// Bound by the bytes of those rows: 100 sequences of 5 drafts over 130 001 words 35.9 us, 2.9 TB/s (one: 7.3 us, trips to memory one
+// Bound by the bytes of those rows: 100 sequences of 5 drafts over 130 001 words 29.5 us, 3.5 TB/s (one: 7.3 us, trips to memory one
 // behind the other: the drafts' probabilities, the row, the stretch).  A cluster of CTAs takes a sequence, every warp a stretch of the row: one pass for the
 // stretches' sums, which the CTAs hand each other through distributed shared memory, and a second look at the one stretch (a 64th of
 // the row or less) in which the limit is passed.  Every CTA finds n on its own, which saves a step of waiting.
