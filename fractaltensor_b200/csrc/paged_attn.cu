@@ -306,7 +306,7 @@ extern "C" int ftb_paged_attn_fwd(const void* q, long long q_row, long long q_he
   if (static_cast<long long>(kv_heads) * group > 65536 || static_cast<long long>(T) * group > INT_MAX) return FTB_ERR_ARG;
   if (((q_row | q_head) & 7) != 0) return FTB_ERR_ALIGN;
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(k_cache) |
-        reinterpret_cast<uintptr_t>(v_cache)) & 15) != 0)
+        reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(k_exp) | reinterpret_cast<uintptr_t>(v_exp)) & 15) != 0)
     return FTB_ERR_ALIGN;
   if (workspace == nullptr || workspace_bytes < ftb_workspace_bytes()) return FTB_ERR_WORKSPACE;
   if (T == 0) return FTB_OK;

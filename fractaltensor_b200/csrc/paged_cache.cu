@@ -207,7 +207,8 @@ int check_sizes(const Sizes& n, const void* k, const void* v, const void* k_exp,
   if (n.T < 0 || n.B <= 0 || n.W <= 0 || n.pages <= 0 || n.kv_heads <= 0 || n.kv_heads > 65536) return FTB_ERR_ARG;
   if (n.page_size != 16 && n.page_size != 32 && n.page_size != 64 && n.page_size != 128) return FTB_ERR_ARG;
   if (n.d != 64 && n.d != 128) return FTB_ERR_ARG;
-  if (((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) != 0) return FTB_ERR_ALIGN;
+  if (((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(k_exp) | reinterpret_cast<uintptr_t>(v_exp)) & 15) != 0)
+    return FTB_ERR_ALIGN;
   return FTB_OK;
 }
 PagedBatch batch_of(const Sizes& n, const int* table, const int* lens, const int* starts) {

@@ -407,7 +407,7 @@ int ftb_gemm_nt(const void* A, const void* Bt, void* out, int M, int N, int K, i
  * Cache: pages [pages, kv_heads, page_size, d] for keys and the same for values; page_size 16, 32, 64 or 128, d 64 or 128.
  * 16-bit pages hold the model's type.  8-bit pages (k_exp and v_exp not NULL) hold e4m3 codes, with an exponent byte e for each
  * row of d numbers, [pages, kv_heads, page_size]: a number is code * 2^(e - 127), and e the smallest from 1 on with
- * max |row| <= 448 * 2^(e - 127).  A row with a number that is not finite is stored as NaN (e = 255).
+ * max |row| <= 448 * 2^(e - 127).  All of them begin on 16-byte boundaries.  A row with a number that is not finite is stored as NaN (e = 255).
  *
  * Batch: int32 arrays on the device: starts [B + 1], non-decreasing, the first row of each sequence's new tokens among the
  * T rows; lens [B], the keys of each sequence, the new ones included; table [B, W], its pages in order.  Token i of the n new ones of

@@ -63,6 +63,8 @@ def test_alignment_and_workspace(lib):
     for kw in (dict(q=odd), dict(k=odd), dict(v=odd), dict(o=odd), dict(q_row=4), dict(q_head=63)):
         assert _attn(lib, **kw) == 2, kw
     assert _attn(lib, o=P) == 1  # over the queries
+    for call in (_attn, _write, _read):  # exponents are fetched 16 at a time
+        assert call(lib, ke=odd, ve=P) == call(lib, ke=P, ve=ctypes.c_void_p(17)) == 2
     for kw in (dict(k=odd), dict(vc=odd), dict(kr=4), dict(vh=1)):
         assert _write(lib, **kw) == 2, kw
     for kw in (dict(k=odd), dict(vc=odd)):
