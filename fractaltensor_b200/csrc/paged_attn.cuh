@@ -19,6 +19,11 @@ struct PagedAttn {
   uint32_t* odd;                   // [T, heads]: not 0 where a row of the output has to be computed again, key by key
 };
 
+// 8 bits: values of 2^-30 to 2^30 times a code are ordinary, and maxima of scores with and without the values' exponents that are up to 2^40
+// apart: weights, which end at 2^-126, then reach down to 2^-48 of the largest, and the terms of the sum that divides up to 2^38.
+constexpr float kNear = 30.f;
+constexpr float kNearTops = 40.f;
+
 // Whether a row at position pos of a tile that multiplies keys lo .. hi - 1 has some of them with weight 0 that it does not see: what
 // they hold could have made its result a NaN.
 __device__ __forceinline__ bool hides(const PagedAttn& a, long long pos, int lo, int hi) {

@@ -24,7 +24,8 @@
 //
 // 8-bit caches: a block's codes become fp16 numbers code * 2^(e - e_max), e_max the largest exponent of the block's keys: exact
 // where exponents are within 15 of each other, and off by 2^-33 of the block's largest number otherwise.  2^e_max goes to the
-// scores (keys) and into the weights (values, as in paged_short.cu), once a block.  Where exponents of a block lie further apart and a
+// scores (keys) and into the weights (values, as in paged_short.cu, with
+// a sum apart for blocks whose exponents are not ordinary), once a block.  Where exponents of a block lie further apart and a
 // row does not see all of its keys, the largest may be of one that is hidden from it: that row is made a NaN, and gone through key by
 // key as those are.  bf16 queries are scaled into fp16's range, row by row, by a power of two.
 #include <algorithm>
@@ -69,6 +70,8 @@ struct Control {
   Edge edges[kStretches];
   uint64_t edge_full[kStretches], edge_empty[kStretches], v_fixed[kMostSlots];
   float top[2][128], sum[2][128];  // [slot][row]
+  // 8 bits: what `sum` refers to, and a thread's own: the sum of blocks apart and what it refers to (in registers: 646 for 628 us of drafts)
+  float sum_top[k8 ? 2 : 1][k8 ? 128 : 1], apart_l[k8 ? 2 : 1][k8 ? 128 : 1], apart_n[k8 ? 2 : 1][k8 ? 128 : 1];
   int see_lo[2][128], see_hi[2][128];
   int k_ref[kRefs], v_ref[kRefs];  // e_max of a block; + kFar: exponents more than 15 apart, in one that not every row sees all of
   uint32_t tmem_base;
@@ -522,7 +525,11 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
 
       // ---- blocks
       const Mine m = blocks_of_slot<kTwo>(a, x, t);
-      float top = 0.f, l = 0.f;
+      float top = 0.f, l = 0.f, near = kNear;  // 8 bits: l takes a block's weights where its values' largest exponent is below
+      if constexpr (k8) {
+        ctl.apart_l[t][r] = 0.f;
+        ctl.apart_n[t][r] = -FLT_MAX;
+      }
       for (int k = 0; k < m.n && ok; ++k) {
         const int j = kTwo ? m.j0 + k : 2 * k + t;
         ok = mbar_wait_warp(&ctl.s_full[t], par & 1u, s_abort, status, FTB_ERR_TIMEOUT_MMA);
@@ -577,6 +584,25 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
           }
           // (a row may see nothing of a block: the lowest finite number keeps its weights 0)
           const float m_new = fmaxf(fmaf(mx, f, add), -FLT_MAX);
+          const bool apart = k8 && fabsf(add) > near;  // (the same in all lanes)
+          if constexpr (k8) {
+            if (apart) {
+              const bool both = near > 0.f && k > 0;  // l holds something, and top is near the scores
+              const float n = ctl.apart_n[t][r];
+              float to = fmaxf(n, m_new - add);
+              if (both) to = fmaxf(to, top);
+              float more = ctl.apart_l[t][r] * exp2_fast(n - to) + (both ? l * exp2_fast(top - to) : 0.f);
+#pragma unroll 1
+              for (int n = 0; n < kKeys / kChunk; ++n) {
+                scores(n);
+#pragma unroll
+                for (int e = 0; e < kChunk; ++e) more += exp2_fast(fmaf(__uint_as_float(s[e]), f, -to));
+              }
+              ctl.apart_l[t][r] = more;
+              ctl.apart_n[t][r] = to;
+              l = inv = 0.f;
+            }
+          }
           if (k == 0) {
             top = m_new;
           } else {
@@ -600,6 +626,9 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
               }
               tmem_st_wait();
             }
+          }
+          if constexpr (k8) {
+            if (apart) near = __any_sync(0xffffffffu, fabsf(top - ctl.apart_n[t][r]) > kNearTops) ? -1.f : kNear;
           }
           const float minus = add - top;
           const uint64_t f2 = dup_f32x2(f), minus2 = dup_f32x2(minus);
@@ -641,13 +670,20 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
       if (!ok) break;
       blocks0 += x.blocks;
       if (m.n == 0) top = -FLT_MAX;
+      float l_top = top;  // what l refers to
+      if constexpr (k8) {
+        const float n = ctl.apart_n[t][r];
+        l_top = near > 0.f ? fmaxf(n, top) : n;
+        l = (near > 0.f ? l * exp2_fast(top - l_top) : 0.f) + ctl.apart_l[t][r] * exp2_fast(n - l_top);
+      }
 
       // ---- results: of both slots, where they share the rows
-      float other_m = -FLT_MAX, other_l = 0.f;
+      float other_m = -FLT_MAX, other_l = 0.f, other_top = -FLT_MAX;
       int n_other = 0;
       if (!kTwo && x.blocks > 0) {
         ctl.top[t][r] = top;
         ctl.sum[t][r] = l;
+        if constexpr (k8) ctl.sum_top[t][r] = l_top;
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl.fin);
         ok = mbar_wait_warp(&ctl.fin, par >> 2 & 1u, s_abort, status, FTB_ERR_TIMEOUT_EPI);
@@ -656,6 +692,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
         n_other = blocks_of_slot<kTwo>(a, x, t ^ 1).n;
         other_m = ctl.top[t ^ 1][r];
         other_l = ctl.sum[t ^ 1][r];
+        if constexpr (k8) other_top = ctl.sum_top[t ^ 1][r];
       }
       if (m.n > 0) ok = mbar_wait_warp(&ctl.pv_done[t], ((par >> (4 + t)) + m.n - 1) & 1u, s_abort, status, FTB_ERR_TIMEOUT_MMA);
       if (ok && n_other > 0) ok = mbar_wait_warp(&ctl.pv_done[t ^ 1], ((par >> (4 + (t ^ 1))) + n_other - 1) & 1u, s_abort, status, FTB_ERR_TIMEOUT_MMA);
@@ -663,7 +700,8 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
       par ^= static_cast<uint32_t>(m.n & 1) << (4 + t) ^ static_cast<uint32_t>(n_other & 1) << (4 + (t ^ 1));
       tc_fence_after();
       const float all_m = fmaxf(top, other_m), keep = exp2_fast(top - all_m), take = exp2_fast(other_m - all_m);
-      const float sum = l * keep + other_l * take;
+      const float all_top = k8 ? fmaxf(l_top, other_top) : all_m;
+      const float sum = k8 ? l * exp2_fast(l_top - all_top) + other_l * exp2_fast(other_top - all_top) : l * keep + other_l * take;
       // this thread's columns, 16 at a time
       auto columns = [&](int ch, float (&y)[16]) {
         uint32_t o[16], o2[16];
@@ -674,7 +712,11 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
         for (int e = 0; e < 16; ++e)
           y[e] = (m.n > 0 ? __uint_as_float(o[e]) * keep : 0.f) + (n_other > 0 ? __uint_as_float(o2[e]) * take : 0.f);
       };
-      const float scale = x.whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
+      float scale = x.whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f, scale2 = 1.f;
+      if constexpr (k8) {  // to what the sum refers to (in two steps: it may be 2^135, where the numbers are small)
+        scale2 = exp2_fast(0.5f * (all_m - all_top));
+        scale *= scale2;
+      }
       bool odd = false;
       if (busy) {
         place();
@@ -687,6 +729,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             y[e] *= scale;
+            if constexpr (k8) y[e] *= scale2;
             odd |= y[e] != y[e];
           }
           if (mine) {
@@ -707,7 +750,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
           using Flag = typename std::conditional<kCols == D, uint32_t, uint16_t>::type;
           reinterpret_cast<Flag*>(a.odd + static_cast<long long>(tok) * a.kv_heads * a.group + head)[c0 / kCols] = again ? 1 : 0;
         }
-        if (mine && !x.whole && c0 == 0) *reinterpret_cast<float2*>(place_of + R * D + 2 * row) = make_float2(all_m, sum);
+        if (mine && !x.whole && c0 == 0) *reinterpret_cast<float2*>(place_of + R * D + 2 * row) = make_float2(all_top, sum);
       }
       tc_fence_before();
       __syncwarp();
