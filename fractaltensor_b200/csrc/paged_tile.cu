@@ -547,9 +547,11 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
               kr &= kFar - 1;
               vr &= kFar - 1;
               if (lo_col > max(0, x.keys.lo - key0) || hi_col < min(kKeys, x.keys.hi - key0) - 1) factor = __uint_as_float(0x7fffffffu);
-              f = factor;
             }
-            f *= exponent_scale(kr);
+            // (hidden scores are -inf already: times 0, as of a row of zeros and small keys, they would be NaN, as a score of 0 times
+            // infinity.  No score moves: they are below 2^17 here.)
+            f = fminf(fmaxf(factor * exponent_scale(kr), FLT_MIN), FLT_MAX);
+            if (factor != factor) f = factor;
             add = static_cast<float>(vr - 127);
             inv = exponent_scale(254 - vr);
           }

@@ -188,3 +188,20 @@ def test_many_whole_tiles_with_values_of_zero(zero):
     o = _ops().paged_attention(q, cache, table, ln, st, scale=0.3)
     _ops().check_status()
     _check(o, q, cache, table, lens, new, 0.3)
+
+
+@pytest.mark.parametrize("keys", ["all", "first 128", "every second", "behind 200", None])
+@pytest.mark.parametrize("kv,group,d,page,new,lens,window", SHAPES)
+def test_queries_of_zero(kv, group, d, page, new, lens, window, keys):
+    """Rows of queries that are zeros, or the smallest numbers, over keys of zeros and others: the mean of the values."""
+    table, ln, st, pages = _batch(new, lens, page)
+    cache = _cache(pages, kv, page, d, 3)
+    _change(cache, 0, table, lens, lambda n: torch.arange(n) >= 0, -20)
+    if keys:
+        _change(cache, 0, table, lens, ROWS[keys], None)
+    q = _numbers((sum(new), kv * group, d), 1)
+    q[::2] = 0.0
+    q[1::4] *= 2.0 ** -120
+    o = _ops().paged_attention(q, cache, table, ln, st, scale=0.3, window=window)
+    _ops().check_status()
+    _check(o, q, cache, table, lens, new, 0.3, window)
