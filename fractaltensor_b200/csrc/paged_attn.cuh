@@ -42,13 +42,13 @@ __device__ __noinline__ void attend_row(const PagedAttn& a, int b, int t, int he
 #pragma unroll
   for (int c = 0; c < kPer / 2; ++c) {
     const float2 f = unpack2<T>(src[c]);
-    q[2 * c] = f.x * a.scale_log2;
-    q[2 * c + 1] = f.y * a.scale_log2;
+    q[2 * c] = f.x;
+    q[2 * c + 1] = f.y;
   }
-  // this lane's numbers of a row of the cache
-  auto numbers = [&](const unsigned char* cache, const unsigned char* exps, long long row, float (&f)[kPer]) {
+  // this lane's numbers of a row of the cache; 8 bits: times 2^by
+  auto numbers = [&](const unsigned char* cache, int by, long long row, float (&f)[kPer]) {
     if constexpr (k8) {
-      const float e = exponent_scale(exps[row]);
+      const float e = exponent_scale(127 + by);
 #pragma unroll
       for (int c = 0; c < kPer / 2; ++c) {
         const float2 g = unpack2<__half>(e4m3x2_to_f16x2(reinterpret_cast<const unsigned short*>(cache + row * D)[lane * (kPer / 2) + c]));
@@ -70,14 +70,18 @@ __device__ __noinline__ void attend_row(const PagedAttn& a, int b, int t, int he
   for (long long j0 = begin / kBatch * kBatch; j0 < end; j0 += kBatch) {
     const int page = max(0, page_of(a.batch, b, j0, a.status));
     const long long row0 = ((static_cast<long long>(page) * a.kv_heads + h) << a.batch.page_shift) + (j0 & ((1 << a.batch.page_shift) - 1));
-    float s[kBatch], v[kBatch][kPer];
+    float s[kBatch], s_by[kBatch], v[kBatch][kPer];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       s[i] = -INFINITY;
+      s_by[i] = 1.f;
       if (j0 + i >= begin && j0 + i < end) {
         float k[kPer];
-        numbers(a.k, a.k_exp, row0 + i, k);
-        numbers(a.v, a.v_exp, row0 + i, v[i]);
+        // (half of a key's scale before the product with the query and the rest behind it: either alone may lead out of fp32's range)
+        const int ke = k8 ? a.k_exp[row0 + i] - 127 : 0, half = ke >> 1;
+        s_by[i] = exponent_scale(127 + ke - half);
+        numbers(a.k, half, row0 + i, k);
+        numbers(a.v, k8 ? a.v_exp[row0 + i] - 127 : 0, row0 + i, v[i]);
         s[i] = 0.f;
 #pragma unroll
         for (int c = 0; c < kPer; ++c) s[i] = fmaf(q[c], k[c], s[i]);
@@ -88,6 +92,7 @@ __device__ __noinline__ void attend_row(const PagedAttn& a, int b, int t, int he
     for (int i = 0; i < kBatch; ++i) {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
+      s[i] = s[i] * s_by[i] * a.scale_log2;  // (behind the product: a query's number times it may be too small to keep all its bits)
       m_new = fmaxf(m_new, s[i]);
     }
     const float keep = exp2_fast(m - m_new);

@@ -281,16 +281,10 @@ paged_short_kernel(const __grid_constant__ PagedAttn a, float* __restrict__ part
               mma16816<C>(sc[nt], w0[2 * i], w1[2 * i], w0[2 * i + 1], w1[2 * i + 1], q[nt][2 * j + i][0], q[nt][2 * j + i][1]);
         }
       }
-      float inv0 = 1.f, inv1 = 1.f, add0 = 0.f, add1 = 0.f;
+      float inv0 = 1.f, inv1 = 1.f, add0 = 0.f, add1 = 0.f, s0 = 1.f, s1 = 1.f;
       if constexpr (k8) {
-        const float s0 = exponent_scale(ke[0]), s1 = exponent_scale(ke[1]);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          sc[nt][0] *= s0;
-          sc[nt][1] *= s0;
-          sc[nt][2] *= s1;
-          sc[nt][3] *= s1;
-        }
+        s0 = exponent_scale(ke[0]);
+        s1 = exponent_scale(ke[1]);
         add0 = static_cast<float>(ve[0] - 127);
         add1 = static_cast<float>(ve[1] - 127);
         inv0 = exponent_scale(max(0, 254 - ve[0]));
@@ -300,7 +294,11 @@ paged_short_kernel(const __grid_constant__ PagedAttn a, float* __restrict__ part
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[nt][i] = fmaf(sc[nt][i], factor[nt][i & 1], i < 2 ? add0 : add1);
+        for (int i = 0; i < 4; ++i) {
+          // (the scales of query and key meet before the score: either alone may lead out of fp32's range.  A score of 0 stays one.)
+          const float f = k8 ? fminf(factor[nt][i & 1] * (i < 2 ? s0 : s1), FLT_MAX) : factor[nt][i & 1];
+          sc[nt][i] = fmaf(sc[nt][i], f, i < 2 ? add0 : add1);
+        }
       const bool edge = key0 + 15 > all_hi || key0 < all_lo;
       if (edge) {
 #pragma unroll

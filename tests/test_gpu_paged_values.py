@@ -205,3 +205,28 @@ def test_queries_of_zero(kv, group, d, page, new, lens, window, keys):
     o = _ops().paged_attention(q, cache, table, ln, st, scale=0.3, window=window)
     _ops().check_status()
     _check(o, q, cache, table, lens, new, 0.3, window)
+
+
+@pytest.mark.parametrize("hidden", [False, True])
+@pytest.mark.parametrize("steps", [-118, -90, 90, 118, 126])
+@pytest.mark.parametrize("kv,group,d,page,new,lens,window", SHAPES)
+def test_sizes_of_queries_and_keys_that_cancel(kv, group, d, page, new, lens, window, steps, hidden):
+    """Keys 2^steps times as large, queries 2^-steps times: ordinary scores.  hidden: a value of the last position is NaN, which rows that
+    do not see it are computed key by key for."""
+    table, ln, st, pages = _batch(new, lens, page)
+    cache = _cache(pages, kv, page, d, 3)
+    _change(cache, 0, table, lens, lambda n: torch.arange(n) >= 0, steps)
+    q = (_numbers((sum(new), kv * group, d), 1).float() * 2.0 ** -steps).to(BF16)
+    bad = tuple(c.clone() for c in cache)
+    if hidden:
+        for b, n in enumerate(lens):
+            at = int(table[b, (n - 1) // page]), slice(None), (n - 1) % page
+            bad[1].view(torch.uint8)[at] = 0x7F
+            bad[3][at] = 255
+    o = _ops().paged_attention(q, bad, table, ln, st, scale=0.3, window=window)
+    _ops().check_status()
+    if hidden:  # the last token of each sequence sees it
+        last = st[1:].long() - 1
+        assert bool(torch.isnan(o[last].float()).all())
+        o[last] = _exact(q, cache, table, lens, new, 0.3, window)[0].to(BF16).cuda()[last]
+    _check(o, q, cache, table, lens, new, 0.3, window)
