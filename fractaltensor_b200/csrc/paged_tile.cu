@@ -22,12 +22,12 @@
 // 128 to a slot, and a K or V block serves both.  Of 128: the slots take turns at the blocks; each has sums of its own for the same
 // rows, which lie in the same lanes of tensor memory and are put together there.
 //
-// 8-bit caches: a block's codes become fp16 numbers code * 2^(e - e_max), e_max the largest exponent of the block's keys: exact
-// where exponents are within 15 of each other, and off by 2^-33 of the block's largest number otherwise.  2^e_max goes to the
-// scores (keys) and into the weights (values, as in paged_short.cu, with
-// a sum apart for blocks whose exponents are not ordinary), once a block.  Where exponents of a block lie further apart and a
-// row does not see all of its keys, the largest may be of one that is hidden from it: that row is made a NaN, and gone through key by
-// key as those are.  bf16 queries are scaled into fp16's range, row by row, by a power of two.
+// 8-bit caches: a block's codes become fp16 numbers code * 2^(7 + e - e_max), e_max the largest exponent of the block's keys (448 * 2^7 is
+// below fp16's end): exact where exponents are within 22 of each other, off by 2^-39 of the block's largest number where within 31,
+// and by 2^-31 of it behind that, where they are 0.  2^(e_max - 7) goes to the scores (keys) and into the weights (values, as in
+// paged_short.cu, with a sum apart for blocks whose exponents are not ordinary), once a block.  Where exponents of a block lie further
+// apart than 22 and a row does not see all of its keys, the largest may be of one that is hidden from it: that row is made a NaN, and
+// gone through key by key as those are.  bf16 queries are scaled into fp16's range, row by row, by a power of two.
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -42,6 +42,7 @@ namespace ftb {
 namespace {
 
 constexpr int kKeys = 128, kAtLeast = 1, kStretches = 4, kRefs = 8, kFar = 256;
+constexpr int kUp = 7, kExact = 15 + kUp;  // 8 bits: codes as fp16 are times 2^kUp; the smallest code is 2^-9, fp16's smallest number 2^-24
 constexpr int kMostSlots = 14;
 constexpr float kAbove = 8.f;  // as in flash_attn.cu: the maximum in use may lie 2^8 below the real one
 
@@ -73,7 +74,7 @@ struct Control {
   // 8 bits: what `sum` refers to, and a thread's own: the sum of blocks apart and what it refers to (in registers: 646 for 628 us of drafts)
   float sum_top[k8 ? 2 : 1][k8 ? 128 : 1], apart_l[k8 ? 2 : 1][k8 ? 128 : 1], apart_n[k8 ? 2 : 1][k8 ? 128 : 1];
   int see_lo[2][128], see_hi[2][128];
-  int k_ref[kRefs], v_ref[kRefs];  // e_max of a block; + kFar: exponents more than 15 apart, in one that not every row sees all of
+  int k_ref[kRefs], v_ref[kRefs];  // e_max of a block; + kFar: exponents more than kExact apart, in one that not every row sees all of
   uint32_t tmem_base;
   int abort, dead;
 };
@@ -479,7 +480,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
         ctl.see_hi[t][r] = static_cast<int>(max(-1ll, min(pos, static_cast<long long>(x.keys.hi) - 1)));
         ctl.see_lo[t][r] = a.window > 0 ? static_cast<int>(max(0ll, min(pos - a.window + 1, static_cast<long long>(INT_MAX)))) : 0;
       }
-      float factor = a.scale_log2;
+      float factor = a.scale_log2 * (k8 ? 1.f / (1 << kUp) : 1.f);
 
       // ---- queries: this thread's columns are those that it finishes
       if (busy) {
@@ -549,11 +550,11 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
               if (lo_col > max(0, x.keys.lo - key0) || hi_col < min(kKeys, x.keys.hi - key0) - 1) factor = __uint_as_float(0x7fffffffu);
             }
             // (hidden scores are -inf already: times 0, as of a row of zeros and small keys, they would be NaN, as a score of 0 times
-            // infinity.  No score moves: they are below 2^17 here.)
+            // infinity.  No score moves: they are below 2^40 here.)
             f = fminf(fmaxf(factor * exponent_scale(kr), FLT_MIN), FLT_MAX);
             if (factor != factor) f = factor;
-            add = static_cast<float>(vr - 127);
-            inv = exponent_scale(254 - vr);
+            add = static_cast<float>(vr - 127 - kUp);
+            inv = exponent_scale(min(254, 254 + kUp - vr));  // (of use where `add` is ordinary)
           }
           // kChunk scores at a time, read again for the weights.  (A thread that spills goes to L2 for it: shared memory has taken
           // L1's room.  And loops instead of straight code: with several roles on an SM its instruction cache is what runs out.)
@@ -849,8 +850,8 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
                 w = __vminu4(w, w >> 16 | w << 16);
                 return min(w & 0xffu, w >> 8 & 0xffu);
               };
-              if (top - static_cast<int>(__reduce_min_sync(0xffffffffu, smallest(kw))) > 15 ||
-                  v_top - static_cast<int>(__reduce_min_sync(0xffffffffu, smallest(vw))) > 15)
+              if (top - static_cast<int>(__reduce_min_sync(0xffffffffu, smallest(kw))) > kExact ||
+                  v_top - static_cast<int>(__reduce_min_sync(0xffffffffu, smallest(vw))) > kExact)
                 far = kFar;
             }
             if (lane == 0) {
@@ -861,7 +862,8 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
         }
         const int e = __shfl_sync(0xffffffffu, mine, cw * 8 + (lane >> 2)) >> (8 * (lane & 3)) & 0xff;  // of key cw * 32 + lane
         const int below = max(0, top - e);
-        uint32_t by = below < 15 ? static_cast<uint32_t>(15 - below) << 10 : below <= 24 ? 1u << (24 - below) : 0u;  // 2^-below as fp16
+        // 2^(kUp - below) as fp16
+        uint32_t by = below < kExact ? static_cast<uint32_t>(kExact - below) << 10 : below <= 24 + kUp ? 1u << (24 + kUp - below) : 0u;
         by |= by << 16;
         ok = mbar_wait_warp(&ctl.kv_empty[slot], ((count + n) / kSlots & 1) ^ 1u, s_abort, status, FTB_ERR_TIMEOUT_SLOT);
         if (!ok) break;

@@ -230,3 +230,43 @@ def test_sizes_of_queries_and_keys_that_cancel(kv, group, d, page, new, lens, wi
         assert bool(torch.isnan(o[last].float()).all())
         o[last] = _exact(q, cache, table, lens, new, 0.3, window)[0].to(BF16).cuda()[last]
     _check(o, q, cache, table, lens, new, 0.3, window)
+
+
+@pytest.mark.parametrize("apart", [16, 23, 25, 28, 31])
+@pytest.mark.parametrize("new,lens", [([30] * 3, [700, 800, 900]), ([200], [900])])
+def test_values_far_below_the_largest_of_their_block(new, lens, apart):
+    """One value of each 128, 2^apart times as large as the others, whose key weighs nothing: the others' mean is left."""
+    kv, group, d, page = 2, 4, 64, 16
+    table, ln, st, pages = _batch(new, lens, page)
+    cache = _cache(pages, kv, page, d, 3)
+    q = _numbers((sum(new), kv * group, d), 1)
+    q[..., 0] = 8.0
+    rows = lambda n: (torch.arange(n) % 128 == 5) & (torch.arange(n) < 600)  # before the first token that asks
+    _change(cache, 1, table, lens, rows, apart)
+    for b, n in enumerate(lens):  # their keys: a code of -448 in the first place, zeros behind
+        j = rows(n).nonzero()[:, 0]
+        at = table[b].cpu().long()[j // page].cuda(), slice(None), (j % page).cuda()
+        cache[0].view(torch.uint8)[at] = 0
+        cache[0].view(torch.uint8)[at + (0,)] = 0xFE
+        cache[2][at] = 124
+    o = _ops().paged_attention(q, cache, table, ln, st, scale=0.3)
+    _ops().check_status()
+    want, (mean, size, most) = _exact(q, cache, table, lens, new, 0.3, None)
+    # as in test_large_values_without_weight, and values as products take them: fp16 numbers code * 2^(7 - below) in units of
+    # 2^(e - 134), e the block's largest exponent; off by 2^-25 of them, that is 2^-32 * 2^(e - 127), and 2^(e - 127) is below the
+    # largest value / 224
+    eps = torch.finfo(BF16).eps
+    tol = eps / 2 * want.abs() + (2.0 ** -11 + 4 * (d + 4) * 2.0 ** -24 * size[..., None] + 2.0 ** -15) * mean + 900 * 2.0 ** -24 * 8
+    # Rows here have exponents one or two apart, so that some lie 32 or more below the largest: 2^(7 - below) is 0 in fp16 then (its
+    # smallest number is 2^-24), and they are off by themselves.  Their part of the mean of |values|:
+    lost = tuple(c.clone() for c in cache)
+    for b, n in enumerate(lens):
+        j = torch.arange(n, device="cuda")
+        at = table[b].long()[j // page], slice(None), j % page
+        e = cache[3][at].int()  # [n, kv]
+        top = torch.cat([x.amax(0, keepdim=True).expand_as(x) for x in e.split(128)])
+        assert apart >= 30 or not bool((top - e > 31).any())
+        lost[1].view(torch.uint8)[at] = lost[1].view(torch.uint8)[at] * (top - e > 31)[..., None]
+    tol = (tol + 2.0 ** -32 / 224 * most[..., None] + _exact(q, lost, table, lens, new, 0.3, None)[1][0]) * (1 + eps)
+    err = (o.double().cpu() - want).abs()
+    assert bool((err <= tol).all()), float((err / tol).nan_to_num(9e9).max())
