@@ -8,7 +8,7 @@
 // Only one row of p (and of q) a sequence is read whole.  Sums are kept in 64 bits: the chosen index follows from a
 // comparison with a partial sum of up to V numbers, and in 32 bits the order of summation would decide it.
 //
-// Bound by the bytes of those rows: 100 sequences of 5 drafts over 130 001 words 29.5 us, 3.5 TB/s (one: 7.3 us, trips to memory one
+// Bound by the bytes of those rows: 100 sequences of 5 drafts over 130 001 words 30.3 us, 3.4 TB/s (one: 7.5 us, trips to memory one
 // behind the other: the drafts' probabilities, the row, the stretch).  A cluster of CTAs takes a sequence, every warp a stretch of the row: one pass for the
 // stretches' sums, which the CTAs hand each other through distributed shared memory, and a second look at the one stretch (a 64th of
 // the row or less) in which the limit is passed.  Every CTA finds n on its own, which saves a step of waiting.
@@ -33,8 +33,14 @@ struct Drafts {
   int K, V;
 };
 
+// What is not positive and finite counts as 0, in the target's rows and in the draft's.
+__device__ __forceinline__ double probability(float x) {
+  x = fmaxf(x, 0.f);  // (0 of a NaN)
+  return static_cast<double>(x < __int_as_float(0x7f800000) ? x : 0.f);
+}
+
 __device__ __forceinline__ double weight_of(float p, float q, int j, int without) {
-  const double w = static_cast<double>(p) - static_cast<double>(q);
+  const double w = static_cast<double>(p) - probability(q);  // (nothing is left of a p that is not positive)
   return w > 0.0 && p < __int_as_float(0x7f800000) && j != without ? w : 0.0;
 }
 
@@ -76,8 +82,8 @@ verify_drafts_kernel(Drafts a, long long* __restrict__ tokens, int* __restrict__
     if (i >= kThreads) id = x[i];
     bool taken = false;
     if (id >= 0 && id < V) {
-      const double qx = q != nullptr ? static_cast<double>(q[i * a.q_row + id]) : 1.0;
-      taken = static_cast<double>(u[i]) * qx < static_cast<double>(p[i * a.p_row + id]);
+      const double qx = q != nullptr ? probability(q[i * a.q_row + id]) : 1.0;
+      taken = static_cast<double>(u[i]) * qx < probability(p[i * a.p_row + id]);
     } else if (rank == 0) {
       atomicCAS(status, 0, FTB_ERR_INDEX);
     }

@@ -71,6 +71,8 @@ def verify(probs, drafts, u, draft_probs=None, counts=None):
     tokens = torch.full((B, K + 1), -1, dtype=torch.int64)
     n_out = torch.zeros(B, dtype=torch.int32)
     clean = lambda x: torch.where(torch.isfinite(x) & (x > 0), x, 0.0)
+    probs = clean(probs)
+    draft_probs = clean(draft_probs) if draft_probs is not None else None
     for b in range(B):
         mine = K if counts is None else min(max(int(counts[b]), 0), K)
         n = 0
@@ -83,17 +85,16 @@ def verify(probs, drafts, u, draft_probs=None, counts=None):
                 break
             tokens[b, n] = x
             n += 1
-        p = probs[b, n].double()
-        w = clean(p)
+        w = p = probs[b, n].double()
         if n < mine:
             x = int(drafts[b, n])
             if draft_probs is not None:
-                w = torch.where(torch.isfinite(p), clean(p - draft_probs[b, n].double()), 0.0)
+                w = clean(p - draft_probs[b, n].double())
             elif 0 <= x < V:
                 w = w.clone()
                 w[x] = 0.0
             if not float(w.sum()) > 0:
-                w = clean(p)
+                w = p
         if float(w.sum()) > 0:
             sums = w.cumsum(0)
             above = (sums > float(u[b, K]) * float(sums[-1])).nonzero()
