@@ -768,7 +768,7 @@ def paged_cache_read(cache, table, lens, starts, rows, dtype=None, out=None):
 
     With starts[b+1] - starts[b] == lens[b] that is sequence b whole.  rows: what starts ends with, or more: rows that belong to
     no sequence are left as they were.  dtype: 16-bit caches: their own; 8-bit ones: float32, float16 or bfloat16 (the
-    default, which holds every such number exactly)."""
+    default, which holds every number of a row with an exponent byte of 3 to 246 exactly; below lie its smallest numbers, above its end)."""
     if out is None:
         done = host.paged_cache_read(cache, table, lens, starts, rows, _DT.get(_read_dtype(cache, dtype), -1), _workspaces)
         if done is not None:

@@ -270,3 +270,27 @@ def test_values_far_below_the_largest_of_their_block(new, lens, apart):
     tol = (tol + 2.0 ** -32 / 224 * most[..., None] + _exact(q, lost, table, lens, new, 0.3, None)[1][0]) * (1 + eps)
     err = (o.double().cpu() - want).abs()
     assert bool((err <= tol).all()), float((err / tol).nan_to_num(9e9).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16, F16])
+@pytest.mark.parametrize("first", [1, 3, 100, 244])
+def test_reading_at_the_ends_of_the_exponents(dtype, first):
+    """Every code under the first, last and some exponents that rows are stored with: rounded once, and bf16 exact from 3 to 246."""
+    kv, d, page = 4, 128, 16
+    table, ln, st, pages = _batch([16], [16], page)
+    cache = _ops().paged_cache(pages, kv, page, d, E4M3)
+    at = int(table[0, 0])
+    codes = torch.arange(256, dtype=torch.uint8).view(2, d).repeat(page // 2, 1)
+    for h in range(kv):
+        for i in range(2):
+            cache[i].view(torch.uint8)[at, h] = codes.cuda()
+            cache[2 + i][at, h] = first + h
+    got = _ops().paged_cache_read(cache, table, ln, st, 16, dtype=dtype)
+    _ops().check_status()
+    for h in range(kv):
+        numbers = paged.values(codes, torch.full((page,), first + h, dtype=torch.uint8))
+        want = numbers.float().to(dtype)  # (the numbers have four bits: fp32 has them all, or infinity)
+        for x in got:
+            assert torch.equal(x[:, h].cpu().nan_to_num(nan=3.0), want.nan_to_num(nan=3.0))
+            if dtype == BF16 and 3 <= first + h <= 246:
+                assert torch.equal(x[:, h].cpu().double().nan_to_num(nan=3.0), numbers.nan_to_num(nan=3.0))
