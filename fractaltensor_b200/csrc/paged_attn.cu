@@ -20,6 +20,8 @@ namespace {
 
 constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kJoinRows = 4, kMostCuts = 4 * kJoinThreads;
 
+constexpr float kLog2E = 1.4426950408889634f;
+
 struct Pieces {
   const float* parts;
   const PagedCut* cuts;
@@ -302,7 +304,7 @@ extern "C" int ftb_paged_attn_fwd(const void* q, long long q_row, long long q_he
   if (T < 0 || B <= 0 || W <= 0 || pages <= 0 || kv_heads <= 0 || group <= 0 || window < 0) return FTB_ERR_ARG;
   if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) return FTB_ERR_ARG;
   if ((d != 64 && d != 128) || (dtype != FTB_F16 && dtype != FTB_BF16)) return FTB_ERR_ARG;
-  if (!(scale > 0.f) || !(scale <= FLT_MAX)) return FTB_ERR_ARG;  // hidden scores are -inf behind the scale
+  if (!(scale > 0.f) || !(scale * kLog2E <= FLT_MAX)) return FTB_ERR_ARG;  // hidden scores are -inf behind the scale, those of 0 are not
   if (static_cast<long long>(kv_heads) * group > 65536 || static_cast<long long>(T) * group > INT_MAX) return FTB_ERR_ARG;
   if (((q_row | q_head) & 7) != 0) return FTB_ERR_ALIGN;
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(k_cache) |
@@ -327,7 +329,7 @@ extern "C" int ftb_paged_attn_fwd(const void* q, long long q_row, long long q_he
   a.kv_heads = kv_heads;
   a.group = group;
   a.window = window;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale * kLog2E;
   a.status = static_cast<int*>(workspace);
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (scratch == nullptr || scratch_bytes < ftb_paged_attn_scratch_bytes(T, B, kv_heads, group, d)) return FTB_ERR_WORKSPACE;

@@ -433,7 +433,7 @@ int ftb_paged_cache_read(const void* k_cache, const void* v_cache, const unsigne
 /* Attention of the new tokens, whose keys and values are in the cache already: o = softmax(scale * q . k^T) v over the keys
  * j <= pos of a token at position pos, with window > 0 over pos - window < j <= pos only.  q: T rows of kv_heads * group heads of d
  * numbers of `dtype`, `q_row` and `q_head` numbers apart; head i reads the keys of kv head i / group; o [T, kv_heads * group, d].
- * scale > 0; o is not q's memory.  A token that sees nothing gets zeros.  Keys that a token does not see have no part in its result, whatever they and the
+ * scale > 0 (and scale * log2(e) finite); o is not q's memory.  A token that sees nothing gets zeros.  Keys that a token does not see have no part in its result, whatever they and the
  * unwritten rows of a page hold.  16-bit pages have the type of q.  scratch: ftb_paged_attn_scratch_bytes. */
 size_t ftb_paged_attn_scratch_bytes(int T, int B, int kv_heads, int group, int d);
 int ftb_paged_attn_fwd(const void* q, long long q_row, long long q_head, const void* k_cache, const void* v_cache,

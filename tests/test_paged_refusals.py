@@ -119,3 +119,8 @@ def test_oracle_verification_takes_by_the_ratio():
     for u, want in ((0.49, [0, 0]), (0.51, [1, -1])):
         got, n = paged.verify(p, torch.tensor([[0]]), torch.tensor([[u, 0.3]]), q)
         assert got.tolist() == [want] and n.tolist() == [2 if u < 0.5 else 1]
+
+
+@pytest.mark.parametrize("scale", [2.5e38, 3.4e38])
+def test_a_scale_that_is_infinite_in_log2_is_refused(lib, scale):
+    assert _attn(lib, o=ctypes.c_void_p(1 << 20), scale=scale) == 1
