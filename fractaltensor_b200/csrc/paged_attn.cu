@@ -8,6 +8,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <climits>
+#include <cstdlib>
 #include <type_traits>
 
 #include "../../include/ftb200.h"
@@ -278,6 +279,19 @@ Form form_of(int T, int B, int group) {
   return {few, few, many};
 }
 
+// Whether n numbers at o (16 bits) meet the numbers of some of T rows of heads at q.
+bool over_rows(const void* o, long long n, const void* q, int T, long long q_row, int heads, long long q_head, int d) {
+  const long long span = (heads - 1) * q_head, lo = std::min(0ll, span), hi = std::max(0ll, span) + d;  // of a row
+  const long long step = T > 1 ? std::abs(q_row) : 0, first = T > 1 && q_row < 0 ? (T - 1) * q_row : 0;
+  // o's beginning, in numbers from where the lowest row is (both on 16-byte boundaries)
+  const long long at = static_cast<long long>(reinterpret_cast<uintptr_t>(o) - reinterpret_cast<uintptr_t>(q)) / 2 - first;
+  if (step == 0) return at < hi && at + n > lo;
+  // rows r with r * step + hi > at and r * step + lo < at + n
+  auto floor_div = [](long long x, long long y) { return x >= 0 ? x / y : -((-x + y - 1) / y); };
+  const long long r0 = std::max(0ll, floor_div(at - hi, step) + 1), r1 = std::min(T - 1ll, floor_div(at + n - lo - 1, step));
+  return r0 <= r1;
+}
+
 size_t places(int pieces, int rows, int d) { return 2 * static_cast<size_t>(pieces) * rows * (d + 2) * sizeof(float) + pieces * sizeof(PagedCut); }
 size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -312,7 +326,13 @@ extern "C" int ftb_paged_attn_fwd(const void* q, long long q_row, long long q_he
     return FTB_ERR_ALIGN;
   if (workspace == nullptr || workspace_bytes < ftb_workspace_bytes()) return FTB_ERR_WORKSPACE;
   if (T == 0) return FTB_OK;
-  if (q == o) return FTB_ERR_ARG;  // queries are read again by other blocks than those that write their rows
+  // queries are read again by other blocks than those that write their rows, and so are pages
+  const int heads = kv_heads * group;
+  const size_t o_bytes = 2 * static_cast<size_t>(T) * heads * d, numbers = static_cast<size_t>(pages) * kv_heads * page_size * d;
+  const size_t cache_bytes = k_exp != nullptr ? numbers : 2 * numbers, exp_bytes = k_exp != nullptr ? numbers / d : 0;
+  if (over_rows(o, static_cast<long long>(o_bytes / 2), q, T, q_row, heads, q_head, d) || overlap(o, o_bytes, k_cache, cache_bytes) ||
+      overlap(o, o_bytes, v_cache, cache_bytes) || overlap(o, o_bytes, k_exp, exp_bytes) || overlap(o, o_bytes, v_exp, exp_bytes))
+    return FTB_ERR_ARG;
   const int rc = check_device_sm100();
   if (rc) return rc;
   PagedAttn a;

@@ -285,6 +285,13 @@ extern "C" int ftb_paged_cache_read(const void* k_cache, const void* v_cache, co
   if (((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15) != 0) return FTB_ERR_ALIGN;
   if (workspace == nullptr || workspace_bytes < ftb_workspace_bytes()) return FTB_ERR_WORKSPACE;
   if (T == 0) return FTB_OK;
+  const size_t numbers = static_cast<size_t>(pages) * kv_heads * page_size * d, cache_bytes = k8 ? numbers : 2 * numbers;
+  const size_t out_bytes = static_cast<size_t>(T) * kv_heads * d * dtype_size(dtype), exp_bytes = k8 ? numbers / d : 0;
+  if (overlap(k_out, out_bytes, v_out, out_bytes)) return FTB_ERR_ARG;
+  for (const void* out : {k_out, v_out})
+    if (overlap(out, out_bytes, k_cache, cache_bytes) || overlap(out, out_bytes, v_cache, cache_bytes) ||
+        overlap(out, out_bytes, k_exp, exp_bytes) || overlap(out, out_bytes, v_exp, exp_bytes))
+      return FTB_ERR_ARG;
   if ((rc = check_device_sm100())) return rc;
   const Cache cache{const_cast<unsigned char*>(static_cast<const unsigned char*>(k_cache)),
                     const_cast<unsigned char*>(static_cast<const unsigned char*>(v_cache)),

@@ -123,6 +123,12 @@ inline cudaError_t launch_light(void (*kfn)(KArgs...), dim3 grid, dim3 block, si
   return cudaLaunchKernelEx(&cfg, kfn, static_cast<KArgs>(args)...);
 }
 
+// Whether n bytes at a and m at b have one in common.
+inline bool overlap(const void* a, size_t n, const void* b, size_t m) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return n > 0 && m > 0 && (x <= y ? y - x < n : x - y < m);
+}
+
 // Process-wide count of kernels this library has launched (reported by ftb_launch_count()).
 void count_launch(int n = 1);
 long long launches_so_far();

@@ -798,7 +798,7 @@ def paged_attention(q, cache, table, lens, starts, scale=None, window=None, out=
 
     q: [T, heads, d], heads a multiple of the cache's kv_heads, rows as in paged_cache_write -> [T, heads, d]: for a token
     at position p softmax(scale * q . k_j) v over the keys j <= p, with `window` over p - window < j <= p only.  Tokens that see
-    nothing get zeros; rows that belong to no sequence are left as they were.  out is not q's memory."""
+    nothing get zeros; rows that belong to no sequence are left as they were.  out overlaps neither q nor the cache."""
     done = host.paged_attention(q, cache, table, lens, starts, out, 1.0 if scale is None else scale, 0 if window is None else window or -1,
                                 _workspaces)
     if done is not None:

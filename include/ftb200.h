@@ -420,7 +420,7 @@ int ftb_gemm_nt(const void* A, const void* Bt, void* out, int M, int N, int K, i
  * ftb_paged_cache_write: k, v: T rows of kv_heads rows of d numbers of `dtype` (fp16 or bf16), `*_row` and `*_head` numbers apart
  * (multiples of 8; the slices of a fused product are taken as they are).
  * ftb_paged_cache_read: the same tokens out of the cache into k_out, v_out [T, kv_heads, d] of `dtype` (16-bit pages: their own type;
- * 8-bit ones: fp32, fp16 or bf16). */
+ * 8-bit ones: fp32, fp16 or bf16).  They overlap neither each other nor the cache. */
 int ftb_paged_cache_write(const void* k, const void* v, long long k_row, long long k_head, long long v_row, long long v_head,
                           void* k_cache, void* v_cache, unsigned char* k_exp, unsigned char* v_exp, const int* table,
                           const int* lens, const int* starts, int T, int B, int W, int pages, int kv_heads, int page_size,
@@ -433,7 +433,7 @@ int ftb_paged_cache_read(const void* k_cache, const void* v_cache, const unsigne
 /* Attention of the new tokens, whose keys and values are in the cache already: o = softmax(scale * q . k^T) v over the keys
  * j <= pos of a token at position pos, with window > 0 over pos - window < j <= pos only.  q: T rows of kv_heads * group heads of d
  * numbers of `dtype`, `q_row` and `q_head` numbers apart; head i reads the keys of kv head i / group; o [T, kv_heads * group, d].
- * scale > 0 (and scale * log2(e) finite); o is not q's memory.  A token that sees nothing gets zeros.  Keys that a token does not see have no part in its result, whatever they and the
+ * scale > 0 (and scale * log2(e) finite); o has no part of q's rows or of the cache.  A token that sees nothing gets zeros.  Keys that a token does not see have no part in its result, whatever they and the
  * unwritten rows of a page hold.  16-bit pages have the type of q.  scratch: ftb_paged_attn_scratch_bytes. */
 size_t ftb_paged_attn_scratch_bytes(int T, int B, int kv_heads, int group, int d);
 int ftb_paged_attn_fwd(const void* q, long long q_row, long long q_head, const void* k_cache, const void* v_cache,
