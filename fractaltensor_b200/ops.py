@@ -815,10 +815,10 @@ def paged_attention(q, cache, table, lens, starts, scale=None, window=None, out=
     if out is None:
         out = torch.empty(T, heads, d, dtype=q.dtype, device=q.device)
     _req_like(out, "out", q.dtype, (T, heads, d), q)
-    # of the call's own: calls on other streams, and graphs replayed at the same time, have others
-    n = lib.ftb_paged_attn_scratch_bytes(T, B, kv, heads // kv, d)
     ws = workspace(kc.device)
     with _on(kc.device):
+        # of the call's own: calls on other streams, and graphs replayed at the same time, have others
+        n = lib.ftb_paged_attn_scratch_bytes(T, B, kv, heads // kv, d)
         scratch = torch.empty(n, dtype=torch.uint8, device=kc.device) if n else None
         check(lib.ftb_paged_attn_fwd(qp, qr, qh, *args, _ptr(out), T, B, W, pages, kv, heads // kv, page_size, d,
                                      min(int(window), 0x7fffffff) if window is not None else 0, 1.0 if scale is None else float(scale),

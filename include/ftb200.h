@@ -434,7 +434,8 @@ int ftb_paged_cache_read(const void* k_cache, const void* v_cache, const unsigne
  * j <= pos of a token at position pos, with window > 0 over pos - window < j <= pos only.  q: T rows of kv_heads * group heads of d
  * numbers of `dtype`, `q_row` and `q_head` numbers apart; head i reads the keys of kv head i / group; o [T, kv_heads * group, d].
  * scale > 0 (and scale * log2(e) finite); o has no part of q's rows or of the cache.  A token that sees nothing gets zeros.  Keys that a token does not see have no part in its result, whatever they and the
- * unwritten rows of a page hold.  16-bit pages have the type of q.  scratch: ftb_paged_attn_scratch_bytes. */
+ * unwritten rows of a page hold.  16-bit pages have the type of q.  scratch: ftb_paged_attn_scratch_bytes, asked for with
+ * the call's device as the current one. */
 size_t ftb_paged_attn_scratch_bytes(int T, int B, int kv_heads, int group, int d);
 int ftb_paged_attn_fwd(const void* q, long long q_row, long long q_head, const void* k_cache, const void* v_cache,
                        const unsigned char* k_exp, const unsigned char* v_exp, const int* table, const int* lens,
