@@ -267,8 +267,10 @@ struct Form {
 };
 Form form_of(int T, int B, int group) {
   const long long rows = static_cast<long long>(T) * group;
-  // Not more tokens than sequences: a decoding step.  (Where one of them has them all the others are empty, and its tiles
-  // are read through L2.)
+  // Not more tokens than sequences: a decoding step.  Where one of them has most of the tokens, its tiles read the keys once each, through
+  // L2: 256 sequences, all but one without a token, 8 kv heads, 1000 keys, 24 tokens 23 us (with paged_tile.cu beside it 32), 100 tokens
+  // 56 (39), 200 tokens 108 (41).  A step of a token each pays for that second launch: 8 sequences 15 us (23), 64 of up to 8000 keys 179
+  // (186).  Which it is stands on the device alone.
   if (T <= B) return {rows <= 8ll * B ? 8 : 16, INT_MAX, 0};
   if (rows <= 16) return {rows <= 8 ? 8 : 16, INT_MAX, 0};
   const int many = rows > 128ll * B ? 256 : 128;
