@@ -270,17 +270,6 @@ __device__ __forceinline__ void st_cluster_16(T* p, uint32_t rank, T x) {
   asm volatile("st.shared::cluster.u16 [%0], %1;" ::"r"(map_to_cta(smem_u32(p), rank)),
                "h"(*reinterpret_cast<const unsigned short*>(&x)) : "memory");
 }
-// D += A B of 16 x 8 x 16, A rows of 16-bit numbers, fp32 sums.
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 
 template <typename T>
 __global__ void __launch_bounds__(kDecThreads)
@@ -422,7 +411,7 @@ attn_decode_kernel(const T* __restrict__ enc, const T* __restrict__ enc_proj, co
         b0 = *reinterpret_cast<const uint32_t*>(&s_v[col][k + 2 * (lane & 3)]);
         b1 = *reinterpret_cast<const uint32_t*>(&s_v[col][k + 8 + 2 * (lane & 3)]);
       }
-      mma16816(d, a, b0, b1, T());
+      mma16816<T>(d, a[0], a[1], a[2], a[3], b0, b1);
     }
     if ((lane & 3) == 0) {
       s_z[half][0][m0 + col] = d[0];
