@@ -29,15 +29,19 @@ struct Pieces {
   int pieces, rows;  // rows of a tile
 };
 
-// Rows of whole tiles that have to be computed again: none, unless something in the cache is not finite.  `warp` of `warps` in the grid.
+// Rows of whole tiles that have to be computed again: none, unless something in the cache is not finite, or dwarfs what is seen of its
+// 8-bit block.  `warp` of `warps` in the grid.  Those of a tile lie side by side: a warp looks at four times eight (a sector of flags) far
+// from each other.
 template <typename T, bool k8, int D>
 __device__ __forceinline__ void again_rows(const PagedAttn& a, long long warp, long long warps, int lane) {
   const int heads = a.kv_heads * a.group;
   const long long rows = static_cast<long long>(a.T) * heads;
-  for (long long r0 = warp * 32; r0 < rows; r0 += warps * 32) {
-    unsigned again = __ballot_sync(0xffffffffu, r0 + lane < rows && a.odd[min(r0 + lane, rows - 1)] != 0);
+  for (long long r0 = warp * 8; r0 < rows; r0 += warps * 32) {
+    const long long mine = r0 + (lane >> 3) * warps * 8 + (lane & 7);
+    unsigned again = __ballot_sync(0xffffffffu, mine < rows && a.odd[min(mine, rows - 1)] != 0);
     while (again != 0) {
-      const long long row = r0 + __ffs(again) - 1;
+      const int first = __ffs(again) - 1;
+      const long long row = __shfl_sync(0xffffffffu, mine, first);
       again &= again - 1;
       const int t = static_cast<int>(row / heads);
       const RowPlace at = place_of_row(a.batch, t, lane);
