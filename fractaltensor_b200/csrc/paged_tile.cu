@@ -574,7 +574,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
           }
           // (a row may see nothing of a block: the lowest finite number keeps its weights 0)
           const float m_new = fmaxf(fmaf(mx, f, add), -FLT_MAX);
-          const bool apart = k8 && fabsf(add) > near;  // (the same in all lanes)
+          const bool apart = k8 && fabsf(add + kUp) > near;  // (the same in all lanes)
           if constexpr (k8) {
             if (apart) {
               const bool both = near > 0.f && k > 0;  // l holds something, and top is near the scores
