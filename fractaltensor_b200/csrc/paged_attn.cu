@@ -5,6 +5,9 @@
 // paged_tile.cu for those with many, by matrix products on tiles of rows.  A call with both kinds runs both, each on its own; the
 // lengths are on the device, so that it is there that a sequence is one or the other's.  Here: the choice, and what joins the tiles
 // that the cuts between pieces of work went through.
+//
+// Scores, maxima, sums and results in the making have 32 bits.  Weights are rounded to the 16 bits that the second product takes (of the cache's
+// type, fp16 over 8 bits): with bf16 results the error against 64 bits is 0.0019 of their size, 0.0017 where weights keep 32 bits.
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -280,7 +283,7 @@ Form form_of(int T, int B, int group) {
   const int many = rows > 128ll * B ? 256 : 128;
   if (B == 1) return {0, 0, many};
   // One tile of paged_short.cu: a second one would read the keys again.  96 sequences, 8 kv heads, 4500 keys of 16 bits: 8 rows
-  // 270 us, 16 rows 296, as rows of paged_tile.cu 24 336, 64 360, 128 398; 8500 keys of 8 bits: 311, 433, then 660, 640, 656.
+  // 273 us, 16 rows 302, as rows of paged_tile.cu 24 349, 64 367, 128 405; 8500 keys of 8 bits: 327, 400, then 650, 679, 728.
   const int few = group <= 8 && rows > 16ll * B ? 8 : 16;
   return {few, few, many};
 }

@@ -4,7 +4,7 @@
 //
 // 2048 tokens behind 14 336 keys, 32 heads of 128 over 8 kv heads, bf16: 558 us, 0.92 PFLOP/s; bound by the chain of a row's scores, 4300
 // cycles a block of 256 rows beside 2048 of products, and by the joins (25 us).  96 sequences of 8500 keys on average in 8 bits, 5 tokens
-// of 64 heads: 645 us, 0.2 PFLOP/s and 2.5 TB/s; bound by the instructions that make 8-bit keys operands (1.6 to 1.9 a cycle and SM).
+// of 64 heads: 660 us, 0.2 PFLOP/s and 2.5 TB/s (847 where values are of 2^-40, with the sum apart for every block); bound by the instructions that make 8-bit keys operands (1.6 to 1.9 a cycle and SM).
 // Measured and not kept, the chunk: all 128 scores of a row in registers 616 us (spills; L1 is shared memory's), 32 scores loaded ahead of
 // 32 in work 580, a warp for each slot's products 617, the slots' exponentials in turns 575, the second product in two halves 568 (of 566).
 //
