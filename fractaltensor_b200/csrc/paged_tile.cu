@@ -832,7 +832,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
             const int ref = (blocks0 + y.j) & (kRefs - 1);
             int v_top = __reduce_max_sync(0xffffffffu, largest(vw)), far = 0;
             if (key0 + kKeys - 1 > all_hi || key0 < all_lo) {
-              auto smallest = [](uint32_t w) -> uint32_t {  // (of those above 1: rows of zeros lose nothing)
+              auto smallest = [](uint32_t w) -> uint32_t {  // (of those above 1: rows of zeros lose nothing, and others with 1, below 2^-117, count as zeros)
                 w |= __vcmpleu4(w, 0x01010101u);
                 w = __vminu4(w, w >> 16 | w << 16);
                 return min(w & 0xffu, w >> 8 & 0xffu);
