@@ -72,6 +72,13 @@ SIGNATURES = {
     "ftb_paged_attn_fwd": (_i, [_vp, ctypes.c_longlong, ctypes.c_longlong] + [_vp] * 8 + [_i] * 9 + [_f, _i, _vp, _sz, _vp, _sz, _vp]),
     "ftb_verify_drafts": (_i, [_vp, ctypes.c_longlong, ctypes.c_longlong, _vp, ctypes.c_longlong, ctypes.c_longlong] + [_vp] * 5 +
                           [_i] * 3 + [_vp, _sz, _vp]),
+    "ftb_paged_attn_tree_fwd": (_i, [_vp, ctypes.c_longlong, ctypes.c_longlong] + [_vp] * 8 + [_i, _vp, _vp] + [_i] * 9 +
+                                [_f, _i, _vp, _sz, _vp, _sz, _vp]),
+    "ftb_tree_mask": (_i, [_vp, _vp, _i, _i, _vp]),
+    "ftb_verify_tree": (_i, [_vp, ctypes.c_longlong, ctypes.c_longlong] + [_vp] * 6 + [_i] * 3 + [_vp, _sz, _vp]),
+    "ftb_paged_cache_keep": (_i, [_vp] * 6 + [ctypes.c_longlong, ctypes.c_longlong] + [_vp] * 4 + [_i] * 8 + [_vp, _sz, _vp]),
+    "ftb_paged_attn_weights": (_i, [_vp, ctypes.c_longlong, ctypes.c_longlong] + [_vp] * 7 + [_i] * 9 + [_f, _i, _vp, _sz, _vp]),
+    "ftb_paged_cache_evict": (_i, [_vp] * 10 + [_i] * 9 + [_vp, _sz, _vp]),
     "ftb_gemm_nt": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, ctypes.POINTER(_i), _vp, _sz, _vp]),
 }
 
@@ -103,6 +110,7 @@ class _NoHost:
     b2b_gemm = flash_attention = sparse_attention = _decline
     embedding_gather = lstm_pack_weights = lstm_stacked_ragged = project_softmax = _decline
     paged_cache_write = paged_cache_read = paged_attention = verify_drafts = _decline
+    tree_mask = verify_tree = paged_cache_keep = paged_attention_weights = paged_cache_evict = _decline
 
     @staticmethod
     def current_stream(dev):

@@ -385,14 +385,27 @@ PyObject* project_softmax(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
-// A cache and a batch's description as the paged entry points take them.
+// A cache and a batch's description as the paged entry points take them; lens and starts where a call has them.
 struct PagedCall {
-  const at::Tensor *k, *v, *k_exp = nullptr, *v_exp = nullptr, *table, *lens, *starts;
+  const at::Tensor *k, *v, *k_exp = nullptr, *v_exp = nullptr, *table, *lens = nullptr, *starts = nullptr;
   int B, W, pages, kv, page_size, d;
 
   const unsigned char* exps(const at::Tensor* t) const { return t ? static_cast<const unsigned char*>(t->data_ptr()) : nullptr; }
-  const int* ints(const at::Tensor* t) const { return static_cast<const int*>(t->data_ptr()); }
+  const int* ints(const at::Tensor* t) const { return t ? static_cast<const int*>(t->data_ptr()) : nullptr; }
+  unsigned char* bytes(const at::Tensor* t) const { return t ? static_cast<unsigned char*>(t->data_ptr()) : nullptr; }
+  // a contiguous tensor of the cache's device
+  const at::Tensor* here(PyObject* o, at::ScalarType type, at::IntArrayRef shape) const {
+    const at::Tensor* t = cuda_tensor(o);
+    return t && t->scalar_type() == type && t->device() == k->device() && t->sizes() == shape ? t : nullptr;
+  }
 };
+bool paged_table(PyObject* o, const PagedCall& c, const at::Tensor** table) {
+  *table = cuda_tensor(o);
+  const at::Tensor* t = *table;
+  return t && t->scalar_type() == at::kInt && t->device() == c.k->device() && t->dim() == 2 && t->size(0) > 0 && t->size(1) > 0 &&
+         t->size(0) < 0x7fffffff && t->size(1) <= 0x7fffffff;
+}
+// (lens, starts: nullptr where the call has none)
 bool paged_call(PyObject* cache, PyObject* table, PyObject* lens, PyObject* starts, PagedCall* c) {
   if (!PyTuple_CheckExact(cache) || (PyTuple_GET_SIZE(cache) != 2 && PyTuple_GET_SIZE(cache) != 4)) return false;
   const bool eight = PyTuple_GET_SIZE(cache) == 4;
@@ -409,16 +422,9 @@ bool paged_call(PyObject* cache, PyObject* table, PyObject* lens, PyObject* star
     for (const at::Tensor* e : {c->k_exp, c->v_exp})
       if (!e || e->scalar_type() != at::kByte || e->device() != c->k->device() || e->sizes() != c->k->sizes().slice(0, 3)) return false;
   }
-  c->table = cuda_tensor(table);
-  c->lens = cuda_tensor(lens);
-  c->starts = cuda_tensor(starts);
-  for (const at::Tensor* t : {c->table, c->lens, c->starts})
-    if (!t || t->scalar_type() != at::kInt || t->device() != c->k->device()) return false;
-  if (c->table->dim() != 2 || c->table->size(0) <= 0 || c->table->size(1) <= 0 || c->table->size(0) >= 0x7fffffff ||
-      c->table->size(1) > 0x7fffffff)
-    return false;
-  if (c->lens->dim() != 1 || c->lens->size(0) != c->table->size(0) || c->starts->dim() != 1 || c->starts->size(0) != c->table->size(0) + 1)
-    return false;
+  if (!paged_table(table, *c, &c->table)) return false;
+  if (lens != nullptr && !(c->lens = c->here(lens, at::kInt, {c->table->size(0)}))) return false;
+  if (starts != nullptr && !(c->starts = c->here(starts, at::kInt, {c->table->size(0) + 1}))) return false;
   c->B = static_cast<int>(c->table->size(0));
   c->W = static_cast<int>(c->table->size(1));
   c->pages = static_cast<int>(c->k->size(0));
@@ -496,10 +502,10 @@ PyObject* paged_cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
-// (q, cache, table, lens, starts, out | None, scale, window (0: none), workspaces)
+// (q, cache, table, lens, starts, out | None, scale, window (0: none), tree | None, lse | None, workspaces)
 PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    DECLINE_UNLESS(n == 9);
+    DECLINE_UNLESS(n == 11);
     PagedCall c;
     DECLINE_UNLESS(paged_call(args[1], args[2], args[3], args[4], &c));
     int64_t qr, qh, window;
@@ -507,8 +513,18 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor* q = rows_of(args[0], c, &qr, &qh);
     DECLINE_UNLESS(q && get_float(args[6], &scale) && get_int(args[7], &window) && window >= 0 && c.kv > 0 && q->size(1) > 0 &&
                    q->size(1) % c.kv == 0);
+    const at::Tensor *tree = nullptr, *lse = nullptr;
+    if (args[8] != Py_None) {
+      tree = cuda_tensor(args[8]);
+      DECLINE_UNLESS(tree && tree->scalar_type() == at::kInt && tree->device() == c.k->device() && tree->dim() == 2 && tree->size(0) == q->size(0) &&
+                     tree->size(1) > 0 && tree->size(1) <= 0x7fffffff && window == 0);
+    }
+    if (args[9] != Py_None) {
+      lse = c.here(args[9], at::kFloat, {q->size(0), q->size(1)});
+      DECLINE_UNLESS(lse);
+    }
     const c10::DeviceIndex dev = c.k->device().index();
-    const at::Tensor ws = workspace_of(args[8], dev, ftb_workspace_bytes());
+    const at::Tensor ws = workspace_of(args[10], dev, ftb_workspace_bytes());
     DECLINE_UNLESS(ws.defined());
     at::Tensor out;
     DECLINE_UNLESS(given_result(args[5], *q, q->sizes(), &out));
@@ -521,10 +537,11 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       const size_t bytes = ftb_paged_attn_scratch_bytes(T, c.B, c.kv, group, c.d);
       at::Tensor scratch;
       if (bytes > 0) scratch = at::empty({static_cast<int64_t>(bytes)}, at::TensorOptions().dtype(at::kByte).device(q->device()));
-      rc = ftb_paged_attn_fwd(q->data_ptr(), qr, qh, c.k->data_ptr(), c.v->data_ptr(), c.exps(c.k_exp), c.exps(c.v_exp), c.ints(c.table),
-                              c.ints(c.lens), c.ints(c.starts), out.data_ptr(), T, c.B, c.W, c.pages, c.kv, group, c.page_size, c.d,
-                              static_cast<int>(window), scale, dtype_code(*q), bytes > 0 ? scratch.data_ptr() : nullptr, bytes,
-                              ws.data_ptr(), ws.numel(), stream_of(dev));
+      rc = ftb_paged_attn_tree_fwd(q->data_ptr(), qr, qh, c.k->data_ptr(), c.v->data_ptr(), c.exps(c.k_exp), c.exps(c.v_exp), c.ints(c.table),
+                                   c.ints(c.lens), c.ints(c.starts), c.ints(tree), tree ? static_cast<int>(tree->size(1)) : 0, out.data_ptr(),
+                                   lse ? static_cast<float*>(lse->data_ptr()) : nullptr, T, c.B, c.W, c.pages, c.kv, group, c.page_size, c.d,
+                                   static_cast<int>(window), scale, dtype_code(*q), bytes > 0 ? scratch.data_ptr() : nullptr, bytes,
+                                   ws.data_ptr(), ws.numel(), stream_of(dev));
     }
     return rc == 0 ? THPVariable_Wrap(out) : PyLong_FromLong(rc);
   });
@@ -580,6 +597,166 @@ PyObject* verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
+// (parents) -> mask
+PyObject* tree_mask(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    DECLINE_UNLESS(n == 1);
+    const at::Tensor* parents = cuda_tensor(args[0]);
+    DECLINE_UNLESS(parents && parents->scalar_type() == at::kInt && parents->dim() == 2 && parents->size(1) > 0 && parents->numel() <= 0x7fffffff &&
+                   parents->size(0) <= 0x7fffffff);
+    const int64_t B = parents->size(0), N = parents->size(1);
+    at::Tensor mask;
+    int rc;
+    {
+      const WithoutGil released;
+      const c10::DeviceIndex dev = parents->device().index();
+      const c10::cuda::CUDAGuard guard(dev);
+      mask = new_result(*parents, {B, N, (N + 31) / 32});
+      rc = ftb_tree_mask(static_cast<const int*>(parents->data_ptr()), static_cast<int*>(mask.data_ptr()), static_cast<int>(B), static_cast<int>(N),
+                         stream_of(dev));
+    }
+    return rc == 0 ? THPVariable_Wrap(mask) : PyLong_FromLong(rc);
+  });
+}
+
+// (probs, tokens, parents, u, workspaces) -> (tokens, path, counts)
+PyObject* verify_tree(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    DECLINE_UNLESS(n == 5);
+    const at::Tensor *tokens = cuda_tensor(args[1]), *parents = cuda_tensor(args[2]), *u = cuda_tensor(args[3]);
+    DECLINE_UNLESS(tokens && parents && u && THPVariable_Check(args[0]));
+    const at::Tensor& p = THPVariable_Unpack(args[0]);
+    DECLINE_UNLESS(parents->scalar_type() == at::kInt && parents->dim() == 2 && parents->size(1) > 0);
+    const int64_t B = parents->size(0), N = parents->size(1);
+    DECLINE_UNLESS(B <= 0x7fffffff && N <= 0x7fffffff);
+    DECLINE_UNLESS(tokens->scalar_type() == at::kLong && tokens->device() == parents->device() && tokens->sizes() == parents->sizes());
+    DECLINE_UNLESS(u->scalar_type() == at::kFloat && u->device() == parents->device() && u->sizes() == parents->sizes());
+    DECLINE_UNLESS(p.is_cuda() && p.device() == parents->device() && p.scalar_type() == at::kFloat && p.dim() == 3 && p.size(0) == B && p.size(1) == N);
+    const int64_t V = p.size(2);
+    DECLINE_UNLESS(V > 0 && V <= 0x7fffffff && (V == 1 || p.stride(2) == 1));
+    const c10::DeviceIndex dev = parents->device().index();
+    const at::Tensor ws = workspace_of(args[4], dev, ftb_workspace_bytes());
+    DECLINE_UNLESS(ws.defined());
+    at::Tensor out, path, counts;
+    int rc;
+    {
+      const WithoutGil released;
+      const c10::cuda::CUDAGuard guard(dev);
+      out = new_result(*tokens, {B, N});
+      path = new_result(*parents, {B, N});
+      counts = new_result(*parents, {B});
+      rc = ftb_verify_tree(static_cast<const float*>(p.data_ptr()), p.stride(0), p.stride(1), static_cast<const long long*>(tokens->data_ptr()),
+                           static_cast<const int*>(parents->data_ptr()), static_cast<const float*>(u->data_ptr()),
+                           static_cast<long long*>(out.data_ptr()), static_cast<int*>(path.data_ptr()), static_cast<int*>(counts.data_ptr()),
+                           static_cast<int>(B), static_cast<int>(N), static_cast<int>(V), ws.data_ptr(), ws.numel(), stream_of(dev));
+    }
+    if (rc != 0) return PyLong_FromLong(rc);
+    return Py_BuildValue("(NNN)", THPVariable_Wrap(out), THPVariable_Wrap(path), THPVariable_Wrap(counts));
+  });
+}
+
+// Pages to move to: *into stays nullptr for None.
+bool paged_into(PyObject* o, const PagedCall& c, const at::Tensor** into) {
+  *into = nullptr;
+  return o == Py_None || (paged_table(o, c, into) && (*into)->size(0) == c.B);
+}
+
+// (cache, kept, counts, table, first | None, into | None, weights | None, workspaces) -> True
+PyObject* paged_cache_keep(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    DECLINE_UNLESS(n == 8);
+    PagedCall c;
+    DECLINE_UNLESS(paged_call(args[0], args[3], nullptr, nullptr, &c));
+    const at::Tensor *kept = cuda_tensor(args[1]), *counts = c.here(args[2], at::kInt, {c.B}), *into, *first = nullptr, *weights = nullptr;
+    DECLINE_UNLESS(kept && kept->scalar_type() == at::kInt && kept->device() == c.k->device() && counts && paged_into(args[5], c, &into));
+    DECLINE_UNLESS((kept->dim() == 2 || (kept->dim() == 3 && kept->size(1) == c.kv)) && kept->size(0) == c.B && kept->size(-1) <= 0x7fffffff);
+    if (args[4] != Py_None) {
+      first = c.here(args[4], at::kInt, {c.B});
+      DECLINE_UNLESS(first);
+    }
+    if (args[6] != Py_None) {
+      weights = c.here(args[6], at::kFloat, {c.pages, c.kv, c.page_size});
+      DECLINE_UNLESS(weights);
+    }
+    const c10::DeviceIndex dev = c.k->device().index();
+    const at::Tensor ws = workspace_of(args[7], dev, ftb_workspace_bytes());
+    DECLINE_UNLESS(ws.defined());
+    int rc;
+    {
+      const WithoutGil released;
+      const c10::cuda::CUDAGuard guard(dev);
+      const int64_t K = kept->size(-1);
+      const bool per_head = kept->dim() == 3;
+      rc = ftb_paged_cache_keep(c.k->data_ptr(), c.v->data_ptr(), c.bytes(c.k_exp), c.bytes(c.v_exp),
+                                weights ? static_cast<float*>(weights->data_ptr()) : nullptr, c.ints(kept), per_head ? K * c.kv : K, per_head ? K : 0,
+                                c.ints(counts), c.ints(first), c.ints(c.table), c.ints(into), c.B, c.W, into ? static_cast<int>(into->size(1)) : 0,
+                                static_cast<int>(K), c.pages, c.kv, c.page_size, c.d, ws.data_ptr(), ws.numel(), stream_of(dev));
+    }
+    if (rc != 0) return PyLong_FromLong(rc);
+    Py_RETURN_TRUE;
+  });
+}
+
+// (q, cache, weights, lse, table, lens, starts, scale, window (0: none), workspaces) -> True
+PyObject* paged_attention_weights(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    DECLINE_UNLESS(n == 10);
+    PagedCall c;
+    DECLINE_UNLESS(paged_call(args[1], args[4], args[5], args[6], &c));
+    int64_t qr, qh, window;
+    float scale;
+    const at::Tensor* q = rows_of(args[0], c, &qr, &qh);
+    DECLINE_UNLESS(q && get_float(args[7], &scale) && get_int(args[8], &window) && window >= 0 && c.kv > 0 && q->size(1) > 0 &&
+                   q->size(1) % c.kv == 0);
+    const at::Tensor *weights = c.here(args[2], at::kFloat, {c.pages, c.kv, c.page_size}), *lse = c.here(args[3], at::kFloat, {q->size(0), q->size(1)});
+    DECLINE_UNLESS(weights && lse);
+    const c10::DeviceIndex dev = c.k->device().index();
+    const at::Tensor ws = workspace_of(args[9], dev, ftb_workspace_bytes());
+    DECLINE_UNLESS(ws.defined());
+    int rc;
+    {
+      const WithoutGil released;
+      const c10::cuda::CUDAGuard guard(dev);
+      rc = ftb_paged_attn_weights(q->data_ptr(), qr, qh, c.k->data_ptr(), c.exps(c.k_exp), static_cast<const float*>(lse->data_ptr()),
+                                  c.ints(c.table), c.ints(c.lens), c.ints(c.starts), static_cast<float*>(weights->data_ptr()),
+                                  static_cast<int>(q->size(0)), c.B, c.W, c.pages, c.kv, static_cast<int>(q->size(1) / c.kv), c.page_size, c.d,
+                                  static_cast<int>(window), scale, dtype_code(*q), ws.data_ptr(), ws.numel(), stream_of(dev));
+    }
+    if (rc != 0) return PyLong_FromLong(rc);
+    Py_RETURN_TRUE;
+  });
+}
+
+// (cache, weights, table, lens, keep, recent, into | None, workspaces) -> (lens, kept)
+PyObject* paged_cache_evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    DECLINE_UNLESS(n == 8);
+    PagedCall c;
+    DECLINE_UNLESS(paged_call(args[0], args[2], args[3], nullptr, &c));
+    const at::Tensor *weights = c.here(args[1], at::kFloat, {c.pages, c.kv, c.page_size}), *into;
+    int64_t keep, recent;
+    DECLINE_UNLESS(weights && get_int(args[4], &keep) && get_int(args[5], &recent) && keep > 0 && recent >= 0 && recent <= keep &&
+                   paged_into(args[6], c, &into));
+    const c10::DeviceIndex dev = c.k->device().index();
+    const at::Tensor ws = workspace_of(args[7], dev, ftb_workspace_bytes());
+    DECLINE_UNLESS(ws.defined());
+    at::Tensor now, kept;
+    int rc;
+    {
+      const WithoutGil released;
+      const c10::cuda::CUDAGuard guard(dev);
+      now = new_result(*c.lens, {c.B});
+      kept = new_result(*c.lens, {c.B, c.kv, keep});
+      rc = ftb_paged_cache_evict(c.k->data_ptr(), c.v->data_ptr(), c.bytes(c.k_exp), c.bytes(c.v_exp), static_cast<float*>(weights->data_ptr()),
+                                 c.ints(c.table), c.ints(c.lens), c.ints(into), static_cast<int*>(now.data_ptr()), static_cast<int*>(kept.data_ptr()),
+                                 c.B, c.W, into ? static_cast<int>(into->size(1)) : 0, static_cast<int>(keep), static_cast<int>(recent), c.pages, c.kv,
+                                 c.page_size, c.d, ws.data_ptr(), ws.numel(), stream_of(dev));
+    }
+    if (rc != 0) return PyLong_FromLong(rc);
+    return Py_BuildValue("(NN)", THPVariable_Wrap(now), THPVariable_Wrap(kept));
+  });
+}
+
 // (device index, -1: the current one) -> handle of its current stream.  (torch.cuda.current_stream makes a
 // stream object for it: 2 us, three times in a call of the word program.)
 PyObject* current_stream(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -611,6 +788,11 @@ PyMethodDef kMethods[] = {
     {"paged_cache_read", as_method(paged_cache_read), METH_FASTCALL, nullptr},
     {"paged_attention", as_method(paged_attention), METH_FASTCALL, nullptr},
     {"verify_drafts", as_method(verify_drafts), METH_FASTCALL, nullptr},
+    {"tree_mask", as_method(tree_mask), METH_FASTCALL, nullptr},
+    {"verify_tree", as_method(verify_tree), METH_FASTCALL, nullptr},
+    {"paged_cache_keep", as_method(paged_cache_keep), METH_FASTCALL, nullptr},
+    {"paged_attention_weights", as_method(paged_attention_weights), METH_FASTCALL, nullptr},
+    {"paged_cache_evict", as_method(paged_cache_evict), METH_FASTCALL, nullptr},
     {"current_stream", as_method(current_stream), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

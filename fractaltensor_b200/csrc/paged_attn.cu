@@ -35,7 +35,7 @@ struct Pieces {
 // Rows of whole tiles that have to be computed again: none, unless something in the cache is not finite, or dwarfs what is seen of its
 // 8-bit block.  `warp` of `warps` in the grid.  Those of a tile lie side by side: a warp looks at four times eight (a sector of flags) far
 // from each other.
-template <typename T, bool k8, int D>
+template <typename T, bool k8, int D, bool kMore>
 __device__ __forceinline__ void again_rows(const PagedAttn& a, long long warp, long long warps, int lane) {
   const int heads = a.kv_heads * a.group;
   const long long rows = static_cast<long long>(a.T) * heads;
@@ -49,14 +49,14 @@ __device__ __forceinline__ void again_rows(const PagedAttn& a, long long warp, l
       const int t = static_cast<int>(row / heads);
       const RowPlace at = place_of_row(a.batch, t, lane);
       if (at.b < a.batch.B)  // (what no sequence has was not written either)
-        attend_row<T, k8, D>(a, at.b, t, static_cast<int>(row - static_cast<long long>(t) * heads), at.pos, lane);
+        attend_row<T, k8, D, kMore>(a, at.b, t, static_cast<int>(row - static_cast<long long>(t) * heads), at.pos, lane);
     }
   }
 }
 
-// Row r of a cut tile by one warp, its numbers x over the weights' sum l, to the output.
-template <typename T, bool k8, int D>
-__device__ __forceinline__ void finish_row(const PagedAttn& a, const PagedCut& c, int r, float l, float (&x)[D / 32], int lane) {
+// Row r of a cut tile by one warp, its numbers x over the weights' sum l (of 2^(score - m)), to the output.
+template <typename T, bool k8, int D, bool kMore>
+__device__ __forceinline__ void finish_row(const PagedAttn& a, const PagedCut& c, int r, float m, float l, float (&x)[D / 32], int lane) {
   const int heads = a.kv_heads * a.group;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   float all = 0.f;
@@ -69,8 +69,9 @@ __device__ __forceinline__ void finish_row(const PagedAttn& a, const PagedCut& c
   uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(a.o) + (static_cast<long long>(t) * heads + head) * D) + lane * (D / 64);
 #pragma unroll
   for (int e = 0; e < D / 64; ++e) out[e] = Fmt<T>::pack2(x[2 * e], x[2 * e + 1]);
+  if (kMore && a.lse != nullptr && lane == 0) put_lse(a, static_cast<long long>(t) * heads + head, m, l);
   // (rows that something unseen may have made a NaN: key by key)
-  if (__any_sync(0xffffffffu, all != all) && hides(a, c.pos0 + t, c.lo, c.hi)) attend_row<T, k8, D>(a, c.b, t, head, c.pos0 + t, lane);
+  if (__any_sync(0xffffffffu, all != all) && hides<kMore>(a, c.pos0 + t, c.lo, c.hi)) attend_row<T, k8, D, kMore>(a, c.b, t, head, c.pos0 + t, lane);
 }
 
 // Parts first, first + by, .. of n of a row, added up: (m, l, x).
@@ -115,7 +116,7 @@ __device__ __forceinline__ void add_parts(Part part, int R, int r, int first, in
 // What the kernel for few rows leaves alone: block (x, y) takes row y of the tile with cut x, the parts spread over its warps: such
 // tiles may have hundreds, and what they cost are trips to memory one behind the other.
 constexpr int kFewWarps = 4;
-template <typename T, bool k8, int D>
+template <typename T, bool k8, int D, bool kMore>
 __global__ void __launch_bounds__(kFewWarps * 32)
 paged_join_few_kernel(const __grid_constant__ PagedAttn a, Pieces few) {
   __shared__ float s_sum[kFewWarps][D];
@@ -124,7 +125,7 @@ paged_join_few_kernel(const __grid_constant__ PagedAttn a, Pieces few) {
   grid_dependency_wait();
   grid_launch_dependents();
   const int last = few.cuts[cut].last;
-  again_rows<T, k8, D>(a, (static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x) * kFewWarps + warp,
+  again_rows<T, k8, D, kMore>(a, (static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x) * kFewWarps + warp,
                        static_cast<long long>(gridDim.x) * gridDim.y * kFewWarps, lane);
   if (last < 0) return;
   const PagedCut c = few.cuts[cut];
@@ -155,12 +156,12 @@ paged_join_few_kernel(const __grid_constant__ PagedAttn a, Pieces few) {
 #pragma unroll
     for (int e = 0; e < D / 32; ++e) x[e] = fmaf(s_sum[w][lane * (D / 32) + e], k, x[e]);
   }
-  finish_row<T, k8, D>(a, c, r, l, x, lane);
+  finish_row<T, k8, D, kMore>(a, c, r, top, l, x, lane);
 }
 
 // What both kernels leave.  Every block finds the cuts that have something to join, and the warps take the rows of those tiles in turn,
 // kJoinRows at a time, all on their way at once where there are two parts, as of most tiles of many rows.
-template <typename T, bool k8, int D>
+template <typename T, bool k8, int D, bool kMore>
 __global__ void __launch_bounds__(kJoinThreads, 3)
 paged_join_kernel(const __grid_constant__ PagedAttn a, Pieces few, Pieces many) {
   constexpr int kPer = D / 32;  // numbers of a row a lane
@@ -169,7 +170,7 @@ paged_join_kernel(const __grid_constant__ PagedAttn a, Pieces few, Pieces many) 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_dependency_wait();
   grid_launch_dependents();
-  again_rows<T, k8, D>(a, static_cast<long long>(blockIdx.x) * kJoinWarps + warp, static_cast<long long>(gridDim.x) * kJoinWarps, lane);
+  again_rows<T, k8, D, kMore>(a, static_cast<long long>(blockIdx.x) * kJoinWarps + warp, static_cast<long long>(gridDim.x) * kJoinWarps, lane);
   // turns of every cut, and how many lie in front of it
   const int cuts = few.pieces + many.pieces;
   {
@@ -235,31 +236,35 @@ paged_join_kernel(const __grid_constant__ PagedAttn a, Pieces few, Pieces many) 
         float x[kPer];
 #pragma unroll
         for (int e = 0; e < kPer; ++e) x[e] = reinterpret_cast<const float*>(&v[k][0])[e] * w0 + reinterpret_cast<const float*>(&v[k][1])[e] * w1;
-        finish_row<T, k8, D>(a, c, r0 + k, ml[k][0].y * w0 + ml[k][1].y * w1, x, lane);
+        finish_row<T, k8, D, kMore>(a, c, r0 + k, top, ml[k][0].y * w0 + ml[k][1].y * w1, x, lane);
       }
       continue;
     }
     for (int r = r0; r < min(r0 + kJoinRows, c.rows); ++r) {
       float m, l, x[kPer];
       add_parts<D>(part, R, r, 0, 1, n, lane, m, l, x);
-      finish_row<T, k8, D>(a, c, r, l, x, lane);
+      finish_row<T, k8, D, kMore>(a, c, r, m, l, x, lane);
     }
   }
 }
 
-template <typename T, bool k8, int D>
+template <typename T, bool k8, int D, bool kMore>
 int launch_join(const PagedAttn& a, const Pieces& few, const Pieces& many, cudaStream_t stream) {
   if (few.pieces + many.pieces > kMostCuts) return FTB_ERR_ARG;  // (a device of 256 SMs)
   static std::atomic<unsigned long long> divided{0}, divided_few{0};
-  if (!set_smem_carveout(paged_join_kernel<T, k8, D>, kPagedCarveout, divided) ||
-      !set_smem_carveout(paged_join_few_kernel<T, k8, D>, kPagedCarveout, divided_few))
+  if (!set_smem_carveout(paged_join_kernel<T, k8, D, kMore>, kPagedCarveout, divided) ||
+      !set_smem_carveout(paged_join_few_kernel<T, k8, D, kMore>, kPagedCarveout, divided_few))
     return FTB_ERR_LAUNCH;
   const cudaError_t err =
-      many.pieces == 0 ? launch_dependent(paged_join_few_kernel<T, k8, D>, dim3(few.pieces, few.rows), dim3(kFewWarps * 32), 0, stream, a, few)
-                       : launch_dependent(paged_join_kernel<T, k8, D>, dim3(3 * current_sm_count()), dim3(kJoinThreads), 0, stream, a, few, many);
+      many.pieces == 0 ? launch_dependent(paged_join_few_kernel<T, k8, D, kMore>, dim3(few.pieces, few.rows), dim3(kFewWarps * 32), 0, stream, a, few)
+                       : launch_dependent(paged_join_kernel<T, k8, D, kMore>, dim3(3 * current_sm_count()), dim3(kJoinThreads), 0, stream, a, few, many);
   count_launch();
   if (err != cudaSuccess) cudaGetLastError();
   return err == cudaSuccess ? FTB_OK : FTB_ERR_LAUNCH;
+}
+template <typename T, bool k8, int D>
+int launch_join(const PagedAttn& a, const Pieces& few, const Pieces& many, cudaStream_t stream) {
+  return a.more() ? launch_join<T, k8, D, true>(a, few, many, stream) : launch_join<T, k8, D, false>(a, few, many, stream);
 }
 template <typename T>
 int launch_join(const PagedAttn& a, int d, const Pieces& few, const Pieces& many, cudaStream_t stream) {
@@ -288,19 +293,6 @@ Form form_of(int T, int B, int group) {
   return {few, few, many};
 }
 
-// Whether n numbers at o (16 bits) meet the numbers of some of T rows of heads at q.
-bool over_rows(const void* o, long long n, const void* q, int T, long long q_row, int heads, long long q_head, int d) {
-  const long long span = (heads - 1) * q_head, lo = std::min(0ll, span), hi = std::max(0ll, span) + d;  // of a row
-  const long long step = T > 1 ? std::abs(q_row) : 0, first = T > 1 && q_row < 0 ? (T - 1) * q_row : 0;
-  // o's beginning, in numbers from where the lowest row is (both on 16-byte boundaries)
-  const long long at = static_cast<long long>(reinterpret_cast<uintptr_t>(o) - reinterpret_cast<uintptr_t>(q)) / 2 - first;
-  if (step == 0) return at < hi && at + n > lo;
-  // rows r with r * step + hi > at and r * step + lo < at + n
-  auto floor_div = [](long long x, long long y) { return x >= 0 ? x / y : -((-x + y - 1) / y); };
-  const long long r0 = std::max(0ll, floor_div(at - hi, step) + 1), r1 = std::min(T - 1ll, floor_div(at + n - lo - 1, step));
-  return r0 <= r1;
-}
-
 size_t places(int pieces, int rows, int d) { return 2 * static_cast<size_t>(pieces) * rows * (d + 2) * sizeof(float) + pieces * sizeof(PagedCut); }
 size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -322,7 +314,17 @@ extern "C" int ftb_paged_attn_fwd(const void* q, long long q_row, long long q_he
                                   const unsigned char* k_exp, const unsigned char* v_exp, const int* table, const int* lens,
                                   const int* starts, void* o, int T, int B, int W, int pages, int kv_heads, int group,
                                   int page_size, int d, int window, float scale, int dtype, void* scratch, size_t scratch_bytes,
-                                  void* workspace, size_t workspace_bytes, void* stream_) {
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  return ftb_paged_attn_tree_fwd(q, q_row, q_head, k_cache, v_cache, k_exp, v_exp, table, lens, starts, nullptr, 0, o, nullptr, T, B, W, pages,
+                                 kv_heads, group, page_size, d, window, scale, dtype, scratch, scratch_bytes, workspace, workspace_bytes, stream);
+}
+
+extern "C" int ftb_paged_attn_tree_fwd(const void* q, long long q_row, long long q_head, const void* k_cache, const void* v_cache,
+                                       const unsigned char* k_exp, const unsigned char* v_exp, const int* table, const int* lens,
+                                       const int* starts, const int* tree, int tree_words, void* o, float* lse, int T, int B, int W,
+                                       int pages, int kv_heads, int group, int page_size, int d, int window, float scale, int dtype,
+                                       void* scratch, size_t scratch_bytes, void* workspace, size_t workspace_bytes, void* stream_) {
+  if (tree_words < 0 || (tree != nullptr && (tree_words == 0 || window != 0))) return FTB_ERR_ARG;
   if ((T > 0 && (!q || !o)) || !k_cache || !v_cache || !table || !lens || !starts || (k_exp == nullptr) != (v_exp == nullptr)) return FTB_ERR_ARG;
   if (T < 0 || B <= 0 || W <= 0 || pages <= 0 || kv_heads <= 0 || group <= 0 || window < 0) return FTB_ERR_ARG;
   if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) return FTB_ERR_ARG;
@@ -342,6 +344,16 @@ extern "C" int ftb_paged_attn_fwd(const void* q, long long q_row, long long q_he
   if (over_rows(o, static_cast<long long>(o_bytes / 2), q, T, q_row, heads, q_head, d) || overlap(o, o_bytes, k_cache, cache_bytes) ||
       overlap(o, o_bytes, v_cache, cache_bytes) || overlap(o, o_bytes, k_exp, exp_bytes) || overlap(o, o_bytes, v_exp, exp_bytes))
     return FTB_ERR_ARG;
+  const size_t tree_bytes = tree != nullptr ? static_cast<size_t>(T) * tree_words * sizeof(int) : 0;
+  if (overlap(o, o_bytes, tree, tree_bytes)) return FTB_ERR_ARG;
+  if (lse != nullptr) {
+    const size_t lse_bytes = static_cast<size_t>(T) * heads * sizeof(float);
+    if ((reinterpret_cast<uintptr_t>(lse) & 15) != 0) return FTB_ERR_ALIGN;
+    if (over_rows(lse, static_cast<long long>(lse_bytes / 2), q, T, q_row, heads, q_head, d) || overlap(lse, lse_bytes, o, o_bytes) ||
+        overlap(lse, lse_bytes, k_cache, cache_bytes) || overlap(lse, lse_bytes, v_cache, cache_bytes) || overlap(lse, lse_bytes, k_exp, exp_bytes) ||
+        overlap(lse, lse_bytes, v_exp, exp_bytes) || overlap(lse, lse_bytes, tree, tree_bytes))
+      return FTB_ERR_ARG;
+  }
   const int rc = check_device_sm100();
   if (rc) return rc;
   PagedAttn a;
@@ -360,6 +372,9 @@ extern "C" int ftb_paged_attn_fwd(const void* q, long long q_row, long long q_he
   a.window = window;
   a.scale_log2 = scale * kLog2E;
   a.status = static_cast<int*>(workspace);
+  a.tree = reinterpret_cast<const uint32_t*>(tree);
+  a.tree_words = tree_words;
+  a.lse = lse;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (scratch == nullptr || scratch_bytes < ftb_paged_attn_scratch_bytes(T, B, kv_heads, group, d)) return FTB_ERR_WORKSPACE;
   if ((reinterpret_cast<uintptr_t>(scratch) & 15) != 0) return FTB_ERR_ALIGN;

@@ -17,7 +17,30 @@ struct PagedAttn {
   float scale_log2;
   int* status;
   uint32_t* odd;                   // [T, heads]: not 0 where a row of the output has to be computed again, key by key
+  const uint32_t* tree;            // [T, tree_words] or nullptr: bit j of a row's words: it sees new token j of its sequence
+  int tree_words;
+  float* lse;                      // [T, heads] or nullptr: log(sum(exp(scale * q . k))) of a row
+
+  bool more() const { return tree != nullptr || lse != nullptr; }
 };
+
+// kMore: kernels for calls with a tree or lse.  The others are compiled without (with both decided when they run, chunks took 586 us for
+// 558, 8-bit drafts 698 for 663, a decoding step 185.5 for 182.6: registers).
+
+// Word i of row t's bits.  What the mask has no word for, and what lies in front of the new tokens, is seen as far as positions go.
+__device__ __forceinline__ uint32_t tree_word(const PagedAttn& a, int t, long long i) {
+  return i < 0 || i >= a.tree_words ? 0xffffffffu : a.tree[static_cast<long long>(t) * a.tree_words + i];
+}
+// Whether row t sees new token j of its sequence (negative: a key in front of them), where the positions allow it.
+__device__ __forceinline__ bool in_tree(const PagedAttn& a, int t, long long j) {
+  return (tree_word(a, t, j >> 5) >> (j & 31) & 1u) != 0;
+}
+
+// A row's log(sum(exp)) from the sum of 2^(x - m) of its scores x in log2: -inf for a row that sees nothing.
+__device__ __forceinline__ void put_lse(const PagedAttn& a, long long row, float m, float sum) {
+  constexpr float kLn2 = 0.6931471805599453f;
+  a.lse[row] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
+}
 
 // 8 bits: values of 2^-30 to 2^30 times a code are ordinary, and maxima of scores with and without the values' exponents that are up to 2^40
 // apart: weights, which end at 2^-126, then reach down to 2^-48 of the largest, and the terms of the sum that divides up to 2^38.
@@ -26,8 +49,9 @@ constexpr float kNearTops = 40.f;
 
 // Whether a row at position pos of a tile that multiplies keys lo .. hi - 1 has some of them with weight 0 that it does not see: what
 // they hold could have made its result a NaN.
+template <bool kMore>
 __device__ __forceinline__ bool hides(const PagedAttn& a, long long pos, int lo, int hi) {
-  return pos + 1 < hi || (a.window > 0 && pos + 1 - a.window > lo);
+  return pos + 1 < hi || (a.window > 0 && pos + 1 - a.window > lo) || (kMore && a.tree != nullptr);
 }
 
 // The output of one (token, head) by one warp, key by key: nothing of a key that the token does not see has a part
@@ -35,7 +59,7 @@ __device__ __forceinline__ bool hides(const PagedAttn& a, long long pos, int lo,
 // keys at a time, which are of one page and on their way together.  For rows that the kernels' products have made a NaN through such keys.
 // It is for what should not happen: a row of 65 536 keys takes 9 ms (36 with a trip to memory for every key).  2048 tokens of 32 heads behind
 // 14 336 keys, 0.5 ms, take 36 ms with a NaN at the last position, which the last 64 tokens do not see, and 86 with one in their middle.
-template <typename T, bool k8, int D>
+template <typename T, bool k8, int D, bool kMore>
 __device__ __noinline__ void attend_row(const PagedAttn& a, int b, int t, int head, long long pos, int lane) {
   constexpr int kPer = D / 32, kBatch = 8;
   const int h = head / a.group;
@@ -68,6 +92,8 @@ __device__ __noinline__ void attend_row(const PagedAttn& a, int b, int t, int he
   };
   const long long end = min(pos + 1, static_cast<long long>(a.batch.W) << a.batch.page_shift);
   const long long begin = a.window > 0 ? max(0ll, pos + 1 - a.window) : 0;
+  const long long base = kMore && a.tree != nullptr ? pos - (t - max(0, a.batch.starts[b])) : end;  // of the sequence's new tokens
+  auto sees = [&](long long j) { return j >= begin && j < end && (!kMore || j < base || in_tree(a, t, j - base)); };
   float m = -FLT_MAX, l = 0.f;
   for (long long j0 = begin / kBatch * kBatch; j0 < end; j0 += kBatch) {
     const int page = max(0, page_of(a.batch, b, j0, a.status));
@@ -91,7 +117,7 @@ __device__ __noinline__ void attend_row(const PagedAttn& a, int b, int t, int he
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
       // (the scale behind the product: a query's number times it may be too small to keep all its bits)
-      s[i] = j0 + i >= begin && j0 + i < end ? s[i] * s_by[i] * a.scale_log2 : -INFINITY;
+      s[i] = sees(j0 + i) ? s[i] * s_by[i] * a.scale_log2 : -INFINITY;
       m_new = fmaxf(m_new, s[i]);
     }
     const float keep = exp2_fast(m - m_new);
@@ -101,7 +127,7 @@ __device__ __noinline__ void attend_row(const PagedAttn& a, int b, int t, int he
     for (int c = 0; c < kPer; ++c) acc[c] *= keep;
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const bool seen = j0 + i >= begin && j0 + i < end;
+      const bool seen = sees(j0 + i);
       const float p = seen ? exp2_fast(s[i] - m) : 0.f;
       l += p;
 #pragma unroll
@@ -112,6 +138,7 @@ __device__ __noinline__ void attend_row(const PagedAttn& a, int b, int t, int he
   uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(a.o) + (static_cast<long long>(t) * a.kv_heads * a.group + head) * D) + lane * (kPer / 2);
 #pragma unroll
   for (int c = 0; c < kPer / 2; ++c) out[c] = Fmt<T>::pack2(acc[2 * c] * inv, acc[2 * c + 1] * inv);
+  if (kMore && a.lse != nullptr && lane == 0) put_lse(a, static_cast<long long>(t) * a.kv_heads * a.group + head, m, l);
 }
 
 }  // namespace ftb

@@ -1,0 +1,388 @@
+// Which keys of a paged cache stay, and the moves of their rows.
+//
+// paged_choose: of a sequence of more than `keep` keys the last `recent` and, of those in front, the keep - recent with the largest
+// weights stay, of equal weights those in front; for each kv head on its own.  The weight of the last one that stays is found digit by digit
+// (radix selection on the weights' bits, put in the order of the numbers): a histogram of eight bits of what agrees with the digits
+// so far, four times, then the positions in their order by counts of what lies in front.
+//
+// paged_move: row first + kept[i] goes to first + i, i < counts, of keys, values, exponents and weights.  Into other pages every step of rows
+// is on its own.  In the same pages a chain of steps is one CTA's: kept ascends, so that kept[i] >= i, and what a step writes (up to
+// row i) is never read by a later one (kept[j] > kept[i] >= i); within a step all rows are read before one is written.  Chains run side
+// by side for the pieces of a row, which do not meet.
+#include <algorithm>
+#include <climits>
+
+#include "../../include/ftb200.h"
+#include "paged.cuh"
+#include "tmap.h"
+
+namespace ftb {
+namespace {
+
+// --------------------------------------------------------------------------------------------- choice
+struct Choose {
+  PagedBatch batch;
+  const float* weights;  // [pages, kv_heads, page_size]
+  int* kept;             // [B, kv_heads, keep]
+  int* lens_out;
+  int kv_heads, keep, recent;
+  int* status;
+};
+
+constexpr int kChooseThreads = 512, kChooseWarps = kChooseThreads / 32, kBins = 256, kCopies = 4;
+
+// Unsigned numbers in the order of the weights; NaN is below all of them.
+__device__ __forceinline__ uint32_t order_of(float w) {
+  const uint32_t u = __float_as_uint(w + 0.f);  // (-0 is 0)
+  if (w != w) return 0u;
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
+  int x;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(x) : "r"(addr) : "memory");
+  return x;
+}
+
+// C CTAs for each sequence and kv head, a stretch of the keys each.
+template <int C>
+__global__ void __launch_bounds__(kChooseThreads)
+paged_choose_kernel(const __grid_constant__ Choose a) {
+  __shared__ int bins[kCopies][kBins], sums[2][kBins], above_of[kChooseWarps], equal_of[kChooseWarps], mine[2];
+  __shared__ int s_digit, s_left;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rank = C > 1 ? static_cast<int>(cluster_ctarank()) : 0, head = blockIdx.x / C;
+  const int b = head / a.kv_heads, h = head - b * a.kv_heads;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const long long room = static_cast<long long>(a.batch.W) << a.batch.page_shift;
+  const int asked = max(0, a.batch.lens[b]), L = static_cast<int>(min(room, static_cast<long long>(asked)));
+  if (threadIdx.x == 0 && rank == 0 && h == 0) {
+    if (asked > L) atomicCAS(a.status, 0, FTB_ERR_INDEX);  // a table too narrow for the length
+    a.lens_out[b] = min(L, a.keep);
+  }
+  int* kept = a.kept + static_cast<long long>(head) * a.keep;
+  const int at = rank * kChooseThreads + threadIdx.x;
+  if (L <= a.keep) {
+    for (int i = at; i < a.keep; i += C * kChooseThreads) kept[i] = i < L ? i : -1;
+    return;
+  }
+  const int old = L - a.recent, want = a.keep - a.recent;  // 0 <= want < old
+  for (int i = at; i < a.recent; i += C * kChooseThreads) kept[want + i] = old + i;
+  if (want == 0) return;
+  const int* table = a.batch.table + static_cast<long long>(b) * a.batch.W;
+  const int shift = a.batch.page_shift, in_page = (1 << shift) - 1;
+  auto key_at = [&](int i) -> uint32_t {
+    const int page = __ldg(table + (i >> shift));
+    if (page < 0 || page >= a.batch.pages) {
+      atomicCAS(a.status, 0, FTB_ERR_INDEX);
+      return 0u;
+    }
+    return order_of(a.weights[(((static_cast<long long>(page) * a.kv_heads) + h) << shift) + (i & in_page)]);
+  };
+  // a warp's stretch: whole groups of 32
+  const int stretch = (old + C * kChooseThreads - 1) / (C * kChooseThreads) * 32;
+  const int from = static_cast<int>(min(static_cast<long long>(old), static_cast<long long>(rank * kChooseWarps + warp) * stretch));
+  const int to = static_cast<int>(min(static_cast<long long>(old), static_cast<long long>(from) + stretch));
+  uint32_t prefix = 0, known = 0;  // the digits so far, and which bits they are
+  int left = want;
+  for (int d = 0; d < 4; ++d) {
+    const int low = 24 - 8 * d;
+    for (int i = threadIdx.x; i < kCopies * kBins; i += kChooseThreads) (&bins[0][0])[i] = 0;
+    __syncthreads();
+    for (int i = from + lane; i < to; i += 32) {
+      const uint32_t key = key_at(i);
+      if ((key & known) == prefix) atomicAdd(&bins[warp % kCopies][key >> low & 255u], 1);
+    }
+    __syncthreads();
+    int* of_cta = sums[d & 1];  // (the other one may still be read by a CTA of the cluster)
+    if (threadIdx.x < kBins) {
+      int n = 0;
+#pragma unroll
+      for (int c = 0; c < kCopies; ++c) n += bins[c][threadIdx.x];
+      of_cta[threadIdx.x] = n;
+    }
+    if constexpr (C > 1) cluster_sync_all();
+    else __syncthreads();
+    if (warp == 0) {  // lane i: the eight bins from 255 - 8 i downwards
+      int n[8], sum = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int bin = 255 - (lane * 8 + k);
+        n[k] = 0;
+        if constexpr (C > 1) {
+#pragma unroll
+          for (int r = 0; r < C; ++r) n[k] += ld_cluster_s32(map_to_cta(smem_u32(&of_cta[bin]), r));
+        } else {
+          n[k] = of_cta[bin];
+        }
+        sum += n[k];
+      }
+      int upto = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+      }
+      int before = upto - sum;
+      if (before < left && upto >= left) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (before < left && before + n[k] >= left) {
+            s_digit = 255 - (lane * 8 + k);
+            s_left = left - before;
+          }
+          before += n[k];
+        }
+      }
+    }
+    __syncthreads();
+    prefix |= static_cast<uint32_t>(s_digit) << low;
+    known |= 255u << low;
+    left = s_left;
+  }
+  // what is above stays, of what is equal the first `left`
+  int above = 0, equal = 0;
+  for (int i = from + lane; i < to; i += 32) {
+    const uint32_t key = key_at(i);
+    above += key > prefix;
+    equal += key == prefix;
+  }
+  above = __reduce_add_sync(0xffffffffu, above);
+  equal = __reduce_add_sync(0xffffffffu, equal);
+  if (lane == 0) {
+    above_of[warp] = above;
+    equal_of[warp] = equal;
+  }
+  __syncthreads();
+  above = equal = 0;  // in front of this warp's stretch
+  int all_above = 0, all_equal = 0;
+#pragma unroll
+  for (int w = 0; w < kChooseWarps; ++w) {
+    if (w < warp) {
+      above += above_of[w];
+      equal += equal_of[w];
+    }
+    all_above += above_of[w];
+    all_equal += equal_of[w];
+  }
+  if constexpr (C > 1) {
+    if (threadIdx.x == 0) {
+      mine[0] = all_above;
+      mine[1] = all_equal;
+    }
+    cluster_sync_all();
+    for (int r = 0; r < rank; ++r) {
+      above += ld_cluster_s32(map_to_cta(smem_u32(&mine[0]), r));
+      equal += ld_cluster_s32(map_to_cta(smem_u32(&mine[1]), r));
+    }
+  }
+  for (int i0 = from; i0 < to; i0 += 32) {
+    const int i = i0 + lane;
+    const uint32_t key = i < to ? key_at(i) : 0u;
+    const unsigned is_above = __ballot_sync(0xffffffffu, i < to && key > prefix), is_equal = __ballot_sync(0xffffffffu, i < to && key == prefix);
+    const unsigned in_front = (1u << lane) - 1u;
+    const int equals = equal + __popc(is_equal & in_front);
+    if ((is_above >> lane & 1u) != 0 || ((is_equal >> lane & 1u) != 0 && equals < left))
+      kept[above + __popc(is_above & in_front) + min(left, equals)] = i;
+    above += __popc(is_above);
+    equal += __popc(is_equal);
+  }
+  if constexpr (C > 1) cluster_sync_all();  // nobody leaves while its counts may be read
+}
+
+// ---------------------------------------------------------------------------------------------- moves
+struct Move {
+  PagedBatch batch;       // of what is read
+  const int* into;        // the table of what is written, into_W wide
+  int into_W;
+  const int *kept, *counts, *first;  // first may be nullptr: 0
+  long long kept_seq, kept_head;     // distances in numbers
+  int most;               // rows of a sequence
+  int kv_heads;
+  unsigned char *k, *v, *k_exp, *v_exp;
+  float* weights;
+  int* status;
+};
+
+constexpr int kMoveThreads = 256, kMoveAtOnce = 8;
+
+// Rows of cache planes that a kept row comes from and goes to; -1: none.
+struct Rows {
+  long long from, to;
+};
+__device__ __forceinline__ Rows rows_of(const Move& a, int b, int h, long long first, const int* kept, int i) {
+  const int k = kept[i];
+  PagedBatch into = a.batch;
+  into.table = a.into;
+  into.W = a.into_W;
+  Rows r{-1, -1};
+  if (k < 0 || first < 0) {
+    atomicCAS(a.status, 0, FTB_ERR_INDEX);
+    return r;
+  }
+  const int shift = a.batch.page_shift, in_page = (1 << shift) - 1;
+  const long long src = first + k, dst = first + i;
+  if (src == dst && a.into == a.batch.table) return r;  // where it is
+  const int from = page_of(a.batch, b, src, a.status), to = page_of(into, b, dst, a.status);
+  if (from < 0 || to < 0) return r;
+  r.from = ((static_cast<long long>(from) * a.kv_heads + h) << shift) + (src & in_page);
+  r.to = ((static_cast<long long>(to) * a.kv_heads + h) << shift) + (dst & in_page);
+  return r;
+}
+
+// Block (x, y, z): sequence and kv head x, part y of a row, every gridDim.z-th step of rows.  kRow: 16-byte pieces of a key or value,
+// kOfPart: pieces of a part of both together; the last part, behind those, is exponents and weights.
+template <int kRow, int kOfPart>
+__global__ void __launch_bounds__(kMoveThreads)
+paged_move_kernel(const __grid_constant__ Move a, bool in_place) {
+  const int b = blockIdx.x / a.kv_heads, h = blockIdx.x - b * a.kv_heads, part = blockIdx.y;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int n = min(max(a.counts[b], 0), a.most);
+  const long long first = a.first != nullptr ? a.first[b] : 0;
+  const int* kept = a.kept + b * a.kept_seq + h * a.kept_head;
+  if (part < 2 * kRow / kOfPart) {
+    constexpr int kTogether = kMoveThreads / kOfPart, kStep = kTogether * kMoveAtOnce;
+    const int r = threadIdx.x / kOfPart, piece = part * kOfPart + threadIdx.x % kOfPart;
+    uint4* plane = reinterpret_cast<uint4*>(piece < kRow ? a.k : a.v) + (piece < kRow ? piece : piece - kRow);
+    for (int i0 = blockIdx.z * kStep; i0 < n; i0 += gridDim.z * kStep) {
+      Rows rows[kMoveAtOnce];
+      uint4 x[kMoveAtOnce];
+#pragma unroll
+      for (int u = 0; u < kMoveAtOnce; ++u) {
+        const int i = i0 + u * kTogether + r;
+        rows[u] = i < n ? rows_of(a, b, h, first, kept, i) : Rows{-1, -1};
+      }
+#pragma unroll
+      for (int u = 0; u < kMoveAtOnce; ++u)
+        if (rows[u].from >= 0) x[u] = plane[rows[u].from * kRow];
+      if (in_place) __syncthreads();
+#pragma unroll
+      for (int u = 0; u < kMoveAtOnce; ++u)
+        if (rows[u].from >= 0) plane[rows[u].to * kRow] = x[u];
+    }
+    return;
+  }
+  constexpr int kStep = kMoveThreads * kMoveAtOnce;
+  for (int i0 = blockIdx.z * kStep; i0 < n; i0 += gridDim.z * kStep) {
+    Rows rows[kMoveAtOnce];
+    unsigned char ke[kMoveAtOnce], ve[kMoveAtOnce];
+    float w[kMoveAtOnce];
+#pragma unroll
+    for (int u = 0; u < kMoveAtOnce; ++u) {
+      const int i = i0 + u * kMoveThreads + threadIdx.x;
+      rows[u] = i < n ? rows_of(a, b, h, first, kept, i) : Rows{-1, -1};
+      if (rows[u].from < 0) continue;
+      if (a.k_exp != nullptr) {
+        ke[u] = a.k_exp[rows[u].from];
+        ve[u] = a.v_exp[rows[u].from];
+      }
+      if (a.weights != nullptr) w[u] = a.weights[rows[u].from];
+    }
+    if (in_place) __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kMoveAtOnce; ++u) {
+      if (rows[u].from < 0) continue;
+      if (a.k_exp != nullptr) {
+        a.k_exp[rows[u].to] = ke[u];
+        a.v_exp[rows[u].to] = ve[u];
+      }
+      if (a.weights != nullptr) a.weights[rows[u].to] = w[u];
+    }
+  }
+}
+
+int launched(cudaError_t err) {
+  count_launch();
+  if (err != cudaSuccess) cudaGetLastError();
+  return err == cudaSuccess ? FTB_OK : FTB_ERR_LAUNCH;
+}
+
+template <int kRow, int kOfPart>
+int launch_move(const Move& a, int B, cudaStream_t stream) {
+  const bool in_place = a.into == a.batch.table;
+  const int parts = 2 * kRow / kOfPart + (a.k_exp != nullptr || a.weights != nullptr ? 1 : 0);
+  constexpr int kStep = kMoveThreads / kOfPart * kMoveAtOnce;
+  const long long heads = static_cast<long long>(B) * a.kv_heads;
+  const int steps = in_place ? 1 : static_cast<int>(std::min(static_cast<long long>((a.most + kStep - 1) / kStep), std::max(1ll, 65535ll)));
+  return launched(launch_light(paged_move_kernel<kRow, kOfPart>, dim3(static_cast<unsigned>(heads), parts, steps), dim3(kMoveThreads), 0, stream,
+                               a, in_place));
+}
+template <int kRow>
+int launch_move(const Move& a, int B, cudaStream_t stream) {
+  const long long heads = static_cast<long long>(B) * a.kv_heads;
+  // In the same pages a part of a row is a chain: narrow parts where there are few of them and long.
+  const bool in_place = a.into == a.batch.table;
+  if (in_place && a.most > 64 && heads * 8 <= 4ll * current_sm_count()) return launch_move<kRow, kRow / 4>(a, B, stream);
+  return launch_move<kRow, 2 * kRow>(a, B, stream);
+}
+int move(const Move& a, int row_bytes, int B, cudaStream_t stream) {
+  return row_bytes == 256 ? launch_move<16>(a, B, stream) : row_bytes == 128 ? launch_move<8>(a, B, stream) : launch_move<4>(a, B, stream);
+}
+
+// What both entry points ask of a cache: 0, or the reason for a refusal.
+int check_cache(const void* k, const void* v, const void* k_exp, const void* v_exp, const int* table, const int* into, int B, int W, int into_W,
+                int pages, int kv_heads, int page_size, int d) {
+  if (!k || !v || !table || (k_exp == nullptr) != (v_exp == nullptr)) return FTB_ERR_ARG;
+  if (B <= 0 || W <= 0 || (into != nullptr && into_W <= 0) || pages <= 0 || kv_heads <= 0 || kv_heads > 65536) return FTB_ERR_ARG;
+  if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) return FTB_ERR_ARG;
+  if ((d != 64 && d != 128) || static_cast<long long>(B) * kv_heads > INT_MAX / 8) return FTB_ERR_ARG;
+  if (((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(k_exp) | reinterpret_cast<uintptr_t>(v_exp)) & 15) != 0)
+    return FTB_ERR_ALIGN;
+  return FTB_OK;
+}
+
+}  // namespace
+}  // namespace ftb
+
+using namespace ftb;
+
+extern "C" int ftb_paged_cache_keep(void* k_cache, void* v_cache, unsigned char* k_exp, unsigned char* v_exp, float* weights,
+                                    const int* kept, long long kept_seq, long long kept_head, const int* counts, const int* first,
+                                    const int* table, const int* into, int B, int W, int into_W, int K, int pages, int kv_heads,
+                                    int page_size, int d, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_cache(k_cache, v_cache, k_exp, v_exp, table, into, B, W, into_W, pages, kv_heads, page_size, d);
+  if (rc) return rc;
+  if (K < 0 || (K > 0 && !kept) || !counts) return FTB_ERR_ARG;
+  if (workspace == nullptr || workspace_bytes < ftb_workspace_bytes()) return FTB_ERR_WORKSPACE;
+  if (K == 0) return FTB_OK;
+  if ((rc = check_device_sm100())) return rc;
+  const PagedBatch batch{table, nullptr, nullptr, B, W, pages, 31 - __builtin_clz(static_cast<unsigned>(page_size))};
+  const Move m{batch, into != nullptr ? into : table, into != nullptr ? into_W : W, kept, counts, first, kept_seq, kept_head, K, kv_heads,
+               static_cast<unsigned char*>(k_cache), static_cast<unsigned char*>(v_cache), k_exp, v_exp, weights, static_cast<int*>(workspace)};
+  return move(m, k_exp != nullptr ? d : 2 * d, B, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int ftb_paged_cache_evict(void* k_cache, void* v_cache, unsigned char* k_exp, unsigned char* v_exp, float* weights,
+                                     const int* table, const int* lens, const int* into, int* lens_out, int* kept, int B, int W, int into_W,
+                                     int keep, int recent, int pages, int kv_heads, int page_size, int d, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  int rc = check_cache(k_cache, v_cache, k_exp, v_exp, table, into, B, W, into_W, pages, kv_heads, page_size, d);
+  if (rc) return rc;
+  if (!weights || !lens || !lens_out || !kept || keep <= 0 || recent < 0 || recent > keep) return FTB_ERR_ARG;
+  if ((reinterpret_cast<uintptr_t>(weights) & 15) != 0) return FTB_ERR_ALIGN;
+  if (workspace == nullptr || workspace_bytes < ftb_workspace_bytes()) return FTB_ERR_WORKSPACE;
+  const size_t rows = static_cast<size_t>(pages) * kv_heads * page_size, row = k_exp != nullptr ? d : 2 * d;
+  const size_t kept_bytes = static_cast<size_t>(B) * kv_heads * keep * sizeof(int), lens_bytes = static_cast<size_t>(B) * sizeof(int);
+  if (overlap(kept, kept_bytes, lens_out, lens_bytes)) return FTB_ERR_ARG;
+  const void* out[2] = {kept, lens_out};
+  const size_t out_bytes[2] = {kept_bytes, lens_bytes};
+  for (int i = 0; i < 2; ++i)  // (the moves read what the choice has written; lens and table are read by all blocks)
+    if (overlap(out[i], out_bytes[i], k_cache, rows * row) || overlap(out[i], out_bytes[i], v_cache, rows * row) ||
+        (k_exp && (overlap(out[i], out_bytes[i], k_exp, rows) || overlap(out[i], out_bytes[i], v_exp, rows))) ||
+        overlap(out[i], out_bytes[i], weights, rows * sizeof(float)) || overlap(out[i], out_bytes[i], lens, lens_bytes) ||
+        overlap(out[i], out_bytes[i], table, lens_bytes * W) || (into && overlap(out[i], out_bytes[i], into, lens_bytes * into_W)))
+      return FTB_ERR_ARG;
+  if ((rc = check_device_sm100())) return rc;
+  const PagedBatch batch{table, lens, nullptr, B, W, pages, 31 - __builtin_clz(static_cast<unsigned>(page_size))};
+  int* status = static_cast<int*>(workspace);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const Choose c{batch, weights, kept, lens_out, kv_heads, keep, recent, status};
+  const unsigned heads = static_cast<unsigned>(B) * kv_heads;
+  rc = launched(launch_light(paged_choose_kernel<1>, dim3(heads), dim3(kChooseThreads), 0, s, c));
+  if (rc) return rc;
+  const Move m{batch, into != nullptr ? into : table, into != nullptr ? into_W : W, kept, lens_out, nullptr, static_cast<long long>(kv_heads) * keep,
+               keep, keep, kv_heads, static_cast<unsigned char*>(k_cache), static_cast<unsigned char*>(v_cache), k_exp, v_exp, weights, status};
+  return move(m, static_cast<int>(row), B, s);
+}

@@ -26,6 +26,7 @@
 #include <type_traits>
 
 #include "../../include/ftb200.h"
+#include "paged_query.cuh"
 #include "paged_work.cuh"
 #include "paged_forms.h"
 #include "tmap.h"
@@ -58,7 +59,7 @@ struct Merge {
 // tiles of two groups of warps that share the keys through L1, were slower than the tiles of paged_tile.cu by 2 to 4 times.)
 constexpr int blocks_per_sm(int nt) { return nt == 1 ? 3 : 2; }
 
-template <typename T, bool k8, int D, int NT>
+template <typename T, bool k8, int D, int NT, bool kMore>
 __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm(NT))
 paged_short_kernel(const __grid_constant__ PagedAttn a, float* __restrict__ parts, PagedCut* __restrict__ cuts) {
   using C = typename std::conditional<k8, __half, T>::type;
@@ -104,48 +105,7 @@ paged_short_kernel(const __grid_constant__ PagedAttn a, float* __restrict__ part
     int see_lo[NT][2], see_hi[NT][2];  // keys see_lo .. see_hi
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int row = nt * 8 + g;
-      const int flat = flat0 + row, token = flat / a.group;
-      const T* src = static_cast<const T*>(a.q) + static_cast<long long>(s.first + token) * a.q_row +
-                     static_cast<long long>(h * a.group + flat - token * a.group) * a.q_head;
-      uint4 x[D / 32];
-#pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
-        x[j] = make_uint4(0u, 0u, 0u, 0u);
-        const int d0 = k8 ? (j >> 1) * 64 + c * 16 + (j & 1) * 8 : j * 32 + c * 8;
-        if (row < rows) x[j] = *reinterpret_cast<const uint4*>(src + d0);
-      }
-      float mine = a.scale_log2;
-      if constexpr (k8 && !std::is_same<T, __half>::value) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-          const uint32_t w = __vmaxu2(__vmaxu2(x[j].x & 0x7fff7fffu, x[j].y & 0x7fff7fffu), __vmaxu2(x[j].z & 0x7fff7fffu, x[j].w & 0x7fff7fffu));
-          m = max(m, max(w & 0xffffu, w >> 16));
-        }
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        // the row times 2^(127 - e), e its largest number's exponent: that one is in [1, 2).  (A row that is not finite stays so.)
-        const int e = min(253, max(1, static_cast<int>(m >> 7)));
-        const float by = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
-        mine *= __uint_as_float(static_cast<uint32_t>(e) << 23);
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-          uint32_t* w = reinterpret_cast<uint32_t*>(&x[j]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = unpack2<T>(w[i]);
-            w[i] = Fmt<__half>::pack2(f.x * by, f.y * by);
-          }
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
-        q[nt][2 * j][0] = x[j].x;
-        q[nt][2 * j][1] = x[j].y;
-        q[nt][2 * j + 1][0] = x[j].z;
-        q[nt][2 * j + 1][1] = x[j].w;
-      }
+      const float mine = load_query<T, k8, D>(a, s.first, h, flat0, nt * 8 + g, rows, c, q[nt]);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         factor[nt][e] = __shfl_sync(0xffffffffu, mine, (2 * c + e) * 4);
@@ -158,6 +118,8 @@ paged_short_kernel(const __grid_constant__ PagedAttn a, float* __restrict__ part
     // chunks that every row sees whole need no mask: [all_lo, all_hi]
     int all_lo = 0, all_hi = static_cast<int>(max(-1ll, min(first_pos, static_cast<long long>(hi) - 1)));
     if (a.window > 0) all_lo = static_cast<int>(max(0ll, min(last_pos - a.window + 1, static_cast<long long>(INT_MAX))));
+    const long long base = s.pos0 + s.first;  // of the sequence's new tokens
+    if (kMore && a.tree != nullptr) all_hi = static_cast<int>(max(-1ll, min(base - 1, static_cast<long long>(all_hi))));
 
     float oacc[kSteps][NT][4], m[NT][2], l[NT][2];
     float near = kNear;  // 8 bits: l takes a chunk's weights where the values' exponents are below
@@ -294,6 +256,16 @@ paged_short_kernel(const __grid_constant__ PagedAttn a, float* __restrict__ part
             const int key = key0 + g + (i >> 1) * 8;
             if (key > see_hi[nt][i & 1] || key < see_lo[nt][i & 1]) sc[nt][i] = -INFINITY;
           }
+        if (kMore && a.tree != nullptr) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int r = nt * 8 + 2 * c + (i & 1);
+              const long long j = key0 + g + (i >> 1) * 8 - base;
+              if (j >= 0 && r < rows && !in_tree(a, s.first + (flat0 + r) / a.group, j)) sc[nt][i] = -INFINITY;
+            }
+        }
       }
       if constexpr (k8) {
         if (__any_sync(0xffffffffu, fmaxf(fabsf(add0), fabsf(add1)) > near)) {
@@ -477,6 +449,7 @@ paged_short_kernel(const __grid_constant__ PagedAttn a, float* __restrict__ part
         const int flat = flat0 + r, t = s.first + flat / a.group, head = h * a.group + flat % a.group;
         *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + (static_cast<long long>(t) * a.kv_heads * a.group + head) * D + d) =
             make_uint2(Fmt<T>::pack2(x.x, x.y), Fmt<T>::pack2(x.z, x.w));
+        if (kMore && a.lse != nullptr && d == 0) put_lse(a, static_cast<long long>(t) * a.kv_heads * a.group + head, top_n, sum);
       } else {
         *reinterpret_cast<float4*>(part + r * D + d) = x;
         if (d == 0) {
@@ -490,15 +463,15 @@ paged_short_kernel(const __grid_constant__ PagedAttn a, float* __restrict__ part
     if (threadIdx.x < rows) {
       const int flat = flat0 + threadIdx.x, t = s.first + flat / a.group;
       a.odd[static_cast<long long>(t) * a.kv_heads * a.group + h * a.group + flat % a.group] =
-          s_odd[threadIdx.x] != 0 && hides(a, s.pos0 + t, lo, hi) ? 1u : 0u;
+          s_odd[threadIdx.x] != 0 && hides<kMore>(a, s.pos0 + t, lo, hi) ? 1u : 0u;
     }
   }
 }
 
-template <typename T, bool k8, int D, int NT>
+template <typename T, bool k8, int D, int NT, bool kMore>
 int launch(const PagedAttn& a, void* scratch, cudaStream_t stream) {
   static std::atomic<unsigned long long> configured{0};
-  auto kfn = paged_short_kernel<T, k8, D, NT>;
+  auto kfn = paged_short_kernel<T, k8, D, NT, kMore>;
   constexpr int kSmem = sizeof(Merge<D, NT>);
   if (!ensure_dynamic_smem(kfn, kSmem, configured)) return FTB_ERR_LAUNCH;
   // No more shared memory than the blocks need: what is on its way to registers passes L1, which has the rest.  (Left to itself
@@ -513,6 +486,10 @@ int launch(const PagedAttn& a, void* scratch, cudaStream_t stream) {
   count_launch();
   if (err != cudaSuccess) cudaGetLastError();
   return err == cudaSuccess ? FTB_OK : FTB_ERR_LAUNCH;
+}
+template <typename T, bool k8, int D, int NT>
+int launch(const PagedAttn& a, void* scratch, cudaStream_t stream) {
+  return a.more() ? launch<T, k8, D, NT, true>(a, scratch, stream) : launch<T, k8, D, NT, false>(a, scratch, stream);
 }
 template <typename T, int D, int NT>
 int launch(const PagedAttn& a, void* scratch, cudaStream_t stream) {

@@ -60,7 +60,7 @@ struct Edge {  // values in ring slot `slot`, with its next fill's parity: of th
   uint32_t phase;
 };
 
-template <bool k8, bool kTwo>
+template <bool k8, bool kTwo, bool kMore>
 struct Control {
   PagedLineRoom line;
   Stretch ring[kStretches];
@@ -74,17 +74,18 @@ struct Control {
   // 8 bits: what `sum` refers to, and a thread's own: the sum of blocks apart and what it refers to (in registers: 646 for 628 us of drafts)
   float sum_top[k8 ? 2 : 1][k8 ? 128 : 1], apart_l[k8 ? 2 : 1][k8 ? 128 : 1], apart_n[k8 ? 2 : 1][k8 ? 128 : 1];
   int see_lo[2][128], see_hi[2][128];
+  uint32_t tree[kMore ? 2 : 1][4][kMore ? 128 : 1];  // [slot][word][row]: the bits of a block's keys, a thread's own
   int k_ref[kRefs], v_ref[kRefs];  // e_max of a block; + kFar: exponents more than kExact apart, in one that not every row sees all of
   uint32_t tmem_base;
   int abort, dead;
 };
 
-template <bool k8, int D, int R>
+template <bool k8, int D, int R, bool kMore>
 struct Plan {
   static constexpr bool kTwo = R == 256;
   static constexpr int kHalf = 128 * 128, kTile = D / 64 * kHalf;
   static constexpr int kQ = (kTwo ? 2 : 1) * kTile;
-  static constexpr int kControl = (sizeof(Control<k8, kTwo>) + 15) / 16 * 16, kRoom = 232448 - 1024 - kControl - kQ;
+  static constexpr int kControl = (sizeof(Control<k8, kTwo, kMore>) + 15) / 16 * 16, kRoom = 232448 - 1024 - kControl - kQ;
   static constexpr int kSlots = k8 ? (D == 128 ? 3 : 6) : kRoom / kTile < kMostSlots ? kRoom / kTile : kMostSlots;
   // 8-bit: a block's codes, and the exponents of its keys and values; as many on their way as there is room for
   static constexpr int kRaw = 128 * D + 256, kRawRoom = (kRoom - kSlots * kTile) / kRaw;
@@ -134,11 +135,11 @@ __device__ __forceinline__ Mine blocks_of_slot(const PagedAttn& a, const Stretch
   return {j0, j1, max(0, j1 - j0 + 1)};
 }
 
-template <typename T, bool k8, int D, int R>
-__global__ void __launch_bounds__(Plan<k8, D, R>::kThreads, 1)
+template <typename T, bool k8, int D, int R, bool kMore>
+__global__ void __launch_bounds__(Plan<k8, D, R, kMore>::kThreads, 1)
 paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
                   float* __restrict__ parts, PagedCut* __restrict__ cuts) {
-  using P = Plan<k8, D, R>;
+  using P = Plan<k8, D, R, kMore>;
   using C = typename std::conditional<k8, __half, T>::type;
   constexpr bool kTwo = P::kTwo;
   constexpr int kSlots = P::kSlots, kRawSlots = P::kRawSlots;
@@ -148,7 +149,8 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
   uint8_t* sQ = smem;
   uint8_t* sKV = sQ + P::kQ;
   uint8_t* sRaw = sKV + kSlots * P::kTile;
-  Control<k8, kTwo>& ctl = *reinterpret_cast<Control<k8, kTwo>*>(sRaw + kRawSlots * P::kRaw);
+  using Ctl = Control<k8, kTwo, kMore>;
+  Ctl& ctl = *reinterpret_cast<Ctl*>(sRaw + kRawSlots * P::kRaw);
   volatile int* s_abort = &ctl.abort;
   int* status = a.status;
 
@@ -528,13 +530,23 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
           const int key0 = (x.block0 + j) * kKeys;
           const int lo_col = ctl.see_lo[t][r] - key0, hi_col = ctl.see_hi[t][r] - key0;
           const bool cut = __any_sync(0xffffffffu, mine && (lo_col > 0 || hi_col < kKeys - 1));
+          const long long in_new = key0 - (x.pos0 + x.first);  // of the block's first key among the sequence's new tokens
+          const bool masked = kMore && a.tree != nullptr && in_new > -kKeys;
+          if (masked) {
+            place();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const long long j = in_new + 32 * i;
+              ctl.tree[t][i][r] = mine ? __funnelshift_r(tree_word(a, tok, j >> 5), tree_word(a, tok, (j >> 5) + 1), static_cast<uint32_t>(j & 31)) : 0u;
+            }
+          }
           float f = factor, add = 0.f, inv = 1.f;
           if constexpr (k8) {
             int kr = ctl.k_ref[(blocks0 + j) & (kRefs - 1)], vr = ctl.v_ref[(blocks0 + j) & (kRefs - 1)];
             if ((kr | vr) & kFar) {
               kr &= kFar - 1;
               vr &= kFar - 1;
-              if (lo_col > max(0, x.keys.lo - key0) || hi_col < min(kKeys, x.keys.hi - key0) - 1) factor = __uint_as_float(0x7fffffffu);
+              if (masked || lo_col > max(0, x.keys.lo - key0) || hi_col < min(kKeys, x.keys.hi - key0) - 1) factor = __uint_as_float(0x7fffffffu);
             }
             // (hidden scores are -inf already: times 0, as of a row of zeros and small keys, they would be NaN, as a score of 0 times
             // infinity.  No score moves: they are below 2^40 here.)
@@ -557,6 +569,16 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
 #pragma unroll
               for (int e = 0; e < kChunk; ++e)
                 if (e < lo || e > hi) s[e] = 0xff800000u;
+            }
+            if (masked) {
+              asm volatile("" ::: "memory");
+#pragma unroll
+              for (int i = 0; i < kChunk / 32; ++i) {
+                const uint32_t bits = ctl.tree[t][n * (kChunk / 32) + i][r];
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  if ((bits >> e & 1u) == 0) s[32 * i + e] = 0xff800000u;
+              }
             }
           };
           float mx = -INFINITY;
@@ -736,11 +758,12 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
         }
         // rows that something unseen may have made a NaN are left to the joining kernel, which goes through them key by key
         if (mine) {
-          const bool again = odd && x.whole && hides(a, x.pos0 + tok, x.keys.lo, x.keys.hi);
+          const bool again = odd && x.whole && hides<kMore>(a, x.pos0 + tok, x.keys.lo, x.keys.hi);
           using Flag = typename std::conditional<kCols == D, uint32_t, uint16_t>::type;
           reinterpret_cast<Flag*>(a.odd + static_cast<long long>(tok) * a.kv_heads * a.group + head)[c0 / kCols] = again ? 1 : 0;
         }
         if (mine && !x.whole && c0 == 0) *reinterpret_cast<float2*>(place_of + R * D + 2 * row) = make_float2(all_top, sum);
+        if (mine && x.whole && c0 == 0 && kMore && a.lse != nullptr) put_lse(a, static_cast<long long>(tok) * a.kv_heads * a.group + head, all_top, sum);
       }
       tc_fence_before();
       __syncwarp();
@@ -796,7 +819,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
       const Stretch& x = ctl.ring[i % kStretches];
       const int tiles = 2 * x.blocks;
       // keys that every row sees: up to the first one's position, from the last one's window on
-      const long long all_hi = x.pos0 + x.first + x.flat0 / a.group;
+      const long long all_hi = x.pos0 + x.first + (kMore && a.tree != nullptr ? -1 : x.flat0 / a.group);
       const long long all_lo = a.window > 0 ? x.pos0 + x.first + (x.flat0 + x.rows - 1) / a.group - a.window + 1 : 0;
       for (int n = (group - count) & (kGroups - 1); n < tiles && ok; n += kGroups) {
         const StreamTile y = stream_tile<kTwo>(n, x.blocks);
@@ -897,11 +920,11 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
   }
 }
 
-template <typename T, bool k8, int D, int R>
+template <typename T, bool k8, int D, int R, bool kMore>
 int launch(const PagedAttn& a, const CUtensorMap& mK, const CUtensorMap& mV, void* scratch, cudaStream_t stream) {
-  using P = Plan<k8, D, R>;
+  using P = Plan<k8, D, R, kMore>;
   static std::atomic<unsigned long long> configured{0};
-  auto kfn = paged_tile_kernel<T, k8, D, R>;
+  auto kfn = paged_tile_kernel<T, k8, D, R, kMore>;
   if (!ensure_dynamic_smem(kfn, P::kSmem, configured)) return FTB_ERR_LAUNCH;
   const int pieces = paged_tile_pieces();
   float* parts = static_cast<float*>(scratch);
@@ -910,6 +933,10 @@ int launch(const PagedAttn& a, const CUtensorMap& mK, const CUtensorMap& mV, voi
   count_launch();
   if (err != cudaSuccess) cudaGetLastError();
   return err == cudaSuccess ? FTB_OK : FTB_ERR_LAUNCH;
+}
+template <typename T, bool k8, int D, int R>
+int launch(const PagedAttn& a, const CUtensorMap& mK, const CUtensorMap& mV, void* scratch, cudaStream_t stream) {
+  return a.more() ? launch<T, k8, D, R, true>(a, mK, mV, scratch, stream) : launch<T, k8, D, R, false>(a, mK, mV, scratch, stream);
 }
 template <typename T, int D, int R>
 int launch(const PagedAttn& a, int dtype, void* scratch, cudaStream_t stream) {

@@ -1,0 +1,236 @@
+// What new tokens attend to, added up over a cache's keys: w_j += sum over tokens and heads of a kv head of exp(scale * q . k_j - lse), for
+// the keys that a token sees; a new token's own key begins at 0.  lse is log(sum(exp(scale * q . k))) of each row, from the attention in front.
+//
+// With the keys on the M side of the products, S^T = K Q^T (mma.m16n8k16), a key's sum is over a row of the result: each key belongs to
+// one warp, which goes through all rows (token, head of the group) that see it, in their order.  No two CTAs meet in a weight, and
+// the sums are the same from call to call.  Keys go from global memory straight into the registers that the products take them from, as in
+// paged_short.cu.  8-bit caches are taken as fp16, as there: a query row scaled into fp16's range by a power of two, a key's scale
+// 2^e to its scores.
+//
+// The work: blocks of 64 keys of a sequence and kv head, in a line that is cut into as many pieces as there are CTAs, a block counting
+// as often as there are tiles of rows.
+#include <cfloat>
+#include <climits>
+#include <type_traits>
+
+#include "../../include/ftb200.h"
+#include "paged_forms.h"
+#include "paged_query.cuh"
+#include "paged_work.cuh"
+#include "tmap.h"
+
+namespace ftb {
+namespace {
+
+constexpr float kLog2E = 1.4426950408889634f;
+constexpr int kWarps = 4, kBlockKeys = 16 * kWarps;
+static_assert(kWarps * 32 == kLineThreads, "the line is laid out by a block");
+
+struct Weigh {
+  PagedAttn attn;  // (without results)
+  float* weights;
+  const float* lse;
+};
+
+// Blocks of the keys that some row of a sequence sees, and the cost of one.
+__device__ __forceinline__ PagedKeys all_keys(const PagedAttn& a, const PagedSeq& s) {
+  return s.flats > 0 ? keys_of_rows(a, s.pos0, s.first, s.hi, 0, s.flats) : PagedKeys{0, 0};
+}
+__device__ __forceinline__ int blocks_of(const PagedKeys& k) {
+  return k.hi > k.lo ? (k.hi + kBlockKeys - 1) / kBlockKeys - k.lo / kBlockKeys : 0;
+}
+template <int R>
+__device__ __forceinline__ int cost_of(const PagedSeq& s) { return (s.flats + R - 1) / R; }
+
+template <typename T, bool k8, int D, int NT>
+__global__ void __launch_bounds__(kWarps * 32)
+paged_weigh_kernel(const __grid_constant__ Weigh x) {
+  using C = typename std::conditional<k8, __half, T>::type;
+  constexpr int R = NT * 8, kSteps = D / 16, kKLoads = k8 ? D / 64 : D / 32;
+  __shared__ PagedLineRoom s_line;
+  const PagedAttn& a = x.attn;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  int b;
+  long long at;
+  const PagedLine line = paged_line_of(a, blockIdx.x, gridDim.x, 1, s_line, &b, &at, [&](const PagedSeq& s) {
+    return static_cast<long long>(blocks_of(all_keys(a, s))) * cost_of<R>(s);
+  });
+  if (static_cast<int>(blockIdx.x) >= line.pieces || line.total == 0) return;
+  const long long begin = piece_begin(line, blockIdx.x), end = piece_begin(line, blockIdx.x + 1);
+  const int page_mask = (1 << a.batch.page_shift) - 1, heads = a.kv_heads * a.group;
+
+  // the sequence that unit `at` is in, and its blocks; a block is the piece's that its first unit is in
+  for (; b < a.batch.B && at < end; ++b) {
+    const PagedSeq s = paged_sequence(a, b);
+    const PagedKeys keys = all_keys(a, s);
+    const int blocks = blocks_of(keys), cost = cost_of<R>(s), first_block = keys.lo / kBlockKeys;
+    const long long all = static_cast<long long>(blocks) * a.kv_heads, before = at;
+    at += all * cost;
+    if (all == 0) continue;
+    const int* table = a.batch.table + static_cast<long long>(b) * a.batch.W;
+    const long long base = s.pos0 + s.first;  // of the new tokens
+    const long long n0 = begin > before ? (begin - before + cost - 1) / cost : 0;
+    for (long long n = n0; n < all && before + n * cost < end; ++n) {
+      const int h = static_cast<int>(n / blocks), key0 = (first_block + static_cast<int>(n - static_cast<long long>(h) * blocks)) * kBlockKeys + warp * 16;
+      if (key0 >= keys.hi || key0 + 16 <= keys.lo) continue;
+      int page = table[key0 >> a.batch.page_shift];
+      const bool there = page >= 0 && page < a.batch.pages;
+      if (!there) {
+        atomicCAS(a.status, 0, FTB_ERR_INDEX);
+        continue;
+      }
+      const long long row = ((static_cast<long long>(page) * a.kv_heads + h) << a.batch.page_shift) + (key0 & page_mask);
+      uint4 kf[2][kKLoads];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < kKLoads; ++j) kf[i][j] = *reinterpret_cast<const uint4*>(a.k + (row + g + 8 * i) * (k8 ? D : 2 * D) + j * 64 + c * 16);
+      float s0 = 1.f, s1 = 1.f;
+      if constexpr (k8) {
+        s0 = exponent_scale(a.k_exp[row + g]);
+        s1 = exponent_scale(a.k_exp[row + g + 8]);
+      }
+      float sum0 = 0.f, sum1 = 0.f;
+      for (int flat0 = 0; flat0 < s.flats; flat0 += R) {
+        const int rows = min(R, s.flats - flat0);
+        if (base + (flat0 + rows - 1) / a.group < key0) continue;                                   // in front of the keys
+        if (a.window > 0 && base + flat0 / a.group - a.window >= key0 + 15) continue;  // they have left the window
+        uint32_t q[NT][kSteps][2];
+        float factor[NT][2], minus[NT][2];
+        int see_lo[NT][2], see_hi[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float mine = load_query<T, k8, D>(a, s.first, h, flat0, nt * 8 + g, rows, c, q[nt]);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            factor[nt][e] = __shfl_sync(0xffffffffu, mine, (2 * c + e) * 4);
+            const int r = nt * 8 + 2 * c + e, flat = flat0 + r, token = flat / a.group;
+            float lse = INFINITY;
+            if (r < rows) lse = x.lse[static_cast<long long>(s.first + token) * heads + h * a.group + flat - token * a.group];
+            const bool fine = fabsf(lse) < INFINITY;  // (not of a row that sees nothing, or something that is not finite)
+            minus[nt][e] = -lse * kLog2E;
+            const long long pos = fine ? base + token : -1ll;
+            see_hi[nt][e] = static_cast<int>(max(-1ll, min(pos, static_cast<long long>(keys.hi) - 1)));
+            see_lo[nt][e] = a.window > 0 ? static_cast<int>(max(0ll, min(pos - a.window + 1, static_cast<long long>(INT_MAX)))) : 0;
+          }
+        }
+        float sc[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+#pragma unroll
+        for (int j = 0; j < kKLoads; ++j) {
+          const uint32_t w0[4] = {kf[0][j].x, kf[0][j].y, kf[0][j].z, kf[0][j].w}, w1[4] = {kf[1][j].x, kf[1][j].y, kf[1][j].z, kf[1][j].w};
+          if constexpr (k8) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t a0, a1, a2, a3;
+              e4m3x4_to_f16x2(w0[i], a0, a2);
+              e4m3x4_to_f16x2(w1[i], a1, a3);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma16816<C>(sc[nt], a0, a1, a2, a3, q[nt][4 * j + i][0], q[nt][4 * j + i][1]);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                mma16816<C>(sc[nt], w0[2 * i], w1[2 * i], w0[2 * i + 1], w1[2 * i + 1], q[nt][2 * j + i][0], q[nt][2 * j + i][1]);
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int e = i & 1, key = key0 + g + (i >> 1) * 8;
+            // (the scales of query and key meet before the score: either alone may lead out of fp32's range)
+            const float f = k8 ? fminf(factor[nt][e] * (i < 2 ? s0 : s1), FLT_MAX) : factor[nt][e];
+            const float p = key <= see_hi[nt][e] && key >= see_lo[nt][e] ? exp2_fast(fmaf(sc[nt][i], f, minus[nt][e])) : 0.f;
+            if (i < 2) sum0 += p;
+            else sum1 += p;
+          }
+      }
+      sum0 += __shfl_xor_sync(0xffffffffu, sum0, 1);
+      sum1 += __shfl_xor_sync(0xffffffffu, sum1, 1);
+      sum0 += __shfl_xor_sync(0xffffffffu, sum0, 2);
+      sum1 += __shfl_xor_sync(0xffffffffu, sum1, 2);
+      if (c < 2) {  // lane (g, 0) has key g, lane (g, 1) key g + 8
+        const int key = key0 + g + 8 * c;
+        if (key >= keys.lo && key < keys.hi) {
+          float* w = x.weights + row + g + 8 * c;
+          const float sum = c == 0 ? sum0 : sum1;
+          *w = key >= base ? sum : *w + sum;
+        }
+      }
+    }
+  }
+}
+
+template <typename T, bool k8, int D, int NT>
+int launch(const Weigh& x, cudaStream_t stream) {
+  const cudaError_t err = launch_dependent(paged_weigh_kernel<T, k8, D, NT>, dim3(current_sm_count() * 4), dim3(kWarps * 32), 0, stream, x);
+  count_launch();
+  if (err != cudaSuccess) cudaGetLastError();
+  return err == cudaSuccess ? FTB_OK : FTB_ERR_LAUNCH;
+}
+template <typename T, int D>
+int launch(const Weigh& x, int rows, cudaStream_t stream) {
+  if (x.attn.k_exp != nullptr) return rows == 8 ? launch<T, true, D, 1>(x, stream) : launch<T, true, D, 2>(x, stream);
+  return rows == 8 ? launch<T, false, D, 1>(x, stream) : launch<T, false, D, 2>(x, stream);
+}
+template <typename T>
+int launch(const Weigh& x, int d, int rows, cudaStream_t stream) {
+  return d == 128 ? launch<T, 128>(x, rows, stream) : launch<T, 64>(x, rows, stream);
+}
+
+}  // namespace
+}  // namespace ftb
+
+using namespace ftb;
+
+extern "C" int ftb_paged_attn_weights(const void* q, long long q_row, long long q_head, const void* k_cache, const unsigned char* k_exp,
+                                      const float* lse, const int* table, const int* lens, const int* starts, float* weights, int T, int B,
+                                      int W, int pages, int kv_heads, int group, int page_size, int d, int window, float scale, int dtype,
+                                      void* workspace, size_t workspace_bytes, void* stream) {
+  if ((T > 0 && (!q || !lse)) || !k_cache || !weights || !table || !lens || !starts) return FTB_ERR_ARG;
+  if (T < 0 || B <= 0 || W <= 0 || pages <= 0 || kv_heads <= 0 || group <= 0 || window < 0) return FTB_ERR_ARG;
+  if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) return FTB_ERR_ARG;
+  if ((d != 64 && d != 128) || (dtype != FTB_F16 && dtype != FTB_BF16)) return FTB_ERR_ARG;
+  if (!(scale > 0.f) || !(scale * kLog2E <= FLT_MAX)) return FTB_ERR_ARG;
+  if (static_cast<long long>(kv_heads) * group > 65536 || static_cast<long long>(T) * group > INT_MAX) return FTB_ERR_ARG;
+  if (((q_row | q_head) & 7) != 0) return FTB_ERR_ALIGN;
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(k_exp) |
+        reinterpret_cast<uintptr_t>(weights) | reinterpret_cast<uintptr_t>(lse)) & 15) != 0)
+    return FTB_ERR_ALIGN;
+  if (workspace == nullptr || workspace_bytes < ftb_workspace_bytes()) return FTB_ERR_WORKSPACE;
+  if (T == 0) return FTB_OK;
+  const int heads = kv_heads * group;
+  const size_t rows = static_cast<size_t>(pages) * kv_heads * page_size, bytes = rows * sizeof(float);
+  if (overlap(weights, bytes, k_cache, rows * d * (k_exp != nullptr ? 1 : 2)) || (k_exp != nullptr && overlap(weights, bytes, k_exp, rows)) ||
+      overlap(weights, bytes, lse, static_cast<size_t>(T) * heads * sizeof(float)) || over_rows(weights, static_cast<long long>(bytes / 2), q, T, q_row, heads, q_head, d))
+    return FTB_ERR_ARG;
+  const int rc = check_device_sm100();
+  if (rc) return rc;
+  Weigh x = {};
+  PagedAttn& a = x.attn;
+  a.batch = {table, lens, starts, B, W, pages, 31 - __builtin_clz(static_cast<unsigned>(page_size))};
+  a.q = q;
+  a.q_row = q_row;
+  a.q_head = q_head;
+  a.k = static_cast<const unsigned char*>(k_cache);
+  a.k_exp = k_exp;
+  a.T = T;
+  a.kv_heads = kv_heads;
+  a.group = group;
+  a.window = window;
+  a.least_rows = 1;
+  a.most_rows = INT_MAX;
+  a.scale_log2 = scale * kLog2E;
+  a.status = static_cast<int*>(workspace);
+  x.weights = weights;
+  x.lse = lse;
+  const int tile = static_cast<long long>(T) * group <= 8ll * B ? 8 : 16;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return dtype == FTB_F16 ? launch<__half>(x, d, tile, s) : launch<__nv_bfloat16>(x, d, tile, s);
+}

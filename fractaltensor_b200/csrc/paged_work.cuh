@@ -76,14 +76,15 @@ __device__ __forceinline__ long long piece_begin(const PagedLine& line, int g) {
 }
 
 // All threads of a block, kLineThreads or more: the line, and the sequence that the first unit of piece g belongs to (B: none)
-// with that sequence's beginning.  at_least: units of a piece where there are few.
-template <int R, int kUnitKeys>
-__device__ __forceinline__ PagedLine paged_line(const PagedAttn& a, int g, int most_pieces, int at_least, PagedLineRoom& room, int* seq, long long* begin) {
+// with that sequence's beginning.  at_least: units of a piece where there are few; of_head: units of one kv head of a sequence.
+template <typename OfHead>
+__device__ __forceinline__ PagedLine paged_line_of(const PagedAttn& a, int g, int most_pieces, int at_least, PagedLineRoom& room, int* seq, long long* begin,
+                                                   OfHead of_head) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (a.batch.B + kLineThreads - 1) / kLineThreads;
   const int b0 = min(a.batch.B, tid * per), b1 = tid < kLineThreads ? min(a.batch.B, b0 + per) : b0;
   long long mine = 0;
-  for (int b = b0; b < b1; ++b) mine += units_of_head<R, kUnitKeys>(a, paged_sequence(a, b)) * a.kv_heads;
+  for (int b = b0; b < b1; ++b) mine += of_head(paged_sequence(a, b)) * a.kv_heads;
   long long sum = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -109,7 +110,7 @@ __device__ __forceinline__ PagedLine paged_line(const PagedAttn& a, int g, int m
     long long at = before + sum - mine;
     if (u >= at && u < at + mine) {
       for (int b = b0; b < b1; ++b) {
-        const long long c = units_of_head<R, kUnitKeys>(a, paged_sequence(a, b)) * a.kv_heads;
+        const long long c = of_head(paged_sequence(a, b)) * a.kv_heads;
         if (u < at + c) {
           room.seq = b;
           room.begin = at;
@@ -123,6 +124,10 @@ __device__ __forceinline__ PagedLine paged_line(const PagedAttn& a, int g, int m
   *seq = room.seq;
   *begin = room.begin;
   return line;
+}
+template <int R, int kUnitKeys>
+__device__ __forceinline__ PagedLine paged_line(const PagedAttn& a, int g, int most_pieces, int at_least, PagedLineRoom& room, int* seq, long long* begin) {
+  return paged_line_of(a, g, most_pieces, at_least, room, seq, begin, [&](const PagedSeq& s) { return units_of_head<R, kUnitKeys>(a, s); });
 }
 
 // A stretch of a tile that a piece works on: units r0 .. r1 - 1 of its `units`.

@@ -15,13 +15,11 @@
 #include <climits>
 
 #include "../../include/ftb200.h"
-#include "ptx.cuh"
+#include "draft_draw.cuh"
 #include "tmap.h"
 
 namespace ftb {
 namespace {
-
-constexpr int kUnroll = 8;
 
 struct Drafts {
   const float* p;
@@ -33,38 +31,30 @@ struct Drafts {
   int K, V;
 };
 
-// What is not positive and finite counts as 0, in the target's rows and in the draft's.
-__device__ __forceinline__ double probability(float x) {
-  x = fmaxf(x, 0.f);  // (0 of a NaN)
-  return static_cast<double>(x < __int_as_float(0x7f800000) ? x : 0.f);
-}
+// What is left of p where q is taken from it, without one draft.
+struct DraftRow {
+  const float *pr, *qr;  // qr may be nullptr
+  int without;           // or -1
 
-__device__ __forceinline__ double weight_of(float p, float q, int j, int without) {
-  const double w = static_cast<double>(p) - probability(q);  // (nothing is left of a p that is not positive)
-  return w > 0.0 && p < __int_as_float(0x7f800000) && j != without ? w : 0.0;
-}
-
-__device__ __forceinline__ double warp_sum(double x) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  return x;
-}
-
-__device__ __forceinline__ double ld_cluster_f64(uint32_t addr) {
-  double x;
-  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(x) : "r"(addr) : "memory");
-  return x;
-}
+  __device__ __forceinline__ float p(int j) const { return pr[j]; }
+  __device__ __forceinline__ float q(int j) const { return qr != nullptr ? qr[j] : 0.f; }
+  __device__ __forceinline__ void look(int) const {}
+  __device__ __forceinline__ double weight(float p, float q, int j) const {
+    const double w = static_cast<double>(p) - probability(q);  // (nothing is left of a p that is not positive)
+    return w > 0.0 && p < __int_as_float(0x7f800000) && j != without ? w : 0.0;
+  }
+  __device__ __forceinline__ void all() {
+    qr = nullptr;
+    without = -1;
+  }
+};
 
 // C: CTAs of a cluster, 1 or 8.
 template <int C, int kThreads>
 __global__ void __launch_bounds__(kThreads, 1536 / kThreads)
 verify_drafts_kernel(Drafts a, long long* __restrict__ tokens, int* __restrict__ counts_out, int* __restrict__ status) {
-  constexpr int kWarps = kThreads / 32;
-  __shared__ double sums[kWarps], totals[2];  // of the warps; of this CTA (in the two tries)
-  __shared__ double s_total[C];
-  __shared__ int s_n, s_found, s_heavy;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ DrawRoom<C, kThreads> room;
+  __shared__ int s_n;
   const int b = blockIdx.x / C, rank = C > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   if (threadIdx.x == 0) s_n = a.K;
   __syncthreads();
@@ -91,145 +81,9 @@ verify_drafts_kernel(Drafts a, long long* __restrict__ tokens, int* __restrict__
   }
   __syncthreads();
   const int n = min(s_n, mine);
-  const float* pr = p + n * a.p_row;
-  const float* qr = q != nullptr && n < mine ? q + n * a.q_row : nullptr;
-  int without = q == nullptr && n < mine && x[n] >= 0 && x[n] < V ? static_cast<int>(x[n]) : -1;
-  // a warp's stretch of the row: whole groups of 32
-  const int stretch = ((V + C * kThreads - 1) / (C * kThreads)) * 32;
-  const int from = static_cast<int>(min(static_cast<long long>(V), static_cast<long long>(rank * kWarps + warp) * stretch)), to = min(V, from + stretch);
-  double total = 0.0, before = 0.0;  // of the row; of the CTAs in front of this one
-  for (int tries = 0; tries < 2; ++tries) {  // where p and q are the same, nothing is left of the difference: p itself
-    double s = 0.0;
-    for (int j = from; j < to; j += 32 * kUnroll) {
-      float pv[kUnroll], qv[kUnroll];
-#pragma unroll
-      for (int k = 0; k < kUnroll; ++k) {
-        const int at = j + k * 32 + lane;
-        pv[k] = at < to ? pr[at] : 0.f;
-        qv[k] = qr != nullptr && at < to ? qr[at] : 0.f;
-      }
-#pragma unroll
-      for (int k = 0; k < kUnroll; ++k) s += weight_of(pv[k], qv[k], j + k * 32 + lane, without);
-    }
-    s = warp_sum(s);
-    if (lane == 0) sums[warp] = s;
-    __syncthreads();
-    double cta = 0.0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) cta += sums[w];
-    if constexpr (C == 1) {
-      total = cta;
-      __syncthreads();
-    } else {
-      if (threadIdx.x == 0) totals[tries] = cta;
-      cluster_sync_all();
-      if (threadIdx.x < C) s_total[threadIdx.x] = ld_cluster_f64(map_to_cta(smem_u32(&totals[tries]), threadIdx.x));
-      __syncthreads();
-      total = before = 0.0;
-#pragma unroll
-      for (int r = 0; r < C; ++r) {
-        if (r < rank) before += s_total[r];
-        total += s_total[r];
-      }
-    }
-    if (total > 0.0) break;
-    qr = nullptr;
-    without = -1;
-  }
-  // The stretch in which the limit is passed: sums[] are this CTA's still.  (u of 1 or above, or sums that round down: the last
-  // stretch that weighs anything.)
-  const double limit = share * total;
-  // Which CTA has it follows from the CTAs' sums alone, the same in all of them.
-  const bool passed = total > limit;
-  bool past = false, own = C == 1;
-  if constexpr (C > 1) {
-    double at = 0.0;
-    int weighs = -1;
-#pragma unroll
-    for (int r = 0; r < C; ++r) {
-      at += s_total[r];
-      if (passed && !past && at > limit) {
-        past = true;
-        own = r == rank;
-      }
-      if (s_total[r] > 0.0) weighs = r;
-    }
-    if (!passed) own = weighs == rank;
-  }
-  int first = -1, last = -1;
-  double in_front = before, begin = before;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (first < 0 && begin + sums[w] > limit) {
-      first = w;
-      in_front = begin;
-    }
-    begin += sums[w];
-    if (sums[w] > 0.0) last = w;
-  }
-  const bool heaviest = !passed || first < 0;  // (sums that round differently: the last one too)
-  if (heaviest) first = last;
-  // That stretch again, by all warps of the CTA, kUnroll numbers side by side a lane: one scan over the warps' sums for
-  // kThreads * kUnroll of them.
-  if (own && total > 0.0) {  // of all CTAs, one
-    const int begin_at = static_cast<int>(min(static_cast<long long>(V), static_cast<long long>(rank * kWarps + first) * stretch)), end_at = min(V, begin_at + stretch);
-    int found = INT_MAX, heavy = -1;
-    double run = in_front;
-    for (int j0 = begin_at; j0 < end_at && found == INT_MAX; j0 += kThreads * kUnroll) {
-      const int j = j0 + static_cast<int>(threadIdx.x) * kUnroll;
-      double w[kUnroll], sum = 0.0;
-      float pv[kUnroll], qv[kUnroll];
-#pragma unroll
-      for (int k = 0; k < kUnroll; ++k) {
-        pv[k] = j + k < end_at ? pr[j + k] : 0.f;
-        qv[k] = qr != nullptr && j + k < end_at ? qr[j + k] : 0.f;
-      }
-#pragma unroll
-      for (int k = 0; k < kUnroll; ++k) {
-        w[k] = weight_of(pv[k], qv[k], j + k, without);
-        sum += w[k];
-      }
-      double ends = sum;  // sum of the warp's lanes up to this one
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double y = __shfl_up_sync(0xffffffffu, ends, o);
-        if (lane >= o) ends += y;
-      }
-      const double begins = __shfl_up_sync(0xffffffffu, ends, 1);
-      __syncthreads();  // (sums, s_found and s_heavy have been read)
-      if (lane == 31) sums[warp] = ends;
-      if (threadIdx.x == 0) {
-        s_found = INT_MAX;
-        s_heavy = -1;
-      }
-      __syncthreads();
-      double upto = run + (lane > 0 ? begins : 0.0);
-#pragma unroll
-      for (int v = 0; v < kWarps; ++v) {
-        if (v < warp) upto += sums[v];
-        run += sums[v];
-      }
-      int here_found = INT_MAX, here_heavy = -1;
-#pragma unroll
-      for (int k = 0; k < kUnroll; ++k) {
-        upto += w[k];
-        if (w[k] > 0.0) {
-          if (here_found == INT_MAX && !heaviest && upto > limit) here_found = j + k;
-          here_heavy = j + k;
-        }
-      }
-      here_found = __reduce_min_sync(0xffffffffu, here_found);
-      here_heavy = __reduce_max_sync(0xffffffffu, here_heavy);
-      if (lane == 0) {
-        if (here_found != INT_MAX) atomicMin(&s_found, here_found);
-        if (here_heavy >= 0) atomicMax(&s_heavy, here_heavy);
-      }
-      __syncthreads();
-      found = s_found;
-      if (s_heavy >= 0) heavy = s_heavy;
-    }
-    if (threadIdx.x == 0) tokens[static_cast<long long>(b) * (K + 1) + n] = found != INT_MAX ? found : heavy;
-  }
+  DraftRow row{p + n * a.p_row, q != nullptr && n < mine ? q + n * a.q_row : nullptr,
+               q == nullptr && n < mine && x[n] >= 0 && x[n] < V ? static_cast<int>(x[n]) : -1};
+  const double total = draw_token<C, kThreads>(row, V, share, rank, room, tokens + static_cast<long long>(b) * (K + 1) + n);
   if (rank == 0) {
     for (int i = threadIdx.x; i <= K; i += kThreads)
       if (i != n || !(total > 0.0)) tokens[static_cast<long long>(b) * (K + 1) + i] = i < n ? x[i] : -1;

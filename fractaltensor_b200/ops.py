@@ -687,8 +687,8 @@ def paged_cache(pages, kv_heads, page_size, d, dtype, device="cuda"):
     return tuple(t.view(dtype) for t in made) + tuple(torch.ones(rows, dtype=torch.uint8, device=device) for _ in range(2))
 
 
-def _paged_args(where, cache, table, lens, starts):
-    """Checks a cache and a batch's description -> (k, v, k_exp, v_exp, table, lens, starts as pointers, B, W, cache's shape)."""
+def _paged_cache_args(where, cache):
+    """Checks a cache -> (k, v, k_exp, v_exp as pointers)."""
     if not isinstance(cache, (tuple, list)) or len(cache) not in (2, 4):
         raise TypeError("%s: the cache is (k, v) or (k, v, k_exp, v_exp)" % where)
     k, v = cache[0], cache[1]
@@ -704,14 +704,23 @@ def _paged_args(where, cache, table, lens, starts):
         _req_like(e, "cache exponents", torch.uint8, k.shape[:3], k)
     if k.shape[2] not in (16, 32, 64, 128) or k.shape[3] not in (64, 128):
         raise ValueError("%s: page_size 16, 32, 64 or 128 and d 64 or 128 are supported, got %s and %s" % (where, k.shape[2], k.shape[3]))
-    _req(table, "table", torch.int32)
+    return [_ptr(k), _ptr(v)] + ([_ptr(e) for e in cache[2:]] or [0, 0])
+
+
+def _paged_table(where, table, k, name="table"):
+    _req(table, name, torch.int32)
     if table.dim() != 2 or 0 in table.shape or table.device != k.device:
         raise ValueError("%s: the table is [sequences, pages of one], on the cache's device" % where)
-    B, W = table.shape
+    return table.shape
+
+
+def _paged_args(where, cache, table, lens, starts):
+    """Checks a cache and a batch's description -> (k, v, k_exp, v_exp, table, lens, starts as pointers, B, W)."""
+    args, k = _paged_cache_args(where, cache), cache[0]
+    B, W = _paged_table(where, table, k)
     _req_like(lens, "lens", torch.int32, (B,), k)
     _req_like(starts, "starts", torch.int32, (B + 1,), k)
-    exps = [_ptr(e) for e in cache[2:]] or [0, 0]
-    return [_ptr(k), _ptr(v)] + exps + [_ptr(table), _ptr(lens), _ptr(starts)], B, W
+    return args + [_ptr(table), _ptr(lens), _ptr(starts)], B, W
 
 
 def _rows_of(t, name, dtype, like, heads=None):
@@ -793,16 +802,22 @@ def paged_cache_read(cache, table, lens, starts, rows, dtype=None, out=None):
     return tuple(out)
 
 
-def paged_attention(q, cache, table, lens, starts, scale=None, window=None, out=None):
+def paged_attention(q, cache, table, lens, starts, scale=None, window=None, out=None, tree=None, lse=None):
     """Attention of new tokens over a paged cache that holds their keys and values already (paged_cache_write).
 
     q: [T, heads, d], heads a multiple of the cache's kv_heads, rows as in paged_cache_write -> [T, heads, d]: for a token
     at position p softmax(scale * q . k_j) v over the keys j <= p, with `window` over p - window < j <= p only.  Tokens that see
-    nothing get zeros; rows that belong to no sequence are left as they were.  out overlaps neither q nor the cache."""
+    nothing get zeros; rows that belong to no sequence are left as they were.  out overlaps neither q nor the cache.
+
+    tree: int32 [T, words], the bits of the new tokens that a token sees (tree_mask): bit j % 32 of word j // 32 for new token j of
+    its sequence, counted from the sequence's first one.  All of them see the keys in front of the new tokens, none a token
+    behind its own place; tokens that the mask has no column for are seen as without it.  A tree has no window.
+    lse: fp32 [T, heads], takes log(sum(exp(scale * q . k_j))) over the keys that a row sees (paged_attention_weights)."""
+    where = "ftb_paged_attn_fwd" if tree is None and lse is None else "ftb_paged_attn_tree_fwd"
     done = host.paged_attention(q, cache, table, lens, starts, out, 1.0 if scale is None else scale, 0 if window is None else window or -1,
-                                _workspaces)
+                                tree, lse, _workspaces)
     if done is not None:
-        return _done(done, "ftb_paged_attn_fwd")
+        return _done(done, where)
     args, B, W = _paged_args("paged_attention", cache, table, lens, starts)
     kc = cache[0]
     pages, kv, page_size, d = kc.shape
@@ -815,14 +830,27 @@ def paged_attention(q, cache, table, lens, starts, scale=None, window=None, out=
     if out is None:
         out = torch.empty(T, heads, d, dtype=q.dtype, device=q.device)
     _req_like(out, "out", q.dtype, (T, heads, d), q)
+    words = 0
+    if tree is not None:
+        _req(tree, "tree", torch.int32)
+        if tree.dim() != 2 or tree.shape[0] != T or tree.shape[1] == 0 or tree.device != kc.device:
+            raise ValueError("paged_attention: the tree is [%d, words] on the cache's device, got %s on %s" % (T, tuple(tree.shape), tree.device))
+        if window is not None:
+            raise ValueError("paged_attention: a tree has no window")
+        words = tree.shape[1]
+    if lse is not None:
+        _req_like(lse, "lse", torch.float32, (T, heads), q)
     ws = workspace(kc.device)
     with _on(kc.device):
         # of the call's own: calls on other streams, and graphs replayed at the same time, have others
         n = lib.ftb_paged_attn_scratch_bytes(T, B, kv, heads // kv, d)
         scratch = torch.empty(n, dtype=torch.uint8, device=kc.device) if n else None
-        check(lib.ftb_paged_attn_fwd(qp, qr, qh, *args, _ptr(out), T, B, W, pages, kv, heads // kv, page_size, d,
-                                     min(int(window), 0x7fffffff) if window is not None else 0, 1.0 if scale is None else float(scale),
-                                     _dtype_code(q), _ptr(scratch), n, _ptr(ws), ws.numel(), _stream()), "ftb_paged_attn_fwd")
+        rest = (T, B, W, pages, kv, heads // kv, page_size, d, min(int(window), 0x7fffffff) if window is not None else 0,
+                1.0 if scale is None else float(scale), _dtype_code(q), _ptr(scratch), n, _ptr(ws), ws.numel(), _stream())
+        if tree is None and lse is None:
+            check(lib.ftb_paged_attn_fwd(qp, qr, qh, *args, _ptr(out), *rest), where)
+        else:
+            check(lib.ftb_paged_attn_tree_fwd(qp, qr, qh, *args, _ptr(tree), words, _ptr(out), _ptr(lse), *rest), where)
     return out
 
 
@@ -873,3 +901,154 @@ def verify_drafts(probs, drafts, u, draft_probs=None, counts=None):
                                     q.stride(1) if q is not None else 0, _ptr(drafts), _ptr(u), _ptr(counts), _ptr(tokens),
                                     _ptr(taken), B, K, V, _ptr(ws), ws.numel(), _stream()), "ftb_verify_drafts")
     return tokens, taken
+
+
+# ------------------------------------------------------------------------------- trees of drafted tokens, eviction
+def _tree_shape(where, parents):
+    _req(parents, "parents", torch.int32)
+    if parents.dim() != 2 or parents.shape[1] == 0:
+        raise ValueError("%s: parents must be [B, N], got %s" % (where, tuple(parents.shape)))
+    return parents.shape
+
+
+def tree_mask(parents):
+    """What the tokens of drafted trees see of each other: the `tree` of paged_attention.
+
+    parents: int32 [B, N], for each of a sequence's new tokens the one that it was drafted behind, which lies in front of it; anything else: none
+    -> int32 [B, N, ceil(N / 32)]: the bits of a token and of those on the way up from it."""
+    done = host.tree_mask(parents)
+    if done is not None:
+        return _done(done, "ftb_tree_mask")
+    B, N = _tree_shape("tree_mask", parents)
+    mask = torch.empty(B, N, (N + 31) // 32, dtype=torch.int32, device=parents.device)
+    with _on(parents.device):
+        check(lib.ftb_tree_mask(_ptr(parents), _ptr(mask), B, N, _stream()), "ftb_tree_mask")
+    return mask
+
+
+def verify_tree(probs, tokens, parents, u):
+    """Trees of drafted tokens against the target's probabilities, from random numbers of the caller's.
+
+    tokens: int64 [B, N], token 0 the last one that is certain; parents: int32 [B, N] as in tree_mask (a token without one is not
+    part of the tree); probs: fp32 [B, N, V], the target's behind each token; u: fp32 [B, N] in [0, 1).  From token 0
+    on: those drafted behind the last token of the path are asked in their order, and c is taken if u[c] * (1 - r) < p(x_c), r the
+    probability of those refused before it; where none is taken, u[0] draws a token from what is left.  This is a sample of the target's
+    probabilities whatever was drafted.  -> (int64 [B, N]: the path's tokens behind token 0, the drawn one, then -1; int32
+    [B, N]: the path, indices from 0 on, then -1 (`kept` of paged_cache_keep); int32 [B]: how many tokens, the path's length)."""
+    done = host.verify_tree(probs, tokens, parents, u, _workspaces)
+    if done is not None:
+        return _done(done, "ftb_verify_tree")
+    B, N = _tree_shape("verify_tree", parents)
+    if not isinstance(probs, torch.Tensor):
+        raise TypeError("probs must be a torch.Tensor")
+    if probs.dtype != torch.float32:
+        raise TypeError("probs must have dtype torch.float32, got %s" % probs.dtype)
+    if (probs.dim() != 3 or tuple(probs.shape[:2]) != (B, N) or probs.shape[2] == 0 or (probs.shape[2] != 1 and probs.stride(2) != 1) or
+            probs.device != parents.device):
+        raise ValueError("probs must be [%d, %d, V] with the numbers of a row side by side, on the parents' device, got %s" % (B, N, tuple(probs.shape)))
+    _req_like(tokens, "tokens", torch.int64, (B, N), parents)
+    _req_like(u, "u", torch.float32, (B, N), parents)
+    out = torch.empty(B, N, dtype=torch.int64, device=parents.device)
+    path = torch.empty(B, N, dtype=torch.int32, device=parents.device)
+    counts = torch.empty(B, dtype=torch.int32, device=parents.device)
+    ws = workspace(parents.device)
+    with _on(parents.device):
+        check(lib.ftb_verify_tree(_ptr(probs), probs.stride(0), probs.stride(1), _ptr(tokens), _ptr(parents), _ptr(u), _ptr(out), _ptr(path),
+                                  _ptr(counts), B, N, probs.shape[2], _ptr(ws), ws.numel(), _stream()), "ftb_verify_tree")
+    return out, path, counts
+
+
+def _paged_into(where, cache, table, into):
+    B, W = _paged_table(where, table, cache[0])
+    if into is None:
+        return B, W, 0
+    if _paged_table(where, into, cache[0], "into")[0] != B:
+        raise ValueError("%s: into has %d sequences, the table %d" % (where, into.shape[0], B))
+    return B, W, into.shape[1]
+
+
+def paged_cache_keep(cache, kept, counts, table, first=None, into=None, weights=None):
+    """Moves the rows of a cache that stay behind one another, as those of the accepted path of a tree.
+
+    kept: int32 [B, K], or [B, kv_heads, K] with a choice for each head, ascending; counts: int32 [B]; first: int32 [B] or None: 0.
+    Position first[b] + kept[b, i] of sequence b goes to first[b] + i, i < counts[b].  into: int32 [B, W2], pages to move to, none
+    of which this call reads, or None: the same ones (which belong to one sequence each).  weights (paged_attention_weights) move too.  Other
+    rows stay as they were."""
+    done = host.paged_cache_keep(cache, kept, counts, table, first, into, weights, _workspaces)
+    if done is not None:
+        _done(done, "ftb_paged_cache_keep")
+        return
+    args, k = _paged_cache_args("paged_cache_keep", cache), cache[0]
+    B, W, into_W = _paged_into("paged_cache_keep", cache, table, into)
+    pages, kv, page_size, d = k.shape
+    _req(kept, "kept", torch.int32)
+    if tuple(kept.shape[:-1]) not in ((B,), (B, kv)) or kept.device != k.device:
+        raise ValueError("paged_cache_keep: kept is [%d, K] or [%d, %d, K] on the cache's device, got %s" % (B, B, kv, tuple(kept.shape)))
+    _req_like(counts, "counts", torch.int32, (B,), k)
+    if first is not None:
+        _req_like(first, "first", torch.int32, (B,), k)
+    if weights is not None:
+        _req_like(weights, "weights", torch.float32, (pages, kv, page_size), k)
+    K = kept.shape[-1]
+    per_head = kept.dim() == 3
+    ws = workspace(k.device)
+    with _on(k.device):
+        check(lib.ftb_paged_cache_keep(*args, _ptr(weights), _ptr(kept), K * (kv if per_head else 1), K if per_head else 0, _ptr(counts), _ptr(first),
+                                       _ptr(table), _ptr(into), B, W, into_W, K, pages, kv, page_size, d, _ptr(ws), ws.numel(), _stream()),
+              "ftb_paged_cache_keep")
+
+
+def paged_attention_weights(q, cache, weights, lse, table, lens, starts, scale=None, window=None):
+    """Adds up what new tokens attend to: weights[key] += sum of exp(scale * q . k - lse) over the tokens that see the key and the
+    heads of its kv head's group; a new token's own key begins at 0.
+
+    weights: fp32 [pages, kv_heads, page_size], beside the cache's pages; lse: fp32 [T, heads], as paged_attention gave it for the same call
+    (rows whose lse is not finite add nothing); the others as there.  A page belongs to one sequence: a key's sum is one warp's."""
+    done = host.paged_attention_weights(q, cache, weights, lse, table, lens, starts, 1.0 if scale is None else scale,
+                                        0 if window is None else window or -1, _workspaces)
+    if done is not None:
+        _done(done, "ftb_paged_attn_weights")
+        return
+    args, B, W = _paged_args("paged_attention_weights", cache, table, lens, starts)
+    kc = cache[0]
+    pages, kv, page_size, d = kc.shape
+    qp, qr, qh = _rows_of(q, "q", None if len(cache) == 4 else kc.dtype, kc)
+    T, heads = q.shape[0], q.shape[1]
+    if heads == 0 or heads % kv:
+        raise ValueError("paged_attention_weights: %d heads are no multiple of the cache's %d" % (heads, kv))
+    if window is not None and window < 1:
+        raise ValueError("paged_attention_weights: a window holds one key or more, got %s" % window)
+    _req_like(weights, "weights", torch.float32, (pages, kv, page_size), kc)
+    _req_like(lse, "lse", torch.float32, (T, heads), kc)
+    ws = workspace(kc.device)
+    with _on(kc.device):
+        check(lib.ftb_paged_attn_weights(qp, qr, qh, args[0], args[2], _ptr(lse), *args[4:], _ptr(weights), T, B, W, pages, kv, heads // kv, page_size,
+                                         d, min(int(window), 0x7fffffff) if window is not None else 0, 1.0 if scale is None else float(scale),
+                                         _dtype_code(q), _ptr(ws), ws.numel(), _stream()), "ftb_paged_attn_weights")
+
+
+def paged_cache_evict(cache, weights, table, lens, keep, recent=0, into=None):
+    """Evicts from sequences of more than `keep` keys, for each kv head, all but the last `recent` ones and the keep - recent of the
+    largest weights in front of them (of equal ones the first; NaN is below all numbers).
+
+    What stays is moved to positions 0, 1, .. in its order, with its weights: in its own pages, or into those of `into` (as in
+    paged_cache_keep, and shorter sequences as they are).  -> (int32 [B]: the lengths, min(lens, keep); int32 [B, kv_heads, keep]: the
+    positions that stayed, then -1)."""
+    done = host.paged_cache_evict(cache, weights, table, lens, keep, recent, into, _workspaces)
+    if done is not None:
+        return _done(done, "ftb_paged_cache_evict")
+    args, k = _paged_cache_args("paged_cache_evict", cache), cache[0]
+    B, W, into_W = _paged_into("paged_cache_evict", cache, table, into)
+    pages, kv, page_size, d = k.shape
+    _req_like(weights, "weights", torch.float32, (pages, kv, page_size), k)
+    _req_like(lens, "lens", torch.int32, (B,), k)
+    keep, recent = int(keep), int(recent)
+    if not 0 <= recent <= keep or not 0 < keep <= 0x7fffffff:
+        raise ValueError("paged_cache_evict: keep is 1 or more and recent 0 to keep, got %d and %d" % (keep, recent))
+    now = torch.empty(B, dtype=torch.int32, device=k.device)
+    kept = torch.empty(B, kv, keep, dtype=torch.int32, device=k.device)
+    ws = workspace(k.device)
+    with _on(k.device):
+        check(lib.ftb_paged_cache_evict(*args, _ptr(weights), _ptr(table), _ptr(lens), _ptr(into), _ptr(now), _ptr(kept), B, W, into_W, keep, recent,
+                                        pages, kv, page_size, d, _ptr(ws), ws.numel(), _stream()), "ftb_paged_cache_evict")
+    return now, kept

@@ -443,6 +443,17 @@ int ftb_paged_attn_fwd(const void* q, long long q_row, long long q_head, const v
                        int d, int window, float scale, int dtype, void* scratch, size_t scratch_bytes, void* workspace,
                        size_t workspace_bytes, void* stream);
 
+/* The same for trees of drafted tokens, and with the sums that the softmax divides by.  tree: int32 [T, tree_words] or NULL: bit j
+ * (bit j % 32 of word j / 32) of a row is 1 if the token sees new token j of its sequence, counted from the sequence's first new one.
+ * The keys in front of the new tokens are seen by all of them, a new one behind a token's own place by none; new tokens that the mask has no
+ * column for are seen as without it.  A tree has no window.  ftb_tree_mask makes such a mask.  lse: fp32 [T, kv_heads * group], 16-byte
+ * aligned, or NULL: log(sum(exp(scale * q . k))) over the keys that a row sees, -inf where it sees none; it overlaps nothing that is read or written. */
+int ftb_paged_attn_tree_fwd(const void* q, long long q_row, long long q_head, const void* k_cache, const void* v_cache,
+                            const unsigned char* k_exp, const unsigned char* v_exp, const int* table, const int* lens,
+                            const int* starts, const int* tree, int tree_words, void* o, float* lse, int T, int B, int W,
+                            int pages, int kv_heads, int group, int page_size, int d, int window, float scale, int dtype,
+                            void* scratch, size_t scratch_bytes, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Drafted tokens against the target's probabilities, from random numbers that the caller gives.  probs: fp32, for each of B
  * sequences K + 1 rows of V (up to 2^30) probabilities (`p_seq` and `p_row` numbers apart; ftb_project_softmax_fwd gives such rows);
  * draft_probs: fp32, K rows that the drafts were drawn from, or NULL: each draft was certain; drafts: int64 [B, K]; u: fp32
@@ -455,6 +466,56 @@ int ftb_paged_attn_fwd(const void* q, long long q_row, long long q_head, const v
 int ftb_verify_drafts(const float* probs, long long p_seq, long long p_row, const float* draft_probs, long long q_seq,
                       long long q_row, const long long* drafts, const float* u, const int* counts, long long* tokens,
                       int* counts_out, int B, int K, int V, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Trees of drafted tokens: N tokens of each of B sequences, token 0 the last one that is certain, the others drafted; parents: int32
+ * [B, N], the token that each was drafted behind, 0 <= parents[i] < i (anything else: none, the token is not part of the tree;
+ * parents[0] is not looked at by ftb_verify_tree).
+ * ftb_tree_mask: mask int32 [B, N, (N + 31) / 32]: bit j of token i is 1 if j is i or lies on the way from i up through the parents.
+ * ftb_verify_tree: probs fp32, for each sequence N rows of V (up to 2^30) probabilities, row i behind token i (`p_seq` and `p_row` numbers
+ * apart); tokens int64 [B, N]; u fp32 [B, N] in [0, 1); N up to 1024.  The path begins at token 0.  The tokens drafted behind the one
+ * that it has come to are asked in their order: with r the sum of the row's probabilities of those refused before, token c is taken if u_c *
+ * (1 - r) < p(x_c), and the path goes on from it; a token that has been refused before counts as 0.  Where none is taken a token is drawn:
+ * the first j with w_0 + .. + w_j > u_0 * sum(w), w the row without those refused (the row itself where nothing is left).  Results: path
+ * int32 [B, N], the tokens of the path from 0 on, then -1; counts_out int32 [B], how many; tokens_out int64 [B, N]: the path's tokens
+ * behind token 0, the drawn one, then -1.  Sums in 64 bits.  Probabilities that are not positive and finite count as 0; a row without
+ * any gives -1 and, as a drafted token outside [0, V), which is not taken, sets the (sticky) status word to 22.  No two results, and no
+ * result and tokens, parents or u, overlap. */
+int ftb_tree_mask(const int* parents, int* mask, int B, int N, void* stream);
+int ftb_verify_tree(const float* probs, long long p_seq, long long p_row, const long long* tokens, const int* parents,
+                    const float* u, long long* tokens_out, int* path, int* counts_out, int B, int N, int V, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
+/* Rows of a paged cache that stay, one behind the other: position first[b] + kept[b, h, i] of sequence b and kv head h goes to position
+ * first[b] + i, i < counts[b] (cut to 0 .. K).  kept: int32, rows of K numbers that ascend, `kept_seq` and `kept_head` numbers apart
+ * (`kept_head` 0: the same for all heads); first: int32 [B] or NULL: 0.  table [B, W]: the pages that rows come from; into [B, into_W]: the
+ * pages that they go to, none of which this call reads, or NULL (or table itself): the same pages, which belong to one sequence each.
+ * Keys, values, exponents and, if not NULL, weights (fp32 [pages, kv_heads, page_size]) move together.  All other rows stay as they
+ * were.  A row whose page one of the tables does not have, or with a negative number in kept, is not moved and sets the
+ * (sticky) status word to 22. */
+int ftb_paged_cache_keep(void* k_cache, void* v_cache, unsigned char* k_exp, unsigned char* v_exp, float* weights,
+                         const int* kept, long long kept_seq, long long kept_head, const int* counts, const int* first,
+                         const int* table, const int* into, int B, int W, int into_W, int K, int pages, int kv_heads,
+                         int page_size, int d, void* workspace, size_t workspace_bytes, void* stream);
+
+/* What new tokens attend to: weights[j] += sum of exp(scale * q . k_j - lse) over the tokens that see key j and the heads of its kv head's
+ * group; the sum alone where j is a new token's own place.  weights: fp32 [pages, kv_heads, page_size]; lse: fp32
+ * [T, kv_heads * group], of ftb_paged_attn_tree_fwd for the same call (a row whose lse is not finite adds nothing).  Each weight is the sum of
+ * the rows in their order, without atomics: a page belongs to one sequence.  A key whose page the table does not have gets
+ * nothing and sets the (sticky) status word to 22. */
+int ftb_paged_attn_weights(const void* q, long long q_row, long long q_head, const void* k_cache, const unsigned char* k_exp,
+                           const float* lse, const int* table, const int* lens, const int* starts, float* weights, int T,
+                           int B, int W, int pages, int kv_heads, int group, int page_size, int d, int window, float scale,
+                           int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Eviction: of a sequence of lens[b] > keep keys, for each kv head, the last `recent` (0 .. keep) stay and, of those in front of
+ * them, the keep - recent with the largest weights, of equal weights those in front (NaN is below all numbers).  What stays is moved as by
+ * ftb_paged_cache_keep, weights too; shorter sequences stay whole.  lens_out int32 [B]: min(lens[b], keep); kept int32
+ * [B, kv_heads, keep]: the positions that stay, ascending, then -1.  A length that the table is too narrow for is cut and sets the (sticky)
+ * status word to 22. */
+int ftb_paged_cache_evict(void* k_cache, void* v_cache, unsigned char* k_exp, unsigned char* v_exp, float* weights,
+                          const int* table, const int* lens, const int* into, int* lens_out, int* kept, int B, int W,
+                          int into_W, int keep, int recent, int pages, int kv_heads, int page_size, int d, void* workspace,
+                          size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
