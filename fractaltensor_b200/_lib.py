@@ -77,7 +77,8 @@ SIGNATURES = {
     "ftb_tree_mask": (_i, [_vp, _vp, _i, _i, _vp]),
     "ftb_verify_tree": (_i, [_vp, ctypes.c_longlong, ctypes.c_longlong] + [_vp] * 6 + [_i] * 3 + [_vp, _sz, _vp]),
     "ftb_paged_cache_keep": (_i, [_vp] * 6 + [ctypes.c_longlong, ctypes.c_longlong] + [_vp] * 4 + [_i] * 8 + [_vp, _sz, _vp]),
-    "ftb_paged_attn_weights": (_i, [_vp, ctypes.c_longlong, ctypes.c_longlong] + [_vp] * 7 + [_i] * 9 + [_f, _i, _vp, _sz, _vp]),
+    "ftb_paged_attn_weights_scratch_bytes": (_sz, [_i] * 5),
+    "ftb_paged_attn_weights": (_i, [_vp, ctypes.c_longlong, ctypes.c_longlong] + [_vp] * 7 + [_i] * 9 + [_f, _i, _vp, _sz, _vp, _sz, _vp]),
     "ftb_paged_cache_evict": (_i, [_vp] * 10 + [_i] * 9 + [_vp, _sz, _vp]),
     "ftb_gemm_nt": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, ctypes.POINTER(_i), _vp, _sz, _vp]),
 }

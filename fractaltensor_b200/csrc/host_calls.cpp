@@ -717,10 +717,14 @@ PyObject* paged_attention_weights(PyObject*, PyObject* const* args, Py_ssize_t n
     {
       const WithoutGil released;
       const c10::cuda::CUDAGuard guard(dev);
+      const size_t bytes = ftb_paged_attn_weights_scratch_bytes(static_cast<int>(q->size(0)), c.B, c.kv, static_cast<int>(q->size(1) / c.kv), c.d);
+      at::Tensor scratch;
+      if (bytes > 0) scratch = at::empty({static_cast<int64_t>(bytes)}, at::TensorOptions().dtype(at::kByte).device(q->device()));
       rc = ftb_paged_attn_weights(q->data_ptr(), qr, qh, c.k->data_ptr(), c.exps(c.k_exp), static_cast<const float*>(lse->data_ptr()),
                                   c.ints(c.table), c.ints(c.lens), c.ints(c.starts), static_cast<float*>(weights->data_ptr()),
                                   static_cast<int>(q->size(0)), c.B, c.W, c.pages, c.kv, static_cast<int>(q->size(1) / c.kv), c.page_size, c.d,
-                                  static_cast<int>(window), scale, dtype_code(*q), ws.data_ptr(), ws.numel(), stream_of(dev));
+                                  static_cast<int>(window), scale, dtype_code(*q), bytes > 0 ? scratch.data_ptr() : nullptr, bytes, ws.data_ptr(),
+                                  ws.numel(), stream_of(dev));
     }
     if (rc != 0) return PyLong_FromLong(rc);
     Py_RETURN_TRUE;

@@ -16,7 +16,7 @@
 #include "../../include/ftb200.h"
 #include "paged_forms.h"
 #include "paged_query.cuh"
-#include "paged_work.cuh"
+#include "paged_weigh.cuh"
 #include "tmap.h"
 
 namespace ftb {
@@ -26,19 +26,7 @@ constexpr float kLog2E = 1.4426950408889634f;
 constexpr int kWarps = 4, kBlockKeys = 16 * kWarps;
 static_assert(kWarps * 32 == kLineThreads, "the line is laid out by a block");
 
-struct Weigh {
-  PagedAttn attn;  // (without results)
-  float* weights;
-  const float* lse;
-};
-
-// Blocks of the keys that some row of a sequence sees, and the cost of one.
-__device__ __forceinline__ PagedKeys all_keys(const PagedAttn& a, const PagedSeq& s) {
-  return s.flats > 0 ? keys_of_rows(a, s.pos0, s.first, s.hi, 0, s.flats) : PagedKeys{0, 0};
-}
-__device__ __forceinline__ int blocks_of(const PagedKeys& k) {
-  return k.hi > k.lo ? (k.hi + kBlockKeys - 1) / kBlockKeys - k.lo / kBlockKeys : 0;
-}
+// What a block of a sequence counts as.
 template <int R>
 __device__ __forceinline__ int cost_of(const PagedSeq& s) { return (s.flats + R - 1) / R; }
 
@@ -55,7 +43,7 @@ paged_weigh_kernel(const __grid_constant__ Weigh x) {
   int b;
   long long at;
   const PagedLine line = paged_line_of(a, blockIdx.x, gridDim.x, 1, s_line, &b, &at, [&](const PagedSeq& s) {
-    return static_cast<long long>(blocks_of(all_keys(a, s))) * cost_of<R>(s);
+    return static_cast<long long>(blocks_of<kBlockKeys>(all_keys(a, s))) * cost_of<R>(s);
   });
   if (static_cast<int>(blockIdx.x) >= line.pieces || line.total == 0) return;
   const long long begin = piece_begin(line, blockIdx.x), end = piece_begin(line, blockIdx.x + 1);
@@ -65,7 +53,7 @@ paged_weigh_kernel(const __grid_constant__ Weigh x) {
   for (; b < a.batch.B && at < end; ++b) {
     const PagedSeq s = paged_sequence(a, b);
     const PagedKeys keys = all_keys(a, s);
-    const int blocks = blocks_of(keys), cost = cost_of<R>(s), first_block = keys.lo / kBlockKeys;
+    const int blocks = blocks_of<kBlockKeys>(keys), cost = cost_of<R>(s), first_block = keys.lo / kBlockKeys;
     const long long all = static_cast<long long>(blocks) * a.kv_heads, before = at;
     at += all * cost;
     if (all == 0) continue;
@@ -184,15 +172,32 @@ int launch(const Weigh& x, int d, int rows, cudaStream_t stream) {
   return d == 128 ? launch<T, 128>(x, rows, stream) : launch<T, 64>(x, rows, stream);
 }
 
+// Which kernels run: few > 0: tiles of so many rows, for sequences of up to `most`; many: paged_weigh_tile.cu for the others.
+struct Form {
+  int few, most;
+  bool many;
+};
+Form form_of(int T, int B, int group) {
+  const long long rows = static_cast<long long>(T) * group;
+  if (T <= B || rows <= 16) return {rows <= 8ll * B ? 8 : 16, INT_MAX, false};
+  if (B == 1) return {0, 0, true};
+  return {16, 16, true};
+}
+
 }  // namespace
 }  // namespace ftb
 
 using namespace ftb;
 
+extern "C" size_t ftb_paged_attn_weights_scratch_bytes(int T, int B, int kv_heads, int group, int d) {
+  if (T <= 0 || B <= 0 || kv_heads <= 0 || group <= 0 || d <= 0 || !form_of(T, B, group).many) return 0;
+  return paged_weigh_tile_scratch(T, kv_heads, group, d);
+}
+
 extern "C" int ftb_paged_attn_weights(const void* q, long long q_row, long long q_head, const void* k_cache, const unsigned char* k_exp,
                                       const float* lse, const int* table, const int* lens, const int* starts, float* weights, int T, int B,
                                       int W, int pages, int kv_heads, int group, int page_size, int d, int window, float scale, int dtype,
-                                      void* workspace, size_t workspace_bytes, void* stream) {
+                                      void* scratch, size_t scratch_bytes, void* workspace, size_t workspace_bytes, void* stream) {
   if ((T > 0 && (!q || !lse)) || !k_cache || !weights || !table || !lens || !starts) return FTB_ERR_ARG;
   if (T < 0 || B <= 0 || W <= 0 || pages <= 0 || kv_heads <= 0 || group <= 0 || window < 0) return FTB_ERR_ARG;
   if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) return FTB_ERR_ARG;
@@ -224,13 +229,27 @@ extern "C" int ftb_paged_attn_weights(const void* q, long long q_row, long long 
   a.kv_heads = kv_heads;
   a.group = group;
   a.window = window;
-  a.least_rows = 1;
-  a.most_rows = INT_MAX;
   a.scale_log2 = scale * kLog2E;
   a.status = static_cast<int*>(workspace);
   x.weights = weights;
   x.lse = lse;
-  const int tile = static_cast<long long>(T) * group <= 8ll * B ? 8 : 16;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == FTB_F16 ? launch<__half>(x, d, tile, s) : launch<__nv_bfloat16>(x, d, tile, s);
+  const Form f = form_of(T, B, group);
+  if (f.many) {
+    if (static_cast<long long>(T) * heads > INT_MAX) return FTB_ERR_ARG;  // a copy's coordinates have 32 bits
+    if (scratch == nullptr || scratch_bytes < paged_weigh_tile_scratch(T, kv_heads, group, d)) return FTB_ERR_WORKSPACE;
+    if ((reinterpret_cast<uintptr_t>(scratch) & 15) != 0) return FTB_ERR_ALIGN;
+  }
+  int err = FTB_OK;
+  if (f.few > 0) {
+    a.least_rows = 1;
+    a.most_rows = f.most;
+    err = dtype == FTB_F16 ? launch<__half>(x, d, f.few, s) : launch<__nv_bfloat16>(x, d, f.few, s);
+  }
+  if (f.many && err == FTB_OK) {
+    a.least_rows = f.most + 1;
+    a.most_rows = INT_MAX;
+    err = paged_weigh_tile_launch(x, d, dtype, scratch, s);
+  }
+  return err;
 }

@@ -1022,9 +1022,11 @@ def paged_attention_weights(q, cache, weights, lse, table, lens, starts, scale=N
     _req_like(lse, "lse", torch.float32, (T, heads), kc)
     ws = workspace(kc.device)
     with _on(kc.device):
+        n = lib.ftb_paged_attn_weights_scratch_bytes(T, B, kv, heads // kv, d)
+        scratch = torch.empty(n, dtype=torch.uint8, device=kc.device) if n else None  # of the call's own
         check(lib.ftb_paged_attn_weights(qp, qr, qh, args[0], args[2], _ptr(lse), *args[4:], _ptr(weights), T, B, W, pages, kv, heads // kv, page_size,
                                          d, min(int(window), 0x7fffffff) if window is not None else 0, 1.0 if scale is None else float(scale),
-                                         _dtype_code(q), _ptr(ws), ws.numel(), _stream()), "ftb_paged_attn_weights")
+                                         _dtype_code(q), _ptr(scratch), n, _ptr(ws), ws.numel(), _stream()), "ftb_paged_attn_weights")
 
 
 def paged_cache_evict(cache, weights, table, lens, keep, recent=0, into=None):

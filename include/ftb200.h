@@ -501,11 +501,13 @@ int ftb_paged_cache_keep(void* k_cache, void* v_cache, unsigned char* k_exp, uns
  * group; the sum alone where j is a new token's own place.  weights: fp32 [pages, kv_heads, page_size]; lse: fp32
  * [T, kv_heads * group], of ftb_paged_attn_tree_fwd for the same call (a row whose lse is not finite adds nothing).  Each weight is the sum of
  * the rows in their order, without atomics: a page belongs to one sequence.  A key whose page the table does not have gets
- * nothing and sets the (sticky) status word to 22. */
+ * nothing and sets the (sticky) status word to 22.  scratch: ftb_paged_attn_weights_scratch_bytes (0: none needed), asked for with the call's
+ * device as the current one. */
+size_t ftb_paged_attn_weights_scratch_bytes(int T, int B, int kv_heads, int group, int d);
 int ftb_paged_attn_weights(const void* q, long long q_row, long long q_head, const void* k_cache, const unsigned char* k_exp,
                            const float* lse, const int* table, const int* lens, const int* starts, float* weights, int T,
                            int B, int W, int pages, int kv_heads, int group, int page_size, int d, int window, float scale,
-                           int dtype, void* workspace, size_t workspace_bytes, void* stream);
+                           int dtype, void* scratch, size_t scratch_bytes, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Eviction: of a sequence of lens[b] > keep keys, for each kv head, the last `recent` (0 .. keep) stay and, of those in front of
  * them, the keep - recent with the largest weights, of equal weights those in front (NaN is below all numbers).  What stays is moved as by

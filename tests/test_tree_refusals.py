@@ -26,7 +26,7 @@ def _attn(lib, **kw):
 
 def _weights(lib, **kw):
     a = dict(q=A(1), q_row=256, q_head=64, k=A(2), ke=Z, lse=A(9), table=A(4), lens=A(5), starts=A(6), weights=A(7), T=1, B=1, W=1, pages=1, kv=1,
-             group=4, page=16, d=64, window=0, scale=1.0, dtype=2, ws=A(10), wb=256, stream=Z)
+             group=4, page=16, d=64, window=0, scale=1.0, dtype=2, scratch=Z, sb=0, ws=A(10), wb=256, stream=Z)
     a.update(kw)
     return lib.ftb_paged_attn_weights(*a.values())
 
