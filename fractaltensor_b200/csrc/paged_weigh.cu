@@ -212,6 +212,7 @@ extern "C" int ftb_paged_attn_weights(const void* q, long long q_row, long long 
   if (T == 0) return FTB_OK;
   const int heads = kv_heads * group;
   const size_t rows = static_cast<size_t>(pages) * kv_heads * page_size, bytes = rows * sizeof(float);
+  if (rows > INT_MAX) return FTB_ERR_ARG;
   if (overlap(weights, bytes, k_cache, rows * d * (k_exp != nullptr ? 1 : 2)) || (k_exp != nullptr && overlap(weights, bytes, k_exp, rows)) ||
       overlap(weights, bytes, lse, static_cast<size_t>(T) * heads * sizeof(float)) || over_rows(weights, static_cast<long long>(bytes / 2), q, T, q_row, heads, q_head, d))
     return FTB_ERR_ARG;

@@ -8,10 +8,16 @@
 //
 // One persistent CTA per SM takes an equal piece of the line of work, whose unit is a tile of rows against a block:
 //   warp 0        the walk, announced through a ring of stretches, and the loads of the rows (TMA)
-//   warp 1        issues the products
-//   warps 2..9    exponentials and sums: a thread a key
-//   warps 10..13  load the keys of the next block and make them operands (8-bit codes as fp16; a key's scale goes to its scores)
+//   warp 1        issues the products, into one of two buffers of scores
+//   warps 2..17   exponentials and sums, while the next tile's scores are made: a thread has a key of either half of the block and a quarter
+//                 of the tile's rows
+//   warps 18..21  load the keys of the next block and make them operands (8-bit codes as fp16; a key's scale goes to its scores)
 // A block that a cut goes through leaves parts of its sums, which a second kernel adds up in their order.
+//
+// 2048 tokens of 32 heads of 128 over 8 kv heads, 16 384 keys of 8 bits: 331 us, 0.78 PFLOP/s.  Bound by no unit alone: without the
+// exponentials (16 a cycle and SM, 245 us) it takes 285 us, without the products (122) 324, with neither 173, which is the rows' way from L2 for
+// every block and the hand-overs between the warps.  Measured and not kept: a quarter to a half of the exponentials by a polynomial on the units that
+// multiply and add (334 to 383 us), blocks of 512 keys (346), eight warps for the sums (352), each half of the warps with a buffer of its own (351).
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -25,7 +31,7 @@ namespace ftb {
 namespace {
 
 constexpr float kLog2E = 1.4426950408889634f;
-constexpr int kBlock = 256, kRows = 128, kStretches = 4, kThreads = 32 * 14, kPackThreads = 256;
+constexpr int kBlock = 256, kRows = 128, kSplit = 4, kPart = kRows / kSplit, kStretches = 4, kBeside = 4, kSums = 16, kLoaders = 4, kThreads = 32 * (2 + kSums + kLoaders), kPackThreads = 256;
 
 // Rows as the products take them: [kv_heads][T * group][d], with [kv_heads][T * group] numbers each.
 struct Packed {
@@ -104,6 +110,19 @@ __device__ __forceinline__ long long tiles_of_head(const PagedAttn& a, const Pag
   return sum;
 }
 
+// The tiles of a stretch with rows that see a key of the block's half h: first .. last - 1.
+struct Tiles {
+  int first, last;
+};
+__device__ __forceinline__ Tiles tiles_of_half(const PagedAttn& a, const Stretch& y, int h) {
+  const int k0 = max(y.key0 + h * 128, y.keys.lo), k1 = min(y.key0 + (h + 1) * 128, y.keys.hi);
+  if (k0 >= k1) return {0, 0};
+  const long long f0 = max(0ll, k0 - y.base) * a.group - y.flat0;
+  long long f1 = y.flat1 - y.flat0;
+  if (a.window > 0) f1 = min(f1, max(0ll, k1 - 1 + a.window - y.base) * a.group - y.flat0);
+  return {static_cast<int>(max(0ll, f0) / kRows), static_cast<int>((max(0ll, f1) + kRows - 1) / kRows)};
+}
+
 struct Cut {
   int last;  // the last piece with a part; -1: nothing to add up
   int b, h, key0;
@@ -115,19 +134,21 @@ template <int D, bool kFactors>
 struct Plan {
   static constexpr int kHalf = 128 * 128, kTile = D / 64 * kHalf;  // 128 rows of 64 and of d numbers
   static constexpr int kStages = D == 128 ? 2 : 4;
-  static constexpr int kMeta = kRows * 4 * (kFactors ? 2 : 1);
 };
 
 template <int D, bool kFactors>
 struct Control {
   using P = Plan<D, kFactors>;
-  alignas(16) float minus[P::kStages][kRows], factor[kFactors ? P::kStages : 1][kRows];
-  float scale[2][kBlock];     // of a key's scores
-  long long row[2][kBlock];   // of the cache, -1: none
+  // what goes with the rows of a tile, in a ring of its own: the rows' room is free again when the products are done
+  alignas(16) float minus[kBeside][kRows], factor[kFactors ? kBeside : 1][kRows];
+  int odd[kBeside];           // whether some row adds nothing
+  float scale[2][kBlock];     // of a key's scores; of every second stretch, as the next one
+  int row[2][kBlock];         // of the cache, -1: none
   PagedLineRoom line;
   Stretch ring[kStretches];
   uint64_t ring_full[kStretches], ring_empty[kStretches];
-  uint64_t q_full[P::kStages], q_empty[P::kStages], k_full[2], k_empty[2], s_full[2], s_empty[2];
+  uint64_t q_full[P::kStages], q_empty[P::kStages], beside_full[kBeside], beside_empty[kBeside], k_full[2], k_empty[2], s_full[2], s_empty[2], other_full[2];
+  float other[2][kSplit - 1][kBlock];  // sums over the other quarters of the tiles
   uint32_t tmem_base;
   int abort, dead;
 };
@@ -152,17 +173,22 @@ paged_weigh_tile_kernel(const __grid_constant__ Weigh x, const __grid_constant__
     prefetch_tmap(&mapQ);
     for (int i = 0; i < kStretches; ++i) {
       mbar_init(&ctl.ring_full[i], 1);
-      mbar_init(&ctl.ring_empty[i], 1 + 8 + 4);
+      mbar_init(&ctl.ring_empty[i], 1 + kSums + kLoaders);
     }
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&ctl.q_full[i], 1);
-      mbar_init(&ctl.q_empty[i], 1 + 8);
+      mbar_init(&ctl.q_empty[i], 1);
+    }
+    for (int i = 0; i < kBeside; ++i) {
+      mbar_init(&ctl.beside_full[i], 1);
+      mbar_init(&ctl.beside_empty[i], kSums);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&ctl.k_full[i], 4);
-      mbar_init(&ctl.k_empty[i], 1 + 8);
+      mbar_init(&ctl.k_full[i], kLoaders);
+      mbar_init(&ctl.k_empty[i], 1 + kSums);
       mbar_init(&ctl.s_full[i], 1);
-      mbar_init(&ctl.s_empty[i], 8);
+      mbar_init(&ctl.s_empty[i], kSums);
+      mbar_init(&ctl.other_full[i], kSums - kSums / kSplit);
     }
     ctl.abort = 0;
     fence_barrier_init();
@@ -189,7 +215,7 @@ paged_weigh_tile_kernel(const __grid_constant__ Weigh x, const __grid_constant__
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = ctl.tmem_base;  // scores of a tile: buffer p, keys of half t: columns 256 p + 128 t .. + 127
+  const uint32_t tmem_base = ctl.tmem_base;  // scores: buffer p, half h of the keys: columns 256 p + 128 h .. + 127
 
   auto await = [&](int i) -> bool {
     return mbar_wait_warp(&ctl.ring_full[i % kStretches], (i / kStretches) & 1, s_abort, status, FTB_ERR_TIMEOUT_TMA);
@@ -263,7 +289,7 @@ paged_weigh_tile_kernel(const __grid_constant__ Weigh x, const __grid_constant__
     const long long all = static_cast<long long>(a.T) * a.group, numbers = all * a.kv_heads;
     Stretch now, next;
     bool ok = publish(next);
-    int stage = 0;
+    int stage = 0, tile = 0;
     uint32_t phase = 0;
     for (bool more = true; ok && more;) {
       now = next;
@@ -278,13 +304,18 @@ paged_weigh_tile_kernel(const __grid_constant__ Weigh x, const __grid_constant__
         if constexpr (kFactors) factor = make_float4(take(packed.factor, 0), take(packed.factor, 1), take(packed.factor, 2), take(packed.factor, 3));
       };
       fetch(now.flat0);
-      for (int k = 0; ok && k < now.tiles; ++k) {
-        const int flat = now.flat0 + k * kRows;
+      for (int k = 0; ok && k < now.tiles; ++k, ++tile) {
+        const int flat = now.flat0 + k * kRows, beside = tile % kBeside;
+        ok = mbar_wait_warp(&ctl.beside_empty[beside], ((tile / kBeside) & 1) ^ 1u, s_abort, status, FTB_ERR_TIMEOUT_SLOT);
+        if (!ok) break;
+        reinterpret_cast<float4*>(ctl.minus[beside])[lane] = minus;
+        if constexpr (kFactors) reinterpret_cast<float4*>(ctl.factor[beside])[lane] = factor;
+        const bool odd = __any_sync(0xffffffffu, fminf(fminf(minus.x, minus.y), fminf(minus.z, minus.w)) == -INFINITY);
+        if (lane == 0) ctl.odd[beside] = odd;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.beside_full[beside]);
         ok = mbar_wait_warp(&ctl.q_empty[stage], phase ^ 1u, s_abort, status, FTB_ERR_TIMEOUT_SLOT);
         if (!ok) break;
-        reinterpret_cast<float4*>(ctl.minus[stage])[lane] = minus;
-        if constexpr (kFactors) reinterpret_cast<float4*>(ctl.factor[stage])[lane] = factor;
-        __syncwarp();
         if (lane == 0) {
           mbar_arrive_expect_tx(&ctl.q_full[stage], P::kTile);
           const int y = static_cast<int>(row0 + flat);
@@ -308,12 +339,12 @@ paged_weigh_tile_kernel(const __grid_constant__ Weigh x, const __grid_constant__
     bool ok = true;
     for (int i = 0; ok; ++i) {
       if (!await(i)) break;
-      const int tiles = ctl.ring[i % kStretches].tiles;
-      const bool last = ctl.ring[i % kStretches].last != 0;
+      const Stretch y = ctl.ring[i % kStretches];
       give_back(i);
       const int buffer = i & 1;
+      const Tiles met[2] = {tiles_of_half(a, y, 0), tiles_of_half(a, y, 1)};
       ok = mbar_wait_warp(&ctl.k_full[buffer], (i >> 1) & 1, s_abort, status, FTB_ERR_TIMEOUT_TMA);
-      for (int k = 0; ok && k < tiles; ++k, ++tile) {
+      for (int k = 0; ok && k < y.tiles; ++k, ++tile) {
         const int p = tile & 1;
         ok = mbar_wait_warp(&ctl.q_full[stage], phase, s_abort, status, FTB_ERR_TIMEOUT_TMA) &&
              mbar_wait_warp(&ctl.s_empty[p], ((tile >> 1) & 1) ^ 1u, s_abort, status, FTB_ERR_TIMEOUT_EPI);
@@ -321,125 +352,154 @@ paged_weigh_tile_kernel(const __grid_constant__ Weigh x, const __grid_constant__
         tc_fence_after();
         if (leader) {
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const uint64_t dk = dK + static_cast<uint64_t>(((buffer * 2 + t) * P::kTile) >> 4), dq = dQ + static_cast<uint64_t>((stage * P::kTile) >> 4);
+          for (int h = 0; h < 2; ++h) {
+            if (k < met[h].first || k >= met[h].last) continue;
+            const uint64_t dk = dK + static_cast<uint64_t>(((buffer * 2 + h) * P::kTile) >> 4), dq = dQ + static_cast<uint64_t>((stage * P::kTile) >> 4);
 #pragma unroll
             for (int j = 0; j < D / 16; ++j) {
               const uint32_t off = ((j >> 2) * P::kHalf + (j & 3) * 32) >> 4;
-              umma_ss(tmem_base + p * 256 + t * 128, dk + off, dq + off, idesc, j != 0 ? 1u : 0u);
+              umma_ss(tmem_base + p * 256 + h * 128, dk + off, dq + off, idesc, j != 0 ? 1u : 0u);
             }
           }
           umma_commit(&ctl.s_full[p]);
           umma_commit(&ctl.q_empty[stage]);
-          if (k + 1 == tiles) umma_commit(&ctl.k_empty[buffer]);
+          if (k + 1 == y.tiles) umma_commit(&ctl.k_empty[buffer]);
         }
         if (++stage == kStages) {
           stage = 0;
           phase ^= 1u;
         }
       }
-      if (last) break;
+      if (y.last) break;
     }
-  } else if (warp < 10) {
+  } else if (warp < 2 + kSums) {
     // ------------------------------------------------ exponentials and sums: key `mine` of a block
-    const int t = (warp - 2) >> 2, quad = warp & 3, mine = t * 128 + quad * 32 + lane;
-    const uint32_t addr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + t * 128;
-    int stage = 0, tile = 0;
-    uint32_t phase = 0;
+    const int part = (warp - 2) >> 2, quad = warp & 3, lane_key = quad * 32 + lane;
+    const uint32_t addr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + part * kPart;
+    int tile = 0;
     bool ok = true;
     for (int i = 0; ok; ++i) {
       if (!await(i)) break;
       const Stretch& y = ctl.ring[i % kStretches];
-      const int buffer = i & 1, tiles = y.tiles, key = y.key0 + mine;
-      // the rows that see this key lie side by side: see0 .. see1 - 1 of the stretch's first tile and so on
-      long long see0 = 0, see1 = 0;
-      if (key >= y.keys.lo && key < y.keys.hi) {
-        see0 = max(0ll, key - y.base) * a.group - y.flat0;
-        see1 = y.flat1 - y.flat0;
-        if (a.window > 0) see1 = min(see1, max(0ll, key + a.window - y.base) * a.group - y.flat0);
-      }
-      const int from = static_cast<int>(max(0ll, see0)), to = static_cast<int>(max(0ll, see1));
+      const int buffer = i & 1, tiles = y.tiles;
       ok = mbar_wait_warp(&ctl.k_full[buffer], (i >> 1) & 1, s_abort, status, FTB_ERR_TIMEOUT_TMA);
       if (!ok) break;
-      const float scale = ctl.scale[buffer][mine];
-      const uint64_t scale2 = dup_f32x2(scale);
-      float sum = 0.f;
+      // of this thread's keys: the rows that see one lie side by side, from .. to - 1 counted from the stretch's first one
+      int from[2], to[2];
+      float scale[2], sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int key = y.key0 + h * 128 + lane_key;
+        long long see0 = 0, see1 = 0;
+        if (key >= y.keys.lo && key < y.keys.hi) {
+          see0 = max(0ll, key - y.base) * a.group - y.flat0;
+          see1 = y.flat1 - y.flat0;
+          if (a.window > 0) see1 = min(see1, max(0ll, key + a.window - y.base) * a.group - y.flat0);
+        }
+        from[h] = static_cast<int>(max(0ll, see0)) - part * kPart;
+        to[h] = static_cast<int>(max(0ll, see1)) - part * kPart;
+        scale[h] = ctl.scale[buffer][h * 128 + lane_key];
+      }
+      // Tiles whose rows this warp's keys see all of.  (In the others a key sees none, or rows from .. to - 1.)
+      const int plain0 = __reduce_max_sync(0xffffffffu, max(max(from[0], from[1]), 0) + kRows - 1) / kRows;
+      const int plain1 = __reduce_min_sync(0xffffffffu, max(min(to[0], to[1]) + kRows - kPart, 0)) / kRows;
       for (int k = 0; k < tiles; ++k, ++tile) {
-        const int p = tile & 1;
-        ok = mbar_wait_warp(&ctl.q_full[stage], phase, s_abort, status, FTB_ERR_TIMEOUT_TMA) &&  // (what goes with the rows)
+        const int p = tile & 1, beside = tile % kBeside;
+        ok = mbar_wait_warp(&ctl.beside_full[beside], (tile / kBeside) & 1, s_abort, status, FTB_ERR_TIMEOUT_TMA) &&
              mbar_wait_warp(&ctl.s_full[p], (tile >> 1) & 1, s_abort, status, FTB_ERR_TIMEOUT_MMA);
         if (!ok) break;
         tc_fence_after();
         const uint32_t s_addr = addr + p * 256;
-        const float *minus = ctl.minus[stage], *factor = ctl.factor[kFactors ? stage : 0];
-        const int lo = from - k * kRows, hi = to - k * kRows;
-        float part = 0.f;
-        bool plain = __all_sync(0xffffffffu, lo <= 0 && hi >= kRows);
-        if (plain) {
-          uint64_t sum4[4] = {0, 0, 0, 0};
-#pragma unroll 1
-          for (int c0 = 0; c0 < kRows; c0 += 32) {
-            uint32_t s[32];
-            tmem_ld32(s_addr + c0, s);
+        const float *minus = ctl.minus[beside] + part * kPart, *factor = ctl.factor[kFactors ? beside : 0] + (kFactors ? part * kPart : 0);
+        auto give_back_scores = [&] {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl.s_empty[p]);
+        };
+        if (k >= plain0 && k < plain1 && ctl.odd[beside] == 0) {
+          // (both keys' scores beside one another: what goes with a row comes out of shared memory once for them.  And the scores' room is
+          // given back as soon as they are in registers: what is to do with them does not hold up the products.)
+          uint64_t sum2[2][2] = {};
+#pragma unroll
+          for (int n = 0; n < kPart / 16; ++n) {
+            uint32_t s[2][16];
+            tmem_ld16(s_addr + n * 16, s[0]);
+            tmem_ld16(s_addr + 128 + n * 16, s[1]);
             tmem_ld_wait();
+            if (n + 1 == kPart / 16) give_back_scores();
 #pragma unroll
-            for (int c = 0; c < 32; c += 4) {
-              const ulonglong2 m = *reinterpret_cast<const ulonglong2*>(minus + c0 + c);
+            for (int c = 0; c < 16; c += 4) {
+              const ulonglong2 m = *reinterpret_cast<const ulonglong2*>(minus + n * 16 + c);
               float4 f;
-              if constexpr (kFactors) f = *reinterpret_cast<const float4*>(factor + c0 + c);
+              if constexpr (kFactors) f = *reinterpret_cast<const float4*>(factor + n * 16 + c);
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const uint64_t s2 = pair_f32x2(__uint_as_float(s[c + 2 * e]), __uint_as_float(s[c + 2 * e + 1]));
-                uint64_t f2 = scale2;
-                if constexpr (kFactors)
-                  f2 = pair_f32x2(fminf((e == 0 ? f.x : f.z) * scale, FLT_MAX), fminf((e == 0 ? f.y : f.w) * scale, FLT_MAX));
-                float p0, p1;
-                unpair_f32x2(fma_to_f32x2(s2, f2, e == 0 ? m.x : m.y), p0, p1);
-                add_f32x2(sum4[(c / 2 + e) & 3], pair_f32x2(exp2_fast(p0), exp2_fast(p1)));
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const uint64_t s2 = pair_f32x2(__uint_as_float(s[h][c + 2 * e]), __uint_as_float(s[h][c + 2 * e + 1]));
+                  uint64_t f2 = dup_f32x2(scale[h]);
+                  if constexpr (kFactors)
+                    f2 = pair_f32x2(fminf((e == 0 ? f.x : f.z) * scale[h], FLT_MAX), fminf((e == 0 ? f.y : f.w) * scale[h], FLT_MAX));
+                  const uint64_t x2 = fma_to_f32x2(s2, f2, e == 0 ? m.x : m.y);
+                  float p0, p1;
+                  unpair_f32x2(x2, p0, p1);
+                  add_f32x2(sum2[h][e], pair_f32x2(exp2_fast(p0), exp2_fast(p1)));
+                }
+            }
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            add_f32x2(sum2[h][0], sum2[h][1]);
+            float p0, p1;
+            unpair_f32x2(sum2[h][0], p0, p1);
+            sum[h] += p0 + p1;
+          }
+        } else {
+          // at the edges, and where rows that add nothing may have met something that is not finite: number by number
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            const float by = h == 0 ? scale[0] : scale[1];
+            const int lo = max(0, (h == 0 ? from[0] : from[1]) - k * kRows), hi = min(kPart, (h == 0 ? to[0] : to[1]) - k * kRows);
+            if (__all_sync(0xffffffffu, lo >= hi)) continue;  // (no scores have been made where nobody sees one)
+            float all = 0.f;
+#pragma unroll 1
+            for (int c0 = 0; c0 < kPart; c0 += 16) {
+              uint32_t s[16];
+              tmem_ld16(s_addr + h * 128 + c0, s);
+              tmem_ld_wait();
+#pragma unroll
+              for (int c = 0; c < 16; ++c) {
+                const float m = minus[c0 + c], f = kFactors ? fminf(factor[c0 + c] * by, FLT_MAX) : by;
+                const bool counts = c0 + c >= lo && c0 + c < hi && m > -INFINITY;
+                all += counts ? exp2_fast(fmaf(__uint_as_float(s[c]), f, m)) : 0.f;
               }
             }
+            if (h == 0) sum[0] += all;
+            else sum[1] += all;
           }
-          add_f32x2(sum4[0], sum4[1]);
-          add_f32x2(sum4[2], sum4[3]);
-          add_f32x2(sum4[0], sum4[2]);
-          float p0, p1;
-          unpair_f32x2(sum4[0], p0, p1);
-          part = p0 + p1;
+          give_back_scores();
         }
-        // at the edges, and where something that is not finite has met rows that add nothing: number by number
-        if (!plain || __any_sync(0xffffffffu, part != part)) {
-          part = 0.f;
-#pragma unroll 1
-          for (int c0 = 0; c0 < kRows; c0 += 32) {
-            uint32_t s[32];
-            tmem_ld32(s_addr + c0, s);
-            tmem_ld_wait();
-#pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              const float m = minus[c0 + c], f = kFactors ? fminf(factor[c0 + c] * scale, FLT_MAX) : scale;
-              const bool counts = c0 + c >= lo && c0 + c < hi && m > -INFINITY;
-              part += counts ? exp2_fast(fmaf(__uint_as_float(s[c]), f, m)) : 0.f;
-            }
-          }
-        }
-        sum += part;
-        tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&ctl.s_empty[p]);
-          mbar_arrive(&ctl.q_empty[stage]);
-        }
-        if (++stage == kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
+        if (lane == 0) mbar_arrive(&ctl.beside_empty[beside]);
       }
       if (!ok) break;
-      if (y.whole) {
-        const long long row = ctl.row[buffer][mine];
-        if (row >= 0) x.weights[row] = key >= y.base ? sum : x.weights[row] + sum;
+      if (part != 0) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) ctl.other[buffer][part - 1][h * 128 + lane_key] = sum[h];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.other_full[buffer]);
       } else {
-        parts[static_cast<long long>(y.place) * kBlock + mine] = sum;
+        ok = mbar_wait_warp(&ctl.other_full[buffer], (i >> 1) & 1, s_abort, status, FTB_ERR_TIMEOUT_EPI);
+        if (!ok) break;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int mine = h * 128 + lane_key, key = y.key0 + mine, row = ctl.row[buffer][mine];
+          float all = sum[h];
+#pragma unroll
+          for (int o = 0; o < kSplit - 1; ++o) all += ctl.other[buffer][o][mine];
+          if (!y.whole) parts[static_cast<long long>(y.place) * kBlock + mine] = all;
+          else if (row >= 0) x.weights[row] = key >= y.base ? all : x.weights[row] + all;
+        }
       }
       const bool last = y.last != 0;
       __syncwarp();
@@ -449,14 +509,14 @@ paged_weigh_tile_kernel(const __grid_constant__ Weigh x, const __grid_constant__
     }
   } else {
     // ------------------------------------------------------------- the keys: 64 of a block a warp
-    const int of_block = (warp - 10) * 64;
+    const int of_block = (warp - 2 - kSums) * 64;
     bool ok = true;
     for (int i = 0; ok; ++i) {
       if (!await(i)) break;
       const Stretch& y = ctl.ring[i % kStretches];
       const int buffer = i & 1;
       const int* table = a.batch.table + static_cast<long long>(y.b) * a.batch.W;
-      long long rows[2];
+      int rows[2];
       float scales[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {  // lane's keys
@@ -465,13 +525,12 @@ paged_weigh_tile_kernel(const __grid_constant__ Weigh x, const __grid_constant__
         if (key >= y.keys.lo && key < y.keys.hi) {
           const int page = table[key >> a.batch.page_shift];
           if (page >= 0 && page < a.batch.pages)
-            rows[e] = ((static_cast<long long>(page) * a.kv_heads + y.h) << a.batch.page_shift) + (key & ((1 << a.batch.page_shift) - 1));
+            rows[e] = ((page * a.kv_heads + y.h) << a.batch.page_shift) + (key & ((1 << a.batch.page_shift) - 1));
           else
             atomicCAS(status, 0, FTB_ERR_INDEX);
         }
         scales[e] = kFactors ? 1.f : a.scale_log2;
-        if constexpr (k8) scales[e] *= rows[e] >= 0 ? exponent_scale(a.k_exp[rows[e]]) : 1.f;
-        if constexpr (k8) scales[e] = fminf(scales[e], FLT_MAX);
+        if constexpr (k8) scales[e] = rows[e] >= 0 ? fminf(scales[e] * exponent_scale(a.k_exp[rows[e]]), FLT_MAX) : 1.f;
       }
       ok = mbar_wait_warp(&ctl.k_empty[buffer], ((i >> 1) & 1) ^ 1u, s_abort, status, FTB_ERR_TIMEOUT_SLOT);
       if (!ok) break;
@@ -490,12 +549,12 @@ paged_weigh_tile_kernel(const __grid_constant__ Weigh x, const __grid_constant__
           uint4 v[kAtOnce];
 #pragma unroll
           for (int k = 0; k < kAtOnce; ++k) {
-            const long long row = __shfl_sync(0xffffffffu, rows[e], r0 + k * kTogether + lane / kPieces);
-            v[k] = row >= 0 ? *reinterpret_cast<const uint4*>(a.k + row * (k8 ? D : 2 * D) + piece_of * 16) : make_uint4(0u, 0u, 0u, 0u);
+            const int row = __shfl_sync(0xffffffffu, rows[e], r0 + k * kTogether + lane / kPieces);
+            v[k] = row >= 0 ? *reinterpret_cast<const uint4*>(a.k + static_cast<long long>(row) * (k8 ? D : 2 * D) + piece_of * 16) : make_uint4(0u, 0u, 0u, 0u);
           }
 #pragma unroll
           for (int k = 0; k < kAtOnce; ++k) {
-            const int r = (of_block + e * 32 + r0 + k * kTogether + lane / kPieces) & 127;
+            const int r = (of_block & 64) + e * 32 + r0 + k * kTogether + lane / kPieces;
             auto put = [&](int q, const uint4& w) {
               *reinterpret_cast<uint4*>(tile + (q >> 3) * P::kHalf + r * 128 + (((q & 7) ^ (r & 7)) << 4)) = w;
             };
