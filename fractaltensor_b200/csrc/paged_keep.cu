@@ -29,7 +29,7 @@ struct Choose {
   int* status;
 };
 
-constexpr int kChooseThreads = 512, kChooseWarps = kChooseThreads / 32, kBins = 256, kCopies = 4;
+constexpr int kChooseThreads = 512, kChooseWarps = kChooseThreads / 32, kBins = 256, kCopies = 4, kChooseAtOnce = 8;
 
 // Unsigned numbers in the order of the weights; NaN is below all of them.
 __device__ __forceinline__ uint32_t order_of(float w) {
@@ -44,10 +44,11 @@ __device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
   return x;
 }
 
-// C CTAs for each sequence and kv head, a stretch of the keys each.
+// C CTAs for each sequence and kv head, a stretch of the keys each, of which `room` stay in shared memory after they have been read.
 template <int C>
 __global__ void __launch_bounds__(kChooseThreads)
-paged_choose_kernel(const __grid_constant__ Choose a) {
+paged_choose_kernel(const __grid_constant__ Choose a, int room) {
+  extern __shared__ uint32_t known_keys[];
   __shared__ int bins[kCopies][kBins], sums[2][kBins], above_of[kChooseWarps], equal_of[kChooseWarps], mine[2];
   __shared__ int s_digit, s_left;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -55,8 +56,7 @@ paged_choose_kernel(const __grid_constant__ Choose a) {
   const int b = head / a.kv_heads, h = head - b * a.kv_heads;
   grid_launch_dependents();
   grid_dependency_wait();
-  const long long room = static_cast<long long>(a.batch.W) << a.batch.page_shift;
-  const int asked = max(0, a.batch.lens[b]), L = static_cast<int>(min(room, static_cast<long long>(asked)));
+  const int asked = max(0, a.batch.lens[b]), L = static_cast<int>(min(static_cast<long long>(a.batch.W) << a.batch.page_shift, static_cast<long long>(asked)));
   if (threadIdx.x == 0 && rank == 0 && h == 0) {
     if (asked > L) atomicCAS(a.status, 0, FTB_ERR_INDEX);  // a table too narrow for the length
     a.lens_out[b] = min(L, a.keep);
@@ -74,25 +74,52 @@ paged_choose_kernel(const __grid_constant__ Choose a) {
   const int shift = a.batch.page_shift, in_page = (1 << shift) - 1;
   auto key_at = [&](int i) -> uint32_t {
     const int page = __ldg(table + (i >> shift));
-    if (page < 0 || page >= a.batch.pages) {
-      atomicCAS(a.status, 0, FTB_ERR_INDEX);
-      return 0u;
-    }
+    if (page < 0 || page >= a.batch.pages) return 0u;  // (which is said where it is first read)
     return order_of(a.weights[(((static_cast<long long>(page) * a.kv_heads) + h) << shift) + (i & in_page)]);
   };
   // a warp's stretch: whole groups of 32
   const int stretch = (old + C * kChooseThreads - 1) / (C * kChooseThreads) * 32;
   const int from = static_cast<int>(min(static_cast<long long>(old), static_cast<long long>(rank * kChooseWarps + warp) * stretch));
   const int to = static_cast<int>(min(static_cast<long long>(old), static_cast<long long>(from) + stretch));
+  const int first = static_cast<int>(min(static_cast<long long>(old), static_cast<long long>(rank) * kChooseWarps * stretch));  // of the CTA's
+  auto key_of = [&](int i) -> uint32_t { return i - first < room ? known_keys[i - first] : key_at(i); };
   uint32_t prefix = 0, known = 0;  // the digits so far, and which bits they are
   int left = want;
   for (int d = 0; d < 4; ++d) {
     const int low = 24 - 8 * d;
     for (int i = threadIdx.x; i < kCopies * kBins; i += kChooseThreads) (&bins[0][0])[i] = 0;
     __syncthreads();
-    for (int i = from + lane; i < to; i += 32) {
-      const uint32_t key = key_at(i);
-      if ((key & known) == prefix) atomicAdd(&bins[warp % kCopies][key >> low & 255u], 1);
+    if (d == 0) {
+      for (int i0 = from; i0 < to; i0 += 32 * kChooseAtOnce) {
+        int page[kChooseAtOnce];
+        float w[kChooseAtOnce];
+#pragma unroll
+        for (int u = 0; u < kChooseAtOnce; ++u) {
+          const int i = i0 + u * 32 + lane;
+          page[u] = i < to ? __ldg(table + (i >> shift)) : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < kChooseAtOnce; ++u) {
+          const int i = i0 + u * 32 + lane;
+          w[u] = __int_as_float(0x7fffffff);
+          if (i >= to) continue;
+          if (page[u] >= 0 && page[u] < a.batch.pages) w[u] = a.weights[(((static_cast<long long>(page[u]) * a.kv_heads) + h) << shift) + (i & in_page)];
+          else atomicCAS(a.status, 0, FTB_ERR_INDEX);
+        }
+#pragma unroll
+        for (int u = 0; u < kChooseAtOnce; ++u) {
+          const int i = i0 + u * 32 + lane;
+          if (i >= to) continue;
+          const uint32_t key = order_of(w[u]);
+          if (i - first < room) known_keys[i - first] = key;
+          atomicAdd(&bins[warp % kCopies][key >> low], 1);
+        }
+      }
+    } else {
+      for (int i = from + lane; i < to; i += 32) {
+        const uint32_t key = key_of(i);
+        if ((key & known) == prefix) atomicAdd(&bins[warp % kCopies][key >> low & 255u], 1);
+      }
     }
     __syncthreads();
     int* of_cta = sums[d & 1];  // (the other one may still be read by a CTA of the cluster)
@@ -144,7 +171,7 @@ paged_choose_kernel(const __grid_constant__ Choose a) {
   // what is above stays, of what is equal the first `left`
   int above = 0, equal = 0;
   for (int i = from + lane; i < to; i += 32) {
-    const uint32_t key = key_at(i);
+    const uint32_t key = key_of(i);
     above += key > prefix;
     equal += key == prefix;
   }
@@ -179,7 +206,7 @@ paged_choose_kernel(const __grid_constant__ Choose a) {
   }
   for (int i0 = from; i0 < to; i0 += 32) {
     const int i = i0 + lane;
-    const uint32_t key = i < to ? key_at(i) : 0u;
+    const uint32_t key = i < to ? key_of(i) : 0u;
     const unsigned is_above = __ballot_sync(0xffffffffu, i < to && key > prefix), is_equal = __ballot_sync(0xffffffffu, i < to && key == prefix);
     const unsigned in_front = (1u << lane) - 1u;
     const int equals = equal + __popc(is_equal & in_front);
@@ -205,90 +232,100 @@ struct Move {
   int* status;
 };
 
-constexpr int kMoveThreads = 256, kMoveAtOnce = 8;
+constexpr int kMoveThreads = 256, kMoveAtOnce = 8, kMostRoom = 48 * 1024;
 
 // Rows of cache planes that a kept row comes from and goes to; -1: none.
 struct Rows {
-  long long from, to;
+  int from, to;
 };
-__device__ __forceinline__ Rows rows_of(const Move& a, int b, int h, long long first, const int* kept, int i) {
+__device__ __forceinline__ Rows rows_of(const Move& a, int b, int h, int first, const int* kept, int i) {
   const int k = kept[i];
   PagedBatch into = a.batch;
   into.table = a.into;
   into.W = a.into_W;
-  Rows r{-1, -1};
   if (k < 0 || first < 0) {
     atomicCAS(a.status, 0, FTB_ERR_INDEX);
-    return r;
+    return {-1, -1};
   }
   const int shift = a.batch.page_shift, in_page = (1 << shift) - 1;
-  const long long src = first + k, dst = first + i;
-  if (src == dst && a.into == a.batch.table) return r;  // where it is
+  const long long src = static_cast<long long>(first) + k, dst = static_cast<long long>(first) + i;
+  if (src == dst && a.into == a.batch.table) return {-1, -1};  // where it is
   const int from = page_of(a.batch, b, src, a.status), to = page_of(into, b, dst, a.status);
-  if (from < 0 || to < 0) return r;
-  r.from = ((static_cast<long long>(from) * a.kv_heads + h) << shift) + (src & in_page);
-  r.to = ((static_cast<long long>(to) * a.kv_heads + h) << shift) + (dst & in_page);
-  return r;
+  if (from < 0 || to < 0) return {-1, -1};
+  return {((from * a.kv_heads + h) << shift) + static_cast<int>(src & in_page), ((to * a.kv_heads + h) << shift) + static_cast<int>(dst & in_page)};
 }
 
-// Block (x, y, z): sequence and kv head x, part y of a row, every gridDim.z-th step of rows.  kRow: 16-byte pieces of a key or value,
-// kOfPart: pieces of a part of both together; the last part, behind those, is exponents and weights.
-template <int kRow, int kOfPart>
+// A chain is kChain threads': block (x, y, z) has the chains of sequences and kv heads 256 / kChain * x and on, part y of a row, every
+// gridDim.z-th step of rows.  kRow: 16-byte pieces of a key or value, kOfPart: pieces of a part of both together; exponents and weights go with part 0.
+// The rows of the next step are looked up while this one's are on their way.
+template <int kRow, int kOfPart, int kChain>
 __global__ void __launch_bounds__(kMoveThreads)
-paged_move_kernel(const __grid_constant__ Move a, bool in_place) {
-  const int b = blockIdx.x / a.kv_heads, h = blockIdx.x - b * a.kv_heads, part = blockIdx.y;
+paged_move_kernel(const __grid_constant__ Move a, int chains, bool in_place) {
+  constexpr int kTogether = kChain / kOfPart, kStep = kTogether * kMoveAtOnce, kBeside = (kStep + kChain - 1) / kChain;
+  __shared__ Rows looked_up[kMoveThreads / kChain][2][kStep];
+  const int chain = blockIdx.x * (kMoveThreads / kChain) + threadIdx.x / kChain, tid = threadIdx.x % kChain, part = blockIdx.y;
   grid_launch_dependents();
   grid_dependency_wait();
-  const int n = min(max(a.counts[b], 0), a.most);
-  const long long first = a.first != nullptr ? a.first[b] : 0;
+  if (kChain < kMoveThreads && chain >= chains) return;  // (a warp leaves as one)
+  const int b = chain / a.kv_heads, h = chain - b * a.kv_heads;
+  const int n = min(max(a.counts[b], 0), a.most), first = a.first != nullptr ? a.first[b] : 0;
   const int* kept = a.kept + b * a.kept_seq + h * a.kept_head;
-  if (part < 2 * kRow / kOfPart) {
-    constexpr int kTogether = kMoveThreads / kOfPart, kStep = kTogether * kMoveAtOnce;
-    const int r = threadIdx.x / kOfPart, piece = part * kOfPart + threadIdx.x % kOfPart;
-    uint4* plane = reinterpret_cast<uint4*>(piece < kRow ? a.k : a.v) + (piece < kRow ? piece : piece - kRow);
-    for (int i0 = blockIdx.z * kStep; i0 < n; i0 += gridDim.z * kStep) {
-      Rows rows[kMoveAtOnce];
-      uint4 x[kMoveAtOnce];
+  auto meet = [] {
+    if constexpr (kChain == 32) __syncwarp();
+    else __syncthreads();
+  };
+  auto look_up = [&](int i0, Rows* to) {
 #pragma unroll
-      for (int u = 0; u < kMoveAtOnce; ++u) {
-        const int i = i0 + u * kTogether + r;
-        rows[u] = i < n ? rows_of(a, b, h, first, kept, i) : Rows{-1, -1};
-      }
-#pragma unroll
-      for (int u = 0; u < kMoveAtOnce; ++u)
-        if (rows[u].from >= 0) x[u] = plane[rows[u].from * kRow];
-      if (in_place) __syncthreads();
-#pragma unroll
-      for (int u = 0; u < kMoveAtOnce; ++u)
-        if (rows[u].from >= 0) plane[rows[u].to * kRow] = x[u];
+    for (int e = 0; e < kBeside; ++e) {
+      const int r = e * kChain + tid;
+      if (kStep % kChain == 0 || r < kStep) to[r] = i0 + r < n ? rows_of(a, b, h, first, kept, i0 + r) : Rows{-1, -1};
     }
-    return;
-  }
-  constexpr int kStep = kMoveThreads * kMoveAtOnce;
-  for (int i0 = blockIdx.z * kStep; i0 < n; i0 += gridDim.z * kStep) {
-    Rows rows[kMoveAtOnce];
-    unsigned char ke[kMoveAtOnce], ve[kMoveAtOnce];
-    float w[kMoveAtOnce];
+  };
+  const int r = tid / kOfPart, piece = part * kOfPart + tid % kOfPart;
+  uint4* plane = reinterpret_cast<uint4*>(piece < kRow ? a.k : a.v) + (piece < kRow ? piece : piece - kRow);
+  const bool beside = part == 0 && (a.k_exp != nullptr || a.weights != nullptr);
+  int i0 = blockIdx.z * kStep, buffer = 0;
+  if (i0 < n) look_up(i0, looked_up[threadIdx.x / kChain][0]);
+  meet();
+  for (; i0 < n; i0 += gridDim.z * kStep, buffer ^= 1) {
+    const Rows* rows = looked_up[threadIdx.x / kChain][buffer];
+    Rows mine[kMoveAtOnce], of_beside[kBeside];
+    uint4 x[kMoveAtOnce];
+    unsigned char ke[kBeside], ve[kBeside];
+    float w[kBeside];
 #pragma unroll
     for (int u = 0; u < kMoveAtOnce; ++u) {
-      const int i = i0 + u * kMoveThreads + threadIdx.x;
-      rows[u] = i < n ? rows_of(a, b, h, first, kept, i) : Rows{-1, -1};
-      if (rows[u].from < 0) continue;
-      if (a.k_exp != nullptr) {
-        ke[u] = a.k_exp[rows[u].from];
-        ve[u] = a.v_exp[rows[u].from];
-      }
-      if (a.weights != nullptr) w[u] = a.weights[rows[u].from];
+      mine[u] = rows[u * kTogether + r];
+      if (mine[u].from >= 0) x[u] = plane[static_cast<long long>(mine[u].from) * kRow];
     }
-    if (in_place) __syncthreads();
+    if (beside) {
 #pragma unroll
-    for (int u = 0; u < kMoveAtOnce; ++u) {
-      if (rows[u].from < 0) continue;
-      if (a.k_exp != nullptr) {
-        a.k_exp[rows[u].to] = ke[u];
-        a.v_exp[rows[u].to] = ve[u];
+      for (int e = 0; e < kBeside; ++e) {
+        const int at = e * kChain + tid;
+        of_beside[e] = kStep % kChain == 0 || at < kStep ? rows[at] : Rows{-1, -1};
+        if (of_beside[e].from < 0) continue;
+        if (a.k_exp != nullptr) {
+          ke[e] = a.k_exp[of_beside[e].from];
+          ve[e] = a.v_exp[of_beside[e].from];
+        }
+        if (a.weights != nullptr) w[e] = a.weights[of_beside[e].from];
       }
-      if (a.weights != nullptr) a.weights[rows[u].to] = w[u];
+    }
+    if (i0 + static_cast<int>(gridDim.z) * kStep < n) look_up(i0 + gridDim.z * kStep, looked_up[threadIdx.x / kChain][buffer ^ 1]);
+    meet();  // all of the step has been read, and the next one's rows are there
+#pragma unroll
+    for (int u = 0; u < kMoveAtOnce; ++u)
+      if (mine[u].from >= 0) plane[static_cast<long long>(mine[u].to) * kRow] = x[u];
+    if (beside) {
+#pragma unroll
+      for (int e = 0; e < kBeside; ++e) {
+        if (of_beside[e].from < 0) continue;
+        if (a.k_exp != nullptr) {
+          a.k_exp[of_beside[e].to] = ke[e];
+          a.v_exp[of_beside[e].to] = ve[e];
+        }
+        if (a.weights != nullptr) a.weights[of_beside[e].to] = w[e];
+      }
     }
   }
 }
@@ -299,23 +336,52 @@ int launched(cudaError_t err) {
   return err == cudaSuccess ? FTB_OK : FTB_ERR_LAUNCH;
 }
 
-template <int kRow, int kOfPart>
+template <int C>
+int launch_choose(const Choose& a, int B, cudaStream_t stream) {
+  static std::atomic<unsigned long long> configured{0};
+  // room for a CTA's stretch of the longest sequence that the table allows, as far as there is some
+  const long long longest = static_cast<long long>(a.batch.W) << a.batch.page_shift, stretch = (longest + C * kChooseThreads - 1) / (C * kChooseThreads) * kChooseThreads;
+  const int room = static_cast<int>(std::min(stretch, static_cast<long long>(kMostRoom)));
+  if (!ensure_dynamic_smem(paged_choose_kernel<C>, kMostRoom * 4, configured)) return FTB_ERR_LAUNCH;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(B) * a.kv_heads * C);
+  cfg.blockDim = dim3(kChooseThreads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(room) * 4;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = C;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = C > 1 ? 2 : 1;
+  return launched(cudaLaunchKernelEx(&cfg, paged_choose_kernel<C>, a, room));
+}
+int launch_choose(const Choose& a, int B, cudaStream_t stream) {
+  // Clusters where there are more keys than a few a thread and heads leave SMs without work.
+  const bool apart = (static_cast<long long>(a.batch.W) << a.batch.page_shift) > 4096 && static_cast<long long>(B) * a.kv_heads * 8 <= 4ll * current_sm_count();
+  return apart ? launch_choose<8>(a, B, stream) : launch_choose<1>(a, B, stream);
+}
+
+template <int kRow, int kOfPart, int kChain>
 int launch_move(const Move& a, int B, cudaStream_t stream) {
-  const bool in_place = a.into == a.batch.table;
-  const int parts = 2 * kRow / kOfPart + (a.k_exp != nullptr || a.weights != nullptr ? 1 : 0);
-  constexpr int kStep = kMoveThreads / kOfPart * kMoveAtOnce;
-  const long long heads = static_cast<long long>(B) * a.kv_heads;
-  const int steps = in_place ? 1 : static_cast<int>(std::min(static_cast<long long>((a.most + kStep - 1) / kStep), std::max(1ll, 65535ll)));
-  return launched(launch_light(paged_move_kernel<kRow, kOfPart>, dim3(static_cast<unsigned>(heads), parts, steps), dim3(kMoveThreads), 0, stream,
-                               a, in_place));
+  constexpr int kStep = kChain / kOfPart * kMoveAtOnce, kChains = kMoveThreads / kChain;
+  const int chains = B * a.kv_heads, blocks = (chains + kChains - 1) / kChains;
+  // into other pages: enough blocks for every SM's room for them twice, so that one's end lies under others' work
+  const int steps = (a.most + kStep - 1) / kStep;
+  const int z = a.into == a.batch.table ? 1 : std::min(steps, std::max(1, 16 * current_sm_count() / blocks));
+  return launched(launch_light(paged_move_kernel<kRow, kOfPart, kChain>, dim3(blocks, 2 * kRow / kOfPart, z), dim3(kMoveThreads), 0, stream, a, chains,
+                               a.into == a.batch.table));
 }
 template <int kRow>
 int launch_move(const Move& a, int B, cudaStream_t stream) {
-  const long long heads = static_cast<long long>(B) * a.kv_heads;
+  // A few rows of a tree: a warp has them in one step or two.
+  if (a.most <= 64) return launch_move<kRow, 2 * kRow, 32>(a, B, stream);
   // In the same pages a part of a row is a chain: narrow parts where there are few of them and long.
-  const bool in_place = a.into == a.batch.table;
-  if (in_place && a.most > 64 && heads * 8 <= 4ll * current_sm_count()) return launch_move<kRow, kRow / 4>(a, B, stream);
-  return launch_move<kRow, 2 * kRow>(a, B, stream);
+  if (a.into == a.batch.table && static_cast<long long>(B) * a.kv_heads * 8 <= 4ll * current_sm_count())
+    return launch_move<kRow, kRow / 4, kMoveThreads>(a, B, stream);
+  return launch_move<kRow, 2 * kRow, kMoveThreads>(a, B, stream);
 }
 int move(const Move& a, int row_bytes, int B, cudaStream_t stream) {
   return row_bytes == 256 ? launch_move<16>(a, B, stream) : row_bytes == 128 ? launch_move<8>(a, B, stream) : launch_move<4>(a, B, stream);
@@ -328,6 +394,7 @@ int check_cache(const void* k, const void* v, const void* k_exp, const void* v_e
   if (B <= 0 || W <= 0 || (into != nullptr && into_W <= 0) || pages <= 0 || kv_heads <= 0 || kv_heads > 65536) return FTB_ERR_ARG;
   if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) return FTB_ERR_ARG;
   if ((d != 64 && d != 128) || static_cast<long long>(B) * kv_heads > INT_MAX / 8) return FTB_ERR_ARG;
+  if (static_cast<long long>(pages) * kv_heads > INT_MAX / page_size) return FTB_ERR_ARG;  // rows are counted in 32 bits (so many would be 137 GB or more)
   if (((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(k_exp) | reinterpret_cast<uintptr_t>(v_exp)) & 15) != 0)
     return FTB_ERR_ALIGN;
   return FTB_OK;
@@ -379,8 +446,7 @@ extern "C" int ftb_paged_cache_evict(void* k_cache, void* v_cache, unsigned char
   int* status = static_cast<int*>(workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const Choose c{batch, weights, kept, lens_out, kv_heads, keep, recent, status};
-  const unsigned heads = static_cast<unsigned>(B) * kv_heads;
-  rc = launched(launch_light(paged_choose_kernel<1>, dim3(heads), dim3(kChooseThreads), 0, s, c));
+  rc = launch_choose(c, B, s);
   if (rc) return rc;
   const Move m{batch, into != nullptr ? into : table, into != nullptr ? into_W : W, kept, lens_out, nullptr, static_cast<long long>(kv_heads) * keep,
                keep, keep, kv_heads, static_cast<unsigned char*>(k_cache), static_cast<unsigned char*>(v_cache), k_exp, v_exp, weights, status};
