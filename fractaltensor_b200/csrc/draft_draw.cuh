@@ -10,8 +10,6 @@
 
 namespace ftb {
 
-constexpr int kUnroll = 8;
-
 // What is not positive and finite counts as 0, in the target's rows and in the draft's.
 __device__ __forceinline__ double probability(float x) {
   x = fmaxf(x, 0.f);  // (0 of a NaN)
@@ -37,12 +35,13 @@ struct DrawRoom {  // in shared memory
   int found, heavy;
 };
 
-// The row: row.p(j) and row.q(j) load what row.weight(p, q, j) takes; a warp says row.look(j) before it weighs numbers of j .. j + 32 * kUnroll - 1;
-// row.all() stops leaving out what it leaves out, for the case that nothing else weighs anything.  C: CTAs of a cluster.  All threads; one thread of one of the CTAs writes the token; -> sum(w),
+// The row: row.p(j) and row.q(j) load what row.weight(p, q, j) takes; a warp says row.look(j, n) before it weighs numbers of j .. j + n - 1;
+// row.all() stops leaving out what it leaves out, for the case that nothing else weighs anything.  C: CTAs of a cluster; kAhead: the next numbers are on their way while
+// some are weighed.  All threads; one thread of one of the CTAs writes the token; -> sum(w),
 // where it is 0 nothing is written.  A cluster meets once more before one of its CTAs leaves.
-template <int C, int kThreads, typename Row>
+template <int C, int kThreads, bool kAhead, typename Row>
 __device__ __forceinline__ double draw_token(Row& row, int V, double share, int rank, DrawRoom<C, kThreads>& room, long long* token) {
-  constexpr int kWarps = kThreads / 32;
+  constexpr int kWarps = kThreads / 32, kUnroll = 8;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // a warp's stretch of the row: whole groups of 32
   const int stretch = ((V + C * kThreads - 1) / (C * kThreads)) * 32;
@@ -50,17 +49,28 @@ __device__ __forceinline__ double draw_token(Row& row, int V, double share, int 
   double total = 0.0, before = 0.0;  // of the row; of the CTAs in front of this one
   for (int tries = 0; tries < 2; ++tries) {  // where p and q are the same, nothing is left of the difference: p itself
     double s = 0.0;
-    for (int j = from; j < to; j += 32 * kUnroll) {
-      float pv[kUnroll], qv[kUnroll];
+    float pv[kUnroll], qv[kUnroll];
+    auto load = [&](int j) {
 #pragma unroll
       for (int k = 0; k < kUnroll; ++k) {
         const int at = j + k * 32 + lane;
         pv[k] = at < to ? row.p(at) : 0.f;
         qv[k] = at < to ? row.q(at) : 0.f;
       }
-      row.look(j);
+    };
+    if (kAhead) load(from);
+    for (int j = from; j < to; j += 32 * kUnroll) {
+      float p[kUnroll], q[kUnroll];
+      if (!kAhead) load(j);
 #pragma unroll
-      for (int k = 0; k < kUnroll; ++k) s += row.weight(pv[k], qv[k], j + k * 32 + lane);
+      for (int k = 0; k < kUnroll; ++k) {
+        p[k] = pv[k];
+        q[k] = qv[k];
+      }
+      if (kAhead) load(j + 32 * kUnroll);
+      row.look(j, 32 * kUnroll);
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k) s += row.weight(p[k], q[k], j + k * 32 + lane);
     }
     s = warp_sum(s);
     if (lane == 0) room.sums[warp] = s;
@@ -134,7 +144,7 @@ __device__ __forceinline__ double draw_token(Row& row, int V, double share, int 
         pv[k] = j + k < end_at ? row.p(j + k) : 0.f;
         qv[k] = j + k < end_at ? row.q(j + k) : 0.f;
       }
-      row.look(j - lane * kUnroll);
+      row.look(j - lane * kUnroll, 32 * kUnroll);
 #pragma unroll
       for (int k = 0; k < kUnroll; ++k) {
         w[k] = row.weight(pv[k], qv[k], j + k);

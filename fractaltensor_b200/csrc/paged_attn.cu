@@ -25,6 +25,7 @@ namespace {
 constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kJoinRows = 4, kMostCuts = 4 * kJoinThreads;
 
 constexpr float kLog2E = 1.4426950408889634f;
+constexpr int kShortUnits = 5500;
 
 struct Pieces {
   const float* parts;
@@ -276,6 +277,7 @@ int launch_join(const PagedAttn& a, int d, const Pieces& few, const Pieces& many
 // of so many for the others.
 struct Form {
   int few, most, many;
+  bool split;  // the rows behind a sequence's last whole tile of paged_tile.cu, if they make one tile of paged_short.cu, go there
 };
 Form form_of(int T, int B, int group) {
   const long long rows = static_cast<long long>(T) * group;
@@ -283,14 +285,32 @@ Form form_of(int T, int B, int group) {
   // L2: 256 sequences, all but one without a token, 8 kv heads, 1000 keys, 24 tokens 23 us (with paged_tile.cu beside it 32), 100 tokens
   // 56 (39), 200 tokens 108 (41).  A step of a token each pays for that second launch: 8 sequences 15 us (23), 64 of up to 8000 keys 179
   // (186).  Which it is stands on the device alone.
-  if (T <= B) return {rows <= 8ll * B ? 8 : 16, INT_MAX, 0};
-  if (rows <= 16) return {rows <= 8 ? 8 : 16, INT_MAX, 0};
+  if (T <= B) return {rows <= 8ll * B ? 8 : 16, INT_MAX, 0, false};
+  if (rows <= 16) return {rows <= 8 ? 8 : 16, INT_MAX, 0, false};
   const int many = rows > 128ll * B ? 256 : 128;
-  if (B == 1) return {0, 0, many};
+  if (B == 1) return {0, 0, many, false};
   // One tile of paged_short.cu: a second one would read the keys again.  96 sequences, 8 kv heads, 4500 keys of 16 bits: 8 rows
   // 273 us, 16 rows 302, as rows of paged_tile.cu 24 349, 64 367, 128 405; 8500 keys of 8 bits: 327, 400, then 650, 679, 728.
   const int few = group <= 8 && rows > 16ll * B ? 8 : 16;
-  return {few, few, many};
+  return {few, few, many, false};
+}
+
+// The same for trees, of which a sequence has a few dozen tokens; `keys`: as many as the table has room for.  While the tiles of
+// paged_short.cu make few units of 64 keys, its CTAs, two of them an SM, are done sooner, however many tiles read the same keys: one sequence of
+// 25 tokens, 32 heads over 8 kv heads, 16 bits: 800 keys (728 units) 23.5 us and 27.6 with paged_tile.cu, 3200: 30.9 and 36.6, 6400 (5600): 40.6 and
+// 43.7; of 60 tokens, 3200 keys (6000): 46.0 and 46.0, 6400: 67.5 and 58.2.
+Form form_of_tree(int T, int B, int group, int kv_heads, long long keys) {
+  Form f = form_of(T, B, group);
+  if (f.many == 0) return f;
+  const long long rows = static_cast<long long>(T) * group;
+  if ((rows + 16ll * B - 1) / (16ll * B) * B * kv_heads * ((keys + 63) / 64) <= kShortUnits) return {16, INT_MAX, 0, false};
+  // A second tile for a few rows costs as much as the first: 32 sequences of 33 tokens of 8 heads each of 8 kv heads, up to 16 000 keys of 8 bits, 720 us
+  // with the last 8 rows apart, 945 without.
+  const long long behind = rows / B > f.many ? rows / B % f.many : 0;
+  if (B == 1 && (behind == 0 || behind > 16)) return f;
+  if (behind > 0 && behind <= 16) f.few = f.most = behind <= 8 ? 8 : 16;
+  f.split = true;
+  return f;
 }
 
 size_t places(int pieces, int rows, int d) { return 2 * static_cast<size_t>(pieces) * rows * (d + 2) * sizeof(float) + pieces * sizeof(PagedCut); }
@@ -304,8 +324,10 @@ using namespace ftb;
 extern "C" size_t ftb_paged_attn_scratch_bytes(int T, int B, int kv_heads, int group, int d) {
   if (T <= 0 || B <= 0 || kv_heads <= 0 || group <= 0 || d <= 0) return 0;
   const Form f = form_of(T, B, group);
-  size_t n = rounded(static_cast<size_t>(T) * kv_heads * group * sizeof(uint32_t));
-  if (f.few > 0) n += rounded(places(paged_short_pieces(f.few), f.few, d));
+  size_t n = rounded(static_cast<size_t>(T) * kv_heads * group * sizeof(uint32_t)), few = 0;
+  for (int rows = 8; rows <= 16; rows += 8)  // (a tree may take either)
+    if (f.few == rows || f.many > 0) few = std::max(few, rounded(places(paged_short_pieces(rows), rows, d)));
+  n += few;
   if (f.many > 0) n += rounded(places(paged_tile_pieces(), f.many, d));
   return n;
 }
@@ -378,7 +400,7 @@ extern "C" int ftb_paged_attn_tree_fwd(const void* q, long long q_row, long long
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (scratch == nullptr || scratch_bytes < ftb_paged_attn_scratch_bytes(T, B, kv_heads, group, d)) return FTB_ERR_WORKSPACE;
   if ((reinterpret_cast<uintptr_t>(scratch) & 15) != 0) return FTB_ERR_ALIGN;
-  const Form f = form_of(T, B, group);
+  const Form f = tree != nullptr ? form_of_tree(T, B, group, kv_heads, static_cast<long long>(W) * page_size) : form_of(T, B, group);
   unsigned char* at = static_cast<unsigned char*>(scratch);
   a.odd = static_cast<uint32_t*>(scratch);
   at += rounded(static_cast<size_t>(T) * kv_heads * group * sizeof(uint32_t));
@@ -388,6 +410,8 @@ extern "C" int ftb_paged_attn_tree_fwd(const void* q, long long q_row, long long
   };
   Pieces few{nullptr, nullptr, 0, 0}, many{nullptr, nullptr, 0, 0};
   int err = FTB_OK;
+  a.split = f.split ? f.many : 0;
+  a.rest = f.few;
   // (the kernel for few rows first: it lives on L1, of which the other one's shared memory leaves next to nothing until an SM is
   // empty: 378 against 294 us behind it for 96 sequences of 16 rows)
   if (f.few > 0) {

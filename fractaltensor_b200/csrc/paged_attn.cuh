@@ -14,6 +14,7 @@ struct PagedAttn {
   const unsigned char *k, *v, *k_exp, *v_exp;
   int T, kv_heads, group, window;  // window 0: none
   int least_rows, most_rows;       // sequences with so many rows (token, head of a group) of a kv head are this launch's
+  int split, rest;                 // split > 0: of longer ones, rows behind the last whole tile of so many go to the kernel for few rows, if `rest` or fewer
   float scale_log2;
   int* status;
   uint32_t* odd;                   // [T, heads]: not 0 where a row of the output has to be computed again, key by key

@@ -29,7 +29,7 @@ struct Choose {
   int* status;
 };
 
-constexpr int kChooseThreads = 512, kChooseWarps = kChooseThreads / 32, kBins = 256, kCopies = 4, kChooseAtOnce = 8;
+constexpr int kBins = 256, kCopies = 4, kChooseAtOnce = 8;
 
 // Unsigned numbers in the order of the weights; NaN is below all of them.
 __device__ __forceinline__ uint32_t order_of(float w) {
@@ -45,11 +45,12 @@ __device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
 }
 
 // C CTAs for each sequence and kv head, a stretch of the keys each, of which `room` stay in shared memory after they have been read.
-template <int C>
-__global__ void __launch_bounds__(kChooseThreads)
+template <int C, int kThreads>
+__global__ void __launch_bounds__(kThreads)
 paged_choose_kernel(const __grid_constant__ Choose a, int room) {
+  constexpr int kWarps = kThreads / 32;
   extern __shared__ uint32_t known_keys[];
-  __shared__ int bins[kCopies][kBins], sums[2][kBins], above_of[kChooseWarps], equal_of[kChooseWarps], mine[2];
+  __shared__ int bins[2][kCopies][kBins], sums[2][kBins], above_of[kWarps], equal_of[kWarps], mine[2], of_warp[kBins / 32];
   __shared__ int s_digit, s_left;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rank = C > 1 ? static_cast<int>(cluster_ctarank()) : 0, head = blockIdx.x / C;
@@ -62,13 +63,13 @@ paged_choose_kernel(const __grid_constant__ Choose a, int room) {
     a.lens_out[b] = min(L, a.keep);
   }
   int* kept = a.kept + static_cast<long long>(head) * a.keep;
-  const int at = rank * kChooseThreads + threadIdx.x;
+  const int at = rank * kThreads + threadIdx.x;
   if (L <= a.keep) {
-    for (int i = at; i < a.keep; i += C * kChooseThreads) kept[i] = i < L ? i : -1;
+    for (int i = at; i < a.keep; i += C * kThreads) kept[i] = i < L ? i : -1;
     return;
   }
   const int old = L - a.recent, want = a.keep - a.recent;  // 0 <= want < old
-  for (int i = at; i < a.recent; i += C * kChooseThreads) kept[want + i] = old + i;
+  for (int i = at; i < a.recent; i += C * kThreads) kept[want + i] = old + i;
   if (want == 0) return;
   const int* table = a.batch.table + static_cast<long long>(b) * a.batch.W;
   const int shift = a.batch.page_shift, in_page = (1 << shift) - 1;
@@ -78,17 +79,19 @@ paged_choose_kernel(const __grid_constant__ Choose a, int room) {
     return order_of(a.weights[(((static_cast<long long>(page) * a.kv_heads) + h) << shift) + (i & in_page)]);
   };
   // a warp's stretch: whole groups of 32
-  const int stretch = (old + C * kChooseThreads - 1) / (C * kChooseThreads) * 32;
-  const int from = static_cast<int>(min(static_cast<long long>(old), static_cast<long long>(rank * kChooseWarps + warp) * stretch));
+  const int stretch = (old + C * kThreads - 1) / (C * kThreads) * 32;
+  const int from = static_cast<int>(min(static_cast<long long>(old), static_cast<long long>(rank * kWarps + warp) * stretch));
   const int to = static_cast<int>(min(static_cast<long long>(old), static_cast<long long>(from) + stretch));
-  const int first = static_cast<int>(min(static_cast<long long>(old), static_cast<long long>(rank) * kChooseWarps * stretch));  // of the CTA's
+  const int first = static_cast<int>(min(static_cast<long long>(old), static_cast<long long>(rank) * kWarps * stretch));  // of the CTA's
   auto key_of = [&](int i) -> uint32_t { return i - first < room ? known_keys[i - first] : key_at(i); };
   uint32_t prefix = 0, known = 0;  // the digits so far, and which bits they are
   int left = want;
+  for (int i = threadIdx.x; i < kCopies * kBins; i += kThreads) (&bins[0][0][0])[i] = 0;
+  __syncthreads();
   for (int d = 0; d < 4; ++d) {
     const int low = 24 - 8 * d;
-    for (int i = threadIdx.x; i < kCopies * kBins; i += kChooseThreads) (&bins[0][0])[i] = 0;
-    __syncthreads();
+    int* bin = bins[d & 1][warp % kCopies];
+    for (int i = threadIdx.x; i < kCopies * kBins; i += kThreads) (&bins[(d & 1) ^ 1][0][0])[i] = 0;  // the next digit's
     if (d == 0) {
       for (int i0 = from; i0 < to; i0 += 32 * kChooseAtOnce) {
         int page[kChooseAtOnce];
@@ -112,55 +115,47 @@ paged_choose_kernel(const __grid_constant__ Choose a, int room) {
           if (i >= to) continue;
           const uint32_t key = order_of(w[u]);
           if (i - first < room) known_keys[i - first] = key;
-          atomicAdd(&bins[warp % kCopies][key >> low], 1);
+          atomicAdd(bin + (key >> low), 1);
         }
       }
     } else {
       for (int i = from + lane; i < to; i += 32) {
         const uint32_t key = key_of(i);
-        if ((key & known) == prefix) atomicAdd(&bins[warp % kCopies][key >> low & 255u], 1);
+        if ((key & known) == prefix) atomicAdd(bin + (key >> low & 255u), 1);
       }
     }
     __syncthreads();
+    // thread i: bin 255 - i, and how many keys are in the bins above
     int* of_cta = sums[d & 1];  // (the other one may still be read by a CTA of the cluster)
+    int count = 0, upto = 0;
     if (threadIdx.x < kBins) {
-      int n = 0;
 #pragma unroll
-      for (int c = 0; c < kCopies; ++c) n += bins[c][threadIdx.x];
-      of_cta[threadIdx.x] = n;
+      for (int c = 0; c < kCopies; ++c) count += bins[d & 1][c][255 - threadIdx.x];
+      of_cta[threadIdx.x] = count;
     }
-    if constexpr (C > 1) cluster_sync_all();
-    else __syncthreads();
-    if (warp == 0) {  // lane i: the eight bins from 255 - 8 i downwards
-      int n[8], sum = 0;
+    if constexpr (C > 1) {
+      cluster_sync_all();
+      if (threadIdx.x < kBins) {
+        count = 0;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int bin = 255 - (lane * 8 + k);
-        n[k] = 0;
-        if constexpr (C > 1) {
-#pragma unroll
-          for (int r = 0; r < C; ++r) n[k] += ld_cluster_s32(map_to_cta(smem_u32(&of_cta[bin]), r));
-        } else {
-          n[k] = of_cta[bin];
-        }
-        sum += n[k];
+        for (int r = 0; r < C; ++r) count += ld_cluster_s32(map_to_cta(smem_u32(&of_cta[threadIdx.x]), r));
       }
-      int upto = sum;
+    }
+    if (threadIdx.x < kBins) {
+      upto = count;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += y;
       }
-      int before = upto - sum;
-      if (before < left && upto >= left) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (before < left && before + n[k] >= left) {
-            s_digit = 255 - (lane * 8 + k);
-            s_left = left - before;
-          }
-          before += n[k];
-        }
+      if (lane == 31) of_warp[warp] = upto;
+    }
+    __syncthreads();
+    if (threadIdx.x < kBins) {
+      for (int w = 0; w < warp; ++w) upto += of_warp[w];
+      if (upto - count < left && upto >= left) {
+        s_digit = 255 - threadIdx.x;
+        s_left = left - (upto - count);
       }
     }
     __syncthreads();
@@ -185,7 +180,7 @@ paged_choose_kernel(const __grid_constant__ Choose a, int room) {
   above = equal = 0;  // in front of this warp's stretch
   int all_above = 0, all_equal = 0;
 #pragma unroll
-  for (int w = 0; w < kChooseWarps; ++w) {
+  for (int w = 0; w < kWarps; ++w) {
     if (w < warp) {
       above += above_of[w];
       equal += equal_of[w];
@@ -238,32 +233,33 @@ constexpr int kMoveThreads = 256, kMoveAtOnce = 8, kMostRoom = 48 * 1024;
 struct Rows {
   int from, to;
 };
-__device__ __forceinline__ Rows rows_of(const Move& a, int b, int h, int first, const int* kept, int i) {
-  const int k = kept[i];
-  PagedBatch into = a.batch;
-  into.table = a.into;
-  into.W = a.into_W;
-  if (k < 0 || first < 0) {
-    atomicCAS(a.status, 0, FTB_ERR_INDEX);
-    return {-1, -1};
-  }
+// The page at position pos of one of a sequence's tables as it stands there; -1 behind its width.
+__device__ __forceinline__ int page_there(const int* table, int W, int shift, long long pos) {
+  const long long i = pos >> shift;
+  return i < W ? __ldg(table + i) : -1;
+}
+__device__ __forceinline__ Rows rows_of(const Move& a, int h, int first, int k, int i, int from, int to) {
   const int shift = a.batch.page_shift, in_page = (1 << shift) - 1;
   const long long src = static_cast<long long>(first) + k, dst = static_cast<long long>(first) + i;
   if (src == dst && a.into == a.batch.table) return {-1, -1};  // where it is
-  const int from = page_of(a.batch, b, src, a.status), to = page_of(into, b, dst, a.status);
-  if (from < 0 || to < 0) return {-1, -1};
+  if (k < 0 || first < 0 || from < 0 || from >= a.batch.pages || to < 0 || to >= a.batch.pages) {
+    atomicCAS(a.status, 0, FTB_ERR_INDEX);
+    return {-1, -1};
+  }
   return {((from * a.kv_heads + h) << shift) + static_cast<int>(src & in_page), ((to * a.kv_heads + h) << shift) + static_cast<int>(dst & in_page)};
 }
 
 // A chain is kChain threads': block (x, y, z) has the chains of sequences and kv heads 256 / kChain * x and on, part y of a row, every
 // gridDim.z-th step of rows.  kRow: 16-byte pieces of a key or value, kOfPart: pieces of a part of both together; exponents and weights go with part 0.
 // The rows of the next step are looked up while this one's are on their way.
-template <int kRow, int kOfPart, int kChain>
+// C: CTAs of a chain, a cluster, which take so many steps at once.
+template <int kRow, int kOfPart, int kChain, int C>
 __global__ void __launch_bounds__(kMoveThreads)
 paged_move_kernel(const __grid_constant__ Move a, int chains, bool in_place) {
   constexpr int kTogether = kChain / kOfPart, kStep = kTogether * kMoveAtOnce, kBeside = (kStep + kChain - 1) / kChain;
   __shared__ Rows looked_up[kMoveThreads / kChain][2][kStep];
-  const int chain = blockIdx.x * (kMoveThreads / kChain) + threadIdx.x / kChain, tid = threadIdx.x % kChain, part = blockIdx.y;
+  const int rank = C > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int chain = blockIdx.x / C * (kMoveThreads / kChain) + threadIdx.x / kChain, tid = threadIdx.x % kChain, part = blockIdx.y;
   grid_launch_dependents();
   grid_dependency_wait();
   if (kChain < kMoveThreads && chain >= chains) return;  // (a warp leaves as one)
@@ -271,23 +267,39 @@ paged_move_kernel(const __grid_constant__ Move a, int chains, bool in_place) {
   const int n = min(max(a.counts[b], 0), a.most), first = a.first != nullptr ? a.first[b] : 0;
   const int* kept = a.kept + b * a.kept_seq + h * a.kept_head;
   auto meet = [] {
-    if constexpr (kChain == 32) __syncwarp();
+    if constexpr (C > 1) cluster_sync_all();
+    else if constexpr (kChain == 32) __syncwarp();
     else __syncthreads();
   };
-  auto look_up = [&](int i0, Rows* to) {
+  const int *table = a.batch.table + static_cast<long long>(b) * a.batch.W, *into = a.into + static_cast<long long>(b) * a.into_W;
+  auto look_up = [&](int i0, Rows* rows) {  // (all loads of a kind together: two trips to memory, however many rows a thread has)
+    int k[kBeside], from[kBeside], to[kBeside];
+#pragma unroll
+    for (int e = 0; e < kBeside; ++e) {
+      const int i = i0 + e * kChain + tid;
+      k[e] = i < n && (kStep % kChain == 0 || e * kChain + tid < kStep) ? __ldg(kept + i) : -1;
+    }
+#pragma unroll
+    for (int e = 0; e < kBeside; ++e) {
+      const bool fine = k[e] >= 0 && first >= 0;
+      from[e] = fine ? page_there(table, a.batch.W, a.batch.page_shift, static_cast<long long>(first) + k[e]) : -1;
+      to[e] = fine ? page_there(into, a.into_W, a.batch.page_shift, static_cast<long long>(first) + i0 + e * kChain + tid) : -1;
+    }
 #pragma unroll
     for (int e = 0; e < kBeside; ++e) {
       const int r = e * kChain + tid;
-      if (kStep % kChain == 0 || r < kStep) to[r] = i0 + r < n ? rows_of(a, b, h, first, kept, i0 + r) : Rows{-1, -1};
+      if (kStep % kChain == 0 || r < kStep) rows[r] = i0 + r < n ? rows_of(a, h, first, k[e], i0 + r, from[e], to[e]) : Rows{-1, -1};
     }
   };
   const int r = tid / kOfPart, piece = part * kOfPart + tid % kOfPart;
   uint4* plane = reinterpret_cast<uint4*>(piece < kRow ? a.k : a.v) + (piece < kRow ? piece : piece - kRow);
   const bool beside = part == 0 && (a.k_exp != nullptr || a.weights != nullptr);
-  int i0 = blockIdx.z * kStep, buffer = 0;
-  if (i0 < n) look_up(i0, looked_up[threadIdx.x / kChain][0]);
-  meet();
-  for (; i0 < n; i0 += gridDim.z * kStep, buffer ^= 1) {
+  const int by = C > 1 ? C * kStep : static_cast<int>(gridDim.z) * kStep;
+  int i0 = (C > 1 ? rank : static_cast<int>(blockIdx.z)) * kStep, buffer = 0;
+  look_up(i0, looked_up[threadIdx.x / kChain][0]);
+  if constexpr (kChain == 32) __syncwarp();
+  else __syncthreads();
+  for (; i0 - rank * kStep < n; i0 += by, buffer ^= 1) {  // (the same steps for all of a cluster)
     const Rows* rows = looked_up[threadIdx.x / kChain][buffer];
     Rows mine[kMoveAtOnce], of_beside[kBeside];
     uint4 x[kMoveAtOnce];
@@ -311,7 +323,7 @@ paged_move_kernel(const __grid_constant__ Move a, int chains, bool in_place) {
         if (a.weights != nullptr) w[e] = a.weights[of_beside[e].from];
       }
     }
-    if (i0 + static_cast<int>(gridDim.z) * kStep < n) look_up(i0 + gridDim.z * kStep, looked_up[threadIdx.x / kChain][buffer ^ 1]);
+    if (i0 - rank * kStep + by < n) look_up(i0 + by, looked_up[threadIdx.x / kChain][buffer ^ 1]);
     meet();  // all of the step has been read, and the next one's rows are there
 #pragma unroll
     for (int u = 0; u < kMoveAtOnce; ++u)
@@ -336,17 +348,13 @@ int launched(cudaError_t err) {
   return err == cudaSuccess ? FTB_OK : FTB_ERR_LAUNCH;
 }
 
-template <int C>
-int launch_choose(const Choose& a, int B, cudaStream_t stream) {
-  static std::atomic<unsigned long long> configured{0};
-  // room for a CTA's stretch of the longest sequence that the table allows, as far as there is some
-  const long long longest = static_cast<long long>(a.batch.W) << a.batch.page_shift, stretch = (longest + C * kChooseThreads - 1) / (C * kChooseThreads) * kChooseThreads;
-  const int room = static_cast<int>(std::min(stretch, static_cast<long long>(kMostRoom)));
-  if (!ensure_dynamic_smem(paged_choose_kernel<C>, kMostRoom * 4, configured)) return FTB_ERR_LAUNCH;
+// Clusters of C along x.
+template <typename... KArgs, typename... Args>
+int launch_clusters(void (*kfn)(KArgs...), int C, dim3 grid, int threads, size_t smem, cudaStream_t stream, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(B) * a.kv_heads * C);
-  cfg.blockDim = dim3(kChooseThreads);
-  cfg.dynamicSmemBytes = static_cast<size_t>(room) * 4;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -356,32 +364,45 @@ int launch_choose(const Choose& a, int B, cudaStream_t stream) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = C > 1 ? 2 : 1;
-  return launched(cudaLaunchKernelEx(&cfg, paged_choose_kernel<C>, a, room));
-}
-int launch_choose(const Choose& a, int B, cudaStream_t stream) {
-  // Clusters where there are more keys than a few a thread and heads leave SMs without work.
-  const bool apart = (static_cast<long long>(a.batch.W) << a.batch.page_shift) > 4096 && static_cast<long long>(B) * a.kv_heads * 8 <= 4ll * current_sm_count();
-  return apart ? launch_choose<8>(a, B, stream) : launch_choose<1>(a, B, stream);
+  return launched(cudaLaunchKernelEx(&cfg, kfn, static_cast<KArgs>(args)...));
 }
 
-template <int kRow, int kOfPart, int kChain>
+template <int C, int kThreads>
+int launch_choose(const Choose& a, int B, cudaStream_t stream) {
+  static std::atomic<unsigned long long> configured{0};
+  // room for a CTA's stretch of the longest sequence that the table allows, as far as there is some
+  const long long longest = static_cast<long long>(a.batch.W) << a.batch.page_shift, stretch = (longest + C * kThreads - 1) / (C * kThreads) * kThreads;
+  const int room = static_cast<int>(std::min(stretch, static_cast<long long>(kMostRoom)));
+  if (!ensure_dynamic_smem(paged_choose_kernel<C, kThreads>, kMostRoom * 4, configured)) return FTB_ERR_LAUNCH;
+  return launch_clusters(paged_choose_kernel<C, kThreads>, C, dim3(static_cast<unsigned>(B) * a.kv_heads * C), kThreads, static_cast<size_t>(room) * 4,
+                         stream, a, room);
+}
+// Whether eight CTAs to a sequence and kv head are no more than the device has room for at a time.
+bool few_heads(int B, int kv_heads) { return static_cast<long long>(B) * kv_heads * 8 <= 2ll * current_sm_count(); }
+
+int launch_choose(const Choose& a, int B, cudaStream_t stream) {
+  const bool apart = (static_cast<long long>(a.batch.W) << a.batch.page_shift) > 4096 && few_heads(B, a.kv_heads);
+  return apart ? launch_choose<8, 1024>(a, B, stream) : launch_choose<1, 512>(a, B, stream);
+}
+
+template <int kRow, int kOfPart, int kChain, int C>
 int launch_move(const Move& a, int B, cudaStream_t stream) {
   constexpr int kStep = kChain / kOfPart * kMoveAtOnce, kChains = kMoveThreads / kChain;
-  const int chains = B * a.kv_heads, blocks = (chains + kChains - 1) / kChains;
+  const int chains = B * a.kv_heads, blocks = (chains + kChains - 1) / kChains * C;
   // into other pages: enough blocks for every SM's room for them twice, so that one's end lies under others' work
   const int steps = (a.most + kStep - 1) / kStep;
   const int z = a.into == a.batch.table ? 1 : std::min(steps, std::max(1, 16 * current_sm_count() / blocks));
-  return launched(launch_light(paged_move_kernel<kRow, kOfPart, kChain>, dim3(blocks, 2 * kRow / kOfPart, z), dim3(kMoveThreads), 0, stream, a, chains,
-                               a.into == a.batch.table));
+  return launch_clusters(paged_move_kernel<kRow, kOfPart, kChain, C>, C, dim3(blocks, 2 * kRow / kOfPart, z), kMoveThreads, 0, stream, a, chains,
+                         a.into == a.batch.table);
 }
 template <int kRow>
 int launch_move(const Move& a, int B, cudaStream_t stream) {
   // A few rows of a tree: a warp has them in one step or two.
-  if (a.most <= 64) return launch_move<kRow, 2 * kRow, 32>(a, B, stream);
-  // In the same pages a part of a row is a chain: narrow parts where there are few of them and long.
-  if (a.into == a.batch.table && static_cast<long long>(B) * a.kv_heads * 8 <= 4ll * current_sm_count())
-    return launch_move<kRow, kRow / 4, kMoveThreads>(a, B, stream);
-  return launch_move<kRow, 2 * kRow, kMoveThreads>(a, B, stream);
+  if (a.most <= 64) return launch_move<kRow, 2 * kRow, 32, 1>(a, B, stream);
+  // In the same pages a part of a row is a chain: narrow parts, and clusters that read thousands of rows before they write them, where there
+  // are few chains and long ones.
+  if (a.into == a.batch.table && few_heads(B, a.kv_heads)) return launch_move<kRow, kRow / 4, kMoveThreads, 8>(a, B, stream);
+  return launch_move<kRow, 2 * kRow, kMoveThreads, 1>(a, B, stream);
 }
 int move(const Move& a, int row_bytes, int B, cudaStream_t stream) {
   return row_bytes == 256 ? launch_move<16>(a, B, stream) : row_bytes == 128 ? launch_move<8>(a, B, stream) : launch_move<4>(a, B, stream);

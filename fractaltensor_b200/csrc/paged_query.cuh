@@ -1,10 +1,17 @@
-// Query rows as operands of mma.m16n8k16 with the keys on the M side.
+// Keys and query rows as operands of mma.m16n8k16 with the keys on the M side.
 #pragma once
 #include <type_traits>
 
 #include "paged_attn.cuh"
 
 namespace ftb {
+
+// 16 bytes that nobody else asks for.
+__device__ __forceinline__ uint4 load_once(const unsigned char* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
 
 // Row `row` of a tile of `rows` that begins with flat0 (token, head of the group) of a sequence whose tokens begin with row `first`: lane (g, c) holds
 // of it what it holds of a key, d = 32 j + 8 c .. + 7 (8-bit caches: 64 j + 16 c .. + 15); zeros behind the last row.  -> what the

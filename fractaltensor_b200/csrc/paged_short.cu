@@ -43,12 +43,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ uint4 load_once(const unsigned char* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-
 template <int D, int NT>
 struct Merge {
   float o[kWarps][NT * 8][D + 4];  // (rows 16 bytes apart in the banks)
@@ -74,11 +68,11 @@ paged_short_kernel(const __grid_constant__ PagedAttn a, float* __restrict__ part
   const int piece = blockIdx.x;
   grid_dependency_wait();
   grid_launch_dependents();
-  PagedWalk<R, kUnitKeys> walk;
+  PagedWalk<R, kUnitKeys, kMore> walk;
   {
     int b;
     long long at;
-    const PagedLine line = paged_line<R, kUnitKeys>(a, piece, gridDim.x, kAtLeast, s_line, &b, &at);
+    const PagedLine line = paged_line<R, kUnitKeys, kMore>(a, piece, gridDim.x, kAtLeast, s_line, &b, &at);
     if (piece >= line.pieces || line.total == 0) {
       if (threadIdx.x == 0) cuts[piece].last = -1;
       return;

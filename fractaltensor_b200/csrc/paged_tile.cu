@@ -199,7 +199,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
   }
   int seq0;
   long long at0;
-  const PagedLine line = paged_line<R, kKeys>(a, piece, gridDim.x, kAtLeast, ctl.line, &seq0, &at0);
+  const PagedLine line = paged_line<R, kKeys, kMore>(a, piece, gridDim.x, kAtLeast, ctl.line, &seq0, &at0);
   const bool idle = piece >= line.pieces || line.total == 0;
   if (idle || ctl.dead != 0) {
     if (threadIdx.x == 0) cuts[piece].last = -1;
@@ -227,7 +227,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
 
   if (warp == 0) {
     // --------------------------------------------------------- the walk, and the loads
-    PagedWalk<R, kKeys> walk;
+    PagedWalk<R, kKeys, kMore> walk;
     walk.begin(a, line, piece, seq0, at0);
     const int pages = kKeys >> a.batch.page_shift;  // of a block
     int slot = 0, edges = 0;

@@ -30,8 +30,10 @@ static_assert(kWarps * 32 == kLineThreads, "the line is laid out by a block");
 template <int R>
 __device__ __forceinline__ int cost_of(const PagedSeq& s) { return (s.flats + R - 1) / R; }
 
+constexpr int blocks_per_sm(int nt) { return nt == 1 ? 4 : 3; }
+
 template <typename T, bool k8, int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, blocks_per_sm(NT))
 paged_weigh_kernel(const __grid_constant__ Weigh x) {
   using C = typename std::conditional<k8, __half, T>::type;
   constexpr int R = NT * 8, kSteps = D / 16, kKLoads = k8 ? D / 64 : D / 32;
@@ -46,118 +48,173 @@ paged_weigh_kernel(const __grid_constant__ Weigh x) {
     return static_cast<long long>(blocks_of<kBlockKeys>(all_keys(a, s))) * cost_of<R>(s);
   });
   if (static_cast<int>(blockIdx.x) >= line.pieces || line.total == 0) return;
+  // The units of this warp, one after the other: a sequence's are in the order kv head, block; a block is the piece's that its first unit is in.
   const long long begin = piece_begin(line, blockIdx.x), end = piece_begin(line, blockIdx.x + 1);
-  const int page_mask = (1 << a.batch.page_shift) - 1, heads = a.kv_heads * a.group;
+  const int shift = a.batch.page_shift, heads = a.kv_heads * a.group;
+  struct Unit {
+    int h, key0, page;  // page -1: none
+    int first, flats, lo, hi;
+    long long base;     // position of the new tokens
+  };
+  PagedSeq s;
+  PagedKeys keys{0, 0};
+  int blocks = 0, cost = 1;
+  long long all = 0, n = 0, before = at;
+  auto enter = [&] {  // sequence b, whose first unit is `before`
+    s = paged_sequence(a, b);
+    keys = all_keys(a, s);
+    blocks = blocks_of<kBlockKeys>(keys);
+    cost = max(1, cost_of<R>(s));
+    all = static_cast<long long>(blocks) * a.kv_heads;
+    n = begin > before ? (begin - before + cost - 1) / cost : 0;
+  };
+  enter();
+  auto next = [&](Unit& u) -> bool {
+    for (;; ++n) {
+      while (n >= all) {
+        before += all * cost;
+        if (++b >= a.batch.B || before >= end) return false;
+        enter();
+      }
+      if (before + n * cost >= end) return false;
+      u.h = static_cast<int>(n / blocks);
+      u.key0 = (keys.lo / kBlockKeys + static_cast<int>(n - static_cast<long long>(u.h) * blocks)) * kBlockKeys + warp * 16;
+      if (u.key0 < keys.hi && u.key0 + 16 > keys.lo) break;
+    }
+    ++n;
+    u.first = s.first;
+    u.flats = s.flats;
+    u.lo = keys.lo;
+    u.hi = keys.hi;
+    u.base = s.pos0 + s.first;
+    u.page = __ldg(a.batch.table + static_cast<long long>(b) * a.batch.W + (u.key0 >> shift));
+    return true;
+  };
+  uint4 kf[2][kKLoads];
+  float s0 = 1.f, s1 = 1.f, old = 0.f;
+  long long row = 0;
+  auto load = [&](Unit& u) {
+    if (u.page < 0 || u.page >= a.batch.pages) {
+      atomicCAS(a.status, 0, FTB_ERR_INDEX);
+      u.page = -1;
+      return;
+    }
+    row = ((static_cast<long long>(u.page) * a.kv_heads + u.h) << shift) + (u.key0 & ((1 << shift) - 1));
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < kKLoads; ++j) kf[i][j] = load_once(a.k + (row + g + 8 * i) * (k8 ? D : 2 * D) + j * 64 + c * 16);
+    if constexpr (k8) {
+      s0 = exponent_scale(a.k_exp[row + g]);
+      s1 = exponent_scale(a.k_exp[row + g + 8]);
+    }
+    if (c < 2) old = x.weights[row + g + 8 * c];  // (lane (g, 0) has key g, lane (g, 1) key g + 8)
+  };
 
-  // the sequence that unit `at` is in, and its blocks; a block is the piece's that its first unit is in
-  for (; b < a.batch.B && at < end; ++b) {
-    const PagedSeq s = paged_sequence(a, b);
-    const PagedKeys keys = all_keys(a, s);
-    const int blocks = blocks_of<kBlockKeys>(keys), cost = cost_of<R>(s), first_block = keys.lo / kBlockKeys;
-    const long long all = static_cast<long long>(blocks) * a.kv_heads, before = at;
-    at += all * cost;
-    if (all == 0) continue;
-    const int* table = a.batch.table + static_cast<long long>(b) * a.batch.W;
-    const long long base = s.pos0 + s.first;  // of the new tokens
-    const long long n0 = begin > before ? (begin - before + cost - 1) / cost : 0;
-    for (long long n = n0; n < all && before + n * cost < end; ++n) {
-      const int h = static_cast<int>(n / blocks), key0 = (first_block + static_cast<int>(n - static_cast<long long>(h) * blocks)) * kBlockKeys + warp * 16;
-      if (key0 >= keys.hi || key0 + 16 <= keys.lo) continue;
-      int page = table[key0 >> a.batch.page_shift];
-      const bool there = page >= 0 && page < a.batch.pages;
-      if (!there) {
-        atomicCAS(a.status, 0, FTB_ERR_INDEX);
-        continue;
-      }
-      const long long row = ((static_cast<long long>(page) * a.kv_heads + h) << a.batch.page_shift) + (key0 & page_mask);
-      uint4 kf[2][kKLoads];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < kKLoads; ++j) kf[i][j] = *reinterpret_cast<const uint4*>(a.k + (row + g + 8 * i) * (k8 ? D : 2 * D) + j * 64 + c * 16);
-      float s0 = 1.f, s1 = 1.f;
-      if constexpr (k8) {
-        s0 = exponent_scale(a.k_exp[row + g]);
-        s1 = exponent_scale(a.k_exp[row + g + 8]);
-      }
-      float sum0 = 0.f, sum1 = 0.f;
-      for (int flat0 = 0; flat0 < s.flats; flat0 += R) {
-        const int rows = min(R, s.flats - flat0);
-        if (base + (flat0 + rows - 1) / a.group < key0) continue;                                   // in front of the keys
-        if (a.window > 0 && base + flat0 / a.group - a.window >= key0 + 15) continue;  // they have left the window
-        uint32_t q[NT][kSteps][2];
-        float factor[NT][2], minus[NT][2];
-        int see_lo[NT][2], see_hi[NT][2];
+  uint32_t q[NT][kSteps][2];
+  float factor[NT][2], minus[NT][2];
+  int see_lo[NT][2], see_hi[NT][2];
+  int q_first = -1, q_h = -1;  // whose rows these are, where a tile has all of them
+  // A unit's keys are on their way while the one's in front are made weights of, and its page's number one unit longer.
+  Unit now, then, later;
+  bool more = next(then), still = more && next(later);
+  if (more) load(then);
+  while (more) {
+    now = then;
+    const float t0 = s0, t1 = s1, was = old;
+    const long long at_row = row;
+    more = still;
+    then = later;
+    auto go_on = [&] {
+      if (more) load(then);
+      still = more && next(later);
+    };
+    if (now.page < 0) {
+      go_on();
+      continue;
+    }
+    float sum0 = 0.f, sum1 = 0.f;
+    bool gone_on = false;
+    for (int flat0 = 0; flat0 < now.flats; flat0 += R) {
+      const int rows = min(R, now.flats - flat0);
+      const bool last = flat0 + R >= now.flats;
+      if (now.base + (flat0 + rows - 1) / a.group < now.key0 ||                                  // in front of the keys
+          (a.window > 0 && now.base + flat0 / a.group - a.window >= now.key0 + 15)) continue;    // they have left the window
+      if (now.flats > R || q_first != now.first || q_h != now.h) {
+        q_first = now.first;
+        q_h = now.h;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float mine = load_query<T, k8, D>(a, s.first, h, flat0, nt * 8 + g, rows, c, q[nt]);
+          const float mine = load_query<T, k8, D>(a, now.first, now.h, flat0, nt * 8 + g, rows, c, q[nt]);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             factor[nt][e] = __shfl_sync(0xffffffffu, mine, (2 * c + e) * 4);
             const int r = nt * 8 + 2 * c + e, flat = flat0 + r, token = flat / a.group;
             float lse = INFINITY;
-            if (r < rows) lse = x.lse[static_cast<long long>(s.first + token) * heads + h * a.group + flat - token * a.group];
+            if (r < rows) lse = x.lse[static_cast<long long>(now.first + token) * heads + now.h * a.group + flat - token * a.group];
             const bool fine = fabsf(lse) < INFINITY;  // (not of a row that sees nothing, or something that is not finite)
             minus[nt][e] = -lse * kLog2E;
-            const long long pos = fine ? base + token : -1ll;
-            see_hi[nt][e] = static_cast<int>(max(-1ll, min(pos, static_cast<long long>(keys.hi) - 1)));
+            const long long pos = fine ? now.base + token : -1ll;
+            see_hi[nt][e] = static_cast<int>(max(-1ll, min(pos, static_cast<long long>(now.hi) - 1)));
             see_lo[nt][e] = a.window > 0 ? static_cast<int>(max(0ll, min(pos - a.window + 1, static_cast<long long>(INT_MAX)))) : 0;
           }
         }
-        float sc[NT][4];
+      }
+      float sc[NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+      for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
 #pragma unroll
-        for (int j = 0; j < kKLoads; ++j) {
-          const uint32_t w0[4] = {kf[0][j].x, kf[0][j].y, kf[0][j].z, kf[0][j].w}, w1[4] = {kf[1][j].x, kf[1][j].y, kf[1][j].z, kf[1][j].w};
-          if constexpr (k8) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t a0, a1, a2, a3;
-              e4m3x4_to_f16x2(w0[i], a0, a2);
-              e4m3x4_to_f16x2(w1[i], a1, a3);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma16816<C>(sc[nt], a0, a1, a2, a3, q[nt][4 * j + i][0], q[nt][4 * j + i][1]);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-                mma16816<C>(sc[nt], w0[2 * i], w1[2 * i], w0[2 * i + 1], w1[2 * i + 1], q[nt][2 * j + i][0], q[nt][2 * j + i][1]);
-          }
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+      for (int j = 0; j < kKLoads; ++j) {
+        const uint32_t w0[4] = {kf[0][j].x, kf[0][j].y, kf[0][j].z, kf[0][j].w}, w1[4] = {kf[1][j].x, kf[1][j].y, kf[1][j].z, kf[1][j].w};
+        if constexpr (k8) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int e = i & 1, key = key0 + g + (i >> 1) * 8;
-            // (the scales of query and key meet before the score: either alone may lead out of fp32's range)
-            const float f = k8 ? fminf(factor[nt][e] * (i < 2 ? s0 : s1), FLT_MAX) : factor[nt][e];
-            const float p = key <= see_hi[nt][e] && key >= see_lo[nt][e] ? exp2_fast(fmaf(sc[nt][i], f, minus[nt][e])) : 0.f;
-            if (i < 2) sum0 += p;
-            else sum1 += p;
+            uint32_t a0, a1, a2, a3;
+            e4m3x4_to_f16x2(w0[i], a0, a2);
+            e4m3x4_to_f16x2(w1[i], a1, a3);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16816<C>(sc[nt], a0, a1, a2, a3, q[nt][4 * j + i][0], q[nt][4 * j + i][1]);
           }
-      }
-      sum0 += __shfl_xor_sync(0xffffffffu, sum0, 1);
-      sum1 += __shfl_xor_sync(0xffffffffu, sum1, 1);
-      sum0 += __shfl_xor_sync(0xffffffffu, sum0, 2);
-      sum1 += __shfl_xor_sync(0xffffffffu, sum1, 2);
-      if (c < 2) {  // lane (g, 0) has key g, lane (g, 1) key g + 8
-        const int key = key0 + g + 8 * c;
-        if (key >= keys.lo && key < keys.hi) {
-          float* w = x.weights + row + g + 8 * c;
-          const float sum = c == 0 ? sum0 : sum1;
-          *w = key >= base ? sum : *w + sum;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma16816<C>(sc[nt], w0[2 * i], w1[2 * i], w0[2 * i + 1], w1[2 * i + 1], q[nt][2 * j + i][0], q[nt][2 * j + i][1]);
         }
       }
+      if (last) {
+        go_on();
+        gone_on = true;
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int e = i & 1, key = now.key0 + g + (i >> 1) * 8;
+          // (the scales of query and key meet before the score: either alone may lead out of fp32's range)
+          const float f = k8 ? fminf(factor[nt][e] * (i < 2 ? t0 : t1), FLT_MAX) : factor[nt][e];
+          const float p = key <= see_hi[nt][e] && key >= see_lo[nt][e] ? exp2_fast(fmaf(sc[nt][i], f, minus[nt][e])) : 0.f;
+          if (i < 2) sum0 += p;
+          else sum1 += p;
+        }
+    }
+    if (!gone_on) go_on();
+    sum0 += __shfl_xor_sync(0xffffffffu, sum0, 1);
+    sum1 += __shfl_xor_sync(0xffffffffu, sum1, 1);
+    sum0 += __shfl_xor_sync(0xffffffffu, sum0, 2);
+    sum1 += __shfl_xor_sync(0xffffffffu, sum1, 2);
+    const int key = now.key0 + g + 8 * c;
+    if (c < 2 && key >= now.lo && key < now.hi) {
+      const float sum = c == 0 ? sum0 : sum1;
+      x.weights[at_row + g + 8 * c] = key >= now.base ? sum : was + sum;
     }
   }
 }
 
 template <typename T, bool k8, int D, int NT>
 int launch(const Weigh& x, cudaStream_t stream) {
-  const cudaError_t err = launch_dependent(paged_weigh_kernel<T, k8, D, NT>, dim3(current_sm_count() * 4), dim3(kWarps * 32), 0, stream, x);
+  const cudaError_t err = launch_dependent(paged_weigh_kernel<T, k8, D, NT>, dim3(current_sm_count() * blocks_per_sm(NT)), dim3(kWarps * 32), 0, stream, x);
   count_launch();
   if (err != cudaSuccess) cudaGetLastError();
   return err == cudaSuccess ? FTB_OK : FTB_ERR_LAUNCH;

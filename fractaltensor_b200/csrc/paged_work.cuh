@@ -14,21 +14,34 @@ namespace ftb {
 struct PagedSeq {
   long long pos0;  // position of row t: pos0 + t
   int first, n;    // rows
-  int flats;       // rows (token, head of the group) of a kv head; 0: not this launch's
+  int begin, flats;  // rows (token, head of the group) of a kv head: begin .. flats - 1; flats 0: not this launch's
   int hi;          // keys 0 .. hi - 1 are seen by some row
 };
 
+template <bool kMore = false>
 __device__ __forceinline__ PagedSeq paged_sequence(const PagedAttn& a, int b) {
   PagedSeq s;
   const int end = a.batch.starts[b + 1];
   s.first = max(0, a.batch.starts[b]);
   s.n = min(end, a.T) - s.first;
   s.pos0 = static_cast<long long>(a.batch.lens[b]) - end;
-  s.flats = s.hi = 0;
+  s.begin = s.flats = s.hi = 0;
   if (s.n <= 0 || s.first >= a.T) return s;
   const int flats = s.n * a.group;  // T * group fits
-  if (flats < a.least_rows || flats > a.most_rows) return s;
-  s.flats = flats;
+  if (kMore && a.split > 0) {
+    const int behind = flats % a.split, rest = flats > a.split && behind <= a.rest ? behind : 0;
+    if (flats < a.least_rows) return s;
+    if (flats > a.most_rows) {  // the kernel for few rows
+      if (rest == 0) return s;
+      s.begin = flats - rest;
+      s.flats = flats;
+    } else {
+      s.flats = a.least_rows > 1 ? flats - rest : flats;
+    }
+  } else {
+    if (flats < a.least_rows || flats > a.most_rows) return s;
+    s.flats = flats;
+  }
   const long long room = static_cast<long long>(a.batch.W) << a.batch.page_shift;
   const long long last = s.pos0 + s.first + s.n - 1;
   if (last >= room) atomicCAS(a.status, 0, FTB_ERR_INDEX);  // a table too narrow for the length
@@ -56,7 +69,7 @@ __device__ __forceinline__ int units_of(const PagedKeys& k) {
 template <int R, int kUnitKeys>
 __device__ __forceinline__ long long units_of_head(const PagedAttn& a, const PagedSeq& s) {
   long long sum = 0;
-  for (int flat0 = 0; flat0 < s.flats; flat0 += R)
+  for (int flat0 = s.begin; flat0 < s.flats; flat0 += R)
     sum += units_of<kUnitKeys>(keys_of_rows(a, s.pos0, s.first, s.hi, flat0, min(R, s.flats - flat0)));
   return sum;
 }
@@ -77,14 +90,14 @@ __device__ __forceinline__ long long piece_begin(const PagedLine& line, int g) {
 
 // All threads of a block, kLineThreads or more: the line, and the sequence that the first unit of piece g belongs to (B: none)
 // with that sequence's beginning.  at_least: units of a piece where there are few; of_head: units of one kv head of a sequence.
-template <typename OfHead>
+template <bool kMore = false, typename OfHead>
 __device__ __forceinline__ PagedLine paged_line_of(const PagedAttn& a, int g, int most_pieces, int at_least, PagedLineRoom& room, int* seq, long long* begin,
                                                    OfHead of_head) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (a.batch.B + kLineThreads - 1) / kLineThreads;
   const int b0 = min(a.batch.B, tid * per), b1 = tid < kLineThreads ? min(a.batch.B, b0 + per) : b0;
   long long mine = 0;
-  for (int b = b0; b < b1; ++b) mine += of_head(paged_sequence(a, b)) * a.kv_heads;
+  for (int b = b0; b < b1; ++b) mine += of_head(paged_sequence<kMore>(a, b)) * a.kv_heads;
   long long sum = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -110,7 +123,7 @@ __device__ __forceinline__ PagedLine paged_line_of(const PagedAttn& a, int g, in
     long long at = before + sum - mine;
     if (u >= at && u < at + mine) {
       for (int b = b0; b < b1; ++b) {
-        const long long c = of_head(paged_sequence(a, b)) * a.kv_heads;
+        const long long c = of_head(paged_sequence<kMore>(a, b)) * a.kv_heads;
         if (u < at + c) {
           room.seq = b;
           room.begin = at;
@@ -125,9 +138,9 @@ __device__ __forceinline__ PagedLine paged_line_of(const PagedAttn& a, int g, in
   *begin = room.begin;
   return line;
 }
-template <int R, int kUnitKeys>
+template <int R, int kUnitKeys, bool kMore>
 __device__ __forceinline__ PagedLine paged_line(const PagedAttn& a, int g, int most_pieces, int at_least, PagedLineRoom& room, int* seq, long long* begin) {
-  return paged_line_of(a, g, most_pieces, at_least, room, seq, begin, [&](const PagedSeq& s) { return units_of_head<R, kUnitKeys>(a, s); });
+  return paged_line_of<kMore>(a, g, most_pieces, at_least, room, seq, begin, [&](const PagedSeq& s) { return units_of_head<R, kUnitKeys>(a, s); });
 }
 
 // A stretch of a tile that a piece works on: units r0 .. r1 - 1 of its `units`.
@@ -139,7 +152,7 @@ struct PagedTile {
 };
 
 // Walks the tiles of a piece in their order.
-template <int R, int kUnitKeys>
+template <int R, int kUnitKeys, bool kMore>
 struct PagedWalk {
   PagedLine line;
   long long u, u_end, at, per;  // at: the sequence's beginning, per: units of one of its kv heads
@@ -154,7 +167,7 @@ struct PagedWalk {
     at = seq_begin;
     per = 0;
     if (u < u_end && b < a.batch.B) {
-      s = paged_sequence(a, b);
+      s = paged_sequence<kMore>(a, b);
       per = units_of_head<R, kUnitKeys>(a, s);
     } else {
       u = u_end;
@@ -165,14 +178,14 @@ struct PagedWalk {
   __device__ __forceinline__ PagedTile next(const PagedAttn& a) {
     while (u >= at + per * a.kv_heads) {
       at += per * a.kv_heads;
-      s = paged_sequence(a, ++b);
+      s = paged_sequence<kMore>(a, ++b);
       per = units_of_head<R, kUnitKeys>(a, s);
     }
     PagedTile t;
     t.b = b;
     t.h = static_cast<int>((u - at) / per);
     t.begin = at + per * t.h;
-    for (t.flat0 = 0;; t.flat0 += R) {
+    for (t.flat0 = s.begin;; t.flat0 += R) {
       t.rows = min(R, s.flats - t.flat0);
       t.keys = keys_of_rows(a, s.pos0, s.first, s.hi, t.flat0, t.rows);
       t.units = units_of<kUnitKeys>(t.keys);

@@ -38,7 +38,7 @@ struct DraftRow {
 
   __device__ __forceinline__ float p(int j) const { return pr[j]; }
   __device__ __forceinline__ float q(int j) const { return qr != nullptr ? qr[j] : 0.f; }
-  __device__ __forceinline__ void look(int) const {}
+  __device__ __forceinline__ void look(int, int) const {}
   __device__ __forceinline__ double weight(float p, float q, int j) const {
     const double w = static_cast<double>(p) - probability(q);  // (nothing is left of a p that is not positive)
     return w > 0.0 && p < __int_as_float(0x7f800000) && j != without ? w : 0.0;
@@ -83,7 +83,7 @@ verify_drafts_kernel(Drafts a, long long* __restrict__ tokens, int* __restrict__
   const int n = min(s_n, mine);
   DraftRow row{p + n * a.p_row, q != nullptr && n < mine ? q + n * a.q_row : nullptr,
                q == nullptr && n < mine && x[n] >= 0 && x[n] < V ? static_cast<int>(x[n]) : -1};
-  const double total = draw_token<C, kThreads>(row, V, share, rank, room, tokens + static_cast<long long>(b) * (K + 1) + n);
+  const double total = draw_token<C, kThreads, false>(row, V, share, rank, room, tokens + static_cast<long long>(b) * (K + 1) + n);
   if (rank == 0) {
     for (int i = threadIdx.x; i <= K; i += kThreads)
       if (i != n || !(total > 0.0)) tokens[static_cast<long long>(b) * (K + 1) + i] = i < n ? x[i] : -1;

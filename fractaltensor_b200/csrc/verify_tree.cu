@@ -5,8 +5,9 @@
 // of p_at of those refused before it, c is taken if u_c * (1 - r) < p_at(x_c), which takes x with probability p_at(x) whatever
 // else was drafted; the path goes on from there.  Where none is taken a token is drawn by u_0 from p_at without those refused.
 //
-// A token comes behind its parent, so that one walk through the tokens in their order finds the path.  What it asks for, every token's
-// number in its parent's row, is loaded beforehand, all of it at once; then one row is read whole (draft_draw.cuh).
+// Whether a token is taken once its parent is on the path depends on its siblings alone, so that a thread a token finds that, all at once:
+// the path is then a chain of first children taken.  (One warp that asked them one behind the other took 4 us for 25 tokens, of 10.)  Every
+// token's number in its parent's row is loaded beforehand; then one row is read whole (draft_draw.cuh).
 #include <climits>
 
 #include "../../include/ftb200.h"
@@ -58,7 +59,7 @@ struct Tree {
   int N, V;
 };
 
-// p without the refused tokens, which a warp looks for before it weighs 32 * kUnroll numbers.  (Looked for at every number, a batch of 60 rows of
+// p without the refused tokens, which a warp looks for before it weighs some hundred numbers.  (Looked for at every number, a batch of 60 rows of
 // 130 001 took 61 us.)
 struct TreeRow {
   const float* pr;
@@ -68,9 +69,9 @@ struct TreeRow {
 
   __device__ __forceinline__ float p(int j) const { return pr[j]; }
   __device__ __forceinline__ float q(int) const { return 0.f; }
-  __device__ __forceinline__ void look(int j) {
+  __device__ __forceinline__ void look(int j, int count) {
     some = false;
-    for (int i = threadIdx.x & 31; i < n; i += 32) some |= static_cast<unsigned>(refused[i] - j) < 32u * kUnroll;
+    for (int i = threadIdx.x & 31; i < n; i += 32) some |= static_cast<unsigned>(refused[i] - j) < static_cast<unsigned>(count);
     some = __any_sync(0xffffffffu, some);
   }
   __device__ __forceinline__ double weight(float p, float, int j) const {
@@ -85,50 +86,51 @@ struct TreeRow {
 };
 
 struct TreeRoom {  // in shared memory
-  int token[kMostTokens], parent[kMostTokens], path[kMostTokens], refused[kMostTokens];
+  int token[kMostTokens], parent[kMostTokens], path[kMostTokens], refused[kMostTokens], next[kMostTokens];
   float u[kMostTokens], p[kMostTokens];
   int length, n_refused;
 };
 
-// One warp: the path.
-__device__ __forceinline__ void walk(TreeRoom& t, int N, int lane) {
-  int at = 0, length = 1, n = 0;
-  double rest = 1.0;
-  if (lane == 0) t.path[0] = 0;
-  for (int i0 = 0; i0 < N; i0 += 32) {
-    const int mine = i0 + lane < N ? t.parent[i0 + lane] : -1;
-    unsigned here = i0 == 0 ? ~1u : ~0u;  // tokens of the 32 that lie in front of us
-    while (unsigned asked = __ballot_sync(0xffffffffu, mine == at && i0 + lane < N) & here) {
-      const int bit = __ffs(asked) - 1, c = i0 + bit, token = t.token[c];
-      here &= bit == 31 ? 0u : ~0u << (bit + 1);
-      bool again = false;  // refused before
-      for (int k = lane; k < n; k += 32) again |= t.refused[k] == token;
-      const double p = token < 0 || __any_sync(0xffffffffu, again) ? 0.0 : probability(t.p[c]);
-      if (static_cast<double>(t.u[c]) * rest < p) {
-        if (lane == 0) t.path[length] = c;
-        ++length;
-        at = c;
-        n = 0;
-        rest = 1.0;
-      } else {
-        rest = fmax(rest - p, 0.0);
-        if (token >= 0) {
-          if (lane == 0) t.refused[n] = token;
-          ++n;
-        }
-      }
-      __syncwarp();
-    }
+// All threads: the path, and the tokens that were refused behind its last one.
+template <int kThreads>
+__device__ __forceinline__ void find_path(TreeRoom& t, int N) {
+  // a token that a sibling in front of it has too counts as 0
+  for (int c = threadIdx.x; c < N; c += kThreads) {
+    const int parent = t.parent[c], token = t.token[c];
+    bool again = false;
+    for (int j = max(parent, 0) + 1; j < c; ++j) again |= t.parent[j] == parent && t.token[j] == token;
+    t.refused[c] = again;
+    t.next[c] = INT_MAX;
   }
-  if (lane == 0) {
-    t.length = length;
-    t.n_refused = n;
+  __syncthreads();
+  for (int c = threadIdx.x; c < N; c += kThreads)
+    if (t.refused[c] != 0) t.p[c] = 0.f;
+  __syncthreads();
+  for (int c = threadIdx.x; c < N; c += kThreads) {
+    const int parent = t.parent[c];
+    if (parent < 0) continue;
+    double rest = 1.0;
+    for (int j = parent + 1; j < c; ++j)
+      if (t.parent[j] == parent) rest = fmax(rest - probability(t.p[j]), 0.0);
+    if (static_cast<double>(t.u[c]) * rest < probability(t.p[c])) atomicMin(&t.next[parent], c);
   }
+  if (threadIdx.x == 0) t.n_refused = 0;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int n = 0;
+    for (int at = 0; at < N; at = t.next[at]) t.path[n++] = at;  // (INT_MAX behind the last one)
+    t.length = n;
+  }
+  __syncthreads();
+  const int last = t.path[t.length - 1];
+  for (int c = threadIdx.x; c < N; c += kThreads)
+    if (t.parent[c] == last && t.token[c] >= 0) t.refused[atomicAdd(&t.n_refused, 1)] = t.token[c];
+  __syncthreads();
 }
 
 // C: CTAs of a cluster, 1 or 8.
 template <int C, int kThreads>
-__global__ void __launch_bounds__(kThreads, 1536 / kThreads)
+__global__ void __launch_bounds__(kThreads, C == 8 && kThreads == 512 ? 1 : 1024 / kThreads)
 verify_tree_kernel(const __grid_constant__ Tree a, long long* __restrict__ tokens, int* __restrict__ path, int* __restrict__ counts_out, int* __restrict__ status) {
   __shared__ DrawRoom<C, kThreads> room;
   __shared__ TreeRoom t;
@@ -149,11 +151,10 @@ verify_tree_kernel(const __grid_constant__ Tree a, long long* __restrict__ token
     t.p[i] = drafted && known ? p[parent * a.p_row + x] : 0.f;
   }
   __syncthreads();
-  if (threadIdx.x < 32) walk(t, N, threadIdx.x);
-  __syncthreads();
+  find_path<kThreads>(t, N);
   const int n = t.length;
   TreeRow row{p + t.path[n - 1] * a.p_row, t.refused, t.n_refused, false};
-  const double total = draw_token<C, kThreads>(row, V, t.u[0], rank, room, tokens + seq + n - 1);
+  const double total = draw_token<C, kThreads, true>(row, V, t.u[0], rank, room, tokens + seq + n - 1);
   if (rank == 0) {
     for (int i = threadIdx.x; i < N; i += kThreads) {
       if (i != n - 1 || !(total > 0.0)) tokens[seq + i] = i < n - 1 ? t.token[t.path[i + 1]] : -1;

