@@ -102,18 +102,17 @@ paged_choose_kernel(const __grid_constant__ Choose a, int room) {
           page[u] = i < to ? __ldg(table + (i >> shift)) : 0;
         }
 #pragma unroll
-        for (int u = 0; u < kChooseAtOnce; ++u) {
-          const int i = i0 + u * 32 + lane;
-          w[u] = __int_as_float(0x7fffffff);
-          if (i >= to) continue;
-          if (page[u] >= 0 && page[u] < a.batch.pages) w[u] = a.weights[(((static_cast<long long>(page[u]) * a.kv_heads) + h) << shift) + (i & in_page)];
-          else atomicCAS(a.status, 0, FTB_ERR_INDEX);
+        for (int u = 0; u < kChooseAtOnce; ++u) {  // (page 0 in a missing one's place, so that nothing stands between the loads)
+          const int i = i0 + u * 32 + lane, there = page[u] >= 0 && page[u] < a.batch.pages ? page[u] : 0;
+          w[u] = a.weights[(((static_cast<long long>(there) * a.kv_heads) + h) << shift) + (i & in_page)];
         }
 #pragma unroll
         for (int u = 0; u < kChooseAtOnce; ++u) {
           const int i = i0 + u * 32 + lane;
           if (i >= to) continue;
-          const uint32_t key = order_of(w[u]);
+          const bool there = page[u] >= 0 && page[u] < a.batch.pages;
+          if (!there) atomicCAS(a.status, 0, FTB_ERR_INDEX);
+          const uint32_t key = there ? order_of(w[u]) : 0u;
           if (i - first < room) known_keys[i - first] = key;
           atomicAdd(bin + (key >> low), 1);
         }
