@@ -370,7 +370,7 @@ extern "C" int ftb_paged_attn_tree_fwd(const void* q, long long q_row, long long
   if (overlap(o, o_bytes, tree, tree_bytes)) return FTB_ERR_ARG;
   if (lse != nullptr) {
     const size_t lse_bytes = static_cast<size_t>(T) * heads * sizeof(float);
-    if ((reinterpret_cast<uintptr_t>(lse) & 15) != 0) return FTB_ERR_ALIGN;
+    if ((reinterpret_cast<uintptr_t>(lse) & 3) != 0) return FTB_ERR_ALIGN;
     if (over_rows(lse, static_cast<long long>(lse_bytes / 2), q, T, q_row, heads, q_head, d) || overlap(lse, lse_bytes, o, o_bytes) ||
         overlap(lse, lse_bytes, k_cache, cache_bytes) || overlap(lse, lse_bytes, v_cache, cache_bytes) || overlap(lse, lse_bytes, k_exp, exp_bytes) ||
         overlap(lse, lse_bytes, v_exp, exp_bytes) || overlap(lse, lse_bytes, tree, tree_bytes))

@@ -74,7 +74,7 @@ paged_choose_kernel(const __grid_constant__ Choose a, int room) {
   const int* table = a.batch.table + static_cast<long long>(b) * a.batch.W;
   const int shift = a.batch.page_shift, in_page = (1 << shift) - 1;
   auto key_at = [&](int i) -> uint32_t {
-    const int page = __ldg(table + (i >> shift));
+    const int page = table[i >> shift];
     if (page < 0 || page >= a.batch.pages) return 0u;  // (which is said where it is first read)
     return order_of(a.weights[(((static_cast<long long>(page) * a.kv_heads) + h) << shift) + (i & in_page)]);
   };
@@ -99,7 +99,7 @@ paged_choose_kernel(const __grid_constant__ Choose a, int room) {
 #pragma unroll
         for (int u = 0; u < kChooseAtOnce; ++u) {
           const int i = i0 + u * 32 + lane;
-          page[u] = i < to ? __ldg(table + (i >> shift)) : 0;
+          page[u] = i < to ? table[i >> shift] : 0;
         }
 #pragma unroll
         for (int u = 0; u < kChooseAtOnce; ++u) {  // (page 0 in a missing one's place, so that nothing stands between the loads)
@@ -235,7 +235,7 @@ struct Rows {
 // The page at position pos of one of a sequence's tables as it stands there; -1 behind its width.
 __device__ __forceinline__ int page_there(const int* table, int W, int shift, long long pos) {
   const long long i = pos >> shift;
-  return i < W ? __ldg(table + i) : -1;
+  return i < W ? table[i] : -1;
 }
 __device__ __forceinline__ Rows rows_of(const Move& a, int h, int first, int k, int i, int from, int to) {
   const int shift = a.batch.page_shift, in_page = (1 << shift) - 1;
@@ -276,7 +276,7 @@ paged_move_kernel(const __grid_constant__ Move a, int chains, bool in_place) {
 #pragma unroll
     for (int e = 0; e < kBeside; ++e) {
       const int i = i0 + e * kChain + tid;
-      k[e] = i < n && (kStep % kChain == 0 || e * kChain + tid < kStep) ? __ldg(kept + i) : -1;
+      k[e] = i < n && (kStep % kChain == 0 || e * kChain + tid < kStep) ? kept[i] : -1;
     }
 #pragma unroll
     for (int e = 0; e < kBeside; ++e) {
@@ -448,7 +448,7 @@ extern "C" int ftb_paged_cache_evict(void* k_cache, void* v_cache, unsigned char
   int rc = check_cache(k_cache, v_cache, k_exp, v_exp, table, into, B, W, into_W, pages, kv_heads, page_size, d);
   if (rc) return rc;
   if (!weights || !lens || !lens_out || !kept || keep <= 0 || recent < 0 || recent > keep) return FTB_ERR_ARG;
-  if ((reinterpret_cast<uintptr_t>(weights) & 15) != 0) return FTB_ERR_ALIGN;
+  if ((reinterpret_cast<uintptr_t>(weights) & 3) != 0) return FTB_ERR_ALIGN;
   if (workspace == nullptr || workspace_bytes < ftb_workspace_bytes()) return FTB_ERR_WORKSPACE;
   const size_t rows = static_cast<size_t>(pages) * kv_heads * page_size, row = k_exp != nullptr ? d : 2 * d;
   const size_t kept_bytes = static_cast<size_t>(B) * kv_heads * keep * sizeof(int), lens_bytes = static_cast<size_t>(B) * sizeof(int);

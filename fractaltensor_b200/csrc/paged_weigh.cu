@@ -37,6 +37,12 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm(NT))
 paged_weigh_kernel(const __grid_constant__ Weigh x) {
   using C = typename std::conditional<k8, __half, T>::type;
   constexpr int R = NT * 8, kSteps = D / 16, kKLoads = k8 ? D / 64 : D / 32;
+  // what the sequences of the units on their way are like (in registers it is the keys' room: 111 for 101 us of a decoding step)
+  struct Of {
+    long long base;  // position of the new tokens
+    int first, flats, lo, hi;
+  };
+  __shared__ Of s_of[kWarps][4];
   __shared__ PagedLineRoom s_line;
   const PagedAttn& a = x.attn;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
@@ -52,14 +58,14 @@ paged_weigh_kernel(const __grid_constant__ Weigh x) {
   const long long begin = piece_begin(line, blockIdx.x), end = piece_begin(line, blockIdx.x + 1);
   const int shift = a.batch.page_shift, heads = a.kv_heads * a.group;
   struct Unit {
-    int h, key0, page;  // page -1: none
-    int first, flats, lo, hi;
-    long long base;     // position of the new tokens
+    int h, key0, page, of;  // page -1: none; of: which sequence's
   };
   PagedSeq s;
   PagedKeys keys{0, 0};
   int blocks = 0, cost = 1;
   long long all = 0, n = 0, before = at;
+  int entered = 0;
+  bool fresh = true;
   auto enter = [&] {  // sequence b, whose first unit is `before`
     s = paged_sequence(a, b);
     keys = all_keys(a, s);
@@ -67,6 +73,7 @@ paged_weigh_kernel(const __grid_constant__ Weigh x) {
     cost = max(1, cost_of<R>(s));
     all = static_cast<long long>(blocks) * a.kv_heads;
     n = begin > before ? (begin - before + cost - 1) / cost : 0;
+    fresh = true;
   };
   enter();
   auto next = [&](Unit& u) -> bool {
@@ -82,12 +89,15 @@ paged_weigh_kernel(const __grid_constant__ Weigh x) {
       if (u.key0 < keys.hi && u.key0 + 16 > keys.lo) break;
     }
     ++n;
-    u.first = s.first;
-    u.flats = s.flats;
-    u.lo = keys.lo;
-    u.hi = keys.hi;
-    u.base = s.pos0 + s.first;
-    u.page = __ldg(a.batch.table + static_cast<long long>(b) * a.batch.W + (u.key0 >> shift));
+    if (fresh) {  // (of two units that are on their way and this one; what a unit in work needs has been taken out)
+      fresh = false;
+      entered = (entered + 1) & 3;
+      __syncwarp();
+      if (lane == 0) s_of[warp][entered] = Of{s.pos0 + s.first, s.first, s.flats, keys.lo, keys.hi};
+      __syncwarp();
+    }
+    u.of = entered;
+    u.page = a.batch.table[static_cast<long long>(b) * a.batch.W + (u.key0 >> shift)];
     return true;
   };
   uint4 kf[2][kKLoads];
@@ -121,6 +131,7 @@ paged_weigh_kernel(const __grid_constant__ Weigh x) {
   if (more) load(then);
   while (more) {
     now = then;
+    const Of of = s_of[warp][now.of];
     const float t0 = s0, t1 = s1, was = old;
     const long long at_row = row;
     more = still;
@@ -135,34 +146,38 @@ paged_weigh_kernel(const __grid_constant__ Weigh x) {
     }
     float sum0 = 0.f, sum1 = 0.f;
     bool gone_on = false;
-    for (int flat0 = 0; flat0 < now.flats; flat0 += R) {
-      const int rows = min(R, now.flats - flat0);
-      const bool last = flat0 + R >= now.flats;
-      if (now.base + (flat0 + rows - 1) / a.group < now.key0 ||                                  // in front of the keys
-          (a.window > 0 && now.base + flat0 / a.group - a.window >= now.key0 + 15)) continue;    // they have left the window
-      if (now.flats > R || q_first != now.first || q_h != now.h) {
-        q_first = now.first;
+    for (int flat0 = 0; flat0 < of.flats; flat0 += R) {
+      const int rows = min(R, of.flats - flat0);
+      const bool last = flat0 + R >= of.flats;
+      if (of.base + (flat0 + rows - 1) / a.group < now.key0 ||                                  // in front of the keys
+          (a.window > 0 && of.base + flat0 / a.group - a.window >= now.key0 + 15)) continue;    // they have left the window
+      if (of.flats > R || q_first != of.first || q_h != now.h) {
+        q_first = of.first;
         q_h = now.h;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float mine = load_query<T, k8, D>(a, now.first, now.h, flat0, nt * 8 + g, rows, c, q[nt]);
+          const float mine = load_query<T, k8, D>(a, of.first, now.h, flat0, nt * 8 + g, rows, c, q[nt]);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             factor[nt][e] = __shfl_sync(0xffffffffu, mine, (2 * c + e) * 4);
             const int r = nt * 8 + 2 * c + e, flat = flat0 + r, token = flat / a.group;
             float lse = INFINITY;
-            if (r < rows) lse = x.lse[static_cast<long long>(now.first + token) * heads + now.h * a.group + flat - token * a.group];
+            if (r < rows) lse = x.lse[static_cast<long long>(of.first + token) * heads + now.h * a.group + flat - token * a.group];
             const bool fine = fabsf(lse) < INFINITY;  // (not of a row that sees nothing, or something that is not finite)
             minus[nt][e] = -lse * kLog2E;
-            const long long pos = fine ? now.base + token : -1ll;
-            see_hi[nt][e] = static_cast<int>(max(-1ll, min(pos, static_cast<long long>(now.hi) - 1)));
+            const long long pos = fine ? of.base + token : -1ll;
+            see_hi[nt][e] = static_cast<int>(max(-1ll, min(pos, static_cast<long long>(of.hi) - 1)));
             see_lo[nt][e] = a.window > 0 ? static_cast<int>(max(0ll, min(pos - a.window + 1, static_cast<long long>(INT_MAX)))) : 0;
           }
         }
       }
-      float sc[NT][4];
+      // (two sums, of half the products each: the unit cuts off what is below a sum's last bit, always downwards, and the fewer steps the
+      // less.  9.9e-7 of the weights for a decoding step in one sum.)
+      float sc[NT][4], sd[NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[nt][i] = sd[nt][i] = 0.f;
 #pragma unroll
       for (int j = 0; j < kKLoads; ++j) {
         const uint32_t w0[4] = {kf[0][j].x, kf[0][j].y, kf[0][j].z, kf[0][j].w}, w1[4] = {kf[1][j].x, kf[1][j].y, kf[1][j].z, kf[1][j].w};
@@ -173,14 +188,14 @@ paged_weigh_kernel(const __grid_constant__ Weigh x) {
             e4m3x4_to_f16x2(w0[i], a0, a2);
             e4m3x4_to_f16x2(w1[i], a1, a3);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma16816<C>(sc[nt], a0, a1, a2, a3, q[nt][4 * j + i][0], q[nt][4 * j + i][1]);
+            for (int nt = 0; nt < NT; ++nt) mma16816<C>(i & 1 ? sd[nt] : sc[nt], a0, a1, a2, a3, q[nt][4 * j + i][0], q[nt][4 * j + i][1]);
           }
         } else {
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma16816<C>(sc[nt], w0[2 * i], w1[2 * i], w0[2 * i + 1], w1[2 * i + 1], q[nt][2 * j + i][0], q[nt][2 * j + i][1]);
+              mma16816<C>(i & 1 ? sd[nt] : sc[nt], w0[2 * i], w1[2 * i], w0[2 * i + 1], w1[2 * i + 1], q[nt][2 * j + i][0], q[nt][2 * j + i][1]);
         }
       }
       if (last) {
@@ -194,7 +209,7 @@ paged_weigh_kernel(const __grid_constant__ Weigh x) {
           const int e = i & 1, key = now.key0 + g + (i >> 1) * 8;
           // (the scales of query and key meet before the score: either alone may lead out of fp32's range)
           const float f = k8 ? fminf(factor[nt][e] * (i < 2 ? t0 : t1), FLT_MAX) : factor[nt][e];
-          const float p = key <= see_hi[nt][e] && key >= see_lo[nt][e] ? exp2_fast(fmaf(sc[nt][i], f, minus[nt][e])) : 0.f;
+          const float p = key <= see_hi[nt][e] && key >= see_lo[nt][e] ? exp2_fast(fmaf(sc[nt][i] + sd[nt][i], f, minus[nt][e])) : 0.f;
           if (i < 2) sum0 += p;
           else sum1 += p;
         }
@@ -205,9 +220,9 @@ paged_weigh_kernel(const __grid_constant__ Weigh x) {
     sum0 += __shfl_xor_sync(0xffffffffu, sum0, 2);
     sum1 += __shfl_xor_sync(0xffffffffu, sum1, 2);
     const int key = now.key0 + g + 8 * c;
-    if (c < 2 && key >= now.lo && key < now.hi) {
+    if (c < 2 && key >= of.lo && key < of.hi) {
       const float sum = c == 0 ? sum0 : sum1;
-      x.weights[at_row + g + 8 * c] = key >= now.base ? sum : was + sum;
+      x.weights[at_row + g + 8 * c] = key >= of.base ? sum : was + sum;
     }
   }
 }
@@ -262,8 +277,8 @@ extern "C" int ftb_paged_attn_weights(const void* q, long long q_row, long long 
   if (!(scale > 0.f) || !(scale * kLog2E <= FLT_MAX)) return FTB_ERR_ARG;
   if (static_cast<long long>(kv_heads) * group > 65536 || static_cast<long long>(T) * group > INT_MAX) return FTB_ERR_ARG;
   if (((q_row | q_head) & 7) != 0) return FTB_ERR_ALIGN;
-  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(k_exp) |
-        reinterpret_cast<uintptr_t>(weights) | reinterpret_cast<uintptr_t>(lse)) & 15) != 0)
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(k_exp)) & 15) != 0 ||
+      ((reinterpret_cast<uintptr_t>(weights) | reinterpret_cast<uintptr_t>(lse)) & 3) != 0)
     return FTB_ERR_ALIGN;
   if (workspace == nullptr || workspace_bytes < ftb_workspace_bytes()) return FTB_ERR_WORKSPACE;
   if (T == 0) return FTB_OK;

@@ -99,7 +99,7 @@ __device__ __forceinline__ BlockRows rows_of_block(const PagedAttn& a, const Pag
   const int k0 = max(block * kBlock, keys.lo), k1 = min((block + 1) * kBlock, keys.hi);  // block * kBlock < keys.hi
   BlockRows r;
   r.flat0 = static_cast<int>(min(static_cast<long long>(s.flats), max(0ll, k0 - base) * a.group));
-  r.flat1 = a.window > 0 ? static_cast<int>(min(static_cast<long long>(s.flats), max(0ll, k1 - 1 + a.window - base) * a.group)) : s.flats;
+  r.flat1 = a.window > 0 ? static_cast<int>(min(static_cast<long long>(s.flats), max(0ll, static_cast<long long>(a.window) + k1 - 1 - base) * a.group)) : s.flats;
   r.tiles = r.flat1 > r.flat0 ? (r.flat1 - r.flat0 + kRows - 1) / kRows : 0;
   return r;
 }
@@ -119,7 +119,7 @@ __device__ __forceinline__ Tiles tiles_of_half(const PagedAttn& a, const Stretch
   if (k0 >= k1) return {0, 0};
   const long long f0 = max(0ll, k0 - y.base) * a.group - y.flat0;
   long long f1 = y.flat1 - y.flat0;
-  if (a.window > 0) f1 = min(f1, max(0ll, k1 - 1 + a.window - y.base) * a.group - y.flat0);
+  if (a.window > 0) f1 = min(f1, max(0ll, static_cast<long long>(a.window) + k1 - 1 - y.base) * a.group - y.flat0);
   return {static_cast<int>(max(0ll, f0) / kRows), static_cast<int>((max(0ll, f1) + kRows - 1) / kRows)};
 }
 
@@ -227,6 +227,7 @@ paged_weigh_tile_kernel(const __grid_constant__ Weigh x, const __grid_constant__
 
   if (warp == 0) {
     // ------------------------------------------------------------- the walk, and the rows
+    fence_proxy_async_all();  // (the rows have been packed by ordinary stores)
     long long u = piece_begin(line, piece);
     const long long u_end = piece_begin(line, piece + 1);
     PagedSeq s = paged_sequence(a, seq);
@@ -299,7 +300,7 @@ paged_weigh_tile_kernel(const __grid_constant__ Weigh x, const __grid_constant__
       float4 minus, factor;
       auto fetch = [&](int flat) {  // four numbers of a tile a lane
         const long long i = row0 + flat + lane * 4;
-        auto take = [&](const float* p, int k) { return i + k < numbers ? __ldg(p + i + k) : 0.f; };
+        auto take = [&](const float* p, int k) { return i + k < numbers ? p[i + k] : 0.f; };
         minus = make_float4(take(packed.minus, 0), take(packed.minus, 1), take(packed.minus, 2), take(packed.minus, 3));
         if constexpr (kFactors) factor = make_float4(take(packed.factor, 0), take(packed.factor, 1), take(packed.factor, 2), take(packed.factor, 3));
       };
@@ -394,7 +395,7 @@ paged_weigh_tile_kernel(const __grid_constant__ Weigh x, const __grid_constant__
         if (key >= y.keys.lo && key < y.keys.hi) {
           see0 = max(0ll, key - y.base) * a.group - y.flat0;
           see1 = y.flat1 - y.flat0;
-          if (a.window > 0) see1 = min(see1, max(0ll, key + a.window - y.base) * a.group - y.flat0);
+          if (a.window > 0) see1 = min(see1, max(0ll, static_cast<long long>(a.window) + key - y.base) * a.group - y.flat0);
         }
         from[h] = static_cast<int>(max(0ll, see0)) - part * kPart;
         to[h] = static_cast<int>(max(0ll, see1)) - part * kPart;

@@ -930,7 +930,7 @@ def verify_tree(probs, tokens, parents, u):
     """Trees of drafted tokens against the target's probabilities, from random numbers of the caller's.
 
     tokens: int64 [B, N], token 0 the last one that is certain; parents: int32 [B, N] as in tree_mask (a token without one is not
-    part of the tree); probs: fp32 [B, N, V], the target's behind each token; u: fp32 [B, N] in [0, 1).  From token 0
+    part of the tree), N up to 1024; probs: fp32 [B, N, V], the target's behind each token; u: fp32 [B, N] in [0, 1).  From token 0
     on: those drafted behind the last token of the path are asked in their order, and c is taken if u[c] * (1 - r) < p(x_c), r the
     probability of those refused before it; where none is taken, u[0] draws a token from what is left.  This is a sample of the target's
     probabilities whatever was drafted.  -> (int64 [B, N]: the path's tokens behind token 0, the drawn one, then -1; int32

@@ -446,8 +446,8 @@ int ftb_paged_attn_fwd(const void* q, long long q_row, long long q_head, const v
 /* The same for trees of drafted tokens, and with the sums that the softmax divides by.  tree: int32 [T, tree_words] or NULL: bit j
  * (bit j % 32 of word j / 32) of a row is 1 if the token sees new token j of its sequence, counted from the sequence's first new one.
  * The keys in front of the new tokens are seen by all of them, a new one behind a token's own place by none; new tokens that the mask has no
- * column for are seen as without it.  A tree has no window.  ftb_tree_mask makes such a mask.  lse: fp32 [T, kv_heads * group], 16-byte
- * aligned, or NULL: log(sum(exp(scale * q . k))) over the keys that a row sees, -inf where it sees none; it overlaps nothing that is read or written. */
+ * column for are seen as without it.  A tree has no window.  ftb_tree_mask makes such a mask.  lse: fp32 [T, kv_heads * group] or
+ * NULL: log(sum(exp(scale * q . k))) over the keys that a row sees, -inf where it sees none; it overlaps nothing that is read or written. */
 int ftb_paged_attn_tree_fwd(const void* q, long long q_row, long long q_head, const void* k_cache, const void* v_cache,
                             const unsigned char* k_exp, const unsigned char* v_exp, const int* table, const int* lens,
                             const int* starts, const int* tree, int tree_words, void* o, float* lse, int T, int B, int W,

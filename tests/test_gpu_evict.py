@@ -121,6 +121,48 @@ def test_scales_of_queries_and_keys_that_cancel(by):
     assert abs(float(weights.sum()) - 4 * kv * group) < 1e-3
 
 
+@pytest.mark.parametrize("eight_bit", [False, True])
+@pytest.mark.parametrize("new,lens", [([1, 1], [40, 70]), ([200, 33], [260, 300])])
+def test_a_window_of_everything(eight_bit, new, lens):
+    ops = _ops()
+    kv, group, d, page = 2, 4, 64, 16
+    table, ln, st, pages = _batch(new, lens, page)
+    cache = _full_cache(pages, kv, page, d, E4M3 if eight_bit else BF16, 3, table, ln)
+    T = int(st[-1])
+    q = _numbers((T, kv * group, d), BF16, 1).cuda()
+    args = (table.cuda(), ln.cuda(), st.cuda())
+    lse = torch.empty(T, kv * group, device="cuda")
+    ops.paged_attention(q, cache, *args, scale=0.1, lse=lse)
+    got = []
+    for window in (None, 2 ** 31 - 1, 2 ** 40):
+        got.append(torch.zeros(pages, kv, page, device="cuda"))
+        ops.paged_attention_weights(q, cache, got[-1], lse, *args, scale=0.1, window=window)
+    ops.check_status()
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+
+
+@pytest.mark.parametrize("eight_bit", [False, True])
+def test_many_stretches_a_piece(eight_bit):
+    """Dozens of sequences with one tile of rows or two to a block of keys: every CTA goes through many blocks, of all lengths."""
+    ops = _ops()
+    kv, group, d, page = 3, 3, 64, 32
+    g = torch.Generator().manual_seed(7)
+    new = torch.randint(6, 60, (90,), generator=g).tolist()
+    lens = [n + int(m) for n, m in zip(new, torch.randint(0, 700, (90,), generator=g))]
+    table, ln, st, pages = _batch(new, lens, page)
+    cache = _full_cache(pages, kv, page, d, E4M3 if eight_bit else BF16, 3, table, ln)
+    T = int(st[-1])
+    q = _numbers((T, kv * group, d), BF16, 1).cuda()
+    args = (table.cuda(), ln.cuda(), st.cuda())
+    lse = torch.empty(T, kv * group, device="cuda")
+    ops.paged_attention(q, cache, *args, scale=0.1, lse=lse)
+    weights = torch.rand(pages, kv, page, generator=g).cuda()
+    before = weights.clone()
+    ops.paged_attention_weights(q, cache, weights, lse, *args, scale=0.1)
+    ops.check_status()
+    _weigh_check(weights, before, q, cache, lse, table, ln, st, 0.1)
+
+
 def test_weights_of_a_page_that_is_not_there():
     ops = _ops()
     from fractaltensor_b200._lib import FtbError

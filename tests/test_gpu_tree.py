@@ -202,6 +202,70 @@ def test_other_branches_have_no_part(eight_bit, what, new, lens):
     assert bool(((lse.double().cpu() - want_lse).abs() <= tol)[rows].all())
 
 
+@pytest.mark.parametrize("new,lens", [([1, 1], [300, 17]), ([9], [90]), ([40, 70], [40, 300]), ([150], [500])])
+def test_lse_over_values_of_very_different_sizes(new, lens):
+    """8 bits: what a value's exponent does to its weight has no part in the logarithm."""
+    ops = _ops()
+    kv, group, d, page = 2, 4, 128, 16
+    table, ln, st, pages = _batch(new, lens, page)
+    k, v = _numbers((pages, kv, page, d), torch.float32, 3), _numbers((pages, kv, page, d), torch.float32, 4)
+    g = torch.Generator().manual_seed(1)
+    by = torch.tensor([0.0, 2.0 ** -100, 2.0 ** -40, 1.0, 2.0 ** 20])[torch.randint(0, 5, (pages, kv, page), generator=g)]
+    (kc, ke), (vc, ve) = paged.quantise(k), paged.quantise(v * by[..., None])
+    cache = tuple(x.cuda() for x in (kc.view(E4M3), vc.view(E4M3), ke, ve))
+    T = int(st[-1])
+    q = _numbers((T, kv * group, d), BF16, 1).cuda()
+    mask = _tree_rows(new, st, T, 5)
+    lse = torch.empty(T, kv * group, device="cuda")
+    ops.paged_attention(q, cache, table.cuda(), ln.cuda(), st.cuda(), scale=0.08, tree=mask.cuda(), lse=lse)
+    ops.check_status()
+    _, bound, want = tree.attention(q, cache, table, ln, st, 0.08, None, mask)
+    err = (lse.double().cpu() - want).abs()
+    assert bool((err <= tree.lse_tolerance(want, bound[1], d, True, max(lens))).all()), float(err.max())
+
+
+def test_logarithms_of_layers_side_by_side():
+    """lse may begin anywhere: a slice of one array for all layers."""
+    ops = _ops()
+    table, ln, st, pages = _batch([3], [40], 16)
+    cache = _full_cache(pages, 1, 16, 64, BF16, 3)
+    q = _numbers((3, 3, 64), BF16, 1).cuda()
+    layers = torch.zeros(4, 3, 3, device="cuda")
+    for x in layers:
+        ops.paged_attention(q, cache, table.cuda(), ln.cuda(), st.cuda(), lse=x)
+    weights = torch.zeros(pages * 16 + 1, device="cuda")[1:].view(pages, 1, 16)
+    ops.paged_attention_weights(q, cache, weights, layers[1], table.cuda(), ln.cuda(), st.cuda())
+    ops.check_status()
+    assert bool((layers == layers[0]).all()) and abs(float(weights.sum()) - 9) < 1e-4
+
+
+def test_calls_on_two_streams_at_once():
+    ops = _ops()
+    kv, group, d, page, N, V = 2, 8, 128, 16, 33, 9000
+    table, ln, st, pages = _batch([N, N], [900, 1500], page)
+    cache = _full_cache(pages, kv, page, d, BF16, 3)
+    qs = [_numbers((2 * N, kv * group, d), BF16, i).cuda() for i in range(2)]
+    trees = [tuple(x.cuda() for x in _forest(2, N, V, i)) for i in range(2)]
+    args = (cache, table.cuda(), ln.cuda(), st.cuda())
+
+    def step(i):
+        probs, tokens, parents, u = trees[i]
+        return (ops.paged_attention(qs[i], *args, scale=0.1, tree=ops.tree_mask(parents).flatten(0, 1)),) + ops.verify_tree(probs, tokens, parents, u)
+
+    want = [step(i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(10):
+        got = []
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append(step(i))
+        torch.cuda.synchronize()
+        for x, y in zip(got, want):
+            assert all(torch.equal(a, b) for a, b in zip(x, y))
+    ops.check_status()
+
+
 def test_refusals():
     ops = _ops()
     table, ln, st, pages = _batch([3], [40], 16)

@@ -90,14 +90,14 @@ def test_mask_arguments(lib):
 
 
 def test_alignment_and_workspace(lib):
-    odd = ctypes.c_void_p((13 << 20) + 8)
-    for kw in (dict(q=odd), dict(k=odd), dict(o=odd), dict(lse=odd), dict(q_row=4)):
+    odd, odder = ctypes.c_void_p((13 << 20) + 8), ctypes.c_void_p((13 << 20) + 2)
+    for kw in (dict(q=odd), dict(k=odd), dict(o=odd), dict(lse=odder), dict(q_row=4)):
         assert _attn(lib, **kw) == 2, kw
-    for kw in (dict(q=odd), dict(k=odd), dict(ke=odd), dict(lse=odd), dict(weights=odd), dict(q_head=7)):
+    for kw in (dict(q=odd), dict(k=odd), dict(ke=odd), dict(lse=odder), dict(weights=odder), dict(q_head=7)):
         assert _weights(lib, **kw) == 2, kw
     for call in (_keep, _evict):
         assert call(lib, k=odd) == call(lib, v=odd) == call(lib, ke=odd, ve=A(11)) == 2
-    assert _evict(lib, weights=odd) == 2
+    assert _evict(lib, weights=odder) == 2
     for call in (_attn, _weights, _keep, _evict, _verify):
         assert call(lib, ws=Z) == call(lib, wb=1) == 3
     # no rows: nothing to do, and nothing is asked of a device
