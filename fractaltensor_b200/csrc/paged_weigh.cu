@@ -55,49 +55,48 @@ paged_weigh_kernel(const __grid_constant__ Weigh x) {
   });
   if (static_cast<int>(blockIdx.x) >= line.pieces || line.total == 0) return;
   // The units of this warp, one after the other: a sequence's are in the order kv head, block; a block is the piece's that its first unit is in.
-  const long long begin = piece_begin(line, blockIdx.x), end = piece_begin(line, blockIdx.x + 1);
   const int shift = a.batch.page_shift, heads = a.kv_heads * a.group;
   struct Unit {
-    int h, key0, page, of;  // page -1: none; of: which sequence's
+    int h, key0, page, of;  // page -1: none; of: which sequence's, -1: none of its keys are this warp's
   };
-  PagedSeq s;
-  PagedKeys keys{0, 0};
-  int blocks = 0, cost = 1;
-  long long all = 0, n = 0, before = at;
-  int entered = 0;
-  bool fresh = true;
-  auto enter = [&] {  // sequence b, whose first unit is `before`
-    s = paged_sequence(a, b);
-    keys = all_keys(a, s);
+  long long skip = piece_begin(line, blockIdx.x) - at, left = piece_begin(line, blockIdx.x + 1) - at;  // from the sequence's first unit
+  int blocks, h, block, lo, hi, entered = 0;
+  long long todo;  // blocks of the sequence that are left
+  auto enter = [&] {
+    const PagedSeq s = paged_sequence(a, b);
+    const PagedKeys keys = all_keys(a, s);
+    lo = keys.lo;
+    hi = keys.hi;
     blocks = blocks_of<kBlockKeys>(keys);
-    cost = max(1, cost_of<R>(s));
-    all = static_cast<long long>(blocks) * a.kv_heads;
-    n = begin > before ? (begin - before + cost - 1) / cost : 0;
-    fresh = true;
+    const int cost = max(1, cost_of<R>(s));
+    const long long all = static_cast<long long>(blocks) * a.kv_heads, n0 = skip > 0 ? (skip + cost - 1) / cost : 0;
+    todo = min(all, (left + cost - 1) / cost) - n0;
+    skip -= all * cost;
+    left -= all * cost;
+    if (todo <= 0) return;
+    h = static_cast<int>(n0 / blocks);
+    block = static_cast<int>(n0 - static_cast<long long>(h) * blocks);
+    // (of two units that are on their way and the next one; what a unit in work needs has been taken out)
+    entered = (entered + 1) & 3;
+    __syncwarp();
+    if (lane == 0) s_of[warp][entered] = Of{s.pos0 + s.first, s.first, s.flats, lo, hi};
+    __syncwarp();
   };
   enter();
   auto next = [&](Unit& u) -> bool {
-    for (;; ++n) {
-      while (n >= all) {
-        before += all * cost;
-        if (++b >= a.batch.B || before >= end) return false;
-        enter();
-      }
-      if (before + n * cost >= end) return false;
-      u.h = static_cast<int>(n / blocks);
-      u.key0 = (keys.lo / kBlockKeys + static_cast<int>(n - static_cast<long long>(u.h) * blocks)) * kBlockKeys + warp * 16;
-      if (u.key0 < keys.hi && u.key0 + 16 > keys.lo) break;
+    while (todo <= 0) {
+      if (left <= 0 || ++b >= a.batch.B) return false;
+      enter();
     }
-    ++n;
-    if (fresh) {  // (of two units that are on their way and this one; what a unit in work needs has been taken out)
-      fresh = false;
-      entered = (entered + 1) & 3;
-      __syncwarp();
-      if (lane == 0) s_of[warp][entered] = Of{s.pos0 + s.first, s.first, s.flats, keys.lo, keys.hi};
-      __syncwarp();
+    u.h = h;
+    u.key0 = (lo / kBlockKeys + block) * kBlockKeys + warp * 16;
+    u.of = u.key0 < hi && u.key0 + 16 > lo ? entered : -1;
+    u.page = u.of >= 0 ? a.batch.table[static_cast<long long>(b) * a.batch.W + (u.key0 >> shift)] : -1;
+    --todo;
+    if (++block == blocks) {
+      block = 0;
+      ++h;
     }
-    u.of = entered;
-    u.page = a.batch.table[static_cast<long long>(b) * a.batch.W + (u.key0 >> shift)];
     return true;
   };
   uint4 kf[2][kKLoads];
@@ -105,7 +104,7 @@ paged_weigh_kernel(const __grid_constant__ Weigh x) {
   long long row = 0;
   auto load = [&](Unit& u) {
     if (u.page < 0 || u.page >= a.batch.pages) {
-      atomicCAS(a.status, 0, FTB_ERR_INDEX);
+      if (u.of >= 0) atomicCAS(a.status, 0, FTB_ERR_INDEX);
       u.page = -1;
       return;
     }
@@ -124,14 +123,15 @@ paged_weigh_kernel(const __grid_constant__ Weigh x) {
   uint32_t q[NT][kSteps][2];
   float factor[NT][2], minus[NT][2];
   int see_lo[NT][2], see_hi[NT][2];
-  int q_first = -1, q_h = -1;  // whose rows these are, where a tile has all of them
+  int all_lo = 0, all_hi = -1;  // keys that all rows see, where all of their lse are finite
+  int q_first = -1, q_h = -1;   // whose rows these are, where a tile has all of them
   // A unit's keys are on their way while the one's in front are made weights of, and its page's number one unit longer.
   Unit now, then, later;
   bool more = next(then), still = more && next(later);
   if (more) load(then);
   while (more) {
     now = then;
-    const Of of = s_of[warp][now.of];
+    const Of of = s_of[warp][max(0, now.of)];
     const float t0 = s0, t1 = s1, was = old;
     const long long at_row = row;
     more = still;
@@ -154,6 +154,7 @@ paged_weigh_kernel(const __grid_constant__ Weigh x) {
       if (of.flats > R || q_first != of.first || q_h != now.h) {
         q_first = of.first;
         q_h = now.h;
+        bool odd = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const float mine = load_query<T, k8, D>(a, of.first, now.h, flat0, nt * 8 + g, rows, c, q[nt]);
@@ -161,15 +162,19 @@ paged_weigh_kernel(const __grid_constant__ Weigh x) {
           for (int e = 0; e < 2; ++e) {
             factor[nt][e] = __shfl_sync(0xffffffffu, mine, (2 * c + e) * 4);
             const int r = nt * 8 + 2 * c + e, flat = flat0 + r, token = flat / a.group;
-            float lse = INFINITY;
+            float lse = INFINITY;  // (rows that there are none of take away infinity from scores of 0)
             if (r < rows) lse = x.lse[static_cast<long long>(of.first + token) * heads + now.h * a.group + flat - token * a.group];
             const bool fine = fabsf(lse) < INFINITY;  // (not of a row that sees nothing, or something that is not finite)
+            odd |= r < rows && !fine;
             minus[nt][e] = -lse * kLog2E;
             const long long pos = fine ? of.base + token : -1ll;
             see_hi[nt][e] = static_cast<int>(max(-1ll, min(pos, static_cast<long long>(of.hi) - 1)));
             see_lo[nt][e] = a.window > 0 ? static_cast<int>(max(0ll, min(pos - a.window + 1, static_cast<long long>(INT_MAX)))) : 0;
           }
         }
+        const long long pos0 = of.base + flat0 / a.group, pos1 = of.base + (flat0 + rows - 1) / a.group;
+        all_hi = __any_sync(0xffffffffu, odd) ? -1 : static_cast<int>(max(-1ll, min(pos0, static_cast<long long>(of.hi) - 1)));
+        all_lo = max(of.lo, a.window > 0 ? static_cast<int>(max(0ll, min(pos1 - a.window + 1, static_cast<long long>(INT_MAX)))) : 0);
       }
       // (two sums, of half the products each: the unit cuts off what is below a sum's last bit, always downwards, and the fewer steps the
       // less.  9.9e-7 of the weights for a decoding step in one sum.)
@@ -202,17 +207,30 @@ paged_weigh_kernel(const __grid_constant__ Weigh x) {
         go_on();
         gone_on = true;
       }
+      const bool plain = now.key0 + 15 <= all_hi && now.key0 >= all_lo;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int e = i & 1, key = now.key0 + g + (i >> 1) * 8;
+          const int e = i & 1;
           // (the scales of query and key meet before the score: either alone may lead out of fp32's range)
           const float f = k8 ? fminf(factor[nt][e] * (i < 2 ? t0 : t1), FLT_MAX) : factor[nt][e];
-          const float p = key <= see_hi[nt][e] && key >= see_lo[nt][e] ? exp2_fast(fmaf(sc[nt][i] + sd[nt][i], f, minus[nt][e])) : 0.f;
-          if (i < 2) sum0 += p;
-          else sum1 += p;
+          sc[nt][i] = exp2_fast(fmaf(sc[nt][i] + sd[nt][i], f, minus[nt][e]));
         }
+      if (!plain) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int e = i & 1, key = now.key0 + g + (i >> 1) * 8;
+            if (key > see_hi[nt][e] || key < see_lo[nt][e]) sc[nt][i] = 0.f;
+          }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        sum0 += sc[nt][0] + sc[nt][1];
+        sum1 += sc[nt][2] + sc[nt][3];
+      }
     }
     if (!gone_on) go_on();
     sum0 += __shfl_xor_sync(0xffffffffu, sum0, 1);

@@ -13,6 +13,10 @@
     python -m fractaltensor_b200.run_case paged --B 64 --S 4096 --heads 32 --kv-heads 8                # a token for each sequence
     python -m fractaltensor_b200.run_case paged --B 16 --S 8192 --new 8 --cache e4m3                   # drafts
     python -m fractaltensor_b200.run_case verify --B 64 --new 4 --V 50000
+    python -m fractaltensor_b200.run_case tree --B 16 --S 8192 --new 32 --cache e4m3                   # trees of drafts, mask and all
+    python -m fractaltensor_b200.run_case verify_tree --B 64 --new 32 --V 50000
+    python -m fractaltensor_b200.run_case weigh --B 64 --S 4096 --heads 32                             # what new tokens attend to
+    python -m fractaltensor_b200.run_case evict --B 64 --S 4096 --keep 1024                            # down to so many keys, into other pages
 
 A small, fixed workload to put under a profiler or to time by hand; prints the
 average time per call measured with CUDA events.
@@ -29,7 +33,8 @@ DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("case", choices=["lstm", "varlen", "dilated", "grid", "b2b", "attn", "softmax", "sparse_attn", "project", "rnn_attn", "paged", "verify"])
+    ap.add_argument("case", choices=["lstm", "varlen", "dilated", "grid", "b2b", "attn", "softmax", "sparse_attn", "project", "rnn_attn", "paged", "verify", "tree",
+                                     "verify_tree", "weigh", "evict"])
     ap.add_argument("--D", type=int, default=16)
     ap.add_argument("--L", type=int, default=20)
     ap.add_argument("--N", type=int, default=256)
@@ -56,10 +61,11 @@ def main():
     ap.add_argument("--V", type=int, default=10000, help="project: vocabulary, over M rows of H")
     ap.add_argument("--head-dim", type=int, default=64, help="sparse_attn: elements per head")
     ap.add_argument("--as-shipped", action="store_true", help="sparse_attn: the softmax dimension of the shipped example")
-    ap.add_argument("--new", type=int, default=1, help="paged: new tokens of each of B sequences of S keys; verify: drafts")
+    ap.add_argument("--new", type=int, default=1, help="paged, tree, weigh: new tokens of each of B sequences of S keys; verify, verify_tree: drafts")
     ap.add_argument("--kv-heads", type=int, default=8, help="paged: kv heads that the heads share")
     ap.add_argument("--page-size", type=int, default=64, help="paged: keys of a page")
     ap.add_argument("--cache", default="16", choices=["16", "e4m3"], help="paged: 16-bit pages, or codes with an exponent a row")
+    ap.add_argument("--keep", type=int, default=1024, help="evict: keys that stay, an eighth of them the latest")
     ap.add_argument("--graph", action="store_true",
                     help="capture one call in a CUDA graph and time replays (schedules with one launch per level)")
     a = ap.parse_args()
@@ -139,12 +145,15 @@ def main():
         biases, projections = [uni(bound, a.H) for _ in range(2)], [uni(1.0, a.H).to(dt) for _ in range(2)]
         lens = (torch.arange(a.N, device=dev, dtype=torch.int32) % a.L) + 1
         fn = lambda: ops.rnn_attention(src, trg, *weights, *biases, *projections, lens)
-    elif a.case == "paged":
+    elif a.case in ("paged", "tree", "weigh", "evict"):
         # the new tokens are written to the cache and attend to it; page numbers in random order
         per = -(-a.S // a.page_size)
         kv, d = a.kv_heads, 128
-        cache = ops.paged_cache(a.B * per, kv, a.page_size, d, dt if a.cache == "16" else torch.float8_e4m3fn, dev)
-        table = torch.randperm(a.B * per, device=dev, generator=g).int().view(a.B, per)
+        more = -(-a.keep // a.page_size) if a.case == "evict" else 0  # pages of a sequence to move to
+        pages = a.B * (per + more)
+        cache = ops.paged_cache(pages, kv, a.page_size, d, dt if a.cache == "16" else torch.float8_e4m3fn, dev)
+        order = torch.randperm(pages, device=dev, generator=g).int()
+        table, into = order[: a.B * per].view(a.B, per), order[a.B * per:].view(a.B, more)
         lens = torch.full((a.B,), a.S, dtype=torch.int32, device=dev)
         whole = torch.arange(a.B + 1, device=dev, dtype=torch.int32)
         for b in range(a.B):  # (a sequence at a time: all of them at once would take the cache's room again)
@@ -156,6 +165,24 @@ def main():
         def fn():
             ops.paged_cache_write(cache, k, v, table, lens, starts)
             return ops.paged_attention(q, cache, table, lens, starts, scale=1 / math.sqrt(d), window=a.window)
+        weights = rnd(pages, kv, a.page_size).exp_() if a.case in ("weigh", "evict") else None
+        if a.case == "tree":
+            # a token behind one of the eight in front of it
+            parents = torch.stack([torch.randint(max(0, i - 8), max(1, i), (a.B,), device=dev, generator=g) for i in range(a.new)], 1).int()
+            fn = lambda: ops.paged_attention(q, cache, table, lens, starts, scale=1 / math.sqrt(d), tree=ops.tree_mask(parents).flatten(0, 1))
+        elif a.case == "weigh":
+            lse = torch.empty(T, a.heads, device=dev)
+            ops.paged_attention(q, cache, table, lens, starts, scale=1 / math.sqrt(d), window=a.window, lse=lse)
+            fn = lambda: ops.paged_attention_weights(q, cache, weights, lse, table, lens, starts, scale=1 / math.sqrt(d), window=a.window)
+        elif a.case == "evict":
+            fn = lambda: ops.paged_cache_evict(cache, weights, table, lens, a.keep, a.keep // 8, into=into)
+    elif a.case == "verify_tree":
+        N = a.new + 1
+        probs = torch.softmax(3 * rnd(a.B, N, a.V), -1)
+        parents = torch.stack([torch.randint(max(0, i - 8), max(1, i), (a.B,), device=dev, generator=g) for i in range(N)], 1).int()
+        tokens = probs.gather(1, parents.long()[..., None].expand(-1, -1, a.V)).argmax(-1)  # each the likeliest behind its parent
+        u = torch.rand(a.B, N, device=dev, generator=g)
+        fn = lambda: ops.verify_tree(probs, tokens, parents, u)
     elif a.case == "verify":
         p, q = (torch.softmax(2 * rnd(a.B, a.new + i, a.V), -1) for i in (1, 0))
         drafts = torch.multinomial(q.view(-1, a.V), 1, generator=g).view(a.B, a.new)
