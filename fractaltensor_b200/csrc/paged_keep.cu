@@ -8,7 +8,12 @@
 // paged_move: row first + kept[i] goes to first + i, i < counts, of keys, values, exponents and weights.  Into other pages every step of rows
 // is on its own.  In the same pages a chain of steps is one CTA's: kept ascends, so that kept[i] >= i, and what a step writes (up to
 // row i) is never read by a later one (kept[j] > kept[i] >= i); within a step all rows are read before one is written.  Chains run side
-// by side for the pieces of a row, which do not meet.
+// by side for the pieces of a row, which do not meet, and where there are few, a cluster of CTAs takes a step together.
+//
+// 48 sequences of 1500 to 9000 keys of 16 bits, 8 kv heads of 128, to 2048 of them in other pages: 163 us, of which the moves, bound by memory, are 131
+// (6.2 TB/s) and the choice 30, trips and digits one behind the other.  One of 100 001 keys of 8 bits, 4 kv heads, to 8192 in its own pages 28 us
+// (372 with chains of single CTAs that looked rows up one behind the other).  The paths of 128 trees 3.5 us, a launch.  Measured and not kept: lanes with
+// the same digit adding as one (30 for 28 us).
 #include <algorithm>
 #include <climits>
 
