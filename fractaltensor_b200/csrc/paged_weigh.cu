@@ -162,12 +162,13 @@ paged_weigh_kernel(const __grid_constant__ Weigh x) {
         bool odd = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float mine = load_query<T, k8, D>(a, of.first, now.h, flat0, nt * 8 + g, rows, c, q[nt]);
+          // (behind the last row that one again, which takes away infinity: zeros times an infinity of a key would be NaN)
+          const float mine = load_query<T, k8, D>(a, of.first, now.h, flat0, min(nt * 8 + g, rows - 1), rows, c, q[nt]);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             factor[nt][e] = __shfl_sync(0xffffffffu, mine, (2 * c + e) * 4);
             const int r = nt * 8 + 2 * c + e, flat = flat0 + r, token = flat / a.group;
-            float lse = INFINITY;  // (rows that there are none of take away infinity from scores of 0)
+            float lse = INFINITY;
             if (r < rows) lse = x.lse[static_cast<long long>(of.first + token) * heads + now.h * a.group + flat - token * a.group];
             const bool fine = fabsf(lse) < INFINITY;  // (not of a row that sees nothing, or something that is not finite)
             odd |= r < rows && !fine;

@@ -100,6 +100,32 @@ def test_rows_that_are_not_finite_add_nothing(eight_bit, new, lens):
     _weigh_check(weights, before, q.nan_to_num(0.0), cache, lse, table, ln, st, 0.08)
 
 
+@pytest.mark.parametrize("new,lens", [([1, 1], [90, 40]), ([3], [70]), ([20, 30], [400, 30]), ([200], [600])])
+def test_keys_of_minus_infinity_weigh_nothing(new, lens):
+    """Scores of -inf are ordinary: of such keys nothing is added, and beside them everything."""
+    ops = _ops()
+    kv, group, d, page = 2, 3, 128, 16
+    table, ln, st, pages = _batch(new, lens, page)
+    k, v = _full_cache(pages, kv, page, d, BF16, 3)
+    for b, n in enumerate(lens):
+        for j in (0, n // 2, n // 3):
+            if j != n - 1:
+                k[int(table[b, j // page]), :, j % page, 5] = -float("inf")
+    T = int(st[-1])
+    q = _numbers((T, kv * group, d), BF16, 1).cuda()
+    q[..., 5] = q[..., 5].abs() + 0.5
+    args = (table.cuda(), ln.cuda(), st.cuda())
+    seen = torch.arange(T) if T <= 3 else torch.tensor([t for b in range(len(new)) for t in range(int(st[b]), int(st[b + 1])) if lens[b] - new[b] + t - int(st[b]) > 0])
+    lse = torch.empty(T, kv * group, device="cuda")
+    ops.paged_attention(q, (k, v), *args, scale=0.08, lse=lse)
+    assert bool(torch.isfinite(lse[seen.cuda()]).all())
+    weights = torch.zeros(pages, kv, page, device="cuda")
+    ops.paged_attention_weights(q, (k, v), weights, lse, *args, scale=0.08)
+    ops.check_status()
+    assert bool(torch.isfinite(weights).all())
+    _weigh_check(weights, weights * 0, q, (k, v), lse, table, ln, st, 0.08)
+
+
 @pytest.mark.parametrize("by", [2.0 ** 100, 2.0 ** -100])
 def test_scales_of_queries_and_keys_that_cancel(by):
     ops = _ops()
