@@ -92,6 +92,7 @@ paged_choose_kernel(const __grid_constant__ Choose a, int room) {
   uint32_t prefix = 0, known = 0;  // the digits so far, and which bits they are
   int left = want;
   for (int i = threadIdx.x; i < kCopies * kBins; i += kThreads) (&bins[0][0][0])[i] = 0;
+  if (threadIdx.x == 0) s_digit = s_left = 0;
   __syncthreads();
   for (int d = 0; d < 4; ++d) {
     const int low = 24 - 8 * d;
@@ -209,8 +210,9 @@ paged_choose_kernel(const __grid_constant__ Choose a, int room) {
     const unsigned is_above = __ballot_sync(0xffffffffu, i < to && key > prefix), is_equal = __ballot_sync(0xffffffffu, i < to && key == prefix);
     const unsigned in_front = (1u << lane) - 1u;
     const int equals = equal + __popc(is_equal & in_front);
-    if ((is_above >> lane & 1u) != 0 || ((is_equal >> lane & 1u) != 0 && equals < left))
-      kept[above + __popc(is_above & in_front) + min(left, equals)] = i;
+    // (weights that another stream changes meanwhile may give any counts: nothing is written behind the head's own)
+    const int to_at = above + __popc(is_above & in_front) + min(left, equals);
+    if (((is_above >> lane & 1u) != 0 || ((is_equal >> lane & 1u) != 0 && equals < left)) && to_at >= 0 && to_at < want) kept[to_at] = i;
     above += __popc(is_above);
     equal += __popc(is_equal);
   }
