@@ -383,11 +383,9 @@ int launch_choose(const Choose& a, int B, cudaStream_t stream) {
   return launch_clusters(paged_choose_kernel<C, kThreads>, C, dim3(static_cast<unsigned>(B) * a.kv_heads * C), kThreads, static_cast<size_t>(room) * 4,
                          stream, a, room);
 }
-// Whether eight CTAs to a sequence and kv head are no more than the device has room for at a time.
-bool few_heads(int B, int kv_heads) { return static_cast<long long>(B) * kv_heads * 8 <= 2ll * current_sm_count(); }
-
 int launch_choose(const Choose& a, int B, cudaStream_t stream) {
-  const bool apart = (static_cast<long long>(a.batch.W) << a.batch.page_shift) > 4096 && few_heads(B, a.kv_heads);
+  // Clusters where there are more keys than a few a thread and eight CTAs to a sequence and kv head are no more than the device has room for at a time.
+  const bool apart = (static_cast<long long>(a.batch.W) << a.batch.page_shift) > 4096 && static_cast<long long>(B) * a.kv_heads * 8 <= 2ll * current_sm_count();
   return apart ? launch_choose<8, 1024>(a, B, stream) : launch_choose<1, 512>(a, B, stream);
 }
 
@@ -405,9 +403,14 @@ template <int kRow>
 int launch_move(const Move& a, int B, cudaStream_t stream) {
   // A few rows of a tree: a warp has them in one step or two.
   if (a.most <= 64) return launch_move<kRow, 2 * kRow, 32, 1>(a, B, stream);
-  // In the same pages a part of a row is a chain: narrow parts, and clusters that read thousands of rows before they write them, where there
-  // are few chains and long ones.
-  if (a.into == a.batch.table && few_heads(B, a.kv_heads)) return launch_move<kRow, kRow / 4, kMoveThreads, 8>(a, B, stream);
+  // In the same pages a part of a row is a chain, one step behind the other: clusters, which read hundreds of rows before they write them, as
+  // long as their CTAs are on the device at a time, and parts of a row where they fill it with few heads.  2048 of 4096 rows of 16 bits, d 128, with
+  // weights, us, of (heads) 4: parts 5.4, clusters of 8 9.2, of 4 15.8, one CTA 41.6; 32: 21.3, 15.1, 26.5, 44.6; 80: 56.7, 37.4, 36.4, 84.9; 160:
+  // 120, 72, 71, 98; 384: 327, 157, 149, 144.5.  512 rows: 32 heads 18.1, 5.1, 7.7, 11.9; 384 200, 45, 41, 36.
+  const long long heads = static_cast<long long>(B) * a.kv_heads, sms = current_sm_count();
+  if (a.into == a.batch.table && heads * 64 <= 4 * sms) return launch_move<kRow, kRow / 4, kMoveThreads, 8>(a, B, stream);
+  if (a.into == a.batch.table && heads * 8 <= 3 * sms) return launch_move<kRow, 2 * kRow, kMoveThreads, 8>(a, B, stream);
+  if (a.into == a.batch.table && heads * 4 <= 6 * sms) return launch_move<kRow, 2 * kRow, kMoveThreads, 4>(a, B, stream);
   return launch_move<kRow, 2 * kRow, kMoveThreads, 1>(a, B, stream);
 }
 int move(const Move& a, int row_bytes, int B, cudaStream_t stream) {
