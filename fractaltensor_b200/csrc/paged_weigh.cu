@@ -273,15 +273,18 @@ struct Form {
   int few, most;
   bool many;
 };
-Form form_of(int T, int B, int group, bool k8) {
-  // Each tile of 16 rows goes through a block's keys, in registers, again; paged_weigh_tile.cu takes as long for 20 rows as for 128.  8 sequences
-  // of 4000 keys, 8 kv heads, 16 bits: 48 rows 54 us and 70 there, 64 rows 68 and 70, 96 rows 96 and 70; one of 500 keys, 64 rows 10.9 and 14.4.
-  // Of 8 bits, whose codes become fp16 for every tile: 20 rows 53 and 43, 64 rows 95 and 46; one of 500, 32 rows 9.0 and 14.1, 64 rows 12.9 and 14.6.
-  const int most = k8 ? 32 : 64;
+// `keys`: as many as the table has room for.
+Form form_of(int T, int B, int group, int kv_heads, long long keys) {
   const long long rows = static_cast<long long>(T) * group;
-  if (T <= B || rows <= most) return {rows <= 8ll * B ? 8 : 16, INT_MAX, false};
+  if (T <= B || rows <= 16) return {rows <= 8ll * B ? 8 : 16, INT_MAX, false};
+  // Each tile of 16 rows goes through a block's keys, in registers, again, while paged_weigh_tile.cu takes as long for 20 rows as for 128, three
+  // launches at least.  8 kv heads, 16 bits, here and there: one of 500 keys, 48 rows 9.6 and 12.6 us, 96 rows 14.1 and 13.0; of 16 000, 32 rows 23.5
+  // and 30.7, 64 rows 38 and 31; 8 of 4000, 20 rows (8064 units) 39.7 and 37.3; 48 of 500, 32 rows (6144) 30.8 and 31.5; 48 of 4000, 20 rows 193 and 147.
+  // 8 bits: one of 4000 keys, 48 rows 17.4 and 18.7, 64 rows 21 and 18.5; 8 of 4000, 20 rows 52 and 41.
+  const long long tiles = (rows + 16ll * B - 1) / (16ll * B);
+  if (tiles <= 3 && tiles * B * kv_heads * ((keys + 63) / 64) <= 4500) return {16, INT_MAX, false};
   if (B == 1) return {0, 0, true};
-  return {16, most, true};
+  return {16, 16, true};
 }
 
 }  // namespace
@@ -290,7 +293,8 @@ Form form_of(int T, int B, int group, bool k8) {
 using namespace ftb;
 
 extern "C" size_t ftb_paged_attn_weights_scratch_bytes(int T, int B, int kv_heads, int group, int d) {
-  if (T <= 0 || B <= 0 || kv_heads <= 0 || group <= 0 || d <= 0 || !form_of(T, B, group, true).many) return 0;  // (8 bits: what needs it sooner)
+  if (T <= 0 || B <= 0 || kv_heads <= 0 || group <= 0 || d <= 0) return 0;
+  if (T <= B || static_cast<long long>(T) * group <= 16) return 0;  // (never the other kernel; else it is the table's width that says)
   return paged_weigh_tile_scratch(T, kv_heads, group, d);
 }
 
@@ -335,7 +339,7 @@ extern "C" int ftb_paged_attn_weights(const void* q, long long q_row, long long 
   x.weights = weights;
   x.lse = lse;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const Form f = form_of(T, B, group, k_exp != nullptr);
+  const Form f = form_of(T, B, group, kv_heads, static_cast<long long>(W) * page_size);
   if (f.many) {
     if (static_cast<long long>(T) * heads > INT_MAX) return FTB_ERR_ARG;  // a copy's coordinates have 32 bits
     if (scratch == nullptr || scratch_bytes < paged_weigh_tile_scratch(T, kv_heads, group, d)) return FTB_ERR_WORKSPACE;

@@ -11,7 +11,8 @@
 //   warp 1        issues the products, into one of two buffers of scores
 //   warps 2..17   exponentials and sums, while the next tile's scores are made: a thread has a key of either half of the block and a quarter
 //                 of the tile's rows
-//   warps 18..21  load the keys of the next block and make them operands (8-bit codes as fp16; a key's scale goes to its scores)
+//   warps 18..21  load the keys of the next block, all of them on their way at once (8 at a time a warp: 332 for 142 us of 48 sequences of 4000 keys,
+//                 64 rows), and make 8-bit codes fp16; a key's scale goes to its scores
 // A block that a cut goes through leaves parts of its sums, which a second kernel adds up in their order.
 //
 // 2048 tokens of 32 heads of 128 over 8 kv heads, 16 384 keys of 8 bits: 331 us, 0.78 PFLOP/s.  Bound by no unit alone: without the
@@ -541,37 +542,37 @@ paged_weigh_tile_kernel(const __grid_constant__ Weigh x, const __grid_constant__
         ctl.scale[buffer][of_block + e * 32 + lane] = scales[e];
       }
       uint8_t* tile = sK + (buffer * 2 + (of_block >> 7)) * P::kTile;
-      constexpr int kPieces = k8 ? D / 16 : D / 8, kTogether = 32 / kPieces, kAtOnce = kPieces < 8 ? kPieces : 8;  // 16 bytes of a row of the cache a lane
+      // 16 bytes of a row of the cache a lane, as many on their way as there are: 16-bit rows straight into their places, codes by way of registers
+      constexpr int kPieces = k8 ? D / 16 : D / 8, kTogether = 32 / kPieces, kTurns = 64 / kTogether;
       const int piece_of = lane % kPieces;
+      auto put_at = [&](int q, int r) { return tile + (q >> 3) * P::kHalf + r * 128 + (((q & 7) ^ (r & 7)) << 4); };
+      if constexpr (k8) {
+        uint4 v[kTurns];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-#pragma unroll 1
-        for (int r0 = 0; r0 < 32; r0 += kTogether * kAtOnce) {
-          uint4 v[kAtOnce];
-#pragma unroll
-          for (int k = 0; k < kAtOnce; ++k) {
-            const int row = __shfl_sync(0xffffffffu, rows[e], r0 + k * kTogether + lane / kPieces);
-            v[k] = row >= 0 ? *reinterpret_cast<const uint4*>(a.k + static_cast<long long>(row) * (k8 ? D : 2 * D) + piece_of * 16) : make_uint4(0u, 0u, 0u, 0u);
-          }
-#pragma unroll
-          for (int k = 0; k < kAtOnce; ++k) {
-            const int r = (of_block & 64) + e * 32 + r0 + k * kTogether + lane / kPieces;
-            auto put = [&](int q, const uint4& w) {
-              *reinterpret_cast<uint4*>(tile + (q >> 3) * P::kHalf + r * 128 + (((q & 7) ^ (r & 7)) << 4)) = w;
-            };
-            if constexpr (k8) {
-              uint4 o;
-              e4m3x4_to_f16x2(v[k].x, o.x, o.y);
-              e4m3x4_to_f16x2(v[k].y, o.z, o.w);
-              put(2 * piece_of, o);
-              e4m3x4_to_f16x2(v[k].z, o.x, o.y);
-              e4m3x4_to_f16x2(v[k].w, o.z, o.w);
-              put(2 * piece_of + 1, o);
-            } else {
-              put(piece_of, v[k]);
-            }
-          }
+        for (int k = 0; k < kTurns; ++k) {
+          const int row = __shfl_sync(0xffffffffu, rows[k * kTogether / 32], k * kTogether % 32 + lane / kPieces);
+          v[k] = row >= 0 ? *reinterpret_cast<const uint4*>(a.k + static_cast<long long>(row) * D + piece_of * 16) : make_uint4(0u, 0u, 0u, 0u);
         }
+#pragma unroll
+        for (int k = 0; k < kTurns; ++k) {
+          const int r = (of_block & 64) + k * kTogether + lane / kPieces;
+          uint4 o;
+          e4m3x4_to_f16x2(v[k].x, o.x, o.y);
+          e4m3x4_to_f16x2(v[k].y, o.z, o.w);
+          *reinterpret_cast<uint4*>(put_at(2 * piece_of, r)) = o;
+          e4m3x4_to_f16x2(v[k].z, o.x, o.y);
+          e4m3x4_to_f16x2(v[k].w, o.z, o.w);
+          *reinterpret_cast<uint4*>(put_at(2 * piece_of + 1, r)) = o;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < kTurns; ++k) {
+          const int row = __shfl_sync(0xffffffffu, rows[k * kTogether / 32], k * kTogether % 32 + lane / kPieces);
+          copy16_async(reinterpret_cast<float*>(put_at(piece_of, (of_block & 64) + k * kTogether + lane / kPieces)),
+                       reinterpret_cast<const float*>(a.k + static_cast<long long>(max(row, 0)) * (2 * D) + piece_of * 16), row >= 0);
+        }
+        copies_commit();
+        copies_wait();
       }
       fence_proxy_async_smem();
       const bool last = y.last != 0;
