@@ -25,7 +25,7 @@ namespace {
 constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kJoinRows = 4, kMostCuts = 4 * kJoinThreads;
 
 constexpr float kLog2E = 1.4426950408889634f;
-constexpr int kShortUnits = 5500;
+constexpr int kShortUnits = 8000, kTileUnits = 24;  // see form_of_tree
 
 struct Pieces {
   const float* parts;
@@ -296,14 +296,18 @@ Form form_of(int T, int B, int group) {
 }
 
 // The same for trees, of which a sequence has a few dozen tokens; `keys`: as many as the table has room for.  While the tiles of
-// paged_short.cu make few units of 64 keys, its CTAs, two of them an SM, are done sooner, however many tiles read the same keys: one sequence of
-// 25 tokens, 32 heads over 8 kv heads, 16 bits: 800 keys (728 units) 23.5 us and 27.6 with paged_tile.cu, 3200: 30.9 and 36.6, 6400 (5600): 40.6 and
-// 43.7; of 60 tokens, 3200 keys (6000): 46.0 and 46.0, 6400: 67.5 and 58.2.
+// paged_short.cu make few units of 64 keys, its CTAs, two of them an SM, are done sooner, however many tiles read the same keys; each tile's start and end
+// count as 24 units more.  32 heads over 8 kv heads, 16 bits, us there and in paged_tile.cu:
+//   one sequence of 25 tokens     800 keys (2072 units so counted) 23.5 27.6; 3200 (4144) 30.9 36.6; 6400 (6944) 40.6 43.7
+//   one of 60                     3200 (8880) 46.0 46.0; 6400 (14880) 67.5 58.2
+//   four of 25                    200 (6272) 26.1 26.8; 500 (7168) 30.2 28.5; 1000 (8960) 36.4 37.9; 2000 (12544) 50.8 41.5
+//   ten of 25                     70 (8320) 30.8 21.2; 200 (8960) 36.4 34.5; 1000 (12800) 66.0 41.5
+//   31 of 16, 128 heads, d 64     70 (103 168) 96.6 33.1; 500 (126 976) 170 63
 Form form_of_tree(int T, int B, int group, int kv_heads, long long keys) {
   Form f = form_of(T, B, group);
   if (f.many == 0) return f;
   const long long rows = static_cast<long long>(T) * group;
-  if ((rows + 16ll * B - 1) / (16ll * B) * B * kv_heads * ((keys + 63) / 64) <= kShortUnits) return {16, INT_MAX, 0, false};
+  if ((rows + 16ll * B - 1) / (16ll * B) * B * kv_heads * ((keys + 63) / 64 + kTileUnits) <= kShortUnits) return {16, INT_MAX, 0, false};
   // A second tile for a few rows costs as much as the first: 32 sequences of 33 tokens of 8 heads each of 8 kv heads, up to 16 000 keys of 8 bits, 720 us
   // with the last 8 rows apart, 945 without.
   const long long behind = rows / B > f.many ? rows / B % f.many : 0;
