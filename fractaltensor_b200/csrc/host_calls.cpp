@@ -739,7 +739,7 @@ PyObject* paged_cache_evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
     DECLINE_UNLESS(paged_call(args[0], args[2], args[3], nullptr, &c));
     const at::Tensor *weights = c.here(args[1], at::kFloat, {c.pages, c.kv, c.page_size}), *into;
     int64_t keep, recent;
-    DECLINE_UNLESS(weights && get_int(args[4], &keep) && get_int(args[5], &recent) && keep > 0 && recent >= 0 && recent <= keep &&
+    DECLINE_UNLESS(weights && get_int(args[4], &keep) && get_int(args[5], &recent) && keep > 0 && keep <= 1 << 30 && recent >= 0 && recent <= keep &&
                    paged_into(args[6], c, &into));
     const c10::DeviceIndex dev = c.k->device().index();
     const at::Tensor ws = workspace_of(args[7], dev, ftb_workspace_bytes());

@@ -233,6 +233,8 @@ struct Move {
   int* status;
 };
 
+constexpr int kMostKept = 1 << 30;  // positions of a sequence: they are counted in 32 bits, some steps of all threads beyond the last one
+
 constexpr int kMoveThreads = 256, kMoveAtOnce = 8, kMostRoom = 48 * 1024;
 
 // Rows of cache planes that a kept row comes from and goes to; -1: none.
@@ -441,7 +443,7 @@ extern "C" int ftb_paged_cache_keep(void* k_cache, void* v_cache, unsigned char*
                                     int page_size, int d, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_cache(k_cache, v_cache, k_exp, v_exp, table, into, B, W, into_W, pages, kv_heads, page_size, d);
   if (rc) return rc;
-  if (K < 0 || (K > 0 && !kept) || !counts) return FTB_ERR_ARG;
+  if (K < 0 || K > kMostKept || (K > 0 && !kept) || !counts) return FTB_ERR_ARG;
   if (workspace == nullptr || workspace_bytes < ftb_workspace_bytes()) return FTB_ERR_WORKSPACE;
   if (K == 0) return FTB_OK;
   if ((rc = check_device_sm100())) return rc;
@@ -457,7 +459,8 @@ extern "C" int ftb_paged_cache_evict(void* k_cache, void* v_cache, unsigned char
                                      size_t workspace_bytes, void* stream) {
   int rc = check_cache(k_cache, v_cache, k_exp, v_exp, table, into, B, W, into_W, pages, kv_heads, page_size, d);
   if (rc) return rc;
-  if (!weights || !lens || !lens_out || !kept || keep <= 0 || recent < 0 || recent > keep) return FTB_ERR_ARG;
+  if (!weights || !lens || !lens_out || !kept || keep <= 0 || keep > kMostKept || recent < 0 || recent > keep) return FTB_ERR_ARG;
+  if (static_cast<long long>(W) * page_size > kMostKept) return FTB_ERR_ARG;
   if ((reinterpret_cast<uintptr_t>(weights) & 3) != 0) return FTB_ERR_ALIGN;
   if (workspace == nullptr || workspace_bytes < ftb_workspace_bytes()) return FTB_ERR_WORKSPACE;
   const size_t rows = static_cast<size_t>(pages) * kv_heads * page_size, row = k_exp != nullptr ? d : 2 * d;

@@ -1045,8 +1045,8 @@ def paged_cache_evict(cache, weights, table, lens, keep, recent=0, into=None):
     _req_like(weights, "weights", torch.float32, (pages, kv, page_size), k)
     _req_like(lens, "lens", torch.int32, (B,), k)
     keep, recent = int(keep), int(recent)
-    if not 0 <= recent <= keep or not 0 < keep <= 0x7fffffff:
-        raise ValueError("paged_cache_evict: keep is 1 or more and recent 0 to keep, got %d and %d" % (keep, recent))
+    if not 0 <= recent <= keep or not 0 < keep <= 1 << 30:
+        raise ValueError("paged_cache_evict: keep is 1 to 2^30 and recent 0 to keep, got %d and %d" % (keep, recent))
     now = torch.empty(B, dtype=torch.int32, device=k.device)
     kept = torch.empty(B, kv, keep, dtype=torch.int32, device=k.device)
     ws = workspace(k.device)

@@ -490,7 +490,7 @@ int ftb_verify_tree(const float* probs, long long p_seq, long long p_row, const 
  * (`kept_head` 0: the same for all heads); first: int32 [B] or NULL: 0.  table [B, W]: the pages that rows come from; into [B, into_W]: the
  * pages that they go to, none of which this call reads, or NULL (or table itself): the same pages, which belong to one sequence each.
  * Keys, values, exponents and, if not NULL, weights (fp32 [pages, kv_heads, page_size]) move together.  All other rows stay as they
- * were.  A row whose page one of the tables does not have, or with a negative number in kept, is not moved and sets the
+ * were.  K up to 2^30.  A row whose page one of the tables does not have, or with a negative number in kept, is not moved and sets the
  * (sticky) status word to 22. */
 int ftb_paged_cache_keep(void* k_cache, void* v_cache, unsigned char* k_exp, unsigned char* v_exp, float* weights,
                          const int* kept, long long kept_seq, long long kept_head, const int* counts, const int* first,
@@ -513,7 +513,7 @@ int ftb_paged_attn_weights(const void* q, long long q_row, long long q_head, con
  * them, the keep - recent with the largest weights, of equal weights those in front (NaN is below all numbers).  What stays is moved as by
  * ftb_paged_cache_keep, weights too; shorter sequences stay whole.  lens_out int32 [B]: min(lens[b], keep); kept int32
  * [B, kv_heads, keep]: the positions that stay, ascending, then -1.  A length that the table is too narrow for is cut and sets the (sticky)
- * status word to 22. */
+ * status word to 22.  keep, and the positions that the table has room for, up to 2^30. */
 int ftb_paged_cache_evict(void* k_cache, void* v_cache, unsigned char* k_exp, unsigned char* v_exp, float* weights,
                           const int* table, const int* lens, const int* into, int* lens_out, int* kept, int B, int W,
                           int into_W, int keep, int recent, int pages, int kv_heads, int page_size, int d, void* workspace,

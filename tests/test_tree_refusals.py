@@ -77,6 +77,13 @@ def test_evict_arguments(lib, kw):
     assert _evict(lib, **kw) == 1
 
 
+def test_most_positions(lib):
+    most = 1 << 30
+    assert _keep(lib, K=most + 1, ks=most + 1) == 1
+    assert _evict(lib, keep=most + 1) == _evict(lib, keep=(1 << 31) - 1) == 1
+    assert _evict(lib, W=most // 16 + 1) == 1
+
+
 @pytest.mark.parametrize("kw", [dict(p=Z), dict(tokens=Z), dict(parents=Z), dict(u=Z), dict(out=Z), dict(path=Z), dict(counts=Z), dict(B=-1), dict(N=0),
                                 dict(N=1025), dict(V=0), dict(V=(1 << 30) + 1)])
 def test_verify_arguments(lib, kw):
