@@ -10,10 +10,10 @@
 // row i) is never read by a later one (kept[j] > kept[i] >= i); within a step all rows are read before one is written.  Chains run side
 // by side for the pieces of a row, which do not meet, and where there are few, a cluster of CTAs takes a step together.
 //
-// 48 sequences of 1500 to 9000 keys of 16 bits, 8 kv heads of 128, to 2048 of them in other pages: 163 us, of which the moves, bound by memory, are 131
-// (6.2 TB/s) and the choice 30, trips and digits one behind the other.  One of 100 001 keys of 8 bits, 4 kv heads, to 8192 in its own pages 28 us
+// 48 sequences of 1500 to 9000 keys of 16 bits, 8 kv heads of 128, to 2048 of them in other pages: 159.6 us, of which the moves, bound by memory, are 131
+// (6.2 TB/s) and the choice 28, trips and digits one behind the other.  One of 100 001 keys of 8 bits, 4 kv heads, to 8192 in its own pages 28 us
 // (372 with chains of single CTAs that looked rows up one behind the other).  The paths of 128 trees 3.5 us, a launch.  Measured and not kept: lanes with
-// the same digit adding as one (30 for 28 us).
+// the same digit adding as one (30 for 28 us), a bin for every second lane (31).
 #include <algorithm>
 #include <climits>
 
@@ -34,7 +34,7 @@ struct Choose {
   int* status;
 };
 
-constexpr int kBins = 256, kCopies = 4, kChooseAtOnce = 8;
+constexpr int kBins = 256, kCopies = 4;
 
 // Unsigned numbers in the order of the weights; NaN is below all of them.
 __device__ __forceinline__ uint32_t order_of(float w) {
@@ -53,10 +53,10 @@ __device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
 template <int C, int kThreads>
 __global__ void __launch_bounds__(kThreads)
 paged_choose_kernel(const __grid_constant__ Choose a, int room) {
-  constexpr int kWarps = kThreads / 32;
+  constexpr int kWarps = kThreads / 32, kChooseAtOnce = C > 1 ? 8 : 4;  // (8 for one CTA: 161 us of 159.6; 4 for a cluster: 42 of 28)
   extern __shared__ uint32_t known_keys[];
   __shared__ int bins[2][kCopies][kBins], sums[2][kBins], above_of[kWarps], equal_of[kWarps], mine[2], of_warp[kBins / 32];
-  __shared__ int s_digit, s_left;
+  __shared__ int s_digit, s_left, s_all;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rank = C > 1 ? static_cast<int>(cluster_ctarank()) : 0, head = blockIdx.x / C;
   const int b = head / a.kv_heads, h = head - b * a.kv_heads;
@@ -92,7 +92,7 @@ paged_choose_kernel(const __grid_constant__ Choose a, int room) {
   uint32_t prefix = 0, known = 0;  // the digits so far, and which bits they are
   int left = want;
   for (int i = threadIdx.x; i < kCopies * kBins; i += kThreads) (&bins[0][0][0])[i] = 0;
-  if (threadIdx.x == 0) s_digit = s_left = 0;
+  if (threadIdx.x == 0) s_digit = s_left = s_all = 0;
   __syncthreads();
   for (int d = 0; d < 4; ++d) {
     const int low = 24 - 8 * d;
@@ -161,17 +161,19 @@ paged_choose_kernel(const __grid_constant__ Choose a, int room) {
       if (upto - count < left && upto >= left) {
         s_digit = 255 - threadIdx.x;
         s_left = left - (upto - count);
+        s_all = upto == left;
       }
     }
     __syncthreads();
     prefix |= static_cast<uint32_t>(s_digit) << low;
     known |= 255u << low;
     left = s_left;
+    if (s_all != 0) break;  // all that agree with the digits so far stay: mostly known after three of them
   }
   // what is above stays, of what is equal the first `left`
   int above = 0, equal = 0;
   for (int i = from + lane; i < to; i += 32) {
-    const uint32_t key = key_of(i);
+    const uint32_t key = key_of(i) & known;
     above += key > prefix;
     equal += key == prefix;
   }
@@ -206,7 +208,7 @@ paged_choose_kernel(const __grid_constant__ Choose a, int room) {
   }
   for (int i0 = from; i0 < to; i0 += 32) {
     const int i = i0 + lane;
-    const uint32_t key = i < to ? key_of(i) : 0u;
+    const uint32_t key = i < to ? key_of(i) & known : 0u;
     const unsigned is_above = __ballot_sync(0xffffffffu, i < to && key > prefix), is_equal = __ballot_sync(0xffffffffu, i < to && key == prefix);
     const unsigned in_front = (1u << lane) - 1u;
     const int equals = equal + __popc(is_equal & in_front);

@@ -343,6 +343,29 @@ def test_evict_all_equal_and_too_long():
     assert now.tolist() == [10, 0] and kept[0, 0].tolist() == [0, 1, 2, 3, 4, 5, 44, 45, 46, 47] and kept[1, 0].tolist() == [-1] * 10
 
 
+@pytest.mark.parametrize("kind", ["powers of four", "halves of an octave", "last bits", "two values"])
+@pytest.mark.parametrize("sequences", [1, 40])
+def test_evict_by_digits(kind, sequences):
+    """Weights whose order is known after one digit of their bits, two or three, or only after the last."""
+    ops = _ops()
+    page, keep, recent, n = 16, 50, 6, 5000 if kind == "two values" else 240
+    table, ln, _, pages = _batch([0] * sequences, [n] * sequences, page)
+    table = torch.nn.functional.pad(table, (0, max(0, 320 - table.shape[1])), value=-1)  # (as wide as for sequences that have clusters)
+    cache = _full_cache(pages, 2, page, 64, BF16, 3)
+    g = torch.Generator().manual_seed(7)
+    i = torch.arange(pages * 2 * page, dtype=torch.int64)[torch.randperm(pages * 2 * page, generator=g)].view(pages, 2, page)
+    weights = {"powers of four": 4.0 ** (i % 120 - 60).double(), "halves of an octave": 1.0 + (i % 128).double() / 128, "last bits": 1.0 + (i % 256).double() * 2.0**-23,
+               "two values": 1.0 + (i % 100 == 0).double()}[kind].float()
+    want_lens, want_kept = tree.choose(weights, table, [n] * sequences, keep, recent)
+    weights = weights.cuda()
+    planes = _planes(cache, weights)
+    want = tree.keep([x.cpu() for x in planes], want_kept, want_lens, table, None, None)
+    now, kept = ops.paged_cache_evict(cache, weights, table.cuda(), ln.cuda(), keep, recent)
+    ops.check_status()
+    assert torch.equal(now.cpu(), want_lens) and torch.equal(kept.cpu(), want_kept)
+    _same(planes, want)
+
+
 def test_refusals():
     ops = _ops()
     table, ln, st, pages = _batch([1, 1], [40, 20], 16)
