@@ -10,10 +10,11 @@
 // row i) is never read by a later one (kept[j] > kept[i] >= i); within a step all rows are read before one is written.  Chains run side
 // by side for the pieces of a row, which do not meet, and where there are few, a cluster of CTAs takes a step together.
 //
-// 48 sequences of 1500 to 9000 keys of 16 bits, 8 kv heads of 128, to 2048 of them in other pages: 159.6 us, of which the moves, bound by memory, are 131
-// (6.2 TB/s) and the choice 28, trips and digits one behind the other.  One of 100 001 keys of 8 bits, 4 kv heads, to 8192 in its own pages 28 us
-// (372 with chains of single CTAs that looked rows up one behind the other).  The paths of 128 trees 3.5 us, a launch.  Measured and not kept: lanes with
-// the same digit adding as one (30 for 28 us), a bin for every second lane (31).
+// 48 sequences of 1500 to 9000 keys of 16 bits, 8 kv heads of 128, to 2048 of them in other pages: 156.8 us, of which the moves, bound by memory, are 131
+// (6.2 TB/s) and the choice 26, trips and digits one behind the other.  One of 100 001 keys of 8 bits, 4 kv heads, to 8192 in its own pages 23.5 us
+// (372 with chains of single CTAs that looked rows up one behind the other).  Its choice
+// is bound by instructions, some 20 a key and digit, and by a cluster's barriers, 1 us each.  The paths of 128 trees 3.5 us, a launch.  Measured and not kept: lanes with
+// the same digit adding as one (30 for 28 us), a bin for every second lane (31 for 28).
 #include <algorithm>
 #include <climits>
 
@@ -51,9 +52,9 @@ __device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
 
 // C CTAs for each sequence and kv head, a stretch of the keys each, of which `room` stay in shared memory after they have been read.
 template <int C, int kThreads>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, C == 1 ? 3 : 1)
 paged_choose_kernel(const __grid_constant__ Choose a, int room) {
-  constexpr int kWarps = kThreads / 32, kChooseAtOnce = C > 1 ? 8 : 4;  // (8 for one CTA: 161 us of 159.6; 4 for a cluster: 42 of 28)
+  constexpr int kWarps = kThreads / 32, kSweep = 4, kChooseAtOnce = C > 1 ? 8 : 4;  // (the last: 8 for one CTA 161 us for 159.6, 4 for a cluster 42 for 28)
   extern __shared__ uint32_t known_keys[];
   __shared__ int bins[2][kCopies][kBins], sums[2][kBins], above_of[kWarps], equal_of[kWarps], mine[2], of_warp[kBins / 32];
   __shared__ int s_digit, s_left, s_all;
@@ -88,9 +89,26 @@ paged_choose_kernel(const __grid_constant__ Choose a, int room) {
   const int from = static_cast<int>(min(static_cast<long long>(old), static_cast<long long>(rank * kWarps + warp) * stretch));
   const int to = static_cast<int>(min(static_cast<long long>(old), static_cast<long long>(from) + stretch));
   const int first = static_cast<int>(min(static_cast<long long>(old), static_cast<long long>(rank) * kWarps * stretch));  // of the CTA's
-  auto key_of = [&](int i) -> uint32_t { return i - first < room ? known_keys[i - first] : key_at(i); };
+  // f(i, key) for this lane's keys and 0 behind them, all lanes of the warp at once; some of them loaded before one is looked at
+  const int held = static_cast<int>(min(static_cast<long long>(to), static_cast<long long>(first) + room));
+  auto each = [&](auto f) {
+    int i0 = from;
+    for (; i0 < held; i0 += 32 * kSweep) {
+      uint32_t key[kSweep];
+#pragma unroll
+      for (int u = 0; u < kSweep; ++u) key[u] = i0 + u * 32 + lane < held ? known_keys[i0 + u * 32 + lane - first] : 0u;
+      if (i0 + 32 * kSweep > held && held < to) break;  // (the others are not held)
+#pragma unroll
+      for (int u = 0; u < kSweep; ++u) f(i0 + u * 32 + lane, key[u]);
+    }
+    for (; i0 < to; i0 += 32) {
+      const int i = i0 + lane;
+      f(i, i < held ? known_keys[i - first] : i < to ? key_at(i) : 0u);
+    }
+  };
   uint32_t prefix = 0, known = 0;  // the digits so far, and which bits they are
   int left = want;
+  bool all = false;  // whatever agrees with the digits stays
   for (int i = threadIdx.x; i < kCopies * kBins; i += kThreads) (&bins[0][0][0])[i] = 0;
   if (threadIdx.x == 0) s_digit = s_left = s_all = 0;
   __syncthreads();
@@ -124,10 +142,9 @@ paged_choose_kernel(const __grid_constant__ Choose a, int room) {
         }
       }
     } else {
-      for (int i = from + lane; i < to; i += 32) {
-        const uint32_t key = key_of(i);
-        if ((key & known) == prefix) atomicAdd(bin + (key >> low & 255u), 1);
-      }
+      each([&](int i, uint32_t key) {
+        if (i < to && (key & known) == prefix) atomicAdd(bin + (key >> low & 255u), 1);
+      });
     }
     __syncthreads();
     // thread i: bin 255 - i, and how many keys are in the bins above
@@ -157,7 +174,8 @@ paged_choose_kernel(const __grid_constant__ Choose a, int room) {
     }
     __syncthreads();
     if (threadIdx.x < kBins) {
-      for (int w = 0; w < warp; ++w) upto += of_warp[w];
+#pragma unroll
+      for (int w = 0; w < kBins / 32; ++w) upto += w < warp ? of_warp[w] : 0;
       if (upto - count < left && upto >= left) {
         s_digit = 255 - threadIdx.x;
         s_left = left - (upto - count);
@@ -168,14 +186,19 @@ paged_choose_kernel(const __grid_constant__ Choose a, int room) {
     prefix |= static_cast<uint32_t>(s_digit) << low;
     known |= 255u << low;
     left = s_left;
-    if (s_all != 0) break;  // all that agree with the digits so far stay: mostly known after three of them
+    all = s_all != 0;
+    if (all) break;  // mostly after three digits
   }
-  // what is above stays, of what is equal the first `left`
+  // what is above stays, of what is equal the first `left`; where all of that stays, it counts as above
+  const uint32_t least = all ? prefix : prefix + 1;
   int above = 0, equal = 0;
-  for (int i = from + lane; i < to; i += 32) {
-    const uint32_t key = key_of(i) & known;
-    above += key > prefix;
-    equal += key == prefix;
+  if (all) {
+    each([&](int i, uint32_t key) { above += i < to && (key & known) >= least; });
+  } else {
+    each([&](int i, uint32_t key) {
+      above += i < to && key >= least;
+      equal += i < to && key == prefix;
+    });
   }
   above = __reduce_add_sync(0xffffffffu, above);
   equal = __reduce_add_sync(0xffffffffu, equal);
@@ -184,39 +207,41 @@ paged_choose_kernel(const __grid_constant__ Choose a, int room) {
     equal_of[warp] = equal;
   }
   __syncthreads();
-  above = equal = 0;  // in front of this warp's stretch
-  int all_above = 0, all_equal = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) {
-      above += above_of[w];
-      equal += equal_of[w];
-    }
-    all_above += above_of[w];
-    all_equal += equal_of[w];
-  }
+  const int its_above = lane < kWarps ? above_of[lane] : 0, its_equal = lane < kWarps ? equal_of[lane] : 0;
+  above = __reduce_add_sync(0xffffffffu, lane < warp ? its_above : 0);  // in front of this warp's stretch
+  equal = __reduce_add_sync(0xffffffffu, lane < warp ? its_equal : 0);
   if constexpr (C > 1) {
-    if (threadIdx.x == 0) {
-      mine[0] = all_above;
-      mine[1] = all_equal;
+    if (warp == 0) {
+      const int all_above = __reduce_add_sync(0xffffffffu, its_above), all_equal = __reduce_add_sync(0xffffffffu, its_equal);
+      if (lane == 0) {
+        mine[0] = all_above;
+        mine[1] = all_equal;
+      }
     }
     cluster_sync_all();
-    for (int r = 0; r < rank; ++r) {
-      above += ld_cluster_s32(map_to_cta(smem_u32(&mine[0]), r));
-      equal += ld_cluster_s32(map_to_cta(smem_u32(&mine[1]), r));
-    }
+    above += __reduce_add_sync(0xffffffffu, lane < rank ? ld_cluster_s32(map_to_cta(smem_u32(&mine[0]), lane)) : 0);
+    equal += __reduce_add_sync(0xffffffffu, lane < rank ? ld_cluster_s32(map_to_cta(smem_u32(&mine[1]), lane)) : 0);
   }
-  for (int i0 = from; i0 < to; i0 += 32) {
-    const int i = i0 + lane;
-    const uint32_t key = i < to ? key_of(i) & known : 0u;
-    const unsigned is_above = __ballot_sync(0xffffffffu, i < to && key > prefix), is_equal = __ballot_sync(0xffffffffu, i < to && key == prefix);
-    const unsigned in_front = (1u << lane) - 1u;
-    const int equals = equal + __popc(is_equal & in_front);
-    // (weights that another stream changes meanwhile may give any counts: nothing is written behind the head's own)
-    const int to_at = above + __popc(is_above & in_front) + min(left, equals);
-    if (((is_above >> lane & 1u) != 0 || ((is_equal >> lane & 1u) != 0 && equals < left)) && to_at >= 0 && to_at < want) kept[to_at] = i;
-    above += __popc(is_above);
-    equal += __popc(is_equal);
+  // (weights that another stream changes meanwhile may give any counts: nothing is written behind the head's own)
+  const unsigned in_front = (1u << lane) - 1u;
+  if (all) {
+    each([&](int i, uint32_t key) {
+      const bool stays = i < to && (key & known) >= least;
+      const unsigned those = __ballot_sync(0xffffffffu, stays);
+      const unsigned to_at = above + __popc(those & in_front);
+      if (stays && to_at < static_cast<unsigned>(want)) kept[to_at] = i;
+      above += __popc(those);
+    });
+  } else {
+    each([&](int i, uint32_t key) {
+      const bool is_above = i < to && key >= least, is_equal = i < to && key == prefix;
+      const unsigned those = __ballot_sync(0xffffffffu, is_above), equals = __ballot_sync(0xffffffffu, is_equal);
+      const int before = equal + __popc(equals & in_front);
+      const unsigned to_at = above + __popc(those & in_front) + min(left, before);
+      if ((is_above || (is_equal && before < left)) && to_at < static_cast<unsigned>(want)) kept[to_at] = i;
+      above += __popc(those);
+      equal += __popc(equals);
+    });
   }
   if constexpr (C > 1) cluster_sync_all();  // nobody leaves while its counts may be read
 }
@@ -383,14 +408,22 @@ int launch_choose(const Choose& a, int B, cudaStream_t stream) {
   // room for a CTA's stretch of the longest sequence that the table allows, as far as there is some
   const long long longest = static_cast<long long>(a.batch.W) << a.batch.page_shift, stretch = (longest + C * kThreads - 1) / (C * kThreads) * kThreads;
   const int room = static_cast<int>(std::min(stretch, static_cast<long long>(kMostRoom)));
+  if (C > 8 && cudaFuncSetAttribute(paged_choose_kernel<C, kThreads>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+    cudaGetLastError();
+    return FTB_ERR_LAUNCH;
+  }
   if (!ensure_dynamic_smem(paged_choose_kernel<C, kThreads>, kMostRoom * 4, configured)) return FTB_ERR_LAUNCH;
   return launch_clusters(paged_choose_kernel<C, kThreads>, C, dim3(static_cast<unsigned>(B) * a.kv_heads * C), kThreads, static_cast<size_t>(room) * 4,
                          stream, a, room);
 }
 int launch_choose(const Choose& a, int B, cudaStream_t stream) {
-  // Clusters where there are more keys than a few a thread and eight CTAs to a sequence and kv head are no more than the device has room for at a time.
-  const bool apart = (static_cast<long long>(a.batch.W) << a.batch.page_shift) > 4096 && static_cast<long long>(B) * a.kv_heads * 8 <= 2ll * current_sm_count();
-  return apart ? launch_choose<8, 1024>(a, B, stream) : launch_choose<1, 512>(a, B, stream);
+  // One CTA, 8 or 16 of a cluster for each sequence and kv head, as the table has room for keys; us with the moves of 1032 rows, of (heads)
+  // 4: 5000 keys 14.4 18.0 21.1, 8000 18.1 18.4 20.9, 30 000 38.5 18.2 21.4, 70 000 255 23.8 23.1, 200 001 728 34.4 28.6; 12: 200 001 keys 734 35.6
+  // 50.4; 18: 12 000 keys 28.0 29.4, 30 000 39.0 30.1; 32: 30 000 39.4 42.0, 44 000 51.7 47.4, 70 000 267 58.3.  (One CTA keeps up to kMostRoom keys.)
+  const long long longest = static_cast<long long>(a.batch.W) << a.batch.page_shift, heads = static_cast<long long>(B) * a.kv_heads, sms = current_sm_count();
+  if (longest > 65536 && heads * 24 <= sms) return launch_choose<16, 1024>(a, B, stream);
+  if ((longest > 8192 && heads * 8 <= sms) || (longest > kMostRoom && heads * 8 <= 2 * sms)) return launch_choose<8, 1024>(a, B, stream);
+  return launch_choose<1, 512>(a, B, stream);
 }
 
 template <int kRow, int kOfPart, int kChain, int C>

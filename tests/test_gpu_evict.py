@@ -298,6 +298,7 @@ def test_keep_without_a_place():
     (1, 128, 16, [5000, 1200, 1300], 1200, 100, True),
     (1, 128, 16, [9000], 2500, 500, False),
     (2, 64, 128, [40000], 700, 30, False),
+    (2, 64, 128, [70000], 700, 30, False),
 ])
 def test_evict(eight_bit, kv, d, page, lens, keep, recent, elsewhere):
     ops = _ops()
@@ -344,13 +345,13 @@ def test_evict_all_equal_and_too_long():
 
 
 @pytest.mark.parametrize("kind", ["powers of four", "halves of an octave", "last bits", "two values"])
-@pytest.mark.parametrize("sequences", [1, 40])
-def test_evict_by_digits(kind, sequences):
+@pytest.mark.parametrize("sequences,width", [(1, 0), (1, 600), (1, 4100), (40, 0), (16, 2900)])
+def test_evict_by_digits(kind, sequences, width):
     """Weights whose order is known after one digit of their bits, two or three, or only after the last."""
     ops = _ops()
     page, keep, recent, n = 16, 50, 6, 5000 if kind == "two values" else 240
     table, ln, _, pages = _batch([0] * sequences, [n] * sequences, page)
-    table = torch.nn.functional.pad(table, (0, max(0, 320 - table.shape[1])), value=-1)  # (as wide as for sequences that have clusters)
+    table = torch.nn.functional.pad(table, (0, max(0, width - table.shape[1])), value=-1)  # (as wide as for sequences of one CTA, or of a cluster of 8 or 16)
     cache = _full_cache(pages, 2, page, 64, BF16, 3)
     g = torch.Generator().manual_seed(7)
     i = torch.arange(pages * 2 * page, dtype=torch.int64)[torch.randperm(pages * 2 * page, generator=g)].view(pages, 2, page)
