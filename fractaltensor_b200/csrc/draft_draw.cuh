@@ -37,10 +37,10 @@ struct DrawRoom {  // in shared memory
 
 // The row: row.p(j) and row.q(j) load what row.weight(p, q, j) takes; a warp says row.look(j, n) before it weighs numbers of j .. j + n - 1;
 // row.all() stops leaving out what it leaves out, for the case that nothing else weighs anything.  C: CTAs of a cluster; kAhead: the next numbers are on their way while
-// some are weighed.  All threads; one thread of one of the CTAs writes the token; -> sum(w),
-// where it is 0 nothing is written.  A cluster meets once more before one of its CTAs leaves.
-template <int C, int kThreads, bool kAhead, typename Row>
-__device__ __forceinline__ double draw_token(Row& row, int V, double share, int rank, DrawRoom<C, kThreads>& room, long long* token) {
+// some are weighed.  All threads; *share is read when it is needed (a register pair less while the row is read); one thread of one of the CTAs says put(token); -> sum(w),
+// where it is 0 nothing is put.  A cluster meets once more before one of its CTAs leaves.
+template <int C, int kThreads, bool kAhead, typename Row, typename Put>
+__device__ __forceinline__ double draw_token(Row& row, int V, const float* share, int rank, DrawRoom<C, kThreads>& room, Put put) {
   constexpr int kWarps = kThreads / 32, kUnroll = 8;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // a warp's stretch of the row: whole groups of 32
@@ -98,7 +98,7 @@ __device__ __forceinline__ double draw_token(Row& row, int V, double share, int 
   }
   // The stretch in which the limit is passed: room.sums[] are this CTA's still.  (u of 1 or above, or sums that round down: the last
   // stretch that weighs anything.)
-  const double limit = share * total;
+  const double limit = static_cast<double>(*share) * total;
   // Which CTA has it follows from the CTAs' sums alone, the same in all of them.
   const bool passed = total > limit;
   bool past = false, own = C == 1;
@@ -189,7 +189,7 @@ __device__ __forceinline__ double draw_token(Row& row, int V, double share, int 
       found = room.found;
       if (room.heavy >= 0) heavy = room.heavy;
     }
-    if (threadIdx.x == 0) *token = found != INT_MAX ? found : heavy;
+    if (threadIdx.x == 0) put(found != INT_MAX ? found : heavy);
   }
   return total;
 }

@@ -8,7 +8,7 @@
 // Only one row of p (and of q) a sequence is read whole.  Sums are kept in 64 bits: the chosen index follows from a
 // comparison with a partial sum of up to V numbers, and in 32 bits the order of summation would decide it.
 //
-// Bound by the bytes of those rows: 100 sequences of 5 drafts over 130 001 words 30.3 us, 3.4 TB/s (one: 7.5 us, trips to memory one
+// Bound by the bytes of those rows: 100 sequences of 5 drafts over 130 001 words 29.9 us, 3.5 TB/s (one: 7.1 us, trips to memory one
 // behind the other: the drafts' probabilities, the row, the stretch).  A cluster of CTAs takes a sequence, every warp a stretch of the row: one pass for the
 // stretches' sums, which the CTAs hand each other through distributed shared memory, and a second look at the one stretch (a 64th of
 // the row or less) in which the limit is passed.  Every CTA finds n on its own, which saves a step of waiting.
@@ -49,9 +49,10 @@ struct DraftRow {
   }
 };
 
-// C: CTAs of a cluster, 1 or 8.
+// C: CTAs of a cluster, 1 or 8.  (512 threads and a cluster: for few sequences, a CTA an SM at most; the others have 40 registers, without spills.  With 28 and 16
+// bytes of them, as when draw_token took the random number and the token's place as values, a batch took 31.4 us and one 7.9.)
 template <int C, int kThreads>
-__global__ void __launch_bounds__(kThreads, 1536 / kThreads)
+__global__ void __launch_bounds__(kThreads, C == 8 && kThreads == 512 ? 1 : 1536 / kThreads)
 verify_drafts_kernel(Drafts a, long long* __restrict__ tokens, int* __restrict__ counts_out, int* __restrict__ status) {
   __shared__ DrawRoom<C, kThreads> room;
   __shared__ int s_n;
@@ -65,7 +66,6 @@ verify_drafts_kernel(Drafts a, long long* __restrict__ tokens, int* __restrict__
   const float* u = a.u + static_cast<long long>(b) * (K + 1);
   const float* p = a.p + b * a.p_seq;
   const float* q = a.q != nullptr ? a.q + b * a.q_seq : nullptr;
-  const double share = u[K];
   long long id = threadIdx.x < K ? x[threadIdx.x] : 0;  // (on its way beside the count)
   const int mine = a.counts != nullptr ? min(max(a.counts[b], 0), K) : K;
   for (int i = threadIdx.x; i < mine; i += kThreads) {
@@ -83,7 +83,7 @@ verify_drafts_kernel(Drafts a, long long* __restrict__ tokens, int* __restrict__
   const int n = min(s_n, mine);
   DraftRow row{p + n * a.p_row, q != nullptr && n < mine ? q + n * a.q_row : nullptr,
                q == nullptr && n < mine && x[n] >= 0 && x[n] < V ? static_cast<int>(x[n]) : -1};
-  const double total = draw_token<C, kThreads, false>(row, V, share, rank, room, tokens + static_cast<long long>(b) * (K + 1) + n);
+  const double total = draw_token<C, kThreads, false>(row, V, u + K, rank, room, [&](int token) { tokens[static_cast<long long>(b) * (K + 1) + n] = token; });
   if (rank == 0) {
     for (int i = threadIdx.x; i <= K; i += kThreads)
       if (i != n || !(total > 0.0)) tokens[static_cast<long long>(b) * (K + 1) + i] = i < n ? x[i] : -1;

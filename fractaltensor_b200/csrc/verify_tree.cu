@@ -158,7 +158,7 @@ verify_tree_kernel(const __grid_constant__ Tree a, long long* __restrict__ token
   find_path<kThreads>(t, N);
   const int n = t.length;
   TreeRow row{p + t.path[n - 1] * a.p_row, t.refused, t.n_refused, false};
-  const double total = draw_token<C, kThreads, true>(row, V, t.u[0], rank, room, tokens + seq + n - 1);
+  const double total = draw_token<C, kThreads, true>(row, V, &t.u[0], rank, room, [&](int token) { tokens[seq + n - 1] = token; });
   if (rank == 0) {
     for (int i = threadIdx.x; i < N; i += kThreads) {
       if (i != n - 1 || !(total > 0.0)) tokens[seq + i] = i < n - 1 ? t.token[t.path[i + 1]] : -1;
