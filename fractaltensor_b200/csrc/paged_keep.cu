@@ -276,7 +276,7 @@ __device__ __forceinline__ int page_there(const int* table, int W, int shift, lo
 __device__ __forceinline__ Rows rows_of(const Move& a, int h, int first, int k, int i, int from, int to) {
   const int shift = a.batch.page_shift, in_page = (1 << shift) - 1;
   const long long src = static_cast<long long>(first) + k, dst = static_cast<long long>(first) + i;
-  if (src == dst && a.into == a.batch.table) return {-1, -1};  // where it is
+  if (src == dst && a.into == a.batch.table) return {-1, -1};  // where it is, page or not
   if (k < 0 || first < 0 || from < 0 || from >= a.batch.pages || to < 0 || to >= a.batch.pages) {
     atomicCAS(a.status, 0, FTB_ERR_INDEX);
     return {-1, -1};

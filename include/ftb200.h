@@ -490,8 +490,9 @@ int ftb_verify_tree(const float* probs, long long p_seq, long long p_row, const 
  * (`kept_head` 0: the same for all heads); first: int32 [B] or NULL: 0.  table [B, W]: the pages that rows come from; into [B, into_W]: the
  * pages that they go to, none of which this call reads, or NULL (or table itself): the same pages, which belong to one sequence each.
  * Keys, values, exponents and, if not NULL, weights (fp32 [pages, kv_heads, page_size]) move together.  All other rows stay as they
- * were.  K up to 2^30.  A row whose page one of the tables does not have, or with a negative number in kept, is not moved and sets the
- * (sticky) status word to 22. */
+ * were.  K up to 2^30.  A row whose page one of the tables does not have, or with a negative number in kept or a negative place in front of it
+ * (first), is not moved and sets the (sticky) status word to 22; but a row that stays where it is (kept[i] = i in the same pages) is not looked
+ * at, so that sequences without pages may stand in a batch with a path of token 0 alone. */
 int ftb_paged_cache_keep(void* k_cache, void* v_cache, unsigned char* k_exp, unsigned char* v_exp, float* weights,
                          const int* kept, long long kept_seq, long long kept_head, const int* counts, const int* first,
                          const int* table, const int* into, int B, int W, int into_W, int K, int pages, int kv_heads,
