@@ -290,7 +290,7 @@ __device__ __forceinline__ Rows rows_of(const Move& a, int h, int first, int k, 
 // C: CTAs of a chain, a cluster, which take so many steps at once.
 template <int kRow, int kOfPart, int kChain, int C>
 __global__ void __launch_bounds__(kMoveThreads)
-paged_move_kernel(const __grid_constant__ Move a, int chains, bool in_place) {
+paged_move_kernel(const __grid_constant__ Move a, int chains) {
   constexpr int kTogether = kChain / kOfPart, kStep = kTogether * kMoveAtOnce, kBeside = (kStep + kChain - 1) / kChain;
   __shared__ Rows looked_up[kMoveThreads / kChain][2][kStep];
   const int rank = C > 1 ? static_cast<int>(cluster_ctarank()) : 0;
@@ -433,8 +433,7 @@ int launch_move(const Move& a, int B, cudaStream_t stream) {
   // into other pages: enough blocks for every SM's room for them twice, so that one's end lies under others' work
   const int steps = (a.most + kStep - 1) / kStep;
   const int z = a.into == a.batch.table ? 1 : std::min(steps, std::max(1, 16 * current_sm_count() / blocks));
-  return launch_clusters(paged_move_kernel<kRow, kOfPart, kChain, C>, C, dim3(blocks, 2 * kRow / kOfPart, z), kMoveThreads, 0, stream, a, chains,
-                         a.into == a.batch.table);
+  return launch_clusters(paged_move_kernel<kRow, kOfPart, kChain, C>, C, dim3(blocks, 2 * kRow / kOfPart, z), kMoveThreads, 0, stream, a, chains);
 }
 template <int kRow>
 int launch_move(const Move& a, int B, cudaStream_t stream) {
