@@ -24,10 +24,10 @@ int paged_tile_pieces();
 int paged_tile_launch(const PagedAttn& a, int d, int dtype, int rows, void* scratch, cudaStream_t stream);
 
 // Whether n numbers at o (16 bits) meet the numbers of some of T rows of heads at q.
-inline bool over_rows(const void* o, long long n, const void* q, int T, long long q_row, int heads, long long q_head, int d) {
+inline bool over_rows(const void* o, long long n, const void* q, int T, long long q_row, int heads, long long q_head, long long d) {
   const long long span = (heads - 1) * q_head, lo = std::min(0ll, span), hi = std::max(0ll, span) + d;  // of a row
   const long long step = T > 1 ? std::abs(q_row) : 0, first = T > 1 && q_row < 0 ? (T - 1) * q_row : 0;
-  // o's beginning, in numbers from where the lowest row is (both on 16-byte boundaries)
+  // o's beginning, in numbers from where the lowest row is (both on 2-byte boundaries)
   const long long at = static_cast<long long>(reinterpret_cast<uintptr_t>(o) - reinterpret_cast<uintptr_t>(q)) / 2 - first;
   if (step == 0) return at < hi && at + n > lo;
   // rows r with r * step + hi > at and r * step + lo < at + n

@@ -16,6 +16,7 @@
 
 #include "../../include/ftb200.h"
 #include "draft_draw.cuh"
+#include "paged_forms.h"
 #include "tmap.h"
 
 namespace ftb {
@@ -229,6 +230,7 @@ extern "C" int ftb_verify_tree(const float* probs, long long p_seq, long long p_
   for (int o = 0; o < 3; ++o) {
     for (int i = 0; i < 3; ++i)
       if (overlap(out[o], out_bytes[o], in[i], in_bytes[i])) return FTB_ERR_ARG;
+    if (over_rows(out[o], static_cast<long long>(out_bytes[o] / 2), probs, B, 2 * p_seq, N, 2 * p_row, 2ll * V)) return FTB_ERR_ARG;
     for (int i = 0; i < o; ++i)
       if (overlap(out[o], out_bytes[o], out[i], out_bytes[i])) return FTB_ERR_ARG;
   }

@@ -479,7 +479,7 @@ int ftb_verify_drafts(const float* probs, long long p_seq, long long p_row, cons
  * int32 [B, N], the tokens of the path from 0 on, then -1; counts_out int32 [B], how many; tokens_out int64 [B, N]: the path's tokens
  * behind token 0, the drawn one, then -1.  Sums in 64 bits.  Probabilities that are not positive and finite count as 0; a row without
  * any gives -1 and, as a drafted token outside [0, V), which is not taken, sets the (sticky) status word to 22.  No two results, and no
- * result and tokens, parents or u, overlap. */
+ * result and probs (a sequence's first to last row), tokens, parents or u, overlap. */
 int ftb_tree_mask(const int* parents, int* mask, int B, int N, void* stream);
 int ftb_verify_tree(const float* probs, long long p_seq, long long p_row, const long long* tokens, const int* parents,
                     const float* u, long long* tokens_out, int* path, int* counts_out, int B, int N, int V, void* workspace,
