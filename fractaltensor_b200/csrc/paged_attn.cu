@@ -371,6 +371,7 @@ extern "C" int ftb_paged_attn_tree_fwd(const void* q, long long q_row, long long
       overlap(o, o_bytes, v_cache, cache_bytes) || overlap(o, o_bytes, k_exp, exp_bytes) || overlap(o, o_bytes, v_exp, exp_bytes))
     return FTB_ERR_ARG;
   const size_t tree_bytes = tree != nullptr ? static_cast<size_t>(T) * tree_words * sizeof(int) : 0;
+  if ((reinterpret_cast<uintptr_t>(tree) & 3) != 0) return FTB_ERR_ALIGN;
   if (overlap(o, o_bytes, tree, tree_bytes)) return FTB_ERR_ARG;
   if (lse != nullptr) {
     const size_t lse_bytes = static_cast<size_t>(T) * heads * sizeof(float);

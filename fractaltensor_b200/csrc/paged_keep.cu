@@ -478,6 +478,7 @@ extern "C" int ftb_paged_cache_keep(void* k_cache, void* v_cache, unsigned char*
   int rc = check_cache(k_cache, v_cache, k_exp, v_exp, table, into, B, W, into_W, pages, kv_heads, page_size, d);
   if (rc) return rc;
   if (K < 0 || K > kMostKept || (K > 0 && !kept) || !counts) return FTB_ERR_ARG;
+  if ((reinterpret_cast<uintptr_t>(weights) & 3) != 0) return FTB_ERR_ALIGN;
   if (workspace == nullptr || workspace_bytes < ftb_workspace_bytes()) return FTB_ERR_WORKSPACE;
   if (K == 0) return FTB_OK;
   if ((rc = check_device_sm100())) return rc;

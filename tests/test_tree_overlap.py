@@ -1,7 +1,7 @@
 """What the calls on trees of drafts and on a cache's rows refuse by address, before they touch a device."""
 import ctypes
 
-from test_tree_refusals import _verify, lib  # noqa: F401
+from test_tree_refusals import _attn, _keep, _verify, lib  # noqa: F401
 
 
 def test_verification_over_its_probabilities(lib):
@@ -21,3 +21,9 @@ def test_verification_over_its_probabilities(lib):
     assert call("counts", P + 4 * (row + V)) != 1 and call("counts", P + 4 * V) == 1
     # the longest rows
     assert _verify(lib, p=ctypes.c_void_p(1 << 44), V=1 << 30, ps=2 << 30, pr=1 << 30, counts=ctypes.c_void_p((1 << 44) + (8 << 30) - 8)) == 1
+
+
+def test_words_that_begin_anywhere(lib):
+    """Masks and weights are read four bytes at a time."""
+    odd = ctypes.c_void_p((13 << 20) + 2)
+    assert _attn(lib, tree=odd) == 2 and _keep(lib, weights=odd) == 2
