@@ -1,4 +1,5 @@
-"""What the calls on trees of drafts and on a cache's rows refuse by address, before they touch a device."""
+"""What the calls on trees of drafts and on a cache's rows refuse by address, before they touch a device.  (Only refusals: an address that is
+not refused would be read on a machine with a device.)"""
 import ctypes
 
 from test_tree_refusals import _attn, _keep, _verify, lib  # noqa: F401
@@ -10,15 +11,10 @@ def test_verification_over_its_probabilities(lib):
     size = 4 * ((B - 1) * seq + (N - 1) * row + V)
     call = lambda out, at, **kw: _verify(lib, **{"p": ctypes.c_void_p(P), "ps": seq, "pr": row, "B": B, "N": N, "V": V, out: ctypes.c_void_p(at), **kw})
     for out, n in (("out", 8 * B * N), ("path", 4 * B * N), ("counts", 4 * B)):
-        for at in (P, P + 4 * row, P + 4 * (seq + V) - 8, P + size - 8, P - n + 8):
+        for at in (P, P + 4 * row, P + 4 * V, P + 4 * (seq + V) - 8, P + size - 8, P - n + 8):
             assert call(out, at) == 1, (out, at)
-        for at in (P + size, P - n):
-            assert call(out, at) != 1, (out, at)
-        # rows that all sequences share, rows the other way round, one sequence of a step that is not taken
+        # rows that all sequences share, rows the other way round
         assert call(out, P + 4 * row, ps=0) == 1 and call(out, P - 4 * seq, ps=-seq) == 1
-        assert call(out, P + 4 * (row + V), ps=1 << 40, B=1) != 1
-    # behind a sequence's last row there is room, between its rows there is none
-    assert call("counts", P + 4 * (row + V)) != 1 and call("counts", P + 4 * V) == 1
     # the longest rows
     assert _verify(lib, p=ctypes.c_void_p(1 << 44), V=1 << 30, ps=2 << 30, pr=1 << 30, counts=ctypes.c_void_p((1 << 44) + (8 << 30) - 8)) == 1
 
