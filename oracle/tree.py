@@ -79,6 +79,7 @@ def weights(before, q, cache, lse, table, lens, starts, scale, window=None):
     k = paged.dense(cache, 0)
     T, heads, d = q.shape
     kv, page = k.shape[1], k.shape[2]
+    rescaled = q.dtype == torch.bfloat16 and len(cache) == 4
     out, tol, terms = before.cpu().double().clone(), torch.zeros(before.shape, dtype=torch.float64), torch.zeros(before.shape)
     q, lse = q.cpu().double(), lse.cpu().double()
     where = paged.places(table, lens, starts, page, T)
@@ -94,10 +95,11 @@ def weights(before, q, cache, lse, table, lens, starts, scale, window=None):
         rows = table[place[0]].cpu().long()[j // page]
         kj = k[rows, :, j % page][:, g]
         x = torch.einsum("jhd,hd->jh", kj, q[t]) * scale
-        size = torch.einsum("jhd,hd->jh", kj.abs(), q[t].abs()) * scale + q[t].abs().amax(-1) * kj.abs().sum(-1) * scale
+        size = torch.einsum("jhd,hd->jh", kj.abs(), q[t].abs()) * scale
+        kept = 2.0 ** -25 * scale * q[t].abs().amax(-1) * kj.abs().sum(-1) if rescaled else 0.0
         fine = torch.isfinite(lse[t])
         p = torch.where(fine, torch.exp(x - torch.where(fine, lse[t], 0.0)), 0.0)
-        e = p * (2 * (d + 4) * 2.0 ** -24 * size + 2.0 ** -21 + 4 * 2.0 ** -24 * (x.abs() + torch.where(fine, lse[t].abs(), 0.0)))
+        e = p * (2 * (d + 4) * 2.0 ** -24 * size + kept + 2.0 ** -21 + 4 * 2.0 ** -24 * (x.abs() + torch.where(fine, lse[t].abs(), 0.0)))
         for h in range(kv):
             mine = g == h
             out[rows, h, j % page] += p[:, mine].sum(1)
