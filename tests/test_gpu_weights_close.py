@@ -51,8 +51,10 @@ def _close(before, q, cache, lse, table, ln, st, scale):
     return out, tol + (terms + 1) * 2.0 ** -24 * out.abs() + 2.0 ** -24 * old
 
 
-def _weigh(kv, group, d, page, new, lens, dtype, eight_bit, width=0):
+def _weigh(kv, group, d, page, new, lens, dtype, eight_bit, launches, width=0):
+    """launches: 1: the kernel for few rows; 3: packing, the one for many and the join; 4: both."""
     ops = _ops()
+    from fractaltensor_b200._lib import lib
     table, ln, st, pages = _batch(new, lens, page, width=width)
     cache = _full_cache(pages, kv, page, d, E4M3 if eight_bit else dtype, 3)
     T = int(st[-1])
@@ -63,7 +65,9 @@ def _weigh(kv, group, d, page, new, lens, dtype, eight_bit, width=0):
     before = weights.clone()
     args = (table.cuda(), ln.cuda(), st.cuda())
     ops.paged_attention(q, cache, *args, scale=scale, lse=lse)
+    n = lib.ftb_launch_count()
     ops.paged_attention_weights(q, cache, weights, lse, *args, scale=scale)
+    assert lib.ftb_launch_count() - n == launches
     ops.check_status()
     want, tol = _close(before, q, cache, lse, table, ln, st, scale)
     err = (weights.double().cpu() - want).abs()
@@ -76,30 +80,31 @@ def _weigh(kv, group, d, page, new, lens, dtype, eight_bit, width=0):
 
 @pytest.mark.parametrize("eight_bit", [False, True])
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("kv,group,d,page,new,lens", [
-    (2, 4, 128, 16, [1, 1], [900, 333]),       # tiles of 8 rows, a token each
-    (2, 16, 128, 16, [1], [900]),              # tiles of 16
-    (1, 4, 64, 32, [7], [500]),                # two of them
-    (2, 4, 128, 16, [25], [700]),              # 128 rows on the tensor cores
-    (1, 3, 64, 64, [30, 23], [600, 257]),
+@pytest.mark.parametrize("kv,group,d,page,new,lens,launches", [
+    (2, 4, 128, 16, [1, 1], [900, 333], 1),    # tiles of 8 rows, a token each
+    (2, 16, 128, 16, [1], [900], 1),           # tiles of 16
+    (1, 4, 64, 32, [7], [500], 1),             # two of them
+    (2, 4, 128, 16, [25], [700], 3),           # 128 rows on the tensor cores
+    (1, 3, 64, 64, [30, 23], [600, 257], 4),
 ])
-def test_close(dtype, eight_bit, kv, group, d, page, new, lens):
-    _weigh(kv, group, d, page, new, lens, dtype, eight_bit)
+def test_close(dtype, eight_bit, kv, group, d, page, new, lens, launches):
+    _weigh(kv, group, d, page, new, lens, dtype, eight_bit, launches)
 
 
 @pytest.mark.parametrize("eight_bit", [False, True])
-@pytest.mark.parametrize("group,d,page,new,lens", [
-    (4, 128, 64, [1], [40_003]),               # a token
-    (4, 64, 16, [6], [20_011]),                # two tiles of 16 rows
-    (2, 64, 128, [35], [20_011]),              # many rows behind many blocks that all of them see
-    (2, 64, 32, [35, 1, 9], [9001, 15_000, 44]),
+@pytest.mark.parametrize("group,d,page,new,lens,launches", [
+    (4, 128, 64, [1], [40_003], 1),            # a token
+    (4, 64, 16, [6], [20_011], 1),             # two tiles of 16 rows
+    (2, 64, 128, [35], [20_011], 3),           # many rows behind many blocks that all of them see
+    (2, 64, 32, [35, 1, 9], [9001, 15_000, 44], 1),
+    (2, 64, 32, [65, 1, 9], [9001, 15_000, 44], 4),
 ])
-def test_long_sequences(eight_bit, group, d, page, new, lens):
-    _weigh(1, group, d, page, new, lens, BF16, eight_bit)
+def test_long_sequences(eight_bit, group, d, page, new, lens, launches):
+    _weigh(1, group, d, page, new, lens, BF16, eight_bit, launches)
 
 
 @pytest.mark.parametrize("eight_bit", [False, True])
-@pytest.mark.parametrize("new,lens", [([5, 9], [300, 77]), ([12], [301]), ([1, 1, 1], [300, 20, 1])])
-def test_tables_wider_than_the_sequences(eight_bit, new, lens):
+@pytest.mark.parametrize("new,lens,launches", [([5, 9], [300, 77], 4), ([12], [301], 3), ([1, 1, 1], [300, 20, 1], 1)])
+def test_tables_wider_than_the_sequences(eight_bit, new, lens, launches):
     """Rows of a table for sequences of 128 000 keys: a few dozen rows go to the tensor cores."""
-    _weigh(2, 4, 128, 128, new, lens, F16, eight_bit, width=1000)
+    _weigh(2, 4, 128, 128, new, lens, F16, eight_bit, launches, width=1000)
