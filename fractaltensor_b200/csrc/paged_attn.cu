@@ -36,7 +36,7 @@ struct Pieces {
 // Rows of whole tiles that have to be computed again: none, unless something in the cache is not finite, or dwarfs what is seen of its
 // 8-bit block.  `warp` of `warps` in the grid.  Those of a tile lie side by side: a warp looks at four times eight (a sector of flags) far
 // from each other.
-template <typename T, bool k8, int D, bool kMore>
+template <typename T, bool k8, int D, int kWhat>
 __device__ __forceinline__ void again_rows(const PagedAttn& a, long long warp, long long warps, int lane) {
   const int heads = a.kv_heads * a.group;
   const long long rows = static_cast<long long>(a.T) * heads;
@@ -50,13 +50,13 @@ __device__ __forceinline__ void again_rows(const PagedAttn& a, long long warp, l
       const int t = static_cast<int>(row / heads);
       const RowPlace at = place_of_row(a.batch, t, lane);
       if (at.b < a.batch.B)  // (what no sequence has was not written either)
-        attend_row<T, k8, D, kMore>(a, at.b, t, static_cast<int>(row - static_cast<long long>(t) * heads), at.pos, lane);
+        attend_row<T, k8, D, kWhat>(a, at.b, t, static_cast<int>(row - static_cast<long long>(t) * heads), at.pos, lane);
     }
   }
 }
 
 // Row r of a cut tile by one warp, its numbers x over the weights' sum l (of 2^(score - m)), to the output.
-template <typename T, bool k8, int D, bool kMore>
+template <typename T, bool k8, int D, int kWhat>
 __device__ __forceinline__ void finish_row(const PagedAttn& a, const PagedCut& c, int r, float m, float l, float (&x)[D / 32], int lane) {
   const int heads = a.kv_heads * a.group;
   const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -70,9 +70,9 @@ __device__ __forceinline__ void finish_row(const PagedAttn& a, const PagedCut& c
   uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(a.o) + (static_cast<long long>(t) * heads + head) * D) + lane * (D / 64);
 #pragma unroll
   for (int e = 0; e < D / 64; ++e) out[e] = Fmt<T>::pack2(x[2 * e], x[2 * e + 1]);
-  if (kMore && a.lse != nullptr && lane == 0) put_lse(a, static_cast<long long>(t) * heads + head, m, l);
+  if (wants_lse<kWhat>(a) && lane == 0) put_lse(a, static_cast<long long>(t) * heads + head, m, l);
   // (rows that something unseen may have made a NaN: key by key)
-  if (__any_sync(0xffffffffu, all != all) && hides<kMore>(a, c.pos0 + t, c.lo, c.hi)) attend_row<T, k8, D, kMore>(a, c.b, t, head, c.pos0 + t, lane);
+  if (__any_sync(0xffffffffu, all != all) && hides<kWhat>(a, c.pos0 + t, c.lo, c.hi)) attend_row<T, k8, D, kWhat>(a, c.b, t, head, c.pos0 + t, lane);
 }
 
 // Parts first, first + by, .. of n of a row, added up: (m, l, x).
@@ -117,7 +117,7 @@ __device__ __forceinline__ void add_parts(Part part, int R, int r, int first, in
 // What the kernel for few rows leaves alone: block (x, y) takes row y of the tile with cut x, the parts spread over its warps: such
 // tiles may have hundreds, and what they cost are trips to memory one behind the other.
 constexpr int kFewWarps = 4;
-template <typename T, bool k8, int D, bool kMore>
+template <typename T, bool k8, int D, int kWhat>
 __global__ void __launch_bounds__(kFewWarps * 32)
 paged_join_few_kernel(const __grid_constant__ PagedAttn a, Pieces few) {
   __shared__ float s_sum[kFewWarps][D];
@@ -126,7 +126,7 @@ paged_join_few_kernel(const __grid_constant__ PagedAttn a, Pieces few) {
   grid_dependency_wait();
   grid_launch_dependents();
   const int last = few.cuts[cut].last;
-  again_rows<T, k8, D, kMore>(a, (static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x) * kFewWarps + warp,
+  again_rows<T, k8, D, kWhat>(a, (static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x) * kFewWarps + warp,
                        static_cast<long long>(gridDim.x) * gridDim.y * kFewWarps, lane);
   if (last < 0) return;
   const PagedCut c = few.cuts[cut];
@@ -157,12 +157,12 @@ paged_join_few_kernel(const __grid_constant__ PagedAttn a, Pieces few) {
 #pragma unroll
     for (int e = 0; e < D / 32; ++e) x[e] = fmaf(s_sum[w][lane * (D / 32) + e], k, x[e]);
   }
-  finish_row<T, k8, D, kMore>(a, c, r, top, l, x, lane);
+  finish_row<T, k8, D, kWhat>(a, c, r, top, l, x, lane);
 }
 
 // What both kernels leave.  Every block finds the cuts that have something to join, and the warps take the rows of those tiles in turn,
 // kJoinRows at a time, all on their way at once where there are two parts, as of most tiles of many rows.
-template <typename T, bool k8, int D, bool kMore>
+template <typename T, bool k8, int D, int kWhat>
 __global__ void __launch_bounds__(kJoinThreads, 3)
 paged_join_kernel(const __grid_constant__ PagedAttn a, Pieces few, Pieces many) {
   constexpr int kPer = D / 32;  // numbers of a row a lane
@@ -171,7 +171,7 @@ paged_join_kernel(const __grid_constant__ PagedAttn a, Pieces few, Pieces many) 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_dependency_wait();
   grid_launch_dependents();
-  again_rows<T, k8, D, kMore>(a, static_cast<long long>(blockIdx.x) * kJoinWarps + warp, static_cast<long long>(gridDim.x) * kJoinWarps, lane);
+  again_rows<T, k8, D, kWhat>(a, static_cast<long long>(blockIdx.x) * kJoinWarps + warp, static_cast<long long>(gridDim.x) * kJoinWarps, lane);
   // turns of every cut, and how many lie in front of it
   const int cuts = few.pieces + many.pieces;
   {
@@ -237,35 +237,37 @@ paged_join_kernel(const __grid_constant__ PagedAttn a, Pieces few, Pieces many) 
         float x[kPer];
 #pragma unroll
         for (int e = 0; e < kPer; ++e) x[e] = reinterpret_cast<const float*>(&v[k][0])[e] * w0 + reinterpret_cast<const float*>(&v[k][1])[e] * w1;
-        finish_row<T, k8, D, kMore>(a, c, r0 + k, top, ml[k][0].y * w0 + ml[k][1].y * w1, x, lane);
+        finish_row<T, k8, D, kWhat>(a, c, r0 + k, top, ml[k][0].y * w0 + ml[k][1].y * w1, x, lane);
       }
       continue;
     }
     for (int r = r0; r < min(r0 + kJoinRows, c.rows); ++r) {
       float m, l, x[kPer];
       add_parts<D>(part, R, r, 0, 1, n, lane, m, l, x);
-      finish_row<T, k8, D, kMore>(a, c, r, m, l, x, lane);
+      finish_row<T, k8, D, kWhat>(a, c, r, m, l, x, lane);
     }
   }
 }
 
-template <typename T, bool k8, int D, bool kMore>
+template <typename T, bool k8, int D, int kWhat>
 int launch_join(const PagedAttn& a, const Pieces& few, const Pieces& many, cudaStream_t stream) {
   if (few.pieces + many.pieces > kMostCuts) return FTB_ERR_ARG;  // (a device of 256 SMs)
   static std::atomic<unsigned long long> divided{0}, divided_few{0};
-  if (!set_smem_carveout(paged_join_kernel<T, k8, D, kMore>, kPagedCarveout, divided) ||
-      !set_smem_carveout(paged_join_few_kernel<T, k8, D, kMore>, kPagedCarveout, divided_few))
+  if (!set_smem_carveout(paged_join_kernel<T, k8, D, kWhat>, kPagedCarveout, divided) ||
+      !set_smem_carveout(paged_join_few_kernel<T, k8, D, kWhat>, kPagedCarveout, divided_few))
     return FTB_ERR_LAUNCH;
   const cudaError_t err =
-      many.pieces == 0 ? launch_dependent(paged_join_few_kernel<T, k8, D, kMore>, dim3(few.pieces, few.rows), dim3(kFewWarps * 32), 0, stream, a, few)
-                       : launch_dependent(paged_join_kernel<T, k8, D, kMore>, dim3(3 * current_sm_count()), dim3(kJoinThreads), 0, stream, a, few, many);
+      many.pieces == 0 ? launch_dependent(paged_join_few_kernel<T, k8, D, kWhat>, dim3(few.pieces, few.rows), dim3(kFewWarps * 32), 0, stream, a, few)
+                       : launch_dependent(paged_join_kernel<T, k8, D, kWhat>, dim3(3 * current_sm_count()), dim3(kJoinThreads), 0, stream, a, few, many);
   count_launch();
   if (err != cudaSuccess) cudaGetLastError();
   return err == cudaSuccess ? FTB_OK : FTB_ERR_LAUNCH;
 }
 template <typename T, bool k8, int D>
 int launch_join(const PagedAttn& a, const Pieces& few, const Pieces& many, cudaStream_t stream) {
-  return a.more() ? launch_join<T, k8, D, true>(a, few, many, stream) : launch_join<T, k8, D, false>(a, few, many, stream);
+  return a.tree != nullptr  ? launch_join<T, k8, D, kTrees>(a, few, many, stream)
+         : a.lse != nullptr ? launch_join<T, k8, D, kLse>(a, few, many, stream)
+                            : launch_join<T, k8, D, kPlain>(a, few, many, stream);
 }
 template <typename T>
 int launch_join(const PagedAttn& a, int d, const Pieces& few, const Pieces& many, cudaStream_t stream) {

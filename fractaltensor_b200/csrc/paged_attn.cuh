@@ -21,12 +21,16 @@ struct PagedAttn {
   const uint32_t* tree;            // [T, tree_words] or nullptr: bit j of a row's words: it sees new token j of its sequence
   int tree_words;
   float* lse;                      // [T, heads] or nullptr: log(sum(exp(scale * q . k))) of a row
-
-  bool more() const { return tree != nullptr || lse != nullptr; }
 };
 
-// kMore: kernels for calls with a tree or lse.  The others are compiled without (with both decided when they run, chunks took 586 us for
-// 558, 8-bit drafts 698 for 663, a decoding step 185.5 for 182.6: registers).
+// What a call wants besides the results: kernels are compiled apart for calls with a tree (with or without lse), for calls with lse alone and for the
+// others.  us, of the others, with lse alone, and with lse where that and the tree are both decided when the kernel runs (registers, and the room for a
+// mask's bits): decoding step 180.0, 180.8, 183.1; chunk 551, 565, 588; 8-bit drafts 647, 661, 692; 8-bit prompts with a window 77.6, 80.0, 90.2.
+constexpr int kPlain = 0, kLse = 1, kTrees = 2;
+template <int kWhat>
+__device__ __forceinline__ bool wants_lse(const PagedAttn& a) {
+  return kWhat == kLse || (kWhat == kTrees && a.lse != nullptr);
+}
 
 // Word i of row t's bits.  What the mask has no word for, and what lies in front of the new tokens, is seen as far as positions go.
 __device__ __forceinline__ uint32_t tree_word(const PagedAttn& a, int t, long long i) {
@@ -50,9 +54,9 @@ constexpr float kNearTops = 40.f;
 
 // Whether a row at position pos of a tile that multiplies keys lo .. hi - 1 has some of them with weight 0 that it does not see: what
 // they hold could have made its result a NaN.
-template <bool kMore>
+template <int kWhat>
 __device__ __forceinline__ bool hides(const PagedAttn& a, long long pos, int lo, int hi) {
-  return pos + 1 < hi || (a.window > 0 && pos + 1 - a.window > lo) || (kMore && a.tree != nullptr);
+  return pos + 1 < hi || (a.window > 0 && pos + 1 - a.window > lo) || kWhat == kTrees;
 }
 
 // The output of one (token, head) by one warp, key by key: nothing of a key that the token does not see has a part
@@ -60,7 +64,7 @@ __device__ __forceinline__ bool hides(const PagedAttn& a, long long pos, int lo,
 // keys at a time, which are of one page and on their way together.  For rows that the kernels' products have made a NaN through such keys.
 // It is for what should not happen: a row of 65 536 keys takes 9 ms (36 with a trip to memory for every key).  2048 tokens of 32 heads behind
 // 14 336 keys, 0.5 ms, take 36 ms with a NaN at the last position, which the last 64 tokens do not see, and 86 with one in their middle.
-template <typename T, bool k8, int D, bool kMore>
+template <typename T, bool k8, int D, int kWhat>
 __device__ __noinline__ void attend_row(const PagedAttn& a, int b, int t, int head, long long pos, int lane) {
   constexpr int kPer = D / 32, kBatch = 8;
   const int h = head / a.group;
@@ -93,8 +97,8 @@ __device__ __noinline__ void attend_row(const PagedAttn& a, int b, int t, int he
   };
   const long long end = min(pos + 1, static_cast<long long>(a.batch.W) << a.batch.page_shift);
   const long long begin = a.window > 0 ? max(0ll, pos + 1 - a.window) : 0;
-  const long long base = kMore && a.tree != nullptr ? pos - (t - max(0, a.batch.starts[b])) : end;  // of the sequence's new tokens
-  auto sees = [&](long long j) { return j >= begin && j < end && (!kMore || j < base || in_tree(a, t, j - base)); };
+  const long long base = kWhat == kTrees ? pos - (t - max(0, a.batch.starts[b])) : end;  // of the sequence's new tokens
+  auto sees = [&](long long j) { return j >= begin && j < end && (kWhat != kTrees || j < base || in_tree(a, t, j - base)); };
   float m = -FLT_MAX, l = 0.f;
   for (long long j0 = begin / kBatch * kBatch; j0 < end; j0 += kBatch) {
     const int page = max(0, page_of(a.batch, b, j0, a.status));
@@ -139,7 +143,7 @@ __device__ __noinline__ void attend_row(const PagedAttn& a, int b, int t, int he
   uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(a.o) + (static_cast<long long>(t) * a.kv_heads * a.group + head) * D) + lane * (kPer / 2);
 #pragma unroll
   for (int c = 0; c < kPer / 2; ++c) out[c] = Fmt<T>::pack2(acc[2 * c] * inv, acc[2 * c + 1] * inv);
-  if (kMore && a.lse != nullptr && lane == 0) put_lse(a, static_cast<long long>(t) * a.kv_heads * a.group + head, m, l);
+  if (wants_lse<kWhat>(a) && lane == 0) put_lse(a, static_cast<long long>(t) * a.kv_heads * a.group + head, m, l);
 }
 
 }  // namespace ftb

@@ -53,7 +53,7 @@ struct Merge {
 // tiles of two groups of warps that share the keys through L1, were slower than the tiles of paged_tile.cu by 2 to 4 times.)
 constexpr int blocks_per_sm(int nt) { return nt == 1 ? 3 : 2; }
 
-template <typename T, bool k8, int D, int NT, bool kMore>
+template <typename T, bool k8, int D, int NT, int kWhat>
 __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm(NT))
 paged_short_kernel(const __grid_constant__ PagedAttn a, float* __restrict__ parts, PagedCut* __restrict__ cuts) {
   using C = typename std::conditional<k8, __half, T>::type;
@@ -68,11 +68,11 @@ paged_short_kernel(const __grid_constant__ PagedAttn a, float* __restrict__ part
   const int piece = blockIdx.x;
   grid_dependency_wait();
   grid_launch_dependents();
-  PagedWalk<R, kUnitKeys, kMore> walk;
+  PagedWalk<R, kUnitKeys, kWhat> walk;
   {
     int b;
     long long at;
-    const PagedLine line = paged_line<R, kUnitKeys, kMore>(a, piece, gridDim.x, kAtLeast, s_line, &b, &at);
+    const PagedLine line = paged_line<R, kUnitKeys, kWhat>(a, piece, gridDim.x, kAtLeast, s_line, &b, &at);
     if (piece >= line.pieces || line.total == 0) {
       if (threadIdx.x == 0) cuts[piece].last = -1;
       return;
@@ -113,7 +113,7 @@ paged_short_kernel(const __grid_constant__ PagedAttn a, float* __restrict__ part
     int all_lo = 0, all_hi = static_cast<int>(max(-1ll, min(first_pos, static_cast<long long>(hi) - 1)));
     if (a.window > 0) all_lo = static_cast<int>(max(0ll, min(last_pos - a.window + 1, static_cast<long long>(INT_MAX))));
     const long long base = s.pos0 + s.first;  // of the sequence's new tokens
-    if (kMore && a.tree != nullptr) all_hi = static_cast<int>(max(-1ll, min(base - 1, static_cast<long long>(all_hi))));
+    if (kWhat == kTrees) all_hi = static_cast<int>(max(-1ll, min(base - 1, static_cast<long long>(all_hi))));
 
     float oacc[kSteps][NT][4], m[NT][2], l[NT][2];
     float near = kNear;  // 8 bits: l takes a chunk's weights where the values' exponents are below
@@ -250,7 +250,7 @@ paged_short_kernel(const __grid_constant__ PagedAttn a, float* __restrict__ part
             const int key = key0 + g + (i >> 1) * 8;
             if (key > see_hi[nt][i & 1] || key < see_lo[nt][i & 1]) sc[nt][i] = -INFINITY;
           }
-        if (kMore && a.tree != nullptr) {
+        if (kWhat == kTrees) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -443,7 +443,7 @@ paged_short_kernel(const __grid_constant__ PagedAttn a, float* __restrict__ part
         const int flat = flat0 + r, t = s.first + flat / a.group, head = h * a.group + flat % a.group;
         *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + (static_cast<long long>(t) * a.kv_heads * a.group + head) * D + d) =
             make_uint2(Fmt<T>::pack2(x.x, x.y), Fmt<T>::pack2(x.z, x.w));
-        if (kMore && a.lse != nullptr && d == 0) put_lse(a, static_cast<long long>(t) * a.kv_heads * a.group + head, top_n, sum);
+        if (wants_lse<kWhat>(a) && d == 0) put_lse(a, static_cast<long long>(t) * a.kv_heads * a.group + head, top_n, sum);
       } else {
         *reinterpret_cast<float4*>(part + r * D + d) = x;
         if (d == 0) {
@@ -457,15 +457,15 @@ paged_short_kernel(const __grid_constant__ PagedAttn a, float* __restrict__ part
     if (threadIdx.x < rows) {
       const int flat = flat0 + threadIdx.x, t = s.first + flat / a.group;
       a.odd[static_cast<long long>(t) * a.kv_heads * a.group + h * a.group + flat % a.group] =
-          s_odd[threadIdx.x] != 0 && hides<kMore>(a, s.pos0 + t, lo, hi) ? 1u : 0u;
+          s_odd[threadIdx.x] != 0 && hides<kWhat>(a, s.pos0 + t, lo, hi) ? 1u : 0u;
     }
   }
 }
 
-template <typename T, bool k8, int D, int NT, bool kMore>
+template <typename T, bool k8, int D, int NT, int kWhat>
 int launch(const PagedAttn& a, void* scratch, cudaStream_t stream) {
   static std::atomic<unsigned long long> configured{0};
-  auto kfn = paged_short_kernel<T, k8, D, NT, kMore>;
+  auto kfn = paged_short_kernel<T, k8, D, NT, kWhat>;
   constexpr int kSmem = sizeof(Merge<D, NT>);
   if (!ensure_dynamic_smem(kfn, kSmem, configured)) return FTB_ERR_LAUNCH;
   // No more shared memory than the blocks need: what is on its way to registers passes L1, which has the rest.  (Left to itself
@@ -483,7 +483,9 @@ int launch(const PagedAttn& a, void* scratch, cudaStream_t stream) {
 }
 template <typename T, bool k8, int D, int NT>
 int launch(const PagedAttn& a, void* scratch, cudaStream_t stream) {
-  return a.more() ? launch<T, k8, D, NT, true>(a, scratch, stream) : launch<T, k8, D, NT, false>(a, scratch, stream);
+  return a.tree != nullptr  ? launch<T, k8, D, NT, kTrees>(a, scratch, stream)
+         : a.lse != nullptr ? launch<T, k8, D, NT, kLse>(a, scratch, stream)
+                            : launch<T, k8, D, NT, kPlain>(a, scratch, stream);
 }
 template <typename T, int D, int NT>
 int launch(const PagedAttn& a, void* scratch, cudaStream_t stream) {

@@ -5,7 +5,7 @@
 // 2048 tokens behind 14 336 keys, 32 heads of 128 over 8 kv heads, bf16: 558 us, 0.92 PFLOP/s; bound by the chain of a row's scores, 4300
 // cycles a block of 256 rows beside 2048 of products, and by the joins (25 us).  96 sequences of 8500 keys on average in 8 bits, 5 tokens
 // of 64 heads: 660 us, 0.2 PFLOP/s and 2.5 TB/s (847 where values are of 2^-40, with the sum apart for every block); bound by the instructions that make 8-bit keys operands (1.6 to 1.9 a cycle and SM).
-// Trees of drafts (kMore): a row's bits of the block's keys are laid out in shared memory when a block reaches into the new tokens, and taken with
+// Trees of drafts (kTrees): a row's bits of the block's keys are laid out in shared memory when a block reaches into the new tokens, and taken with
 // every look at the scores.  32 sequences of 33 tokens of 64 heads, up to 16 000 keys of 8 bits: 587 us for 256 of their 264 rows.
 // Measured and not kept, the chunk: all 128 scores of a row in registers 616 us (spills; L1 is shared memory's), 32 scores loaded ahead of
 // 32 in work 580, a warp for each slot's products 617, the slots' exponentials in turns 575, the second product in two halves 568 (of 566).
@@ -62,7 +62,7 @@ struct Edge {  // values in ring slot `slot`, with its next fill's parity: of th
   uint32_t phase;
 };
 
-template <bool k8, bool kTwo, bool kMore>
+template <bool k8, bool kTwo, int kWhat>
 struct Control {
   PagedLineRoom line;
   Stretch ring[kStretches];
@@ -76,18 +76,18 @@ struct Control {
   // 8 bits: what `sum` refers to, and a thread's own: the sum of blocks apart and what it refers to (in registers: 646 for 628 us of drafts)
   float sum_top[k8 ? 2 : 1][k8 ? 128 : 1], apart_l[k8 ? 2 : 1][k8 ? 128 : 1], apart_n[k8 ? 2 : 1][k8 ? 128 : 1];
   int see_lo[2][128], see_hi[2][128];
-  uint32_t tree[kMore ? 2 : 1][4][kMore ? 128 : 1];  // [slot][word][row]: the bits of a block's keys, a thread's own
+  uint32_t tree[kWhat == kTrees ? 2 : 1][4][kWhat == kTrees ? 128 : 1];  // [slot][word][row]: the bits of a block's keys, a thread's own
   int k_ref[kRefs], v_ref[kRefs];  // e_max of a block; + kFar: exponents more than kExact apart, in one that not every row sees all of
   uint32_t tmem_base;
   int abort, dead;
 };
 
-template <bool k8, int D, int R, bool kMore>
+template <bool k8, int D, int R, int kWhat>
 struct Plan {
   static constexpr bool kTwo = R == 256;
   static constexpr int kHalf = 128 * 128, kTile = D / 64 * kHalf;
   static constexpr int kQ = (kTwo ? 2 : 1) * kTile;
-  static constexpr int kControl = (sizeof(Control<k8, kTwo, kMore>) + 15) / 16 * 16, kRoom = 232448 - 1024 - kControl - kQ;
+  static constexpr int kControl = (sizeof(Control<k8, kTwo, kWhat>) + 15) / 16 * 16, kRoom = 232448 - 1024 - kControl - kQ;
   static constexpr int kSlots = k8 ? (D == 128 ? 3 : 6) : kRoom / kTile < kMostSlots ? kRoom / kTile : kMostSlots;
   // 8-bit: a block's codes, and the exponents of its keys and values; as many on their way as there is room for
   static constexpr int kRaw = 128 * D + 256, kRawRoom = (kRoom - kSlots * kTile) / kRaw;
@@ -137,11 +137,11 @@ __device__ __forceinline__ Mine blocks_of_slot(const PagedAttn& a, const Stretch
   return {j0, j1, max(0, j1 - j0 + 1)};
 }
 
-template <typename T, bool k8, int D, int R, bool kMore>
-__global__ void __launch_bounds__(Plan<k8, D, R, kMore>::kThreads, 1)
+template <typename T, bool k8, int D, int R, int kWhat>
+__global__ void __launch_bounds__(Plan<k8, D, R, kWhat>::kThreads, 1)
 paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
                   float* __restrict__ parts, PagedCut* __restrict__ cuts) {
-  using P = Plan<k8, D, R, kMore>;
+  using P = Plan<k8, D, R, kWhat>;
   using C = typename std::conditional<k8, __half, T>::type;
   constexpr bool kTwo = P::kTwo;
   constexpr int kSlots = P::kSlots, kRawSlots = P::kRawSlots;
@@ -151,7 +151,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
   uint8_t* sQ = smem;
   uint8_t* sKV = sQ + P::kQ;
   uint8_t* sRaw = sKV + kSlots * P::kTile;
-  using Ctl = Control<k8, kTwo, kMore>;
+  using Ctl = Control<k8, kTwo, kWhat>;
   Ctl& ctl = *reinterpret_cast<Ctl*>(sRaw + kRawSlots * P::kRaw);
   volatile int* s_abort = &ctl.abort;
   int* status = a.status;
@@ -201,7 +201,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
   }
   int seq0;
   long long at0;
-  const PagedLine line = paged_line<R, kKeys, kMore>(a, piece, gridDim.x, kAtLeast, ctl.line, &seq0, &at0);
+  const PagedLine line = paged_line<R, kKeys, kWhat>(a, piece, gridDim.x, kAtLeast, ctl.line, &seq0, &at0);
   const bool idle = piece >= line.pieces || line.total == 0;
   if (idle || ctl.dead != 0) {
     if (threadIdx.x == 0) cuts[piece].last = -1;
@@ -229,7 +229,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
 
   if (warp == 0) {
     // --------------------------------------------------------- the walk, and the loads
-    PagedWalk<R, kKeys, kMore> walk;
+    PagedWalk<R, kKeys, kWhat> walk;
     walk.begin(a, line, piece, seq0, at0);
     const int pages = kKeys >> a.batch.page_shift;  // of a block
     int slot = 0, edges = 0;
@@ -533,7 +533,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
           const int lo_col = ctl.see_lo[t][r] - key0, hi_col = ctl.see_hi[t][r] - key0;
           const bool cut = __any_sync(0xffffffffu, mine && (lo_col > 0 || hi_col < kKeys - 1));
           const long long in_new = key0 - (x.pos0 + x.first);  // of the block's first key among the sequence's new tokens
-          const bool masked = kMore && a.tree != nullptr && in_new > -kKeys;
+          const bool masked = kWhat == kTrees && in_new > -kKeys;
           if (masked) {
             place();
 #pragma unroll
@@ -760,12 +760,12 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
         }
         // rows that something unseen may have made a NaN are left to the joining kernel, which goes through them key by key
         if (mine) {
-          const bool again = odd && x.whole && hides<kMore>(a, x.pos0 + tok, x.keys.lo, x.keys.hi);
+          const bool again = odd && x.whole && hides<kWhat>(a, x.pos0 + tok, x.keys.lo, x.keys.hi);
           using Flag = typename std::conditional<kCols == D, uint32_t, uint16_t>::type;
           reinterpret_cast<Flag*>(a.odd + static_cast<long long>(tok) * a.kv_heads * a.group + head)[c0 / kCols] = again ? 1 : 0;
         }
         if (mine && !x.whole && c0 == 0) *reinterpret_cast<float2*>(place_of + R * D + 2 * row) = make_float2(all_top, sum);
-        if (mine && x.whole && c0 == 0 && kMore && a.lse != nullptr) put_lse(a, static_cast<long long>(tok) * a.kv_heads * a.group + head, all_top, sum);
+        if (mine && x.whole && c0 == 0 && wants_lse<kWhat>(a)) put_lse(a, static_cast<long long>(tok) * a.kv_heads * a.group + head, all_top, sum);
       }
       tc_fence_before();
       __syncwarp();
@@ -821,7 +821,7 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
       const Stretch& x = ctl.ring[i % kStretches];
       const int tiles = 2 * x.blocks;
       // keys that every row sees: up to the first one's position, from the last one's window on
-      const long long all_hi = x.pos0 + x.first + (kMore && a.tree != nullptr ? -1 : x.flat0 / a.group);
+      const long long all_hi = x.pos0 + x.first + (kWhat == kTrees ? -1 : x.flat0 / a.group);
       const long long all_lo = a.window > 0 ? x.pos0 + x.first + (x.flat0 + x.rows - 1) / a.group - a.window + 1 : 0;
       for (int n = (group - count) & (kGroups - 1); n < tiles && ok; n += kGroups) {
         const StreamTile y = stream_tile<kTwo>(n, x.blocks);
@@ -922,11 +922,11 @@ paged_tile_kernel(const __grid_constant__ PagedAttn a, const __grid_constant__ C
   }
 }
 
-template <typename T, bool k8, int D, int R, bool kMore>
+template <typename T, bool k8, int D, int R, int kWhat>
 int launch(const PagedAttn& a, const CUtensorMap& mK, const CUtensorMap& mV, void* scratch, cudaStream_t stream) {
-  using P = Plan<k8, D, R, kMore>;
+  using P = Plan<k8, D, R, kWhat>;
   static std::atomic<unsigned long long> configured{0};
-  auto kfn = paged_tile_kernel<T, k8, D, R, kMore>;
+  auto kfn = paged_tile_kernel<T, k8, D, R, kWhat>;
   if (!ensure_dynamic_smem(kfn, P::kSmem, configured)) return FTB_ERR_LAUNCH;
   const int pieces = paged_tile_pieces();
   float* parts = static_cast<float*>(scratch);
@@ -938,7 +938,9 @@ int launch(const PagedAttn& a, const CUtensorMap& mK, const CUtensorMap& mV, voi
 }
 template <typename T, bool k8, int D, int R>
 int launch(const PagedAttn& a, const CUtensorMap& mK, const CUtensorMap& mV, void* scratch, cudaStream_t stream) {
-  return a.more() ? launch<T, k8, D, R, true>(a, mK, mV, scratch, stream) : launch<T, k8, D, R, false>(a, mK, mV, scratch, stream);
+  return a.tree != nullptr  ? launch<T, k8, D, R, kTrees>(a, mK, mV, scratch, stream)
+         : a.lse != nullptr ? launch<T, k8, D, R, kLse>(a, mK, mV, scratch, stream)
+                            : launch<T, k8, D, R, kPlain>(a, mK, mV, scratch, stream);
 }
 template <typename T, int D, int R>
 int launch(const PagedAttn& a, int dtype, void* scratch, cudaStream_t stream) {

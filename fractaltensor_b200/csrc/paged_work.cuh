@@ -18,7 +18,7 @@ struct PagedSeq {
   int hi;          // keys 0 .. hi - 1 are seen by some row
 };
 
-template <bool kMore = false>
+template <int kWhat = kPlain>
 __device__ __forceinline__ PagedSeq paged_sequence(const PagedAttn& a, int b) {
   PagedSeq s;
   const int end = a.batch.starts[b + 1];
@@ -28,7 +28,7 @@ __device__ __forceinline__ PagedSeq paged_sequence(const PagedAttn& a, int b) {
   s.begin = s.flats = s.hi = 0;
   if (s.n <= 0 || s.first >= a.T) return s;
   const int flats = s.n * a.group;  // T * group fits
-  if (kMore && a.split > 0) {
+  if (kWhat == kTrees && a.split > 0) {
     const int behind = flats % a.split, rest = flats > a.split && behind <= a.rest ? behind : 0;
     if (flats < a.least_rows) return s;
     if (flats > a.most_rows) {  // the kernel for few rows
@@ -90,14 +90,14 @@ __device__ __forceinline__ long long piece_begin(const PagedLine& line, int g) {
 
 // All threads of a block, kLineThreads or more: the line, and the sequence that the first unit of piece g belongs to (B: none)
 // with that sequence's beginning.  at_least: units of a piece where there are few; of_head: units of one kv head of a sequence.
-template <bool kMore = false, typename OfHead>
+template <int kWhat = kPlain, typename OfHead>
 __device__ __forceinline__ PagedLine paged_line_of(const PagedAttn& a, int g, int most_pieces, int at_least, PagedLineRoom& room, int* seq, long long* begin,
                                                    OfHead of_head) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (a.batch.B + kLineThreads - 1) / kLineThreads;
   const int b0 = min(a.batch.B, tid * per), b1 = tid < kLineThreads ? min(a.batch.B, b0 + per) : b0;
   long long mine = 0;
-  for (int b = b0; b < b1; ++b) mine += of_head(paged_sequence<kMore>(a, b)) * a.kv_heads;
+  for (int b = b0; b < b1; ++b) mine += of_head(paged_sequence<kWhat>(a, b)) * a.kv_heads;
   long long sum = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -123,7 +123,7 @@ __device__ __forceinline__ PagedLine paged_line_of(const PagedAttn& a, int g, in
     long long at = before + sum - mine;
     if (u >= at && u < at + mine) {
       for (int b = b0; b < b1; ++b) {
-        const long long c = of_head(paged_sequence<kMore>(a, b)) * a.kv_heads;
+        const long long c = of_head(paged_sequence<kWhat>(a, b)) * a.kv_heads;
         if (u < at + c) {
           room.seq = b;
           room.begin = at;
@@ -138,9 +138,9 @@ __device__ __forceinline__ PagedLine paged_line_of(const PagedAttn& a, int g, in
   *begin = room.begin;
   return line;
 }
-template <int R, int kUnitKeys, bool kMore>
+template <int R, int kUnitKeys, int kWhat>
 __device__ __forceinline__ PagedLine paged_line(const PagedAttn& a, int g, int most_pieces, int at_least, PagedLineRoom& room, int* seq, long long* begin) {
-  return paged_line_of<kMore>(a, g, most_pieces, at_least, room, seq, begin, [&](const PagedSeq& s) { return units_of_head<R, kUnitKeys>(a, s); });
+  return paged_line_of<kWhat>(a, g, most_pieces, at_least, room, seq, begin, [&](const PagedSeq& s) { return units_of_head<R, kUnitKeys>(a, s); });
 }
 
 // A stretch of a tile that a piece works on: units r0 .. r1 - 1 of its `units`.
@@ -152,7 +152,7 @@ struct PagedTile {
 };
 
 // Walks the tiles of a piece in their order.
-template <int R, int kUnitKeys, bool kMore>
+template <int R, int kUnitKeys, int kWhat>
 struct PagedWalk {
   PagedLine line;
   long long u, u_end, at, per;  // at: the sequence's beginning, per: units of one of its kv heads
@@ -167,7 +167,7 @@ struct PagedWalk {
     at = seq_begin;
     per = 0;
     if (u < u_end && b < a.batch.B) {
-      s = paged_sequence<kMore>(a, b);
+      s = paged_sequence<kWhat>(a, b);
       per = units_of_head<R, kUnitKeys>(a, s);
     } else {
       u = u_end;
@@ -178,7 +178,7 @@ struct PagedWalk {
   __device__ __forceinline__ PagedTile next(const PagedAttn& a) {
     while (u >= at + per * a.kv_heads) {
       at += per * a.kv_heads;
-      s = paged_sequence<kMore>(a, ++b);
+      s = paged_sequence<kWhat>(a, ++b);
       per = units_of_head<R, kUnitKeys>(a, s);
     }
     PagedTile t;
