@@ -297,6 +297,18 @@ Form form_of(int T, int B, int group) {
   return {few, few, many, false};
 }
 
+constexpr Form kShortAlone = {16, INT_MAX, 0, false};
+// Tiles of many rows for trees, of what form_of says.
+Form form_of_split(Form f, long long rows, int B) {
+  // A second tile for a few rows costs as much as the first: 32 sequences of 33 tokens of 8 heads each of 8 kv heads, up to 16 000 keys of 8 bits, 720 us
+  // with the last 8 rows apart, 945 without.
+  const long long behind = rows / B > f.many ? rows / B % f.many : 0;
+  if (B == 1 && (behind == 0 || behind > 16)) return f;
+  if (behind > 0 && behind <= 16) f.few = f.most = behind <= 8 ? 8 : 16;
+  f.split = true;
+  return f;
+}
+
 // The same for trees, of which a sequence has a few dozen tokens; `keys`: as many as the table has room for.  While the tiles of
 // paged_short.cu make few units of 64 keys, its CTAs, two of them an SM, are done sooner, however many tiles read the same keys; each tile's start and end
 // count as 24 units more.  32 heads over 8 kv heads, 16 bits, us there and in paged_tile.cu:
@@ -306,17 +318,11 @@ Form form_of(int T, int B, int group) {
 //   ten of 25                     70 (8320) 30.8 21.2; 200 (8960) 36.4 34.5; 1000 (12800) 66.0 41.5
 //   31 of 16, 128 heads, d 64     70 (103 168) 96.6 33.1; 500 (126 976) 170 63
 Form form_of_tree(int T, int B, int group, int kv_heads, long long keys) {
-  Form f = form_of(T, B, group);
+  const Form f = form_of(T, B, group);
   if (f.many == 0) return f;
   const long long rows = static_cast<long long>(T) * group;
-  if ((rows + 16ll * B - 1) / (16ll * B) * B * kv_heads * ((keys + 63) / 64 + kTileUnits) <= kShortUnits) return {16, INT_MAX, 0, false};
-  // A second tile for a few rows costs as much as the first: 32 sequences of 33 tokens of 8 heads each of 8 kv heads, up to 16 000 keys of 8 bits, 720 us
-  // with the last 8 rows apart, 945 without.
-  const long long behind = rows / B > f.many ? rows / B % f.many : 0;
-  if (B == 1 && (behind == 0 || behind > 16)) return f;
-  if (behind > 0 && behind <= 16) f.few = f.most = behind <= 8 ? 8 : 16;
-  f.split = true;
-  return f;
+  if ((rows + 16ll * B - 1) / (16ll * B) * B * kv_heads * ((keys + 63) / 64 + kTileUnits) <= kShortUnits) return kShortAlone;
+  return form_of_split(f, rows, B);
 }
 
 size_t places(int pieces, int rows, int d) { return 2 * static_cast<size_t>(pieces) * rows * (d + 2) * sizeof(float) + pieces * sizeof(PagedCut); }
@@ -330,12 +336,12 @@ using namespace ftb;
 extern "C" size_t ftb_paged_attn_scratch_bytes(int T, int B, int kv_heads, int group, int d) {
   if (T <= 0 || B <= 0 || kv_heads <= 0 || group <= 0 || d <= 0) return 0;
   const Form f = form_of(T, B, group);
-  size_t n = rounded(static_cast<size_t>(T) * kv_heads * group * sizeof(uint32_t)), few = 0;
-  for (int rows = 8; rows <= 16; rows += 8)  // (a tree may take either)
-    if (f.few == rows || f.many > 0) few = std::max(few, rounded(places(paged_short_pieces(rows), rows, d)));
-  n += few;
-  if (f.many > 0) n += rounded(places(paged_tile_pieces(), f.many, d));
-  return n;
+  auto room = [&](const Form& f) {
+    return (f.few > 0 ? rounded(places(paged_short_pieces(f.few), f.few, d)) : 0) + (f.many > 0 ? rounded(places(paged_tile_pieces(), f.many, d)) : 0);
+  };
+  size_t most = room(f);
+  if (f.many > 0) most = std::max({most, room(kShortAlone), room(form_of_split(f, static_cast<long long>(T) * group, B))});  // (what a tree may take)
+  return rounded(static_cast<size_t>(T) * kv_heads * group * sizeof(uint32_t)) + most;
 }
 
 extern "C" int ftb_paged_attn_fwd(const void* q, long long q_row, long long q_head, const void* k_cache, const void* v_cache,
