@@ -1003,7 +1003,9 @@ def paged_attention_weights(q, cache, weights, lse, table, lens, starts, scale=N
     heads of its kv head's group; a new token's own key begins at 0.
 
     weights: fp32 [pages, kv_heads, page_size], beside the cache's pages; lse: fp32 [T, heads], as paged_attention gave it for the same call
-    (rows whose lse is not finite add nothing); the others as there.  A page belongs to one sequence: a key's sum is one warp's."""
+    (rows whose lse is not finite add nothing), without a tree: of a tree the path's rows of q and lse count, once paged_cache_keep has moved it; the
+    others as there.  A page belongs to one sequence: of two that share one, the sums of one are lost.  The same call gives the same bits; the order of a
+    key's terms, and so their roundings, depends on the batch."""
     done = host.paged_attention_weights(q, cache, weights, lse, table, lens, starts, 1.0 if scale is None else scale,
                                         0 if window is None else window or -1, _workspaces)
     if done is not None:
