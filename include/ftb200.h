@@ -502,10 +502,10 @@ int ftb_paged_cache_keep(void* k_cache, void* v_cache, unsigned char* k_exp, uns
  * group; the sum alone where j is a new token's own place.  weights: fp32 [pages, kv_heads, page_size]; lse: fp32
  * [T, kv_heads * group], of ftb_paged_attn_tree_fwd for the same call (a row whose lse is not finite adds nothing), which had no tree: of a
  * tree the path counts, with its rows of q and lse, once it has been kept.  Sums are made without atomics, in an order that follows from the
- * call's sizes and lengths: the same call gives the same bits, and a row in another batch may be rounded differently.  A page with new
- * tokens or keys of theirs belongs to one sequence: of two that share one, the sums of one are lost, which nothing notices.  A key whose page the
- * table does not have gets nothing and sets the (sticky) status word to 22.  scratch: ftb_paged_attn_weights_scratch_bytes (0: none needed), asked for with the call's
- * device as the current one. */
+ * call's sizes and lengths: the same call gives the same bits, and a row in another batch may be rounded differently.  A page belongs
+ * to one sequence: of two that share one, the sums of one are lost, which nothing notices.  A key whose page the table does not have gets
+ * nothing and sets the (sticky) status word to 22.  scratch: ftb_paged_attn_weights_scratch_bytes (0: none needed), asked for with the
+ * call's device as the current one. */
 size_t ftb_paged_attn_weights_scratch_bytes(int T, int B, int kv_heads, int group, int d);
 int ftb_paged_attn_weights(const void* q, long long q_row, long long q_head, const void* k_cache, const unsigned char* k_exp,
                            const float* lse, const int* table, const int* lens, const int* starts, float* weights, int T,
