@@ -300,8 +300,8 @@ Form form_of(int T, int B, int group) {
 constexpr Form kShortAlone = {16, INT_MAX, 0, false};
 // Tiles of many rows for trees, of what form_of says.
 Form form_of_split(Form f, long long rows, int B) {
-  // A second tile for a few rows costs as much as the first: 32 sequences of 33 tokens of 8 heads each of 8 kv heads, up to 16 000 keys of 8 bits, 720 us
-  // with the last 8 rows apart, 945 without.
+  // A second tile for a few rows costs as much as the first: 32 sequences of 33 tokens of 8 heads each of 8 kv heads, up to 16 000 keys of 8 bits, 677 us
+  // with the last 8 rows apart, 892 without.  (35 tokens leave 24 rows, and pay for a second tile: 770.)
   const long long behind = rows / B > f.many ? rows / B % f.many : 0;
   if (B == 1 && (behind == 0 || behind > 16)) return f;
   if (behind > 0 && behind <= 16) f.few = f.most = behind <= 8 ? 8 : 16;
@@ -309,7 +309,8 @@ Form form_of_split(Form f, long long rows, int B) {
   return f;
 }
 
-// The same for trees, of which a sequence has a few dozen tokens; `keys`: as many as the table has room for.  While the tiles of
+// The same for trees, of which a sequence has a few dozen tokens; `keys`: as many as the table has room for, the lengths being on the device (measured
+// with tables as wide as the longest sequence; one user's tree of 25 behind 752 keys 25.0 us, with a table for 131 072 keys 29.7).  While the tiles of
 // paged_short.cu make few units of 64 keys, its CTAs, two of them an SM, are done sooner, however many tiles read the same keys; each tile's start and end
 // count as 24 units more.  32 heads over 8 kv heads, 16 bits, us there and in paged_tile.cu:
 //   one sequence of 25 tokens     800 keys (2072 units so counted) 23.5 27.6; 3200 (4144) 30.9 36.6; 6400 (6944) 40.6 43.7

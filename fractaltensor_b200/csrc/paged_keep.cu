@@ -10,8 +10,8 @@
 // row i) is never read by a later one (kept[j] > kept[i] >= i); within a step all rows are read before one is written.  Chains run side
 // by side for the pieces of a row, which do not meet, and where there are few, a cluster of CTAs takes a step together.
 //
-// 48 sequences of 1500 to 9000 keys of 16 bits, 8 kv heads of 128, to 2048 of them in other pages: 156.8 us, of which the moves, bound by memory, are 131
-// (6.2 TB/s) and the choice 26, trips and digits one behind the other.  One of 100 001 keys of 8 bits, 4 kv heads, to 8192 in its own pages 23.5 us
+// 48 sequences of 1500 to 9000 keys of 16 bits, 8 kv heads of 128, to 2048 of them in other pages: 156.8 us (194 with a table for 131 072 keys, whose room leaves one CTA an SM to the choice), of which the moves, bound by memory, are 131
+// (6.2 TB/s) and the choice 26, trips and digits one behind the other.  One of 100 001 keys of 8 bits, 4 kv heads, to 8192 in its own pages 23.5 to 24.7 us
 // (372 with chains of single CTAs that looked rows up one behind the other).  Its choice
 // is bound by instructions, some 20 a key and digit, and by a cluster's barriers, 1 us each.  The paths of 128 trees 3.5 us, a launch.  Measured and not kept: lanes with
 // the same digit adding as one (30 for 28 us), a bin for every second lane (31 for 28).

@@ -6,7 +6,7 @@
 // cycles a block of 256 rows beside 2048 of products, and by the joins (25 us).  96 sequences of 8500 keys on average in 8 bits, 5 tokens
 // of 64 heads: 660 us, 0.2 PFLOP/s and 2.5 TB/s (847 where values are of 2^-40, with the sum apart for every block); bound by the instructions that make 8-bit keys operands (1.6 to 1.9 a cycle and SM).
 // Trees of drafts (kTrees): a row's bits of the block's keys are laid out in shared memory when a block reaches into the new tokens, and taken with
-// every look at the scores.  32 sequences of 33 tokens of 64 heads, up to 16 000 keys of 8 bits: 587 us for 256 of their 264 rows.
+// every look at the scores.  32 sequences of 33 tokens of 64 heads, up to 16 000 keys of 8 bits: 530 us for 256 of their 264 rows.
 // Measured and not kept, the chunk: all 128 scores of a row in registers 616 us (spills; L1 is shared memory's), 32 scores loaded ahead of
 // 32 in work 580, a warp for each slot's products 617, the slots' exponentials in turns 575, the second product in two halves 568 (of 566).
 //

@@ -11,7 +11,7 @@
 // as often as there are tiles of rows.  A warp's next 16 keys are on their way while these are made weights of, the number of the page behind
 // them one step longer.
 //
-// Bound by the bytes of the keys: 64 sequences of up to 8000 keys of 16 bits, 8 kv heads of 128, a token of 32 heads each 92.6 us, 6.1 TB/s (126 without
+// Bound by the bytes of the keys: 64 sequences of up to 8000 keys of 16 bits, 8 kv heads of 128, a token of 32 heads each 91 to 95 us (several GPUs), 6.1 TB/s (126 without
 // keys on their way ahead); 4096 keys each 88 us, over 8 bits 75, 3.6 TB/s: there the trips of a warp's 16 keys, 2 KB, are what is short.  One
 // sequence of 777 keys 6.2 us, a launch and four trips to memory one behind the other.
 #include <cfloat>
@@ -273,7 +273,7 @@ struct Form {
   int few, most;
   bool many;
 };
-// `keys`: as many as the table has room for.
+// `keys`: as many as the table has room for, the lengths being on the device (8 of 500 keys, 24 rows each: 12.1 us, with a table for 131 072 keys 17.5).
 Form form_of(int T, int B, int group, int kv_heads, long long keys) {
   const long long rows = static_cast<long long>(T) * group;
   if (T <= B || rows <= 16) return {rows <= 8ll * B ? 8 : 16, INT_MAX, false};

@@ -15,10 +15,15 @@
 //                 64 rows), and make 8-bit codes fp16; a key's scale goes to its scores
 // A block that a cut goes through leaves parts of its sums, which a second kernel adds up in their order.
 //
+// A score is one sum of the tensor core over all of d, which cuts off downwards: a chunk's weights are 3.4e-7 off (paged_weigh.cu has two sums for that reason).  Warps with a key
+// that is not there, in a sequence's last block, go number by number.
+//
 // 2048 tokens of 32 heads of 128 over 8 kv heads, 16 384 keys of 8 bits: 331 us, 0.78 PFLOP/s.  Bound by no unit alone: without the
 // exponentials (16 a cycle and SM, 245 us) it takes 285 us, without the products (122) 324, with neither 173, which is the rows' way from L2 for
 // every block and the hand-overs between the warps.  Measured and not kept: a quarter to a half of the exponentials by a polynomial on the units that
 // multiply and add (334 to 383 us), blocks of 512 keys (346), eight warps for the sums (352), each half of the warps with a buffer of its own (351).
+// A few dozen rows behind a long sequence are bound by what comes before the first load: a thread of every CTA goes through the sequence's blocks, up to three times.  32 rows behind
+// 131 072 keys, 8 kv heads: 178 us (42 by the keys' bytes), behind 524 288 keys of 8 bits of one kv head 449 (11).
 #include <algorithm>
 #include <cfloat>
 #include <climits>
